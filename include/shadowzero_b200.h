@@ -247,6 +247,83 @@ int sz_mma_cols_scratch_bytes(int cols, int m, int64_t* bytes);
 int sz_mma_cols(const sz_tensor* w, uint64_t x, int64_t xs, uint64_t y, int64_t ys, int m, uint64_t scratch, int64_t scratch_bytes, uint64_t stream);
 int sz_mma_cols_status(uint64_t scratch, int init, int* code, uint64_t stream);
 
+/* ---- a cache in pages, for hosts that serve many conversations: append, attend ---------------------------------------------------------
+ * No counterpart in the reference (a session's cache there is one range, its server answers one request at a time).  The keys and values
+ * of a layer lie in two pools of pages; a sequence's positions are the pages of its row of a table, in order.  The first `shared_len`
+ * positions may be one list of pages for ALL sequences of a call (a system prompt): they are read once for the batch, not once a sequence.
+ * lens[b] counts all positions of sequence b, the shared ones and the rows of this call included: its rows row_start[b] .. row_start[b + 1)
+ * of the inputs and outputs are its LAST positions.  Tables and lengths are device memory, read when the kernels run, so that a captured
+ * graph serves a growing batch; rows at and behind row_start[n_seq] (a padded batch) are left as they were.
+ * The cache's heads: f16 or bf16 values, or the session's packed form (SZ_TYPE_Q8_KV: head_dim int8, then head_dim / 32 f16 scales
+ * zero-padded to 16 bytes; kernels/forward.cu:3652-3687).  head_dim 64, 128 or 256; n_head a multiple of n_kv_head. */
+#define SZ_TYPE_Q8_KV 1101
+typedef struct sz_paged_cache {
+    int32_t type;                 /* SZ_TYPE_F16, SZ_TYPE_BF16 or SZ_TYPE_Q8_KV */
+    int32_t n_kv_head, head_dim;
+    int32_t page_size;            /* positions a page: a power of two from 8 to 1024 */
+    int32_t n_pages, reserved;
+    uint64_t k, v;                /* the pools, 16-byte aligned */
+    int64_t page_stride, head_stride, pos_stride;   /* bytes between pages, key heads and positions, for both pools: multiples of 16, so any order of the three */
+} sz_paged_cache;
+typedef struct sz_paged_batch {
+    int32_t n_seq;                /* 1 .. 4096 */
+    int32_t rows;                 /* rows of the inputs and outputs; row_start[n_seq] may be less */
+    int32_t max_pages;            /* entries of a sequence's row of the table */
+    int32_t shared_len;           /* positions that all sequences share (0: none); a sequence's own pages start behind them */
+    uint64_t pages;               /* int32 [n_seq][max_pages] */
+    uint64_t row_start;           /* int32 [n_seq + 1], not descending */
+    uint64_t lens;                /* int32 [n_seq] */
+    uint64_t shared_pages;        /* int32 [ceil(shared_len / page_size)]; 0 with shared_len = 0 */
+} sz_paged_batch;
+/* What happens to a head before it is stored (a key) or given back (a query): with a norm weight (f32 [head_dim]; 0: none)
+ * x / sqrt(mean(x^2) + eps) * w, then the first `dims` dimensions are turned, i with i + dims / 2 by the angle position / theta^(2 i / dims)
+ * (forward.rs:290-299; angles in f64).  dims: even, 0 .. head_dim; 0: no rotation. */
+typedef struct sz_paged_rope {
+    int32_t dims;
+    float eps;
+    double theta;
+    uint64_t q_norm, k_norm;
+} sz_paged_rope;
+/* One scratch serves both calls for any batch of up to batch->rows rows and batch->n_seq sequences of this cache shape (256-byte aligned; a
+ * call with another shared_len or fewer rows fits where this one does).  Calls that can overlap on the GPU need one each, captured
+ * graphs too.  sz_paged_status(scratch, 1, NULL, stream) once after it is allocated; sz_paged_status(scratch, 0, &code, stream)
+ * synchronises and reports (and keeps) what calls have met: bit 0: a page id out of range, bit 1: a position behind the table's end, bit 2: a
+ * row of sz_paged_append at a shared position, bit 3: row_start past `rows` - the position, or the row, is then left out -, bit 4: a bounded wait ran out. */
+int sz_paged_scratch_bytes(const sz_paged_cache* cache, const sz_paged_batch* batch, int n_head, int64_t* bytes);
+int sz_paged_status(uint64_t scratch, int init, int* code, uint64_t stream);
+/* Stores row r's key and value heads at its position and, where q is given, writes its query heads, normed and turned, to q_out.
+ * io_type: SZ_TYPE_F32, F16 or BF16, the type of k, v, q and q_out.  k, v: [rows][n_kv_head][head_dim], q_out [rows][n_head][head_dim], q
+ * [rows][n_head] heads q_head_stride apart (2 head_dim where queries and gates alternate); row strides in elements; heads and rows
+ * 16-byte aligned.  A row at a negative position (lens[b] < the sequence's rows) is left out.  q_out may be q.  No position may
+ * be appended by two rows of a call. */
+int sz_paged_append(const sz_paged_cache* cache, const sz_paged_batch* batch, const sz_paged_rope* rope, int io_type, int n_head, uint64_t k, int64_t k_stride,
+                    uint64_t v, int64_t v_stride, uint64_t q, int64_t q_stride, int64_t q_head_stride, uint64_t q_out, int64_t q_out_stride, uint64_t scratch,
+                    int64_t scratch_bytes, uint64_t stream);
+/* out[r][h] = sum over the positions t up to row r's own of softmax_t(scale q[r][h] . k_t) v_t, times sigmoid(gate[r][h]) where gate
+ * is given; head h reads key head h / (n_head / n_kv_head).  q, out [rows][n_head][head_dim], gate's heads gate_head_stride apart, all of
+ * io_type; lse (f32 [rows][n_head], 0: not wanted): the logarithm of the softmax's denominator, for hosts that join it with further keys.  A row
+ * without a position of its own (lens[b] - shared_len below the sequence's rows: a padded sequence) gives zeros and -inf.
+ * Scores, softmax and sums are f32; f32 queries keep theirs over any cache type, weights are split likewise (f16 and bf16 outputs: to
+ * 16 bits and more before the last rounding). */
+int sz_paged_attend(const sz_paged_cache* cache, const sz_paged_batch* batch, int io_type, int n_head, float scale, uint64_t q, int64_t q_stride, uint64_t gate,
+                    int64_t gate_stride, int64_t gate_head_stride, uint64_t out, int64_t out_stride, uint64_t lse, uint64_t scratch, int64_t scratch_bytes,
+                    uint64_t stream);
+
+/* ---- draws over whole rows of logits -----------------------------------------------------------------------------------------------------
+ * Sampler::sample (crates/shadowzero-serve/src/sampler.rs:112-210, no penalties) for every row of logits at once, from uniform numbers the caller
+ * gives (sz_uniform, or its own generator): what sz_sample_top draws where a row's top-64 hold every candidate, without that limit.
+ * Candidates are ordered by logit, equal ones by id.  Weight of a candidate: exp((logit - largest) / temperature), the
+ * difference and its product with 1 / temperature in f32, the exponential and all sums far beyond it; those more than 18 temperatures below the
+ * largest are dropped, then those behind the first top_k (below 1: 1), then those with less than min_p times the largest weight, then those behind
+ * the first whose running sum reaches top_p of the sum after top_k (top_p >= 1: none).  The token is the first whose running sum over
+ * what is left exceeds uniform times its total; prob its weight over that total.  A temperature of 0 or less, or NaN: the best token.  A NaN logit
+ * counts as -inf; a row without a finite largest logit gives the lowest id of its largest, prob 1.
+ * logits: [rows][vocab] of logits_type (SZ_TYPE_F32, F16 or BF16), row stride in elements; vocab 1 .. 262,144.  temperature, top_p, min_p f32 [rows], top_k
+ * int32 [rows] - any may be 0: 1, no limit, 1 and 0 -, uniform f64 [rows] in [0, 1), token int32 [rows], prob f32 [rows] (0: not wanted).
+ * Needs no scratch; deterministic (sums are integers). */
+int sz_sample_rows(int logits_type, uint64_t logits, int64_t logits_stride, int rows, int vocab, uint64_t temperature, uint64_t top_k, uint64_t top_p,
+                   uint64_t min_p, uint64_t uniform, uint64_t token, uint64_t prob, uint64_t stream);
+
 /* ---- the session: the verify surface ------------------------------------------------------------------------------------
  * Replaces the verify subset of GpuSession (crates/shadowzero-cuda/src/session.rs): step_batch_verify_top (6061-6072), rollback
  * (6217-6276), note_verify, capacity, tokens, and prefill by passes.  One engine thread owns a session (engine.rs:340-420).

@@ -2,6 +2,7 @@
 #include "sz_common.cuh"
 
 #include <string.h>
+#include <atomic>
 
 static thread_local char g_err[512] = "";
 
@@ -22,6 +23,23 @@ int sz_fail(int code, const char* fmt, ...) {
 
 extern "C" const char* sz_version(void) { return "shadowzero_b200 0.1 (sm_100a)"; }
 extern "C" const char* sz_last_error(void) { return g_err; }
+
+int sz_allow_smem(const void* kernel, int smem) {
+    static std::atomic<uintptr_t> seen[512];      // kernel and device; a full table asks every time
+    int dev = 0;
+    SZ_CUDA(cudaGetDevice(&dev));
+    const uintptr_t key = (uintptr_t)kernel * 64 + (uintptr_t)(dev & 63);
+    for (int i = 0; i < 512; i++) {
+        uintptr_t x = seen[i].load(std::memory_order_acquire);
+        if (x == key) return SZ_OK;
+        if (x) continue;
+        SZ_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+        seen[i].compare_exchange_strong(x, key);   // (another thread took the place: asked again next time)
+        return SZ_OK;
+    }
+    SZ_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+    return SZ_OK;
+}
 
 // ---- per-kernel timing --------------------------------------------------------------------------------------------------------
 // The role of the reference's SHADOWZERO_KTIME switch (crates/shadowzero-cuda/src/kernels.rs:527-536,604): while a trace is open,

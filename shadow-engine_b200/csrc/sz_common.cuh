@@ -25,6 +25,9 @@ int sz_fail(int code, const char* fmt, ...);
 
 static inline bool sz_aligned16(u64 p) { return (p & 15) == 0; }
 
+// Allows a kernel `smem` bytes of dynamic shared memory on the current device (asked of the runtime once for each kernel and device).
+int sz_allow_smem(const void* kernel, int smem);
+
 // Per-kernel timing (sz_trace_begin): records the next caller-provided event on `stream` under `name`.  No-op when tracing is off.
 void sz_trace_mark(const char* name, cudaStream_t stream);
 bool sz_trace_active();

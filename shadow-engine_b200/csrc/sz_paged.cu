@@ -1,0 +1,403 @@
+// A cache in pages (sz_paged_*): the append kernel, the kernel that joins the attention's parts, and the C ABI.  sz_paged.cuh has the
+// attention itself.
+#include "sz_paged.cuh"
+
+#include <math.h>
+
+namespace {
+
+constexpr int PG_BLOCKS = 148;       // multiprocessors (a GPU with another number: more or fewer blocks than places, the same results)
+
+// ---- append ------------------------------------------------------------------------------------------------------------------------------------
+struct PgAppend {
+    const u8 *k, *v, *q;
+    u8* qo;
+    long long k_stride, v_stride, q_stride, q_head_stride, qo_stride;   // bytes
+    const float *q_norm, *k_norm;
+    int type, esz, hd, nh, half, heads;     // heads: nh (0 without q) + 2 nkv
+    float eps;
+    double freq[128];                // 1 / theta^(2 i / dims)
+};
+
+// The sequence of row r (its last one that begins at or before r), by the whole block; -1: none.
+template <int NTH>
+__device__ int pg_seq_of(const PgBatch& d, int r) {
+    int n = 0;
+    for (int b0 = 0; b0 <= d.n_seq; b0 += NTH) n += __syncthreads_count(b0 + (int)threadIdx.x <= d.n_seq && pg_row(d, b0 + threadIdx.x) <= r);
+    return n > d.n_seq ? -1 : n - 1;
+}
+
+// A block has 8 heads of one row, a warp each (grid.y: the row's eights of heads, queries first, then keys, then values).  What bounds it is
+// latency with few rows - row, sequence, length, page, head, one after the other - and with many the bytes.  The angles of the row
+// are taken once a block, in f64 (a far position's angle has no digits left in f32), reduced to [-pi, pi] there, and the sine and
+// cosine of the reduced angle in f32 with its rounding put back by their derivatives.
+template <int CT>
+__global__ void __launch_bounds__(256) sz_pg_append_kernel(const __grid_constant__ PgBatch d, const __grid_constant__ PgAppend a) {
+    __shared__ float2 turn[128];
+    __shared__ float tmp[8][256];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r = blockIdx.x;
+    sz_pdl_wait();
+    sz_pdl_trigger();
+    const int b = pg_seq_of<256>(d, r);
+    if (r == 0 && blockIdx.y == 0 && threadIdx.x == 0 && __ldg(d.row_start + d.n_seq) > d.rows) atomicOr(d.err, PG_E_ROWS);
+    if (b < 0) return;
+    const int pos = __ldg(d.lens + b) - (pg_row(d, b + 1) - r);
+    if (pos < 0) return;
+    for (int i = threadIdx.x; i < a.half; i += 256) {
+        const double f = (double)pos * a.freq[i];
+        const double kq = rint(f * 0.15915494309189535);
+        double rd = fma(-kq, 6.283185307179586, f);
+        rd = fma(-kq, 2.4492935982947064e-16, rd);
+        const float hi = (float)rd, lo = (float)(rd - (double)hi);
+        float sn, cs;
+        sincosf(hi, &sn, &cs);
+        turn[i] = make_float2(fmaf(-sn, lo, cs), fmaf(cs, lo, sn));
+    }
+    __syncthreads();
+    const int x = blockIdx.y * 8 + warp, nq = a.q ? a.nh : 0;
+    if (x >= a.heads) return;
+    const int kind = x < nq ? 0 : x < nq + d.nkv ? 1 : 2, h = kind == 0 ? x : (x - nq) % d.nkv;
+    u8* dst = nullptr;
+    if (kind) {                      // where the position lies
+        const int o = pos - d.shared_len;
+        if (o < 0) { if (lane == 0) atomicOr(d.err, PG_E_SHARED); return; }
+        if ((long long)o >= (long long)d.max_pages << d.ps_log2) { if (lane == 0) atomicOr(d.err, PG_E_END); return; }
+        const int page = __ldg(d.pages + (size_t)b * d.max_pages + (o >> d.ps_log2));
+        if ((u32)page >= (u32)d.n_pages) { if (lane == 0) atomicOr(d.err, PG_E_PAGE); return; }
+        dst = (u8*)(kind == 1 ? d.k : d.v) + (long long)page * d.page_stride + (long long)(o & ((1 << d.ps_log2) - 1)) * d.pos_stride + (long long)h * d.head_stride;
+    }
+    const u8* src = kind == 0 ? a.q + (long long)r * a.q_stride + (long long)h * a.q_head_stride
+                              : (kind == 1 ? a.k + (long long)r * a.k_stride : a.v + (long long)r * a.v_stride) + (long long)h * a.hd * a.esz;
+    float2 f[4];
+#pragma unroll
+    for (int i = 0; i < 4; i++)
+        if (64 * i < a.hd) f[i] = pg_load2(src + (long long)(2 * (lane + 32 * i)) * a.esz, a.type);
+    const float* w = kind == 0 ? a.q_norm : kind == 1 ? a.k_norm : nullptr;
+    if (w) {
+        double ss = 0.0;
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+            if (64 * i < a.hd) ss += (double)f[i].x * (double)f[i].x + (double)f[i].y * (double)f[i].y;
+        ss = sz_warp_sum(ss);
+        const double rr = sz_rsqrt64(ss / (double)a.hd + (double)a.eps);
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+            if (64 * i < a.hd) {
+                const float2 ww = *(const float2*)(w + 2 * (lane + 32 * i));
+                f[i] = make_float2((float)((double)f[i].x * rr) * ww.x, (float)((double)f[i].y * rr) * ww.y);
+            }
+    }
+    if (kind < 2 && a.half) {        // the pair (i, i + half) of a rotation lies in two lanes: through shared memory
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+            if (64 * i < a.hd) *(float2*)(tmp[warp] + 2 * (lane + 32 * i)) = f[i];
+        __syncwarp();
+        for (int i = lane; i < a.half; i += 32) {
+            const float2 t = turn[i];
+            const float u = tmp[warp][i], v = tmp[warp][i + a.half];
+            tmp[warp][i] = u * t.x - v * t.y;
+            tmp[warp][i + a.half] = v * t.x + u * t.y;
+        }
+        __syncwarp();
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+            if (64 * i < a.hd) f[i] = *(const float2*)(tmp[warp] + 2 * (lane + 32 * i));
+    }
+    if (kind == 0) {
+        u8* out = a.qo + (long long)r * a.qo_stride + (long long)h * a.hd * a.esz;
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+            if (64 * i < a.hd) pg_store2(out + (long long)(2 * (lane + 32 * i)) * a.esz, a.type, f[i].x, f[i].y);
+        return;
+    }
+    if (CT != PG_Q8) {
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+            if (64 * i < a.hd) *(u32*)(dst + 4 * (lane + 32 * i)) = pg_pack<CT>(f[i].x, f[i].y);
+        return;
+    }
+    // packed: a group of 32 dimensions is 16 lanes of a pair each
+#pragma unroll
+    for (int i = 0; i < 4; i++)
+        if (64 * i < a.hd) {
+            float big = fmaxf(fabsf(f[i].x), fabsf(f[i].y));
+#pragma unroll
+            for (int s = 8; s > 0; s >>= 1) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, s));
+            const __half sh = __float2half_rn(big > 0.0f ? big * (1.0f / 127.0f) : 0.0f);
+            const float sr = __half2float(sh), inv = sr > 0.0f ? 1.0f / sr : 0.0f;
+            int c0 = __float2int_rn(f[i].x * inv), c1 = __float2int_rn(f[i].y * inv);
+            c0 = c0 < -127 ? -127 : (c0 > 127 ? 127 : c0);
+            c1 = c1 < -127 ? -127 : (c1 > 127 ? 127 : c1);
+            *(u16*)(dst + 2 * (lane + 32 * i)) = (u16)((c0 & 255) | (c1 & 255) << 8);
+            if ((lane & 15) == 0) *(u16*)(dst + a.hd + 2 * (2 * i + (lane >> 4))) = __half_as_ushort(sh);
+        }
+    if (lane >= a.hd / 32 && lane < 8)                           // the 16 bytes behind the codes: those behind the scales are zero
+        *(u16*)(dst + a.hd + 2 * lane) = 0;
+}
+
+// ---- the plan of a call with more sequences or tiles than a block plans for itself ---------------------------------------------------------
+__global__ void __launch_bounds__(1024) sz_pg_plan_kernel(const __grid_constant__ PgBatch d, const __grid_constant__ PgPart a, const __grid_constant__ PgPart s) {
+    __shared__ u32 scan[32];
+    sz_pdl_wait();
+    sz_pdl_trigger();
+    if (a.planned) pg_plan<1024>(d, 0, a.tq, a.tiles, a.units, scan);
+    __syncthreads();
+    if (s.planned) pg_plan<1024>(d, 1, s.tq, s.tiles, s.units, scan);
+}
+
+// ---- joining the parts -----------------------------------------------------------------------------------------------------------------------------
+// A block has one row and head: the parts of its item over the shared positions, then those over its own, in the order of the positions.
+// Threads in groups of hd / 4 take the parts in turn (four columns each); the groups' sums are added in order.
+constexpr int PG_MERGE = 128, PG_PARTS = 2 * 4 * PG_BLOCKS;
+struct PgList { int n, first, alone, lane; };     // parts of an item: their number, the block of the first; by row and head; the vector's place in its tile
+__device__ PgList pg_list(const PgBatch& d, const PgPart& p, int r0, int first_row, int b, int h, int r, int E) {
+    PgList l = {};
+    const int vec = (r - r0) * d.G + h % d.G, t = vec / p.tq, e = p.shared ? t : (int)p.tiles[b] + t;
+    const u32 us = p.units[e], n = p.units[e + 1] - us;
+    if (!n) return l;
+    const long long U = (long long)p.units[E] * d.nkv, at = (long long)us * d.nkv + (long long)(h / d.G) * n;
+    const int blocks = (int)min((long long)p.blocks, U), last = pg_block_of(at + n - 1, U, blocks);
+    l.first = pg_block_of(at, U, blocks);
+    l.n = last - l.first + 1;
+    l.alone = l.n == 1;
+    l.lane = vec % p.tq;
+    return l;
+}
+template <int HD>
+__global__ void __launch_bounds__(PG_MERGE) sz_pg_merge_kernel(const __grid_constant__ PgBatch d, const __grid_constant__ PgIo io, const __grid_constant__ PgPart own,
+                                                               const __grid_constant__ PgPart shr) {
+    __shared__ float wgt[PG_PARTS];
+    __shared__ float red[PG_MERGE / 32], redl[PG_MERGE / 32];
+    __shared__ float4 sums[PG_MERGE];
+    const int r = blockIdx.x, h = blockIdx.y, nh = d.nkv * d.G, tid = threadIdx.x;
+    sz_pdl_wait();
+    sz_pdl_trigger();
+    const int b = pg_seq_of<PG_MERGE>(d, r);
+    if (b < 0) return;
+    const int r0 = pg_row(d, b), m = pg_row(d, b + 1) - r0, start = pg_row(d, 0);
+    const long long seen = (long long)__ldg(d.lens + b) - d.shared_len - (m - 1 - (r - r0));     // own positions the row sees
+    u8* op = io.out + (long long)r * io.out_stride + (long long)h * HD * io.esz;
+    PgList lo = pg_list(d, own, r0, 0, b, h, r, (int)own.tiles[d.n_seq]), ls = {};
+    if (seen > 0 && own.direct && lo.alone) return;                // (written by the block that did it)
+    if (shr.on && seen > 0) ls = pg_list(d, shr, start, 0, 0, h, r, ((pg_row(d, d.n_seq) - start) * d.G + shr.tq - 1) / shr.tq);
+    if (seen <= 0) lo.n = 0;
+    const int n = ls.n + lo.n;
+    auto where = [&](int i, const float2*& ml) -> const float* {
+        const PgPart& p = i < ls.n ? shr : own;
+        const PgList& l = i < ls.n ? ls : lo;
+        const int k = i < ls.n ? i : i - ls.n;
+        const size_t at = l.alone ? (size_t)r * nh + h : (size_t)(k == 0 ? 2 * l.first + 1 : 2 * (l.first + k)) * p.tq + l.lane;
+        ml = (l.alone ? p.row_ml : p.ml) + at;
+        return (l.alone ? p.row_o : p.o) + at * HD;
+    };
+    float M = -INFINITY;
+    for (int i = tid; i < n; i += PG_MERGE) { const float2* ml; where(i, ml); const float x = ml->x; wgt[i] = x; M = fmaxf(M, x); }
+#pragma unroll
+    for (int s = 16; s > 0; s >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, s));
+    if ((tid & 31) == 0) red[tid >> 5] = M;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < PG_MERGE / 32; w++) M = fmaxf(M, red[w]);
+    float L = 0.f;
+    for (int i = tid; i < n; i += PG_MERGE) {
+        const float2* ml;
+        where(i, ml);
+        const float c = wgt[i] == -INFINITY ? 0.f : pg_ex2(wgt[i] - M);
+        wgt[i] = c;
+        L += c * ml->y;
+    }
+    L = sz_warp_sum(L);
+    if ((tid & 31) == 0) redl[tid >> 5] = L;
+    __syncthreads();
+    L = 0.f;
+#pragma unroll
+    for (int w = 0; w < PG_MERGE / 32; w++) L += redl[w];
+    constexpr int TG = HD / 4, GN = PG_MERGE / TG;
+    const int grp = tid / TG, col = tid % TG;
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+    for (int i = grp; i < n; i += GN) {
+        const float2* ml;
+        const float4 x = *(const float4*)(where(i, ml) + 4 * col);
+        const float c = wgt[i];
+        acc.x = fmaf(c, x.x, acc.x); acc.y = fmaf(c, x.y, acc.y); acc.z = fmaf(c, x.z, acc.z); acc.w = fmaf(c, x.w, acc.w);
+    }
+    sums[tid] = acc;
+    __syncthreads();
+    if (grp) return;
+#pragma unroll
+    for (int k = 1; k < GN; k++) { const float4 x = sums[k * TG + col]; acc.x += x.x; acc.y += x.y; acc.z += x.z; acc.w += x.w; }
+    const bool none = n == 0 || L == 0.f;                             // nothing the row may see
+    const float inv = none ? 0.f : 1.f / L;
+    float y[4] = {acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv};
+    if (none) y[0] = y[1] = y[2] = y[3] = 0.f;
+    if (io.gate) {
+        const u8* gp = io.gate + (long long)r * io.gate_stride + (long long)h * io.gate_head_stride + 4 * col * io.esz;
+        const float2 g0 = pg_load2(gp, io.type), g1 = pg_load2(gp + 2 * io.esz, io.type);
+        y[0] *= sz_sigmoid(g0.x); y[1] *= sz_sigmoid(g0.y); y[2] *= sz_sigmoid(g1.x); y[3] *= sz_sigmoid(g1.y);
+        if (none) y[0] = y[1] = y[2] = y[3] = 0.f;
+    }
+    pg_store2(op + 4 * col * io.esz, io.type, y[0], y[1]);
+    pg_store2(op + (4 * col + 2) * io.esz, io.type, y[2], y[3]);
+    if (io.lse && tid == 0) io.lse[(size_t)r * nh + h] = none ? -INFINITY : (M + log2f(L)) * 0.6931471805599453f;
+}
+
+// ---- the host side -------------------------------------------------------------------------------------------------------------------------------
+int pg_head_bytes(int type, int hd) { return type == SZ_TYPE_Q8_KV ? hd + ((hd / 32 * 2 + 15) & ~15) : 2 * hd; }
+int pg_esz(int type) { return type == SZ_TYPE_F32 ? 4 : 2; }
+
+int pg_check(const sz_paged_cache* c, const sz_paged_batch* b, int n_head, const char* who) {
+    if (!c || !b) return sz_fail(SZ_E_ARG, "%s: null cache or batch", who);
+    if (c->type != SZ_TYPE_F16 && c->type != SZ_TYPE_BF16 && c->type != SZ_TYPE_Q8_KV) return sz_fail(SZ_E_TYPE, "%s: cache type %d (F16, BF16 and Q8_KV have kernels)", who, c->type);
+    if (c->head_dim != 64 && c->head_dim != 128 && c->head_dim != 256) return sz_fail(SZ_E_ARG, "%s: heads of %d (64, 128 and 256 have kernels)", who, c->head_dim);
+    if (c->n_kv_head < 1 || c->n_kv_head > 1024 || n_head < c->n_kv_head || n_head % c->n_kv_head || n_head > 4096)
+        return sz_fail(SZ_E_ARG, "%s: %d heads on %d key heads", who, n_head, c->n_kv_head);
+    if (c->page_size < 8 || c->page_size > 1024 || (c->page_size & (c->page_size - 1))) return sz_fail(SZ_E_ARG, "%s: pages of %d positions (a power of two from 8 to 1024)", who, c->page_size);
+    if (c->n_pages < 1) return sz_fail(SZ_E_ARG, "%s: %d pages", who, c->n_pages);
+    const int64_t hb = pg_head_bytes(c->type, c->head_dim);
+    if ((c->page_stride | c->head_stride | c->pos_stride) & 15 || c->page_stride < hb || c->pos_stride < hb || (c->n_kv_head > 1 && c->head_stride < hb) || c->head_stride < 0)
+        return sz_fail(SZ_E_ARG, "%s: strides of pages, heads and positions are multiples of 16 and at least a head's %lld bytes", who, (long long)hb);
+    if (b->n_seq < 1 || b->n_seq > PG_MAX_SEQ || b->rows < 1 || b->rows > (1 << 20) || b->max_pages < 1 || b->shared_len < 0)
+        return sz_fail(SZ_E_ARG, "%s: %d sequences (1 .. %d), %d rows (1 .. 1048576), %d pages a sequence, %d shared positions", who, b->n_seq, PG_MAX_SEQ, b->rows, b->max_pages, b->shared_len);
+    return SZ_OK;
+}
+int pg_check_tables(const sz_paged_cache* c, const sz_paged_batch* b, const char* who) {
+    if (!c->k || !c->v || ((c->k | c->v) & 15)) return sz_fail(SZ_E_ARG, "%s: null or misaligned pools (16 bytes)", who);
+    if (!b->pages || !b->row_start || !b->lens || (b->shared_len > 0 && !b->shared_pages) || ((b->pages | b->row_start | b->lens | b->shared_pages) & 3))
+        return sz_fail(SZ_E_ARG, "%s: null or misaligned tables", who);
+    return SZ_OK;
+}
+int pg_check_rows(uint64_t p, int64_t stride, int64_t head_stride, int n_head, int hd, int rows, int esz, const char* name, const char* who) {
+    if (!p || (p & 15) || (stride * esz & 15) || (head_stride * esz & 15)) return sz_fail(SZ_E_ARG, "%s: %s null, or its rows or heads not 16-byte aligned", who, name);
+    if (head_stride < hd || (rows > 1 && stride < (n_head - 1) * head_stride + hd)) return sz_fail(SZ_E_ARG, "%s: rows or heads of %s overlap", who, name);
+    return SZ_OK;
+}
+PgBatch pg_batch(const sz_paged_cache* c, const sz_paged_batch* b, int n_head, uint64_t scratch) {
+    PgBatch d = {};
+    d.k = (const u8*)c->k; d.v = (const u8*)c->v;
+    d.page_stride = c->page_stride; d.head_stride = c->head_stride; d.pos_stride = c->pos_stride;
+    d.pages = (const int32_t*)b->pages; d.row_start = (const int32_t*)b->row_start; d.lens = (const int32_t*)b->lens; d.shared_pages = (const int32_t*)b->shared_pages;
+    d.n_seq = b->n_seq; d.rows = b->rows; d.max_pages = b->max_pages; d.shared_len = b->shared_len; d.n_pages = c->n_pages;
+    while ((1 << d.ps_log2) < c->page_size) d.ps_log2++;
+    d.nkv = c->n_kv_head; d.G = n_head / c->n_kv_head;
+    d.err = (u32*)scratch;
+    return d;
+}
+// Tiles of 16 query vectors a block: as many as a sequence's rows fill on average, up to 4 (more vectors share a key read from memory; a
+// sequence with more makes more items).
+int pg_tiles_of(long long vectors) { return vectors <= 16 ? 1 : vectors <= 32 ? 2 : 4; }
+
+// The scratch: the status word, then for own and shared positions the plan's tables, the blocks' parts, the whole items by row.
+struct PgScratch { PgPart own, shr; int64_t bytes; };
+PgScratch pg_scratch(int n_seq, int rows, int nh, int hd, uint64_t base) {
+    PgScratch s = {};
+    int64_t off = 256;
+    auto take = [&](int64_t n) { const int64_t at = off; off += (n + 255) & ~(int64_t)255; return base + at; };
+    for (PgPart* p : {&s.own, &s.shr}) {
+        const int64_t slots = 2ll * PG_BLOCKS * 64;      // vectors of the blocks' parts: blocks a multiprocessor x vectors a tile is 64 at most
+        p->tiles = (u32*)take(4ll * (n_seq + 1));
+        p->units = (u32*)take(4ll * ((int64_t)rows * nh / 16 + n_seq + 2));
+        p->o = (float*)take(slots * hd * 4);
+        p->ml = (float2*)take(slots * 8);
+        p->row_o = (float*)take((int64_t)rows * nh * hd * 4);
+        p->row_ml = (float2*)take((int64_t)rows * nh * 8);
+    }
+    s.bytes = off;
+    return s;
+}
+
+int pg_launch_attend(const PgKernels& k, const PgBatch& d, const PgIo& io, const PgPart& p, const char* name, cudaStream_t st) {
+    const int rc = sz_allow_smem(k.fn, k.smem);
+    if (rc) return rc;
+    SZ_CUDA(sz_launch(name, (void (*)(PgBatch, PgIo, PgPart))k.fn, dim3(p.blocks), dim3(k.threads), k.smem, st, true, d, io, p));
+    return SZ_OK;
+}
+
+}  // namespace
+
+extern "C" int sz_paged_scratch_bytes(const sz_paged_cache* cache, const sz_paged_batch* batch, int n_head, int64_t* bytes) {
+    int rc = pg_check(cache, batch, n_head, "sz_paged_scratch_bytes");
+    if (rc) return rc;
+    if (!bytes) return sz_fail(SZ_E_ARG, "sz_paged_scratch_bytes: null result");
+    *bytes = pg_scratch(batch->n_seq, batch->rows, n_head, cache->head_dim, 0).bytes;
+    return SZ_OK;
+}
+
+extern "C" int sz_paged_status(uint64_t scratch, int init, int* code, uint64_t stream) {
+    if (!scratch || (scratch & 255)) return sz_fail(SZ_E_ARG, "sz_paged_status: null or misaligned scratch");
+    cudaStream_t st = (cudaStream_t)stream;
+    if (init) { SZ_CUDA(cudaMemsetAsync((void*)scratch, 0, 256, st)); return SZ_OK; }
+    if (!code) return sz_fail(SZ_E_ARG, "sz_paged_status: null code");
+    u32 v = 0;
+    SZ_CUDA(cudaMemcpyAsync(&v, (const void*)scratch, 4, cudaMemcpyDeviceToHost, st));
+    SZ_CUDA(cudaStreamSynchronize(st));
+    *code = (int)v;
+    return v ? sz_fail(SZ_E_DEVICE, "sz_paged: the tables of a call did not fit (%s%s%s%s%s)", v & PG_E_PAGE ? " page id out of range;" : "", v & PG_E_END ? " position behind the table;" : "",
+                       v & PG_E_SHARED ? " row at a shared position;" : "", v & PG_E_ROWS ? " row_start past the rows;" : "", v & PG_E_WAIT ? " a bounded wait ran out;" : "")
+             : SZ_OK;
+}
+
+extern "C" int sz_paged_append(const sz_paged_cache* cache, const sz_paged_batch* batch, const sz_paged_rope* rope, int io_type, int n_head, uint64_t k, int64_t k_stride, uint64_t v,
+                               int64_t v_stride, uint64_t q, int64_t q_stride, int64_t q_head_stride, uint64_t q_out, int64_t q_out_stride, uint64_t scratch, int64_t scratch_bytes,
+                               uint64_t stream) {
+    const char* who = "sz_paged_append";
+    int rc = pg_check(cache, batch, n_head, who);
+    if (rc || (rc = pg_check_tables(cache, batch, who))) return rc;
+    if (io_type != SZ_TYPE_F32 && io_type != SZ_TYPE_F16 && io_type != SZ_TYPE_BF16) return sz_fail(SZ_E_TYPE, "%s: inputs of type %d", who, io_type);
+    const int esz = pg_esz(io_type), hd = cache->head_dim, nkv = cache->n_kv_head;
+    if (!rope || rope->dims < 0 || rope->dims > hd || rope->dims % 2 || (rope->dims && !(rope->theta > 0.0 && isfinite(rope->theta))) || !(rope->eps >= 0.f))
+        return sz_fail(SZ_E_ARG, "%s: rope: an even number of dimensions up to %d, theta > 0, eps >= 0", who, hd);
+    if ((rope->q_norm | rope->k_norm) & 15) return sz_fail(SZ_E_ARG, "%s: norm weights 16-byte aligned", who);
+    if ((rc = pg_check_rows(k, k_stride, hd, nkv, hd, batch->rows, esz, "k", who)) || (rc = pg_check_rows(v, v_stride, hd, nkv, hd, batch->rows, esz, "v", who))) return rc;
+    if (q && ((rc = pg_check_rows(q, q_stride, q_head_stride, n_head, hd, batch->rows, esz, "q", who)) ||
+              (rc = pg_check_rows(q_out, q_out_stride, hd, n_head, hd, batch->rows, esz, "q_out", who))))
+        return rc;
+    if (q && q == q_out && (q_stride != q_out_stride || q_head_stride != hd)) return sz_fail(SZ_E_ARG, "%s: q_out may be q with the same strides only", who);
+    if (!scratch || (scratch & 255) || scratch_bytes < 256) return sz_fail(SZ_E_SCRATCH, "%s: the scratch is 256-byte aligned and holds the status word at least", who);
+    const PgBatch d = pg_batch(cache, batch, n_head, scratch);
+    PgAppend a = {};
+    a.k = (const u8*)k; a.v = (const u8*)v; a.q = (const u8*)q; a.qo = (u8*)q_out;
+    a.k_stride = k_stride * esz; a.v_stride = v_stride * esz; a.q_stride = q_stride * esz; a.q_head_stride = q_head_stride * esz; a.qo_stride = q_out_stride * esz;
+    a.q_norm = (const float*)rope->q_norm; a.k_norm = (const float*)rope->k_norm;
+    a.type = io_type; a.esz = esz; a.hd = hd; a.nh = n_head; a.half = rope->dims / 2; a.heads = (q ? n_head : 0) + 2 * nkv; a.eps = rope->eps;
+    for (int i = 0; i < a.half; i++) a.freq[i] = 1.0 / pow(rope->theta, 2.0 * i / rope->dims);
+    const dim3 grid(batch->rows, (a.heads + 7) / 8);
+    auto* fn = cache->type == SZ_TYPE_F16 ? sz_pg_append_kernel<PG_F16> : cache->type == SZ_TYPE_BF16 ? sz_pg_append_kernel<PG_BF16> : sz_pg_append_kernel<PG_Q8>;
+    SZ_CUDA(sz_launch("paged_append", fn, grid, dim3(256), 0, (cudaStream_t)stream, true, d, a));
+    return SZ_OK;
+}
+
+extern "C" int sz_paged_attend(const sz_paged_cache* cache, const sz_paged_batch* batch, int io_type, int n_head, float scale, uint64_t q, int64_t q_stride, uint64_t gate,
+                               int64_t gate_stride, int64_t gate_head_stride, uint64_t out, int64_t out_stride, uint64_t lse, uint64_t scratch, int64_t scratch_bytes, uint64_t stream) {
+    const char* who = "sz_paged_attend";
+    int rc = pg_check(cache, batch, n_head, who);
+    if (rc || (rc = pg_check_tables(cache, batch, who))) return rc;
+    if (io_type != SZ_TYPE_F32 && io_type != SZ_TYPE_F16 && io_type != SZ_TYPE_BF16) return sz_fail(SZ_E_TYPE, "%s: queries of type %d", who, io_type);
+    const int esz = pg_esz(io_type), hd = cache->head_dim, nkv = cache->n_kv_head, G = n_head / nkv;
+    if (!isfinite(scale)) return sz_fail(SZ_E_ARG, "%s: scale is not finite", who);
+    if ((rc = pg_check_rows(q, q_stride, hd, n_head, hd, batch->rows, esz, "q", who)) || (rc = pg_check_rows(out, out_stride, hd, n_head, hd, batch->rows, esz, "out", who))) return rc;
+    if (gate && (rc = pg_check_rows(gate, gate_stride, gate_head_stride, n_head, hd, batch->rows, esz, "gate", who))) return rc;
+    if (lse & 3) return sz_fail(SZ_E_ARG, "%s: lse misaligned", who);
+    PgScratch s = pg_scratch(batch->n_seq, batch->rows, n_head, hd, scratch);
+    if (!scratch || (scratch & 255) || scratch_bytes < s.bytes) return sz_fail(SZ_E_SCRATCH, "%s: %lld bytes of scratch given, %lld needed, 256-byte aligned", who, (long long)scratch_bytes, (long long)s.bytes);
+    cudaStream_t st = (cudaStream_t)stream;
+    const PgBatch d = pg_batch(cache, batch, n_head, scratch);
+    PgIo io = {};
+    io.q = (const u8*)q; io.q_stride = q_stride * esz; io.gate = (const u8*)gate; io.gate_stride = gate_stride * esz; io.gate_head_stride = gate_head_stride * esz;
+    io.out = (u8*)out; io.out_stride = out_stride * esz; io.lse = (float*)lse; io.type = io_type; io.esz = esz; io.scale_log2 = scale * 1.4426950408889634f;
+    const int ct = cache->type == SZ_TYPE_F16 ? PG_F16 : cache->type == SZ_TYPE_BF16 ? PG_BF16 : PG_Q8;
+    const bool wide = io_type == SZ_TYPE_F32 || (io_type == SZ_TYPE_F16 && ct != PG_F16);
+    auto kernels = [&](int nqt) { return ct == PG_F16 ? pg_kernels_f16(wide, hd, nqt) : ct == PG_BF16 ? pg_kernels_bf16(wide, hd, nqt) : pg_kernels_q8(wide, hd, nqt); };
+    const int64_t per_seq = (int64_t)G * ((batch->rows + batch->n_seq - 1) / batch->n_seq), all = (int64_t)G * batch->rows;
+    const PgKernels ko = kernels(pg_tiles_of(per_seq)), ks = kernels(pg_tiles_of(all));
+    s.own.on = 1; s.own.tq = ko.tq; s.own.blocks = PG_BLOCKS * ko.occ; s.own.direct = batch->shared_len == 0;
+    s.own.planned = batch->n_seq > PG_PLAN || batch->n_seq + all / ko.tq > PG_PLAN;
+    s.shr.on = batch->shared_len > 0; s.shr.tq = ks.tq; s.shr.blocks = PG_BLOCKS * ks.occ; s.shr.shared = 1;
+    s.shr.planned = s.shr.on && (all + ks.tq - 1) / ks.tq > PG_PLAN;
+    if (s.own.planned || s.shr.planned) SZ_CUDA(sz_launch("paged_plan", sz_pg_plan_kernel, dim3(1), dim3(1024), 0, st, true, d, s.own, s.shr));
+    if (s.shr.on && (rc = pg_launch_attend(ks, d, io, s.shr, "paged_attend_shared", st))) return rc;
+    if ((rc = pg_launch_attend(ko, d, io, s.own, "paged_attend", st))) return rc;
+    auto* merge = hd == 64 ? sz_pg_merge_kernel<64> : hd == 128 ? sz_pg_merge_kernel<128> : sz_pg_merge_kernel<256>;
+    SZ_CUDA(sz_launch("paged_merge", merge, dim3(batch->rows, n_head), dim3(PG_MERGE), 0, st, true, d, io, s.own, s.shr));
+    return SZ_OK;
+}

@@ -1,0 +1,705 @@
+// A cache in pages: what the append, attention and merge kernels share, and the attention kernel for any number of queries a sequence.
+//
+// Attention of a query vector (row, head) over the positions it may see: s_t = scale q . k_t, o = sum_t e^(s_t) v_t / sum_t e^(s_t).  A
+// sum over positions splits into parts that are joined exactly: a part is (m, l, O) = (largest score, sum of 2^(s - m), sum of 2^(s - m) v),
+// scores in units of log 2; two parts join with the factors 2^(m_i - M), M the larger m.
+//
+// Work.  The query vectors of a sequence that share a key head (its rows times the G heads of the group) are cut into tiles of TQ; an ITEM
+// is a tile, a key head and the positions that the tile's last row sees; a UNIT is 64 positions of an item.  The units of all items in a row
+// are shared out evenly to as many blocks as the GPU holds at once, so that ragged contexts leave no block idle and one long conversation
+// fills the GPU; an item cut by a block's boundary leaves parts, which sz_pg_merge_kernel joins in the order of the positions.  The plan (units
+// before every item) is made by every block from the lengths in device memory: nothing about a step is fixed when a graph is captured.
+// The positions that all sequences share are items of their own, whose tiles run over the rows of the whole batch (SHARED).
+#pragma once
+#include "sz_common.cuh"
+#include "sz_dense.cuh"
+
+constexpr int PG_T = 64;             // positions a unit
+constexpr int PG_PLAN = 512;         // sequences and tiles that a block plans for itself; above, sz_pg_plan_kernel does once
+constexpr int PG_MAX_SEQ = 4096;
+enum { PG_F16 = 0, PG_BF16 = 1, PG_Q8 = 2 };
+enum { PG_E_PAGE = 1, PG_E_END = 2, PG_E_SHARED = 4, PG_E_ROWS = 8, PG_E_WAIT = 16 };
+
+struct PgBatch {                     // the tables of a call, as the kernels read them
+    const u8 *k, *v;
+    long long page_stride, head_stride, pos_stride;
+    const int32_t *pages, *row_start, *lens, *shared_pages;
+    int n_seq, rows, max_pages, shared_len, n_pages, ps_log2, nkv, G;
+    u32* err;
+};
+struct PgIo {                        // rows of queries and outputs; strides in bytes
+    const u8* q;
+    long long q_stride;
+    const u8* gate;
+    long long gate_stride, gate_head_stride;
+    u8* out;
+    long long out_stride;
+    float* lse;
+    int type, esz;                   // SZ_TYPE_F32 / F16 / BF16, bytes an element
+    float scale_log2;                // scale / log 2
+};
+// One attention launch's plan and parts.  Block i of `blocks` takes units [i U / blocks, (i + 1) U / blocks) of U.  Parts: slot 2 i is what
+// block i adds to an item that an earlier block began, slot 2 i + 1 what it begins and a later one goes on with; an item that one block
+// does alone lies by row and head.
+struct PgPart {
+    u32 *tiles, *units;              // [n_seq + 1] tiles before a sequence, [tiles + 1] units (of one key head) before a tile
+    float* o;                        // [slot][tq][hd]
+    float2* ml;                      // [slot][tq]
+    float* row_o;                    // [row][head][hd]: an item that one block did alone
+    float2* row_ml;                  // [row][head]
+    int blocks, tq, shared, planned; // planned: the plan was made by sz_pg_plan_kernel
+    int direct;                      // an item that one block does alone goes straight to the output
+    int on;
+};
+
+__device__ __forceinline__ int pg_row(const PgBatch& d, int i) { return min(max(__ldg(d.row_start + i), 0), d.rows); }
+// Units of tile t of a sequence with m rows whose own positions end at `end` (exclusive), and the tile's own end.
+__device__ __forceinline__ int pg_tile_end(const PgBatch& d, int m, long long end, int t, int tq) {
+    const int last = (min((t + 1) * tq, m * d.G) - 1) / d.G;
+    const long long e = end - (m - 1 - last), room = (long long)d.max_pages << d.ps_log2;
+    return (int)max(0ll, min(e, room));
+}
+// Which block has unit u when `blocks` share U units: the last i with i U / blocks <= u.
+__device__ __forceinline__ int pg_block_of(long long u, long long U, int blocks) { return (int)(((u + 1) * blocks - 1) / U); }
+
+__device__ __forceinline__ float pg_ex2(float x) { float y; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x)); return y; }
+// two neighbouring elements at p
+__device__ __forceinline__ float2 pg_load2(const u8* p, int type) {
+    if (type == SZ_TYPE_F32) return *(const float2*)p;
+    const u32 w = *(const u32*)p;
+    if (type == SZ_TYPE_F16) return __half22float2(*(const __half2*)&w);
+    return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+}
+__device__ __forceinline__ u32 pg_pack_bf16(float a, float b) {      // round to nearest even, as the type's own conversion does
+    u32 r;
+    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(b), "f"(a));
+    return r;
+}
+__device__ __forceinline__ u32 pg_pack_f16(float a, float b) { const __half2 h = __floats2half2_rn(a, b); return *(const u32*)&h; }
+__device__ __forceinline__ void pg_store2(u8* p, int type, float a, float b) {
+    if (type == SZ_TYPE_F32) *(float2*)p = make_float2(a, b);
+    else *(u32*)p = type == SZ_TYPE_F16 ? pg_pack_f16(a, b) : pg_pack_bf16(a, b);
+}
+
+// ---- the plan: by all NTH threads of a block, into shared or global memory -----------------------------------------------------------------
+template <int NTH>
+__device__ u32 pg_scan(u32 v, u32& total, u32* sm) {                // exclusive prefix over the block's threads
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    u32 x = v;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) { const u32 y = __shfl_up_sync(0xffffffffu, x, o); if (lane >= o) x += y; }
+    __syncthreads();
+    if (lane == 31) sm[warp] = x;
+    __syncthreads();
+    u32 before = 0;
+    total = 0;
+#pragma unroll
+    for (int w = 0; w < NTH / 32; w++) { const u32 s = sm[w]; if (w < warp) before += s; total += s; }
+    return before + x - v;
+}
+// tiles[0 .. n_seq], units[0 .. tiles[n_seq]]; returns the number of tiles.  (SHARED: one tile list over the rows of all sequences.)
+template <int NTH>
+__device__ int pg_plan(const PgBatch& d, int shared, int tq, u32* tiles, u32* units, u32* sm) {
+    if (shared) {
+        const int vec = (pg_row(d, d.n_seq) - pg_row(d, 0)) * d.G, E = max(0, (vec + tq - 1) / tq);
+        const u32 un = (u32)((d.shared_len + PG_T - 1) / PG_T);
+        for (int e = threadIdx.x; e <= E; e += NTH) units[e] = (u32)e * un;
+        if (threadIdx.x == 0) tiles[0] = 0;
+        __syncthreads();
+        return E;
+    }
+    u32 carry = 0, total;
+    for (int b0 = 0; b0 < d.n_seq; b0 += NTH) {
+        const int b = b0 + threadIdx.x;
+        const u32 n = b < d.n_seq ? (u32)((max(pg_row(d, b + 1) - pg_row(d, b), 0) * d.G + tq - 1) / tq) : 0u;
+        const u32 at = pg_scan<NTH>(n, total, sm);
+        if (b < d.n_seq) tiles[b] = carry + at;
+        carry += total;
+    }
+    const int E = (int)carry;
+    if (threadIdx.x == 0) tiles[d.n_seq] = carry;
+    __syncthreads();
+    carry = 0;
+    for (int e0 = 0; e0 < E; e0 += NTH) {
+        const int e = e0 + threadIdx.x;
+        u32 n = 0;
+        if (e < E) {
+            int lo = 0, hi = d.n_seq - 1;                           // the last sequence whose tiles begin at or before e
+            while (lo < hi) { const int mid = (lo + hi + 1) >> 1; if (tiles[mid] <= (u32)e) lo = mid; else hi = mid - 1; }
+            const int m = pg_row(d, lo + 1) - pg_row(d, lo);
+            n = (u32)((pg_tile_end(d, m, (long long)__ldg(d.lens + lo) - d.shared_len, e - (int)tiles[lo], tq) + PG_T - 1) / PG_T);
+        }
+        const u32 at = pg_scan<NTH>(n, total, sm);
+        if (e < E) units[e] = carry + at;
+        carry += total;
+    }
+    if (threadIdx.x == 0) units[E] = carry;
+    __syncthreads();
+    return E;
+}
+
+// ---- the attention kernel ---------------------------------------------------------------------------------------------------------------------
+// A block has NQT tiles of 16 query vectors (TQ = 16 NQT) and takes its units one after the other.  Warps: NQT tiles x WAYS shares of a unit's
+// positions; a warp keeps its tile's (m, l, O) for its positions in registers from unit to unit, so nothing but keys, values and queries
+// goes through shared memory, and with one tile (decoding) warps load their own positions and meet only where an item begins or ends.
+// Keys and values come as asynchronous copies of 16 bytes through a ring of half units (64 keys, then their 64 values), rows swizzled (16-bit
+// types: chunk c of row r at c ^ (r & 7)) so that ldmatrix meets no bank twice; packed rows of 272 / 144 / 80 bytes spread by themselves.
+// Both products run on mma.sync m16n8k16 with f32 sums.  (tcgen05 wants 64 rows and more: decoding has G queries a key head, and the
+// kernel waits for memory, not for the tensor pipe.)  Rounding: queries and weights enter as sums of QN and PN pieces of the cache's type -
+//   WIDE (f32 queries, or f16 ones over a packed or bf16 cache): f16 2 pieces (22 bits), bf16 3 (24), so that f32 results keep f32's accuracy;
+//   else the queries are exact in one piece, weights take two (f16 22 bits, bf16 16), one over a packed cache for bf16 results (11 bits, a
+//   quarter of the step that the result itself is rounded to).
+// f16 pieces are kept in range: queries are divided by a power of two near their largest element, weights are 2^15 times themselves (so
+// that small ones do not run into f16's subnormals), and both are taken back in f32.  A packed value's scale goes into the weight (times a
+// power of two that follows the scales, CSC), a packed key's into the 32-dimension partial scores in f32: codes themselves are exact in f16.
+template <int CT, bool WIDE, int HD, int NQT>
+struct PgCfg {
+    static constexpr int NW = NQT == 1 ? 4 : 8, NTH = 32 * NW, WAYS = NW / NQT, SG = PG_T / 16 / WAYS, TQ = 16 * NQT;
+    static constexpr int HB = CT == PG_Q8 ? HD + ((HD / 32 * 2 + 15) & ~15) : 2 * HD, CPR = HB / 16, HALF = PG_T * HB;
+    static constexpr int PPW = PG_T / NW;               // positions a warp loads
+    static constexpr int QN = CT == PG_BF16 ? (WIDE ? 3 : 1) : (WIDE ? 2 : 1);
+    static constexpr int PN = CT == PG_BF16 ? (WIDE ? 3 : 2) : CT == PG_F16 ? 2 : (WIDE ? 2 : 1);
+    static constexpr int KS = HD / 16, NT = HD / 8;
+    static constexpr int QB = QN * NQT * KS * 512, MB = (WAYS - 1) * NQT * 16 * 64 * 4, QM = QB > MB ? QB : MB;
+    static constexpr int MISC = 2 * (PG_PLAN + 1) * 4 + 8 * 4 + TQ * 8 + WAYS * TQ * 8 + 8 * 8 + 64;
+    static constexpr int OCC = NQT > 1 ? 1 : HD == 256 ? (CT == PG_Q8 ? 2 : 1) : HD == 128 ? 2 : 4;
+    static constexpr int ROOM = (227 * 1024 / OCC - 1024 - QM - MISC) / HALF;
+    static constexpr int NR = ROOM > 6 ? 6 : ROOM;      // halves in the ring
+    static_assert(NR >= 3, "the ring needs three halves");
+    static constexpr int SMEM = NR * HALF + QM + MISC;
+    static constexpr float PSCALE = CT == PG_BF16 ? 0.f : 15.f;
+};
+
+template <int CT>
+__device__ __forceinline__ void pg_mma(float* c, const u32* a, u32 b0, u32 b1) {
+    if (CT == PG_BF16)
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+            : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+    else sz_mma16816_zn(c, a, b0, b1);
+}
+template <int CT>
+__device__ __forceinline__ u32 pg_pack(float a, float b) { return CT == PG_BF16 ? pg_pack_bf16(a, b) : pg_pack_f16(a, b); }
+template <int CT>
+__device__ __forceinline__ float2 pg_unpack(u32 w) {
+    if (CT == PG_BF16) return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+    return __half22float2(*(const __half2*)&w);
+}
+// a pair as N pieces: the first the pair rounded, each further one what is left, rounded
+template <int CT, int N>
+__device__ __forceinline__ void pg_pieces(float a, float b, u32* w) {
+#pragma unroll
+    for (int i = 0; i < N; i++) {
+        w[i] = pg_pack<CT>(a, b);
+        if (i + 1 < N) { const float2 f = pg_unpack<CT>(w[i]); a -= f.x; b -= f.y; }
+    }
+}
+__device__ __forceinline__ void pg_cp16(u32 dst, const u8* src, u32 bytes) {     // bytes 0: zeros
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void pg_ldsm4(u32* r, u32 addr) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void pg_ldsm4t(u32* r, u32 addr) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+
+struct PgItem { int e, h, i, n, b, t, end; };       // tile, key head, unit and units of the item; its sequence, tile of it, end of its positions
+
+template <int CT, bool WIDE, int HD, int NQT>
+__global__ void __launch_bounds__(PgCfg<CT, WIDE, HD, NQT>::NTH, PgCfg<CT, WIDE, HD, NQT>::OCC)
+sz_pg_attend_kernel(const __grid_constant__ PgBatch d, const __grid_constant__ PgIo io, const __grid_constant__ PgPart pt) {
+    using C = PgCfg<CT, WIDE, HD, NQT>;
+    extern __shared__ __align__(128) u8 smem[];
+    u8* const ring = smem;
+    u8* const qm = smem + C::NR * C::HALF;                // query pieces as A fragments; at an item's end what the ways add up
+    u32* const s_tiles = (u32*)(qm + C::QM);
+    u32* const s_units = s_tiles + PG_PLAN + 1;
+    u32* const s_scan = s_units + PG_PLAN + 1;
+    float* const s_fac = (float*)(s_scan + 8);            // [TQ] what a vector's raw scores are multiplied by
+    int* const s_lim = (int*)(s_fac + C::TQ);             // [TQ] positions a vector sees
+    float2* const s_ml = (float2*)(s_lim + C::TQ);        // [WAYS][TQ]
+    u8* const s_ok = (u8*)(s_ml + C::WAYS * C::TQ);       // [ring half][warp] which of the positions are there (a bit each, 16 a way)
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g8 = lane >> 2, q4 = lane & 3;
+    const int qt = warp % NQT, way = warp / NQT;
+    sz_pdl_wait();
+    sz_pdl_trigger();
+    const u32 *tiles = s_tiles, *units = s_units;
+    int E;
+    if (pt.planned) {
+        tiles = pt.tiles; units = pt.units;
+        E = pt.shared ? max(0, ((pg_row(d, d.n_seq) - pg_row(d, 0)) * d.G + C::TQ - 1) / C::TQ) : (int)tiles[d.n_seq];
+    } else {
+        E = pg_plan<C::NTH>(d, pt.shared, C::TQ, s_tiles, s_units, s_scan);
+        if (blockIdx.x == 0) {                            // for the merge
+            if (!pt.shared) for (int i = tid; i <= d.n_seq; i += C::NTH) pt.tiles[i] = s_tiles[i];
+            for (int i = tid; i <= E; i += C::NTH) pt.units[i] = s_units[i];
+        }
+    }
+    if (blockIdx.x == 0 && !pt.shared) {                  // what the lengths ask for that is not there
+        for (int b = tid; b < d.n_seq; b += C::NTH)
+            if (pg_row(d, b + 1) > pg_row(d, b) && (long long)__ldg(d.lens + b) - d.shared_len > ((long long)d.max_pages << d.ps_log2)) atomicOr(d.err, PG_E_END);
+        if (tid == 0 && __ldg(d.row_start + d.n_seq) > d.rows) atomicOr(d.err, PG_E_ROWS);
+    }
+    const long long U = (long long)units[E] * d.nkv;
+    const int blocks = (int)min((long long)pt.blocks, U);
+    if ((int)blockIdx.x >= blocks) return;
+    const long long u0 = U * blockIdx.x / blocks, u1 = U * (blockIdx.x + 1) / blocks;
+    const int room = (int)min((long long)d.max_pages << d.ps_log2, 0x7fffffc0ll);
+
+    auto locate = [&](long long u) {
+        PgItem it;
+        const u32 un = (u32)(u / d.nkv);                  // (an entry's units times nkv: the entry of u is that of u / nkv)
+        int lo = 0, hi = E - 1;
+        while (lo < hi) { const int mid = (lo + hi + 1) >> 1; if (units[mid] <= un) lo = mid; else hi = mid - 1; }
+        it.e = lo;
+        it.n = (int)(units[lo + 1] - units[lo]);
+        const u32 rem = (u32)(u - (long long)units[lo] * d.nkv);
+        it.h = (int)(rem / (u32)it.n);
+        it.i = (int)(rem % (u32)it.n);
+        if (pt.shared) { it.b = 0; it.t = lo; it.end = d.shared_len; return it; }
+        int bl = 0, bh = d.n_seq - 1;
+        while (bl < bh) { const int mid = (bl + bh + 1) >> 1; if (tiles[mid] <= (u32)lo) bl = mid; else bh = mid - 1; }
+        it.b = bl;
+        it.t = lo - (int)tiles[bl];
+        it.end = pg_tile_end(d, pg_row(d, bl + 1) - pg_row(d, bl), (long long)__ldg(d.lens + bl) - d.shared_len, it.t, C::TQ);
+        return it;
+    };
+    // ---- loads: step s of the block is the keys (even) or values (odd) of unit u0 + s / 2
+    PgItem ld = locate(u0);
+    long long lu = u0;
+    int page = -1;                                        // lane l < PPW: the page of the warp's position l of the unit to load next
+    long long off = -1;                                   // .. and its offset in the pools, of the unit being loaded
+    auto peek = [&]() {
+        const int c = ld.i * PG_T + warp * C::PPW + lane;
+        page = -1;
+        if (lane < C::PPW && c < ld.end) page = __ldg((pt.shared ? d.shared_pages : d.pages + (size_t)ld.b * d.max_pages) + (c >> d.ps_log2));
+    };
+    int lslot = 0, steps_left = (int)(2 * (u1 - u0));
+    auto issue = [&](int which) {
+        if (steps_left > 0) {
+            steps_left--;
+            if (which == 0) {
+                const int c = ld.i * PG_T + warp * C::PPW + lane;
+                const bool there = lane < C::PPW && c < ld.end;
+                const bool ok = there && (u32)page < (u32)d.n_pages;
+                if (there && !ok) atomicOr(d.err, PG_E_PAGE);
+                off = ok ? (long long)page * d.page_stride + (long long)(c & ((1 << d.ps_log2) - 1)) * d.pos_stride + (long long)ld.h * d.head_stride : -1;
+                const u32 bits = __ballot_sync(0xffffffffu, ok);
+                if (lane == 0) { if (C::PPW == 16) *(u16*)(s_ok + lslot * 8 + 2 * warp) = (u16)bits; else s_ok[lslot * 8 + warp] = (u8)bits; }
+            }
+            const u8* base = which ? d.v : d.k;
+            const u32 dst = sz_smem_addr(ring) + (u32)(lslot * C::HALF + warp * C::PPW * C::HB);
+            constexpr int N = C::PPW * C::CPR;
+#pragma unroll
+            for (int i = 0; i < (N + 31) / 32; i++) {
+                const int x = i * 32 + lane, r = x / C::CPR, ch = x % C::CPR;
+                const long long o = __shfl_sync(0xffffffffu, off, r & 31);
+                if (N % 32 == 0 || x < N) {
+                    const int cs = CT == PG_Q8 ? ch : ch ^ ((warp * C::PPW + r) & 7);
+                    pg_cp16(dst + (u32)(r * C::HB + cs * 16), base + (o < 0 ? 0 : o + ch * 16), o < 0 ? 0u : 16u);
+                }
+            }
+            if (which) {                                  // on to the next unit
+                lu++;
+                if (lu < u1) {
+                    if (++ld.i == ld.n) ld = locate(lu);
+                    peek();
+                }
+            }
+        }
+        lslot = lslot + 1 == C::NR ? 0 : lslot + 1;
+        sz_cp_async_commit();
+    };
+    peek();
+#pragma unroll
+    for (int s = 0; s < C::NR - 1; s++) issue(s & 1);
+    int ipar = (C::NR - 1) & 1;                           // which of the two the next issue loads
+
+    float o[C::NT][4], p[C::SG][8], m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f, csc = 1.f;
+    bool fresh = true;                                    // the maxima moved since the values' scale was chosen
+    int lim0 = 0, lim1 = 0;
+    float f0 = 0.f, f1 = 0.f;
+    int cslot = 0;
+    const int pw = way * 16 * C::SG;                      // the warp's first position of a unit
+    const u32 rbase = sz_smem_addr(ring);
+
+    PgItem it = locate(u0);
+    for (long long u = u0; u < u1; u++) {
+        if (u != u0 && ++it.i == it.n) it = locate(u);
+        if (u == u0 || it.i == 0) {                       // ---- an item begins: its queries
+            __syncthreads();
+            const int r0 = pg_row(d, it.b), m = (pt.shared ? pg_row(d, d.n_seq) : pg_row(d, it.b + 1)) - r0;
+            const long long oend = pt.shared ? (long long)d.shared_len : (long long)__ldg(d.lens + it.b) - d.shared_len;
+#pragma unroll 4
+            for (int v = warp; v < C::TQ; v += C::NW) {
+                const int vec = it.t * C::TQ + v, row = vec / d.G, head = it.h * d.G + vec % d.G;
+                float2 x[HD / 64];
+                float big = 0.f;
+#pragma unroll
+                for (int i = 0; i < HD / 64; i++) {
+                    x[i] = row < m ? pg_load2(io.q + (long long)(r0 + row) * io.q_stride + (long long)(head * HD + 2 * (lane + 32 * i)) * io.esz, io.type) : make_float2(0.f, 0.f);
+                    big = fmaxf(big, fmaxf(fabsf(x[i].x), fabsf(x[i].y)));
+                }
+                float down = 1.f, fac = io.scale_log2;
+                if (CT != PG_BF16) {                      // by a power of two to below 1
+#pragma unroll
+                    for (int s = 16; s > 0; s >>= 1) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, s));
+                    const int ex = min(max((int)((__float_as_uint(big) >> 23) & 255u) - 126, -100), 126);
+                    down = __uint_as_float((u32)(127 - ex) << 23);
+                    fac = io.scale_log2 * __uint_as_float((u32)(127 + ex) << 23);
+                }
+#pragma unroll
+                for (int i = 0; i < HD / 64; i++) {
+                    const int dm = 2 * (lane + 32 * i), ks = dm / 16, dd = dm % 16;
+                    // the pair's lane and register in the A fragment of k-step ks.  16-bit keys: k slots are the dimensions in order; packed
+                    // ones: a lane's four slots are four neighbouring dimensions, a word of codes
+                    const int ql = CT == PG_Q8 ? dd / 4 : (dd % 8) / 2, rg = (CT == PG_Q8 ? (dd % 4) / 2 : dd / 8) * 2 + ((v & 15) >> 3);
+                    u32 w[C::QN];
+                    pg_pieces<CT, C::QN>(x[i].x * down, x[i].y * down, w);
+#pragma unroll
+                    for (int k = 0; k < C::QN; k++)
+                        *(u32*)(qm + (((size_t)(k * NQT + (v >> 4)) * C::KS + ks) * 32 + (v & 7) * 4 + ql) * 16 + rg * 4) = w[k];
+                }
+                if (lane == 0) {
+                    s_fac[v] = fac;
+                    s_lim[v] = row < m ? (int)max(0ll, min(pt.shared ? oend : oend - (m - 1 - row), (long long)room)) : 0;
+                    if (pt.shared && row < m) s_lim[v] = d.shared_len;
+                }
+            }
+            __syncthreads();
+            lim0 = s_lim[qt * 16 + g8]; lim1 = s_lim[qt * 16 + g8 + 8];
+            f0 = s_fac[qt * 16 + g8]; f1 = s_fac[qt * 16 + g8 + 8];
+#pragma unroll
+            for (int b = 0; b < C::NT; b++) { o[b][0] = 0.f; o[b][1] = 0.f; o[b][2] = 0.f; o[b][3] = 0.f; }
+            m0 = m1 = -INFINITY; l0 = l1 = 0.f; csc = 1.f; fresh = true;
+        }
+        // ---- the unit's keys: scores, maxima, weights
+        sz_cp_async_wait<C::NR - 2>();
+        if (NQT == 1) __syncwarp(); else __syncthreads();
+        issue(ipar); ipar ^= 1;
+        const int c0 = it.i * PG_T + pw;
+        const u32 kb = rbase + (u32)(cslot * C::HALF);
+        u32 okb;                                          // 16 SG bits from the warp's first position on
+        if (C::SG == 1) okb = *(const u16*)(s_ok + cslot * 8 + 2 * way); else okb = *(const u32*)(s_ok + cslot * 8 + 4 * way);
+        float s[C::SG][2][4];
+#pragma unroll
+        for (int g = 0; g < C::SG; g++)
+#pragma unroll
+            for (int n = 0; n < 2; n++) { s[g][n][0] = 0.f; s[g][n][1] = 0.f; s[g][n][2] = 0.f; s[g][n][3] = 0.f; }
+        if constexpr (CT != PG_Q8) {
+            const int r = pw + ((lane >> 4) << 3) + (lane & 7);
+            const u32 ra = kb + (u32)(r * C::HB);
+            const int cx = (lane >> 3) & 1, sw = r & 7;
+#pragma unroll
+            for (int ks = 0; ks < C::KS; ks++) {
+                u32 b[C::SG][4];
+#pragma unroll
+                for (int g = 0; g < C::SG; g++) pg_ldsm4(b[g], ra + (u32)(g * 16 * C::HB + (((2 * ks + cx) ^ sw) << 4)));
+#pragma unroll
+                for (int k = 0; k < C::QN; k++) {
+                    const uint4 q = *(const uint4*)(qm + (((size_t)(k * NQT + qt) * C::KS + ks) * 32 + lane) * 16);
+                    const u32 a[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+                    for (int g = 0; g < C::SG; g++) { pg_mma<CT>(s[g][0], a, b[g][0], b[g][1]); pg_mma<CT>(s[g][1], a, b[g][2], b[g][3]); }
+                }
+            }
+        } else {
+            const u8* kr = ring + (size_t)cslot * C::HALF + (size_t)pw * C::HB;
+#pragma unroll 2
+            for (int gr = 0; gr < HD / 32; gr++) {        // 32 dimensions share a scale
+                float tt[C::SG][2][4];
+#pragma unroll
+                for (int g = 0; g < C::SG; g++)
+#pragma unroll
+                    for (int n = 0; n < 2; n++) { tt[g][n][0] = 0.f; tt[g][n][1] = 0.f; tt[g][n][2] = 0.f; tt[g][n][3] = 0.f; }
+#pragma unroll
+                for (int kk = 0; kk < 2; kk++) {
+                    const int ks = 2 * gr + kk;
+                    u32 b0[C::SG][2], b1[C::SG][2];
+#pragma unroll
+                    for (int g = 0; g < C::SG; g++)
+#pragma unroll
+                        for (int n = 0; n < 2; n++) sz_q8_quad(*(const u32*)(kr + (size_t)(16 * g + 8 * n + g8) * C::HB + ks * 16 + 4 * q4), b0[g][n], b1[g][n]);
+#pragma unroll
+                    for (int k = 0; k < C::QN; k++) {
+                        const uint4 q = *(const uint4*)(qm + (((size_t)(k * NQT + qt) * C::KS + ks) * 32 + lane) * 16);
+                        const u32 a[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+                        for (int g = 0; g < C::SG; g++)
+#pragma unroll
+                            for (int n = 0; n < 2; n++) pg_mma<CT>(tt[g][n], a, b0[g][n], b1[g][n]);
+                    }
+                }
+#pragma unroll
+                for (int g = 0; g < C::SG; g++)
+#pragma unroll
+                    for (int n = 0; n < 2; n++) {
+                        const u8* sp = kr + (size_t)(16 * g + 8 * n + 2 * q4) * C::HB + HD + 2 * gr;
+                        const float sa = sz_f16_to_f32(*(const u16*)sp), sb = sz_f16_to_f32(*(const u16*)(sp + C::HB));
+                        s[g][n][0] = fmaf(sa, tt[g][n][0], s[g][n][0]); s[g][n][1] = fmaf(sb, tt[g][n][1], s[g][n][1]);
+                        s[g][n][2] = fmaf(sa, tt[g][n][2], s[g][n][2]); s[g][n][3] = fmaf(sb, tt[g][n][3], s[g][n][3]);
+                    }
+            }
+        }
+        bool hidden = false;                              // a position that is there, but not for this lane's rows
+        float x0 = -INFINITY, x1 = -INFINITY;
+#pragma unroll
+        for (int g = 0; g < C::SG; g++)
+#pragma unroll
+            for (int n = 0; n < 2; n++)
+#pragma unroll
+                for (int c = 0; c < 2; c++) {
+                    const int pi = 16 * g + 8 * n + 2 * q4 + c;
+                    const bool ok = (okb >> pi) & 1u, a = ok && c0 + pi < lim0, b = ok && c0 + pi < lim1;
+                    s[g][n][c] = a ? s[g][n][c] * f0 : -INFINITY;
+                    s[g][n][2 + c] = b ? s[g][n][2 + c] * f1 : -INFINITY;
+                    hidden |= ok && !(a && b);
+                    x0 = fmaxf(x0, s[g][n][c]); x1 = fmaxf(x1, s[g][n][2 + c]);
+                }
+#pragma unroll
+        for (int k = 1; k < 4; k <<= 1) { x0 = fmaxf(x0, __shfl_xor_sync(0xffffffffu, x0, k)); x1 = fmaxf(x1, __shfl_xor_sync(0xffffffffu, x1, k)); }
+        if (__any_sync(0xffffffffu, x0 > m0 || x1 > m1)) {
+            const float n0 = fmaxf(m0, x0), n1 = fmaxf(m1, x1);
+            const float a0 = m0 == -INFINITY ? 0.f : pg_ex2(m0 - n0), a1 = m1 == -INFINITY ? 0.f : pg_ex2(m1 - n1);   // (nothing summed yet: 0 times 0)
+#pragma unroll
+            for (int b = 0; b < C::NT; b++) { o[b][0] *= a0; o[b][1] *= a0; o[b][2] *= a1; o[b][3] *= a1; }
+            l0 *= a0; l1 *= a1; m0 = n0; m1 = n1;
+            fresh = true;
+        }
+        {
+            const float e0 = (m0 == -INFINITY ? 0.f : m0) - C::PSCALE, e1 = (m1 == -INFINITY ? 0.f : m1) - C::PSCALE;
+#pragma unroll
+            for (int g = 0; g < C::SG; g++)
+#pragma unroll
+                for (int n = 0; n < 2; n++)
+#pragma unroll
+                    for (int c = 0; c < 2; c++) {
+                        p[g][4 * n + c] = pg_ex2(s[g][n][c] - e0); p[g][4 * n + 2 + c] = pg_ex2(s[g][n][2 + c] - e1);
+                        l0 += p[g][4 * n + c]; l1 += p[g][4 * n + 2 + c];
+                    }
+        }
+        cslot = cslot + 1 == C::NR ? 0 : cslot + 1;
+        // ---- its values: O += P V
+        sz_cp_async_wait<C::NR - 2>();
+        if (NQT == 1) __syncwarp(); else __syncthreads();
+        issue(ipar); ipar ^= 1;
+        const u32 vb = rbase + (u32)(cslot * C::HALF);
+        if constexpr (CT != PG_Q8) {
+            const int r = pw + (lane & 15), sw = r & 7, cx = lane >> 4;
+            const u32 ra = vb + (u32)(r * C::HB);
+            bool plain = true;
+            if (__any_sync(0xffffffffu, hidden)) {
+                // 0 times an infinity or NaN in a row's hidden positions would reach its sums: looked for where some row hides some
+                u32 bad = 0;
+#pragma unroll 4
+                for (int b2 = 0; b2 < HD / 16; b2++)
+#pragma unroll
+                    for (int g = 0; g < C::SG; g++) {
+                        u32 w[4];
+                        pg_ldsm4t(w, ra + (u32)(g * 16 * C::HB + (((2 * b2 + cx) ^ sw) << 4)));
+                        constexpr u32 X = CT == PG_BF16 ? 0x7f80u : 0x7c00u;
+#pragma unroll
+                        for (int k = 0; k < 4; k++) bad |= (u32)((w[k] & X) == X) | (u32)((w[k] & (X << 16)) == (X << 16));
+                    }
+                plain = !__any_sync(0xffffffffu, bad != 0);
+            }
+            if (plain) {
+#pragma unroll
+                for (int g = 0; g < C::SG; g++) {
+                    u32 af[C::PN][4];
+#pragma unroll
+                    for (int r4 = 0; r4 < 4; r4++) {
+                        u32 w[C::PN];
+                        pg_pieces<CT, C::PN>(p[g][2 * r4], p[g][2 * r4 + 1], w);
+#pragma unroll
+                        for (int k = 0; k < C::PN; k++) af[k][r4] = w[k];
+                    }
+#pragma unroll
+                    for (int b2 = 0; b2 < HD / 16; b2++) {
+                        u32 w[4];
+                        pg_ldsm4t(w, ra + (u32)(g * 16 * C::HB + (((2 * b2 + cx) ^ sw) << 4)));
+#pragma unroll
+                        for (int k = 0; k < C::PN; k++) { pg_mma<CT>(o[2 * b2], af[k], w[0], w[1]); pg_mma<CT>(o[2 * b2 + 1], af[k], w[2], w[3]); }
+                    }
+                }
+            } else {                                      // position by position, only for the rows that see it
+                const u8* vr = ring + (size_t)cslot * C::HALF;
+#pragma unroll
+                for (int g = 0; g < C::SG; g++)
+#pragma unroll
+                    for (int k = 0; k < 16; k++) {
+                        const int src = (lane & ~3) | ((k & 7) >> 1), pos = pw + 16 * g + k;
+                        const float w0 = __shfl_sync(0xffffffffu, p[g][4 * (k >> 3) + (k & 1)], src), w1 = __shfl_sync(0xffffffffu, p[g][4 * (k >> 3) + 2 + (k & 1)], src);
+                        const bool ok = (okb >> (16 * g + k)) & 1u, a = ok && it.i * PG_T + pos < lim0, b = ok && it.i * PG_T + pos < lim1;
+#pragma unroll
+                        for (int nt = 0; nt < C::NT; nt++) {
+                            const float2 f = pg_unpack<CT>(*(const u32*)(vr + (size_t)pos * C::HB + ((nt ^ (pos & 7)) << 4) + 4 * q4));
+                            if (a) { o[nt][0] = fmaf(w0, f.x, o[nt][0]); o[nt][1] = fmaf(w0, f.y, o[nt][1]); }
+                            if (b) { o[nt][2] = fmaf(w1, f.x, o[nt][2]); o[nt][3] = fmaf(w1, f.y, o[nt][3]); }
+                        }
+                    }
+            }
+        } else {
+            const u8* vr = ring + (size_t)cslot * C::HALF + (size_t)pw * C::HB;
+            {   // the power of two that brings this unit's largest value scale to [2^-1, 1) (weights: 2^15 at most)
+                u32 top = 0;
+#pragma unroll
+                for (int i = 0; i < (16 * C::SG * HD / 64 + 31) / 32; i++) {
+                    const int x = lane + 32 * i, r = x / (HD / 64), w2 = x % (HD / 64);
+                    if (16 * C::SG * HD / 64 % 32 == 0 || r < 16 * C::SG) {
+                        const u32 w = *(const u32*)(vr + (size_t)r * C::HB + HD + 4 * w2);
+                        top = max(top, max(w & 0x7fffu, (w >> 16) & 0x7fffu));
+                    }
+                }
+                top = __reduce_max_sync(0xffffffffu, top);
+                const int ex = top >> 10 ? (int)(top >> 10) - 14 : -14;             // scale < 2^ex
+                const float want = __uint_as_float((u32)(127 - ex) << 23);
+                if (want < csc || (fresh && want != csc)) {
+                    const float by = want / csc;                                     // (powers of two: exact)
+#pragma unroll
+                    for (int b = 0; b < C::NT; b++) { o[b][0] *= by; o[b][1] *= by; o[b][2] *= by; o[b][3] *= by; }
+                    csc = want;
+                }
+                fresh = false;
+            }
+#pragma unroll
+            for (int g = 0; g < C::SG; g++)
+#pragma unroll
+                for (int gr = 0; gr < HD / 32; gr++) {
+                    u32 v4[4];
+                    float vs[4];
+#pragma unroll
+                    for (int r4 = 0; r4 < 4; r4++) {      // positions 2 q4, + 1, + 8, + 9: the lane's k slots; a word: dimensions 32 gr + 4 g8 ..
+                        const u8* row = vr + (size_t)(16 * g + 2 * q4 + (r4 & 1) + 8 * (r4 >> 1)) * C::HB;
+                        v4[r4] = *(const u32*)(row + 32 * gr + 4 * g8);
+                        vs[r4] = sz_f16_to_f32(*(const u16*)(row + HD + 2 * gr)) * csc;
+                    }
+                    u32 af[C::PN][4];
+#pragma unroll
+                    for (int r4 = 0; r4 < 4; r4++) {
+                        u32 w[C::PN];
+                        const float pa = p[g][2 * r4], pb = p[g][2 * r4 + 1];
+                        pg_pieces<CT, C::PN>(pa > 0.f ? pa * vs[2 * (r4 >> 1)] : 0.f, pb > 0.f ? pb * vs[2 * (r4 >> 1) + 1] : 0.f, w);
+#pragma unroll
+                        for (int k = 0; k < C::PN; k++) af[k][r4] = w[k];
+                    }
+#pragma unroll
+                    for (int b = 0; b < 4; b++) {         // tile b's column n is dimension 32 gr + 4 n + b
+                        const u32 w0 = sz_q8_pair(__byte_perm(v4[0], v4[1], b | ((4 + b) << 4) | 0x4400) & 0xffffu);
+                        const u32 w1 = sz_q8_pair(__byte_perm(v4[2], v4[3], b | ((4 + b) << 4) | 0x4400) & 0xffffu);
+#pragma unroll
+                        for (int k = 0; k < C::PN; k++) pg_mma<CT>(o[4 * gr + b], af[k], w0, w1);
+                    }
+                }
+        }
+        cslot = cslot + 1 == C::NR ? 0 : cslot + 1;
+        if (u + 1 < u1 && it.i + 1 < it.n) continue;
+        // ---- the block's last unit of the item: the ways' parts added up, then out
+        {
+            const float back = CT == PG_BF16 ? 1.f : 1.f / 32768.f;
+#pragma unroll
+            for (int k = 1; k < 4; k <<= 1) { l0 += __shfl_xor_sync(0xffffffffu, l0, k); l1 += __shfl_xor_sync(0xffffffffu, l1, k); }
+            if (q4 == 0) { s_ml[way * C::TQ + qt * 16 + g8] = make_float2(m0, l0 * back); s_ml[way * C::TQ + qt * 16 + g8 + 8] = make_float2(m1, l1 * back); }
+            __syncthreads();
+            float M0 = -INFINITY, M1 = -INFINITY, L0 = 0.f, L1 = 0.f;
+#pragma unroll
+            for (int w = 0; w < C::WAYS; w++) { M0 = fmaxf(M0, s_ml[w * C::TQ + qt * 16 + g8].x); M1 = fmaxf(M1, s_ml[w * C::TQ + qt * 16 + g8 + 8].x); }
+#pragma unroll
+            for (int w = 0; w < C::WAYS; w++) {
+                const float2 a = s_ml[w * C::TQ + qt * 16 + g8], b = s_ml[w * C::TQ + qt * 16 + g8 + 8];
+                L0 += a.x == -INFINITY ? 0.f : a.y * pg_ex2(a.x - M0);
+                L1 += b.x == -INFINITY ? 0.f : b.y * pg_ex2(b.x - M1);
+            }
+            const float un = back / csc, w0 = m0 == -INFINITY ? 0.f : pg_ex2(m0 - M0) * un, w1 = m1 == -INFINITY ? 0.f : pg_ex2(m1 - M1) * un;
+#pragma unroll
+            for (int b = 0; b < C::NT; b++) { o[b][0] *= w0; o[b][1] *= w0; o[b][2] *= w1; o[b][3] *= w1; }
+            const long long us = (long long)units[it.e] * d.nkv + (long long)it.h * it.n;        // the item's first unit
+            const int b0 = pg_block_of(us, U, blocks), b1 = pg_block_of(us + it.n - 1, U, blocks);
+            const int slot = 2 * blockIdx.x + ((int)blockIdx.x == b0 ? 1 : 0);
+            float* buf = (float*)qm;                      // [way - 1][tile][16][64]
+            const bool direct = pt.direct && b0 == b1;
+            const int r0 = pg_row(d, it.b), mrows = (pt.shared ? pg_row(d, d.n_seq) : pg_row(d, it.b + 1)) - r0;
+#pragma unroll
+            for (int sl = 0; sl < HD / 64; sl++) {        // 64 columns (n-tiles 8 sl ..) at a time
+                if (C::WAYS > 1) {
+                    if (sl) __syncthreads();
+                    if (way > 0) {
+                        float* w = buf + ((size_t)((way - 1) * NQT + qt) * 16 + g8) * 64 + 2 * q4;
+#pragma unroll
+                        for (int b = 0; b < 8; b++) {
+                            *(float2*)(w + 8 * b) = make_float2(o[8 * sl + b][0], o[8 * sl + b][1]);
+                            *(float2*)(w + 8 * 64 + 8 * b) = make_float2(o[8 * sl + b][2], o[8 * sl + b][3]);
+                        }
+                    }
+                    __syncthreads();
+                    if (way == 0) {
+#pragma unroll
+                        for (int x = 1; x < C::WAYS; x++) {
+                            const float* w = buf + ((size_t)((x - 1) * NQT + qt) * 16 + g8) * 64 + 2 * q4;
+#pragma unroll
+                            for (int b = 0; b < 8; b++) {
+                                const float2 a = *(const float2*)(w + 8 * b), c = *(const float2*)(w + 8 * 64 + 8 * b);
+                                o[8 * sl + b][0] += a.x; o[8 * sl + b][1] += a.y; o[8 * sl + b][2] += c.x; o[8 * sl + b][3] += c.y;
+                            }
+                        }
+                    }
+                }
+                if (way == 0) {
+#pragma unroll
+                    for (int hf = 0; hf < 2; hf++) {
+                        const int v = qt * 16 + g8 + 8 * hf, vec = it.t * C::TQ + v, row = vec / d.G, hh = vec % d.G;
+                        const float M = hf ? M1 : M0, L = hf ? L1 : L0;
+                        // packed values: the lane's columns of the four tiles of a 32-dimension group are eight neighbouring dimensions
+                        auto value = [&](int i) {         // i-th of the lane's 16 values of the slice, and its dimension
+                            return CT == PG_Q8 ? o[8 * sl + (i >> 3) * 4 + (i & 3)][2 * hf + ((i >> 2) & 1)] : o[8 * sl + (i >> 1)][2 * hf + (i & 1)];
+                        };
+                        auto dim = [&](int i) { return 64 * sl + (CT == PG_Q8 ? (i >> 3) * 32 + 8 * q4 + (i & 7) : (i >> 1) * 8 + 2 * q4 + (i & 1)); };
+                        if (row >= mrows) continue;
+                        const int head = it.h * d.G + hh;
+                        if (!direct) {
+                            const size_t at = b0 == b1 ? (size_t)(r0 + row) * (d.nkv * d.G) + head : (size_t)slot * C::TQ + v;
+                            float* w = (b0 == b1 ? pt.row_o : pt.o) + at * HD;
+#pragma unroll
+                            for (int i = 0; i < 16; i += 2) *(float2*)(w + dim(i)) = make_float2(value(i), value(i + 1));
+                            if (sl == 0 && q4 == 0) (b0 == b1 ? pt.row_ml : pt.ml)[at] = make_float2(M, L);
+                        } else {
+                            const float inv = (hf ? lim1 : lim0) > 0 && L != 0.f ? 1.f / L : 0.f;
+                            const u8* gp = io.gate ? io.gate + (long long)(r0 + row) * io.gate_stride + (long long)head * io.gate_head_stride : nullptr;
+                            u8* op = io.out + (long long)(r0 + row) * io.out_stride + (long long)head * HD * io.esz;
+#pragma unroll
+                            for (int i = 0; i < 16; i += 2) {
+                                float a = value(i) * inv, b = value(i + 1) * inv;
+                                if (inv == 0.f) { a = 0.f; b = 0.f; }
+                                if (gp) { const float2 z = pg_load2(gp + dim(i) * io.esz, io.type); a *= sz_sigmoid(z.x); b *= sz_sigmoid(z.y); }
+                                pg_store2(op + dim(i) * io.esz, io.type, a, b);
+                            }
+                            if (io.lse && sl == 0 && q4 == 0) io.lse[(size_t)(r0 + row) * (d.nkv * d.G) + head] = inv == 0.f ? -INFINITY : (M + log2f(L)) * 0.6931471805599453f;
+                        }
+                    }
+                }
+            }
+        }
+    }
+    asm volatile("cp.async.wait_all;" ::: "memory");
+}
+
+// What a set of kernels offers the host.
+struct PgKernels {
+    const void* fn;
+    int threads, smem, occ, tq;
+};
+PgKernels pg_kernels_f16(bool wide, int hd, int nqt);
+PgKernels pg_kernels_bf16(bool wide, int hd, int nqt);
+PgKernels pg_kernels_q8(bool wide, int hd, int nqt);
+
+template <int CT, bool WIDE, int HD, int NQT>
+PgKernels pg_one() {
+    using C = PgCfg<CT, WIDE, HD, NQT>;
+    return {(const void*)sz_pg_attend_kernel<CT, WIDE, HD, NQT>, C::NTH, C::SMEM, C::OCC, C::TQ};
+}
+template <int CT, bool WIDE, int HD>
+PgKernels pg_of_tiles(int nqt) { return nqt == 1 ? pg_one<CT, WIDE, HD, 1>() : nqt == 2 ? pg_one<CT, WIDE, HD, 2>() : pg_one<CT, WIDE, HD, 4>(); }
+template <int CT, bool WIDE>
+PgKernels pg_of_hd(int hd, int nqt) { return hd == 64 ? pg_of_tiles<CT, WIDE, 64>(nqt) : hd == 128 ? pg_of_tiles<CT, WIDE, 128>(nqt) : pg_of_tiles<CT, WIDE, 256>(nqt); }
+template <int CT>
+PgKernels pg_of(bool wide, int hd, int nqt) { return wide ? pg_of_hd<CT, true>(hd, nqt) : pg_of_hd<CT, false>(hd, nqt); }

@@ -7,6 +7,7 @@ LIB_PATH = os.path.join(_HERE, "libshadowzero_b200.so")
 
 OK, E_ARG, E_TYPE, E_CUDA, E_SCRATCH, E_DEVICE = 0, 1, 2, 3, 4, 5
 TYPE_F32, TYPE_F16, TYPE_Q8_0, TYPE_IQ3_S, TYPE_BF16 = 0, 1, 8, 21, 30
+TYPE_Q8_KV = 1101
 MAX_VERIFY, MAX_TOPK = 8, 16
 
 
@@ -151,6 +152,13 @@ SYMBOLS = {
     "sz_mma_cols_scratch_bytes": (C.c_int, [C.c_int, C.c_int, C.POINTER(C.c_int64)]),
     "sz_mma_cols": (C.c_int, [C.c_void_p, C.c_uint64, C.c_int64, C.c_uint64, C.c_int64, C.c_int, C.c_uint64, C.c_int64, C.c_uint64]),
     "sz_mma_cols_status": (C.c_int, [C.c_uint64, C.c_int, C.POINTER(C.c_int), C.c_uint64]),
+    "sz_paged_scratch_bytes": (C.c_int, [C.c_void_p, C.c_void_p, C.c_int, C.POINTER(C.c_int64)]),
+    "sz_paged_status": (C.c_int, [C.c_uint64, C.c_int, C.POINTER(C.c_int), C.c_uint64]),
+    "sz_paged_append": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_int, C.c_int, C.c_uint64, C.c_int64, C.c_uint64, C.c_int64, C.c_uint64, C.c_int64, C.c_int64,
+                                  C.c_uint64, C.c_int64, C.c_uint64, C.c_int64, C.c_uint64]),
+    "sz_paged_attend": (C.c_int, [C.c_void_p, C.c_void_p, C.c_int, C.c_int, C.c_float, C.c_uint64, C.c_int64, C.c_uint64, C.c_int64, C.c_int64, C.c_uint64, C.c_int64,
+                                  C.c_uint64, C.c_uint64, C.c_int64, C.c_uint64]),
+    "sz_sample_rows": (C.c_int, [C.c_int, C.c_uint64, C.c_int64, C.c_int, C.c_int] + [C.c_uint64] * 8),
     "sz_ep_unique_id": (C.c_int, [C.c_void_p]),
     "sz_ep_init": (C.c_int, [C.c_int, C.c_int, C.c_void_p]),
     "sz_ep_world": (C.c_int, []),

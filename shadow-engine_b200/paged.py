@@ -1,0 +1,143 @@
+"""A cache in pages (`sz_paged_*`): rows are appended to it and attend to it, over a prefix that the whole batch shares, too."""
+import ctypes as C
+import math
+
+import torch
+
+from . import lib as szlib
+
+TYPES = {torch.float32: szlib.TYPE_F32, torch.float16: szlib.TYPE_F16, torch.bfloat16: szlib.TYPE_BF16}
+
+
+class PagedCacheC(C.Structure):
+    """struct sz_paged_cache"""
+    _fields_ = [("type", C.c_int32), ("n_kv_head", C.c_int32), ("head_dim", C.c_int32), ("page_size", C.c_int32), ("n_pages", C.c_int32),
+                ("reserved", C.c_int32), ("k", C.c_uint64), ("v", C.c_uint64), ("page_stride", C.c_int64), ("head_stride", C.c_int64), ("pos_stride", C.c_int64)]
+
+
+class PagedBatchC(C.Structure):
+    """struct sz_paged_batch"""
+    _fields_ = [("n_seq", C.c_int32), ("rows", C.c_int32), ("max_pages", C.c_int32), ("shared_len", C.c_int32), ("pages", C.c_uint64),
+                ("row_start", C.c_uint64), ("lens", C.c_uint64), ("shared_pages", C.c_uint64)]
+
+
+class PagedRopeC(C.Structure):
+    """struct sz_paged_rope"""
+    _fields_ = [("dims", C.c_int32), ("eps", C.c_float), ("theta", C.c_double), ("q_norm", C.c_uint64), ("k_norm", C.c_uint64)]
+
+
+def head_bytes(head_dim):
+    """Bytes of a packed head (SZ_TYPE_Q8_KV): head_dim codes, then head_dim / 32 f16 scales, padded to 16 bytes."""
+    return head_dim + ((head_dim // 32 * 2 + 15) & ~15)
+
+
+class Cache:
+    """The pools of one layer: k and v [pages, kv heads, positions a page, head_dim] of f16 or bf16, or of uint8 packed heads
+    [.., head_bytes(head_dim)].  Any order of the first three dimensions (a transposed view is one), the last contiguous."""
+
+    def __init__(self, k, v, head_dim):
+        if k.dim() != 4 or v.shape != k.shape or v.stride() != k.stride() or v.dtype != k.dtype or v.device != k.device:
+            raise ValueError("k and v: two pools of one shape, type and layout, [pages, kv heads, positions, head]")
+        packed = k.dtype == torch.uint8
+        if not packed and k.dtype not in (torch.float16, torch.bfloat16):
+            raise ValueError("pools of float16, bfloat16 or uint8 (packed heads)")
+        if k.stride(3) != 1 or k.shape[3] != (head_bytes(head_dim) if packed else head_dim):
+            raise ValueError("a head is %d contiguous elements" % (head_bytes(head_dim) if packed else head_dim))
+        self.k, self.v, self.device, self.head_dim = k, v, k.device, head_dim
+        e = k.element_size()
+        self.c = PagedCacheC(type=szlib.TYPE_Q8_KV if packed else TYPES[k.dtype], n_kv_head=k.shape[1], head_dim=head_dim, page_size=k.shape[2], n_pages=k.shape[0],
+                             k=k.data_ptr(), v=v.data_ptr(), page_stride=max(k.stride(0) * e, k.shape[3] * e), head_stride=k.stride(1) * e, pos_stride=k.stride(2) * e)
+
+
+class Step:
+    """The tables of a batch over a cache, and the scratch of its calls.  pages int32 [sequences, pages of one], row_start int32 [sequences + 1],
+    lens int32 [sequences] (all positions, the step's rows included) are the caller's tensors: change their values from step to step.
+    shared_pages int32: the pages of the first shared_len positions, the same for all sequences.  Calls on one Step follow one another on
+    a stream; what may overlap needs a Step each."""
+
+    def __init__(self, cache, pages, row_start, lens, rows, n_head, shared_pages=None, shared_len=0):
+        self.lib = szlib.load()
+        for name, t, dims in (("pages", pages, 2), ("row_start", row_start, 1), ("lens", lens, 1)) + ((("shared_pages", shared_pages, 1),) if shared_len else ()):
+            if t is None or t.dtype != torch.int32 or t.dim() != dims or not t.is_contiguous() or t.device != cache.device:
+                raise ValueError("%s: a contiguous int32 tensor of %d dimension(s) on the cache's device" % (name, dims))
+        n = lens.shape[0]
+        if pages.shape[0] != n or row_start.shape[0] != n + 1:
+            raise ValueError("pages and row_start: one row a sequence, one entry more than sequences")
+        if shared_len and shared_pages.shape[0] * cache.c.page_size < shared_len:
+            raise ValueError("shared_pages hold %d positions, shared_len is %d" % (shared_pages.shape[0] * cache.c.page_size, shared_len))
+        self.cache, self.n_head, self.rows, self.device = cache, n_head, rows, cache.device
+        self._keep = (pages, row_start, lens, shared_pages)
+        self.b = PagedBatchC(n_seq=n, rows=rows, max_pages=pages.shape[1], shared_len=shared_len, pages=pages.data_ptr(), row_start=row_start.data_ptr(),
+                             lens=lens.data_ptr(), shared_pages=shared_pages.data_ptr() if shared_len else 0)
+        need = C.c_int64()
+        self._c, self._b = C.byref(cache.c), C.byref(self.b)
+        szlib.check(self.lib.sz_paged_scratch_bytes(self._c, self._b, n_head, C.byref(need)))
+        with torch.cuda.device(self.device):
+            self._mem = torch.empty(need.value + 256, dtype=torch.uint8, device=self.device)
+            self.scratch, self.scratch_bytes = self._mem.data_ptr() + (-self._mem.data_ptr()) % 256, need.value
+            szlib.check(self.lib.sz_paged_status(self.scratch, 1, None, self._stream()))
+        self._rope = {}
+
+    def _stream(self):
+        return torch.cuda.current_stream(self.device).cuda_stream
+
+    def _rows(self, name, t, heads, dtype=None):
+        if t.dim() != 3 or t.shape[0] != self.rows or t.shape[1] != heads or t.shape[2] != self.cache.head_dim or t.stride(2) != 1 or t.device != self.device:
+            raise ValueError("%s: [%d, %d, %d], the last dimension contiguous, on the cache's device" % (name, self.rows, heads, self.cache.head_dim))
+        if t.dtype not in TYPES or (dtype is not None and t.dtype != dtype):
+            raise ValueError("%s: float32, float16 or bfloat16, the same for all rows of a call" % name)
+        return t
+
+    def append(self, k, v, q=None, q_out=None, rope_dims=0, theta=1e4, q_norm=None, k_norm=None, eps=1e-6):
+        """Stores the rows' keys (normed, turned) and values at their positions; returns the rows' queries, normed and turned (None without q).
+        k, v [rows, kv heads, head_dim]; q [rows, heads, head_dim] (any stride of heads); q_norm, k_norm float32 [head_dim]."""
+        nkv = self.cache.c.n_kv_head
+        self._rows("k", k, nkv), self._rows("v", v, nkv, k.dtype)
+        hd = self.cache.head_dim
+        if q is not None:
+            self._rows("q", q, self.n_head, k.dtype)
+            if q_out is None:
+                q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+            self._rows("q_out", q_out, self.n_head, k.dtype)
+        for name, t in (("k", k), ("v", v)) + ((("q_out", q_out),) if q is not None else ()):
+            if t.shape[1] > 1 and t.stride(1) != hd:
+                raise ValueError("%s: heads side by side" % name)
+        for w in (q_norm, k_norm):
+            if w is not None and (w.dtype != torch.float32 or w.shape != (hd,) or w.stride(0) != 1 or w.device != self.device):
+                raise ValueError("norm weights: float32 [%d] on the cache's device" % hd)
+        rope = PagedRopeC(rope_dims, eps, theta, 0 if q_norm is None else q_norm.data_ptr(), 0 if k_norm is None else k_norm.data_ptr())
+        with torch.cuda.device(self.device):
+            szlib.check(self.lib.sz_paged_append(self._c, self._b, C.byref(rope), TYPES[k.dtype], self.n_head, k.data_ptr(), k.stride(0), v.data_ptr(), v.stride(0),
+                                                 0 if q is None else q.data_ptr(), 0 if q is None else q.stride(0), 0 if q is None else max(q.stride(1), hd),
+                                                 0 if q is None else q_out.data_ptr(), 0 if q is None else q_out.stride(0), self.scratch, self.scratch_bytes, self._stream()))
+        return q_out
+
+    def attend(self, q, out=None, scale=None, gate=None, lse=None):
+        """Attention of the rows over their sequences' positions up to their own, shared ones first.  q [rows, heads, head_dim]; gate: the
+        same (any stride of heads), out *= sigmoid(gate); lse float32 [rows, heads] receives the logarithm of the softmax's denominator; scale 1 / sqrt(head_dim)."""
+        hd = self.cache.head_dim
+        self._rows("q", q, self.n_head)
+        if out is None:
+            out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        self._rows("out", out, self.n_head, q.dtype)
+        for name, t in (("q", q), ("out", out)):
+            if t.shape[1] > 1 and t.stride(1) != hd:
+                raise ValueError("%s: heads side by side" % name)
+        if gate is not None:
+            self._rows("gate", gate, self.n_head, q.dtype)
+        if lse is not None and (lse.dtype != torch.float32 or lse.shape != (self.rows, self.n_head) or not lse.is_contiguous() or lse.device != self.device):
+            raise ValueError("lse: float32 [%d, %d] on the cache's device" % (self.rows, self.n_head))
+        with torch.cuda.device(self.device):
+            szlib.check(self.lib.sz_paged_attend(self._c, self._b, TYPES[q.dtype], self.n_head, 1 / math.sqrt(hd) if scale is None else scale, q.data_ptr(), q.stride(0),
+                                                 0 if gate is None else gate.data_ptr(), 0 if gate is None else gate.stride(0), 0 if gate is None else max(gate.stride(1), hd),
+                                                 out.data_ptr(), out.stride(0), 0 if lse is None else lse.data_ptr(), self.scratch, self.scratch_bytes, self._stream()))
+        return out
+
+    def status(self):
+        """What the calls so far have met (synchronises): 0, or the bits of sz_paged_status."""
+        code = C.c_int()
+        with torch.cuda.device(self.device):
+            rc = self.lib.sz_paged_status(self.scratch, 0, C.byref(code), self._stream())
+        if rc not in (szlib.OK, szlib.E_DEVICE):
+            szlib.check(rc)
+        return code.value

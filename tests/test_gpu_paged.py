@@ -1,0 +1,482 @@
+"""The paged cache on the GPU: append and attention against plain 64-bit arithmetic, at the sizes, types, layouts and masks where they can go wrong."""
+import math
+
+import numpy as np
+import pytest
+import torch
+
+from tests.util import pkg
+
+paged, szlib = pkg.paged, pkg.lib
+pytestmark = pytest.mark.gpu
+
+IO = {"f32": torch.float32, "f16": torch.float16, "bf16": torch.bfloat16}
+HALF_STEP = {torch.float32: 2.0 ** -24, torch.float16: 2.0 ** -11, torch.bfloat16: 2.0 ** -8}
+
+
+# ---- the plain side ---------------------------------------------------------------------------------------------------------------------
+def q8_pack(x):
+    """The session's packed heads (per-32 symmetric int8, f16 scales), the oracle's arithmetic in torch."""
+    hd = x.shape[-1]
+    g = x.float().reshape(*x.shape[:-1], hd // 32, 32)
+    sc = (g.abs().amax(-1) * np.float32(1 / 127)).half()
+    inv = torch.where(sc > 0, 1 / sc.float(), torch.zeros_like(sc, dtype=torch.float32))
+    codes = torch.round(g * inv[..., None]).clamp(-127, 127).to(torch.int8).reshape(x.shape).view(torch.uint8)
+    out = torch.zeros(*x.shape[:-1], paged.head_bytes(hd), dtype=torch.uint8, device=x.device)
+    out[..., :hd] = codes
+    out[..., hd:hd + hd // 16] = sc.view(torch.uint8)
+    return out
+
+
+def values(pool, hd):
+    if pool.dtype != torch.uint8:
+        return pool.double()
+    sc = pool[..., hd:hd + hd // 16].contiguous().view(torch.float16).double()
+    return (pool[..., :hd].view(torch.int8).double().reshape(*pool.shape[:-1], hd // 32, 32) * sc[..., None]).reshape(*pool.shape[:-1], hd)
+
+
+class Case:
+    """A batch over a paged cache.  lens: positions of the sequences, ms: their rows; `pad` rows follow the last sequence."""
+
+    def __init__(self, lens, ms, nh=4, nkv=2, hd=64, page=16, io="f32", cache="f16", shared=0, pad=0, layout="hnd", seed=0, scale_kv=1.0, extra_pages=0):
+        g = torch.Generator(device="cuda").manual_seed(seed)
+        self.rnd = lambda *s: torch.randn(*s, device="cuda", generator=g)
+        self.lens, self.ms, self.nh, self.nkv, self.hd, self.ps, self.shared, self.cache_type = lens, ms, nh, nkv, hd, page, shared, cache
+        self.io = IO[io]
+        n = len(lens)
+        own = [max(0, -(-(x - shared) // page)) for x in lens]
+        width, nsh = max(own + [1]) + extra_pages, -(-shared // page)
+        total = sum(own) + nsh + 3
+        order = torch.randperm(total, device="cuda", generator=g).to(torch.int32)
+        pages = torch.full((n, width), -7, dtype=torch.int32, device="cuda")          # entries that no position needs are no pages
+        at = 0
+        for b in range(n):
+            pages[b, :own[b]] = order[at:at + own[b]]
+            at += own[b]
+        self.pages, self.shared_pages = pages, order[at:at + nsh].contiguous()
+        self.rows = sum(ms) + pad
+        starts = np.concatenate([[0], np.cumsum(ms)]).astype(np.int32)
+        self.row_start = torch.from_numpy(starts).cuda()
+        self.len_t = torch.tensor(lens, dtype=torch.int32, device="cuda")
+        shape = (total, nkv, page, hd) if layout == "hnd" else (total, page, nkv, hd)
+        k, v = scale_kv * self.rnd(*shape), scale_kv * self.rnd(*shape)
+        k, v = (q8_pack(k), q8_pack(v)) if cache == "q8" else (k.to(IO[cache]), v.to(IO[cache]))
+        if layout == "nhd":
+            k, v = k.transpose(1, 2), v.transpose(1, 2)
+        self.k, self.v = k, v
+        self.q = (1.5 * self.rnd(self.rows, nh, hd)).to(self.io)
+        self.make_step()
+
+    def make_step(self):
+        self.cache = paged.Cache(self.k, self.v, self.hd)
+        self.step = paged.Step(self.cache, self.pages, self.row_start, self.len_t, self.rows, self.nh, shared_pages=self.shared_pages, shared_len=self.shared)
+
+    def positions(self, pool, b):
+        """[positions of sequence b, kv heads, hd] in 64 bits."""
+        of = lambda ids, n: values(pool[ids.long()], self.hd).transpose(1, 2).reshape(-1, self.nkv, self.hd)[:n]  # noqa: E731
+        own = max(0, self.lens[b] - self.shared)
+        parts = [of(self.shared_pages, self.shared)] if self.shared else []
+        if own:
+            parts.append(of(self.pages[b, :-(-own // self.ps)], own))
+        return torch.cat(parts) if parts else torch.zeros(0, self.nkv, self.hd, dtype=torch.float64, device="cuda")
+
+    def want(self, gate=None, scale=None):
+        """(outputs, the sum of weights times |values|, log of the denominators), 64-bit; rows behind the sequences are not set."""
+        out = torch.zeros(self.rows, self.nh, self.hd, dtype=torch.float64, device="cuda")
+        mag, lse = torch.zeros_like(out), torch.full((self.rows, self.nh), -math.inf, dtype=torch.float64, device="cuda")
+        scale = 1 / math.sqrt(self.hd) if scale is None else scale
+        r = 0
+        for b, m in enumerate(self.ms):
+            k, v = self.positions(self.k, b), self.positions(self.v, b)
+            for j in range(m):
+                p = self.lens[b] - m + j
+                if p >= self.shared:
+                    for h in range(self.nh):
+                        s = scale * (k[:p + 1, h // (self.nh // self.nkv)] @ self.q[r, h].double())
+                        w = torch.softmax(s, 0)
+                        out[r, h], mag[r, h] = w @ v[:p + 1, h // (self.nh // self.nkv)], w @ v[:p + 1, h // (self.nh // self.nkv)].abs()
+                        lse[r, h] = torch.logsumexp(s, 0)
+                r += 1
+        if gate is not None:
+            z = torch.sigmoid(gate.double())
+            out, mag = out * z, mag * z
+        return out, mag, lse
+
+    def tolerance(self, want, mag):
+        """Half a step of the result's type; before it, f32 arithmetic: a score is a sum of hd products (hd 2^-23 of their magnitudes, |q||k| scale below 12
+        sigma = 30 here, in units of its own exponent), which moves every weight by that much, and sums of up to 64 partial sums - 2^-13 of the
+        weighted magnitudes holds f32's part with a wide margin; 16-bit results carry weights of 11 bits and more: 2^-10 of the magnitudes."""
+        return HALF_STEP[self.io] * want.abs() + (2.0 ** -13 if self.io == torch.float32 else 2.0 ** -10) * mag + 1e-30
+
+    def check(self, gate=None, **kw):
+        out = torch.full_like(self.q, 77.0)
+        lse = torch.full((self.rows, self.nh), 77.0, device="cuda")
+        self.step.attend(self.q, out=out, gate=gate, lse=lse, **kw)
+        assert self.step.status() == 0
+        want, mag, wl = self.want(gate, **kw)
+        n = sum(self.ms)
+        off = (out.double() - want).abs() / self.tolerance(want, mag)
+        assert float(off[:n].max()) < 1.0, "%.3g of the tolerance at %s" % (float(off[:n].max()), np.unravel_index(int(off[:n].argmax()), off[:n].shape))
+        assert bool((out[n:] == 77.0).all()) and bool((lse[n:] == 77.0).all())          # a padded batch's rows are left as they were
+        seen = torch.isfinite(wl[:n])
+        assert bool(((lse[:n].double() - wl[:n]).abs()[seen] < 2e-4).all()) and bool((lse[:n][~seen] == -math.inf).all())
+        return out
+
+
+# ---- attention ---------------------------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("cache", ["f16", "bf16", "q8"])
+@pytest.mark.parametrize("io", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("hd", [64, 128, 256])
+def test_every_type_and_width(io, cache, hd):
+    Case([1, 77, 130], [1, 2, 5], nh=8, nkv=2, hd=hd, io=io, cache=cache, seed=hd).check()
+
+
+@pytest.mark.parametrize("lens", [[1], [2], [63], [64], [65], [16 * 64], [1000, 1, 64, 129], [0, 5, 0], [3, 0, 0, 700]])
+def test_lengths_from_nothing_on(lens):
+    c = Case(lens, [1] * len(lens), io="bf16", cache="bf16")
+    out = c.check()
+    for b, x in enumerate(lens):
+        if x == 0:
+            assert bool((out[b] == 0).all())
+
+
+@pytest.mark.parametrize("nh,nkv", [(1, 1), (5, 5), (6, 2), (7, 1), (16, 2), (64, 1), (3, 1)])
+@pytest.mark.parametrize("m", [1, 3, 9])
+def test_head_groups(nh, nkv, m):
+    Case([150, 40 + m], [m, m], nh=nh, nkv=nkv, hd=64, seed=nh * 10 + m).check()
+
+
+@pytest.mark.parametrize("page", [8, 16, 64, 128, 1024])
+@pytest.mark.parametrize("layout", ["hnd", "nhd"])
+def test_pages_and_layouts(page, layout):
+    Case([300, 17, page + 1], [2, 1, 4], page=page, layout=layout, cache="q8", hd=128, seed=page).check()
+
+
+@pytest.mark.parametrize("ms", [[17], [100], [1, 60, 3], [33, 0, 2]])
+@pytest.mark.parametrize("before", [0, 1, 200])
+def test_prompts(ms, before):
+    Case([m + before for m in ms], ms, nh=4, nkv=1, hd=128, io="bf16", cache="bf16", seed=before).check()
+
+
+@pytest.mark.parametrize("shared", [1, 16, 63, 64, 500, 1037])
+@pytest.mark.parametrize("io,cache", [("f32", "q8"), ("bf16", "bf16"), ("f16", "f16")])
+def test_a_shared_prefix(shared, io, cache):
+    Case([shared + x for x in (1, 40, 3, 130, 2)], [1, 4, 3, 2, 1], nh=8, nkv=2, hd=64, io=io, cache=cache, shared=shared, pad=2, seed=shared).check()
+
+
+def test_a_shared_prefix_of_many_rows():
+    Case([700 + 5 * i for i in range(40)], [1 + i % 4 for i in range(40)], nh=16, nkv=2, hd=128, io="bf16", cache="bf16", shared=641, seed=3).check()
+
+
+def test_sequences_in_front_of_the_shared_positions_attend_to_nothing():
+    c = Case([70, 64, 10, 0], [2, 1, 1, 1], shared=64, seed=5)
+    out = c.check()
+    assert bool((out[2:] == 0).all())
+
+
+def test_rows_before_the_first_position():
+    c = Case([3, 200], [5, 2], seed=6)              # two rows of a padded sequence lie before position 0
+    out = c.check()
+    assert bool((out[:2] == 0).all())
+
+
+@pytest.mark.parametrize("cache", ["f16", "bf16", "q8"])
+def test_a_long_sequence_beside_short_ones(cache):
+    Case([20000, 3, 900], [1, 2, 1], nh=8, nkv=1, hd=128, io="f32", cache=cache, page=64, seed=8).check()
+
+
+def test_more_sequences_than_a_block_plans_for():
+    Case([1 + (7 * i) % 50 for i in range(600)], [1] * 600, nh=2, nkv=1, hd=64, io="bf16", cache="bf16", seed=9).check()
+
+
+def test_more_tiles_than_a_block_plans_for():
+    Case([2600], [2600], nh=16, nkv=1, hd=64, io="bf16", cache="bf16", seed=10, page=128).check()
+
+
+def test_gate_scale_and_strides():
+    c = Case([90, 300], [3, 1], nh=8, nkv=2, hd=64, io="bf16", cache="bf16", seed=11)
+    both = c.rnd(c.rows, c.nh, 2 * c.hd).to(c.io)      # queries and gates alternate
+    c.check(gate=both[:, :, c.hd:])
+    c.check(scale=0.3)
+    wide = torch.zeros(c.rows, c.nh * c.hd + 64, dtype=c.io, device="cuda")
+    wide[:, :c.nh * c.hd] = c.q.reshape(c.rows, -1)
+    out = torch.full_like(wide, 5.0)
+    c.step.attend(wide[:, :c.nh * c.hd].view(c.rows, c.nh, c.hd), out=out[:, :c.nh * c.hd].view(c.rows, c.nh, c.hd))
+    assert torch.equal(out[:, :c.nh * c.hd].reshape(c.q.shape), c.check()) and bool((out[:, c.nh * c.hd:] == 5.0).all())
+
+
+@pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf])
+@pytest.mark.parametrize("cache", ["f16", "bf16"])
+def test_what_hidden_positions_hold_does_not_matter(cache, bad):
+    """Behind a sequence's end in its last page, and at positions later than a row's own, keys and values may be anything."""
+    c = Case([70, 33], [4, 2], cache=cache, io="f32", nh=8, nkv=2, seed=12)
+    before = c.check()
+    last = c.pages[0, (70 - 1) // 16]
+    c.k[last, :, 70 % 16:] = bad
+    c.v[last, :, 70 % 16:] = bad
+    out = torch.empty_like(c.q)
+    c.step.attend(c.q, out=out)
+    assert torch.equal(out, before)
+    c.v[last, :, 69 % 16, 5] = bad                     # the last row's own value: its output, and no other row's
+    c.step.attend(c.q, out=out)
+    rel = (out[:3].double() - before[:3].double()).abs().max() / before.abs().max()
+    assert float(rel) < 2.0 ** -13 and torch.equal(out[4:], before[4:])
+    hit = out[3, :, 5]
+    assert not bool(torch.isfinite(hit).any()) and bool(torch.isfinite(out[3, :, :5]).all())
+
+
+@pytest.mark.parametrize("io,cache", [("f32", "f16"), ("f32", "q8"), ("bf16", "bf16"), ("f32", "bf16")])
+def test_large_and_small_magnitudes(io, cache):
+    for kv, q in ((1e-3, 100.0), (100.0, 0.01), (300.0, 0.003)):
+        c = Case([130, 64], [2, 1], io=io, cache=cache, nh=8, nkv=2, seed=13, scale_kv=kv)
+        c.q.mul_(q)
+        c.check()
+
+
+def test_far_apart_scores():
+    """One position takes all the weight; the largest comes first, and last."""
+    for at in (0, 199):
+        c = Case([200], [1], io="f32", cache="f16", nh=2, nkv=1, hd=64, seed=14)
+        page, slot = int(c.pages[0, at // 16]), at % 16
+        c.k[page, 0, slot] = (c.q[0, 0] * 30).half()
+        c.check()
+
+
+def test_bad_pages_are_left_out_and_reported():
+    c = Case([100, 50], [1, 1], nh=4, nkv=2, hd=64, seed=15)
+    keep = c.pages.clone()
+    for bad in (-1, c.k.shape[0], 2 ** 31 - 1):
+        c.pages.copy_(keep)
+        c.pages[0, 2] = bad                            # positions 32 .. 47
+        c.step.attend(c.q)
+        assert c.step.status() == 1
+        szlib.check(c.step.lib.sz_paged_status(c.step.scratch, 1, None, 0))
+        torch.cuda.synchronize()
+        out = c.step.attend(c.q)
+        c.pages.copy_(keep)
+        k, v = c.positions(c.k, 0), c.positions(c.v, 0)
+        seen = torch.cat([torch.arange(32), torch.arange(48, 100)]).cuda()
+        for h in range(4):
+            w = torch.softmax(k[seen, h // 2] @ c.q[0, h].double() / 8, 0)
+            assert float((w @ v[seen, h // 2] - out[0, h].double()).abs().max()) < 1e-4
+        szlib.check(c.step.lib.sz_paged_status(c.step.scratch, 1, None, 0))
+
+
+def test_lengths_behind_the_table_and_row_starts_behind_the_rows():
+    c = Case([40, 20], [1, 1], seed=16)
+    c.len_t[1] = 16 * c.pages.shape[1] + 1
+    c.pages[1] = c.pages[0]
+    c.step.attend(c.q)
+    assert c.step.status() == 2
+    c = Case([40, 20], [1, 1], seed=16)
+    c.row_start[2] = 9
+    c.step.attend(c.q)
+    assert c.step.status() == 8
+
+
+def test_a_row_is_the_same_whoever_shares_the_step():
+    """16-bit caches: nothing but the cuts between blocks depends on the other sequences - within f32 rounding of each other."""
+    a = Case([333], [2], nh=8, nkv=2, hd=128, io="f32", cache="f16", seed=17)
+    out = a.step.attend(a.q)
+    again = a.step.attend(a.q)
+    assert torch.equal(out, again)
+
+
+def test_a_captured_step_serves_a_growing_batch():
+    c = Case([100, 37, 64], [1, 1, 1], nh=8, nkv=2, hd=128, io="bf16", cache="bf16", seed=18, extra_pages=2)
+    new = torch.randperm(c.k.shape[0], device="cuda").to(torch.int32)
+    out, kin, vin = torch.empty_like(c.q), c.rnd(3, 2, 128).bfloat16(), c.rnd(3, 2, 128).bfloat16()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        c.step.append(kin, vin, rope_dims=64)
+        c.step.attend(c.q, out=out)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        c.step.append(kin, vin, rope_dims=64)
+        c.step.attend(c.q, out=out)
+    for grow in range(3):
+        c.lens = [x + (5 if grow else 0) for x in c.lens]
+        for b, x in enumerate(c.lens):                 # sequences go on into further pages (any: what is checked is what they then hold)
+            need = -(-x // 16)
+            c.pages[b, need - 1] = new[(grow * 3 + b) % len(new)] if int(c.pages[b, need - 1]) < 0 else c.pages[b, need - 1]
+        c.len_t.copy_(torch.tensor(c.lens, dtype=torch.int32))
+        c.q.copy_(c.rnd(*c.q.shape))
+        graph.replay()
+        torch.cuda.synchronize()
+        want, mag, _ = c.want()
+        assert float(((out.double() - want).abs() / c.tolerance(want, mag)).max()) < 1.0
+    assert c.step.status() == 0
+
+
+def test_another_stream():
+    c = Case([500, 70], [2, 3], nh=8, nkv=2, hd=64, io="bf16", cache="bf16", seed=19)
+    want = c.check()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        out = c.step.attend(c.q)
+    side.synchronize()
+    assert torch.equal(out, want)
+
+
+# ---- append ------------------------------------------------------------------------------------------------------------------------------
+def rotated(x, w, pos, dims, theta, eps):
+    x = x.double()
+    if w is not None:
+        x = x / torch.sqrt((x * x).mean(-1, keepdim=True) + eps) * w.double()
+    if not dims:
+        return x
+    h = dims // 2
+    a = torch.outer(pos.double(), theta ** (-torch.arange(0, dims, 2, dtype=torch.float64, device=x.device) / dims))[:, None, :]
+    u, v = x[..., :h], x[..., h:dims]
+    return torch.cat([u * a.cos() - v * a.sin(), v * a.cos() + u * a.sin(), x[..., dims:]], -1)
+
+
+def check_append(c, dims, norm, theta=1e7, with_q=True, q=None, q_out=None):
+    nkv, hd, n = c.nkv, c.hd, sum(c.ms)
+    kin, vin = c.rnd(c.rows, nkv, hd).to(c.io), c.rnd(c.rows, nkv, hd).to(c.io)
+    q = c.q if q is None else q
+    qn, kn = (1 + 0.1 * c.rnd(hd), 1 + 0.1 * c.rnd(hd)) if norm else (None, None)
+    k0, v0 = c.k.clone(), c.v.clone()
+    if with_q and q_out is None:
+        q_out = torch.full((c.rows, c.nh, hd), 55.0, dtype=c.io, device="cuda")
+    qin = q.clone()
+    got = c.step.append(kin, vin, q=q if with_q else None, q_out=q_out if with_q else None, rope_dims=dims, theta=theta, q_norm=qn, k_norm=kn, eps=1e-6)
+    assert c.step.status() == 0
+    pos = torch.cat([torch.arange(x - m, x) for x, m in zip(c.lens, c.ms)]).cuda()
+    kw, vw = rotated(kin[:n], kn, pos, dims, theta, 1e-6), vin[:n].double()
+    touched = torch.zeros(c.k.shape[0], c.ps, dtype=torch.bool, device="cuda")
+    r = 0
+    for b, (x, m) in enumerate(zip(c.lens, c.ms)):
+        for p in range(x - m, x):
+            if p >= 0:
+                o = p - c.shared
+                page, slot = int(c.pages[b, o // c.ps]), o % c.ps
+                touched[page, slot] = True
+                for pool, want in ((c.k, kw[r]), (c.v, vw[r])):
+                    have = values(pool[page, :, slot], hd)
+                    if pool.dtype == torch.uint8:      # half a code, and f16's rounding of the scale over 127 codes of it, and f32's before
+                        big = want.reshape(nkv, hd // 32, 32).abs().amax(-1, keepdim=True).expand(-1, -1, 32).reshape(nkv, hd)
+                        tol = big / 127 * (0.5 + 127 * 2.0 ** -11 + 127 * 2.0 ** -21) + 2.0 ** -24
+                        assert bool((pool[page, :, slot, hd + hd // 16:] == 0).all())
+                    else:                              # a rounding of the cache's type, f32's rounding of norm and rotation (of a pair's length) before it
+                        tol = HALF_STEP[pool.dtype] * want.abs() + 2.0 ** -20 * want.abs().amax() + 2.0 ** -25
+                    assert bool(((have - want).abs() <= tol).all())
+            r += 1
+    keep = ~touched[:, None, :, None].expand(*c.k.shape)
+    assert torch.equal(c.k[keep], k0[keep]) and torch.equal(c.v[keep], v0[keep])      # no other position
+    if with_q:
+        want = rotated(qin[:n], qn, pos, dims, theta, 1e-6)
+        there = pos >= 0
+        tol = HALF_STEP[c.io] * want.abs() + 2.0 ** -20 * want.abs().amax()
+        assert bool(((got[:n].double() - want).abs() <= tol)[there].all())
+        if got is not q:
+            assert bool((got[:n][~there] == 55.0).all()) and bool((got[n:] == 55.0).all())
+
+
+@pytest.mark.parametrize("cache", ["f16", "bf16", "q8"])
+@pytest.mark.parametrize("io", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("hd,dims,norm", [(64, 32, True), (128, 128, False), (256, 64, True), (64, 0, True), (128, 2, False), (256, 256, True)])
+def test_append(io, cache, hd, dims, norm):
+    check_append(Case([1, 40, 17], [1, 3, 17], nh=4, nkv=2, hd=hd, io=io, cache=cache, seed=hd + dims), dims, norm)
+
+
+@pytest.mark.parametrize("page,layout", [(8, "nhd"), (128, "hnd"), (1024, "nhd")])
+def test_append_pages_and_layouts(page, layout):
+    check_append(Case([300, 17, page + 1], [2, 1, 4], page=page, layout=layout, io="bf16", cache="q8", hd=128, seed=page, pad=3), 128, False)
+
+
+def test_append_behind_a_shared_prefix_and_without_queries():
+    check_append(Case([70, 101], [2, 37], shared=64, page=16, seed=21), 32, True)
+    check_append(Case([70, 101], [2, 37], page=16, seed=22), 32, True, with_q=False)
+
+
+def test_append_in_place_and_from_alternating_heads():
+    c = Case([9, 33], [2, 5], nh=4, hd=128, io="bf16", cache="bf16", seed=23)
+    check_append(c, 64, True, q=c.q, q_out=c.q)
+    both = c.rnd(c.rows, c.nh, 2 * c.hd).to(c.io)
+    check_append(c, 64, True, q=both[:, :, :c.hd])
+
+
+def test_append_leaves_out_rows_before_position_zero():
+    check_append(Case([3, 20], [5, 2], seed=24), 32, False)
+
+
+@pytest.mark.parametrize("far", [24576, 1048575, 16777217])
+def test_append_at_far_positions(far):
+    """The table's early pages may be anything; the angle of a far position keeps its digits."""
+    c = Case([20], [2], nh=4, nkv=1, hd=64, io="f32", cache="f16", page=1024, seed=25)
+    width = far // 1024 + 1
+    c.pages = torch.zeros(1, width, dtype=torch.int32, device="cuda")
+    c.lens = [far + 1]
+    c.len_t.fill_(far + 1)
+    c.make_step()
+    check_append(c, 64, False, theta=1e4)
+
+
+def test_append_reports_what_it_leaves_out():
+    c = Case([40, 20], [1, 1], seed=26)
+    kin = c.rnd(2, 2, 64)
+    k0 = c.k.clone()
+    c.pages[0, 2] = 10 ** 6
+    c.step.append(kin, kin)
+    assert c.step.status() == 1
+    o = 19
+    page = int(c.pages[1, 1])
+    k0[page, :, o % 16] = kin[1].half()
+    assert torch.equal(c.k, k0)
+    c = Case([70, 30], [1, 1], shared=64, seed=27)
+    k0 = c.k.clone()
+    c.step.append(c.rnd(2, 2, 64), c.rnd(2, 2, 64))
+    assert c.step.status() == 4
+    k0[int(c.pages[0, 0]), :, 5] = c.k[int(c.pages[0, 0]), :, 5]
+    assert torch.equal(c.k, k0)
+    c = Case([40, 20], [1, 1], seed=28)
+    c.len_t[0] = 16 * c.pages.shape[1] + 1
+    c.step.append(c.rnd(2, 2, 64), c.rnd(2, 2, 64))
+    assert c.step.status() == 2
+
+
+def test_steps_as_a_server_makes_them():
+    """A prompt behind a shared system prompt, then tokens one after the other and drafts: what is appended is what is attended to."""
+    nh, nkv, hd, ps, shared = 8, 2, 128, 16, 50
+    g = torch.Generator(device="cuda").manual_seed(31)
+    rnd = lambda *s: torch.randn(*s, device="cuda", generator=g)  # noqa: E731
+    n, width = 3, 8
+    total = n * width + 4
+    k, v = torch.full((total, nkv, ps, hd), math.nan, device="cuda").half(), torch.full((total, nkv, ps, hd), math.nan, device="cuda").half()
+    cache = paged.Cache(k, v, hd)
+    order = torch.randperm(total, device="cuda", generator=g).to(torch.int32)
+    pages, shared_pages = order[:n * width].view(n, width).contiguous(), order[n * width:].contiguous()
+    lens, rs = torch.zeros(n, dtype=torch.int32, device="cuda"), torch.zeros(n + 1, dtype=torch.int32, device="cuda")
+    sys_k, sys_v = rnd(shared, nkv, hd), rnd(shared, nkv, hd)
+    # the system prompt goes in as a sequence of its own, whose pages are then the shared list
+    one = paged.Step(cache, shared_pages.view(1, -1), torch.tensor([0, shared], dtype=torch.int32, device="cuda"), torch.tensor([shared], dtype=torch.int32, device="cuda"), shared, nh)
+    one.append(sys_k, sys_v, rope_dims=hd)
+    assert one.status() == 0
+    hist_k = [rotated(sys_k, None, torch.arange(shared, device="cuda"), hd, 1e4, 0) for _ in range(n)]
+    hist_v = [sys_v.double() for _ in range(n)]
+    for ms in ([20, 7, 33], [1, 1, 1], [4, 1, 3], [1, 4, 1]):
+        R = sum(ms)
+        rs.copy_(torch.tensor([0] + list(np.cumsum(ms)), dtype=torch.int32))
+        lens += torch.tensor(ms, dtype=torch.int32, device="cuda") + (shared if ms[0] == 20 else 0)
+        step = paged.Step(cache, pages, rs, lens, R, nh, shared_pages=shared_pages, shared_len=shared)
+        kin, vin, q = rnd(R, nkv, hd), rnd(R, nkv, hd), rnd(R, nh, hd)
+        qr = step.append(kin, vin, q=q, rope_dims=hd)
+        out = step.attend(qr)
+        assert step.status() == 0
+        r = 0
+        for b, m in enumerate(ms):
+            pos = torch.arange(hist_k[b].shape[0], hist_k[b].shape[0] + m, device="cuda")
+            hist_k[b] = torch.cat([hist_k[b], rotated(kin[r:r + m], None, pos, hd, 1e4, 0)])
+            hist_v[b] = torch.cat([hist_v[b], vin[r:r + m].double()])
+            qw = rotated(q[r:r + m], None, pos, hd, 1e4, 0)
+            for j in range(m):
+                for h in range(nh):
+                    K, V = hist_k[b][:pos[j] + 1, h // 4].half().double(), hist_v[b][:pos[j] + 1, h // 4].half().double()
+                    w = torch.softmax(K @ qw[j, h] / math.sqrt(hd), 0)
+                    # keys that round to the other f16 neighbour: 2^-11 of a key here and there; scores move by 2^-11 |q| at most
+                    assert float((out[r + j, h].double() - w @ V).abs().max()) < 2.0 ** -11 * float(qw[j, h].norm()) * float(w @ V.abs().amax(-1)) + 1e-4
+            r += m
