@@ -8,10 +8,11 @@
 // top down to it) are gathered and ranked.  A bin with more members than the list holds (thousands of equal logits) is cut again by
 // (logit, id) as an integer until they fit.
 //
-// Sums are integers, weights times 2^45 (2^18 of them stay below 2^63): exact whatever the order of the atomics, so the token depends on
-// nothing but the inputs.  f32 would not do: between two of 150,000 candidates lie 10^-5 of the sum or less, and an error of 10^-8 at every
-// border moves a draw in a thousand.  A weight is e^(-b width), from a table, times e^d with d = x + b width exact in f32 and below the bin's
-// width in size: five terms of the exponential series in f64 leave 10^-15.
+// Sums are integers: exact whatever the order of the atomics, so the token depends on nothing but the inputs.  f32 would not do: between two of
+// 150,000 candidates lie 10^-5 of the sum or less, and an error of 10^-8 at every border moves a draw in a thousand.  A candidate in bin b weighs
+// e^(-b width) (1 + r), r = e^d - 1, d = x + b width: x and b width are f32 numbers close to each other, so d is exact; r is d itself
+// plus d^2 / 2 + .. <= 5 10^-5, which f32 holds to 10^-11.  A bin's sum of r in units of 2^-36 and its count then give its weight in f64, in units of
+// 2^-45 (2^18 candidates stay below 2^63); the listed candidates' weights are f64 exponentials.
 //
 // A row is a cluster of blocks, each with its part of the row in shared memory: logits are read from memory once.  What bounds it: with few rows
 // the chain of steps (load, maximum, sums, scan, gather, rank; a cluster barrier between), with many the sums' pass over all candidates.
@@ -21,8 +22,9 @@
 
 namespace {
 
-constexpr int SA_BINS = 1024, SA_LIST = 1024, SA_NTH = 512, SA_MAX_VOCAB = 1 << 18, SA_ID = 18;
-constexpr float SA_CUT = 18.0f, SA_W = SA_CUT / SA_BINS;       // (a bin's width, 9 / 512: exact, as are its multiples)
+constexpr int SA_BINS = 1024, SA_LIST = 1024, SA_NTH = 512, SA_MAX_VOCAB = 1 << 18, SA_ID = 18, SA_FEW = 512;
+constexpr float SA_CUT = 18.0f, SA_W = 37.0f / 2048;           // a bin's width: its multiples are exact, and SA_CUT is 997 of them
+constexpr double SA_ONE = 35184372088832.0;                    // 2^45: the weight 1
 static_assert(SA_BINS == 2 * SA_NTH, "a thread scans two bins");
 
 struct SaArgs {
@@ -36,32 +38,31 @@ struct SaArgs {
     float* prob;
 };
 
-enum { SA_DONE = 0, SA_GATHER = 1, SA_FINER = 2, SA_AGAIN = 3 };
-struct SaCtrl {                      // block 0 of the cluster tells the others what to do
-    int cmd, bin0, bin1;             // members of bins bin0 .. bin1
-    int shift;                       // .. whose (key, id) >> shift is `prefix` (shift 63: all)
+// What the blocks of a row do next; block 0 decides.
+enum { SA_DONE = 0, SA_GATHER = 1, SA_SUM = 2, SA_LARGEST = 3 };
+struct SaCtrl {
+    int cmd, bin0, bin1;             // SA_GATHER: the members of bins bin0 .. bin1 into the list.  SA_SUM: their bins' sums
+    int shift;                       // .. only those whose key >> shift is `prefix` (63: all)
+    int cut;                         // SA_SUM, >= 0: in bins by the ten bits of their keys from bit `cut` on
+    int count;                       // SA_SUM: and how many weigh min_p and more
     u64 prefix;
-    int n;                           // the list's length
-    // found by a search
-    int at;
-    u32 rank0;
-    u64 mass0;
 };
 struct SaSmem {
-    double table[SA_BINS];           // e^(-b width) 2^45
-    u64 mass[SA_BINS];
-    u64 gmass[SA_BINS + 1];          // block 0: weights before bin b, of the whole row
-    u64 list[SA_LIST];               // (key, id) of the gathered
-    u64 sorted[SA_LIST + 1];
+    union {
+        struct { u32 lo[SA_BINS], hi[SA_BINS]; } h;      // a bin's sums of this block (sa_add)
+        u64 sorted[SA_LIST];                              // block 0, later: the list in order
+    };
+    u64 list[SA_LIST];               // keys of the gathered
     u64 cum[SA_LIST + 1];            // weight of the sorted list before i
-    u32 cnt[SA_BINS];
+    u64 gmass[SA_BINS + 1];          // block 0: weights before bin b, of the whole row
     u32 gcnt[SA_BINS + 1];
-    float red[SA_NTH / 32];
+    float top[8 * SA_NTH / 32];      // the largest of every warp of every block
     u32 redi[SA_NTH / 32];
     u64 redm[SA_NTH / 32];
-    float top;                       // this block's largest
-    u32 top_id, above;               // .. its lowest id; members with a weight of min_p and more
+    u32 top_id, above;               // this block's lowest id of the largest; block 0: candidates with a weight of min_p and more
     SaCtrl c;
+    u32 n;                           // the list's length
+    int at;                          // found by a search
 };
 
 __device__ __forceinline__ u32 sa_at(const void* p, int rank) {
@@ -84,34 +85,27 @@ __device__ __forceinline__ float sa_value(u64 key) {
     const u32 up = ~(u32)(key >> SA_ID);
     return __uint_as_float(up & 0x80000000u ? up & 0x7fffffffu : ~up);
 }
-struct SaRow { float max, inv_t, cut; };
-__device__ __forceinline__ int sa_bin(float x, float& d) {           // d = x + bin * width, in (-width, 0] but for the last bin
-    x = fmaxf(x, -1.5f * SA_CUT);                                    // (a difference that overflowed)
-    int b = min((int)(-x * (SA_BINS / SA_CUT)), SA_BINS - 1);
-    d = fmaf((float)b, SA_W, x);
-    if (d > 0.f) { b--; d = fmaf((float)b, SA_W, x); }              // (the product above was rounded up)
-    return b;
+struct SaRow { float max, inv_t, cut, floor_x; };                    // floor_x: the least x whose weight is min_p and more
+__device__ __forceinline__ float sa_x(const SaRow& R, float v) { return (v - R.max) * R.inv_t; }
+// The bin nearest to x, and d = x + bin * width (exact), at most half a width in size (x from -18.25 on).
+__device__ __forceinline__ int sa_bin(float x, float& d) {
+    const float t = fmaf(x, -1.0f / SA_W, 12582912.0f);          // + 1.5 * 2^23: the integer nearest, in the low bits
+    d = fmaf(t - 12582912.0f, SA_W, x);
+    return (int)(__float_as_uint(t) & (SA_BINS - 1));
 }
-__device__ __forceinline__ u64 sa_weight(const double* table, int b, float d) {
-    const double y = (double)d;
-    const double e = fma(fma(fma(fma(fma(y, 1.0 / 120, 1.0 / 24), y, 1.0 / 6), y, 0.5), y, 1.0), y, 1.0);
-    return (u64)(__double_as_longlong(fma(table[b], e, 4503599627370496.0)) & 0xfffffffffffffll);      // + 2^52: the integer nearest, in the low bits
+// A bin's sums: members, and e^d - 1 of each in units of 2^-36, 2^30 added so that it is positive: below 2^31, and 2^46 for the 2^15 members a
+// block can have; count and the sum's upper half share a word.  (One 64-bit atomic in shared memory costs five times these two.)
+__device__ __forceinline__ void sa_add(SaSmem* S, int b, float d) {
+    const float q = d * d * fmaf(fmaf(fmaf(d, 1.0f / 120, 1.0f / 24), d, 1.0f / 6), d, 0.5f);
+    // (q below 2^22 units: the integer nearest is in the low bits of the sum with 1.5 * 2^23)
+    const u32 r = (u32)__float2int_rn(d * 68719476736.0f) + __float_as_uint(fmaf(q, 68719476736.0f, 12582912.0f)) + ((1u << 30) - 0x4b400000u);
+    const u32 old = atomicAdd(&S->h.lo[b], r);
+    atomicAdd(&S->h.hi[b], 65536u + (old + r < old));
 }
-__device__ __forceinline__ u64 sa_weight_of(const SaSmem* S, const SaRow& R, float v) {
-    float d;
-    const int b = sa_bin((v - R.max) * R.inv_t, d);
-    return sa_weight(S->table, b, d);
-}
+__device__ __forceinline__ u64 sa_weight(const SaRow& R, float v) { return (u64)__double2ull_rn(exp((double)sa_x(R, v)) * SA_ONE); }
 
-template <int TYPE>
-__device__ __forceinline__ float sa_one(const u8* p, long long i) {
-    float v;
-    if (TYPE == SZ_TYPE_F32) v = __ldg((const float*)p + i);
-    else if (TYPE == SZ_TYPE_F16) v = sz_f16_to_f32(__ldg((const u16*)p + i));
-    else v = sz_bf16_to_f32(__ldg((const u16*)p + i));
-    return v != v ? -INFINITY : v;
-}
-// 16 bytes as their 4 or 8 values
+// 16 bytes as their 4 or 8 values, NaN as -inf
+template <int TYPE> struct SaVec { static constexpr int E = TYPE == SZ_TYPE_F32 ? 4 : 8, ESZ = 16 / E; };
 template <int TYPE>
 __device__ __forceinline__ void sa_spread(uint4 w, float* v) {
     const u32 x[4] = {w.x, w.y, w.z, w.w};
@@ -122,62 +116,91 @@ __device__ __forceinline__ void sa_spread(uint4 w, float* v) {
         else { v[2 * i] = __uint_as_float(x[i] << 16); v[2 * i + 1] = __uint_as_float(x[i] & 0xffff0000u); }
     }
 #pragma unroll
-    for (int i = 0; i < (TYPE == SZ_TYPE_F32 ? 4 : 8); i++) v[i] = v[i] != v[i] ? -INFINITY : v[i];
+    for (int i = 0; i < SaVec<TYPE>::E; i++) v[i] = v[i] != v[i] ? -INFINITY : v[i];
 }
+template <int TYPE> __device__ __forceinline__ u32 sa_none() { return TYPE == SZ_TYPE_F32 ? 0xff800000u : TYPE == SZ_TYPE_F16 ? 0xfc00u : 0xff80u; }      // -inf
 
 __device__ __forceinline__ void sa_sync(int C) { if (C > 1) sz_cluster_sync(); else __syncthreads(); }
 
 template <int TYPE>
-__global__ void __launch_bounds__(SA_NTH) sz_sample_kernel(const __grid_constant__ SaArgs a) {
+__global__ void __launch_bounds__(SA_NTH, 2) sz_sample_kernel(const __grid_constant__ SaArgs a) {
+    constexpr int E = SaVec<TYPE>::E, ESZ = SaVec<TYPE>::ESZ;
     extern __shared__ __align__(16) u8 smem[];
     SaSmem* const S = (SaSmem*)smem;
-    float* const val = (float*)(smem + sizeof(SaSmem));
+    uint4* const val = (uint4*)(smem + ((sizeof(SaSmem) + 15) & ~(size_t)15));
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int row = blockIdx.x / a.C, rank = blockIdx.x % a.C;
-    const int i0 = rank * a.per, n = max(0, min(a.per, a.vocab - i0));
+    const int i0 = rank * a.per, n = max(0, min(a.per, a.vocab - i0)), units = (n + E - 1) / E;
+    if (a.C > 1) sz_cluster_arrive();
     sz_pdl_wait();
     sz_pdl_trigger();
-    // ---- the part of the row, its largest
+    // ---- the part of the row, its largest (thread t has units t, t + 512 .. throughout)
     float big = -INFINITY;
     {
-        const u8* p = a.logits + (long long)row * a.stride + (long long)i0 * (TYPE == SZ_TYPE_F32 ? 4 : 2);
-        constexpr int E = TYPE == SZ_TYPE_F32 ? 4 : 8;
+        const u8* p = a.logits + (long long)row * a.stride + (long long)i0 * ESZ;
         const int whole = ((u64)p & 15) == 0 ? n / E : 0;
-#pragma unroll 4
-        for (int i = tid; i < whole; i += SA_NTH) {
+#pragma unroll 5
+        for (int u = tid; u < whole; u += SA_NTH) {
+            const uint4 w = __ldg((const uint4*)p + u);
             float v[E];
-            sa_spread<TYPE>(__ldg((const uint4*)p + i), v);
-#pragma unroll
-            for (int k = 0; k < E; k += 4) *(float4*)(val + i * E + k) = make_float4(v[k], v[k + 1], v[k + 2], v[k + 3]);
+            val[u] = w;
+            sa_spread<TYPE>(w, v);
 #pragma unroll
             for (int k = 0; k < E; k++) big = fmaxf(big, v[k]);
         }
-#pragma unroll 4
-        for (int i = whole * E + tid; i < n; i += SA_NTH) { const float v = sa_one<TYPE>(p, i); val[i] = v; big = fmaxf(big, v); }
-    }
-    const float T = a.temperature ? __ldg(a.temperature + row) : 1.f, inv_t = 1.0f / T;
-    for (int b = tid; b < SA_BINS; b += SA_NTH) { S->table[b] = exp(-(double)SA_W * b) * 35184372088832.0; S->cnt[b] = 0; S->mass[b] = 0; }
+        for (int u = whole + tid - whole % SA_NTH; u < units; u += SA_NTH) {      // the last unit, or a row that does not begin on 16 bytes
+            if (u < whole) continue;
+            u32 w[4] = {};
 #pragma unroll
-    for (int s = 16; s > 0; s >>= 1) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, s));
-    if (lane == 0) S->red[warp] = big;
-    __syncthreads();
-    if (tid == 0) {
-        for (int w = 0; w < SA_NTH / 32; w++) big = fmaxf(big, S->red[w]);
-        S->top = big;
-        S->top_id = 0xffffffffu;
-        S->above = 0;
-        S->c.n = 0;
+            for (int k = 0; k < E; k++) {
+                const int i = u * E + k;
+                const u32 x = i >= n ? sa_none<TYPE>() : TYPE == SZ_TYPE_F32 ? __ldg((const u32*)p + i) : (u32)__ldg((const u16*)p + i);
+                w[k * ESZ / 4] |= TYPE == SZ_TYPE_F32 ? x : x << (16 * (k & 1));
+            }
+            const uint4 q = make_uint4(w[0], w[1], w[2], w[3]);
+            float v[E];
+            val[u] = q;
+            sa_spread<TYPE>(q, v);
+#pragma unroll
+            for (int k = 0; k < E; k++) big = fmaxf(big, v[k]);
+        }
     }
+    const float mine = big;
+    const float T = a.temperature ? __ldg(a.temperature + row) : 1.f, min_p = a.min_p ? __ldg(a.min_p + row) : 0.f, top_p = a.top_p ? __ldg(a.top_p + row) : 1.f;
+    const int top_k = a.top_k ? max(__ldg(a.top_k + row), 1) : 0x7fffffff;
+    const double u01 = __ldg(a.uniform + row);
+    // .. of the whole row: every warp writes its largest to every block
+    {
+        float m = mine;
+#pragma unroll
+        for (int s = 16; s > 0; s >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, s));
+        if (a.C > 1) sz_cluster_wait();                              // (the others have begun)
+        if (lane < a.C) sa_st32(&S->top[rank * (SA_NTH / 32) + warp], lane, __float_as_uint(m));
+    }
+    if (tid == 0) { S->top_id = 0xffffffffu; S->above = 0; }
     sa_sync(a.C);
     SaRow R;
-    R.max = -INFINITY;
-    for (int c = 0; c < a.C; c++) R.max = fmaxf(R.max, __uint_as_float(sa_ld32(&S->top, c)));
-    R.inv_t = inv_t;
+    {
+        float m = -INFINITY;
+        for (int i = lane; i < a.C * (SA_NTH / 32); i += 32) m = fmaxf(m, S->top[i]);
+#pragma unroll
+        for (int s = 16; s > 0; s >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, s));
+        R.max = m;
+    }
+    R.inv_t = 1.0f / T;
     R.cut = R.max - SA_CUT * T;
-    if (!(T > 0.f) || isinf(inv_t) || isinf(R.max)) {               // the best token (no finite largest: the lowest id that has it)
+    auto each = [&](auto f) {                                        // f(value, id) of the block's elements
+#pragma unroll 1
+        for (int u = tid; u < units; u += SA_NTH) {
+            float v[E];
+            sa_spread<TYPE>(val[u], v);
+#pragma unroll
+            for (int k = 0; k < E; k++) f(v[k], (u32)(i0 + u * E + k));
+        }
+    };
+    if (!(T > 0.f) || isinf(R.inv_t) || isinf(R.max)) {             // the best token (no finite largest: the lowest id that has it)
         u32 id = 0xffffffffu;
-        for (int i = tid; i < n; i += SA_NTH)
-            if (val[i] == R.max) { id = min(id, (u32)(i0 + i)); break; }
+        each([&](float v, u32 i) { if (v == R.max && i < (u32)a.vocab) id = min(id, i); });
         id = __reduce_min_sync(0xffffffffu, id);
         if (lane == 0) atomicMin(&S->top_id, id);
         sa_sync(a.C);
@@ -189,239 +212,249 @@ __global__ void __launch_bounds__(SA_NTH) sz_sample_kernel(const __grid_constant
         sa_sync(a.C);                                                // (the others' shared memory is read until here)
         return;
     }
-    const float min_p = a.min_p ? __ldg(a.min_p + row) : 0.f;
-    const double floor_m = (double)min_p * 35184372088832.0;
-    // ---- counts and weights of the bins; returns how many of this thread's weigh min_p and more
-    auto sum_bins = [&]() {
-        u32 above = 0;
-#pragma unroll 2
-        for (int i = tid; i < n; i += SA_NTH) {
-            const float v = val[i];
-            if (v >= R.cut && v > -INFINITY) {
-                float d;
-                const int b = sa_bin((v - R.max) * R.inv_t, d);
-                const u64 w = sa_weight(S->table, b, d);
-                atomicAdd(&S->cnt[b], 1u);
-                atomicAdd((unsigned long long*)&S->mass[b], (unsigned long long)w);
-                above += (double)w >= floor_m;
-            }
-        }
-        return above;
-    };
-    {
-        const u32 above = __reduce_add_sync(0xffffffffu, sum_bins());
-        if (lane == 0) atomicAdd(&S->above, above);
-    }
-    // every block adds up its share of the bins over the row's blocks, in block 0 (which scans them)
-    auto add_bins = [&]() {
-        sa_sync(a.C);
-        const int share = SA_BINS / a.C;
-        for (int b = rank * share + tid; b < (rank + 1) * share; b += SA_NTH) {
-            u32 c = 0;
-            u64 m = 0;
-            for (int k = 0; k < a.C; k++) { c += sa_ld32(&S->cnt[b], k); m += sa_ld64(&S->mass[b], k); }
-            sa_st32(&S->gcnt[b], 0, c);
-            sa_st64(&S->gmass[b], 0, m);
-        }
-        sa_sync(a.C);
-    };
-    add_bins();
+    // e^x >= min_p where x >= log min_p: the least float that is
+    R.floor_x = min_p > 0.f ? __double2float_ru(log((double)min_p)) : min_p <= 0.f ? -INFINITY : INFINITY;
+    // (x far below the cut: a difference that overflowed, weight 0)
+    auto there = [&](float v, float x) { return v >= R.cut && x >= -18.25f; };
 
-    // members of bins bin0 .. bin1 with (key >> shift) == prefix
-    auto member = [&](const SaCtrl& c, float v, int i, u64& key) {
-        if (!(v >= R.cut && v > -INFINITY)) return false;
-        float d;
-        const int b = sa_bin((v - R.max) * R.inv_t, d);
-        if (b < c.bin0 || b > c.bin1) return false;
-        key = sa_key(v, (u32)(i0 + i));
-        return c.shift >= 63 || (key >> c.shift) == c.prefix;
-    };
-    auto gather = [&](const SaCtrl& c) {
-        for (int i = tid; i < n; i += SA_NTH) {
-            u64 key;
-            if (member(c, val[i], i, key)) {
-                const u32 at = sa_add32(&S->c.n, 0, 1u);
-                if (at < (u32)SA_LIST) sa_st64(&S->list[at], 0, key);
-            }
-        }
-    };
-    // the same members into SA_BINS finer bins by the next ten bits of their keys
-    auto finer = [&](const SaCtrl& c) {
-        for (int b = tid; b < SA_BINS; b += SA_NTH) { S->cnt[b] = 0; S->mass[b] = 0; }
-        __syncthreads();
-        const int sh = (c.shift >= 63 ? SA_ID + 32 : c.shift) - 10;
-        for (int i = tid; i < n; i += SA_NTH) {
-            u64 key;
-            const float v = val[i];
-            if (member(c, v, i, key)) {
-                const int b = (int)(key >> sh) & (SA_BINS - 1);          // (ten bits of keys are left at least: fewer would fit the list)
-                atomicAdd(&S->cnt[b], 1u);
-                atomicAdd((unsigned long long*)&S->mass[b], (unsigned long long)sa_weight_of(S, R, v));
-            }
-        }
-        add_bins();
-    };
-    auto again = [&]() {
-        for (int b = tid; b < SA_BINS; b += SA_NTH) { S->cnt[b] = 0; S->mass[b] = 0; }
-        __syncthreads();
-        sum_bins();
-        add_bins();
-    };
-    if (rank != 0) {                                                 // ---- the other blocks do as they are told
-        for (;;) {
-            sz_cluster_sync();
-            SaCtrl c;
-            c.cmd = (int)sa_ld32(&S->c.cmd, 0);
-            c.bin0 = (int)sa_ld32(&S->c.bin0, 0);
-            c.bin1 = (int)sa_ld32(&S->c.bin1, 0);
-            c.shift = (int)sa_ld32(&S->c.shift, 0);
-            c.prefix = sa_ld64(&S->c.prefix, 0);
-            if (c.cmd == SA_GATHER) { gather(c); sz_cluster_sync(); }
-            else if (c.cmd == SA_FINER) finer(c);
-            else if (c.cmd == SA_AGAIN) again();
-            else break;
-        }
-        sz_cluster_sync();
-        return;
-    }
-    // ---- block 0: exclusive sums over the bins, in place
-    auto scan_bins = [&]() {
-        const u32 c0 = S->gcnt[2 * tid], c1 = S->gcnt[2 * tid + 1];
-        const u64 m0 = S->gmass[2 * tid], m1 = S->gmass[2 * tid + 1];
-        u32 c = c0 + c1;
-        u64 m = m0 + m1;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const u32 x = __shfl_up_sync(0xffffffffu, c, o);
-            const u64 y = __shfl_up_sync(0xffffffffu, m, o);
-            if (lane >= o) { c += x; m += y; }
-        }
-        if (lane == 31) { S->redi[warp] = c; S->redm[warp] = m; }
-        __syncthreads();
-        u32 cb = 0;
-        u64 mb = 0;
-        for (int w = 0; w < warp; w++) { cb += S->redi[w]; mb += S->redm[w]; }
-        S->gcnt[2 * tid] = cb + c - c0 - c1; S->gcnt[2 * tid + 1] = cb + c - c1;
-        S->gmass[2 * tid] = mb + m - m0 - m1; S->gmass[2 * tid + 1] = mb + m - m1;
-        if (tid == SA_NTH - 1) { S->gcnt[SA_BINS] = cb + c; S->gmass[SA_BINS] = mb + m; }
-        __syncthreads();
-    };
-    scan_bins();
-    const u32 N = S->gcnt[SA_BINS];
-    const u64 total = S->gmass[SA_BINS];
-    u32 n_above = 0;
-    for (int c = 0; c < a.C; c++) n_above += sa_ld32(&S->above, c);
-    // what the list holds: `len` elements from rank `rank0` on, their running sums from mass0 on
-    u32 len = 0, rank0 = 0;
-    u64 mass0 = 0;
-    bool bins_valid = true;
-    auto tell = [&](int cmd, int bin0, int bin1, int shift, u64 prefix) {
-        if (tid == 0) { S->c.cmd = cmd; S->c.bin0 = bin0; S->c.bin1 = bin1; S->c.shift = shift; S->c.prefix = prefix; S->c.n = 0; }
-        sa_sync(a.C);
-        const SaCtrl c = S->c;
-        if (cmd == SA_GATHER) { gather(c); sa_sync(a.C); }
-        else { if (cmd == SA_FINER) finer(c); else again(); scan_bins(); }
-    };
-    auto rank_list = [&](u32 count) {                                // the gathered keys in order, their running sums
-        u64 key[SA_LIST / SA_NTH];
-        int at[SA_LIST / SA_NTH];
-#pragma unroll
-        for (int k = 0; k < SA_LIST / SA_NTH; k++) { key[k] = (u32)(tid + k * SA_NTH) < count ? S->list[tid + k * SA_NTH] : ~0ull; at[k] = 0; }
-        for (u32 j = 0; j < count; j++) {
-            const u64 x = S->list[j];
-#pragma unroll
-            for (int k = 0; k < SA_LIST / SA_NTH; k++) at[k] += x < key[k];
-        }
-#pragma unroll
-        for (int k = 0; k < SA_LIST / SA_NTH; k++) if ((u32)(tid + k * SA_NTH) < count) S->sorted[at[k]] = key[k];
-        __syncthreads();
-        const u64 w0 = (u32)(2 * tid) < count ? sa_weight_of(S, R, sa_value(S->sorted[2 * tid])) : 0, w1 = (u32)(2 * tid + 1) < count ? sa_weight_of(S, R, sa_value(S->sorted[2 * tid + 1])) : 0;
-        u64 m = w0 + w1;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) { const u64 y = __shfl_up_sync(0xffffffffu, m, o); if (lane >= o) m += y; }
-        if (lane == 31) S->redm[warp] = m;
-        __syncthreads();
-        u64 mb = 0;
-        for (int w = 0; w < warp; w++) mb += S->redm[w];
-        S->cum[2 * tid] = mb + m - w0 - w1; S->cum[2 * tid + 1] = mb + m - w1;
-        if (tid == SA_NTH - 1) S->cum[SA_LIST] = mb + m;
-        __syncthreads();
-    };
-    // The element of rank k (by_rank), or the first whose running sum exceeds t: its place in the list, which is made to hold it.
-    auto find = [&](bool by_rank, u32 k, u64 t) -> u32 {
-        for (;;) {
-            const bool here = len && (by_rank ? k >= rank0 && k < rank0 + len : t >= mass0 && t < mass0 + S->cum[len]);
-            if (here) {
-                __syncthreads();
-                if (by_rank) return k - rank0;
-                for (u32 i = tid; i < len; i += SA_NTH)
-                    if (mass0 + S->cum[i] <= t && t < mass0 + S->cum[i + 1]) S->c.at = (int)i;
-                __syncthreads();
-                return (u32)S->c.at;
-            }
-            if (!bins_valid) {                                       // (an overfull bin was cut finer: the row's bins again)
-                tell(SA_AGAIN, 0, 0, 0, 0);
-                bins_valid = true;
-            }
-            __syncthreads();
-            for (int b = tid; b < SA_BINS; b += SA_NTH)
-                if (by_rank ? S->gcnt[b] <= k && k < S->gcnt[b + 1] : S->gmass[b] <= t && t < S->gmass[b + 1]) { S->c.at = b; S->c.rank0 = S->gcnt[b]; S->c.mass0 = S->gmass[b]; }
-            __syncthreads();
-            int b = S->c.at, shift = 63;
-            u64 prefix = 0;
-            rank0 = S->c.rank0; mass0 = S->c.mass0;
-            u32 count = S->gcnt[b + 1] - rank0;
-            const int bin = b;
-            int first = bin;
-            if (S->gcnt[b + 1] <= (u32)SA_LIST) { first = 0; rank0 = 0; mass0 = 0; count = S->gcnt[b + 1]; }      // all from the top on
-            while (count > (u32)SA_LIST) {
-                bins_valid = false;
-                tell(SA_FINER, bin, bin, shift, prefix);
-                for (int x = tid; x < SA_BINS; x += SA_NTH)
-                    if (by_rank ? rank0 + S->gcnt[x] <= k && k < rank0 + S->gcnt[x + 1] : mass0 + S->gmass[x] <= t && t < mass0 + S->gmass[x + 1]) {
-                        S->c.at = x; S->c.rank0 = rank0 + S->gcnt[x]; S->c.mass0 = mass0 + S->gmass[x];
+    // With a small top_k the bins of the threads' largest elements say as much as all elements': k of them above a line are k elements above it.
+    bool few = top_k <= SA_FEW;
+    SaCtrl c;
+    c.cmd = few ? SA_LARGEST : SA_SUM; c.bin0 = 0; c.bin1 = SA_BINS - 1; c.shift = 63; c.cut = -1; c.count = 1; c.prefix = 0;
+    // block 0: what the list holds - `len` elements in order from rank rank0 on, running sums from mass0 on, up to the weights of mass1 -, the search under way
+    u32 len = 0, rank0 = 0, N = 0, n_above = 0, K = 0, kept = 0;
+    u64 mass0 = 0, mass1 = 0, Z = 0, M = 0;
+    bool bins_valid = true, descending = false, whole = false, known = false;
+    u32 s_from = 0, s_count = 0;
+    u64 s_m0 = 0, s_m1 = 0;
+    int stage = 0;
+#pragma unroll 1
+    for (;;) {
+        // ---- all blocks
+        if (c.cmd == SA_GATHER) {
+            const float lo = -((float)c.bin1 + 0.75f) * SA_W, hi = -((float)c.bin0 - 0.75f) * SA_W;
+            each([&](float v, u32 i) {
+                const float x = sa_x(R, v);
+                if (x >= lo && x <= hi && there(v, x)) {
+                    float d;
+                    const int b = sa_bin(x, d);
+                    const u64 key = sa_key(v, i);
+                    if (b >= c.bin0 && b <= c.bin1 && (c.shift >= 63 || (key >> c.shift) == c.prefix)) {
+                        const u32 at = sa_add32(&S->n, 0, 1u);
+                        if (at < (u32)SA_LIST) sa_st64(&S->list[at], 0, key);
                     }
-                __syncthreads();
-                b = S->c.at;
-                count = S->gcnt[b + 1] - S->gcnt[b];
-                rank0 = S->c.rank0; mass0 = S->c.mass0;
-                prefix = (shift >= 63 ? 0 : prefix << 10) | (u64)b;
-                shift = (shift >= 63 ? SA_ID + 32 : shift) - 10;
+                }
+            });
+        } else {
+            for (int b = tid; b < SA_BINS; b += SA_NTH) { S->h.lo[b] = 0; S->h.hi[b] = 0; }
+            __syncthreads();
+            if (c.cmd == SA_LARGEST) {
+                const float x = sa_x(R, mine);
+                float d;
+                if (there(mine, x)) atomicAdd(&S->h.hi[sa_bin(x, d)], 65536u);
+            } else {
+                u32 above = 0;
+                each([&](float v, u32 i) {
+                    const float x = sa_x(R, v);
+                    if (there(v, x)) {
+                        float d;
+                        int b = sa_bin(x, d);
+                        above += x >= R.floor_x;
+                        if (c.cut >= 0) {
+                            const u64 key = sa_key(v, i);
+                            if (b != c.bin0 || (c.shift < 63 && (key >> c.shift) != c.prefix)) return;
+                            b = (int)(key >> c.cut) & (SA_BINS - 1);
+                        }
+                        sa_add(S, b, d);
+                    }
+                });
+                if (c.count) {
+                    above = __reduce_add_sync(0xffffffffu, above);
+                    if (lane == 0 && above) sa_add32(&S->above, 0, above);
+                }
+            }
+            // every block adds up its share of the bins over the row's blocks, for block 0
+            sa_sync(a.C);
+            const int share = SA_BINS / a.C;
+            for (int b = rank * share + tid; b < (rank + 1) * share; b += SA_NTH) {
+                u64 sum = 0;
+                u32 n_b = 0, h[8], l[8];
+#pragma unroll
+                for (int k = 0; k < 8; k++) { h[k] = k < a.C ? sa_ld32(&S->h.hi[b], k) : 0; l[k] = k < a.C ? sa_ld32(&S->h.lo[b], k) : 0; }
+#pragma unroll
+                for (int k = 0; k < 8; k++) { n_b += h[k] >> 16; sum += ((u64)(h[k] & 65535u) << 32) + l[k]; }
+                const double more = (double)((long long)sum - ((long long)n_b << 30)) * (1.0 / 68719476736.0);
+                sa_st32(&S->gcnt[b], 0, n_b);
+                sa_st64(&S->gmass[b], 0, n_b ? __double2ull_rn(exp(-(double)SA_W * (c.cut >= 0 ? c.bin0 : b)) * SA_ONE * ((double)n_b + more)) : 0ull);
+            }
+        }
+        sa_sync(a.C);
+        // ---- block 0: sums before the bins, or the list in order; then on with the row until something is missing
+        if (rank == 0) {
+            u32 count;
+            if (c.cmd != SA_GATHER) count = SA_BINS;
+            else {
+                count = S->n;
+                if (few && !whole) {
+                    whole = count <= (u32)SA_LIST;
+                    s_count = count; s_from = 0; s_m0 = 0;
+                    few = whole;
+                }
+                if (whole || !few) count = min(count, (u32)SA_LIST);
+                for (u32 k = tid; k < count; k += SA_NTH) {
+                    const u64 key = S->list[k];
+                    int at = 0;
+#pragma unroll 8
+                    for (u32 j = 0; j < count; j++) at += S->list[j] < key;
+                    S->sorted[at] = key;
+                }
                 __syncthreads();
             }
-            tell(SA_GATHER, first, bin, shift, prefix);
-            len = count;
-            rank_list(count);
+            // two elements a thread: sums before them
+            u32 n0 = 0, n1 = 0;
+            u64 w0 = 0, w1 = 0;
+            if (c.cmd != SA_GATHER) { n0 = S->gcnt[2 * tid]; n1 = S->gcnt[2 * tid + 1]; w0 = S->gmass[2 * tid]; w1 = S->gmass[2 * tid + 1]; }
+            else {
+                n0 = (u32)(2 * tid) < count; n1 = (u32)(2 * tid + 1) < count;
+                if (n0) w0 = sa_weight(R, sa_value(S->sorted[2 * tid]));
+                if (n1) w1 = sa_weight(R, sa_value(S->sorted[2 * tid + 1]));
+                if (whole && c.cmd == SA_GATHER) {
+                    u32 above = (n0 && sa_x(R, sa_value(S->sorted[2 * tid])) >= R.floor_x) + (n1 && sa_x(R, sa_value(S->sorted[2 * tid + 1])) >= R.floor_x);
+                    above = __reduce_add_sync(0xffffffffu, above);
+                    if (lane == 0 && above) atomicAdd(&S->above, above);
+                }
+            }
+            u32 n_s = n0 + n1;
+            u64 m = w0 + w1;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const u32 x = __shfl_up_sync(0xffffffffu, n_s, o);
+                const u64 y = __shfl_up_sync(0xffffffffu, m, o);
+                if (lane >= o) { n_s += x; m += y; }
+            }
+            if (lane == 31) { S->redi[warp] = n_s; S->redm[warp] = m; }
+            __syncthreads();
+            u32 nb = lane < warp ? S->redi[lane] : 0;
+            u64 mb = lane < warp ? S->redm[lane] : 0;
+#pragma unroll
+            for (int o = SA_NTH / 64; o > 0; o >>= 1) { nb += __shfl_xor_sync(0xffffffffu, nb, o); mb += __shfl_xor_sync(0xffffffffu, mb, o); }
+            nb = __shfl_sync(0xffffffffu, nb, 0); mb = __shfl_sync(0xffffffffu, mb, 0);
+            u64* const mass = c.cmd != SA_GATHER ? S->gmass : S->cum;
+            mass[2 * tid] = mb + m - w0 - w1; mass[2 * tid + 1] = mb + m - w1;
+            if (tid == SA_NTH - 1) mass[SA_BINS] = mb + m;
+            if (c.cmd != SA_GATHER) {
+                S->gcnt[2 * tid] = nb + n_s - n0 - n1; S->gcnt[2 * tid + 1] = nb + n_s - n1;
+                if (tid == SA_NTH - 1) S->gcnt[SA_BINS] = nb + n_s;
+                len = 0;                                             // (the sorted list lies where the bins are summed)
+            }
+            __syncthreads();
+            if (c.cmd == SA_GATHER) { len = count; rank0 = s_from; mass0 = s_m0; mass1 = whole ? S->cum[len] : s_m1; }
+            auto search = [&](auto at, int n_at) {                   // the one place of n_at for which at() is true
+                for (int i = tid; i < n_at; i += SA_NTH) if (at(i)) S->at = i;
+                __syncthreads();
+                const int i = S->at;
+                __syncthreads();
+                return i;
+            };
+            SaCtrl t = {};
+            t.shift = 63; t.cut = -1;
+#pragma unroll 1
+            for (;;) {
+                bool by_rank = false;
+                u32 k = 0;
+                u64 goal = 0;
+                if (stage == 0) {                                    // the candidates, or as many of them as may be kept
+                    if (c.cmd == SA_LARGEST) {
+                        int line = SA_BINS - 1;
+                        if (S->gcnt[SA_BINS] >= (u32)top_k) line = search([&](int b) { return S->gcnt[b] < (u32)top_k && (u32)top_k <= S->gcnt[b + 1]; }, SA_BINS);
+                        t.cmd = SA_GATHER; t.bin1 = line;
+                        break;
+                    }
+                    if (c.cmd == SA_GATHER && !whole) { t.cmd = SA_SUM; t.bin1 = SA_BINS - 1; t.count = 1; break; }      // more equal ones than the list holds
+                    N = whole ? len : S->gcnt[SA_BINS];
+                    n_above = S->above;
+                    K = min((u32)top_k, N);
+                    Z = whole ? S->cum[K] : S->gmass[SA_BINS];
+                    kept = min(K, max(n_above, 1u));
+                    known = kept == K;
+                    stage = !whole && K < N ? 1 : 2;
+                    M = Z;
+                }
+                if (stage == 1) { by_rank = true; k = K - 1; }       // Z: the sum up to the last of top_k
+                if (stage == 2) {                                    // the first whose running sum is top_p Z and more
+                    if (!(top_p < 1.f)) stage = 3;
+                    else {
+                        const double need = ceil((double)top_p * (double)Z);
+                        goal = need >= 1.0 ? (need > (double)(Z - 1) ? Z - 1 : (u64)need - 1) : 0;
+                    }
+                }
+                if (stage == 3) { if (known) stage = 4; else { by_rank = true; k = kept - 1; } }      // M: the sum of what is kept
+                if (stage == 4) {                                    // the draw
+                    const double g = floor(u01 * (double)M);
+                    goal = g > 0.0 ? (g >= (double)(M - 1) ? M - 1 : (u64)g) : 0;
+                }
+                if (stage == 5) { by_rank = true; k = kept - 1; }    // .. which a rounding of the bins' sums put behind the last kept
+                if (len && (by_rank ? k >= rank0 && k < rank0 + len : goal >= mass0 && goal < mass1)) {
+                    // (the last of the list, where a rounding of the bins' sums leaves none)
+                    const u32 i = by_rank ? k - rank0 : (u32)search([&](int j) { return (j == 0 || mass0 + S->cum[j] <= goal) && (j == (int)len - 1 || goal < mass0 + S->cum[j + 1]); }, (int)len);
+                    const u64 upto = mass0 + S->cum[i + 1];
+                    if (stage == 1) { Z = upto; if (known) M = Z; stage = 2; }
+                    else if (stage == 2) { if (rank0 + i + 1 <= kept) { kept = rank0 + i + 1; M = upto; known = true; } stage = 3; }
+                    else if (stage == 3) { M = upto; stage = 4; }
+                    else if (stage == 4 && rank0 + i >= kept) stage = 5;
+                    else {
+                        if (tid == 0) {
+                            a.token[row] = (int32_t)(S->sorted[i] & ((1u << SA_ID) - 1));
+                            if (a.prob) a.prob[row] = (float)((double)(S->cum[i + 1] - S->cum[i]) / (double)M);
+                        }
+                        t.cmd = SA_DONE;
+                        break;
+                    }
+                    continue;
+                }
+                if (!bins_valid && !descending) {                    // (a full bin was cut finer where they lay)
+                    bins_valid = true;
+                    t.cmd = SA_SUM; t.bin1 = SA_BINS - 1;
+                    break;
+                }
+                const u32 r_at = descending ? s_from : 0;
+                const u64 m_at = descending ? s_m0 : 0;
+                const int b = search([&](int j) {
+                    if (S->gcnt[j] == S->gcnt[j + 1]) return false;
+                    if (by_rank) return r_at + S->gcnt[j] <= k && k < r_at + S->gcnt[j + 1];
+                    return (S->gcnt[j] == 0 || m_at + S->gmass[j] <= goal) && (S->gcnt[j + 1] == S->gcnt[SA_BINS] || goal < m_at + S->gmass[j + 1]);
+                }, SA_BINS);
+                s_count = S->gcnt[b + 1] - S->gcnt[b];
+                s_from = r_at + S->gcnt[b];
+                s_m0 = m_at + S->gmass[b];
+                s_m1 = m_at + S->gmass[b + 1];
+                if (descending) { t.bin0 = t.bin1 = c.bin0; t.prefix = (c.shift >= 63 ? 0 : c.prefix << 10) | (u64)b; t.shift = c.cut; }
+                else {
+                    t.bin0 = t.bin1 = b;
+                    if (S->gcnt[b + 1] <= (u32)SA_LIST / 4) { t.bin0 = 0; s_from = 0; s_m0 = 0; s_count = S->gcnt[b + 1]; }      // all from the top on
+                }
+                descending = s_count > (u32)SA_LIST;
+                t.cmd = descending ? SA_SUM : SA_GATHER;
+                if (descending) { bins_valid = false; t.cut = (t.shift >= 63 ? SA_ID + 32 : t.shift) - 10; }      // (ten bits are left at least: fewer would fit the list)
+                break;
+            }
+            if (tid == 0) { S->c = t; S->n = 0; }
+            c = t;
         }
-    };
-    const u32 K = min((u32)max(a.top_k ? __ldg(a.top_k + row) : 0x7fffffff, 1), N);
-    const double top_p = a.top_p ? (double)__ldg(a.top_p + row) : 1.0, u01 = __ldg(a.uniform + row);
-    u64 Z = total;
-    if (K < N) { const u32 i = find(true, K - 1, 0); Z = mass0 + S->cum[i + 1]; }
-    u32 kept = min(K, max(n_above, 1u));
-    u64 M = Z;
-    bool known = kept == K;
-    if (top_p < 1.0) {
-        const double need = ceil(top_p * (double)Z);                 // the first whose running sum is `need` and more (at least the first of all)
-        const u64 t = need >= 1.0 ? (need > (double)(Z - 1) ? Z - 1 : (u64)need - 1) : 0;
-        const u32 i = find(false, 0, t);
-        if (rank0 + i + 1 <= kept) { kept = rank0 + i + 1; M = mass0 + S->cum[i + 1]; known = true; }
+        sa_sync(a.C);
+        if (rank != 0) {
+            c.cmd = (int)sa_ld32(&S->c.cmd, 0); c.bin0 = (int)sa_ld32(&S->c.bin0, 0); c.bin1 = (int)sa_ld32(&S->c.bin1, 0);
+            c.shift = (int)sa_ld32(&S->c.shift, 0); c.cut = (int)sa_ld32(&S->c.cut, 0); c.count = (int)sa_ld32(&S->c.count, 0);
+            c.prefix = sa_ld64(&S->c.prefix, 0);
+        }
+        if (c.cmd == SA_DONE) break;
     }
-    if (!known) { const u32 i = find(true, kept - 1, 0); M = mass0 + S->cum[i + 1]; }
-    const double goal = floor(u01 * (double)M);
-    const u64 t = goal > 0.0 ? (goal >= (double)(M - 1) ? M - 1 : (u64)goal) : 0;
-    const u32 i = find(false, 0, t);
-    if (tid == 0) {
-        a.token[row] = (int32_t)(S->sorted[i] & ((1u << SA_ID) - 1));
-        if (a.prob) a.prob[row] = (float)((double)(S->cum[i + 1] - S->cum[i]) / (double)M);
-        S->c.cmd = SA_DONE;
-    }
-    if (a.C > 1) { sz_cluster_sync(); sz_cluster_sync(); }
+    sa_sync(a.C);                                                    // (block 0's shared memory is read until here)
 }
 
 template <int TYPE>
 int sa_launch(const SaArgs& a, cudaStream_t st) {
-    const size_t smem = sizeof(SaSmem) + (size_t)a.per * 4;
+    const size_t smem = ((sizeof(SaSmem) + 15) & ~(size_t)15) + (size_t)a.per * SaVec<TYPE>::ESZ;
     const int rc = sz_allow_smem((const void*)sz_sample_kernel<TYPE>, 227 * 1024);
     if (rc) return rc;
     cudaLaunchConfig_t cfg = {};
