@@ -136,23 +136,27 @@ __global__ void __launch_bounds__(256) sz_pg_append_kernel(const __grid_constant
 }
 
 // ---- the plan of a call with more sequences or tiles than a block plans for itself ---------------------------------------------------------
-__global__ void __launch_bounds__(1024) sz_pg_plan_kernel(const __grid_constant__ PgBatch d, const __grid_constant__ PgPart a, const __grid_constant__ PgPart s) {
+struct PgParts { PgPart p[4]; };      // in the order of the positions: shared ones by the tcgen05 kernel, the rest of them, own ones likewise
+enum { PG_SHARED_TC = 0, PG_SHARED = 1, PG_OWN_TC = 2, PG_OWN = 3 };
+__global__ void __launch_bounds__(1024) sz_pg_plan_kernel(const __grid_constant__ PgBatch d, const __grid_constant__ PgParts a) {
     __shared__ u32 scan[32];
+    const PgPart& p = a.p[blockIdx.x];
     sz_pdl_wait();
     sz_pdl_trigger();
-    if (a.planned) pg_plan<1024>(d, 0, a.tq, a.tiles, a.units, scan);
-    __syncthreads();
-    if (s.planned) pg_plan<1024>(d, 1, s.tq, s.tiles, s.units, scan);
+    if (p.on && p.planned) pg_plan<1024>(d, p.shared, p.tc, p.tq, p.tiles, p.units, scan);
 }
 
 // ---- joining the parts -----------------------------------------------------------------------------------------------------------------------------
-// A block has one row and head: the parts of its item over the shared positions, then those over its own, in the order of the positions.
-// Threads in groups of hd / 4 take the parts in turn (four columns each); the groups' sums are added in order.
-constexpr int PG_MERGE = 128, PG_PARTS = 2 * 4 * PG_BLOCKS;
+// A block has one row and head: the parts of its items, in the order of the positions.  Threads in groups of hd / 4 take the parts in turn (four
+// columns each); the groups' sums are added in order.
+constexpr int PG_MERGE = 128, PG_PARTS = 2 * 5 * PG_BLOCKS;
 struct PgList { int n, first, alone, lane; };     // parts of an item: their number, the block of the first; by row and head; the vector's place in its tile
-__device__ PgList pg_list(const PgBatch& d, const PgPart& p, int r0, int first_row, int b, int h, int r, int E) {
+__device__ PgList pg_list(const PgBatch& d, const PgPart& p, int r, int r0, int b, int h) {
     PgList l = {};
-    const int vec = (r - r0) * d.G + h % d.G, t = vec / p.tq, e = p.shared ? t : (int)p.tiles[b] + t;
+    if (!p.on) return l;
+    const int start = p.shared ? pg_row(d, 0) : r0;
+    const int vec = (r - start) * d.G + h % d.G, t = vec / p.tq, e = p.shared ? t : (int)p.tiles[b] + t;
+    const int E = p.shared ? ((pg_row(d, d.n_seq) - start) * d.G + p.tq - 1) / p.tq : (int)p.tiles[d.n_seq];
     const u32 us = p.units[e], n = p.units[e + 1] - us;
     if (!n) return l;
     const long long U = (long long)p.units[E] * d.nkv, at = (long long)us * d.nkv + (long long)(h / d.G) * n;
@@ -164,9 +168,10 @@ __device__ PgList pg_list(const PgBatch& d, const PgPart& p, int r0, int first_r
     return l;
 }
 template <int HD>
-__global__ void __launch_bounds__(PG_MERGE) sz_pg_merge_kernel(const __grid_constant__ PgBatch d, const __grid_constant__ PgIo io, const __grid_constant__ PgPart own,
-                                                               const __grid_constant__ PgPart shr) {
+__global__ void __launch_bounds__(PG_MERGE) sz_pg_merge_kernel(const __grid_constant__ PgBatch d, const __grid_constant__ PgIo io, const __grid_constant__ PgParts a) {
     __shared__ float wgt[PG_PARTS];
+    __shared__ float sum_of[PG_PARTS];
+    __shared__ const float* from[PG_PARTS];
     __shared__ float red[PG_MERGE / 32], redl[PG_MERGE / 32];
     __shared__ float4 sums[PG_MERGE];
     const int r = blockIdx.x, h = blockIdx.y, nh = d.nkv * d.G, tid = threadIdx.x;
@@ -174,37 +179,39 @@ __global__ void __launch_bounds__(PG_MERGE) sz_pg_merge_kernel(const __grid_cons
     sz_pdl_trigger();
     const int b = pg_seq_of<PG_MERGE>(d, r);
     if (b < 0) return;
-    const int r0 = pg_row(d, b), m = pg_row(d, b + 1) - r0, start = pg_row(d, 0);
-    const long long seen = (long long)__ldg(d.lens + b) - d.shared_len - (m - 1 - (r - r0));     // own positions the row sees
+    const int r0 = pg_row(d, b), m = pg_row(d, b + 1) - r0;
+    const bool sees = (long long)__ldg(d.lens + b) - d.shared_len - (m - 1 - (r - r0)) > 0;     // a position of its own
     u8* op = io.out + (long long)r * io.out_stride + (long long)h * HD * io.esz;
-    PgList lo = pg_list(d, own, r0, 0, b, h, r, (int)own.tiles[d.n_seq]), ls = {};
-    if (seen > 0 && own.direct && lo.alone) return;                // (written by the block that did it)
-    if (shr.on && seen > 0) ls = pg_list(d, shr, start, 0, 0, h, r, ((pg_row(d, d.n_seq) - start) * d.G + shr.tq - 1) / shr.tq);
-    if (seen <= 0) lo.n = 0;
-    const int n = ls.n + lo.n;
-    auto where = [&](int i, const float2*& ml) -> const float* {
-        const PgPart& p = i < ls.n ? shr : own;
-        const PgList& l = i < ls.n ? ls : lo;
-        const int k = i < ls.n ? i : i - ls.n;
-        const size_t at = l.alone ? (size_t)r * nh + h : (size_t)(k == 0 ? 2 * l.first + 1 : 2 * (l.first + k)) * p.tq + l.lane;
-        ml = (l.alone ? p.row_ml : p.ml) + at;
-        return (l.alone ? p.row_o : p.o) + at * HD;
-    };
+    int n = 0;
     float M = -INFINITY;
-    for (int i = tid; i < n; i += PG_MERGE) { const float2* ml; where(i, ml); const float x = ml->x; wgt[i] = x; M = fmaxf(M, x); }
+    if (sees) {
+#pragma unroll 1
+        for (int s = 0; s < 4; s++) {
+            const PgPart& p = a.p[s];
+            const PgList l = pg_list(d, p, r, r0, b, h);
+            if (s == PG_OWN && p.direct && l.alone) return;          // (written by the block that did it)
+            for (int i = tid; i < l.n; i += PG_MERGE) {
+                const size_t at = l.alone ? (size_t)r * nh + h : (size_t)(i == 0 ? 2 * l.first + 1 : 2 * (l.first + i)) * p.tq + l.lane;
+                const float2 ml = (l.alone ? p.row_ml : p.ml)[at];
+                wgt[n + i] = ml.x;
+                sum_of[n + i] = ml.y;
+                from[n + i] = (l.alone ? p.row_o : p.o) + at * HD;
+                M = fmaxf(M, ml.x);
+            }
+            n += l.n;
+        }
+    }
 #pragma unroll
     for (int s = 16; s > 0; s >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, s));
     if ((tid & 31) == 0) red[tid >> 5] = M;
-    __syncthreads();
+    __syncthreads();                                                 // (and the lists are there)
 #pragma unroll
     for (int w = 0; w < PG_MERGE / 32; w++) M = fmaxf(M, red[w]);
     float L = 0.f;
     for (int i = tid; i < n; i += PG_MERGE) {
-        const float2* ml;
-        where(i, ml);
         const float c = wgt[i] == -INFINITY ? 0.f : pg_ex2(wgt[i] - M);
         wgt[i] = c;
-        L += c * ml->y;
+        L += c * sum_of[i];
     }
     L = sz_warp_sum(L);
     if ((tid & 31) == 0) redl[tid >> 5] = L;
@@ -217,8 +224,7 @@ __global__ void __launch_bounds__(PG_MERGE) sz_pg_merge_kernel(const __grid_cons
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 4
     for (int i = grp; i < n; i += GN) {
-        const float2* ml;
-        const float4 x = *(const float4*)(where(i, ml) + 4 * col);
+        const float4 x = *(const float4*)(from[i] + 4 * col);
         const float c = wgt[i];
         acc.x = fmaf(c, x.x, acc.x); acc.y = fmaf(c, x.y, acc.y); acc.z = fmaf(c, x.z, acc.z); acc.w = fmaf(c, x.w, acc.w);
     }
@@ -287,20 +293,28 @@ PgBatch pg_batch(const sz_paged_cache* c, const sz_paged_batch* b, int n_head, u
 // sequence with more makes more items).
 int pg_tiles_of(long long vectors) { return vectors <= 16 ? 1 : vectors <= 32 ? 2 : 4; }
 
-// The scratch: the status word, then for own and shared positions the plan's tables, the blocks' parts, the whole items by row.
-struct PgScratch { PgPart own, shr; int64_t bytes; };
-PgScratch pg_scratch(int n_seq, int rows, int nh, int hd, uint64_t base) {
+// Vectors from which the tcgen05 kernel takes whole units: of a sequence on average (own positions), of the batch (shared ones).
+constexpr int PG_TC_MIN = 96;
+bool pg_tc_type(int cache_type) { return cache_type == SZ_TYPE_F16 || cache_type == SZ_TYPE_BF16; }
+
+// The scratch: the status word, then for every kind of part the plan's tables, the blocks' parts, the whole items by row.
+struct PgScratch { PgParts a; int64_t bytes; };
+PgScratch pg_scratch(const sz_paged_cache* c, const sz_paged_batch* b, int nh, uint64_t base) {
     PgScratch s = {};
     int64_t off = 256;
+    const int hd = c->head_dim, G = nh / c->n_kv_head;
     auto take = [&](int64_t n) { const int64_t at = off; off += (n + 255) & ~(int64_t)255; return base + at; };
-    for (PgPart* p : {&s.own, &s.shr}) {
-        const int64_t slots = 2ll * PG_BLOCKS * 64;      // vectors of the blocks' parts: blocks a multiprocessor x vectors a tile is 64 at most
-        p->tiles = (u32*)take(4ll * (n_seq + 1));
-        p->units = (u32*)take(4ll * ((int64_t)rows * nh / 16 + n_seq + 2));
+    for (int i = 0; i < 4; i++) {
+        PgPart* p = &s.a.p[i];
+        const bool tc = i == PG_SHARED_TC || i == PG_OWN_TC;
+        if (tc && (!pg_tc_type(c->type) || (int64_t)G * b->rows < PG_TC_MIN)) continue;      // (fewer rows never need more)
+        const int64_t slots = 2ll * PG_BLOCKS * (tc ? pg_tc_tile(hd) : 64);      // vectors of the blocks' parts (blocks a multiprocessor x vectors a tile is 64 at most)
+        p->tiles = (u32*)take(4ll * (b->n_seq + 1));
+        p->units = (u32*)take(4ll * ((int64_t)b->rows * G / 16 + b->n_seq + 2));
         p->o = (float*)take(slots * hd * 4);
         p->ml = (float2*)take(slots * 8);
-        p->row_o = (float*)take((int64_t)rows * nh * hd * 4);
-        p->row_ml = (float2*)take((int64_t)rows * nh * 8);
+        p->row_o = (float*)take((int64_t)b->rows * nh * hd * 4);
+        p->row_ml = (float2*)take((int64_t)b->rows * nh * 8);
     }
     s.bytes = off;
     return s;
@@ -319,7 +333,7 @@ extern "C" int sz_paged_scratch_bytes(const sz_paged_cache* cache, const sz_page
     int rc = pg_check(cache, batch, n_head, "sz_paged_scratch_bytes");
     if (rc) return rc;
     if (!bytes) return sz_fail(SZ_E_ARG, "sz_paged_scratch_bytes: null result");
-    *bytes = pg_scratch(batch->n_seq, batch->rows, n_head, cache->head_dim, 0).bytes;
+    *bytes = pg_scratch(cache, batch, n_head, 0).bytes;
     return SZ_OK;
 }
 
@@ -378,10 +392,10 @@ extern "C" int sz_paged_attend(const sz_paged_cache* cache, const sz_paged_batch
     if ((rc = pg_check_rows(q, q_stride, hd, n_head, hd, batch->rows, esz, "q", who)) || (rc = pg_check_rows(out, out_stride, hd, n_head, hd, batch->rows, esz, "out", who))) return rc;
     if (gate && (rc = pg_check_rows(gate, gate_stride, gate_head_stride, n_head, hd, batch->rows, esz, "gate", who))) return rc;
     if (lse & 3) return sz_fail(SZ_E_ARG, "%s: lse misaligned", who);
-    PgScratch s = pg_scratch(batch->n_seq, batch->rows, n_head, hd, scratch);
+    PgScratch s = pg_scratch(cache, batch, n_head, scratch);
     if (!scratch || (scratch & 255) || scratch_bytes < s.bytes) return sz_fail(SZ_E_SCRATCH, "%s: %lld bytes of scratch given, %lld needed, 256-byte aligned", who, (long long)scratch_bytes, (long long)s.bytes);
     cudaStream_t st = (cudaStream_t)stream;
-    const PgBatch d = pg_batch(cache, batch, n_head, scratch);
+    PgBatch d = pg_batch(cache, batch, n_head, scratch);
     PgIo io = {};
     io.q = (const u8*)q; io.q_stride = q_stride * esz; io.gate = (const u8*)gate; io.gate_stride = gate_stride * esz; io.gate_head_stride = gate_head_stride * esz;
     io.out = (u8*)out; io.out_stride = out_stride * esz; io.lse = (float*)lse; io.type = io_type; io.esz = esz; io.scale_log2 = scale * 1.4426950408889634f;
@@ -390,14 +404,29 @@ extern "C" int sz_paged_attend(const sz_paged_cache* cache, const sz_paged_batch
     auto kernels = [&](int nqt) { return ct == PG_F16 ? pg_kernels_f16(wide, hd, nqt) : ct == PG_BF16 ? pg_kernels_bf16(wide, hd, nqt) : pg_kernels_q8(wide, hd, nqt); };
     const int64_t per_seq = (int64_t)G * ((batch->rows + batch->n_seq - 1) / batch->n_seq), all = (int64_t)G * batch->rows;
     const PgKernels ko = kernels(pg_tiles_of(per_seq)), ks = kernels(pg_tiles_of(all));
-    s.own.on = 1; s.own.tq = ko.tq; s.own.blocks = PG_BLOCKS * ko.occ; s.own.direct = batch->shared_len == 0;
-    s.own.planned = batch->n_seq > PG_PLAN || batch->n_seq + all / ko.tq > PG_PLAN;
-    s.shr.on = batch->shared_len > 0; s.shr.tq = ks.tq; s.shr.blocks = PG_BLOCKS * ks.occ; s.shr.shared = 1;
-    s.shr.planned = s.shr.on && (all + ks.tq - 1) / ks.tq > PG_PLAN;
-    if (s.own.planned || s.shr.planned) SZ_CUDA(sz_launch("paged_plan", sz_pg_plan_kernel, dim3(1), dim3(1024), 0, st, true, d, s.own, s.shr));
-    if (s.shr.on && (rc = pg_launch_attend(ks, d, io, s.shr, "paged_attend_shared", st))) return rc;
-    if ((rc = pg_launch_attend(ko, d, io, s.own, "paged_attend", st))) return rc;
+    const bool shared = batch->shared_len > 0, tc = pg_tc_type(cache->type) && io_type == cache->type && scale > 0.f;
+    const int tile = pg_tc_tile(hd);
+    auto on = [&](int i, int is_shared, int is_tc, int tq, int blocks) {
+        PgPart& p = s.a.p[i];
+        p.on = 1; p.shared = is_shared; p.tc = is_tc; p.tq = tq; p.blocks = blocks;
+        p.planned = (is_shared ? 0 : batch->n_seq) + (all + tq - 1) / tq > PG_PLAN;
+    };
+    if (tc && shared && all >= PG_TC_MIN && batch->shared_len >= PG_TC) { d.bulk_shared = tile; on(PG_SHARED_TC, 1, 1, tile, PG_BLOCKS); }
+    if (tc && per_seq >= PG_TC_MIN) { d.bulk_own = tile; on(PG_OWN_TC, 0, 1, tile, PG_BLOCKS); }
+    if (shared && !(d.bulk_shared && batch->shared_len % PG_TC == 0)) on(PG_SHARED, 1, 0, ks.tq, PG_BLOCKS * ks.occ);
+    on(PG_OWN, 0, 0, ko.tq, PG_BLOCKS * ko.occ);
+    s.a.p[PG_OWN].direct = !shared && !d.bulk_own;
+    bool planned = false;
+    for (const PgPart& p : s.a.p) planned |= p.planned;
+    if (planned) SZ_CUDA(sz_launch("paged_plan", sz_pg_plan_kernel, dim3(4), dim3(1024), 0, st, true, d, s.a));
+    for (int i = 0; i < 4; i++) {
+        const PgPart& p = s.a.p[i];
+        if (!p.on) continue;
+        static const char* const names[4] = {"paged_attend_shared_tc", "paged_attend_shared", "paged_attend_tc", "paged_attend"};
+        rc = p.tc ? pg_tc_launch(cache->type == SZ_TYPE_BF16, hd, cache->page_size, d, io, p, names[i], st) : pg_launch_attend(p.shared ? ks : ko, d, io, p, names[i], st);
+        if (rc) return rc;
+    }
     auto* merge = hd == 64 ? sz_pg_merge_kernel<64> : hd == 128 ? sz_pg_merge_kernel<128> : sz_pg_merge_kernel<256>;
-    SZ_CUDA(sz_launch("paged_merge", merge, dim3(batch->rows, n_head), dim3(PG_MERGE), 0, st, true, d, io, s.own, s.shr));
+    SZ_CUDA(sz_launch("paged_merge", merge, dim3(batch->rows, n_head), dim3(PG_MERGE), 0, st, true, d, io, s.a));
     return SZ_OK;
 }

@@ -17,6 +17,7 @@
 constexpr int PG_T = 64;             // positions a unit
 constexpr int PG_PLAN = 512;         // sequences and tiles that a block plans for itself; above, sz_pg_plan_kernel does once
 constexpr int PG_MAX_SEQ = 4096;
+constexpr int PG_TC = 128;           // positions a unit of the tcgen05 kernel (sz_paged_tc.cu)
 enum { PG_F16 = 0, PG_BF16 = 1, PG_Q8 = 2 };
 enum { PG_E_PAGE = 1, PG_E_END = 2, PG_E_SHARED = 4, PG_E_ROWS = 8, PG_E_WAIT = 16 };
 
@@ -25,6 +26,7 @@ struct PgBatch {                     // the tables of a call, as the kernels rea
     long long page_stride, head_stride, pos_stride;
     const int32_t *pages, *row_start, *lens, *shared_pages;
     int n_seq, rows, max_pages, shared_len, n_pages, ps_log2, nkv, G;
+    int bulk_own, bulk_shared;       // vectors a tile of the tcgen05 kernel, where it takes the positions that a whole tile sees (0: it does not)
     u32* err;
 };
 struct PgIo {                        // rows of queries and outputs; strides in bytes
@@ -48,17 +50,25 @@ struct PgPart {
     float* row_o;                    // [row][head][hd]: an item that one block did alone
     float2* row_ml;                  // [row][head]
     int blocks, tq, shared, planned; // planned: the plan was made by sz_pg_plan_kernel
+    int tc;                          // units of the tcgen05 kernel
     int direct;                      // an item that one block does alone goes straight to the output
     int on;
 };
 
 __device__ __forceinline__ int pg_row(const PgBatch& d, int i) { return min(max(__ldg(d.row_start + i), 0), d.rows); }
-// Units of tile t of a sequence with m rows whose own positions end at `end` (exclusive), and the tile's own end.
+// Of a sequence with m rows whose own positions end at `end` (exclusive), tile t of tq vectors: where what its last row sees ends ..
+__device__ __forceinline__ int pg_room(const PgBatch& d) { return (int)min((long long)d.max_pages << d.ps_log2, 0x7fffffc0ll); }
 __device__ __forceinline__ int pg_tile_end(const PgBatch& d, int m, long long end, int t, int tq) {
     const int last = (min((t + 1) * tq, m * d.G) - 1) / d.G;
-    const long long e = end - (m - 1 - last), room = (long long)d.max_pages << d.ps_log2;
-    return (int)max(0ll, min(e, room));
+    return (int)max(0ll, min(end - (m - 1 - last), (long long)pg_room(d)));
 }
+// .. and the whole units of PG_TC positions that all rows of the tcgen05 kernel's tile around it see: that kernel's, not this one's.
+__device__ __forceinline__ int pg_bulk(const PgBatch& d, int m, long long end, int t, int tq) {
+    if (!d.bulk_own) return 0;
+    const int first = t * tq / d.bulk_own * d.bulk_own / d.G;
+    return (int)max(0ll, min(end - (m - 1 - first), (long long)pg_room(d))) & ~(PG_TC - 1);
+}
+__device__ __forceinline__ int pg_bulk_shared(const PgBatch& d) { return d.bulk_shared ? d.shared_len & ~(PG_TC - 1) : 0; }
 // Which block has unit u when `blocks` share U units: the last i with i U / blocks <= u.
 __device__ __forceinline__ int pg_block_of(long long u, long long U, int blocks) { return (int)(((u + 1) * blocks - 1) / U); }
 
@@ -99,10 +109,10 @@ __device__ u32 pg_scan(u32 v, u32& total, u32* sm) {                // exclusive
 }
 // tiles[0 .. n_seq], units[0 .. tiles[n_seq]]; returns the number of tiles.  (SHARED: one tile list over the rows of all sequences.)
 template <int NTH>
-__device__ int pg_plan(const PgBatch& d, int shared, int tq, u32* tiles, u32* units, u32* sm) {
+__device__ int pg_plan(const PgBatch& d, int shared, int tc, int tq, u32* tiles, u32* units, u32* sm) {
     if (shared) {
         const int vec = (pg_row(d, d.n_seq) - pg_row(d, 0)) * d.G, E = max(0, (vec + tq - 1) / tq);
-        const u32 un = (u32)((d.shared_len + PG_T - 1) / PG_T);
+        const u32 un = (u32)(tc ? d.shared_len / PG_TC : (d.shared_len - pg_bulk_shared(d) + PG_T - 1) / PG_T);
         for (int e = threadIdx.x; e <= E; e += NTH) units[e] = (u32)e * un;
         if (threadIdx.x == 0) tiles[0] = 0;
         __syncthreads();
@@ -127,7 +137,9 @@ __device__ int pg_plan(const PgBatch& d, int shared, int tq, u32* tiles, u32* un
             int lo = 0, hi = d.n_seq - 1;                           // the last sequence whose tiles begin at or before e
             while (lo < hi) { const int mid = (lo + hi + 1) >> 1; if (tiles[mid] <= (u32)e) lo = mid; else hi = mid - 1; }
             const int m = pg_row(d, lo + 1) - pg_row(d, lo);
-            n = (u32)((pg_tile_end(d, m, (long long)__ldg(d.lens + lo) - d.shared_len, e - (int)tiles[lo], tq) + PG_T - 1) / PG_T);
+            const long long end = (long long)__ldg(d.lens + lo) - d.shared_len;
+            const int t = e - (int)tiles[lo], bulk = pg_bulk(d, m, end, t, tq);
+            n = (u32)(tc ? bulk / PG_TC : (pg_tile_end(d, m, end, t, tq) - bulk + PG_T - 1) / PG_T);
         }
         const u32 at = pg_scan<NTH>(n, total, sm);
         if (e < E) units[e] = carry + at;
@@ -203,7 +215,7 @@ __device__ __forceinline__ void pg_ldsm4t(u32* r, u32 addr) {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
 }
 
-struct PgItem { int e, h, i, n, b, t, end; };       // tile, key head, unit and units of the item; its sequence, tile of it, end of its positions
+struct PgItem { int e, h, i, n, b, t, begin, end; };       // tile, key head, unit and units of the item; its sequence, tile of it, its positions
 
 template <int CT, bool WIDE, int HD, int NQT>
 __global__ void __launch_bounds__(PgCfg<CT, WIDE, HD, NQT>::NTH, PgCfg<CT, WIDE, HD, NQT>::OCC)
@@ -229,7 +241,7 @@ sz_pg_attend_kernel(const __grid_constant__ PgBatch d, const __grid_constant__ P
         tiles = pt.tiles; units = pt.units;
         E = pt.shared ? max(0, ((pg_row(d, d.n_seq) - pg_row(d, 0)) * d.G + C::TQ - 1) / C::TQ) : (int)tiles[d.n_seq];
     } else {
-        E = pg_plan<C::NTH>(d, pt.shared, C::TQ, s_tiles, s_units, s_scan);
+        E = pg_plan<C::NTH>(d, pt.shared, 0, C::TQ, s_tiles, s_units, s_scan);
         if (blockIdx.x == 0) {                            // for the merge
             if (!pt.shared) for (int i = tid; i <= d.n_seq; i += C::NTH) pt.tiles[i] = s_tiles[i];
             for (int i = tid; i <= E; i += C::NTH) pt.units[i] = s_units[i];
@@ -244,7 +256,7 @@ sz_pg_attend_kernel(const __grid_constant__ PgBatch d, const __grid_constant__ P
     const int blocks = (int)min((long long)pt.blocks, U);
     if ((int)blockIdx.x >= blocks) return;
     const long long u0 = U * blockIdx.x / blocks, u1 = U * (blockIdx.x + 1) / blocks;
-    const int room = (int)min((long long)d.max_pages << d.ps_log2, 0x7fffffc0ll);
+    const int room = pg_room(d);
 
     auto locate = [&](long long u) {
         PgItem it;
@@ -256,12 +268,15 @@ sz_pg_attend_kernel(const __grid_constant__ PgBatch d, const __grid_constant__ P
         const u32 rem = (u32)(u - (long long)units[lo] * d.nkv);
         it.h = (int)(rem / (u32)it.n);
         it.i = (int)(rem % (u32)it.n);
-        if (pt.shared) { it.b = 0; it.t = lo; it.end = d.shared_len; return it; }
+        if (pt.shared) { it.b = 0; it.t = lo; it.begin = pg_bulk_shared(d); it.end = d.shared_len; return it; }
         int bl = 0, bh = d.n_seq - 1;
         while (bl < bh) { const int mid = (bl + bh + 1) >> 1; if (tiles[mid] <= (u32)lo) bl = mid; else bh = mid - 1; }
         it.b = bl;
         it.t = lo - (int)tiles[bl];
-        it.end = pg_tile_end(d, pg_row(d, bl + 1) - pg_row(d, bl), (long long)__ldg(d.lens + bl) - d.shared_len, it.t, C::TQ);
+        const int m = pg_row(d, bl + 1) - pg_row(d, bl);
+        const long long end = (long long)__ldg(d.lens + bl) - d.shared_len;
+        it.begin = pg_bulk(d, m, end, it.t, C::TQ);
+        it.end = pg_tile_end(d, m, end, it.t, C::TQ);
         return it;
     };
     // ---- loads: step s of the block is the keys (even) or values (odd) of unit u0 + s / 2
@@ -270,7 +285,7 @@ sz_pg_attend_kernel(const __grid_constant__ PgBatch d, const __grid_constant__ P
     int page = -1;                                        // lane l < PPW: the page of the warp's position l of the unit to load next
     long long off = -1;                                   // .. and its offset in the pools, of the unit being loaded
     auto peek = [&]() {
-        const int c = ld.i * PG_T + warp * C::PPW + lane;
+        const int c = ld.begin + ld.i * PG_T + warp * C::PPW + lane;
         page = -1;
         if (lane < C::PPW && c < ld.end) page = __ldg((pt.shared ? d.shared_pages : d.pages + (size_t)ld.b * d.max_pages) + (c >> d.ps_log2));
     };
@@ -279,7 +294,7 @@ sz_pg_attend_kernel(const __grid_constant__ PgBatch d, const __grid_constant__ P
         if (steps_left > 0) {
             steps_left--;
             if (which == 0) {
-                const int c = ld.i * PG_T + warp * C::PPW + lane;
+                const int c = ld.begin + ld.i * PG_T + warp * C::PPW + lane;
                 const bool there = lane < C::PPW && c < ld.end;
                 const bool ok = there && (u32)page < (u32)d.n_pages;
                 if (there && !ok) atomicOr(d.err, PG_E_PAGE);
@@ -377,7 +392,7 @@ sz_pg_attend_kernel(const __grid_constant__ PgBatch d, const __grid_constant__ P
         sz_cp_async_wait<C::NR - 2>();
         if (NQT == 1) __syncwarp(); else __syncthreads();
         issue(ipar); ipar ^= 1;
-        const int c0 = it.i * PG_T + pw;
+        const int c0 = it.begin + it.i * PG_T + pw;
         const u32 kb = rbase + (u32)(cslot * C::HALF);
         u32 okb;                                          // 16 SG bits from the warp's first position on
         if (C::SG == 1) okb = *(const u16*)(s_ok + cslot * 8 + 2 * way); else okb = *(const u32*)(s_ok + cslot * 8 + 4 * way);
@@ -530,7 +545,7 @@ sz_pg_attend_kernel(const __grid_constant__ PgBatch d, const __grid_constant__ P
                     for (int k = 0; k < 16; k++) {
                         const int src = (lane & ~3) | ((k & 7) >> 1), pos = pw + 16 * g + k;
                         const float w0 = __shfl_sync(0xffffffffu, p[g][4 * (k >> 3) + (k & 1)], src), w1 = __shfl_sync(0xffffffffu, p[g][4 * (k >> 3) + 2 + (k & 1)], src);
-                        const bool ok = (okb >> (16 * g + k)) & 1u, a = ok && it.i * PG_T + pos < lim0, b = ok && it.i * PG_T + pos < lim1;
+                        const bool ok = (okb >> (16 * g + k)) & 1u, a = ok && it.begin + it.i * PG_T + pos < lim0, b = ok && it.begin + it.i * PG_T + pos < lim1;
 #pragma unroll
                         for (int nt = 0; nt < C::NT; nt++) {
                             const float2 f = pg_unpack<CT>(*(const u32*)(vr + (size_t)pos * C::HB + ((nt ^ (pos & 7)) << 4) + 4 * q4));
@@ -691,6 +706,9 @@ struct PgKernels {
 PgKernels pg_kernels_f16(bool wide, int hd, int nqt);
 PgKernels pg_kernels_bf16(bool wide, int hd, int nqt);
 PgKernels pg_kernels_q8(bool wide, int hd, int nqt);
+// The tcgen05 kernel (sz_paged_tc.cu): vectors a tile; the launch over own or shared positions.
+int pg_tc_tile(int hd);
+int pg_tc_launch(bool bf16, int hd, int page_size, const PgBatch& d, const PgIo& io, const PgPart& p, const char* name, cudaStream_t st);
 
 template <int CT, bool WIDE, int HD, int NQT>
 PgKernels pg_one() {

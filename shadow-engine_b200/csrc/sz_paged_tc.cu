@@ -1,0 +1,413 @@
+// Attention of many query vectors over the same positions on the 5th-generation tensor cores: a long prefix that a whole batch shares, or what
+// was fed before a prompt's chunk.  (Few vectors a key head leave the kernel of sz_paged.cuh waiting for memory, not for its mma.sync; with
+// hundreds the products are the work: 4 head_dim operations a vector and position on 4 head_dim bytes.)
+//
+// It takes whole units of 128 positions that EVERY row of a tile sees, so it needs no masks; what is left - a tile's last positions, up to
+// each row's own - is the other kernel's, and the merge joins the parts.  Types: 16-bit queries over a cache of the same type.
+//
+// A block has NQ x 128 query vectors of one key head (two tiles of 128 up to head_dim 128, one above) and the lines of tensor memory:
+//     columns   0 .. 255   scores, two buffers of 128 (f32); the weights lie over the buffer they come from, as pairs of 16 bits
+//     columns 256 .. 511   the tiles' sums, NQ x head_dim
+// Unit u (tile u % NQ, positions u / NQ) has buffer u % 2.  One thread issues, in this order: scores(0), scores(1), then for every u, once
+// its weights are there, sums += weights(u) values, scores(u + 2).  The tensor core works in the order of issue, so scores(u + 2) cannot overwrite
+// weights(u) before they are used; while a tile's softmax runs, the other buffer's products do.
+//   warps 0 .. 3 (and 4 .. 7 for the second tile)   a thread has a query vector, lane = row of tensor memory: it reads its 128 scores
+//               (tcgen05.ld), moves its maximum - only when the largest is 2^8 above what it divides by, for then the sums have to be read,
+//               scaled and written back; weights up to 256 cost f32 and the 16-bit types nothing -, writes the weights (tcgen05.st) and keeps their sum.
+//   last two    keys and values by tiled TMA, a box a page (8 .. 128 positions x 64 dimensions, 128-byte swizzle), through a ring of 128 positions x
+//               128 dimensions; the issuing thread.
+// Operands: queries and keys K-major, values MN-major (their rows are the positions, which the product sums over), weights from tensor memory.
+// Rounding: a weight has 8 (bf16) or 11 bits, as the result; its sum is of the unrounded ones.  (Errors of independent weights average out:
+// the result's error stays below 1.3 of its last rounding's.)
+// A page out of range arrives as zeros (its box lies outside the pool's map) and its positions are masked.  Every wait is bounded.
+#include <cuda.h>
+#include "sz_paged.cuh"
+
+namespace {
+
+constexpr u32 PT_WAIT = 4000000u;
+
+__device__ __forceinline__ u64 pt_desc(u32 addr, u32 lbo, u32 sbo) {      // 128-byte swizzle (layout type 2), version 1
+    return (u64)((addr & 0x3ffffu) >> 4) | ((u64)(lbo >> 4) << 16) | ((u64)(sbo >> 4) << 32) | (1ull << 46) | (2ull << 61);
+}
+// kind::f16: D = f32, A and B f16 (0) or bf16 (1), M = 128, N; B K-major or (values) MN-major
+__host__ __device__ constexpr u32 pt_idesc(bool bf16, int n, bool b_mn) {
+    return (1u << 4) | ((bf16 ? 1u : 0u) << 7) | ((bf16 ? 1u : 0u) << 10) | ((b_mn ? 1u : 0u) << 16) | ((u32)(n >> 3) << 17) | ((128u >> 4) << 24);
+}
+__device__ __forceinline__ void pt_mma_ss(u32 d, u64 a, u64 b, u32 idesc, u32 acc) {
+    asm volatile("{ .reg .pred p; setp.ne.b32 p, %4, 0; tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p; }" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(acc) : "memory");
+}
+__device__ __forceinline__ void pt_mma_ts(u32 d, u32 a, u64 b, u32 idesc, u32 acc) {      // A from tensor memory
+    asm volatile("{ .reg .pred p; setp.ne.b32 p, %4, 0; tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p; }" ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(acc) : "memory");
+}
+__device__ __forceinline__ void pt_commit(u64* bar) {
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(sz_smem_addr(bar)) : "memory");
+}
+__device__ __forceinline__ void pt_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void pt_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void pt_ld32(u32 at, float* v) {              // 32 columns of the thread's row
+    u32* r = (u32*)v;
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]),
+                   "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
+                   "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+                 : "r"(at));
+}
+__device__ __forceinline__ void pt_loaded(float* v) {                    // the registers go through the wait, so that nothing uses them before it
+    u32* r = (u32*)v;
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]),
+                   "+r"(r[13]), "+r"(r[14]), "+r"(r[15]), "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]), "+r"(r[23]), "+r"(r[24]),
+                   "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]), "+r"(r[30]), "+r"(r[31])::"memory");
+}
+__device__ __forceinline__ void pt_st16(u32 at, const u32* r) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15};" ::"r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]),
+                 "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(at) : "memory");
+}
+__device__ __forceinline__ void pt_stored() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ bool pt_wait(u64* bar, u32 phase) { return sz_mbar_wait(bar, phase & 1, PT_WAIT); }
+__device__ __forceinline__ bool pt_wait_warp(u64* bar, u32 phase) { return __all_sync(0xffffffffu, pt_wait(bar, phase)); }
+__device__ __forceinline__ void pt_arrive_warp(u64* bar) { __syncwarp(); if ((threadIdx.x & 31) == 0) sz_mbar_arrive(bar); }
+
+template <int HD>
+struct PtCfg {
+    static constexpr int NQ = HD <= 128 ? 2 : 1, DB = HD < 128 ? HD : 128, NB = HD / DB;     // tiles; dimensions a ring slot, slots a unit's keys
+    static constexpr int SOFT = 128 * NQ, NTH = SOFT + 64, TQ = 128 * NQ;
+    static constexpr int SLOT = PG_TC * DB * 2, QT = 128 * HD * 2, BLK = PG_TC * 128;         // bytes; BLK: 128 rows of 64 dimensions
+    static constexpr int SLOTS = HD == 64 ? 8 : 4;
+    static constexpr int SMEM = 1024 + NQ * QT + SLOTS * SLOT;                                 // (1,024 to align)
+};
+struct PtBars {
+    u64 full[8], empty[8], s_full[2], p_full[2], pv_done[2], q_full[2], o_free[2];
+    u32 tmem, failed;
+    u32 ok[8][4];                    // which positions of a unit are there, of eight units: the eighth next one's keys are asked for after this one's weights were used
+    u32 tiles[PG_PLAN + 1], units[PG_PLAN + 1], scan[16];
+};
+
+template <bool BF, int HD>
+__global__ void __launch_bounds__(PtCfg<HD>::NTH, 1)
+sz_pg_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap, const __grid_constant__ PgBatch d, const __grid_constant__ PgIo io,
+                const __grid_constant__ PgPart pt, int rows_box) {
+    using C = PtCfg<HD>;
+    constexpr int CT = BF ? PG_BF16 : PG_F16;
+    __shared__ PtBars S;
+    extern __shared__ __align__(16) u8 raw[];
+    u8* const base = raw + (1024 - (sz_smem_addr(raw) & 1023)) % 1024;
+    u8* const sq = base;                                   // [tile][HD / 64][128 rows][128 bytes]
+    u8* const ring = sq + C::NQ * C::QT;                   // [slot][DB / 64][128 positions][128 bytes]
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    constexpr int TMA_WARP = C::SOFT / 32, MMA_WARP = TMA_WARP + 1;
+    if (tid == 0) {
+        for (int i = 0; i < 8; i++) { sz_mbar_init(&S.full[i], 1); sz_mbar_init(&S.empty[i], 1); }
+        for (int i = 0; i < 2; i++) { sz_mbar_init(&S.s_full[i], 1); sz_mbar_init(&S.p_full[i], 4); sz_mbar_init(&S.pv_done[i], 1); sz_mbar_init(&S.q_full[i], 4); sz_mbar_init(&S.o_free[i], 4); }
+        S.failed = 0;
+        sz_mbar_fence_init();
+    }
+    if (warp == 0) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(sz_smem_addr(&S.tmem)), "r"(512u) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    pt_before();
+    __syncthreads();
+    pt_after();
+    const u32 tmem = S.tmem;
+    sz_pdl_wait();
+    sz_pdl_trigger();
+    const u32 *tiles = S.tiles, *units = S.units;
+    int E;
+    if (pt.planned) {
+        tiles = pt.tiles; units = pt.units;
+        E = pt.shared ? max(0, ((pg_row(d, d.n_seq) - pg_row(d, 0)) * d.G + C::TQ - 1) / C::TQ) : (int)tiles[d.n_seq];
+    } else {
+        E = pg_plan<C::NTH>(d, pt.shared, 1, C::TQ, S.tiles, S.units, S.scan);
+        if (blockIdx.x == 0) {
+            if (!pt.shared) for (int i = tid; i <= d.n_seq; i += C::NTH) pt.tiles[i] = S.tiles[i];
+            for (int i = tid; i <= E; i += C::NTH) pt.units[i] = S.units[i];
+        }
+    }
+    const long long U = (long long)units[E] * d.nkv;
+    const int blocks = (int)min((long long)pt.blocks, U);
+    const bool work = (int)blockIdx.x < blocks;
+    const long long u0 = work ? U * blockIdx.x / blocks : 0, u1 = work ? U * (blockIdx.x + 1) / blocks : 0;
+    // the next piece of the block's share: an item, units i .. i + T of it
+    auto locate = [&](long long u) {
+        PgItem it;
+        const u32 un = (u32)(u / d.nkv);
+        int lo = 0, hi = E - 1;
+        while (lo < hi) { const int mid = (lo + hi + 1) >> 1; if (units[mid] <= un) lo = mid; else hi = mid - 1; }
+        it.e = lo;
+        it.n = (int)(units[lo + 1] - units[lo]);
+        const u32 rem = (u32)(u - (long long)units[lo] * d.nkv);
+        it.h = (int)(rem / (u32)it.n);
+        it.i = (int)(rem % (u32)it.n);
+        it.begin = 0; it.end = it.n * PG_TC;
+        it.b = 0; it.t = lo;
+        if (pt.shared) return it;
+        int bl = 0, bh = d.n_seq - 1;
+        while (bl < bh) { const int mid = (bl + bh + 1) >> 1; if (tiles[mid] <= (u32)lo) bl = mid; else bh = mid - 1; }
+        it.b = bl;
+        it.t = lo - (int)tiles[bl];
+        return it;
+    };
+    // Where keys (kind 0) and values (1) of unit j come in a piece's order of loads, in slots; T units
+    auto place = [&](int kind, int j, int T) {
+        if (C::NQ == 2) return (2 * j + kind) * C::NB;
+        return (kind == 0 ? (j ? 2 * j - 1 : 0) : (j + 1 < T ? 2 * j + 2 : 2 * T - 1)) * C::NB;
+    };
+    int failed = 0;
+    if (warp == TMA_WARP) {
+        // ---- loads
+        const int pieces = PG_TC / rows_box;
+        u32 seq = 0, units_in = 0;                         // slots filled, units' keys asked for so far
+        for (long long u = u0; u < u1 && !failed;) {
+            const PgItem it = locate(u);
+            const int T = (int)min((long long)(it.n - it.i), u1 - u);
+            const int32_t* table = pt.shared ? d.shared_pages : d.pages + (size_t)it.b * d.max_pages;
+            for (int x = 0; x < 2 * T && !failed; x++) {
+                int kind, j;
+                if (C::NQ == 2) { kind = x & 1; j = x >> 1; }
+                else if (x == 0) { kind = 0; j = 0; }
+                else if (x == 2 * T - 1) { kind = 1; j = T - 1; }
+                else { kind = (x & 1) ^ 1; j = kind ? x / 2 - 1 : (x + 1) / 2; }
+                const int c = (it.i + j) * PG_TC + lane * rows_box;
+                int page = -1;
+                if (lane < pieces) page = __ldg(table + (c >> d.ps_log2));
+                const bool ok = (u32)page < (u32)d.n_pages;
+                if (lane < pieces && !ok) atomicOr(d.err, PG_E_PAGE);
+                for (int nb = 0; nb < C::NB; nb++, seq++) {
+                    const int sl = (int)(seq % C::SLOTS);
+                    if (seq >= C::SLOTS && !pt_wait_warp(&S.empty[sl], seq / C::SLOTS - 1)) { failed = 1; break; }
+                    if (kind == 0 && nb == 0) {            // (read by the softmax threads after the scores are there, which the copies' arrival comes before)
+                        const u32 bits = __ballot_sync(0xffffffffu, ok);
+                        if (lane < 4) {
+                            u32 w = 0;
+                            for (int k = 0; k < 32; k += 8) if ((bits >> ((lane * 32 + k) / rows_box)) & 1u) w |= 0xffu << k;
+                            S.ok[units_in & 7][lane] = w;
+                        }
+                        units_in++;
+                        __syncwarp();
+                    }
+                    if (lane == 0) sz_mbar_expect_tx(&S.full[sl], C::SLOT);
+                    __syncwarp();
+                    if (lane < pieces) {
+#pragma unroll
+                        for (int q = 0; q < C::DB / 64; q++)
+                            asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(
+                                             sz_smem_addr(ring + (size_t)sl * C::SLOT + q * C::BLK + lane * rows_box * 128)),
+                                         "l"(kind ? &vmap : &kmap), "r"(nb * C::DB + q * 64), "r"(c & ((1 << d.ps_log2) - 1)), "r"(it.h), "r"(ok ? page : d.n_pages),
+                                         "r"(sz_smem_addr(&S.full[sl]))
+                                         : "memory");
+                    }
+                }
+            }
+            u += T;
+        }
+        __syncwarp();
+    } else if (warp == MMA_WARP) {
+        // ---- issue: one thread
+        if (lane == 0) {
+            constexpr u32 id_s = pt_idesc(BF, PG_TC, false), id_v = pt_idesc(BF, C::DB, true);
+            const u64 qd = pt_desc(sz_smem_addr(sq), 16, 1024), kd = pt_desc(sz_smem_addr(ring), 16, 1024), vd = pt_desc(sz_smem_addr(ring), C::BLK, 1024);
+            u32 seq0 = 0, piece = 0, used[2] = {0, 0};     // slots before this piece; pieces; weights taken of a buffer
+            u32 buf0 = 0;                                  // the buffer of the piece's unit 0
+            for (long long u = u0; u < u1 && !failed; piece++) {
+                const PgItem it = locate(u);
+                const int T = (int)min((long long)(it.n - it.i), u1 - u), N = T * C::NQ;
+                for (int q = 0; q < C::NQ && !failed; q++) if (!pt_wait(&S.q_full[q], piece)) failed = 2;
+                auto scores = [&](int x) {
+                    const int q = x % C::NQ, j = x / C::NQ, buf = (int)((buf0 + x) & 1);
+                    const u32 at = seq0 + place(0, j, T);
+                    for (int nb = 0; nb < C::NB; nb++) {
+                        const int sl = (int)((at + nb) % C::SLOTS);
+                        if (q == 0 && !pt_wait(&S.full[sl], (at + nb) / C::SLOTS)) { failed = 3; return; }
+                        pt_after();
+#pragma unroll
+                        for (int k = 0; k < C::DB / 16; k++)       // (addresses in 16-byte units: 16 dimensions are 32 bytes of a row)
+                            pt_mma_ss(tmem + buf * 128, qd + (u32)((q * C::QT + (nb * (C::DB / 64) + k / 4) * C::BLK) / 16 + (k % 4) * 2), kd + (u32)((sl * C::SLOT + k / 4 * C::BLK) / 16 + (k % 4) * 2),
+                                      id_s, nb | k);
+                        if (q == C::NQ - 1) pt_commit(&S.empty[sl]);
+                    }
+                    pt_commit(&S.s_full[buf]);
+                };
+                if (!failed) scores(0);
+                if (!failed && N > 1) scores(1);
+                for (int x = 0; x < N && !failed; x++) {
+                    const int q = x % C::NQ, j = x / C::NQ, buf = (int)((buf0 + x) & 1);
+                    if (!pt_wait(&S.p_full[buf], used[buf]++)) { failed = 4; break; }
+                    if (x < C::NQ && piece > 0 && !pt_wait(&S.o_free[q], piece - 1)) { failed = 5; break; }
+                    pt_after();
+                    const u32 at = seq0 + place(1, j, T);
+                    for (int nb = 0; nb < C::NB; nb++) {
+                        const int sl = (int)((at + nb) % C::SLOTS);
+                        if (q == 0 && !pt_wait(&S.full[sl], (at + nb) / C::SLOTS)) { failed = 6; break; }
+                        pt_after();
+#pragma unroll
+                        for (int k = 0; k < PG_TC / 16; k++)       // 16 positions: 8 columns of weight pairs, 16 rows of 128 bytes
+                            pt_mma_ts(tmem + 256 + q * HD + nb * C::DB, tmem + buf * 128 + k * 8, vd + (u32)((sl * C::SLOT + k * 2048) / 16), id_v, (u32)(j | k));
+                        if (q == C::NQ - 1) pt_commit(&S.empty[sl]);
+                    }
+                    if (failed) break;
+                    pt_commit(&S.pv_done[q]);
+                    if (x + 2 < N) scores(x + 2);
+                }
+                seq0 += 2 * T * C::NB;
+                buf0 = (buf0 + N) & 1;
+                u += T;
+            }
+        }
+        __syncwarp();
+    } else {
+        // ---- softmax: thread = query vector
+        const int q = warp / 4, row = tid & 127;
+        const u32 lanes = (u32)((warp & 3) * 32) << 16;
+        u32 piece = 0, taken[2] = {0, 0}, done = 0, buf0 = 0;      // taken: scores of a buffer; done: units of this tile
+        for (long long u = u0; u < u1 && !failed; piece++) {
+            const PgItem it = locate(u);
+            const int T = (int)min((long long)(it.n - it.i), u1 - u);
+            const int r0 = pg_row(d, it.b), m = (pt.shared ? pg_row(d, d.n_seq) : pg_row(d, it.b + 1)) - r0;
+            const int v = q * 128 + row, vec = it.t * C::TQ + v, qr = vec / d.G, head = it.h * d.G + vec % d.G;
+            {   // the query vector into the K-major order: chunk c of 8 dimensions of row r at chunk c ^ (r & 7) of its 128 bytes
+                const uint4* src = (const uint4*)(io.q + (long long)(r0 + qr) * io.q_stride + (long long)head * HD * 2);
+                u8* dst = sq + q * C::QT + row * 128;
+#pragma unroll 8
+                for (int c = 0; c < HD / 8; c++) {
+                    const uint4 w = qr < m ? __ldg(src + c) : make_uint4(0, 0, 0, 0);
+                    *(uint4*)(dst + c / 8 * C::BLK + (((c & 7) ^ (row & 7)) << 4)) = w;
+                }
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                pt_arrive_warp(&S.q_full[q]);
+            }
+            float mx = -INFINITY, l = 0.f;                 // what the row divides by (in units of log 2), the sum of its weights
+            for (int j = 0; j < T; j++) {
+                const int buf = C::NQ == 2 ? q : (int)((buf0 + j) & 1);
+                if (!pt_wait_warp(&S.s_full[buf], taken[buf]++)) { failed = 7; break; }
+                pt_after();
+                float s[128];
+                const u32 at = tmem + lanes + buf * 128;
+#pragma unroll
+                for (int k = 0; k < 4; k++) pt_ld32(at + 32 * k, s + 32 * k);
+#pragma unroll
+                for (int k = 0; k < 4; k++) pt_loaded(s + 32 * k);
+                const u32* ok = S.ok[done & 7];
+                if ((ok[0] & ok[1] & ok[2] & ok[3]) != 0xffffffffu) {
+#pragma unroll
+                    for (int k = 0; k < 128; k++) s[k] = (ok[k / 32] >> (k & 31)) & 1u ? s[k] : -INFINITY;
+                }
+                float big[4] = {s[0], s[1], s[2], s[3]};
+#pragma unroll
+                for (int k = 4; k < 128; k++) big[k & 3] = fmaxf(big[k & 3], s[k]);
+                const float top = fmaxf(fmaxf(big[0], big[1]), fmaxf(big[2], big[3])) * io.scale_log2;
+                const bool up = top > mx + 8.f || (mx == -INFINITY && top > -INFINITY);
+                if (__any_sync(0xffffffffu, up)) {
+                    const float by = !up ? 1.f : mx == -INFINITY ? 0.f : pg_ex2(mx - top);
+                    if (up) { mx = top; l *= by; }
+                    if (j > 0) {                           // the sums so far, once the last product is in them
+                        if (!pt_wait_warp(&S.pv_done[q], done - 1)) { failed = 8; break; }
+                        pt_after();
+#pragma unroll 1
+                        for (int k = 0; k < HD; k += 32) {
+                            float o[32];
+                            pt_ld32(tmem + lanes + 256 + q * HD + k, o);
+                            pt_loaded(o);
+#pragma unroll
+                            for (int e = 0; e < 32; e++) o[e] *= by;
+                            pt_st16(tmem + lanes + 256 + q * HD + k, (const u32*)o);
+                            pt_st16(tmem + lanes + 256 + q * HD + k + 16, (const u32*)o + 16);
+                        }
+                    }
+                }
+                const float sub = mx == -INFINITY ? 0.f : mx;
+                float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int k = 0; k < 128; k += 32) {
+                    u32 w[16];
+#pragma unroll
+                    for (int e = 0; e < 32; e += 2) {
+                        const float a = pg_ex2(fmaf(s[k + e], io.scale_log2, -sub)), b = pg_ex2(fmaf(s[k + e + 1], io.scale_log2, -sub));
+                        sum[(e >> 1) & 3] += a + b;
+                        w[e / 2] = pg_pack<CT>(a, b);
+                    }
+                    pt_st16(at + k / 2, w);
+                }
+                l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+                pt_stored();
+                pt_before();
+                pt_arrive_warp(&S.p_full[buf]);
+                done++;
+            }
+            // ---- the piece's part: (maximum, sum of weights, sums)
+            if (!failed && !pt_wait_warp(&S.pv_done[q], done - 1)) failed = 9;
+            if (failed) break;
+            pt_after();
+            const long long us = (long long)units[it.e] * d.nkv + (long long)it.h * it.n;
+            const int b0 = pg_block_of(us, U, blocks), b1 = pg_block_of(us + it.n - 1, U, blocks);
+            const size_t to = b0 == b1 ? (size_t)(r0 + qr) * (d.nkv * d.G) + head : (size_t)(2 * blockIdx.x + ((int)blockIdx.x == b0 ? 1 : 0)) * C::TQ + v;
+            float* w = (b0 == b1 ? pt.row_o : pt.o) + to * HD;
+#pragma unroll 1
+            for (int k = 0; k < HD; k += 32) {
+                float o[32];
+                pt_ld32(tmem + lanes + 256 + q * HD + k, o);
+                pt_loaded(o);
+                if (qr < m) {
+#pragma unroll
+                    for (int e = 0; e < 32; e += 4) *(float4*)(w + k + e) = make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+                }
+            }
+            if (qr < m) (b0 == b1 ? pt.row_ml : pt.ml)[to] = make_float2(mx, l);
+            pt_before();
+            pt_arrive_warp(&S.o_free[q]);
+            buf0 = (buf0 + T * C::NQ) & 1;
+            u += T;
+        }
+    }
+    if (failed) atomicMax(&S.failed, (u32)failed);
+    pt_before();
+    __syncthreads();
+    if (warp == 0) {
+        pt_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
+    }
+    if (tid == 0 && S.failed) atomicOr(d.err, PG_E_WAIT);
+}
+
+typedef CUresult (*PtEncodeTiled)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*, const cuuint32_t*,
+                                  CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+PtEncodeTiled pt_encoder() {
+    static PtEncodeTiled fn = nullptr;
+    if (!fn) {
+        void* p = nullptr;
+        cudaDriverEntryPointQueryResult q = cudaDriverEntryPointSymbolNotFound;
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) == cudaSuccess && q == cudaDriverEntryPointSuccess) fn = (PtEncodeTiled)p;
+    }
+    return fn;
+}
+
+template <bool BF, int HD>
+int pt_launch(int page_size, const PgBatch& d, const PgIo& io, const PgPart& p, const char* name, cudaStream_t st) {
+    using C = PtCfg<HD>;
+    int rc = sz_allow_smem((const void*)sz_pg_tc_kernel<BF, HD>, C::SMEM);
+    if (rc) return rc;
+    PtEncodeTiled enc = pt_encoder();
+    if (!enc) return sz_fail(SZ_E_CUDA, "sz_paged_attend: the driver has no cuTensorMapEncodeTiled");
+    const int box_rows = page_size < PG_TC ? page_size : PG_TC;
+    CUtensorMap map[2];
+    for (int i = 0; i < 2; i++) {       // a pool as [page][key head][position][dimension]; x is 0 or 64 dimensions on: multiples of 16 bytes
+        const cuuint64_t dim[4] = {(cuuint64_t)HD, (cuuint64_t)page_size, (cuuint64_t)d.nkv, (cuuint64_t)d.n_pages};
+        const cuuint64_t stride[3] = {(cuuint64_t)d.pos_stride, (cuuint64_t)d.head_stride, (cuuint64_t)d.page_stride};
+        const cuuint32_t box[4] = {64, (cuuint32_t)box_rows, 1, 1}, es[4] = {1, 1, 1, 1};
+        const CUresult r = enc(&map[i], BF ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, (void*)(i ? d.v : d.k), dim, stride, box, es,
+                               CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+        if (r != CUDA_SUCCESS) return sz_fail(SZ_E_CUDA, "sz_paged_attend: cuTensorMapEncodeTiled failed (%d)", (int)r);
+    }
+    SZ_CUDA(sz_launch(name, sz_pg_tc_kernel<BF, HD>, dim3(p.blocks), dim3(C::NTH), C::SMEM, st, true, map[0], map[1], d, io, p, box_rows));
+    return SZ_OK;
+}
+
+}  // namespace
+
+int pg_tc_tile(int hd) { return hd <= 128 ? 256 : 128; }
+
+int pg_tc_launch(bool bf16, int hd, int page_size, const PgBatch& d, const PgIo& io, const PgPart& p, const char* name, cudaStream_t st) {
+    if (bf16) return hd == 64 ? pt_launch<true, 64>(page_size, d, io, p, name, st) : hd == 128 ? pt_launch<true, 128>(page_size, d, io, p, name, st) : pt_launch<true, 256>(page_size, d, io, p, name, st);
+    return hd == 64 ? pt_launch<false, 64>(page_size, d, io, p, name, st) : hd == 128 ? pt_launch<false, 128>(page_size, d, io, p, name, st) : pt_launch<false, 256>(page_size, d, io, p, name, st);
+}

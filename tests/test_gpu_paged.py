@@ -105,8 +105,11 @@ class Case:
     def tolerance(self, want, mag):
         """Half a step of the result's type; before it, f32 arithmetic: a score is a sum of hd products (hd 2^-23 of their magnitudes, |q||k| scale below 12
         sigma = 30 here, in units of its own exponent), which moves every weight by that much, and sums of up to 64 partial sums - 2^-13 of the
-        weighted magnitudes holds f32's part with a wide margin; 16-bit results carry weights of 11 bits and more: 2^-10 of the magnitudes."""
-        return HALF_STEP[self.io] * want.abs() + (2.0 ** -13 if self.io == torch.float32 else 2.0 ** -10) * mag + 1e-30
+        weighted magnitudes holds f32's part with a wide margin; 16-bit results carry weights of 11 bits and more: 2^-10 of the magnitudes.
+        Where many rows share positions (tcgen05: 16-bit queries over their own type) weights are rounded to the result's type: half a step of
+        every weight, of the magnitudes in sum."""
+        many = self.io != torch.float32 and self.k.dtype == self.io and self.rows * self.nh // self.nkv >= 96
+        return HALF_STEP[self.io] * (want.abs() + (mag if many else 0)) + (2.0 ** -13 if self.io == torch.float32 else 2.0 ** -10) * mag + 1e-30
 
     def check(self, gate=None, **kw):
         out = torch.full_like(self.q, 77.0)
@@ -319,6 +322,66 @@ def test_another_stream():
         out = c.step.attend(c.q)
     side.synchronize()
     assert torch.equal(out, want)
+
+
+# ---- many rows over the same positions (whole units of 128 on tcgen05, the rest as above) --------------------------------------------------
+@pytest.mark.parametrize("hd", [64, 128, 256])
+@pytest.mark.parametrize("kind", ["bf16", "f16"])
+@pytest.mark.parametrize("lens,ms,shared", [([200], [100], 0), ([1300], [129], 0), ([3000, 260, 128], [40, 200, 128], 0), ([600 + i for i in range(24)], [1 + i % 3 for i in range(24)], 512),
+                                            ([1500 + i for i in range(16)], [2] * 16, 1441), ([10000], [16], 0)])
+def test_many_rows(hd, kind, lens, ms, shared):
+    Case(lens, ms, nh=8, nkv=1, hd=hd, io=kind, cache=kind, shared=shared, seed=hd, page=32).check()
+
+
+@pytest.mark.parametrize("page,layout", [(8, "hnd"), (16, "nhd"), (64, "nhd"), (128, "hnd"), (1024, "nhd")])
+def test_many_rows_pages_and_layouts(page, layout):
+    Case([2900, 300], [60, 111], nh=10, nkv=2, hd=128, io="bf16", cache="bf16", page=page, layout=layout, seed=page, pad=3).check()
+
+
+@pytest.mark.parametrize("nh,nkv", [(3, 3), (14, 2), (48, 1), (200, 1)])
+def test_many_rows_head_groups(nh, nkv):
+    Case([700, 1000], [100, 37], nh=nh, nkv=nkv, hd=64, io="bf16", cache="bf16", seed=nh).check()
+
+
+def test_many_rows_scores_that_climb():
+    """Every unit's largest score is far above the one's before: the sums are scaled again and again; and the other way round."""
+    for way in (1, -1):
+        c = Case([1280], [130], nh=4, nkv=2, hd=128, io="bf16", cache="bf16", seed=3, page=128)
+        for p in range(10):
+            c.k[int(c.pages[0, p])] *= (0.2 + 0.4 * p) if way > 0 else (4.0 - 0.4 * p)
+        c.check()
+
+
+def test_many_rows_bad_pages_are_left_out_and_reported():
+    c = Case([900], [130], nh=4, nkv=1, hd=64, io="bf16", cache="bf16", page=16, seed=4)
+    keep = c.pages.clone()
+    c.pages[0, 3] = -5
+    c.pages[0, 20] = c.k.shape[0]
+    out = c.step.attend(c.q)
+    assert c.step.status() == 1
+    c.pages.copy_(keep)
+    k, v = c.positions(c.k, 0), c.positions(c.v, 0)
+    for j in (0, 64, 129):
+        seen = torch.tensor([t for t in range(900 - 130 + j + 1) if t // 16 not in (3, 20)], device="cuda")
+        for h in range(4):
+            w = torch.softmax(k[seen, 0] @ c.q[j, h].double() / 8, 0)
+            want, mag = w @ v[seen, 0], w @ v[seen, 0].abs()
+            assert bool(((out[j, h].double() - want).abs() < c.tolerance(want, mag)).all())
+
+
+def test_many_rows_hidden_positions_do_not_matter():
+    for bad in (math.nan, math.inf):
+        c = Case([700], [130], nh=4, nkv=1, hd=128, io="bf16", cache="bf16", page=16, seed=5)
+        before = c.check()
+        last = c.pages[0, 699 // 16]
+        c.k[last, :, 700 % 16:] = bad
+        c.v[last, :, 700 % 16:] = bad
+        out = c.step.attend(c.q)
+        assert torch.equal(out, before)
+        c.v[last, :, 699 % 16, 7] = bad                # the last row's own
+        out = c.step.attend(c.q)
+        assert float((out[:129].double() - before[:129].double()).abs().max()) < 2.0 ** -7 * float(before.abs().max())
+        assert not bool(torch.isfinite(out[129, :, 7]).any()) and bool(torch.isfinite(out[129, :, :7]).all())
 
 
 # ---- append ------------------------------------------------------------------------------------------------------------------------------
