@@ -68,7 +68,7 @@ __global__ void __launch_bounds__(256) sz_pg_append_kernel(const __grid_constant
     }
     const u8* src = kind == 0 ? a.q + (long long)r * a.q_stride + (long long)h * a.q_head_stride
                               : (kind == 1 ? a.k + (long long)r * a.k_stride : a.v + (long long)r * a.v_stride) + (long long)h * a.hd * a.esz;
-    float2 f[4];
+    float2 f[4] = {};
 #pragma unroll
     for (int i = 0; i < 4; i++)
         if (64 * i < a.hd) f[i] = pg_load2(src + (long long)(2 * (lane + 32 * i)) * a.esz, a.type);
@@ -136,20 +136,19 @@ __global__ void __launch_bounds__(256) sz_pg_append_kernel(const __grid_constant
 }
 
 // ---- the plan of a call with more sequences or tiles than a block plans for itself ---------------------------------------------------------
-struct PgParts { PgPart p[4]; };      // in the order of the positions: shared ones by the tcgen05 kernel, the rest of them, own ones likewise
-enum { PG_SHARED_TC = 0, PG_SHARED = 1, PG_OWN_TC = 2, PG_OWN = 3 };
+struct PgParts { PgPart p[2]; };      // in the order of the positions
+enum { PG_SHARED = 0, PG_OWN = 1 };
 __global__ void __launch_bounds__(1024) sz_pg_plan_kernel(const __grid_constant__ PgBatch d, const __grid_constant__ PgParts a) {
     __shared__ u32 scan[32];
     const PgPart& p = a.p[blockIdx.x];
     sz_pdl_wait();
     sz_pdl_trigger();
-    if (p.on && p.planned) pg_plan<1024>(d, p.shared, p.tc, p.tq, p.tiles, p.units, scan);
+    if (p.on && p.planned) pg_plan<1024>(d, p.shared, p.unit, p.tq, p.tiles, p.units, scan, nullptr, nullptr);
 }
 
 // ---- joining the parts -----------------------------------------------------------------------------------------------------------------------------
-// A block has one row and head: the parts of its items, in the order of the positions.  Threads in groups of hd / 4 take the parts in turn (four
-// columns each); the groups' sums are added in order.
-constexpr int PG_MERGE = 128, PG_PARTS = 2 * 5 * PG_BLOCKS;
+// W warps have one row and head: the parts of its items, in the order of the positions.  A lane has hd / 32 columns; the warps take the
+// parts in turn and their sums are added in order.  One warp where rows and heads are many, eight where they are few and their parts therefore many.
 struct PgList { int n, first, alone, lane; };     // parts of an item: their number, the block of the first; by row and head; the vector's place in its tile
 __device__ PgList pg_list(const PgBatch& d, const PgPart& p, int r, int r0, int b, int h) {
     PgList l = {};
@@ -159,93 +158,118 @@ __device__ PgList pg_list(const PgBatch& d, const PgPart& p, int r, int r0, int 
     const int E = p.shared ? ((pg_row(d, d.n_seq) - start) * d.G + p.tq - 1) / p.tq : (int)p.tiles[d.n_seq];
     const u32 us = p.units[e], n = p.units[e + 1] - us;
     if (!n) return l;
-    const long long U = (long long)p.units[E] * d.nkv, at = (long long)us * d.nkv + (long long)(h / d.G) * n;
-    const int blocks = (int)min((long long)p.blocks, U), last = pg_block_of(at + n - 1, U, blocks);
-    l.first = pg_block_of(at, U, blocks);
-    l.n = last - l.first + 1;
+    const u32 U = p.units[E] * (u32)d.nkv, at = us * (u32)d.nkv + (u32)(h / d.G) * n;
+    const PgShare share = pg_share(U, (int)min((u32)p.blocks, U));
+    l.first = pg_block_of(share, at);
+    l.n = pg_block_of(share, at + n - 1) - l.first + 1;
     l.alone = l.n == 1;
     l.lane = vec % p.tq;
     return l;
 }
-template <int HD>
-__global__ void __launch_bounds__(PG_MERGE) sz_pg_merge_kernel(const __grid_constant__ PgBatch d, const __grid_constant__ PgIo io, const __grid_constant__ PgParts a) {
-    __shared__ float wgt[PG_PARTS];
-    __shared__ float sum_of[PG_PARTS];
-    __shared__ const float* from[PG_PARTS];
-    __shared__ float red[PG_MERGE / 32], redl[PG_MERGE / 32];
-    __shared__ float4 sums[PG_MERGE];
-    const int r = blockIdx.x, h = blockIdx.y, nh = d.nkv * d.G, tid = threadIdx.x;
+template <int HD, int W>
+__global__ void __launch_bounds__(256) sz_pg_merge_kernel(const __grid_constant__ PgBatch d, const __grid_constant__ PgIo io, const __grid_constant__ PgParts a) {
+    constexpr int E = HD / 32;                                       // columns a lane, in pairs: 2 lane + 64 x
+    __shared__ float2 sums[W > 1 ? W : 1][HD / 2], of_warp[8];
+    const int r = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, sub = warp % W, h = blockIdx.y * (8 / W) + warp / W, nh = d.nkv * d.G;
     sz_pdl_wait();
     sz_pdl_trigger();
-    const int b = pg_seq_of<PG_MERGE>(d, r);
-    if (b < 0) return;
+    const int b = pg_seq_of<256>(d, r);
+    if (b < 0 || h >= nh) return;                                    // (h: W = 8 has one head a block)
     const int r0 = pg_row(d, b), m = pg_row(d, b + 1) - r0;
     const bool sees = (long long)__ldg(d.lens + b) - d.shared_len - (m - 1 - (r - r0)) > 0;     // a position of its own
-    u8* op = io.out + (long long)r * io.out_stride + (long long)h * HD * io.esz;
-    int n = 0;
-    float M = -INFINITY;
+    PgList l[2] = {};
     if (sees) {
-#pragma unroll 1
-        for (int s = 0; s < 4; s++) {
-            const PgPart& p = a.p[s];
-            const PgList l = pg_list(d, p, r, r0, b, h);
-            if (s == PG_OWN && p.direct && l.alone) return;          // (written by the block that did it)
-            for (int i = tid; i < l.n; i += PG_MERGE) {
-                const size_t at = l.alone ? (size_t)r * nh + h : (size_t)(i == 0 ? 2 * l.first + 1 : 2 * (l.first + i)) * p.tq + l.lane;
-                const float2 ml = (l.alone ? p.row_ml : p.ml)[at];
-                wgt[n + i] = ml.x;
-                sum_of[n + i] = ml.y;
-                from[n + i] = (l.alone ? p.row_o : p.o) + at * HD;
-                M = fmaxf(M, ml.x);
-            }
-            n += l.n;
-        }
+        l[PG_OWN] = pg_list(d, a.p[PG_OWN], r, r0, b, h);
+        if (a.p[PG_OWN].direct && l[PG_OWN].alone) return;           // (written by the block that did it)
+        l[PG_SHARED] = pg_list(d, a.p[PG_SHARED], r, r0, b, h);
     }
+    const int s0 = a.p[0].ways == 4 ? 2 : a.p[0].ways - 1, s1 = a.p[1].ways == 4 ? 2 : a.p[1].ways - 1;      // (ways: 1, 2 or 4)
+    const int n0 = l[0].n << s0, n = n0 + (l[1].n << s1);
+    auto place = [&](int i, const float2*& ml) -> const float* {     // part i
+        const bool own = i >= n0;
+        const PgPart& p = a.p[own];
+        const PgList& x = own ? l[1] : l[0];
+        const int sh = own ? s1 : s0, j = own ? i - n0 : i, k = j >> sh;
+        const size_t at = ((x.alone ? (size_t)r * nh + h : (size_t)(k == 0 ? 2 * x.first + 1 : 2 * (x.first + k)) * p.tq + x.lane) << sh) + (j & ((1 << sh) - 1));
+        ml = (x.alone ? p.row_ml : p.ml) + at;
+        return (x.alone ? p.row_o : p.o) + at * HD;
+    };
+    // the warp's parts are sub, sub + W ..: their largest maximum, then 32 at a time their weights, one a lane, and their sums
+    float M = -INFINITY, L = 0.f;
+#pragma unroll 2
+    for (int i = sub + W * lane; i < n; i += 32 * W) { const float2* ml; place(i, ml); M = fmaxf(M, ml->x); }
 #pragma unroll
     for (int s = 16; s > 0; s >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, s));
-    if ((tid & 31) == 0) red[tid >> 5] = M;
-    __syncthreads();                                                 // (and the lists are there)
+    float2 acc[E / 2];
 #pragma unroll
-    for (int w = 0; w < PG_MERGE / 32; w++) M = fmaxf(M, red[w]);
-    float L = 0.f;
-    for (int i = tid; i < n; i += PG_MERGE) {
-        const float c = wgt[i] == -INFINITY ? 0.f : pg_ex2(wgt[i] - M);
-        wgt[i] = c;
-        L += c * sum_of[i];
+    for (int x = 0; x < E / 2; x++) acc[x] = make_float2(0.f, 0.f);
+    for (int i0 = sub; i0 < n; i0 += 32 * W) {
+        const int i = i0 + W * lane;
+        float c = 0.f;
+        const float* from = nullptr;
+        if (i < n) {
+            const float2* ml;
+            from = place(i, ml);
+            const float2 x = *ml;
+            c = x.x == -INFINITY ? 0.f : pg_ex2(x.x - M);
+            if (x.x != -INFINITY) L += c * x.y; else from = nullptr;
+        }
+        u32 left = __ballot_sync(0xffffffffu, from != nullptr);      // (empty parts have no sums)
+        while (left) {
+            constexpr int B = 8;                                     // parts in flight
+            float2 f[B][E / 2];
+            float cw[B];
+#pragma unroll
+            for (int k = 0; k < B; k++) {
+                const int src = left ? __ffs(left) - 1 : 0;
+                const float* pk = (const float*)__shfl_sync(0xffffffffu, (unsigned long long)from, src);
+                cw[k] = __shfl_sync(0xffffffffu, c, src);
+                const bool ok = left != 0;
+                left &= left - 1;
+#pragma unroll
+                for (int x = 0; x < E / 2; x++) f[k][x] = ok ? *(const float2*)(pk + 2 * lane + 64 * x) : make_float2(0.f, 0.f);
+                if (!ok) cw[k] = 0.f;
+            }
+#pragma unroll
+            for (int k = 0; k < B; k++)
+#pragma unroll
+                for (int x = 0; x < E / 2; x++) { acc[x].x = fmaf(cw[k], f[k][x].x, acc[x].x); acc[x].y = fmaf(cw[k], f[k][x].y, acc[x].y); }
+        }
     }
     L = sz_warp_sum(L);
-    if ((tid & 31) == 0) redl[tid >> 5] = L;
-    __syncthreads();
-    L = 0.f;
+    if (W > 1) {
 #pragma unroll
-    for (int w = 0; w < PG_MERGE / 32; w++) L += redl[w];
-    constexpr int TG = HD / 4, GN = PG_MERGE / TG;
-    const int grp = tid / TG, col = tid % TG;
-    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-    for (int i = grp; i < n; i += GN) {
-        const float4 x = *(const float4*)(from[i] + 4 * col);
-        const float c = wgt[i];
-        acc.x = fmaf(c, x.x, acc.x); acc.y = fmaf(c, x.y, acc.y); acc.z = fmaf(c, x.z, acc.z); acc.w = fmaf(c, x.w, acc.w);
+        for (int x = 0; x < E / 2; x++) sums[sub][lane + 32 * x] = acc[x];
+        if (lane == 0) of_warp[sub] = make_float2(M, L);
+        __syncthreads();
+        if (sub) return;
+        float Mw[W], top = M;
+#pragma unroll
+        for (int k = 0; k < W; k++) { Mw[k] = of_warp[k].x; top = fmaxf(top, Mw[k]); }
+        L = 0.f;
+#pragma unroll
+        for (int x = 0; x < E / 2; x++) acc[x] = make_float2(0.f, 0.f);
+#pragma unroll
+        for (int k = 0; k < W; k++) {
+            const float c = Mw[k] == -INFINITY ? 0.f : pg_ex2(Mw[k] - top);
+            L = fmaf(of_warp[k].y, c, L);
+#pragma unroll
+            for (int x = 0; x < E / 2; x++) { const float2 f = sums[k][lane + 32 * x]; acc[x].x = fmaf(f.x, c, acc[x].x); acc[x].y = fmaf(f.y, c, acc[x].y); }
+        }
+        M = top;
     }
-    sums[tid] = acc;
-    __syncthreads();
-    if (grp) return;
-#pragma unroll
-    for (int k = 1; k < GN; k++) { const float4 x = sums[k * TG + col]; acc.x += x.x; acc.y += x.y; acc.z += x.z; acc.w += x.w; }
-    const bool none = n == 0 || L == 0.f;                             // nothing the row may see
+    const bool none = n == 0 || L == 0.f;                            // nothing the row may see
     const float inv = none ? 0.f : 1.f / L;
-    float y[4] = {acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv};
-    if (none) y[0] = y[1] = y[2] = y[3] = 0.f;
-    if (io.gate) {
-        const u8* gp = io.gate + (long long)r * io.gate_stride + (long long)h * io.gate_head_stride + 4 * col * io.esz;
-        const float2 g0 = pg_load2(gp, io.type), g1 = pg_load2(gp + 2 * io.esz, io.type);
-        y[0] *= sz_sigmoid(g0.x); y[1] *= sz_sigmoid(g0.y); y[2] *= sz_sigmoid(g1.x); y[3] *= sz_sigmoid(g1.y);
-        if (none) y[0] = y[1] = y[2] = y[3] = 0.f;
+    u8* const op = io.out + (long long)r * io.out_stride + (long long)h * HD * io.esz;
+    const u8* const gp = io.gate ? io.gate + (long long)r * io.gate_stride + (long long)h * io.gate_head_stride : nullptr;
+#pragma unroll
+    for (int x = 0; x < E / 2; x++) {
+        const int at = (2 * lane + 64 * x) * io.esz;
+        float u = none ? 0.f : acc[x].x * inv, v = none ? 0.f : acc[x].y * inv;
+        if (gp) { const float2 g = pg_load2(gp + at, io.type); u *= sz_sigmoid(g.x); v *= sz_sigmoid(g.y); }
+        pg_store2(op + at, io.type, u, v);
     }
-    pg_store2(op + 4 * col * io.esz, io.type, y[0], y[1]);
-    pg_store2(op + (4 * col + 2) * io.esz, io.type, y[2], y[3]);
-    if (io.lse && tid == 0) io.lse[(size_t)r * nh + h] = none ? -INFINITY : (M + log2f(L)) * 0.6931471805599453f;
+    if (io.lse && lane == 0) io.lse[(size_t)r * nh + h] = none ? -INFINITY : (M + log2f(L)) * 0.6931471805599453f;
 }
 
 // ---- the host side -------------------------------------------------------------------------------------------------------------------------------
@@ -304,26 +328,48 @@ PgScratch pg_scratch(const sz_paged_cache* c, const sz_paged_batch* b, int nh, u
     int64_t off = 256;
     const int hd = c->head_dim, G = nh / c->n_kv_head;
     auto take = [&](int64_t n) { const int64_t at = off; off += (n + 255) & ~(int64_t)255; return base + at; };
-    for (int i = 0; i < 4; i++) {
-        PgPart* p = &s.a.p[i];
-        const bool tc = i == PG_SHARED_TC || i == PG_OWN_TC;
-        if (tc && (!pg_tc_type(c->type) || (int64_t)G * b->rows < PG_TC_MIN)) continue;      // (fewer rows never need more)
-        const int64_t slots = 2ll * PG_BLOCKS * (tc ? pg_tc_tile(hd) : 64);      // vectors of the blocks' parts (blocks a multiprocessor x vectors a tile is 64 at most)
+    for (PgPart* p = s.a.p; p < s.a.p + 2; p++) {
+        const int64_t slots = 2ll * PG_BLOCKS * 256;      // parts of the blocks, by vector: blocks a multiprocessor x vectors a tile x ways is 256 at most, of the tcgen05 kernel too
         p->tiles = (u32*)take(4ll * (b->n_seq + 1));
         p->units = (u32*)take(4ll * ((int64_t)b->rows * G / 16 + b->n_seq + 2));
         p->o = (float*)take(slots * hd * 4);
         p->ml = (float2*)take(slots * 8);
-        p->row_o = (float*)take((int64_t)b->rows * nh * hd * 4);
-        p->row_ml = (float2*)take((int64_t)b->rows * nh * 8);
+        p->row_o = (float*)take((int64_t)b->rows * nh * 4 * hd * 4);      // (4 ways at most)
+        p->row_ml = (float2*)take((int64_t)b->rows * nh * 4 * 8);
     }
     s.bytes = off;
     return s;
 }
 
-int pg_launch_attend(const PgKernels& k, const PgBatch& d, const PgIo& io, const PgPart& p, const char* name, cudaStream_t st) {
+typedef CUresult (*PgEncodeTiled)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*, const cuuint32_t*,
+                                  CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+PgEncodeTiled pg_encoder() {
+    static const PgEncodeTiled fn = [] {
+        void* p = nullptr;
+        cudaDriverEntryPointQueryResult q = cudaDriverEntryPointSymbolNotFound;
+        return cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) == cudaSuccess && q == cudaDriverEntryPointSuccess ? (PgEncodeTiled)p : (PgEncodeTiled)nullptr;
+    }();
+    return fn;
+}
+// A pool as [page][key head][position][dimension] 16-bit words; a box is `rows` positions of a page and 64 dimensions (128 bytes, swizzled), or
+// of whole packed heads.  Its x starts at a multiple of 128 bytes; its outer coordinates may lie outside (a page that is not there: zeros).
+int pg_map(const sz_paged_cache* c, int values, int rows, CUtensorMap* map) {
+    PgEncodeTiled enc = pg_encoder();
+    if (!enc) return sz_fail(SZ_E_CUDA, "sz_paged_attend: the driver has no cuTensorMapEncodeTiled");
+    const bool q8 = c->type == SZ_TYPE_Q8_KV;
+    const cuuint64_t words = (cuuint64_t)pg_head_bytes(c->type, c->head_dim) / 2;
+    const cuuint64_t dim[4] = {words, (cuuint64_t)c->page_size, (cuuint64_t)c->n_kv_head, (cuuint64_t)c->n_pages};
+    const cuuint64_t stride[3] = {(cuuint64_t)c->pos_stride, (cuuint64_t)c->head_stride, (cuuint64_t)c->page_stride};
+    const cuuint32_t box[4] = {q8 ? (cuuint32_t)words : 64u, (cuuint32_t)rows, 1, 1}, es[4] = {1, 1, 1, 1};
+    const CUresult r = enc(map, CU_TENSOR_MAP_DATA_TYPE_UINT16, 4, (void*)(values ? c->v : c->k), dim, stride, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                           q8 ? CU_TENSOR_MAP_SWIZZLE_NONE : CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    return r == CUDA_SUCCESS ? SZ_OK : sz_fail(SZ_E_CUDA, "sz_paged_attend: cuTensorMapEncodeTiled failed (%d)", (int)r);
+}
+
+int pg_launch_attend(const PgKernels& k, const CUtensorMap* maps, int rows_box, const PgBatch& d, const PgIo& io, const PgPart& p, const char* name, cudaStream_t st) {
     const int rc = sz_allow_smem(k.fn, k.smem);
     if (rc) return rc;
-    SZ_CUDA(sz_launch(name, (void (*)(PgBatch, PgIo, PgPart))k.fn, dim3(p.blocks), dim3(k.threads), k.smem, st, true, d, io, p));
+    SZ_CUDA(sz_launch(name, (void (*)(CUtensorMap, CUtensorMap, PgBatch, PgIo, PgPart, int))k.fn, dim3(p.blocks), dim3(k.threads), k.smem, st, true, maps[0], maps[1], d, io, p, rows_box));
     return SZ_OK;
 }
 
@@ -395,7 +441,7 @@ extern "C" int sz_paged_attend(const sz_paged_cache* cache, const sz_paged_batch
     PgScratch s = pg_scratch(cache, batch, n_head, scratch);
     if (!scratch || (scratch & 255) || scratch_bytes < s.bytes) return sz_fail(SZ_E_SCRATCH, "%s: %lld bytes of scratch given, %lld needed, 256-byte aligned", who, (long long)scratch_bytes, (long long)s.bytes);
     cudaStream_t st = (cudaStream_t)stream;
-    PgBatch d = pg_batch(cache, batch, n_head, scratch);
+    const PgBatch d = pg_batch(cache, batch, n_head, scratch);
     PgIo io = {};
     io.q = (const u8*)q; io.q_stride = q_stride * esz; io.gate = (const u8*)gate; io.gate_stride = gate_stride * esz; io.gate_head_stride = gate_head_stride * esz;
     io.out = (u8*)out; io.out_stride = out_stride * esz; io.lse = (float*)lse; io.type = io_type; io.esz = esz; io.scale_log2 = scale * 1.4426950408889634f;
@@ -403,30 +449,38 @@ extern "C" int sz_paged_attend(const sz_paged_cache* cache, const sz_paged_batch
     const bool wide = io_type == SZ_TYPE_F32 || (io_type == SZ_TYPE_F16 && ct != PG_F16);
     auto kernels = [&](int nqt) { return ct == PG_F16 ? pg_kernels_f16(wide, hd, nqt) : ct == PG_BF16 ? pg_kernels_bf16(wide, hd, nqt) : pg_kernels_q8(wide, hd, nqt); };
     const int64_t per_seq = (int64_t)G * ((batch->rows + batch->n_seq - 1) / batch->n_seq), all = (int64_t)G * batch->rows;
-    const PgKernels ko = kernels(pg_tiles_of(per_seq)), ks = kernels(pg_tiles_of(all));
-    const bool shared = batch->shared_len > 0, tc = pg_tc_type(cache->type) && io_type == cache->type && scale > 0.f;
-    const int tile = pg_tc_tile(hd);
-    auto on = [&](int i, int is_shared, int is_tc, int tq, int blocks) {
-        PgPart& p = s.a.p[i];
-        p.on = 1; p.shared = is_shared; p.tc = is_tc; p.tq = tq; p.blocks = blocks;
-        p.planned = (is_shared ? 0 : batch->n_seq) + (all + tq - 1) / tq > PG_PLAN;
-    };
-    if (tc && shared && all >= PG_TC_MIN && batch->shared_len >= PG_TC) { d.bulk_shared = tile; on(PG_SHARED_TC, 1, 1, tile, PG_BLOCKS); }
-    if (tc && per_seq >= PG_TC_MIN) { d.bulk_own = tile; on(PG_OWN_TC, 0, 1, tile, PG_BLOCKS); }
-    if (shared && !(d.bulk_shared && batch->shared_len % PG_TC == 0)) on(PG_SHARED, 1, 0, ks.tq, PG_BLOCKS * ks.occ);
-    on(PG_OWN, 0, 0, ko.tq, PG_BLOCKS * ko.occ);
-    s.a.p[PG_OWN].direct = !shared && !d.bulk_own;
+    const bool tc = pg_tc_type(cache->type) && io_type == cache->type && scale > 0.f;
+    const bool tc_of[2] = {tc && all >= PG_TC_MIN, tc && per_seq >= PG_TC_MIN};
+    PgKernels kern[2];
+    CUtensorMap maps[2][2];              // [of 16 positions, of 128][keys, values]
+    const int box[2] = {cache->page_size < 16 ? cache->page_size : 16, cache->page_size < PG_TC ? cache->page_size : PG_TC};
     bool planned = false;
-    for (const PgPart& p : s.a.p) planned |= p.planned;
-    if (planned) SZ_CUDA(sz_launch("paged_plan", sz_pg_plan_kernel, dim3(4), dim3(1024), 0, st, true, d, s.a));
-    for (int i = 0; i < 4; i++) {
+    for (int i = 0; i < 2; i++) {
+        PgPart& p = s.a.p[i];
+        p.on = i == PG_OWN || batch->shared_len > 0;
+        p.shared = i == PG_SHARED;
+        if (!p.on) continue;
+        kern[i] = kernels(pg_tiles_of(i == PG_SHARED ? all : per_seq));
+        p.unit = tc_of[i] ? PG_TC : PG_T;
+        p.ways = tc_of[i] ? 1 : kern[i].ways;
+        p.tq = tc_of[i] ? pg_tc_tile(hd) : kern[i].tq;
+        p.blocks = tc_of[i] ? PG_BLOCKS : PG_BLOCKS * kern[i].occ;
+        p.planned = (p.shared ? 0 : batch->n_seq) + (all + p.tq - 1) / p.tq > PG_PLAN;
+        planned |= p.planned;
+        for (int x = 0; x < 2; x++) if ((rc = pg_map(cache, x, box[tc_of[i]], &maps[tc_of[i]][x]))) return rc;
+    }
+    s.a.p[PG_OWN].direct = tc_of[PG_OWN] && batch->shared_len == 0;
+    if (planned) SZ_CUDA(sz_launch("paged_plan", sz_pg_plan_kernel, dim3(2), dim3(1024), 0, st, true, d, s.a));
+    for (int i = 0; i < 2; i++) {
         const PgPart& p = s.a.p[i];
         if (!p.on) continue;
-        static const char* const names[4] = {"paged_attend_shared_tc", "paged_attend_shared", "paged_attend_tc", "paged_attend"};
-        rc = p.tc ? pg_tc_launch(cache->type == SZ_TYPE_BF16, hd, cache->page_size, d, io, p, names[i], st) : pg_launch_attend(p.shared ? ks : ko, d, io, p, names[i], st);
+        const char* name = p.shared ? "paged_attend_shared" : "paged_attend";
+        rc = tc_of[i] ? pg_tc_launch(cache->type == SZ_TYPE_BF16, hd, maps[1], box[1], d, io, p, name, st) : pg_launch_attend(kern[i], maps[0], box[0], d, io, p, name, st);
         if (rc) return rc;
     }
-    auto* merge = hd == 64 ? sz_pg_merge_kernel<64> : hd == 128 ? sz_pg_merge_kernel<128> : sz_pg_merge_kernel<256>;
-    SZ_CUDA(sz_launch("paged_merge", merge, dim3(batch->rows, n_head), dim3(PG_MERGE), 0, st, true, d, io, s.a));
+    const bool few = (int64_t)batch->rows * n_head <= 8 * PG_BLOCKS;
+    auto* merge = hd == 64 ? (few ? sz_pg_merge_kernel<64, 8> : sz_pg_merge_kernel<64, 1>) : hd == 128 ? (few ? sz_pg_merge_kernel<128, 8> : sz_pg_merge_kernel<128, 1>)
+                                                                                            : (few ? sz_pg_merge_kernel<256, 8> : sz_pg_merge_kernel<256, 1>);
+    SZ_CUDA(sz_launch("paged_merge", merge, dim3(batch->rows, few ? n_head : (n_head + 7) / 8), dim3(256), 0, st, true, d, io, s.a));
     return SZ_OK;
 }

@@ -2,8 +2,7 @@
 // was fed before a prompt's chunk.  (Few vectors a key head leave the kernel of sz_paged.cuh waiting for memory, not for its mma.sync; with
 // hundreds the products are the work: 4 head_dim operations a vector and position on 4 head_dim bytes.)
 //
-// It takes whole units of 128 positions that EVERY row of a tile sees, so it needs no masks; what is left - a tile's last positions, up to
-// each row's own - is the other kernel's, and the merge joins the parts.  Types: 16-bit queries over a cache of the same type.
+// Types: 16-bit queries over a cache of the same type.
 //
 // A block has NQ x 128 query vectors of one key head (two tiles of 128 up to head_dim 128, one above) and the lines of tensor memory:
 //     columns   0 .. 255   scores, two buffers of 128 (f32); the weights lie over the buffer they come from, as pairs of 16 bits
@@ -20,7 +19,10 @@
 // Rounding: a weight has 8 (bf16) or 11 bits, as the result; its sum is of the unrounded ones.  (Errors of independent weights average out:
 // the result's error stays below 1.3 of its last rounding's.)
 // A page out of range arrives as zeros (its box lies outside the pool's map) and its positions are masked.  Every wait is bounded.
-#include <cuda.h>
+//
+// What a row does not see must not reach it, whatever it is: scores of such positions are replaced, but a weight of 0 times a value that is infinite
+// or NaN would be NaN.  So in a unit that not all rows of a tile see whole, the first tile's threads clear the values behind the sequence's end and
+// those that are not finite, before the product; should there be any of the latter, the rows that see them add them at the end.
 #include "sz_paged.cuh"
 
 namespace {
@@ -80,8 +82,10 @@ struct PtCfg {
 struct PtBars {
     u64 full[8], empty[8], s_full[2], p_full[2], pv_done[2], q_full[2], o_free[2];
     u32 tmem, failed;
+    u32 odd[2];                      // of every other piece: its number + 1, once a value that is not finite was cleared
     u32 ok[8][4];                    // which positions of a unit are there, of eight units: the eighth next one's keys are asked for after this one's weights were used
     u32 tiles[PG_PLAN + 1], units[PG_PLAN + 1], scan[16];
+    int rows[PG_PLAN + 1], ends[PG_PLAN + 1];
 };
 
 template <bool BF, int HD>
@@ -101,6 +105,7 @@ sz_pg_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
         for (int i = 0; i < 8; i++) { sz_mbar_init(&S.full[i], 1); sz_mbar_init(&S.empty[i], 1); }
         for (int i = 0; i < 2; i++) { sz_mbar_init(&S.s_full[i], 1); sz_mbar_init(&S.p_full[i], 4); sz_mbar_init(&S.pv_done[i], 1); sz_mbar_init(&S.q_full[i], 4); sz_mbar_init(&S.o_free[i], 4); }
         S.failed = 0;
+        S.odd[0] = S.odd[1] = 0;
         sz_mbar_fence_init();
     }
     if (warp == 0) {
@@ -112,41 +117,47 @@ sz_pg_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
     pt_after();
     const u32 tmem = S.tmem;
     sz_pdl_wait();
-    sz_pdl_trigger();
     const u32 *tiles = S.tiles, *units = S.units;
     int E;
     if (pt.planned) {
         tiles = pt.tiles; units = pt.units;
         E = pt.shared ? max(0, ((pg_row(d, d.n_seq) - pg_row(d, 0)) * d.G + C::TQ - 1) / C::TQ) : (int)tiles[d.n_seq];
     } else {
-        E = pg_plan<C::NTH>(d, pt.shared, 1, C::TQ, S.tiles, S.units, S.scan);
+        E = pg_plan<C::NTH>(d, pt.shared, PG_TC, C::TQ, S.tiles, S.units, S.scan, S.rows, S.ends);
         if (blockIdx.x == 0) {
             if (!pt.shared) for (int i = tid; i <= d.n_seq; i += C::NTH) pt.tiles[i] = S.tiles[i];
             for (int i = tid; i <= E; i += C::NTH) pt.units[i] = S.units[i];
         }
     }
-    const long long U = (long long)units[E] * d.nkv;
-    const int blocks = (int)min((long long)pt.blocks, U);
+    if (blockIdx.x == 0 && !pt.shared) {                   // what the lengths ask for that is not there
+        for (int b = tid; b < d.n_seq; b += C::NTH)
+            if (pg_row(d, b + 1) > pg_row(d, b) && (long long)__ldg(d.lens + b) - d.shared_len > ((long long)d.max_pages << d.ps_log2)) atomicOr(d.err, PG_E_END);
+        if (tid == 0 && __ldg(d.row_start + d.n_seq) > d.rows) atomicOr(d.err, PG_E_ROWS);
+    }
+    const u32 U = units[E] * (u32)d.nkv;
+    const int blocks = (int)min((u32)pt.blocks, U);
     const bool work = (int)blockIdx.x < blocks;
-    const long long u0 = work ? U * blockIdx.x / blocks : 0, u1 = work ? U * (blockIdx.x + 1) / blocks : 0;
+    const PgShare share = work ? pg_share(U, blocks) : PgShare{1u, 0u};
+    const u32 u0 = work ? pg_first(share, blockIdx.x) : 0, u1 = work ? pg_first(share, blockIdx.x + 1) : 0;
+    auto row_of = [&](int b) { return pt.planned ? pg_row(d, b) : S.rows[b]; };
+    auto end_of = [&](int b) { return (long long)(pt.planned ? __ldg(d.lens + b) - d.shared_len : S.ends[b]); };
     // the next piece of the block's share: an item, units i .. i + T of it
-    auto locate = [&](long long u) {
+    auto locate = [&](u32 u) {
         PgItem it;
-        const u32 un = (u32)(u / d.nkv);
+        const u32 un = u / (u32)d.nkv;
         int lo = 0, hi = E - 1;
         while (lo < hi) { const int mid = (lo + hi + 1) >> 1; if (units[mid] <= un) lo = mid; else hi = mid - 1; }
         it.e = lo;
         it.n = (int)(units[lo + 1] - units[lo]);
-        const u32 rem = (u32)(u - (long long)units[lo] * d.nkv);
+        const u32 rem = u - units[lo] * (u32)d.nkv;
         it.h = (int)(rem / (u32)it.n);
-        it.i = (int)(rem % (u32)it.n);
-        it.begin = 0; it.end = it.n * PG_TC;
-        it.b = 0; it.t = lo;
-        if (pt.shared) return it;
+        it.i = (int)(rem - (u32)it.h * (u32)it.n);
+        if (pt.shared) { it.b = 0; it.t = lo; it.end = d.shared_len; return it; }
         int bl = 0, bh = d.n_seq - 1;
         while (bl < bh) { const int mid = (bl + bh + 1) >> 1; if (tiles[mid] <= (u32)lo) bl = mid; else bh = mid - 1; }
         it.b = bl;
         it.t = lo - (int)tiles[bl];
+        it.end = pg_tile_end(d, row_of(bl + 1) - row_of(bl), end_of(bl), it.t, C::TQ);
         return it;
     };
     // Where keys (kind 0) and values (1) of unit j come in a piece's order of loads, in slots; T units
@@ -159,9 +170,9 @@ sz_pg_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
         // ---- loads
         const int pieces = PG_TC / rows_box;
         u32 seq = 0, units_in = 0;                         // slots filled, units' keys asked for so far
-        for (long long u = u0; u < u1 && !failed;) {
+        for (u32 u = u0; u < u1 && !failed;) {
             const PgItem it = locate(u);
-            const int T = (int)min((long long)(it.n - it.i), u1 - u);
+            const int T = (int)min((u32)(it.n - it.i), u1 - u);
             const int32_t* table = pt.shared ? d.shared_pages : d.pages + (size_t)it.b * d.max_pages;
             for (int x = 0; x < 2 * T && !failed; x++) {
                 int kind, j;
@@ -171,9 +182,10 @@ sz_pg_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
                 else { kind = (x & 1) ^ 1; j = kind ? x / 2 - 1 : (x + 1) / 2; }
                 const int c = (it.i + j) * PG_TC + lane * rows_box;
                 int page = -1;
-                if (lane < pieces) page = __ldg(table + (c >> d.ps_log2));
-                const bool ok = (u32)page < (u32)d.n_pages;
-                if (lane < pieces && !ok) atomicOr(d.err, PG_E_PAGE);
+                const bool there = lane < pieces && c < it.end;
+                if (there) page = __ldg(table + (c >> d.ps_log2));
+                const bool ok = there && (u32)page < (u32)d.n_pages;
+                if (there && !ok) atomicOr(d.err, PG_E_PAGE);
                 for (int nb = 0; nb < C::NB; nb++, seq++) {
                     const int sl = (int)(seq % C::SLOTS);
                     if (seq >= C::SLOTS && !pt_wait_warp(&S.empty[sl], seq / C::SLOTS - 1)) { failed = 1; break; }
@@ -210,9 +222,9 @@ sz_pg_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
             const u64 qd = pt_desc(sz_smem_addr(sq), 16, 1024), kd = pt_desc(sz_smem_addr(ring), 16, 1024), vd = pt_desc(sz_smem_addr(ring), C::BLK, 1024);
             u32 seq0 = 0, piece = 0, used[2] = {0, 0};     // slots before this piece; pieces; weights taken of a buffer
             u32 buf0 = 0;                                  // the buffer of the piece's unit 0
-            for (long long u = u0; u < u1 && !failed; piece++) {
+            for (u32 u = u0; u < u1 && !failed; piece++) {
                 const PgItem it = locate(u);
-                const int T = (int)min((long long)(it.n - it.i), u1 - u), N = T * C::NQ;
+                const int T = (int)min((u32)(it.n - it.i), u1 - u), N = T * C::NQ;
                 for (int q = 0; q < C::NQ && !failed; q++) if (!pt_wait(&S.q_full[q], piece)) failed = 2;
                 auto scores = [&](int x) {
                     const int q = x % C::NQ, j = x / C::NQ, buf = (int)((buf0 + x) & 1);
@@ -260,12 +272,17 @@ sz_pg_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
         // ---- softmax: thread = query vector
         const int q = warp / 4, row = tid & 127;
         const u32 lanes = (u32)((warp & 3) * 32) << 16;
-        u32 piece = 0, taken[2] = {0, 0}, done = 0, buf0 = 0;      // taken: scores of a buffer; done: units of this tile
-        for (long long u = u0; u < u1 && !failed; piece++) {
+        u32 piece = 0, taken[2] = {0, 0}, done = 0, seq0 = 0, buf0 = 0;      // taken: scores of a buffer; done: units of this tile; seq0: ring slots before the piece
+        for (u32 u = u0; u < u1 && !failed; piece++) {
             const PgItem it = locate(u);
-            const int T = (int)min((long long)(it.n - it.i), u1 - u);
-            const int r0 = pg_row(d, it.b), m = (pt.shared ? pg_row(d, d.n_seq) : pg_row(d, it.b + 1)) - r0;
+            const int T = (int)min((u32)(it.n - it.i), u1 - u);
+            const int r0 = row_of(it.b), m = (pt.shared ? row_of(d.n_seq) : row_of(it.b + 1)) - r0;
             const int v = q * 128 + row, vec = it.t * C::TQ + v, qr = vec / d.G, head = it.h * d.G + vec % d.G;
+            // positions this vector sees, and those that all of the tile's do
+            const long long oend = end_of(it.b);
+            const int room = pg_room(d);
+            const int lim = qr >= m ? 0 : pt.shared ? d.shared_len : (int)max(0ll, min(oend - (m - 1 - qr), (long long)room));
+            const int all = pt.shared ? d.shared_len : (int)max(0ll, min(oend - (m - 1 - it.t * C::TQ / d.G), (long long)room));
             {   // the query vector into the K-major order: chunk c of 8 dimensions of row r at chunk c ^ (r & 7) of its 128 bytes
                 const uint4* src = (const uint4*)(io.q + (long long)(r0 + qr) * io.q_stride + (long long)head * HD * 2);
                 u8* dst = sq + q * C::QT + row * 128;
@@ -292,6 +309,12 @@ sz_pg_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
                 if ((ok[0] & ok[1] & ok[2] & ok[3]) != 0xffffffffu) {
 #pragma unroll
                     for (int k = 0; k < 128; k++) s[k] = (ok[k / 32] >> (k & 31)) & 1u ? s[k] : -INFINITY;
+                }
+                const int at_pos = (it.i + j) * PG_TC;
+                if (lim < at_pos + PG_TC) {
+                    const int seen = lim - at_pos;
+#pragma unroll
+                    for (int k = 0; k < 128; k++) s[k] = k < seen ? s[k] : -INFINITY;
                 }
                 float big[4] = {s[0], s[1], s[2], s[3]};
 #pragma unroll
@@ -330,6 +353,33 @@ sz_pg_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
                     pt_st16(at + k / 2, w);
                 }
                 l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+                if (q == 0 && all < at_pos + PG_TC) {      // the values that some row does not see
+                    const u32 at_v = seq0 + place(1, j, T);
+                    for (int nb = 0; nb < C::NB && !failed; nb++) {
+                        const int sl = (int)((at_v + nb) % C::SLOTS);
+                        if (!pt_wait_warp(&S.full[sl], (at_v + nb) / C::SLOTS)) { failed = 10; break; }
+#pragma unroll 4
+                        for (int x = tid; x < C::SLOT / 16; x += 128) {      // (a slot is blocks of 128 rows of 128 bytes)
+                            uint4* const at16 = (uint4*)(ring + (size_t)sl * C::SLOT) + x;
+                            const uint4 w = *at16;
+                            const u32 in[4] = {w.x, w.y, w.z, w.w};
+                            u32 out[4];
+                            const bool behind = at_pos + (x >> 3) % PG_TC >= it.end;
+                            bool odd = false;
+#pragma unroll
+                            for (int k = 0; k < 4; k++) {
+                                constexpr u32 X = BF ? 0x7f80u : 0x7c00u;
+                                const u32 lo = (in[k] & X) == X ? 0u : 0xffffu, hi = (in[k] & (X << 16)) == (X << 16) ? 0u : 0xffff0000u;
+                                odd |= (lo & hi >> 16) != 0xffffu;
+                                out[k] = behind ? 0u : in[k] & (lo | hi);
+                            }
+                            if (behind || odd) *at16 = make_uint4(out[0], out[1], out[2], out[3]);
+                            if (odd && !behind) S.odd[piece & 1] = piece + 1;
+                        }
+                    }
+                    if (failed) break;
+                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                }
                 pt_stored();
                 pt_before();
                 pt_arrive_warp(&S.p_full[buf]);
@@ -339,27 +389,64 @@ sz_pg_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
             if (!failed && !pt_wait_warp(&S.pv_done[q], done - 1)) failed = 9;
             if (failed) break;
             pt_after();
-            const long long us = (long long)units[it.e] * d.nkv + (long long)it.h * it.n;
-            const int b0 = pg_block_of(us, U, blocks), b1 = pg_block_of(us + it.n - 1, U, blocks);
-            const size_t to = b0 == b1 ? (size_t)(r0 + qr) * (d.nkv * d.G) + head : (size_t)(2 * blockIdx.x + ((int)blockIdx.x == b0 ? 1 : 0)) * C::TQ + v;
-            float* w = (b0 == b1 ? pt.row_o : pt.o) + to * HD;
+            const u32 us = units[it.e] * (u32)d.nkv + (u32)it.h * (u32)it.n;
+            const int b0 = pg_block_of(share, us), b1 = pg_block_of(share, us + it.n - 1);
+            const bool alone = b0 == b1, direct = alone && pt.direct, odd = S.odd[piece & 1] == piece + 1;
+            const size_t to = alone ? (size_t)(r0 + qr) * (d.nkv * d.G) + head : (size_t)(2 * blockIdx.x + ((int)blockIdx.x == b0 ? 1 : 0)) * C::TQ + v;
+            float* const w = (alone ? pt.row_o : pt.o) + to * HD;
+            u8* const op = io.out + (long long)(r0 + qr) * io.out_stride + (long long)head * HD * 2;
+            const u8* const gp = io.gate ? io.gate + (long long)(r0 + qr) * io.gate_stride + (long long)head * io.gate_head_stride : nullptr;
+            const bool none = lim <= 0 || l == 0.f;
+            const float inv = none ? 0.f : 1.f / l;
 #pragma unroll 1
             for (int k = 0; k < HD; k += 32) {
                 float o[32];
                 pt_ld32(tmem + lanes + 256 + q * HD + k, o);
                 pt_loaded(o);
-                if (qr < m) {
+                if (qr >= m) continue;
+                if (odd) {                                 // the values that were cleared, where this row sees them
+                    const int32_t* table = pt.shared ? d.shared_pages : d.pages + (size_t)it.b * d.max_pages;
+                    for (int t = max(it.i * PG_TC, all & ~(PG_TC - 1)); t < min(lim, (it.i + T) * PG_TC); t++) {
+                        const int page = __ldg(table + (t >> d.ps_log2));
+                        if ((u32)page >= (u32)d.n_pages) continue;
+                        const u8* src = d.v + (long long)page * d.page_stride + (long long)(t & ((1 << d.ps_log2) - 1)) * d.pos_stride + (long long)it.h * d.head_stride + 2 * k;
+#pragma unroll
+                        for (int e = 0; e < 32; e += 2) {
+                            const float2 f = pg_unpack<CT>(*(const u32*)(src + 2 * e));
+                            if (!isfinite(f.x)) o[e] += f.x;
+                            if (!isfinite(f.y)) o[e + 1] += f.y;
+                        }
+                    }
+                }
+                if (!direct) {
 #pragma unroll
                     for (int e = 0; e < 32; e += 4) *(float4*)(w + k + e) = make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+                    continue;
+                }
+#pragma unroll
+                for (int e = 0; e < 32; e += 8) {
+                    u32 y[4], z[4] = {};
+                    if (gp) { const uint4 g = __ldg((const uint4*)(gp + 2 * (k + e))); z[0] = g.x; z[1] = g.y; z[2] = g.z; z[3] = g.w; }
+#pragma unroll
+                    for (int x = 0; x < 4; x++) {
+                        float a = none ? 0.f : o[e + 2 * x] * inv, b = none ? 0.f : o[e + 2 * x + 1] * inv;
+                        if (gp) { const float2 g = pg_unpack<CT>(z[x]); a *= sz_sigmoid(g.x); b *= sz_sigmoid(g.y); }
+                        y[x] = pg_pack<CT>(a, b);
+                    }
+                    *(uint4*)(op + 2 * (k + e)) = make_uint4(y[0], y[1], y[2], y[3]);
                 }
             }
-            if (qr < m) (b0 == b1 ? pt.row_ml : pt.ml)[to] = make_float2(mx, l);
+            if (l != l && mx == -INFINITY) mx = 0.f;       // (scores that are all NaN have no maximum, and are not an empty part)
+            if (qr < m && !direct) (alone ? pt.row_ml : pt.ml)[to] = make_float2(mx, l);
+            if (qr < m && direct && io.lse) io.lse[to] = none ? -INFINITY : (mx + log2f(l)) * 0.6931471805599453f;
             pt_before();
             pt_arrive_warp(&S.o_free[q]);
+            seq0 += 2 * T * C::NB;
             buf0 = (buf0 + T * C::NQ) & 1;
             u += T;
         }
     }
+    sz_pdl_trigger();
     if (failed) atomicMax(&S.failed, (u32)failed);
     pt_before();
     __syncthreads();
@@ -370,36 +457,12 @@ sz_pg_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
     if (tid == 0 && S.failed) atomicOr(d.err, PG_E_WAIT);
 }
 
-typedef CUresult (*PtEncodeTiled)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*, const cuuint32_t*,
-                                  CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-PtEncodeTiled pt_encoder() {
-    static PtEncodeTiled fn = nullptr;
-    if (!fn) {
-        void* p = nullptr;
-        cudaDriverEntryPointQueryResult q = cudaDriverEntryPointSymbolNotFound;
-        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) == cudaSuccess && q == cudaDriverEntryPointSuccess) fn = (PtEncodeTiled)p;
-    }
-    return fn;
-}
-
 template <bool BF, int HD>
-int pt_launch(int page_size, const PgBatch& d, const PgIo& io, const PgPart& p, const char* name, cudaStream_t st) {
+int pt_launch(const CUtensorMap* maps, int rows_box, const PgBatch& d, const PgIo& io, const PgPart& p, const char* name, cudaStream_t st) {
     using C = PtCfg<HD>;
-    int rc = sz_allow_smem((const void*)sz_pg_tc_kernel<BF, HD>, C::SMEM);
+    const int rc = sz_allow_smem((const void*)sz_pg_tc_kernel<BF, HD>, C::SMEM);
     if (rc) return rc;
-    PtEncodeTiled enc = pt_encoder();
-    if (!enc) return sz_fail(SZ_E_CUDA, "sz_paged_attend: the driver has no cuTensorMapEncodeTiled");
-    const int box_rows = page_size < PG_TC ? page_size : PG_TC;
-    CUtensorMap map[2];
-    for (int i = 0; i < 2; i++) {       // a pool as [page][key head][position][dimension]; x is 0 or 64 dimensions on: multiples of 16 bytes
-        const cuuint64_t dim[4] = {(cuuint64_t)HD, (cuuint64_t)page_size, (cuuint64_t)d.nkv, (cuuint64_t)d.n_pages};
-        const cuuint64_t stride[3] = {(cuuint64_t)d.pos_stride, (cuuint64_t)d.head_stride, (cuuint64_t)d.page_stride};
-        const cuuint32_t box[4] = {64, (cuuint32_t)box_rows, 1, 1}, es[4] = {1, 1, 1, 1};
-        const CUresult r = enc(&map[i], BF ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, (void*)(i ? d.v : d.k), dim, stride, box, es,
-                               CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-        if (r != CUDA_SUCCESS) return sz_fail(SZ_E_CUDA, "sz_paged_attend: cuTensorMapEncodeTiled failed (%d)", (int)r);
-    }
-    SZ_CUDA(sz_launch(name, sz_pg_tc_kernel<BF, HD>, dim3(p.blocks), dim3(C::NTH), C::SMEM, st, true, map[0], map[1], d, io, p, box_rows));
+    SZ_CUDA(sz_launch(name, sz_pg_tc_kernel<BF, HD>, dim3(p.blocks), dim3(C::NTH), C::SMEM, st, true, maps[0], maps[1], d, io, p, rows_box));
     return SZ_OK;
 }
 
@@ -407,7 +470,7 @@ int pt_launch(int page_size, const PgBatch& d, const PgIo& io, const PgPart& p, 
 
 int pg_tc_tile(int hd) { return hd <= 128 ? 256 : 128; }
 
-int pg_tc_launch(bool bf16, int hd, int page_size, const PgBatch& d, const PgIo& io, const PgPart& p, const char* name, cudaStream_t st) {
-    if (bf16) return hd == 64 ? pt_launch<true, 64>(page_size, d, io, p, name, st) : hd == 128 ? pt_launch<true, 128>(page_size, d, io, p, name, st) : pt_launch<true, 256>(page_size, d, io, p, name, st);
-    return hd == 64 ? pt_launch<false, 64>(page_size, d, io, p, name, st) : hd == 128 ? pt_launch<false, 128>(page_size, d, io, p, name, st) : pt_launch<false, 256>(page_size, d, io, p, name, st);
+int pg_tc_launch(bool bf16, int hd, const CUtensorMap* maps, int rows_box, const PgBatch& d, const PgIo& io, const PgPart& p, const char* name, cudaStream_t st) {
+    if (bf16) return hd == 64 ? pt_launch<true, 64>(maps, rows_box, d, io, p, name, st) : hd == 128 ? pt_launch<true, 128>(maps, rows_box, d, io, p, name, st) : pt_launch<true, 256>(maps, rows_box, d, io, p, name, st);
+    return hd == 64 ? pt_launch<false, 64>(maps, rows_box, d, io, p, name, st) : hd == 128 ? pt_launch<false, 128>(maps, rows_box, d, io, p, name, st) : pt_launch<false, 256>(maps, rows_box, d, io, p, name, st);
 }

@@ -228,6 +228,25 @@ def test_what_hidden_positions_hold_does_not_matter(cache, bad):
     assert not bool(torch.isfinite(hit).any()) and bool(torch.isfinite(out[3, :, :5]).all())
 
 
+@pytest.mark.parametrize("io,cache,m", [("f32", "f16", 3), ("f32", "q8", 2), ("bf16", "bf16", 3), ("bf16", "bf16", 70)])
+def test_nan_queries_and_keys(io, cache, m):
+    """A row with a NaN in its query, or in a key that it sees, is NaN - and no other row."""
+    c = Case([300, 200], [m, m], nh=4, nkv=2, hd=64, io=io, cache=cache, seed=20, page=16)
+    before = c.check()
+    c.q[1, 2, 5] = math.nan
+    out = c.step.attend(c.q)
+    assert bool(torch.isnan(out[1, 2]).all())
+    keep = torch.ones(c.rows, 4, dtype=torch.bool, device="cuda")
+    keep[1, 2] = False
+    assert torch.equal(out[keep], before[keep])
+    if cache != "q8":
+        c.q[1, 2, 5] = 0
+        page = c.pages[1, (200 - 1) // 16]
+        c.k[page, 1, 199 % 16, 0] = math.nan            # the second sequence's last position: its last row's heads of the second key head
+        out = c.step.attend(c.q)
+        assert bool(torch.isnan(out[-1, 2:]).all()) and bool(torch.isfinite(out[-1, :2]).all()) and bool(torch.isfinite(out[:-1]).all())
+
+
 @pytest.mark.parametrize("io,cache", [("f32", "f16"), ("f32", "q8"), ("bf16", "bf16"), ("f32", "bf16")])
 def test_large_and_small_magnitudes(io, cache):
     for kv, q in ((1e-3, 100.0), (100.0, 0.01), (300.0, 0.003)):
