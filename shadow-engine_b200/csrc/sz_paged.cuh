@@ -18,7 +18,7 @@
 constexpr int PG_T = 64;             // positions a unit
 constexpr int PG_PLAN = 256;         // sequences and tiles that a block plans for itself; above, sz_pg_plan_kernel does once
 constexpr int PG_MAX_SEQ = 4096;
-constexpr int PG_TC = 128;           // positions a unit of the tcgen05 kernel (sz_paged_tc.cu)
+constexpr int PG_TC = 64;            // positions a unit of the tcgen05 kernel (sz_paged_tc.cu)
 enum { PG_F16 = 0, PG_BF16 = 1, PG_Q8 = 2 };
 enum { PG_E_PAGE = 1, PG_E_END = 2, PG_E_SHARED = 4, PG_E_ROWS = 8, PG_E_WAIT = 16 };
 

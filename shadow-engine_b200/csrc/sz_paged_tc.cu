@@ -4,17 +4,18 @@
 //
 // Types: 16-bit queries over a cache of the same type.
 //
-// A block has NQ x 128 query vectors of one key head (two tiles of 128 up to head_dim 128, one above) and the lines of tensor memory:
-//     columns   0 .. 255   scores, two buffers of 128 (f32); the weights lie over the buffer they come from, as pairs of 16 bits
-//     columns 256 .. 511   the tiles' sums, NQ x head_dim
-// Unit u (tile u % NQ, positions u / NQ) has buffer u % 2.  One thread issues, in this order: scores(0), scores(1), then for every u, once
-// its weights are there, sums += weights(u) values, scores(u + 2).  The tensor core works in the order of issue, so scores(u + 2) cannot overwrite
-// weights(u) before they are used; while a tile's softmax runs, the other buffer's products do.
-//   warps 0 .. 3 (and 4 .. 7 for the second tile)   a thread has a query vector, lane = row of tensor memory: it reads its 128 scores
+// A block has NQ x 128 query vectors of one key head (two tiles of 128 up to head_dim 128, one above) and the columns of tensor memory:
+//     0 .. 255    scores, two buffers of 64 positions a tile (f32); the weights lie over the buffer they come from, as pairs of 16 bits
+//     256 .. 511  the tiles' sums, NQ x head_dim
+// One warp issues the scores' products of unit after unit, another the sums', each when its operands are there and the buffer is free: what they do between
+// two units - waits, a commit, descriptors: 500 cycles - is hidden behind the other's instructions, and a tile's softmax goes from unit to
+// unit without waiting for its products.  (One warp for both: 2,860 cycles for two tiles and 64 positions, whose instructions need 1,280.  Units of 128
+// positions with one buffer a tile, where softmax, products and scores take turns: 5,900 for 128.)
+//   warps 0 .. 3 (and 4 .. 7 for the second tile)   a thread has a query vector, lane = row of tensor memory: it reads its 64 scores
 //               (tcgen05.ld), moves its maximum - only when the largest is 2^8 above what it divides by, for then the sums have to be read,
 //               scaled and written back; weights up to 256 cost f32 and the 16-bit types nothing -, writes the weights (tcgen05.st) and keeps their sum.
-//   last two    keys and values by tiled TMA, a box a page (8 .. 128 positions x 64 dimensions, 128-byte swizzle), through a ring of 128 positions x
-//               128 dimensions; the issuing thread.
+//   last four   keys, and values, by tiled TMA, a box a page (8 .. 64 positions x 64 dimensions, 128-byte swizzle), each through a ring of 64 positions x
+//               128 dimensions; the two issuing warps.
 // Operands: queries and keys K-major, values MN-major (their rows are the positions, which the product sums over), weights from tensor memory.
 // Rounding: a weight has 8 (bf16) or 11 bits, as the result; its sum is of the unrounded ones.  (Errors of independent weights average out:
 // the result's error stays below 1.3 of its last rounding's.)
@@ -36,14 +37,23 @@ __device__ __forceinline__ u64 pt_desc(u32 addr, u32 lbo, u32 sbo) {      // 128
 __host__ __device__ constexpr u32 pt_idesc(bool bf16, int n, bool b_mn) {
     return (1u << 4) | ((bf16 ? 1u : 0u) << 7) | ((bf16 ? 1u : 0u) << 10) | ((b_mn ? 1u : 0u) << 16) | ((u32)(n >> 3) << 17) | ((128u >> 4) << 24);
 }
-__device__ __forceinline__ void pt_mma_ss(u32 d, u64 a, u64 b, u32 idesc, u32 acc) {
-    asm volatile("{ .reg .pred p; setp.ne.b32 p, %4, 0; tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p; }" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(acc) : "memory");
+// Issued by one lane (`one`) of a warp that runs as a whole: in code that a single lane has branched into, every operand of every
+// instruction is moved to the uniform registers anew - 110 cycles an instruction, of which the tensor core needs 64.
+__device__ __forceinline__ void pt_mma_ss(u32 d, u64 a, u64 b, u32 idesc, u32 acc, u32 one) {
+    asm volatile("{ .reg .pred p, q; setp.ne.b32 p, %4, 0; setp.ne.b32 q, %5, 0; @q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p; }" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(acc),
+                 "r"(one) : "memory");
 }
-__device__ __forceinline__ void pt_mma_ts(u32 d, u32 a, u64 b, u32 idesc, u32 acc) {      // A from tensor memory
-    asm volatile("{ .reg .pred p; setp.ne.b32 p, %4, 0; tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p; }" ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(acc) : "memory");
+__device__ __forceinline__ void pt_mma_ts(u32 d, u32 a, u64 b, u32 idesc, u32 acc, u32 one) {      // A from tensor memory
+    asm volatile("{ .reg .pred p, q; setp.ne.b32 p, %4, 0; setp.ne.b32 q, %5, 0; @q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p; }" ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(acc),
+                 "r"(one) : "memory");
 }
-__device__ __forceinline__ void pt_commit(u64* bar) {
-    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(sz_smem_addr(bar)) : "memory");
+__device__ __forceinline__ void pt_commit(u64* bar, u32 one) {
+    asm volatile("{ .reg .pred q; setp.ne.b32 q, %1, 0; @q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0]; }" ::"r"(sz_smem_addr(bar)), "r"(one) : "memory");
+}
+__device__ __forceinline__ u32 pt_elect() {
+    u32 x;
+    asm volatile("{ .reg .pred p; elect.sync _|p, 0xffffffff; selp.u32 %0, 1, 0, p; }" : "=r"(x));
+    return x;
 }
 __device__ __forceinline__ void pt_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void pt_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
@@ -71,19 +81,20 @@ __device__ __forceinline__ bool pt_wait(u64* bar, u32 phase) { return sz_mbar_wa
 __device__ __forceinline__ bool pt_wait_warp(u64* bar, u32 phase) { return __all_sync(0xffffffffu, pt_wait(bar, phase)); }
 __device__ __forceinline__ void pt_arrive_warp(u64* bar) { __syncwarp(); if ((threadIdx.x & 31) == 0) sz_mbar_arrive(bar); }
 
+__device__ __forceinline__ float pt_max3(float a, float b, float c) { float r; asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c)); return r; }
 template <int HD>
 struct PtCfg {
     static constexpr int NQ = HD <= 128 ? 2 : 1, DB = HD < 128 ? HD : 128, NB = HD / DB;     // tiles; dimensions a ring slot, slots a unit's keys
-    static constexpr int SOFT = 128 * NQ, NTH = SOFT + 64, TQ = 128 * NQ;
-    static constexpr int SLOT = PG_TC * DB * 2, QT = 128 * HD * 2, BLK = PG_TC * 128;         // bytes; BLK: 128 rows of 64 dimensions
-    static constexpr int SLOTS = HD == 64 ? 8 : 4;
-    static constexpr int SMEM = 1024 + NQ * QT + SLOTS * SLOT;                                 // (1,024 to align)
+    static constexpr int SOFT = 128 * NQ, NTH = SOFT + 128, TQ = 128 * NQ;
+    static constexpr int SLOT = PG_TC * DB * 2, QT = 128 * HD * 2, BLK = PG_TC * 128, QBLK = 128 * 128;      // bytes; BLK, QBLK: 64 dimensions of the positions, of a tile
+    static constexpr int SLOTS = 4;                        // of a ring, one of keys and one of values
+    static constexpr int SMEM = 1024 + NQ * QT + 2 * SLOTS * SLOT;                                 // (1,024 to align)
 };
 struct PtBars {
-    u64 full[8], empty[8], s_full[2], p_full[2], pv_done[2], q_full[2], o_free[2];
+    u64 full[2][4], empty[2][4], s_full[4], p_full[4], pv_done[4], q_full[2], o_free[2];      // (per tile two where units have turns: one at most is ahead of a waiter)
     u32 tmem, failed;
     u32 odd[2];                      // of every other piece: its number + 1, once a value that is not finite was cleared
-    u32 ok[8][4];                    // which positions of a unit are there, of eight units: the eighth next one's keys are asked for after this one's weights were used
+    __align__(16) u32 ok[8][2];                    // which positions of a unit are there, of eight units: the eighth next one's keys are asked for after this one's weights were used
     u32 tiles[PG_PLAN + 1], units[PG_PLAN + 1], scan[16];
     int rows[PG_PLAN + 1], ends[PG_PLAN + 1];
 };
@@ -98,12 +109,14 @@ sz_pg_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
     extern __shared__ __align__(16) u8 raw[];
     u8* const base = raw + (1024 - (sz_smem_addr(raw) & 1023)) % 1024;
     u8* const sq = base;                                   // [tile][HD / 64][128 rows][128 bytes]
-    u8* const ring = sq + C::NQ * C::QT;                   // [slot][DB / 64][128 positions][128 bytes]
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    constexpr int TMA_WARP = C::SOFT / 32, MMA_WARP = TMA_WARP + 1;
+    u8* const ring = sq + C::NQ * C::QT;                   // [keys, values][slot][DB / 64][64 positions][128 bytes]
+    u8* const vring = ring + C::SLOTS * C::SLOT;
+    const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
+    constexpr int TMA_WARP = C::SOFT / 32, S_WARP = TMA_WARP + 2, PV_WARP = TMA_WARP + 3;
     if (tid == 0) {
-        for (int i = 0; i < 8; i++) { sz_mbar_init(&S.full[i], 1); sz_mbar_init(&S.empty[i], 1); }
-        for (int i = 0; i < 2; i++) { sz_mbar_init(&S.s_full[i], 1); sz_mbar_init(&S.p_full[i], 4); sz_mbar_init(&S.pv_done[i], 1); sz_mbar_init(&S.q_full[i], 4); sz_mbar_init(&S.o_free[i], 4); }
+        for (int i = 0; i < 8; i++) { sz_mbar_init(&S.full[0][i], 1); sz_mbar_init(&S.empty[0][i], 1); }
+        for (int i = 0; i < 4; i++) { sz_mbar_init(&S.s_full[i], 1); sz_mbar_init(&S.p_full[i], 4); sz_mbar_init(&S.pv_done[i], 1); }
+        for (int i = 0; i < 2; i++) { sz_mbar_init(&S.q_full[i], 4); sz_mbar_init(&S.o_free[i], 4); }
         S.failed = 0;
         S.odd[0] = S.odd[1] = 0;
         sz_mbar_fence_init();
@@ -115,7 +128,7 @@ sz_pg_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
     pt_before();
     __syncthreads();
     pt_after();
-    const u32 tmem = S.tmem;
+    const u32 tmem = __shfl_sync(0xffffffffu, S.tmem, 0);
     sz_pdl_wait();
     const u32 *tiles = S.tiles, *units = S.units;
     int E;
@@ -160,54 +173,55 @@ sz_pg_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
         it.end = pg_tile_end(d, row_of(bl + 1) - row_of(bl), end_of(bl), it.t, C::TQ);
         return it;
     };
-    // Where keys (kind 0) and values (1) of unit j come in a piece's order of loads, in slots; T units
-    auto place = [&](int kind, int j, int T) {
-        if (C::NQ == 2) return (2 * j + kind) * C::NB;
-        return (kind == 0 ? (j ? 2 * j - 1 : 0) : (j + 1 < T ? 2 * j + 2 : 2 * T - 1)) * C::NB;
-    };
     int failed = 0;
-    if (warp == TMA_WARP) {
-        // ---- loads
-        const int pieces = PG_TC / rows_box;
-        u32 seq = 0, units_in = 0;                         // slots filled, units' keys asked for so far
+    if (warp == TMA_WARP || warp == TMA_WARP + 1) {
+        // ---- loads, of keys and of values: units in order.  Pages are looked up a window of units ahead (32 entries of the table, one a lane): one after the
+        // other, each look-up took as long as a unit.  The copies, too, are issued by one lane of the whole warp (above): lanes that issued their own
+        // took 300 cycles each.
+        const int kind = warp - TMA_WARP, pieces = PG_TC / rows_box, ahead = 32 / pieces;      // boxes a unit (1 .. 8) and 64 dimensions, units a window
+        const u32 one = pt_elect();
+        const CUtensorMap* const map = kind ? &vmap : &kmap;
+        u8* const to = kind ? vring : ring;
+        u32 g = 0;                                         // units so far
         for (u32 u = u0; u < u1 && !failed;) {
             const PgItem it = locate(u);
             const int T = (int)min((u32)(it.n - it.i), u1 - u);
             const int32_t* table = pt.shared ? d.shared_pages : d.pages + (size_t)it.b * d.max_pages;
-            for (int x = 0; x < 2 * T && !failed; x++) {
-                int kind, j;
-                if (C::NQ == 2) { kind = x & 1; j = x >> 1; }
-                else if (x == 0) { kind = 0; j = 0; }
-                else if (x == 2 * T - 1) { kind = 1; j = T - 1; }
-                else { kind = (x & 1) ^ 1; j = kind ? x / 2 - 1 : (x + 1) / 2; }
-                const int c = (it.i + j) * PG_TC + lane * rows_box;
-                int page = -1;
-                const bool there = lane < pieces && c < it.end;
-                if (there) page = __ldg(table + (c >> d.ps_log2));
-                const bool ok = there && (u32)page < (u32)d.n_pages;
-                if (there && !ok) atomicOr(d.err, PG_E_PAGE);
-                for (int nb = 0; nb < C::NB; nb++, seq++) {
-                    const int sl = (int)(seq % C::SLOTS);
-                    if (seq >= C::SLOTS && !pt_wait_warp(&S.empty[sl], seq / C::SLOTS - 1)) { failed = 1; break; }
+            auto window = [&](int w) {
+                const int c = (it.i + w * ahead) * PG_TC + lane * rows_box;
+                return c < it.end ? __ldg(table + (c >> d.ps_log2)) : -2;       // (behind the end: not there, and no error)
+            };
+            int now = window(0), next = window(1);
+            for (int j = 0; j < T && !failed; j++, g++) {
+                const int k0 = j % ahead * pieces;
+                if (j && k0 == 0) { now = next; next = window(j / ahead + 1); }
+                const u32 there = __ballot_sync(0xffffffffu, (u32)now < (u32)d.n_pages) >> k0;
+                if (kind == 0 && lane >= k0 && lane < k0 + pieces && now != -2 && (u32)now >= (u32)d.n_pages) atomicOr(d.err, PG_E_PAGE);
+#pragma unroll
+                for (int nb = 0; nb < C::NB; nb++) {
+                    const u32 n = g * C::NB + nb;
+                    const int sl = (int)(n % C::SLOTS);
+                    if (n >= C::SLOTS && !pt_wait_warp(&S.empty[kind][sl], n / C::SLOTS - 1)) { failed = 1; break; }
                     if (kind == 0 && nb == 0) {            // (read by the softmax threads after the scores are there, which the copies' arrival comes before)
-                        const u32 bits = __ballot_sync(0xffffffffu, ok);
-                        if (lane < 4) {
+                        if (lane < 2) {
                             u32 w = 0;
-                            for (int k = 0; k < 32; k += 8) if ((bits >> ((lane * 32 + k) / rows_box)) & 1u) w |= 0xffu << k;
-                            S.ok[units_in & 7][lane] = w;
+                            for (int k = 0; k < 32; k += 8) if ((there >> ((lane * 32 + k) / rows_box)) & 1u) w |= 0xffu << k;
+                            S.ok[g & 7][lane] = w;
                         }
-                        units_in++;
                         __syncwarp();
                     }
-                    if (lane == 0) sz_mbar_expect_tx(&S.full[sl], C::SLOT);
-                    __syncwarp();
-                    if (lane < pieces) {
+                    u64* const bar = &S.full[kind][sl];
+                    const u32 dst = sz_smem_addr(to) + (u32)(sl * C::SLOT);
+                    asm volatile("{ .reg .pred q; setp.ne.b32 q, %2, 0; @q mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1; }" ::"r"(sz_smem_addr(bar)), "r"((u32)C::SLOT), "r"(one) : "memory");
+                    for (int p = 0; p < pieces; p++) {
+                        const int page = __shfl_sync(0xffffffffu, now, k0 + p), y = ((it.i + j) * PG_TC + p * rows_box) & ((1 << d.ps_log2) - 1);
+                        const int z = (u32)page < (u32)d.n_pages ? page : d.n_pages;
 #pragma unroll
                         for (int q = 0; q < C::DB / 64; q++)
-                            asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(
-                                             sz_smem_addr(ring + (size_t)sl * C::SLOT + q * C::BLK + lane * rows_box * 128)),
-                                         "l"(kind ? &vmap : &kmap), "r"(nb * C::DB + q * 64), "r"(c & ((1 << d.ps_log2) - 1)), "r"(it.h), "r"(ok ? page : d.n_pages),
-                                         "r"(sz_smem_addr(&S.full[sl]))
+                            asm volatile("{ .reg .pred q; setp.ne.b32 q, %7, 0;\n"
+                                         "  @q cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6]; }" ::"r"(
+                                             dst + (u32)(q * C::BLK + p * rows_box * 128)),
+                                         "l"(map), "r"(nb * C::DB + q * 64), "r"(y), "r"(it.h), "r"(z), "r"(sz_smem_addr(bar)), "r"(one)
                                          : "memory");
                     }
                 }
@@ -215,64 +229,82 @@ sz_pg_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
             u += T;
         }
         __syncwarp();
-    } else if (warp == MMA_WARP) {
-        // ---- issue: one thread
-        if (lane == 0) {
-            constexpr u32 id_s = pt_idesc(BF, PG_TC, false), id_v = pt_idesc(BF, C::DB, true);
-            const u64 qd = pt_desc(sz_smem_addr(sq), 16, 1024), kd = pt_desc(sz_smem_addr(ring), 16, 1024), vd = pt_desc(sz_smem_addr(ring), C::BLK, 1024);
-            u32 seq0 = 0, piece = 0, used[2] = {0, 0};     // slots before this piece; pieces; weights taken of a buffer
-            u32 buf0 = 0;                                  // the buffer of the piece's unit 0
-            for (u32 u = u0; u < u1 && !failed; piece++) {
-                const PgItem it = locate(u);
-                const int T = (int)min((u32)(it.n - it.i), u1 - u), N = T * C::NQ;
-                for (int q = 0; q < C::NQ && !failed; q++) if (!pt_wait(&S.q_full[q], piece)) failed = 2;
-                auto scores = [&](int x) {
-                    const int q = x % C::NQ, j = x / C::NQ, buf = (int)((buf0 + x) & 1);
-                    const u32 at = seq0 + place(0, j, T);
+    } else if (warp == S_WARP) {
+        // ---- the scores' products: a unit's, once its buffer's last weights have been used
+        constexpr u32 id_s = pt_idesc(BF, PG_TC, false);
+        const u32 one = pt_elect();
+        const u64 qd = pt_desc(sz_smem_addr(sq), 16, 1024), kd = pt_desc(sz_smem_addr(ring), 16, 1024);
+        u32 piece = 0, done = 0;                           // pieces; units before this one
+        for (u32 u = u0; u < u1 && !failed; piece++) {
+            const PgItem it = locate(u);
+            const int T = (int)min((u32)(it.n - it.i), u1 - u);
+            for (int q = 0; q < C::NQ && !failed; q++) if (!pt_wait_warp(&S.q_full[q], piece)) failed = 2;
+            for (int j = 0; j < T && !failed; j++) {
+                const u32 g = done + j;
+#pragma unroll
+                for (int q = 0; q < C::NQ; q++) {
+                    const int buf = q * 2 + (int)(g & 1);
+                    if (g >= 2 && !pt_wait_warp(&S.pv_done[buf], (g >> 1) - 1)) { failed = 4; break; }
+#pragma unroll
                     for (int nb = 0; nb < C::NB; nb++) {
-                        const int sl = (int)((at + nb) % C::SLOTS);
-                        if (q == 0 && !pt_wait(&S.full[sl], (at + nb) / C::SLOTS)) { failed = 3; return; }
+                        const int sl = (int)((g * C::NB + nb) % C::SLOTS);
+                        if (q == 0 && !pt_wait_warp(&S.full[0][sl], (g * C::NB + nb) / C::SLOTS)) { failed = 3; break; }
                         pt_after();
+                        const u64 qa = qd + (u32)((q * C::QT + nb * (C::DB / 64) * C::QBLK) / 16), ka = kd + (u32)(sl * (C::SLOT / 16));
 #pragma unroll
                         for (int k = 0; k < C::DB / 16; k++)       // (addresses in 16-byte units: 16 dimensions are 32 bytes of a row)
-                            pt_mma_ss(tmem + buf * 128, qd + (u32)((q * C::QT + (nb * (C::DB / 64) + k / 4) * C::BLK) / 16 + (k % 4) * 2), kd + (u32)((sl * C::SLOT + k / 4 * C::BLK) / 16 + (k % 4) * 2),
-                                      id_s, nb | k);
-                        if (q == C::NQ - 1) pt_commit(&S.empty[sl]);
-                    }
-                    pt_commit(&S.s_full[buf]);
-                };
-                if (!failed) scores(0);
-                if (!failed && N > 1) scores(1);
-                for (int x = 0; x < N && !failed; x++) {
-                    const int q = x % C::NQ, j = x / C::NQ, buf = (int)((buf0 + x) & 1);
-                    if (!pt_wait(&S.p_full[buf], used[buf]++)) { failed = 4; break; }
-                    if (x < C::NQ && piece > 0 && !pt_wait(&S.o_free[q], piece - 1)) { failed = 5; break; }
-                    pt_after();
-                    const u32 at = seq0 + place(1, j, T);
-                    for (int nb = 0; nb < C::NB; nb++) {
-                        const int sl = (int)((at + nb) % C::SLOTS);
-                        if (q == 0 && !pt_wait(&S.full[sl], (at + nb) / C::SLOTS)) { failed = 6; break; }
-                        pt_after();
-#pragma unroll
-                        for (int k = 0; k < PG_TC / 16; k++)       // 16 positions: 8 columns of weight pairs, 16 rows of 128 bytes
-                            pt_mma_ts(tmem + 256 + q * HD + nb * C::DB, tmem + buf * 128 + k * 8, vd + (u32)((sl * C::SLOT + k * 2048) / 16), id_v, (u32)(j | k));
-                        if (q == C::NQ - 1) pt_commit(&S.empty[sl]);
+                            pt_mma_ss(tmem + buf * PG_TC, qa + (u32)(k / 4 * (C::QBLK / 16) + (k % 4) * 2), ka + (u32)(k / 4 * (C::BLK / 16) + (k % 4) * 2), id_s, nb | k, one);
+                        if (q == C::NQ - 1) pt_commit(&S.empty[0][sl], one);
                     }
                     if (failed) break;
-                    pt_commit(&S.pv_done[q]);
-                    if (x + 2 < N) scores(x + 2);
+                    pt_commit(&S.s_full[buf], one);
                 }
-                seq0 += 2 * T * C::NB;
-                buf0 = (buf0 + N) & 1;
-                u += T;
             }
+            done += T;
+            u += T;
+        }
+        __syncwarp();
+    } else if (warp == PV_WARP) {
+        // ---- the sums' products: a unit's, once its weights are there
+        constexpr u32 id_v = pt_idesc(BF, C::DB, true);
+        const u32 one = pt_elect();
+        const u64 vd = pt_desc(sz_smem_addr(vring), C::BLK, 1024);
+        u32 piece = 0, done = 0;
+        for (u32 u = u0; u < u1 && !failed; piece++) {
+            const PgItem it = locate(u);
+            const int T = (int)min((u32)(it.n - it.i), u1 - u);
+            for (int j = 0; j < T && !failed; j++) {
+                const u32 g = done + j;
+#pragma unroll
+                for (int q = 0; q < C::NQ; q++) {
+                    const int buf = q * 2 + (int)(g & 1);
+                    if (j == 0 && piece > 0 && !pt_wait_warp(&S.o_free[q], piece - 1)) { failed = 5; break; }
+                    if (!pt_wait_warp(&S.p_full[buf], g >> 1)) { failed = 4; break; }
+#pragma unroll
+                    for (int nb = 0; nb < C::NB; nb++) {
+                        const int sl = (int)((g * C::NB + nb) % C::SLOTS);
+                        if (q == 0 && !pt_wait_warp(&S.full[1][sl], (g * C::NB + nb) / C::SLOTS)) { failed = 6; break; }
+                        pt_after();
+                        const u64 va = vd + (u32)(sl * (C::SLOT / 16));
+                        const u32 od = tmem + 256 + q * HD + nb * C::DB, pa = tmem + buf * PG_TC;
+#pragma unroll
+                        for (int k = 0; k < PG_TC / 16; k++)       // 16 positions: 8 columns of weight pairs, 16 rows of 128 bytes
+                            pt_mma_ts(od, pa + k * 8, va + (u32)(k * 128), id_v, (u32)(j | k), one);
+                        if (q == C::NQ - 1) pt_commit(&S.empty[1][sl], one);
+                    }
+                    if (failed) break;
+                    pt_commit(&S.pv_done[buf], one);
+                }
+            }
+            done += T;
+            u += T;
         }
         __syncwarp();
     } else {
         // ---- softmax: thread = query vector
         const int q = warp / 4, row = tid & 127;
         const u32 lanes = (u32)((warp & 3) * 32) << 16;
-        u32 piece = 0, taken[2] = {0, 0}, done = 0, seq0 = 0, buf0 = 0;      // taken: scores of a buffer; done: units of this tile; seq0: ring slots before the piece
+        u32 piece = 0, done = 0;                           // done: units so far
         for (u32 u = u0; u < u1 && !failed; piece++) {
             const PgItem it = locate(u);
             const int T = (int)min((u32)(it.n - it.i), u1 - u);
@@ -289,43 +321,43 @@ sz_pg_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
 #pragma unroll 8
                 for (int c = 0; c < HD / 8; c++) {
                     const uint4 w = qr < m ? __ldg(src + c) : make_uint4(0, 0, 0, 0);
-                    *(uint4*)(dst + c / 8 * C::BLK + (((c & 7) ^ (row & 7)) << 4)) = w;
+                    *(uint4*)(dst + c / 8 * C::QBLK + (((c & 7) ^ (row & 7)) << 4)) = w;
                 }
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 pt_arrive_warp(&S.q_full[q]);
             }
             float mx = -INFINITY, l = 0.f;                 // what the row divides by (in units of log 2), the sum of its weights
             for (int j = 0; j < T; j++) {
-                const int buf = C::NQ == 2 ? q : (int)((buf0 + j) & 1);
-                if (!pt_wait_warp(&S.s_full[buf], taken[buf]++)) { failed = 7; break; }
+                const int buf = q * 2 + (int)(done & 1);
+                if (!pt_wait_warp(&S.s_full[buf], done >> 1)) { failed = 7; break; }
                 pt_after();
-                float s[128];
-                const u32 at = tmem + lanes + buf * 128;
+                float s[PG_TC];
+                const u32 at = tmem + lanes + buf * PG_TC;
+                pt_ld32(at, s);
+                pt_ld32(at + 32, s + 32);
+                const uint2 ok = *(const uint2*)S.ok[done & 7];
+                const int at_pos = (it.i + j) * PG_TC, seen = lim - at_pos;
+                const bool whole = __all_sync(0xffffffffu, seen >= PG_TC && (ok.x & ok.y) == 0xffffffffu);
+                pt_loaded(s);
+                pt_loaded(s + 32);
+                if (!whole) {
 #pragma unroll
-                for (int k = 0; k < 4; k++) pt_ld32(at + 32 * k, s + 32 * k);
-#pragma unroll
-                for (int k = 0; k < 4; k++) pt_loaded(s + 32 * k);
-                const u32* ok = S.ok[done & 7];
-                if ((ok[0] & ok[1] & ok[2] & ok[3]) != 0xffffffffu) {
-#pragma unroll
-                    for (int k = 0; k < 128; k++) s[k] = (ok[k / 32] >> (k & 31)) & 1u ? s[k] : -INFINITY;
-                }
-                const int at_pos = (it.i + j) * PG_TC;
-                if (lim < at_pos + PG_TC) {
-                    const int seen = lim - at_pos;
-#pragma unroll
-                    for (int k = 0; k < 128; k++) s[k] = k < seen ? s[k] : -INFINITY;
+                    for (int k = 0; k < PG_TC; k++) s[k] = k < seen && ((k < 32 ? ok.x : ok.y) >> (k & 31)) & 1u ? s[k] : -INFINITY;
                 }
                 float big[4] = {s[0], s[1], s[2], s[3]};
 #pragma unroll
-                for (int k = 4; k < 128; k++) big[k & 3] = fmaxf(big[k & 3], s[k]);
-                const float top = fmaxf(fmaxf(big[0], big[1]), fmaxf(big[2], big[3])) * io.scale_log2;
+                for (int k = 4; k < 60; k += 8) {
+#pragma unroll
+                    for (int e = 0; e < 4; e++) big[e] = pt_max3(big[e], s[k + 2 * e], s[k + 2 * e + 1]);
+                }
+                const float top = pt_max3(pt_max3(big[0], big[1], s[60]), pt_max3(big[2], big[3], s[61]), pt_max3(s[62], s[63], s[63])) * io.scale_log2;
+                if (!(top < INFINITY)) l = NAN;            // (a score that is NaN or infinite: so is the row)
                 const bool up = top > mx + 8.f || (mx == -INFINITY && top > -INFINITY);
                 if (__any_sync(0xffffffffu, up)) {
                     const float by = !up ? 1.f : mx == -INFINITY ? 0.f : pg_ex2(mx - top);
                     if (up) { mx = top; l *= by; }
                     if (j > 0) {                           // the sums so far, once the last product is in them
-                        if (!pt_wait_warp(&S.pv_done[q], done - 1)) { failed = 8; break; }
+                        if (!pt_wait_warp(&S.pv_done[q * 2 + ((done - 1) & 1)], (done - 1) >> 1)) { failed = 8; break; }
                         pt_after();
 #pragma unroll 1
                         for (int k = 0; k < HD; k += 32) {
@@ -342,7 +374,7 @@ sz_pg_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
                 const float sub = mx == -INFINITY ? 0.f : mx;
                 float sum[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                for (int k = 0; k < 128; k += 32) {
+                for (int k = 0; k < PG_TC; k += 32) {
                     u32 w[16];
 #pragma unroll
                     for (int e = 0; e < 32; e += 2) {
@@ -354,13 +386,12 @@ sz_pg_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
                 }
                 l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
                 if (q == 0 && all < at_pos + PG_TC) {      // the values that some row does not see
-                    const u32 at_v = seq0 + place(1, j, T);
                     for (int nb = 0; nb < C::NB && !failed; nb++) {
-                        const int sl = (int)((at_v + nb) % C::SLOTS);
-                        if (!pt_wait_warp(&S.full[sl], (at_v + nb) / C::SLOTS)) { failed = 10; break; }
+                        const int sl = (int)((done * C::NB + nb) % C::SLOTS);
+                        if (!pt_wait_warp(&S.full[1][sl], (done * C::NB + nb) / C::SLOTS)) { failed = 10; break; }
 #pragma unroll 4
-                        for (int x = tid; x < C::SLOT / 16; x += 128) {      // (a slot is blocks of 128 rows of 128 bytes)
-                            uint4* const at16 = (uint4*)(ring + (size_t)sl * C::SLOT) + x;
+                        for (int x = tid; x < C::SLOT / 16; x += 128) {      // (a slot is blocks of 64 rows of 128 bytes)
+                            uint4* const at16 = (uint4*)(vring + (size_t)sl * C::SLOT) + x;
                             const uint4 w = *at16;
                             const u32 in[4] = {w.x, w.y, w.z, w.w};
                             u32 out[4];
@@ -386,7 +417,7 @@ sz_pg_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
                 done++;
             }
             // ---- the piece's part: (maximum, sum of weights, sums)
-            if (!failed && !pt_wait_warp(&S.pv_done[q], done - 1)) failed = 9;
+            if (!failed && !pt_wait_warp(&S.pv_done[q * 2 + ((done - 1) & 1)], (done - 1) >> 1)) failed = 9;
             if (failed) break;
             pt_after();
             const u32 us = units[it.e] * (u32)d.nkv + (u32)it.h * (u32)it.n;
@@ -441,8 +472,6 @@ sz_pg_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
             if (qr < m && direct && io.lse) io.lse[to] = none ? -INFINITY : (mx + log2f(l)) * 0.6931471805599453f;
             pt_before();
             pt_arrive_warp(&S.o_free[q]);
-            seq0 += 2 * T * C::NB;
-            buf0 = (buf0 + T * C::NQ) & 1;
             u += T;
         }
     }
