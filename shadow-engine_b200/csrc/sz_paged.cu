@@ -452,8 +452,8 @@ extern "C" int sz_paged_attend(const sz_paged_cache* cache, const sz_paged_batch
     const bool tc = pg_tc_type(cache->type) && io_type == cache->type && scale > 0.f;
     const bool tc_of[2] = {tc && all >= PG_TC_MIN, tc && per_seq >= PG_TC_MIN};
     PgKernels kern[2];
-    CUtensorMap maps[2][2];              // [of 16 positions, of 128][keys, values]
-    const int box[2] = {cache->page_size < 16 ? cache->page_size : 16, cache->page_size < PG_TC ? cache->page_size : PG_TC};
+    CUtensorMap maps[2][2];              // [of 16 positions, of a tcgen05 unit][keys, values]
+    const int box[2] = {cache->page_size < 16 ? cache->page_size : 16, cache->page_size < pg_tc_unit(hd) ? cache->page_size : pg_tc_unit(hd)};
     bool planned = false;
     for (int i = 0; i < 2; i++) {
         PgPart& p = s.a.p[i];
@@ -461,7 +461,7 @@ extern "C" int sz_paged_attend(const sz_paged_cache* cache, const sz_paged_batch
         p.shared = i == PG_SHARED;
         if (!p.on) continue;
         kern[i] = kernels(pg_tiles_of(i == PG_SHARED ? all : per_seq));
-        p.unit = tc_of[i] ? PG_TC : PG_T;
+        p.unit = tc_of[i] ? pg_tc_unit(hd) : PG_T;
         p.ways = tc_of[i] ? 1 : kern[i].ways;
         p.tq = tc_of[i] ? pg_tc_tile(hd) : kern[i].tq;
         p.blocks = tc_of[i] ? PG_BLOCKS : PG_BLOCKS * kern[i].occ;

@@ -18,7 +18,6 @@
 constexpr int PG_T = 64;             // positions a unit
 constexpr int PG_PLAN = 256;         // sequences and tiles that a block plans for itself; above, sz_pg_plan_kernel does once
 constexpr int PG_MAX_SEQ = 4096;
-constexpr int PG_TC = 64;            // positions a unit of the tcgen05 kernel (sz_paged_tc.cu)
 enum { PG_F16 = 0, PG_BF16 = 1, PG_Q8 = 2 };
 enum { PG_E_PAGE = 1, PG_E_END = 2, PG_E_SHARED = 4, PG_E_ROWS = 8, PG_E_WAIT = 16 };
 
@@ -51,7 +50,7 @@ struct PgPart {
     float2* row_ml;                  // [row][head][ways]
     int ways;                        // parts that a block leaves of an item
     int blocks, tq, shared, planned; // planned: the plan was made by sz_pg_plan_kernel
-    int unit;                        // positions a unit: PG_T, or PG_TC for the tcgen05 kernel
+    int unit;                        // positions a unit: PG_T, or the tcgen05 kernel's
     int direct;                      // (tcgen05 kernel) an item that one block does alone goes straight to the output
     int on;
 };
@@ -725,6 +724,7 @@ PgKernels pg_kernels_bf16(bool wide, int hd, int nqt);
 PgKernels pg_kernels_q8(bool wide, int hd, int nqt);
 // The tcgen05 kernel (sz_paged_tc.cu): vectors a tile; the launch over own or shared positions.
 int pg_tc_tile(int hd);
+int pg_tc_unit(int hd);
 int pg_tc_launch(bool bf16, int hd, const CUtensorMap* maps, int rows_box, const PgBatch& d, const PgIo& io, const PgPart& p, const char* name, cudaStream_t st);
 
 template <int CT, bool WIDE, int HD, int NQT>

@@ -5,7 +5,7 @@
 // Types: 16-bit queries over a cache of the same type.
 //
 // A block has NQ x 128 query vectors of one key head (two tiles of 128 up to head_dim 128, one above) and the columns of tensor memory:
-//     0 .. 255    scores, two buffers of 64 positions a tile (f32); the weights lie over the buffer they come from, as pairs of 16 bits
+//     0 .. 255    scores, two buffers a tile of 64 positions (head_dim 256: 128) in f32; the weights lie over the buffer they come from, as pairs of 16 bits
 //     256 .. 511  the tiles' sums, NQ x head_dim
 // One warp issues the scores' products of unit after unit, another the sums', each when its operands are there and the buffer is free: what they do between
 // two units - waits, a commit, descriptors: 500 cycles - is hidden behind the other's instructions, and a tile's softmax goes from unit to
@@ -85,16 +85,17 @@ __device__ __forceinline__ float pt_max3(float a, float b, float c) { float r; a
 template <int HD>
 struct PtCfg {
     static constexpr int NQ = HD <= 128 ? 2 : 1, DB = HD < 128 ? HD : 128, NB = HD / DB;     // tiles; dimensions a ring slot, slots a unit's keys
+    static constexpr int UT = HD == 256 ? 128 : 64;          // positions a unit
     static constexpr int SOFT = 128 * NQ, NTH = SOFT + 128, TQ = 128 * NQ;
-    static constexpr int SLOT = PG_TC * DB * 2, QT = 128 * HD * 2, BLK = PG_TC * 128, QBLK = 128 * 128;      // bytes; BLK, QBLK: 64 dimensions of the positions, of a tile
-    static constexpr int SLOTS = 4;                        // of a ring, one of keys and one of values
+    static constexpr int SLOT = UT * DB * 2, QT = 128 * HD * 2, BLK = UT * 128, QBLK = 128 * 128;      // bytes; BLK, QBLK: 64 dimensions of the positions, of a tile
+    static constexpr int SLOTS = 256 / UT;                 // of a ring, one of keys and one of values
     static constexpr int SMEM = 1024 + NQ * QT + 2 * SLOTS * SLOT;                                 // (1,024 to align)
 };
 struct PtBars {
     u64 full[2][4], empty[2][4], s_full[4], p_full[4], pv_done[4], q_full[2], o_free[2];      // (per tile two where units have turns: one at most is ahead of a waiter)
     u32 tmem, failed;
     u32 odd[2];                      // of every other piece: its number + 1, once a value that is not finite was cleared
-    __align__(16) u32 ok[8][2];                    // which positions of a unit are there, of eight units: the eighth next one's keys are asked for after this one's weights were used
+    __align__(16) u32 ok[8][4];                    // which positions of a unit are there, of eight units: the eighth next one's keys are asked for after this one's weights were used
     u32 tiles[PG_PLAN + 1], units[PG_PLAN + 1], scan[16];
     int rows[PG_PLAN + 1], ends[PG_PLAN + 1];
 };
@@ -136,7 +137,7 @@ sz_pg_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
         tiles = pt.tiles; units = pt.units;
         E = pt.shared ? max(0, ((pg_row(d, d.n_seq) - pg_row(d, 0)) * d.G + C::TQ - 1) / C::TQ) : (int)tiles[d.n_seq];
     } else {
-        E = pg_plan<C::NTH>(d, pt.shared, PG_TC, C::TQ, S.tiles, S.units, S.scan, S.rows, S.ends);
+        E = pg_plan<C::NTH>(d, pt.shared, C::UT, C::TQ, S.tiles, S.units, S.scan, S.rows, S.ends);
         if (blockIdx.x == 0) {
             if (!pt.shared) for (int i = tid; i <= d.n_seq; i += C::NTH) pt.tiles[i] = S.tiles[i];
             for (int i = tid; i <= E; i += C::NTH) pt.units[i] = S.units[i];
@@ -178,7 +179,7 @@ sz_pg_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
         // ---- loads, of keys and of values: units in order.  Pages are looked up a window of units ahead (32 entries of the table, one a lane): one after the
         // other, each look-up took as long as a unit.  The copies, too, are issued by one lane of the whole warp (above): lanes that issued their own
         // took 300 cycles each.
-        const int kind = warp - TMA_WARP, pieces = PG_TC / rows_box, ahead = 32 / pieces;      // boxes a unit (1 .. 8) and 64 dimensions, units a window
+        const int kind = warp - TMA_WARP, pieces = C::UT / rows_box, ahead = 32 / pieces;      // boxes a unit (1 .. 16) and 64 dimensions, units a window
         const u32 one = pt_elect();
         const CUtensorMap* const map = kind ? &vmap : &kmap;
         u8* const to = kind ? vring : ring;
@@ -188,7 +189,7 @@ sz_pg_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
             const int T = (int)min((u32)(it.n - it.i), u1 - u);
             const int32_t* table = pt.shared ? d.shared_pages : d.pages + (size_t)it.b * d.max_pages;
             auto window = [&](int w) {
-                const int c = (it.i + w * ahead) * PG_TC + lane * rows_box;
+                const int c = (it.i + w * ahead) * C::UT + lane * rows_box;
                 return c < it.end ? __ldg(table + (c >> d.ps_log2)) : -2;       // (behind the end: not there, and no error)
             };
             int now = window(0), next = window(1);
@@ -203,7 +204,7 @@ sz_pg_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
                     const int sl = (int)(n % C::SLOTS);
                     if (n >= C::SLOTS && !pt_wait_warp(&S.empty[kind][sl], n / C::SLOTS - 1)) { failed = 1; break; }
                     if (kind == 0 && nb == 0) {            // (read by the softmax threads after the scores are there, which the copies' arrival comes before)
-                        if (lane < 2) {
+                        if (lane < C::UT / 32) {
                             u32 w = 0;
                             for (int k = 0; k < 32; k += 8) if ((there >> ((lane * 32 + k) / rows_box)) & 1u) w |= 0xffu << k;
                             S.ok[g & 7][lane] = w;
@@ -214,7 +215,7 @@ sz_pg_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
                     const u32 dst = sz_smem_addr(to) + (u32)(sl * C::SLOT);
                     asm volatile("{ .reg .pred q; setp.ne.b32 q, %2, 0; @q mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1; }" ::"r"(sz_smem_addr(bar)), "r"((u32)C::SLOT), "r"(one) : "memory");
                     for (int p = 0; p < pieces; p++) {
-                        const int page = __shfl_sync(0xffffffffu, now, k0 + p), y = ((it.i + j) * PG_TC + p * rows_box) & ((1 << d.ps_log2) - 1);
+                        const int page = __shfl_sync(0xffffffffu, now, k0 + p), y = ((it.i + j) * C::UT + p * rows_box) & ((1 << d.ps_log2) - 1);
                         const int z = (u32)page < (u32)d.n_pages ? page : d.n_pages;
 #pragma unroll
                         for (int q = 0; q < C::DB / 64; q++)
@@ -231,7 +232,7 @@ sz_pg_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
         __syncwarp();
     } else if (warp == S_WARP) {
         // ---- the scores' products: a unit's, once its buffer's last weights have been used
-        constexpr u32 id_s = pt_idesc(BF, PG_TC, false);
+        constexpr u32 id_s = pt_idesc(BF, C::UT, false);
         const u32 one = pt_elect();
         const u64 qd = pt_desc(sz_smem_addr(sq), 16, 1024), kd = pt_desc(sz_smem_addr(ring), 16, 1024);
         u32 piece = 0, done = 0;                           // pieces; units before this one
@@ -253,7 +254,7 @@ sz_pg_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
                         const u64 qa = qd + (u32)((q * C::QT + nb * (C::DB / 64) * C::QBLK) / 16), ka = kd + (u32)(sl * (C::SLOT / 16));
 #pragma unroll
                         for (int k = 0; k < C::DB / 16; k++)       // (addresses in 16-byte units: 16 dimensions are 32 bytes of a row)
-                            pt_mma_ss(tmem + buf * PG_TC, qa + (u32)(k / 4 * (C::QBLK / 16) + (k % 4) * 2), ka + (u32)(k / 4 * (C::BLK / 16) + (k % 4) * 2), id_s, nb | k, one);
+                            pt_mma_ss(tmem + buf * C::UT, qa + (u32)(k / 4 * (C::QBLK / 16) + (k % 4) * 2), ka + (u32)(k / 4 * (C::BLK / 16) + (k % 4) * 2), id_s, nb | k, one);
                         if (q == C::NQ - 1) pt_commit(&S.empty[0][sl], one);
                     }
                     if (failed) break;
@@ -286,9 +287,9 @@ sz_pg_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
                         if (q == 0 && !pt_wait_warp(&S.full[1][sl], (g * C::NB + nb) / C::SLOTS)) { failed = 6; break; }
                         pt_after();
                         const u64 va = vd + (u32)(sl * (C::SLOT / 16));
-                        const u32 od = tmem + 256 + q * HD + nb * C::DB, pa = tmem + buf * PG_TC;
+                        const u32 od = tmem + 256 + q * HD + nb * C::DB, pa = tmem + buf * C::UT;
 #pragma unroll
-                        for (int k = 0; k < PG_TC / 16; k++)       // 16 positions: 8 columns of weight pairs, 16 rows of 128 bytes
+                        for (int k = 0; k < C::UT / 16; k++)       // 16 positions: 8 columns of weight pairs, 16 rows of 128 bytes
                             pt_mma_ts(od, pa + k * 8, va + (u32)(k * 128), id_v, (u32)(j | k), one);
                         if (q == C::NQ - 1) pt_commit(&S.empty[1][sl], one);
                     }
@@ -331,26 +332,27 @@ sz_pg_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
                 const int buf = q * 2 + (int)(done & 1);
                 if (!pt_wait_warp(&S.s_full[buf], done >> 1)) { failed = 7; break; }
                 pt_after();
-                float s[PG_TC];
-                const u32 at = tmem + lanes + buf * PG_TC;
-                pt_ld32(at, s);
-                pt_ld32(at + 32, s + 32);
-                const uint2 ok = *(const uint2*)S.ok[done & 7];
-                const int at_pos = (it.i + j) * PG_TC, seen = lim - at_pos;
-                const bool whole = __all_sync(0xffffffffu, seen >= PG_TC && (ok.x & ok.y) == 0xffffffffu);
-                pt_loaded(s);
-                pt_loaded(s + 32);
+                float s[C::UT];
+                const u32 at = tmem + lanes + buf * C::UT;
+#pragma unroll
+                for (int k = 0; k < C::UT; k += 32) pt_ld32(at + k, s + k);
+                const uint4 ok4 = *(const uint4*)S.ok[done & 7];
+                const u32 ok[4] = {ok4.x, ok4.y, ok4.z, ok4.w};
+                const int at_pos = (it.i + j) * C::UT, seen = lim - at_pos;
+                const bool whole = __all_sync(0xffffffffu, seen >= C::UT && (ok[0] & ok[1] & (C::UT > 64 ? ok[2] & ok[3] : 0xffffffffu)) == 0xffffffffu);
+#pragma unroll
+                for (int k = 0; k < C::UT; k += 32) pt_loaded(s + k);
                 if (!whole) {
 #pragma unroll
-                    for (int k = 0; k < PG_TC; k++) s[k] = k < seen && ((k < 32 ? ok.x : ok.y) >> (k & 31)) & 1u ? s[k] : -INFINITY;
+                    for (int k = 0; k < C::UT; k++) s[k] = k < seen && (ok[k / 32] >> (k & 31)) & 1u ? s[k] : -INFINITY;
                 }
                 float big[4] = {s[0], s[1], s[2], s[3]};
 #pragma unroll
-                for (int k = 4; k < 60; k += 8) {
+                for (int k = 4; k < C::UT - 4; k += 8) {
 #pragma unroll
                     for (int e = 0; e < 4; e++) big[e] = pt_max3(big[e], s[k + 2 * e], s[k + 2 * e + 1]);
                 }
-                const float top = pt_max3(pt_max3(big[0], big[1], s[60]), pt_max3(big[2], big[3], s[61]), pt_max3(s[62], s[63], s[63])) * io.scale_log2;
+                const float top = pt_max3(pt_max3(big[0], big[1], s[C::UT - 4]), pt_max3(big[2], big[3], s[C::UT - 3]), pt_max3(s[C::UT - 2], s[C::UT - 1], s[C::UT - 1])) * io.scale_log2;
                 if (!(top < INFINITY)) l = NAN;            // (a score that is NaN or infinite: so is the row)
                 const bool up = top > mx + 8.f || (mx == -INFINITY && top > -INFINITY);
                 if (__any_sync(0xffffffffu, up)) {
@@ -374,7 +376,7 @@ sz_pg_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
                 const float sub = mx == -INFINITY ? 0.f : mx;
                 float sum[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                for (int k = 0; k < PG_TC; k += 32) {
+                for (int k = 0; k < C::UT; k += 32) {
                     u32 w[16];
 #pragma unroll
                     for (int e = 0; e < 32; e += 2) {
@@ -385,7 +387,7 @@ sz_pg_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
                     pt_st16(at + k / 2, w);
                 }
                 l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-                if (q == 0 && all < at_pos + PG_TC) {      // the values that some row does not see
+                if (q == 0 && all < at_pos + C::UT) {      // the values that some row does not see
                     for (int nb = 0; nb < C::NB && !failed; nb++) {
                         const int sl = (int)((done * C::NB + nb) % C::SLOTS);
                         if (!pt_wait_warp(&S.full[1][sl], (done * C::NB + nb) / C::SLOTS)) { failed = 10; break; }
@@ -395,7 +397,7 @@ sz_pg_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
                             const uint4 w = *at16;
                             const u32 in[4] = {w.x, w.y, w.z, w.w};
                             u32 out[4];
-                            const bool behind = at_pos + (x >> 3) % PG_TC >= it.end;
+                            const bool behind = at_pos + (x >> 3) % C::UT >= it.end;
                             bool odd = false;
 #pragma unroll
                             for (int k = 0; k < 4; k++) {
@@ -437,7 +439,7 @@ sz_pg_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
                 if (qr >= m) continue;
                 if (odd) {                                 // the values that were cleared, where this row sees them
                     const int32_t* table = pt.shared ? d.shared_pages : d.pages + (size_t)it.b * d.max_pages;
-                    for (int t = max(it.i * PG_TC, all & ~(PG_TC - 1)); t < min(lim, (it.i + T) * PG_TC); t++) {
+                    for (int t = max(it.i * C::UT, all & ~(C::UT - 1)); t < min(lim, (it.i + T) * C::UT); t++) {
                         const int page = __ldg(table + (t >> d.ps_log2));
                         if ((u32)page >= (u32)d.n_pages) continue;
                         const u8* src = d.v + (long long)page * d.page_stride + (long long)(t & ((1 << d.ps_log2) - 1)) * d.pos_stride + (long long)it.h * d.head_stride + 2 * k;
@@ -498,6 +500,7 @@ int pt_launch(const CUtensorMap* maps, int rows_box, const PgBatch& d, const PgI
 }  // namespace
 
 int pg_tc_tile(int hd) { return hd <= 128 ? 256 : 128; }
+int pg_tc_unit(int hd) { return hd == 64 ? PtCfg<64>::UT : hd == 128 ? PtCfg<128>::UT : PtCfg<256>::UT; }
 
 int pg_tc_launch(bool bf16, int hd, const CUtensorMap* maps, int rows_box, const PgBatch& d, const PgIo& io, const PgPart& p, const char* name, cudaStream_t st) {
     if (bf16) return hd == 64 ? pt_launch<true, 64>(maps, rows_box, d, io, p, name, st) : hd == 128 ? pt_launch<true, 128>(maps, rows_box, d, io, p, name, st) : pt_launch<true, 256>(maps, rows_box, d, io, p, name, st);
