@@ -14,7 +14,7 @@ struct PgAppend {
     u8* qo;
     long long k_stride, v_stride, q_stride, q_head_stride, qo_stride;   // bytes
     const float *q_norm, *k_norm;
-    int type, esz, hd, nh, half, heads;     // heads: nh (0 without q) + 2 nkv
+    int nh, half, heads;             // heads: nh (0 without q) + 2 nkv
     float eps;
     double freq[128];                // 1 / theta^(2 i / dims)
 };
@@ -27,112 +27,208 @@ __device__ int pg_seq_of(const PgBatch& d, int r) {
     return n > d.n_seq ? -1 : n - 1;
 }
 
-// A block has 8 heads of one row, a warp each (grid.y: the row's eights of heads, queries first, then keys, then values).  What bounds it is
-// latency with few rows - row, sequence, length, page, head, one after the other - and with many the bytes.  The angles of the row
-// are taken once a block, in f64 (a far position's angle has no digits left in f32), reduced to [-pi, pi] there, and the sine and
+// f = head / sqrt(mean(head^2) + eps) * w, then (f_i, f_(i + half)) turned by pos theta^(-2 i / dims).  A lane has hd / 32 neighbouring dimensions, and
+// a rotation's partner is hd / 32 dimensions of another lane.  Sums of squares and rotations in f32, one rounding to the stored type.
+// R = 1 row a block, a warp a head, for few rows: latency bounds those - sequence, length, page, head, one after the other -, so the head is read
+// while its row is looked up.  R = PG_APP where that still gives every multiprocessor a block: a warp a row, its heads four at a time (their loads
+// and their norms' shuffles side by side).  24 heads of 256, keys and values of bf16: 1 row 3.6 us, 64 rows 5.2, 4,093 rows 29.1 against
+// 51 with R = 1 (83 MB: 12.8 us of them; the chains of norm, rotation and store of one wave of warps are the rest).
+// A row's angles are taken once a block, in f64 (a far position's angle has no digits left in f32), reduced to [-pi, pi] there, and the sine and
 // cosine of the reduced angle in f32 with its rounding put back by their derivatives.
-template <int CT>
+constexpr int PG_APP = 8;
+template <int K> struct PgKind { __device__ constexpr operator int() const { return K; } };
+template <int E, int type>
+__device__ __forceinline__ void pg_load_n(const u8* p, float* f) {      // E neighbouring elements
+    if (type == SZ_TYPE_F32) {
+#pragma unroll
+        for (int e = 0; e < E; e += E == 2 ? 2 : 4) {
+            if (E == 2) { const float2 x = *(const float2*)p; f[0] = x.x; f[1] = x.y; }
+            else { const float4 x = *(const float4*)(p + 4 * e); f[e] = x.x; f[e + 1] = x.y; f[(e + 2) % E] = x.z; f[(e + 3) % E] = x.w; }
+        }
+        return;
+    }
+    u32 w[E / 2];
+    if (E == 8) *(uint4*)w = *(const uint4*)p;
+    else if (E == 4) *(uint2*)w = *(const uint2*)p;
+    else w[0] = *(const u32*)p;
+#pragma unroll
+    for (int e = 0; e < E; e += 2) {
+        const float2 x = type == SZ_TYPE_F16 ? __half22float2(*(const __half2*)&w[e / 2]) : make_float2(__uint_as_float(w[e / 2] << 16), __uint_as_float(w[e / 2] & 0xffff0000u));
+        f[e] = x.x; f[e + 1] = x.y;
+    }
+}
+template <int E, int type>
+__device__ __forceinline__ void pg_store_n(u8* p, const float* f) {
+    if (type == SZ_TYPE_F32) {
+#pragma unroll
+        for (int e = 0; e < E; e += E == 2 ? 2 : 4) {
+            if (E == 2) *(float2*)p = make_float2(f[0], f[1]);
+            else *(float4*)(p + 4 * e) = make_float4(f[e], f[e + 1], f[(e + 2) % E], f[(e + 3) % E]);
+        }
+    } else {
+        u32 w[E / 2];
+#pragma unroll
+        for (int e = 0; e < E; e += 2) w[e / 2] = type == SZ_TYPE_F16 ? pg_pack_f16(f[e], f[e + 1]) : pg_pack_bf16(f[e], f[e + 1]);
+        if (E == 8) *(uint4*)p = *(const uint4*)w;
+        else if (E == 4) *(uint2*)p = *(const uint2*)w;
+        else *(u32*)p = w[0];
+    }
+}
+
+template <int CT, int HD, int IO, int R>
 __global__ void __launch_bounds__(256) sz_pg_append_kernel(const __grid_constant__ PgBatch d, const __grid_constant__ PgAppend a) {
-    __shared__ float2 turn[128];
-    __shared__ float tmp[8][256];
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r = blockIdx.x;
+    constexpr int E = HD / 32, ESZ = IO == SZ_TYPE_F32 ? 4 : 2, CTY = CT == PG_F16 ? SZ_TYPE_F16 : SZ_TYPE_BF16;
+    __shared__ float2 turn[R][HD / 2];
+    __shared__ float tmp[8][HD];
+    __shared__ int s_pos[R];               // the row's position; -1: the row is left out
+    __shared__ long long s_off[R];         // where it lies in the pools; -1: it is not stored
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r0 = blockIdx.x * R, half = a.half, d0 = lane * E, nq = a.q ? a.nh : 0;
+    float one[E];                               // R = 1: the warp's head, its kind (0 queries, 1 keys, 2 values) and its number there
+    const int x = blockIdx.y * 8 + warp, kind1 = x < nq ? 0 : x < nq + d.nkv ? 1 : 2, h1 = x - (kind1 == 0 ? 0 : kind1 == 1 ? nq : nq + d.nkv);
+    if ((int)threadIdx.x < R) { s_pos[threadIdx.x] = -1; s_off[threadIdx.x] = -1; }
+    __syncthreads();
     sz_pdl_wait();
     sz_pdl_trigger();
-    const int b = pg_seq_of<256>(d, r);
-    if (r == 0 && blockIdx.y == 0 && threadIdx.x == 0 && __ldg(d.row_start + d.n_seq) > d.rows) atomicOr(d.err, PG_E_ROWS);
-    if (b < 0) return;
-    const int pos = __ldg(d.lens + b) - (pg_row(d, b + 1) - r);
-    if (pos < 0) return;
-    for (int i = threadIdx.x; i < a.half; i += 256) {
-        const double f = (double)pos * a.freq[i];
+    if (R == 1 && x < a.heads)                  // its elements are under way while the row is looked up
+        pg_load_n<E, IO>((kind1 == 0 ? a.q + (long long)r0 * a.q_stride + h1 * a.q_head_stride : (kind1 == 1 ? a.k + (long long)r0 * a.k_stride : a.v + (long long)r0 * a.v_stride) + h1 * (HD * ESZ)) + d0 * ESZ, one);
+    for (int i = threadIdx.x; i < d.n_seq; i += 256) {
+        const int b0 = pg_row(d, i), b1 = pg_row(d, i + 1), len = __ldg(d.lens + i);
+        for (int row = max(b0, r0); row < min(b1, r0 + R); row++) {      // (the block's rows of this sequence)
+            const int pos = len - (b1 - row), o = pos - d.shared_len;
+            if (pos < 0) continue;
+            long long off = -1;
+            u32 bad = 0;
+            if (o < 0) bad = PG_E_SHARED;
+            else if ((long long)o >= (long long)d.max_pages << d.ps_log2) bad = PG_E_END;
+            else {
+                const int page = __ldg(d.pages + (size_t)i * d.max_pages + (o >> d.ps_log2));
+                if ((u32)page >= (u32)d.n_pages) bad = PG_E_PAGE;
+                else off = (long long)page * d.page_stride + (long long)(o & ((1 << d.ps_log2) - 1)) * d.pos_stride;
+            }
+            if (bad) atomicOr(d.err, bad);
+            s_pos[row - r0] = pos; s_off[row - r0] = off;
+        }
+    }
+    if (r0 == 0 && threadIdx.x == 0 && blockIdx.y == 0 && __ldg(d.row_start + d.n_seq) > d.rows) atomicOr(d.err, PG_E_ROWS);
+    __syncthreads();
+    for (int i = threadIdx.x; i < half * R; i += 256) {
+        const int j = i / half, k = i - j * half, pos = s_pos[j];
+        if (pos < 0) continue;
+        const double f = (double)pos * a.freq[k];
         const double kq = rint(f * 0.15915494309189535);
         double rd = fma(-kq, 6.283185307179586, f);
         rd = fma(-kq, 2.4492935982947064e-16, rd);
         const float hi = (float)rd, lo = (float)(rd - (double)hi);
         float sn, cs;
         sincosf(hi, &sn, &cs);
-        turn[i] = make_float2(fmaf(-sn, lo, cs), fmaf(cs, lo, sn));
+        turn[j][k] = make_float2(fmaf(-sn, lo, cs), fmaf(cs, lo, sn));
     }
     __syncthreads();
-    const int x = blockIdx.y * 8 + warp, nq = a.q ? a.nh : 0;
-    if (x >= a.heads) return;
-    const int kind = x < nq ? 0 : x < nq + d.nkv ? 1 : 2, h = kind == 0 ? x : (x - nq) % d.nkv;
-    u8* dst = nullptr;
-    if (kind) {                      // where the position lies
-        const int o = pos - d.shared_len;
-        if (o < 0) { if (lane == 0) atomicOr(d.err, PG_E_SHARED); return; }
-        if ((long long)o >= (long long)d.max_pages << d.ps_log2) { if (lane == 0) atomicOr(d.err, PG_E_END); return; }
-        const int page = __ldg(d.pages + (size_t)b * d.max_pages + (o >> d.ps_log2));
-        if ((u32)page >= (u32)d.n_pages) { if (lane == 0) atomicOr(d.err, PG_E_PAGE); return; }
-        dst = (u8*)(kind == 1 ? d.k : d.v) + (long long)page * d.page_stride + (long long)(o & ((1 << d.ps_log2) - 1)) * d.pos_stride + (long long)h * d.head_stride;
+    const int j = R == 1 ? 0 : warp;
+    const long long r = r0 + j, off = s_off[j];
+    if (s_pos[j] < 0) return;
+    // partners of a lane's dimensions: another lane's, where the halves are whole lanes; f' = c f + s partner, nothing turned: 1, 0
+    const bool lower = d0 < half, by_lane = half % E == 0;
+    const int partner = half ? (lower ? lane + half / E : lane - half / E) & 31 : lane;
+    float c[E], s[E];
+#pragma unroll
+    for (int e = 0; e < E; e++) {
+        const float2 t = by_lane && d0 + e < 2 * half ? turn[j][lower ? d0 + e : d0 + e - half] : make_float2(1.f, 0.f);
+        c[e] = t.x;
+        s[e] = lower ? -t.y : t.y;
     }
-    const u8* src = kind == 0 ? a.q + (long long)r * a.q_stride + (long long)h * a.q_head_stride
-                              : (kind == 1 ? a.k + (long long)r * a.k_stride : a.v + (long long)r * a.v_stride) + (long long)h * a.hd * a.esz;
-    float2 f[4] = {};
+    auto store_cache = [&](u8* dst, const float* f) {
+        if (CT != PG_Q8) { pg_store_n<E, CTY>(dst + 2 * d0, f); return; }
+        float big = 0.f;                        // packed: a group of 32 dimensions is 32 / E lanes
 #pragma unroll
-    for (int i = 0; i < 4; i++)
-        if (64 * i < a.hd) f[i] = pg_load2(src + (long long)(2 * (lane + 32 * i)) * a.esz, a.type);
-    const float* w = kind == 0 ? a.q_norm : kind == 1 ? a.k_norm : nullptr;
-    if (w) {
-        double ss = 0.0;
+        for (int e = 0; e < E; e++) big = fmaxf(big, fabsf(f[e]));
 #pragma unroll
-        for (int i = 0; i < 4; i++)
-            if (64 * i < a.hd) ss += (double)f[i].x * (double)f[i].x + (double)f[i].y * (double)f[i].y;
-        ss = sz_warp_sum(ss);
-        const double rr = sz_rsqrt64(ss / (double)a.hd + (double)a.eps);
+        for (int o = 16 / E; o > 0; o >>= 1) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, o));
+        const __half sh = __float2half_rn(big > 0.0f ? big * (1.0f / 127.0f) : 0.0f);
+        const float sr = __half2float(sh), inv = sr > 0.0f ? 1.0f / sr : 0.0f;
+        u32 code[E];
 #pragma unroll
-        for (int i = 0; i < 4; i++)
-            if (64 * i < a.hd) {
-                const float2 ww = *(const float2*)(w + 2 * (lane + 32 * i));
-                f[i] = make_float2((float)((double)f[i].x * rr) * ww.x, (float)((double)f[i].y * rr) * ww.y);
+        for (int e = 0; e < E; e++) { int q = __float2int_rn(f[e] * inv); q = q < -127 ? -127 : (q > 127 ? 127 : q); code[e] = (u32)q & 255u; }
+        if (E == 8) *(uint2*)(dst + 8 * lane) = make_uint2(code[0] | code[1] << 8 | code[2 % E] << 16 | code[3 % E] << 24, code[4 % E] | code[5 % E] << 8 | code[6 % E] << 16 | code[7 % E] << 24);
+        else if (E == 4) *(u32*)(dst + 4 * lane) = code[0] | code[1] << 8 | code[2 % E] << 16 | code[3 % E] << 24;
+        else *(u16*)(dst + 2 * lane) = (u16)(code[0] | code[1] << 8);
+        if (lane % (32 / E) == 0) *(u16*)(dst + HD + 2 * (lane * E / 32)) = __half_as_ushort(sh);
+        if (lane >= HD / 32 && lane < 8) *(u16*)(dst + HD + 2 * lane) = 0;      // the 16 bytes behind the codes: those behind the scales are zero
+    };
+    auto norm = [&](const float* f) {           // 1 / the root of the mean square
+        float ss = 0.f;
+#pragma unroll
+        for (int e = 0; e < E; e++) ss = fmaf(f[e], f[e], ss);
+        return (float)sz_rsqrt64((double)sz_warp_sum(ss) / HD + (double)a.eps);
+    };
+    auto head = [&](auto kind_, float* f, float rr, const float* w, const float* ww, u8* to) {        // scale, rotation, store of a head
+        const int kind = kind_;
+        if (kind < 2 && w) {
+#pragma unroll
+            for (int e = 0; e < E; e++) f[e] = f[e] * rr * ww[e];
+        }
+        if (kind < 2 && half) {
+            if (by_lane) {
+#pragma unroll
+                for (int e = 0; e < E; e++) {
+                    const float p = __shfl_sync(0xffffffffu, f[e], partner);
+                    f[e] = fmaf(f[e], c[e], p * s[e]);
+                }
+            } else {                            // through shared memory
+#pragma unroll
+                for (int e = 0; e < E; e++) tmp[warp][d0 + e] = f[e];
+                __syncwarp();
+                for (int i = lane; i < half; i += 32) {
+                    const float2 t2 = turn[j][i];
+                    const float u = tmp[warp][i], v = tmp[warp][i + half];
+                    tmp[warp][i] = u * t2.x - v * t2.y;
+                    tmp[warp][i + half] = v * t2.x + u * t2.y;
+                }
+                __syncwarp();
+#pragma unroll
+                for (int e = 0; e < E; e++) f[e] = tmp[warp][d0 + e];
+                __syncwarp();
             }
-    }
-    if (kind < 2 && a.half) {        // the pair (i, i + half) of a rotation lies in two lanes: through shared memory
-#pragma unroll
-        for (int i = 0; i < 4; i++)
-            if (64 * i < a.hd) *(float2*)(tmp[warp] + 2 * (lane + 32 * i)) = f[i];
-        __syncwarp();
-        for (int i = lane; i < a.half; i += 32) {
-            const float2 t = turn[i];
-            const float u = tmp[warp][i], v = tmp[warp][i + a.half];
-            tmp[warp][i] = u * t.x - v * t.y;
-            tmp[warp][i + a.half] = v * t.x + u * t.y;
         }
-        __syncwarp();
+        if (kind == 0) pg_store_n<E, IO>(to + d0 * ESZ, f);
+        else store_cache(to, f);
+    };
+    auto load_w = [&](const float* w, float* ww) {
+        if (!w) return;
 #pragma unroll
-        for (int i = 0; i < 4; i++)
-            if (64 * i < a.hd) f[i] = *(const float2*)(tmp[warp] + 2 * (lane + 32 * i));
-    }
-    if (kind == 0) {
-        u8* out = a.qo + (long long)r * a.qo_stride + (long long)h * a.hd * a.esz;
-#pragma unroll
-        for (int i = 0; i < 4; i++)
-            if (64 * i < a.hd) pg_store2(out + (long long)(2 * (lane + 32 * i)) * a.esz, a.type, f[i].x, f[i].y);
+        for (int e = 0; e < E; e += 2) { const float2 u = __ldg((const float2*)(w + d0 + e)); ww[e] = u.x; ww[e + 1] = u.y; }
+    };
+    if (R == 1) {
+        if (x >= a.heads || (kind1 && off < 0)) return;
+        const float* w = kind1 == 0 ? a.q_norm : kind1 == 1 ? a.k_norm : nullptr;
+        float ww[E];
+        load_w(w, ww);
+        head(kind1, one, w ? norm(one) : 1.f, w, ww, kind1 == 0 ? a.qo + r * a.qo_stride + h1 * (HD * ESZ) : (u8*)(kind1 == 1 ? d.k : d.v) + off + h1 * d.head_stride);
         return;
     }
-    if (CT != PG_Q8) {
+    // A warp has a row and takes its heads four at a time: their loads are under way together.
+    auto heads = [&](auto kind, int n, const u8* src, long long step, u8* dst, long long dst_step, const float* w) {
+        constexpr int B = 4;
+        src += d0 * ESZ;
+        float ww[E];
+        load_w(w, ww);
+        for (int x0 = 0; x0 < n; x0 += B, src += B * step, dst += B * dst_step) {
+            float all[B][E], rr[B];
 #pragma unroll
-        for (int i = 0; i < 4; i++)
-            if (64 * i < a.hd) *(u32*)(dst + 4 * (lane + 32 * i)) = pg_pack<CT>(f[i].x, f[i].y);
-        return;
-    }
-    // packed: a group of 32 dimensions is 16 lanes of a pair each
+            for (int t = 0; t < B; t++) pg_load_n<E, IO>(src + (x0 + t < n ? t * step : 0), all[t]);        // (behind the last: the first once more)
+            if (kind < 2 && w) {
 #pragma unroll
-    for (int i = 0; i < 4; i++)
-        if (64 * i < a.hd) {
-            float big = fmaxf(fabsf(f[i].x), fabsf(f[i].y));
+                for (int t = 0; t < B; t++) rr[t] = norm(all[t]);
+            }
 #pragma unroll
-            for (int s = 8; s > 0; s >>= 1) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, s));
-            const __half sh = __float2half_rn(big > 0.0f ? big * (1.0f / 127.0f) : 0.0f);
-            const float sr = __half2float(sh), inv = sr > 0.0f ? 1.0f / sr : 0.0f;
-            int c0 = __float2int_rn(f[i].x * inv), c1 = __float2int_rn(f[i].y * inv);
-            c0 = c0 < -127 ? -127 : (c0 > 127 ? 127 : c0);
-            c1 = c1 < -127 ? -127 : (c1 > 127 ? 127 : c1);
-            *(u16*)(dst + 2 * (lane + 32 * i)) = (u16)((c0 & 255) | (c1 & 255) << 8);
-            if ((lane & 15) == 0) *(u16*)(dst + a.hd + 2 * (2 * i + (lane >> 4))) = __half_as_ushort(sh);
+            for (int t = 0; t < B; t++)
+                if (x0 + t < n) head(kind, all[t], rr[t], w, ww, dst + t * dst_step);
         }
-    if (lane >= a.hd / 32 && lane < 8)                           // the 16 bytes behind the codes: those behind the scales are zero
-        *(u16*)(dst + a.hd + 2 * lane) = 0;
+    };
+    if (nq) heads(PgKind<0>(), nq, a.q + r * a.q_stride, a.q_head_stride, a.qo + r * a.qo_stride, HD * ESZ, a.q_norm);
+    if (off < 0) return;
+    heads(PgKind<1>(), d.nkv, a.k + r * a.k_stride, HD * ESZ, (u8*)d.k + off, d.head_stride, a.k_norm);
+    heads(PgKind<2>(), d.nkv, a.v + r * a.v_stride, HD * ESZ, (u8*)d.v + off, d.head_stride, nullptr);
 }
 
 // ---- the plan of a call with more sequences or tiles than a block plans for itself ---------------------------------------------------------
@@ -419,10 +515,20 @@ extern "C" int sz_paged_append(const sz_paged_cache* cache, const sz_paged_batch
     a.k = (const u8*)k; a.v = (const u8*)v; a.q = (const u8*)q; a.qo = (u8*)q_out;
     a.k_stride = k_stride * esz; a.v_stride = v_stride * esz; a.q_stride = q_stride * esz; a.q_head_stride = q_head_stride * esz; a.qo_stride = q_out_stride * esz;
     a.q_norm = (const float*)rope->q_norm; a.k_norm = (const float*)rope->k_norm;
-    a.type = io_type; a.esz = esz; a.hd = hd; a.nh = n_head; a.half = rope->dims / 2; a.heads = (q ? n_head : 0) + 2 * nkv; a.eps = rope->eps;
+    a.nh = n_head; a.half = rope->dims / 2; a.heads = (q ? n_head : 0) + 2 * nkv; a.eps = rope->eps;
     for (int i = 0; i < a.half; i++) a.freq[i] = 1.0 / pow(rope->theta, 2.0 * i / rope->dims);
-    const dim3 grid(batch->rows, (a.heads + 7) / 8);
-    auto* fn = cache->type == SZ_TYPE_F16 ? sz_pg_append_kernel<PG_F16> : cache->type == SZ_TYPE_BF16 ? sz_pg_append_kernel<PG_BF16> : sz_pg_append_kernel<PG_Q8>;
+    // eight rows a block where that still gives every multiprocessor one
+    const bool many = batch->rows >= 8 * PG_BLOCKS;
+    const int per = many ? PG_APP : 1;
+    const dim3 grid((batch->rows + per - 1) / per, many ? 1 : (a.heads + 7) / 8);
+    using Kernel = void (*)(PgBatch, PgAppend);
+#define SZ_PG_APP_R(CT, HD, IO) (many ? (Kernel)sz_pg_append_kernel<CT, HD, IO, PG_APP> : (Kernel)sz_pg_append_kernel<CT, HD, IO, 1>)
+#define SZ_PG_APP_IO(CT, HD) (io_type == SZ_TYPE_F32 ? SZ_PG_APP_R(CT, HD, SZ_TYPE_F32) : io_type == SZ_TYPE_F16 ? SZ_PG_APP_R(CT, HD, SZ_TYPE_F16) : SZ_PG_APP_R(CT, HD, SZ_TYPE_BF16))
+#define SZ_PG_APP(CT) (hd == 64 ? SZ_PG_APP_IO(CT, 64) : hd == 128 ? SZ_PG_APP_IO(CT, 128) : SZ_PG_APP_IO(CT, 256))
+    const Kernel fn = cache->type == SZ_TYPE_F16 ? SZ_PG_APP(PG_F16) : cache->type == SZ_TYPE_BF16 ? SZ_PG_APP(PG_BF16) : SZ_PG_APP(PG_Q8);
+#undef SZ_PG_APP_IO
+#undef SZ_PG_APP_R
+#undef SZ_PG_APP
     SZ_CUDA(sz_launch("paged_append", fn, grid, dim3(256), 0, (cudaStream_t)stream, true, d, a));
     return SZ_OK;
 }

@@ -1,4 +1,5 @@
 """A cache in pages (`sz_paged_*`): rows are appended to it and attend to it, over a prefix that the whole batch shares, too."""
+import contextlib
 import ctypes as C
 import math
 
@@ -6,6 +7,7 @@ import torch
 
 from . import lib as szlib
 
+_HERE = contextlib.nullcontext()
 TYPES = {torch.float32: szlib.TYPE_F32, torch.float16: szlib.TYPE_F16, torch.bfloat16: szlib.TYPE_BF16}
 
 
@@ -44,6 +46,8 @@ class Cache:
         if k.stride(3) != 1 or k.shape[3] != (head_bytes(head_dim) if packed else head_dim):
             raise ValueError("a head is %d contiguous elements" % (head_bytes(head_dim) if packed else head_dim))
         self.k, self.v, self.device, self.head_dim = k, v, k.device, head_dim
+        if any(n > 1 and st < k.shape[3] for n, st in zip(k.shape, k.stride()[:3])):
+            raise ValueError("pools whose heads overlap")
         e = k.element_size()
         self.c = PagedCacheC(type=szlib.TYPE_Q8_KV if packed else TYPES[k.dtype], n_kv_head=k.shape[1], head_dim=head_dim, page_size=k.shape[2], n_pages=k.shape[0],
                              k=k.data_ptr(), v=v.data_ptr(), page_stride=max(k.stride(0) * e, k.shape[3] * e), head_stride=k.stride(1) * e, pos_stride=k.stride(2) * e)
@@ -66,6 +70,7 @@ class Step:
         if shared_len and shared_pages.shape[0] * cache.c.page_size < shared_len:
             raise ValueError("shared_pages hold %d positions, shared_len is %d" % (shared_pages.shape[0] * cache.c.page_size, shared_len))
         self.cache, self.n_head, self.rows, self.device = cache, n_head, rows, cache.device
+        self.nkv, self._scale = cache.c.n_kv_head, 1 / math.sqrt(cache.head_dim)
         self._keep = (pages, row_start, lens, shared_pages)
         self.b = PagedBatchC(n_seq=n, rows=rows, max_pages=pages.shape[1], shared_len=shared_len, pages=pages.data_ptr(), row_start=row_start.data_ptr(),
                              lens=lens.data_ptr(), shared_pages=shared_pages.data_ptr() if shared_len else 0)
@@ -76,67 +81,92 @@ class Step:
             self._mem = torch.empty(need.value + 256, dtype=torch.uint8, device=self.device)
             self.scratch, self.scratch_bytes = self._mem.data_ptr() + (-self._mem.data_ptr()) % 256, need.value
             szlib.check(self.lib.sz_paged_status(self.scratch, 1, None, self._stream()))
-        self._rope = {}
+
+    def _here(self):
+        """Makes the cache's device the current one, where another is."""
+        return _HERE if torch.cuda.current_device() == self.device.index else torch.cuda.device(self.device)
 
     def _stream(self):
         return torch.cuda.current_stream(self.device).cuda_stream
 
-    def _rows(self, name, t, heads, dtype=None):
-        if t.dim() != 3 or t.shape[0] != self.rows or t.shape[1] != heads or t.shape[2] != self.cache.head_dim or t.stride(2) != 1 or t.device != self.device:
-            raise ValueError("%s: [%d, %d, %d], the last dimension contiguous, on the cache's device" % (name, self.rows, heads, self.cache.head_dim))
+    def _rows(self, name, t, heads, dtype=None, apart=False):
+        """Checks [rows, heads, head_dim]; returns its address and its strides of rows and (apart: any) heads."""
+        hd = self.cache.head_dim
+        if t.shape != (self.rows, heads, hd) or t.device != self.device:
+            raise ValueError("%s: [%d, %d, %d] on the cache's device" % (name, self.rows, heads, hd))
         if t.dtype not in TYPES or (dtype is not None and t.dtype != dtype):
             raise ValueError("%s: float32, float16 or bfloat16, the same for all rows of a call" % name)
-        return t
+        row, head, one = t.stride()
+        if one != 1:
+            raise ValueError("%s: the last dimension contiguous" % name)
+        if heads == 1:
+            head = hd
+        elif head != hd and (not apart or head < hd):
+            raise ValueError("%s: heads %s" % (name, "that overlap" if apart else "side by side"))
+        need = (heads - 1) * head + hd
+        if row < need:
+            if self.rows > 1:
+                raise ValueError("%s: rows that overlap" % name)
+            row = need
+        return t.data_ptr(), row, head
 
     def append(self, k, v, q=None, q_out=None, rope_dims=0, theta=1e4, q_norm=None, k_norm=None, eps=1e-6):
         """Stores the rows' keys (normed, turned) and values at their positions; returns the rows' queries, normed and turned (None without q).
         k, v [rows, kv heads, head_dim]; q [rows, heads, head_dim] (any stride of heads); q_norm, k_norm float32 [head_dim]."""
-        nkv = self.cache.c.n_kv_head
-        self._rows("k", k, nkv), self._rows("v", v, nkv, k.dtype)
-        hd = self.cache.head_dim
+        hd, nkv, dt = self.cache.head_dim, self.nkv, k.dtype
+        kp, ks, _ = self._rows("k", k, nkv)
+        vp, vs, _ = self._rows("v", v, nkv, dt)
+        qp = qs = qh = op = os = qn = kn = 0
         if q is not None:
-            self._rows("q", q, self.n_head, k.dtype)
+            qp, qs, qh = self._rows("q", q, self.n_head, dt, True)
             if q_out is None:
-                q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-            self._rows("q_out", q_out, self.n_head, k.dtype)
-        for name, t in (("k", k), ("v", v)) + ((("q_out", q_out),) if q is not None else ()):
-            if t.shape[1] > 1 and t.stride(1) != hd:
-                raise ValueError("%s: heads side by side" % name)
-        for w in (q_norm, k_norm):
-            if w is not None and (w.dtype != torch.float32 or w.shape != (hd,) or w.stride(0) != 1 or w.device != self.device):
-                raise ValueError("norm weights: float32 [%d] on the cache's device" % hd)
-        rope = PagedRopeC(rope_dims, eps, theta, 0 if q_norm is None else q_norm.data_ptr(), 0 if k_norm is None else k_norm.data_ptr())
-        with torch.cuda.device(self.device):
-            szlib.check(self.lib.sz_paged_append(self._c, self._b, C.byref(rope), TYPES[k.dtype], self.n_head, k.data_ptr(), k.stride(0), v.data_ptr(), v.stride(0),
-                                                 0 if q is None else q.data_ptr(), 0 if q is None else q.stride(0), 0 if q is None else max(q.stride(1), hd),
-                                                 0 if q is None else q_out.data_ptr(), 0 if q is None else q_out.stride(0), self.scratch, self.scratch_bytes, self._stream()))
+                q_out = torch.empty(q.shape, dtype=dt, device=q.device)
+            op, os, _ = self._rows("q_out", q_out, self.n_head, dt)
+        elif q_out is not None:
+            raise ValueError("q_out without q")
+        if q_norm is not None:
+            qn = self._norm(q_norm, hd)
+        if k_norm is not None:
+            kn = self._norm(k_norm, hd)
+        rope = PagedRopeC(rope_dims, eps, theta, qn, kn)
+        with self._here():
+            rc = self.lib.sz_paged_append(self._c, self._b, C.byref(rope), TYPES[dt], self.n_head, kp, ks, vp, vs, qp, qs, qh, op, os, self.scratch, self.scratch_bytes,
+                                          self._stream())
+        if rc:
+            szlib.check(rc)
         return q_out
+
+    def _norm(self, w, hd):
+        if w.dtype != torch.float32 or w.shape != (hd,) or w.stride(0) != 1 or w.device != self.device:
+            raise ValueError("norm weights: float32 [%d] on the cache's device" % hd)
+        return w.data_ptr()
 
     def attend(self, q, out=None, scale=None, gate=None, lse=None):
         """Attention of the rows over their sequences' positions up to their own, shared ones first.  q [rows, heads, head_dim]; gate: the
         same (any stride of heads), out *= sigmoid(gate); lse float32 [rows, heads] receives the logarithm of the softmax's denominator; scale 1 / sqrt(head_dim)."""
-        hd = self.cache.head_dim
-        self._rows("q", q, self.n_head)
+        qp, qs, _ = self._rows("q", q, self.n_head)
+        dt = q.dtype
         if out is None:
-            out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-        self._rows("out", out, self.n_head, q.dtype)
-        for name, t in (("q", q), ("out", out)):
-            if t.shape[1] > 1 and t.stride(1) != hd:
-                raise ValueError("%s: heads side by side" % name)
+            out = torch.empty(q.shape, dtype=dt, device=q.device)
+        op, os, _ = self._rows("out", out, self.n_head, dt)
+        gp = gs = gh = lp = 0
         if gate is not None:
-            self._rows("gate", gate, self.n_head, q.dtype)
-        if lse is not None and (lse.dtype != torch.float32 or lse.shape != (self.rows, self.n_head) or not lse.is_contiguous() or lse.device != self.device):
-            raise ValueError("lse: float32 [%d, %d] on the cache's device" % (self.rows, self.n_head))
-        with torch.cuda.device(self.device):
-            szlib.check(self.lib.sz_paged_attend(self._c, self._b, TYPES[q.dtype], self.n_head, 1 / math.sqrt(hd) if scale is None else scale, q.data_ptr(), q.stride(0),
-                                                 0 if gate is None else gate.data_ptr(), 0 if gate is None else gate.stride(0), 0 if gate is None else max(gate.stride(1), hd),
-                                                 out.data_ptr(), out.stride(0), 0 if lse is None else lse.data_ptr(), self.scratch, self.scratch_bytes, self._stream()))
+            gp, gs, gh = self._rows("gate", gate, self.n_head, dt, True)
+        if lse is not None:
+            if lse.dtype != torch.float32 or lse.shape != (self.rows, self.n_head) or not lse.is_contiguous() or lse.device != self.device:
+                raise ValueError("lse: float32 [%d, %d] on the cache's device" % (self.rows, self.n_head))
+            lp = lse.data_ptr()
+        with self._here():
+            rc = self.lib.sz_paged_attend(self._c, self._b, TYPES[dt], self.n_head, self._scale if scale is None else scale, qp, qs, gp, gs, gh, op, os, lp, self.scratch,
+                                          self.scratch_bytes, self._stream())
+        if rc:
+            szlib.check(rc)
         return out
 
     def status(self):
         """What the calls so far have met (synchronises): 0, or the bits of sz_paged_status."""
         code = C.c_int()
-        with torch.cuda.device(self.device):
+        with self._here():
             rc = self.lib.sz_paged_status(self.scratch, 0, C.byref(code), self._stream())
         if rc not in (szlib.OK, szlib.E_DEVICE):
             szlib.check(rc)

@@ -3,7 +3,7 @@ for many rows at once, every row with settings of its own, from uniform numbers 
 import torch
 
 from . import lib as szlib
-from .paged import TYPES
+from .paged import _HERE, TYPES
 
 
 def sample_rows(logits, uniform, temperature=None, top_k=None, top_p=None, min_p=None, out=None, prob=None):
@@ -13,15 +13,29 @@ def sample_rows(logits, uniform, temperature=None, top_k=None, top_p=None, min_p
     L = szlib.load()
     if logits.dim() != 2 or logits.dtype not in TYPES or (logits.shape[1] > 1 and logits.stride(1) != 1):
         raise ValueError("logits: [rows, vocab] of float32, float16 or bfloat16, rows contiguous")
-    rows, dev = logits.shape[0], logits.device
+    (rows, vocab), stride, dev = logits.shape, logits.stride(0), logits.device
+    if stride < vocab:
+        if rows > 1:
+            raise ValueError("logits: rows that overlap")
+        stride = vocab
     if out is None:
         out = torch.empty(rows, dtype=torch.int32, device=dev)
-    for name, t, dt in (("uniform", uniform, torch.float64), ("temperature", temperature, torch.float32), ("top_k", top_k, torch.int32), ("top_p", top_p, torch.float32),
-                        ("min_p", min_p, torch.float32), ("out", out, torch.int32), ("prob", prob, torch.float32)):
-        if t is not None and (t.dtype != dt or t.shape != (rows,) or not t.is_contiguous() or t.device != dev):
+    of = (rows,)
+
+    def at(name, t, dt):
+        if t is None:
+            return 0
+        if t.dtype != dt or t.shape != of or t.device != dev or not t.is_contiguous():
             raise ValueError("%s: %s [%d] on the logits' device" % (name, dt, rows))
-    p = lambda t: 0 if t is None else t.data_ptr()  # noqa: E731
-    with torch.cuda.device(dev):
-        szlib.check(L.sz_sample_rows(TYPES[logits.dtype], logits.data_ptr(), max(logits.stride(0), logits.shape[1]), rows, logits.shape[1], p(temperature), p(top_k),
-                                     p(top_p), p(min_p), uniform.data_ptr(), out.data_ptr(), p(prob), torch.cuda.current_stream(dev).cuda_stream))
+        return t.data_ptr()
+
+    if uniform is None:
+        raise ValueError("uniform: a number in [0, 1) a row")
+    f32 = torch.float32
+    ptrs = (at("temperature", temperature, f32), at("top_k", top_k, torch.int32), at("top_p", top_p, f32), at("min_p", min_p, f32), at("uniform", uniform, torch.float64),
+            at("out", out, torch.int32), at("prob", prob, f32))
+    with _HERE if torch.cuda.current_device() == dev.index else torch.cuda.device(dev):
+        rc = L.sz_sample_rows(TYPES[logits.dtype], logits.data_ptr(), stride, rows, vocab, *ptrs, torch.cuda.current_stream(dev).cuda_stream)
+    if rc:
+        szlib.check(rc)
     return out

@@ -470,6 +470,13 @@ def test_append_pages_and_layouts(page, layout):
     check_append(Case([300, 17, page + 1], [2, 1, 4], page=page, layout=layout, io="bf16", cache="q8", hd=128, seed=page, pad=3), 128, False)
 
 
+@pytest.mark.parametrize("io,cache", [("bf16", "bf16"), ("f32", "q8")])
+def test_append_many_rows(io, cache):
+    """Blocks of several rows, rows of several sequences in one, none among them, and rows that are left out."""
+    check_append(Case([1500, 3, 40, 0, 5, 90], [1401, 1, 17, 0, 9, 2], nh=4, nkv=2, hd=128, io=io, cache=cache, seed=9, pad=5), 64, True)
+    check_append(Case([1 + i for i in range(1210)], [1] * 1210, nh=2, nkv=1, hd=64, io=io, cache=cache, seed=10, page=8), 32, True)
+
+
 def test_append_behind_a_shared_prefix_and_without_queries():
     check_append(Case([70, 101], [2, 37], shared=64, page=16, seed=21), 32, True)
     check_append(Case([70, 101], [2, 37], page=16, seed=22), 32, True, with_q=False)
@@ -562,3 +569,23 @@ def test_steps_as_a_server_makes_them():
                     # keys that round to the other f16 neighbour: 2^-11 of a key here and there; scores move by 2^-11 |q| at most
                     assert float((out[r + j, h].double() - w @ V).abs().max()) < 2.0 ** -11 * float(qw[j, h].norm()) * float(w @ V.abs().amax(-1)) + 1e-4
             r += m
+
+
+def test_rows_that_overlap_are_refused():
+    """Expanded rows or heads have strides that the kernels do not take; one row or one head has any."""
+    c = Case([9, 33], [2, 5], nh=4, nkv=2, hd=64, io="bf16", cache="bf16", seed=90)
+    kv, q = c.rnd(c.rows, 2, 64).to(c.io), c.q
+    for bad in (kv[:1].expand(7, 2, 64), kv[:, :1].expand(7, 2, 64)):
+        with pytest.raises(ValueError):
+            c.step.append(bad, kv)
+        with pytest.raises(ValueError):
+            c.step.append(kv, bad)
+    for bad in (q[:1].expand(7, 4, 64), q[:, :1].expand(7, 4, 64)):
+        for call in (lambda: c.step.append(kv, kv, q=bad), lambda: c.step.attend(bad), lambda: c.step.attend(q, gate=bad), lambda: c.step.attend(q, out=bad)):
+            with pytest.raises(ValueError):
+                call()
+    with pytest.raises(ValueError):
+        c.step.append(kv, kv, q_out=q)
+    c = Case([33], [1], nh=2, nkv=1, hd=64, io="bf16", cache="bf16", seed=91)
+    want = c.step.attend(c.q)
+    assert torch.equal(c.step.attend(c.q.expand(1, 2, 64).as_strided((1, 2, 64), (0, 64, 1))), want)

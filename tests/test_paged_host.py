@@ -120,3 +120,15 @@ def test_the_python_side_checks_shapes():
             sampling.sample_rows(lg, **kw)
     with pytest.raises(ValueError):
         sampling.sample_rows(lg.double(), torch.zeros(3, dtype=torch.float64))
+
+
+def test_the_python_side_refuses_overlapping_rows():
+    """A stride below a row's own size (an expanded tensor) would be read at other places than the tensor has."""
+    one = torch.zeros(1, 2, 16, 64, dtype=torch.bfloat16)
+    for bad in (one.expand(4, 2, 16, 64), one[:, :1].expand(1, 2, 16, 64), one[:, :, :1].expand(1, 2, 16, 64)):
+        with pytest.raises(ValueError):
+            paged.Cache(bad, bad, 64)
+    u = torch.zeros(3, dtype=torch.float64)
+    for bad in (torch.zeros(1, 10).expand(3, 10), torch.zeros(12).as_strided((3, 10), (1, 1)), torch.zeros(3, 1).expand(3, 10)):
+        with pytest.raises(ValueError):
+            sampling.sample_rows(bad, u)
