@@ -11,18 +11,26 @@
 // Sums are integers: exact whatever the order of the atomics, so the token depends on nothing but the inputs.  f32 would not do: between two of
 // 150,000 candidates lie 10^-5 of the sum or less, and an error of 10^-8 at every border moves a draw in a thousand.  A candidate in bin b weighs
 // e^(-b width) (1 + r), r = e^d - 1, d = x + b width: x and b width are f32 numbers close to each other, so d is exact; r is d itself
-// plus d^2 / 2 + .. <= 5 10^-5, which f32 holds to 10^-11.  A bin's sum of r in units of 2^-36 and its count then give its weight in f64, in units of
+// plus d^2 / 2 + .. <= 5 10^-5, which f32 holds to 10^-11 (a unit's half is 10^-10 of a weight, and those of a bin's members cancel).  A bin's sum of r in units of 2^-32 and its count then give its weight in f64, in units of
 // 2^-45 (2^18 candidates stay below 2^63); the listed candidates' weights are f64 exponentials.
 //
-// A row is a cluster of blocks, each with its part of the row in shared memory: logits are read from memory once.  What bounds it: with few rows
-// the chain of steps (load, maximum, sums, scan, gather, rank; a cluster barrier between), with many the sums' pass over all candidates.
+// A row is a cluster of 1 to 8 blocks, each with its part of the row, in shared memory where two blocks fit so.  What bounds it: with few rows
+// the chain of steps (load, maximum, sums, scan, gather, order; a cluster barrier between), with many the sums' instructions - 28 and two
+// atomics in shared memory an element - and the passes of the rows that ask for several elements.  Rows of 151,936, chat settings: 1 row 13.4 us;
+// 64 rows of mixed settings, f32, 51 us (39 MB: 6 us of them); 250 rows of bf16 drawn from whole, 93 us (76 MB: 12 us of them).
 #include "sz_common.cuh"
+
+#include <cuda_bf16.h>
 
 #include <math.h>
 
 namespace {
 
 constexpr int SA_BINS = 1024, SA_LIST = 1024, SA_NTH = 512, SA_MAX_VOCAB = 1 << 18, SA_ID = 18, SA_FEW = 512;
+constexpr int SA_RANK = 256;                                   // keys that are put in order by counting (at most SA_NTH)
+constexpr int SA_PLACES = 2 * 148;                             // blocks that run at once
+constexpr double SA_FIXED = 40000;                             // a block's time beside its part of the row, in elements of it
+constexpr size_t SA_KEEP = 113 * 1024;                         // shared memory of a block, two a multiprocessor
 constexpr float SA_CUT = 18.0f, SA_W = 37.0f / 2048;           // a bin's width: its multiples are exact, and SA_CUT is 997 of them
 constexpr double SA_ONE = 35184372088832.0;                    // 2^45: the weight 1
 static_assert(SA_BINS == 2 * SA_NTH, "a thread scans two bins");
@@ -31,6 +39,7 @@ struct SaArgs {
     const u8* logits;
     long long stride;                // bytes
     int rows, vocab, per, C;         // per: elements of a block's part; C: blocks a row
+    int keep;                        // the part stays in shared memory (0: it is read again, from L2)
     const float *temperature, *top_p, *min_p;
     const int32_t* top_k;
     const double* uniform;
@@ -48,22 +57,22 @@ struct SaCtrl {
     u64 prefix;
 };
 struct SaSmem {
-    union {
-        struct { u32 lo[SA_BINS], hi[SA_BINS]; } h;      // a bin's sums of this block (sa_add)
-        u64 sorted[SA_LIST];                              // block 0, later: the list in order
-    };
-    u64 list[SA_LIST];               // keys of the gathered
+    struct { u32 lo[SA_BINS + 32], hi[SA_BINS + 32]; } h;      // a bin's sums of this block (sa_term); behind them those of no candidates, a lane each
+    u64 list[SA_LIST];               // block 0: keys of the gathered, then in order
     u64 cum[SA_LIST + 1];            // weight of the sorted list before i
     u64 gmass[SA_BINS + 1];          // block 0: weights before bin b, of the whole row
     u32 gcnt[SA_BINS + 1];
     float top[8 * SA_NTH / 32];      // the largest of every warp of every block
     u32 redi[SA_NTH / 32];
     u64 redm[SA_NTH / 32];
+    uint4 edge[2];                   // the part's first and last 16 bytes, where they are not all its own
     u32 top_id, above;               // this block's lowest id of the largest; block 0: candidates with a weight of min_p and more
     SaCtrl c;
     u32 n;                           // the list's length
     int at;                          // found by a search
 };
+
+constexpr size_t SA_SMEM = (sizeof(SaSmem) + 15) & ~(size_t)15;
 
 __device__ __forceinline__ u32 sa_at(const void* p, int rank) {
     u32 a;
@@ -91,20 +100,54 @@ __device__ __forceinline__ float sa_x(const SaRow& R, float v) { return (v - R.m
 __device__ __forceinline__ int sa_bin(float x, float& d) {
     const float t = fmaf(x, -1.0f / SA_W, 12582912.0f);          // + 1.5 * 2^23: the integer nearest, in the low bits
     d = fmaf(t - 12582912.0f, SA_W, x);
-    return (int)(__float_as_uint(t) & (SA_BINS - 1));
+    return (int)(__float_as_uint(t) - 0x4b400000u);
 }
-// A bin's sums: members, and e^d - 1 of each in units of 2^-36, 2^30 added so that it is positive: below 2^31, and 2^46 for the 2^15 members a
-// block can have; count and the sum's upper half share a word.  (One 64-bit atomic in shared memory costs five times these two.)
-__device__ __forceinline__ void sa_add(SaSmem* S, int b, float d) {
-    const float q = d * d * fmaf(fmaf(fmaf(d, 1.0f / 120, 1.0f / 24), d, 1.0f / 6), d, 0.5f);
-    // (q below 2^22 units: the integer nearest is in the low bits of the sum with 1.5 * 2^23)
-    const u32 r = (u32)__float2int_rn(d * 68719476736.0f) + __float_as_uint(fmaf(q, 68719476736.0f, 12582912.0f)) + ((1u << 30) - 0x4b400000u);
-    const u32 old = atomicAdd(&S->h.lo[b], r);
-    atomicAdd(&S->h.hi[b], 65536u + (old + r < old));
+// A bin's sums: members, and e^d - 1 of each in units of 2^-32, 2^26 added so that it is positive: below 2^27, and 2^45 for the 2^18 members a
+// block can have; count and the sum's upper 13 bits share a word.  (One 64-bit atomic in shared memory costs five times these two.)
+__device__ __forceinline__ u32 sa_term(float d) {
+    constexpr float U = 4294967296.0f;
+    // (d^2 / 2 + .. is below 2^18 units: the integer nearest is in the low bits of the sum with 1.5 * 2^23; d^5 / 120 is below 2^-40)
+    const float q = fmaf(d * d, fmaf(fmaf(d, U / 24, U / 6), d, U / 2), 12582912.0f);
+    return (u32)__float2int_rn(d * U) + __float_as_uint(q) + ((1u << 26) - 0x4b400000u);
 }
+constexpr u32 SA_MEMBER = 1u << 13;
 __device__ __forceinline__ u64 sa_weight(const SaRow& R, float v) { return (u64)__double2ull_rn(exp((double)sa_x(R, v)) * SA_ONE); }
 
-// 16 bytes as their 4 or 8 values, NaN as -inf
+// The first n keys of the list in order, by all threads.  Up to SA_RANK each one's place is counted (through `other`): 128 keys 0.7 us, 1,024 would be 17.
+// More are compared and exchanged in pairs (a bitonic network; pairs up to 32 apart lie in one warp's 64 keys): 128 keys 2.5 us, 1,024 4.
+__device__ void sa_sort(u64* list, u64* other, u32 n, int tid) {
+    if (n <= (u32)SA_RANK) {
+        if (tid < (int)n) {
+            const u64 key = list[tid];
+            int at = 0;
+#pragma unroll 8
+            for (u32 j = 0; j < n; j++) at += list[j] < key;
+            other[at] = key;
+        }
+        __syncthreads();
+        if (tid < (int)n) list[tid] = other[tid];
+        __syncthreads();
+        return;
+    }
+    u32 m = 2;
+    while (m < n) m *= 2;
+    for (u32 i = n + tid; i < m; i += SA_NTH) list[i] = ~0ull;
+    __syncthreads();
+#pragma unroll 1
+    for (u32 k = 2; k <= m; k *= 2)
+#pragma unroll 1
+        for (u32 j = k / 2; j; j /= 2) {
+            const u32 i = 2 * tid - (tid & (j - 1));
+            if (i + j < m) {
+                const u64 a = list[i], b = list[i + j];
+                if ((a > b) == !(i & k)) { list[i] = b; list[i + j] = a; }
+            }
+            if (j > 32 || (j == 1 && k >= 64)) __syncthreads(); else __syncwarp();
+        }
+    __syncthreads();
+}
+
+// 16 bytes as their 4 or 8 values (NaN is below every one: no comparison holds)
 template <int TYPE> struct SaVec { static constexpr int E = TYPE == SZ_TYPE_F32 ? 4 : 8, ESZ = 16 / E; };
 template <int TYPE>
 __device__ __forceinline__ void sa_spread(uint4 w, float* v) {
@@ -115,8 +158,14 @@ __device__ __forceinline__ void sa_spread(uint4 w, float* v) {
         else if (TYPE == SZ_TYPE_F16) { const float2 f = __half22float2(*(const __half2*)&x[i]); v[2 * i] = f.x; v[2 * i + 1] = f.y; }
         else { v[2 * i] = __uint_as_float(x[i] << 16); v[2 * i + 1] = __uint_as_float(x[i] & 0xffff0000u); }
     }
-#pragma unroll
-    for (int i = 0; i < SaVec<TYPE>::E; i++) v[i] = v[i] != v[i] ? -INFINITY : v[i];
+}
+// The larger of two in every place, a number before NaN; the largest of a word's or a pair's
+template <int TYPE>
+__device__ __forceinline__ u32 sa_max2(u32 a, u32 b) {
+    if (TYPE == SZ_TYPE_F32) return __float_as_uint(fmaxf(__uint_as_float(a), __uint_as_float(b)));
+    if (TYPE == SZ_TYPE_F16) { const __half2 m = __hmax2(*(const __half2*)&a, *(const __half2*)&b); return *(const u32*)&m; }
+    const __nv_bfloat162 m = __hmax2(*(const __nv_bfloat162*)&a, *(const __nv_bfloat162*)&b);
+    return *(const u32*)&m;
 }
 template <int TYPE> __device__ __forceinline__ u32 sa_none() { return TYPE == SZ_TYPE_F32 ? 0xff800000u : TYPE == SZ_TYPE_F16 ? 0xfc00u : 0xff80u; }      // -inf
 
@@ -127,45 +176,50 @@ __global__ void __launch_bounds__(SA_NTH, 2) sz_sample_kernel(const __grid_const
     constexpr int E = SaVec<TYPE>::E, ESZ = SaVec<TYPE>::ESZ;
     extern __shared__ __align__(16) u8 smem[];
     SaSmem* const S = (SaSmem*)smem;
-    uint4* const val = (uint4*)(smem + ((sizeof(SaSmem) + 15) & ~(size_t)15));
+    uint4* const val = (uint4*)(smem + SA_SMEM);
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int row = blockIdx.x / a.C, rank = blockIdx.x % a.C;
-    const int i0 = rank * a.per, n = max(0, min(a.per, a.vocab - i0)), units = (n + E - 1) / E;
+    const int i0 = rank * a.per, n = max(0, min(a.per, a.vocab - i0));
+    // the part in units of 16 aligned bytes: w0 .. w1 - 1 are all its own; element 0 is element `skew` of unit 0
+    const u8* const p0 = a.logits + (long long)row * a.stride + (long long)i0 * ESZ;
+    const int skew = (int)((u64)p0 & 15) / ESZ, units = n ? (n + skew + E - 1) / E : 0, w0 = skew ? 1 : 0, w1 = max(w0, (n + skew) / E);
+    const uint4* const p = (const uint4*)(p0 - skew * ESZ);
     if (a.C > 1) sz_cluster_arrive();
     sz_pdl_wait();
     sz_pdl_trigger();
     // ---- the part of the row, its largest (thread t has units t, t + 512 .. throughout)
-    float big = -INFINITY;
+    u32 big = TYPE == SZ_TYPE_F32 ? 0xff800000u : sa_none<TYPE>() * 65537u;        // the type's values side by side
     {
-        const u8* p = a.logits + (long long)row * a.stride + (long long)i0 * ESZ;
-        const int whole = ((u64)p & 15) == 0 ? n / E : 0;
-#pragma unroll 5
-        for (int u = tid; u < whole; u += SA_NTH) {
-            const uint4 w = __ldg((const uint4*)p + u);
-            float v[E];
-            val[u] = w;
-            sa_spread<TYPE>(w, v);
-#pragma unroll
-            for (int k = 0; k < E; k++) big = fmaxf(big, v[k]);
+        const int first = w0 + (tid - w0 % SA_NTH + SA_NTH) % SA_NTH;
+#pragma unroll 8
+        for (int u = first; u < w1; u += SA_NTH) {
+            const uint4 w = __ldg(p + u);
+            if (a.keep) val[u] = w;
+            big = sa_max2<TYPE>(sa_max2<TYPE>(big, sa_max2<TYPE>(w.x, w.y)), sa_max2<TYPE>(w.z, w.w));
         }
-        for (int u = whole + tid - whole % SA_NTH; u < units; u += SA_NTH) {      // the last unit, or a row that does not begin on 16 bytes
-            if (u < whole) continue;
+#pragma unroll 1
+        for (int side = 0; side < 2; side++) {                       // the first and the last
+            const int u = side ? w1 : 0;
+            if (tid != u % SA_NTH || u >= units || (!side && !w0)) continue;
             u32 w[4] = {};
 #pragma unroll
             for (int k = 0; k < E; k++) {
-                const int i = u * E + k;
-                const u32 x = i >= n ? sa_none<TYPE>() : TYPE == SZ_TYPE_F32 ? __ldg((const u32*)p + i) : (u32)__ldg((const u16*)p + i);
+                const int i = u * E + k - skew;
+                const u32 x = i < 0 || i >= n ? sa_none<TYPE>() : TYPE == SZ_TYPE_F32 ? __ldg((const u32*)p0 + i) : (u32)__ldg((const u16*)p0 + i);
                 w[k * ESZ / 4] |= TYPE == SZ_TYPE_F32 ? x : x << (16 * (k & 1));
             }
             const uint4 q = make_uint4(w[0], w[1], w[2], w[3]);
-            float v[E];
-            val[u] = q;
-            sa_spread<TYPE>(q, v);
-#pragma unroll
-            for (int k = 0; k < E; k++) big = fmaxf(big, v[k]);
+            if (a.keep) val[u] = q;
+            else S->edge[side] = q;
+            big = sa_max2<TYPE>(sa_max2<TYPE>(big, sa_max2<TYPE>(w[0], w[1])), sa_max2<TYPE>(w[2], w[3]));
         }
     }
-    const float mine = big;
+    float mine;
+    {
+        float v[8];
+        sa_spread<TYPE>(make_uint4(big, big, big, big), v);
+        mine = fmaxf(v[0], v[1]);
+    }
     const float T = a.temperature ? __ldg(a.temperature + row) : 1.f, min_p = a.min_p ? __ldg(a.min_p + row) : 0.f, top_p = a.top_p ? __ldg(a.top_p + row) : 1.f;
     const int top_k = a.top_k ? max(__ldg(a.top_k + row), 1) : 0x7fffffff;
     const double u01 = __ldg(a.uniform + row);
@@ -188,19 +242,30 @@ __global__ void __launch_bounds__(SA_NTH, 2) sz_sample_kernel(const __grid_const
         R.max = m;
     }
     R.inv_t = 1.0f / T;
-    R.cut = R.max - SA_CUT * T;
-    auto each = [&](auto f) {                                        // f(value, id) of the block's elements
+    // The least candidate: v >= max - 18 T in f32, a difference that does not overflow, and - where the logits' own steps are wider than T - no
+    // float behind it that the rounding let in
+    R.cut = fmaxf(R.max - SA_CUT * T, R.max - 3.402823466e38f);
+    if (!(sa_x(R, R.cut) >= -18.25f)) R.cut = nextafterf(R.cut, INFINITY);
+    auto each = [&](auto f) {                                        // f(E values, the first's id) of the thread's units
+        const uint4* const at = a.keep ? val : p;
+        const int v0 = a.keep ? 0 : w0, v1 = a.keep ? units : w1;
+        auto unit = [&](int u) { return *(u >= v0 && u < v1 ? at + u : &S->edge[u >= v1]); };
+        uint4 next = tid < units ? unit(tid) : make_uint4(0u, 0u, 0u, 0u);
 #pragma unroll 1
         for (int u = tid; u < units; u += SA_NTH) {
+            const uint4 w = next;
+            if (u + SA_NTH < units) next = unit(u + SA_NTH);
             float v[E];
-            sa_spread<TYPE>(val[u], v);
-#pragma unroll
-            for (int k = 0; k < E; k++) f(v[k], (u32)(i0 + u * E + k));
+            sa_spread<TYPE>(w, v);
+            f(v, (u32)(i0 + u * E - skew));
         }
     };
     if (!(T > 0.f) || isinf(R.inv_t) || isinf(R.max)) {             // the best token (no finite largest: the lowest id that has it)
         u32 id = 0xffffffffu;
-        each([&](float v, u32 i) { if (v == R.max && i < (u32)a.vocab) id = min(id, i); });
+        each([&](const float* v, u32 i) {
+#pragma unroll
+            for (int k = 0; k < E; k++) if ((v[k] == R.max || R.max == -INFINITY) && i + k < (u32)a.vocab) id = min(id, i + k);
+        });
         id = __reduce_min_sync(0xffffffffu, id);
         if (lane == 0) atomicMin(&S->top_id, id);
         sa_sync(a.C);
@@ -214,9 +279,6 @@ __global__ void __launch_bounds__(SA_NTH, 2) sz_sample_kernel(const __grid_const
     }
     // e^x >= min_p where x >= log min_p: the least float that is
     R.floor_x = min_p > 0.f ? __double2float_ru(log((double)min_p)) : min_p <= 0.f ? -INFINITY : INFINITY;
-    // (x far below the cut: a difference that overflowed, weight 0)
-    auto there = [&](float v, float x) { return v >= R.cut && x >= -18.25f; };
-
     // With a small top_k the bins of the threads' largest elements say as much as all elements': k of them above a line are k elements above it.
     bool few = top_k <= SA_FEW;
     SaCtrl c;
@@ -232,13 +294,23 @@ __global__ void __launch_bounds__(SA_NTH, 2) sz_sample_kernel(const __grid_const
     for (;;) {
         // ---- all blocks
         if (c.cmd == SA_GATHER) {
-            const float lo = -((float)c.bin1 + 0.75f) * SA_W, hi = -((float)c.bin0 - 0.75f) * SA_W;
-            each([&](float v, u32 i) {
-                const float x = sa_x(R, v);
-                if (x >= lo && x <= hi && there(v, x)) {
+            // those near the bins by |v - mid| <= half, a little wider than they are, then by their bins
+            const float lo = fmaxf(R.max - ((float)c.bin1 + 0.75f) * SA_W * T, R.cut), hi = fminf(R.max - ((float)c.bin0 - 0.75f) * SA_W * T, R.max);
+            const float mid = 0.5f * lo + 0.5f * hi, half = (0.5f * hi - 0.5f * lo) * 1.00001f + fmaxf(fabsf(lo), fabsf(hi)) * 1e-6f;
+            each([&](const float* v, u32 i) {
+                u32 hits = 0;
+#pragma unroll
+                for (int k = 0; k < E; k++) hits |= fabsf(v[k] - mid) <= half ? 1u << k : 0u;
+                while (hits) {
+                    const int k = __ffs(hits) - 1;
+                    hits &= hits - 1;
+                    float vk = v[0];
+#pragma unroll
+                    for (int j = 1; j < E; j++) vk = k == j ? v[j] : vk;
+                    if (!(vk >= R.cut)) continue;
                     float d;
-                    const int b = sa_bin(x, d);
-                    const u64 key = sa_key(v, i);
+                    const int b = sa_bin(sa_x(R, vk), d);
+                    const u64 key = sa_key(vk, i + k);
                     if (b >= c.bin0 && b <= c.bin1 && (c.shift >= 63 || (key >> c.shift) == c.prefix)) {
                         const u32 at = sa_add32(&S->n, 0, 1u);
                         if (at < (u32)SA_LIST) sa_st64(&S->list[at], 0, key);
@@ -251,21 +323,40 @@ __global__ void __launch_bounds__(SA_NTH, 2) sz_sample_kernel(const __grid_const
             if (c.cmd == SA_LARGEST) {
                 const float x = sa_x(R, mine);
                 float d;
-                if (there(mine, x)) atomicAdd(&S->h.hi[sa_bin(x, d)], 65536u);
+                if (mine >= R.cut) atomicAdd(&S->h.hi[sa_bin(x, d)], SA_MEMBER);
             } else {
                 u32 above = 0;
-                each([&](float v, u32 i) {
-                    const float x = sa_x(R, v);
-                    if (there(v, x)) {
-                        float d;
-                        int b = sa_bin(x, d);
-                        above += x >= R.floor_x;
-                        if (c.cut >= 0) {
-                            const u64 key = sa_key(v, i);
-                            if (b != c.bin0 || (c.shift < 63 && (key >> c.shift) != c.prefix)) return;
-                            b = (int)(key >> c.cut) & (SA_BINS - 1);
+                const u32 lo0 = sz_smem_addr(S->h.lo), none = lo0 + 4u * (SA_BINS + lane);
+                each([&](const float* v, u32 i) {
+#pragma unroll
+                    for (int h = 0; h < E; h += 4) {
+                        u32 at[4], r[4], old[4];
+#pragma unroll
+                        for (int k = 0; k < 4; k++) {
+                            const float x = sa_x(R, v[h + k]);
+                            float d;
+                            const u32 b = lo0 + 4u * (u32)sa_bin(x, d);
+                            const bool in = v[h + k] >= R.cut;
+                            at[k] = in ? b : none;
+                            r[k] = sa_term(d);
+                            above += in && x >= R.floor_x;
                         }
-                        sa_add(S, b, d);
+                        if (c.cut >= 0) {
+#pragma unroll
+                            for (int k = 0; k < 4; k++) {
+                                const u64 key = sa_key(v[h + k], i + h + k);
+                                const bool in = at[k] == lo0 + 4u * (u32)c.bin0 && (c.shift >= 63 || (key >> c.shift) == c.prefix);
+                                at[k] = in ? lo0 + 4u * ((u32)(key >> c.cut) & (SA_BINS - 1)) : none;
+                            }
+                        }
+#pragma unroll
+                        for (int k = 0; k < 4; k++) asm volatile("atom.shared.add.u32 %0, [%1], %2;" : "=r"(old[k]) : "r"(at[k]), "r"(r[k]) : "memory");
+#pragma unroll
+                        for (int k = 0; k < 4; k++) {
+                            u32 more;
+                            asm("{\n\t.reg .u32 t;\n\tadd.cc.u32 t, %1, %2;\n\taddc.u32 %0, %3, 0;\n\t}" : "=r"(more) : "r"(old[k]), "r"(r[k]), "r"(SA_MEMBER));
+                            asm volatile("red.shared.add.u32 [%0], %1;" ::"r"(at[k] + (u32)sizeof(S->h.lo)), "r"(more) : "memory");
+                        }
                     }
                 });
                 if (c.count) {
@@ -282,8 +373,8 @@ __global__ void __launch_bounds__(SA_NTH, 2) sz_sample_kernel(const __grid_const
 #pragma unroll
                 for (int k = 0; k < 8; k++) { h[k] = k < a.C ? sa_ld32(&S->h.hi[b], k) : 0; l[k] = k < a.C ? sa_ld32(&S->h.lo[b], k) : 0; }
 #pragma unroll
-                for (int k = 0; k < 8; k++) { n_b += h[k] >> 16; sum += ((u64)(h[k] & 65535u) << 32) + l[k]; }
-                const double more = (double)((long long)sum - ((long long)n_b << 30)) * (1.0 / 68719476736.0);
+                for (int k = 0; k < 8; k++) { n_b += h[k] / SA_MEMBER; sum += ((u64)(h[k] % SA_MEMBER) << 32) + l[k]; }
+                const double more = (double)((long long)sum - ((long long)n_b << 26)) * (1.0 / 4294967296.0);
                 sa_st32(&S->gcnt[b], 0, n_b);
                 sa_st64(&S->gmass[b], 0, n_b ? __double2ull_rn(exp(-(double)SA_W * (c.cut >= 0 ? c.bin0 : b)) * SA_ONE * ((double)n_b + more)) : 0ull);
             }
@@ -301,14 +392,7 @@ __global__ void __launch_bounds__(SA_NTH, 2) sz_sample_kernel(const __grid_const
                     few = whole;
                 }
                 if (whole || !few) count = min(count, (u32)SA_LIST);
-                for (u32 k = tid; k < count; k += SA_NTH) {
-                    const u64 key = S->list[k];
-                    int at = 0;
-#pragma unroll 8
-                    for (u32 j = 0; j < count; j++) at += S->list[j] < key;
-                    S->sorted[at] = key;
-                }
-                __syncthreads();
+                sa_sort(S->list, S->cum, count, tid);
             }
             // two elements a thread: sums before them
             u32 n0 = 0, n1 = 0;
@@ -316,10 +400,10 @@ __global__ void __launch_bounds__(SA_NTH, 2) sz_sample_kernel(const __grid_const
             if (c.cmd != SA_GATHER) { n0 = S->gcnt[2 * tid]; n1 = S->gcnt[2 * tid + 1]; w0 = S->gmass[2 * tid]; w1 = S->gmass[2 * tid + 1]; }
             else {
                 n0 = (u32)(2 * tid) < count; n1 = (u32)(2 * tid + 1) < count;
-                if (n0) w0 = sa_weight(R, sa_value(S->sorted[2 * tid]));
-                if (n1) w1 = sa_weight(R, sa_value(S->sorted[2 * tid + 1]));
+                if (n0) w0 = sa_weight(R, sa_value(S->list[2 * tid]));
+                if (n1) w1 = sa_weight(R, sa_value(S->list[2 * tid + 1]));
                 if (whole && c.cmd == SA_GATHER) {
-                    u32 above = (n0 && sa_x(R, sa_value(S->sorted[2 * tid])) >= R.floor_x) + (n1 && sa_x(R, sa_value(S->sorted[2 * tid + 1])) >= R.floor_x);
+                    u32 above = (n0 && sa_x(R, sa_value(S->list[2 * tid])) >= R.floor_x) + (n1 && sa_x(R, sa_value(S->list[2 * tid + 1])) >= R.floor_x);
                     above = __reduce_add_sync(0xffffffffu, above);
                     if (lane == 0 && above) atomicAdd(&S->above, above);
                 }
@@ -404,7 +488,7 @@ __global__ void __launch_bounds__(SA_NTH, 2) sz_sample_kernel(const __grid_const
                     else if (stage == 4 && rank0 + i >= kept) stage = 5;
                     else {
                         if (tid == 0) {
-                            a.token[row] = (int32_t)(S->sorted[i] & ((1u << SA_ID) - 1));
+                            a.token[row] = (int32_t)(S->list[i] & ((1u << SA_ID) - 1));
                             if (a.prob) a.prob[row] = (float)((double)(S->cum[i + 1] - S->cum[i]) / (double)M);
                         }
                         t.cmd = SA_DONE;
@@ -454,7 +538,7 @@ __global__ void __launch_bounds__(SA_NTH, 2) sz_sample_kernel(const __grid_const
 
 template <int TYPE>
 int sa_launch(const SaArgs& a, cudaStream_t st) {
-    const size_t smem = ((sizeof(SaSmem) + 15) & ~(size_t)15) + (size_t)a.per * SaVec<TYPE>::ESZ;
+    const size_t smem = SA_SMEM + (a.keep ? (size_t)a.per * SaVec<TYPE>::ESZ + 16 : 0);
     const int rc = sz_allow_smem((const void*)sz_sample_kernel<TYPE>, 227 * 1024);
     if (rc) return rc;
     cudaLaunchConfig_t cfg = {};
@@ -491,8 +575,18 @@ extern "C" int sz_sample_rows(int logits_type, uint64_t logits, int64_t logits_s
     a.logits = (const u8*)logits; a.stride = logits_stride * esz; a.rows = rows; a.vocab = vocab;
     a.temperature = (const float*)temperature; a.top_k = (const int32_t*)top_k; a.top_p = (const float*)top_p; a.min_p = (const float*)min_p;
     a.uniform = (const double*)uniform; a.token = (int32_t*)token; a.prob = (float*)prob;
-    a.C = vocab > 16384 ? 8 : vocab > 4096 ? 4 : vocab > 1024 ? 2 : 1;
+    // Blocks a row: the fewer, the more rows are under way at once and the less their steps wait for one another; the more, the sooner a row is
+    // through.  Waves of blocks times what a block takes (rows of 151,936, us, 1 / 2 / 4 / 8 blocks: 1 row 30 / 22 / 16 / 13.4, 64 rows
+    // 105 / 62 / 51 / 55, 250 rows of bf16 93 / 97 / 115 / 175).
+    const int most = vocab > 16384 ? 8 : vocab > 4096 ? 4 : vocab > 1024 ? 2 : 1;
+    double least = 0;
+    for (int C = 1; C <= most; C *= 2) {
+        const double cost = (double)(((long long)rows * C + SA_PLACES - 1) / SA_PLACES) * (SA_FIXED + (double)vocab / C);
+        if (C == 1 || cost < least) { least = cost; a.C = C; }
+    }
     a.per = ((vocab + a.C - 1) / a.C + 7) & ~7;
+    // read again from L2 where shared memory would hold fewer blocks with their parts than without
+    a.keep = SA_SMEM + (size_t)a.per * esz + 16 <= SA_KEEP;
     cudaStream_t st = (cudaStream_t)stream;
     return logits_type == SZ_TYPE_F32 ? sa_launch<SZ_TYPE_F32>(a, st) : logits_type == SZ_TYPE_F16 ? sa_launch<SZ_TYPE_F16>(a, st) : sa_launch<SZ_TYPE_BF16>(a, st);
 }

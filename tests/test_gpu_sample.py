@@ -199,3 +199,31 @@ def test_a_captured_call():
         g.replay()
         torch.cuda.synchronize()
         assert torch.equal(out, sampling.sample_rows(lg, u))
+
+
+@pytest.mark.parametrize("rows,vocab,dtype", [(300, 40001, torch.bfloat16), (100, 100003, torch.float32), (64, 70002, torch.float16), (37, 262143, torch.float32)])
+def test_rows_in_fewer_blocks(rows, vocab, dtype):
+    """Many rows: one to four blocks a row, whose parts do not fit shared memory and begin at any element."""
+    rng = np.random.default_rng(rows + vocab)
+    lg = torch.from_numpy(rng.normal(size=(rows, vocab)).astype(np.float32) * 2.5).to(dtype)
+    T, k, p, mp, u = settings(rng, rows, vocab)
+    lg[3] = -math.inf
+    lg[4, 5:] = math.nan
+    check(lg, T, k, p, mp, u)
+
+
+def test_most_equal_logits_in_one_block():
+    """262,144 members of one bin in one block: its count and its sum fill their bits."""
+    rows, vocab = 300, 262144
+    lg = torch.zeros(rows, vocab, dtype=torch.float16, device="cuda")
+    u = torch.rand(rows, dtype=torch.float64, generator=torch.Generator().manual_seed(8))
+    u[0], u[1] = 0.0, 1 - 2.0 ** -53
+    assert torch.equal(sampling.sample_rows(lg, u.cuda()).cpu(), (u * vocab).to(torch.int32))
+    lg[:, ::2] = -2.0 ** -9                      # (less than half a bin: two weights in one)
+    tok = sampling.sample_rows(lg, u.cuda()).cpu().numpy()
+    w = np.where(np.arange(vocab) % 2 == 1, 1.0, math.exp(-2.0 ** -9))
+    order = np.concatenate([np.arange(1, vocab, 2), np.arange(0, vocab, 2)])
+    c = np.cumsum(w[order])
+    for r in range(rows):
+        goal = float(u[r]) * c[-1]
+        assert tok[r] == order[min(int((c <= goal).sum()), vocab - 1)] or np.abs(c - goal).min() < 2.0 ** -30 * c[-1], r
