@@ -265,7 +265,7 @@ __device__ PgList pg_list(const PgBatch& d, const PgPart& p, int r, int r0, int 
 template <int HD, int W>
 __global__ void __launch_bounds__(256) sz_pg_merge_kernel(const __grid_constant__ PgBatch d, const __grid_constant__ PgIo io, const __grid_constant__ PgParts a) {
     constexpr int E = HD / 32;                                       // columns a lane, in pairs: 2 lane + 64 x
-    __shared__ float2 sums[W > 1 ? W : 1][HD / 2], of_warp[8];
+    __shared__ float2 sums[8][W > 1 ? HD / 2 : 1], of_warp[8];
     const int r = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, sub = warp % W, h = blockIdx.y * (8 / W) + warp / W, nh = d.nkv * d.G;
     sz_pdl_wait();
     sz_pdl_trigger();
@@ -335,22 +335,22 @@ __global__ void __launch_bounds__(256) sz_pg_merge_kernel(const __grid_constant_
     L = sz_warp_sum(L);
     if (W > 1) {
 #pragma unroll
-        for (int x = 0; x < E / 2; x++) sums[sub][lane + 32 * x] = acc[x];
-        if (lane == 0) of_warp[sub] = make_float2(M, L);
-        __syncthreads();
+        for (int x = 0; x < E / 2; x++) sums[warp][lane + 32 * x] = acc[x];
+        if (lane == 0) of_warp[warp] = make_float2(M, L);
+        asm volatile("bar.sync %0, %1;" ::"r"(1 + warp / W), "n"(32 * W) : "memory");      // (the head's warps: others may have left)
         if (sub) return;
         float Mw[W], top = M;
 #pragma unroll
-        for (int k = 0; k < W; k++) { Mw[k] = of_warp[k].x; top = fmaxf(top, Mw[k]); }
+        for (int k = 0; k < W; k++) { Mw[k] = of_warp[warp + k].x; top = fmaxf(top, Mw[k]); }
         L = 0.f;
 #pragma unroll
         for (int x = 0; x < E / 2; x++) acc[x] = make_float2(0.f, 0.f);
 #pragma unroll
         for (int k = 0; k < W; k++) {
             const float c = Mw[k] == -INFINITY ? 0.f : pg_ex2(Mw[k] - top);
-            L = fmaf(of_warp[k].y, c, L);
+            L = fmaf(of_warp[warp + k].y, c, L);
 #pragma unroll
-            for (int x = 0; x < E / 2; x++) { const float2 f = sums[k][lane + 32 * x]; acc[x].x = fmaf(f.x, c, acc[x].x); acc[x].y = fmaf(f.y, c, acc[x].y); }
+            for (int x = 0; x < E / 2; x++) { const float2 f = sums[warp + k][lane + 32 * x]; acc[x].x = fmaf(f.x, c, acc[x].x); acc[x].y = fmaf(f.y, c, acc[x].y); }
         }
         M = top;
     }
@@ -585,8 +585,10 @@ extern "C" int sz_paged_attend(const sz_paged_cache* cache, const sz_paged_batch
         if (rc) return rc;
     }
     const bool few = (int64_t)batch->rows * n_head <= 8 * PG_BLOCKS;
-    auto* merge = hd == 64 ? (few ? sz_pg_merge_kernel<64, 8> : sz_pg_merge_kernel<64, 1>) : hd == 128 ? (few ? sz_pg_merge_kernel<128, 8> : sz_pg_merge_kernel<128, 1>)
-                                                                                            : (few ? sz_pg_merge_kernel<256, 8> : sz_pg_merge_kernel<256, 1>);
-    SZ_CUDA(sz_launch("paged_merge", merge, dim3(batch->rows, few ? n_head : (n_head + 7) / 8), dim3(256), 0, st, true, d, io, s.a));
+    const int W = few ? 8 : (int64_t)batch->rows * n_head <= 16 * PG_BLOCKS ? 2 : 1;
+#define SZ_PG_MERGE(HD) (W == 1 ? sz_pg_merge_kernel<HD, 1> : W == 2 ? sz_pg_merge_kernel<HD, 2> : sz_pg_merge_kernel<HD, 8>)
+    auto* merge = hd == 64 ? SZ_PG_MERGE(64) : hd == 128 ? SZ_PG_MERGE(128) : SZ_PG_MERGE(256);
+#undef SZ_PG_MERGE
+    SZ_CUDA(sz_launch("paged_merge", merge, dim3(batch->rows, (n_head * W + 7) / 8), dim3(256), 0, st, true, d, io, s.a));
     return SZ_OK;
 }
