@@ -194,6 +194,12 @@ __device__ __forceinline__ void pg_mma(float* c, const u32* a, u32 b0, u32 b1) {
     else sz_mma16816_z(c, a, b0, b1);
 }
 template <int CT>
+__device__ __forceinline__ void pg_mma_first(float* c, const u32* a, u32 b0, u32 b1) {      // sums that begin at 0 (f16)
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+        : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
+}
+__device__ __forceinline__ float pg_half(u32 w, int i) { const __half2 h = *(const __half2*)&w; return i ? __high2float(h) : __low2float(h); }
+template <int CT>
 __device__ __forceinline__ u32 pg_pack(float a, float b) { return CT == PG_BF16 ? pg_pack_bf16(a, b) : pg_pack_f16(a, b); }
 template <int CT>
 __device__ __forceinline__ float2 pg_unpack(u32 w) {
@@ -435,48 +441,48 @@ sz_pg_attend_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_const
             }
         } else {
             const u8* kr = ring + (size_t)cslot * C::HALF + (size_t)pw * C::HB;
-#pragma unroll 2
-            for (int gr = 0; gr < HD / 32; gr++) {        // 32 dimensions share a scale; every piece of the queries has sums of its own (short chains)
-                float tt[C::QN][C::SG][2][4];
-                float sc[C::SG][2][2];
+#pragma unroll 1
+            for (int g2 = 0; g2 < HD / 64; g2++) {        // two groups of 32 dimensions: their scales are read together
+                u32 sc[C::SG][2][2];
 #pragma unroll
                 for (int g = 0; g < C::SG; g++)
 #pragma unroll
                     for (int n = 0; n < 2; n++) {
-                        const u8* sp = kr + (size_t)(16 * g + 8 * n + 2 * q4) * C::HB + HD + 2 * gr;
-                        sc[g][n][0] = sz_f16_to_f32(*(const u16*)sp); sc[g][n][1] = sz_f16_to_f32(*(const u16*)(sp + C::HB));
-#pragma unroll
-                        for (int k = 0; k < C::QN; k++) { tt[k][g][n][0] = 0.f; tt[k][g][n][1] = 0.f; tt[k][g][n][2] = 0.f; tt[k][g][n][3] = 0.f; }
+                        const u8* sp = kr + (size_t)(16 * g + 8 * n + 2 * q4) * C::HB + HD + 4 * g2;
+                        sc[g][n][0] = *(const u32*)sp; sc[g][n][1] = *(const u32*)(sp + C::HB);
                     }
-                u32 b0[2][C::SG][2], b1[2][C::SG][2];
 #pragma unroll
-                for (int kk = 0; kk < 2; kk++)
+                for (int hf = 0; hf < 2; hf++) {
+                    const int gr = 2 * g2 + hf;
+                    float tt[C::SG][2][4];
+                    u32 b0[2][C::SG][2], b1[2][C::SG][2];
 #pragma unroll
-                    for (int g = 0; g < C::SG; g++)
-#pragma unroll
-                        for (int n = 0; n < 2; n++) sz_q8_quad(*(const u32*)(kr + (size_t)(16 * g + 8 * n + g8) * C::HB + (2 * gr + kk) * 16 + 4 * q4), b0[kk][g][n], b1[kk][g][n]);
-#pragma unroll
-                for (int kk = 0; kk < 2; kk++)
-#pragma unroll
-                    for (int k = 0; k < C::QN; k++) {
-                        const uint4 q = *(const uint4*)(qm + (((size_t)(k * NQT + qt) * C::KS + 2 * gr + kk) * 32 + lane) * 16);
-                        const u32 a[4] = {q.x, q.y, q.z, q.w};
+                    for (int kk = 0; kk < 2; kk++)
 #pragma unroll
                         for (int g = 0; g < C::SG; g++)
 #pragma unroll
-                            for (int n = 0; n < 2; n++) pg_mma<CT>(tt[k][g][n], a, b0[kk][g][n], b1[kk][g][n]);
-                    }
+                            for (int n = 0; n < 2; n++) sz_q8_quad(*(const u32*)(kr + (size_t)(16 * g + 8 * n + g8) * C::HB + (2 * gr + kk) * 16 + 4 * q4), b0[kk][g][n], b1[kk][g][n]);
 #pragma unroll
-                for (int g = 0; g < C::SG; g++)
+                    for (int kk = 0; kk < 2; kk++)
 #pragma unroll
-                    for (int n = 0; n < 2; n++)
+                        for (int k = 0; k < C::QN; k++) {
+                            const uint4 q = *(const uint4*)(qm + (((size_t)(k * NQT + qt) * C::KS + 2 * gr + kk) * 32 + lane) * 16);
+                            const u32 a[4] = {q.x, q.y, q.z, q.w};
 #pragma unroll
-                        for (int c = 0; c < 4; c++) {
-                            float x = tt[0][g][n][c];
+                            for (int g = 0; g < C::SG; g++)
 #pragma unroll
-                            for (int k = 1; k < C::QN; k++) x += tt[k][g][n][c];
-                            s[g][n][c] = fmaf(sc[g][n][c & 1], x, s[g][n][c]);
+                                for (int n = 0; n < 2; n++) {
+                                    if (kk == 0 && k == 0) pg_mma_first<CT>(tt[g][n], a, b0[kk][g][n], b1[kk][g][n]);
+                                    else pg_mma<CT>(tt[g][n], a, b0[kk][g][n], b1[kk][g][n]);
+                                }
                         }
+#pragma unroll
+                    for (int g = 0; g < C::SG; g++)
+#pragma unroll
+                        for (int n = 0; n < 2; n++)
+#pragma unroll
+                            for (int c = 0; c < 4; c++) s[g][n][c] = fmaf(pg_half(sc[g][n][c & 1], hf), tt[g][n][c], s[g][n][c]);
+                }
             }
         }
         bool hidden = false;                              // a position that is there, but not for this lane's rows
@@ -612,22 +618,31 @@ sz_pg_attend_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_const
 #pragma unroll
             for (int g = 0; g < C::SG; g++)
 #pragma unroll
+                for (int e = 0; e < 8; e++) p[g][e] *= csc;      // (a power of two: exact, but for weights of 2^-100 and less)
+#pragma unroll
+            for (int g = 0; g < C::SG; g++) {
+                u32 vs[4];
+#pragma unroll
                 for (int gr = 0; gr < HD / 32; gr++) {
                     u32 v4[4];
-                    float vs[4];
 #pragma unroll
                     for (int r4 = 0; r4 < 4; r4++) {      // positions 2 q4, + 1, + 8, + 9: the lane's k slots; a word: dimensions 32 gr + 4 g8 ..
                         const u8* row = vr + (size_t)(16 * g + 2 * q4 + (r4 & 1) + 8 * (r4 >> 1)) * C::HB;
                         v4[r4] = *(const u32*)(row + 32 * gr + 4 * g8) ^ 0x80808080u;
-                        vs[r4] = sz_f16_to_f32(*(const u16*)(row + HD + 2 * gr)) * csc;
+                        if (gr % 2 == 0) vs[r4] = *(const u32*)(row + HD + 2 * gr);      // (this group's scale and the next one's)
+                    }
+                    float pv[8];
+#pragma unroll
+                    for (int e = 0; e < 8; e++) pv[e] = p[g][e] * pg_half(vs[2 * (e >> 2) + (e & 1)], gr & 1);
+                    if (odd) {
+#pragma unroll
+                        for (int e = 0; e < 8; e++) pv[e] = p[g][e] > 0.f ? pv[e] : 0.f;
                     }
                     u32 af[C::PN][4];
 #pragma unroll
                     for (int r4 = 0; r4 < 4; r4++) {
                         u32 w[C::PN];
-                        float pa = p[g][2 * r4] * vs[2 * (r4 >> 1)], pb = p[g][2 * r4 + 1] * vs[2 * (r4 >> 1) + 1];
-                        if (odd) { pa = p[g][2 * r4] > 0.f ? pa : 0.f; pb = p[g][2 * r4 + 1] > 0.f ? pb : 0.f; }
-                        pg_pieces<CT, C::PN>(pa, pb, w);
+                        pg_pieces<CT, C::PN>(pv[2 * r4], pv[2 * r4 + 1], w);
 #pragma unroll
                         for (int k = 0; k < C::PN; k++) af[k][r4] = w[k];
                     }
@@ -642,6 +657,7 @@ sz_pg_attend_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_const
                         for (int k = 0; k < C::PN; k++) pg_mma<CT>(o[4 * gr + b], af[k], *(const u32*)&h0, *(const u32*)&h1);
                     }
                 }
+            }
         }
         if (++cslot == C::NR) { cslot = 0; cphase ^= 1; }
         if (u + 1 < u1 && it.i + 1 < it.n) continue;
