@@ -288,13 +288,13 @@ typedef struct sz_paged_rope {
  * call with another shared_len or fewer rows fits where this one does).  Calls that can overlap on the GPU need one each, captured
  * graphs too.  sz_paged_status(scratch, 1, NULL, stream) once after it is allocated; sz_paged_status(scratch, 0, &code, stream)
  * synchronises and reports (and keeps) what calls have met: bit 0: a page id out of range, bit 1: a position behind the table's end, bit 2: a
- * row of sz_paged_append at a shared position, bit 3: row_start past `rows` - the position, or the row, is then left out -, bit 4: a bounded wait ran out. */
+ * row of sz_paged_append at a shared position, bit 3: row_start past `rows` (the position, or the row, is then left out) or descending (no row attends to its own positions), bit 4: a bounded wait ran out. */
 int sz_paged_scratch_bytes(const sz_paged_cache* cache, const sz_paged_batch* batch, int n_head, int64_t* bytes);
 int sz_paged_status(uint64_t scratch, int init, int* code, uint64_t stream);
 /* Stores row r's key and value heads at its position and, where q is given, writes its query heads, normed and turned, to q_out.
  * io_type: SZ_TYPE_F32, F16 or BF16, the type of k, v, q and q_out.  k, v: [rows][n_kv_head][head_dim], q_out [rows][n_head][head_dim], q
  * [rows][n_head] heads q_head_stride apart (2 head_dim where queries and gates alternate); row strides in elements; heads and rows
- * 16-byte aligned.  A row at a negative position (lens[b] < the sequence's rows) is left out.  q_out may be q.  No position may
+ * 16-byte aligned.  A row at a negative position (lens[b] < the sequence's rows) is left out.  q_out may be q, with the same strides.  No position may
  * be appended by two rows of a call. */
 int sz_paged_append(const sz_paged_cache* cache, const sz_paged_batch* batch, const sz_paged_rope* rope, int io_type, int n_head, uint64_t k, int64_t k_stride,
                     uint64_t v, int64_t v_stride, uint64_t q, int64_t q_stride, int64_t q_head_stride, uint64_t q_out, int64_t q_out_stride, uint64_t scratch,

@@ -244,7 +244,9 @@ __global__ void __launch_bounds__(1024) sz_pg_plan_kernel(const __grid_constant_
 
 // ---- joining the parts -----------------------------------------------------------------------------------------------------------------------------
 // W warps have one row and head: the parts of its items, in the order of the positions.  A lane has hd / 32 columns; the warps take the
-// parts in turn and their sums are added in order.  One warp where rows and heads are many, eight where they are few and their parts therefore many.
+// parts in turn and their sums are added in order.  The fewer rows and heads, the more parts each has (units are shared out evenly): 1, 2 or 8
+// warps (64 rows of 16 heads, 74 parts: 75 / 69 / 58 us for the whole call; 2,048 rows and heads 129 / 126 / 134; 5,216: 404 / 410 / 425).
+// What it waits for is the way to the parts - row, sequence, plan, list, maxima, sums, one after the other: 15 us of 55 with four rows.
 struct PgList { int n, first, alone, lane; };     // parts of an item: their number, the block of the first; by row and head; the vector's place in its tile
 __device__ PgList pg_list(const PgBatch& d, const PgPart& p, int r, int r0, int b, int h) {
     PgList l = {};
@@ -252,6 +254,7 @@ __device__ PgList pg_list(const PgBatch& d, const PgPart& p, int r, int r0, int 
     const int start = p.shared ? pg_row(d, 0) : r0;
     const int vec = (r - start) * d.G + h % d.G, t = vec / p.tq, e = p.shared ? t : (int)p.tiles[b] + t;
     const int E = p.shared ? ((pg_row(d, d.n_seq) - start) * d.G + p.tq - 1) / p.tq : (int)p.tiles[d.n_seq];
+    if (vec < 0 || e >= E) return l;      // (a row_start that descends: there are no tiles)
     const u32 us = p.units[e], n = p.units[e + 1] - us;
     if (!n) return l;
     const u32 U = p.units[E] * (u32)d.nkv, at = us * (u32)d.nkv + (u32)(h / d.G) * n;
@@ -312,7 +315,7 @@ __global__ void __launch_bounds__(256) sz_pg_merge_kernel(const __grid_constant_
         }
         u32 left = __ballot_sync(0xffffffffu, from != nullptr);      // (empty parts have no sums)
         while (left) {
-            constexpr int B = 8;                                     // parts in flight
+            constexpr int B = W == 1 ? 4 : 8;                        // parts in flight (one warp: few parts, and the registers of eight leave half the warps; 2,045 rows 365 -> 350 us)
             float2 f[B][E / 2];
             float cw[B];
 #pragma unroll
@@ -574,6 +577,9 @@ extern "C" int sz_paged_attend(const sz_paged_cache* cache, const sz_paged_batch
         p.blocks = tc_of[i] ? PG_BLOCKS : PG_BLOCKS * kern[i].occ;
         p.planned = (p.shared ? 0 : batch->n_seq) + (all + p.tq - 1) / p.tq > PG_PLAN;
         planned |= p.planned;
+        const int64_t positions = p.shared ? batch->shared_len : (int64_t)batch->max_pages * cache->page_size;
+        const double units = (double)((all + p.tq - 1) / p.tq + (p.shared ? 0 : batch->n_seq)) * (double)((positions + p.unit - 1) / p.unit) * nkv;
+        if (units > 4294967295.0) return sz_fail(SZ_E_ARG, "%s: %d rows over %lld positions are more work than a call takes", who, batch->rows, (long long)positions);
         for (int x = 0; x < 2; x++) if ((rc = pg_map(cache, x, box[tc_of[i]], &maps[tc_of[i]][x]))) return rc;
     }
     s.a.p[PG_OWN].direct = tc_of[PG_OWN] && batch->shared_len == 0;
@@ -585,8 +591,8 @@ extern "C" int sz_paged_attend(const sz_paged_cache* cache, const sz_paged_batch
         rc = tc_of[i] ? pg_tc_launch(cache->type == SZ_TYPE_BF16, hd, maps[1], box[1], d, io, p, name, st) : pg_launch_attend(kern[i], maps[0], box[0], d, io, p, name, st);
         if (rc) return rc;
     }
-    const bool few = (int64_t)batch->rows * n_head <= 8 * PG_BLOCKS;
-    const int W = few ? 8 : (int64_t)batch->rows * n_head <= 16 * PG_BLOCKS ? 2 : 1;
+    const int64_t heads = (int64_t)batch->rows * n_head;
+    const int W = heads <= 8 * PG_BLOCKS ? 8 : heads <= 16 * PG_BLOCKS ? 2 : 1;
 #define SZ_PG_MERGE(HD) (W == 1 ? sz_pg_merge_kernel<HD, 1> : W == 2 ? sz_pg_merge_kernel<HD, 2> : sz_pg_merge_kernel<HD, 8>)
     auto* merge = hd == 64 ? SZ_PG_MERGE(64) : hd == 128 ? SZ_PG_MERGE(128) : SZ_PG_MERGE(256);
 #undef SZ_PG_MERGE

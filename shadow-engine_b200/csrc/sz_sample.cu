@@ -27,6 +27,7 @@
 namespace {
 
 constexpr int SA_BINS = 1024, SA_LIST = 1024, SA_NTH = 512, SA_MAX_VOCAB = 1 << 18, SA_ID = 18, SA_FEW = 512;
+constexpr int SA_ROUNDS = 64;
 constexpr int SA_RANK = 256;                                   // keys that are put in order by counting (at most SA_NTH)
 constexpr int SA_PLACES = 2 * 148;                             // blocks that run at once
 constexpr double SA_FIXED = 40000;                             // a block's time beside its part of the row, in elements of it
@@ -291,7 +292,7 @@ __global__ void __launch_bounds__(SA_NTH, 2) sz_sample_kernel(const __grid_const
     u64 s_m0 = 0, s_m1 = 0;
     int stage = 0;
 #pragma unroll 1
-    for (;;) {
+    for (int round = 0;; round++) {                                  // (a row needs some thirty at most)
         // ---- all blocks
         if (c.cmd == SA_GATHER) {
             // those near the bins by |v - mid| <= half, a little wider than they are, then by their bins
@@ -436,7 +437,7 @@ __global__ void __launch_bounds__(SA_NTH, 2) sz_sample_kernel(const __grid_const
             auto search = [&](auto at, int n_at) {                   // the one place of n_at for which at() is true
                 for (int i = tid; i < n_at; i += SA_NTH) if (at(i)) S->at = i;
                 __syncthreads();
-                const int i = S->at;
+                const int i = min(max(S->at, 0), n_at - 1);          // (logits that somebody writes meanwhile may have none)
                 __syncthreads();
                 return i;
             };
@@ -521,6 +522,13 @@ __global__ void __launch_bounds__(SA_NTH, 2) sz_sample_kernel(const __grid_const
                 t.cmd = descending ? SA_SUM : SA_GATHER;
                 if (descending) { bins_valid = false; t.cut = (t.shift >= 63 ? SA_ID + 32 : t.shift) - 10; }      // (ten bits are left at least: fewer would fit the list)
                 break;
+            }
+            if (round == SA_ROUNDS && t.cmd != SA_DONE) {            // logits that somebody writes meanwhile: no two passes agree
+                t.cmd = SA_DONE;
+                if (tid == 0) {
+                    a.token[row] = 0;
+                    if (a.prob) a.prob[row] = 0.f;
+                }
             }
             if (tid == 0) { S->c = t; S->n = 0; }
             c = t;

@@ -589,3 +589,21 @@ def test_rows_that_overlap_are_refused():
     c = Case([33], [1], nh=2, nkv=1, hd=64, io="bf16", cache="bf16", seed=91)
     want = c.step.attend(c.q)
     assert torch.equal(c.step.attend(c.q.expand(1, 2, 64).as_strided((1, 2, 64), (0, 64, 1))), want)
+
+
+@pytest.mark.parametrize("n,m,shared", [(3, 5, 0), (3, 5, 32), (300, 2, 0), (300, 2, 32)])
+def test_a_descending_row_start_is_reported(n, m, shared):
+    """Its sequences would have more tiles than the tables have room for: no row is attended, nothing but zeros comes out, the status tells."""
+    c = Case([shared + 40] * n, [m] * n, nh=4, nkv=2, hd=64, io="bf16", cache="bf16", shared=shared, seed=92)
+    want = c.step.attend(c.q).clone()
+    good = c.row_start.clone()
+    c.row_start[1::2] = c.rows
+    c.row_start[0] = 0
+    c.row_start[2::2] = 0
+    out = torch.full_like(c.q, 7.0)
+    c.step.attend(c.q, out=out)
+    assert c.step.status() & 8
+    if not shared:
+        assert bool(((out == 0) | (out == 7.0)).all())
+    c.row_start.copy_(good)
+    assert torch.equal(c.step.attend(c.q), want)

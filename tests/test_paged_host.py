@@ -132,3 +132,11 @@ def test_the_python_side_refuses_overlapping_rows():
     for bad in (torch.zeros(1, 10).expand(3, 10), torch.zeros(12).as_strided((3, 10), (1, 1)), torch.zeros(3, 1).expand(3, 10)):
         with pytest.raises(ValueError):
             sampling.sample_rows(bad, u)
+
+
+def test_more_work_than_a_call_takes_is_refused():
+    """Units of work are counted in 32 bits: a million rows of 128 heads over a table of four million positions are not a call."""
+    L = szlib.load()
+    c = cache(n_kv_head=8, page_size=1024, n_pages=1 << 20, page_stride=8 * 1024 * 256, head_stride=1024 * 256)
+    assert attend(L, c=c, b=batch(n_seq=1, rows=1 << 20, max_pages=4096), nh=128, qs=128 * 128, os_=128 * 128, size=1 << 62) == szlib.E_ARG
+    assert b"more work" in L.sz_last_error()
