@@ -52,9 +52,6 @@ struct PgPart {
     int blocks, tq, shared, planned; // planned: the plan was made by sz_pg_plan_kernel
     int unit;                        // positions a unit: PG_T, or the tcgen05 kernel's
     int direct;                      // (tcgen05 kernel) an item that one block does alone goes straight to the output
-    // Of two launches over one batch the first (1) lets the second begin as soon as it runs itself, and the second (2), which reads nothing of it, waits for
-    // its end only before its own: what both wait for before them is then done, and the merge waits for both.
-    int chain;
     int on;
 };
 
@@ -258,8 +255,7 @@ sz_pg_attend_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_const
     if (tid < C::NR * 4) sz_mbar_init(&s_full[tid], NQT == 1 ? 1 : 4);
     if (tid < C::NR * 4) sz_mbar_fence_init();
     __syncthreads();
-    if (pt.chain != 2) sz_pdl_wait();
-    if (pt.chain == 1) sz_pdl_trigger();
+    sz_pdl_wait();
     const u32 *tiles = s_tiles, *units = s_units;
     int E;
     if (pt.planned) {
@@ -279,10 +275,7 @@ sz_pg_attend_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_const
     }
     const u32 U = units[E] * (u32)d.nkv;
     const int blocks = (int)min((u32)pt.blocks, U);
-    if ((int)blockIdx.x >= blocks) {                      // (blocks that leave count as having triggered)
-        if (pt.chain == 2) sz_pdl_wait();
-        return;
-    }
+    if ((int)blockIdx.x >= blocks) return;                // (blocks that leave count as having triggered)
     const PgShare share = pg_share(U, blocks);
     const u32 u0 = pg_first(share, blockIdx.x), u1 = pg_first(share, blockIdx.x + 1);
     const int room = pg_room(d);
@@ -747,7 +740,6 @@ sz_pg_attend_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_const
     }
     // (only now: blocks of the merge that wait on a multiprocessor early took places of this kernel's - 64 sequences 414 -> 530 us)
     sz_pdl_trigger();
-    if (pt.chain == 2) sz_pdl_wait();
 }
 
 // What a set of kernels offers the host.

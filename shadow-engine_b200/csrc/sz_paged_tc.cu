@@ -134,8 +134,7 @@ sz_pg_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
     __syncthreads();
     pt_after();
     const u32 tmem = __shfl_sync(0xffffffffu, S.tmem, 0);
-    if (pt.chain != 2) sz_pdl_wait();
-    if (pt.chain == 1) sz_pdl_trigger();
+    sz_pdl_wait();
     const u32 *tiles = S.tiles, *units = S.units;
     int E;
     if (pt.planned) {
@@ -483,7 +482,6 @@ sz_pg_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
         }
     }
     sz_pdl_trigger();
-    if (pt.chain == 2) sz_pdl_wait();
     if (failed) atomicMax(&S.failed, (u32)failed);
     pt_before();
     __syncthreads();
