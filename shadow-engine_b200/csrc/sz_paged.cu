@@ -574,7 +574,7 @@ extern "C" int sz_paged_attend(const sz_paged_cache* cache, const sz_paged_batch
         p.ways = tc_of[i] ? 1 : kern[i].ways;
         p.tq = tc_of[i] ? pg_tc_tile(hd) : kern[i].tq;
         p.blocks = tc_of[i] ? PG_BLOCKS : PG_BLOCKS * kern[i].occ;
-        p.planned = (p.shared ? 0 : batch->n_seq) + (all + p.tq - 1) / p.tq > PG_PLAN;
+        p.planned = batch->n_seq + (all + p.tq - 1) / p.tq > PG_PLAN;      // (a block's copies of the tables have PG_PLAN places, over shared positions too)
         planned |= p.planned;
         const int64_t positions = p.shared ? batch->shared_len : (int64_t)batch->max_pages * cache->page_size;
         const double units = (double)((all + p.tq - 1) / p.tq + (p.shared ? 0 : batch->n_seq)) * (double)((positions + p.unit - 1) / p.unit) * nkv;

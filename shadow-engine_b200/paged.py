@@ -57,7 +57,7 @@ class Step:
     """The tables of a batch over a cache, and the scratch of its calls.  pages int32 [sequences, pages of one], row_start int32 [sequences + 1],
     lens int32 [sequences] (all positions, the step's rows included) are the caller's tensors: change their values from step to step.
     shared_pages int32: the pages of the first shared_len positions, the same for all sequences.  Calls on one Step follow one another on
-    a stream; what may overlap needs a Step each."""
+    a stream - the one it was made on, or another that waits for that -, and it is kept until they are done; what may overlap needs a Step each."""
 
     def __init__(self, cache, pages, row_start, lens, rows, n_head, shared_pages=None, shared_len=0):
         self.lib = szlib.load()

@@ -607,3 +607,20 @@ def test_a_descending_row_start_is_reported(n, m, shared):
         assert bool(((out == 0) | (out == 7.0)).all())
     c.row_start.copy_(good)
     assert torch.equal(c.step.attend(c.q), want)
+
+
+@pytest.mark.parametrize("hd", [64, 128, 256])
+@pytest.mark.parametrize("seqs,m,nh,nkv,io,cache,shared", [(75, 1, 16, 2, "f32", "q8", 0), (250, 2, 3, 3, "f32", "f16", 0), (40, 1, 30, 6, "bf16", "bf16", 700), (20, 3, 35, 7, "f16", "f16", 0)])
+def test_parts_joined_by_two_warps(hd, seqs, m, nh, nkv, io, cache, shared):
+    """Rows times heads between those that eight warps and those that one joins; heads that are no multiple of a block's."""
+    Case([shared + 100 + 37 * i % 900 for i in range(seqs)], [m] * seqs, nh=nh, nkv=nkv, hd=hd, io=io, cache=cache, shared=shared, seed=hd + seqs, pad=1).check()
+
+
+@pytest.mark.parametrize("n,m,shared,io,cache", [(300, 2, 32, "bf16", "bf16"), (300, 2, 640, "f16", "f16"), (300, 1, 100, "f32", "q8"), (3, 50, 0, "bf16", "bf16"), (3, 50, 130, "f32", "bf16"), (1, 3, 0, "f32", "f16")])
+def test_what_the_scratch_held_does_not_matter(n, m, shared, io, cache):
+    c = Case([shared + 400 // (1 + n // 100)] * n, [m] * n, nh=4, nkv=2, hd=64, io=io, cache=cache, shared=shared, seed=93)
+    first = c.check().clone()
+    at = c.step.scratch - c.step._mem.data_ptr()
+    for byte in (0, 255, 63):
+        c.step._mem[at + 256:].fill_(byte)           # (the first 256 bytes hold the status)
+        assert torch.equal(c.check(), first)
