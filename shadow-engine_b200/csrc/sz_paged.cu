@@ -30,9 +30,9 @@ __device__ int pg_seq_of(const PgBatch& d, int r) {
 // f = head / sqrt(mean(head^2) + eps) * w, then (f_i, f_(i + half)) turned by pos theta^(-2 i / dims).  A lane has hd / 32 neighbouring dimensions, and
 // a rotation's partner is hd / 32 dimensions of another lane.  Sums of squares and rotations in f32, one rounding to the stored type.
 // R = 1 row a block, a warp a head, for few rows: latency bounds those - sequence, length, page, head, one after the other -, so the head is read
-// while its row is looked up.  R = PG_APP where that still gives every multiprocessor a block: a warp a row, its heads four at a time (their loads
-// and their norms' shuffles side by side).  24 heads of 256, keys and values of bf16: 1 row 3.6 us, 64 rows 5.2, 4,093 rows 29.1 against
-// 51 with R = 1 (83 MB: 12.8 us of them; the chains of norm, rotation and store of one wave of warps are the rest).
+// while its row is looked up.  R = PG_APP where that still gives every multiprocessor a block: a warp a row, its heads two at a time (their loads
+// and their norms' shuffles side by side).  16 + 2 + 2 heads of 256, bf16: 1 row 3.4 us, 4,093 rows 22.2 against 51 with R = 1 (83 MB: 12.8 us of
+// them; the chains of norm, rotation and store of one wave of warps are the rest); 163 rows of 32 + 8 + 8 heads of 128 5.2.
 // A row's angles are taken once a block, in f64 (a far position's angle has no digits left in f32), reduced to [-pi, pi] there, and the sine and
 // cosine of the reduced angle in f32 with its rounding put back by their derivatives.
 constexpr int PG_APP = 8;
@@ -76,7 +76,7 @@ __device__ __forceinline__ void pg_store_n(u8* p, const float* f) {
 }
 
 template <int CT, int HD, int IO, int R>
-__global__ void __launch_bounds__(256) sz_pg_append_kernel(const __grid_constant__ PgBatch d, const __grid_constant__ PgAppend a) {
+__global__ void __launch_bounds__(256, R == 1 ? 0 : 4) sz_pg_append_kernel(const __grid_constant__ PgBatch d, const __grid_constant__ PgAppend a) {
     constexpr int E = HD / 32, ESZ = IO == SZ_TYPE_F32 ? 4 : 2, CTY = CT == PG_F16 ? SZ_TYPE_F16 : SZ_TYPE_BF16;
     __shared__ float2 turn[R][HD / 2];
     __shared__ float tmp[8][HD];
@@ -206,9 +206,10 @@ __global__ void __launch_bounds__(256) sz_pg_append_kernel(const __grid_constant
         head(kind1, one, w ? norm(one) : 1.f, w, ww, kind1 == 0 ? a.qo + r * a.qo_stride + h1 * (HD * ESZ) : (u8*)(kind1 == 1 ? d.k : d.v) + off + h1 * d.head_stride);
         return;
     }
-    // A warp has a row and takes its heads four at a time: their loads are under way together.
+    // A warp has a row and takes its heads two at a time: their loads are under way together.  (Four: 80 registers, 24 warps a multiprocessor
+    // instead of 32, 29 us at 4,093 rows where this takes 22.)
     auto heads = [&](auto kind, int n, const u8* src, long long step, u8* dst, long long dst_step, const float* w) {
-        constexpr int B = 4;
+        constexpr int B = 2;
         src += d0 * ESZ;
         float ww[E];
         load_w(w, ww);

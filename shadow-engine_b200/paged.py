@@ -70,6 +70,7 @@ class Step:
         if shared_len and shared_pages.shape[0] * cache.c.page_size < shared_len:
             raise ValueError("shared_pages hold %d positions, shared_len is %d" % (shared_pages.shape[0] * cache.c.page_size, shared_len))
         self.cache, self.n_head, self.rows, self.device = cache, n_head, rows, cache.device
+        self.hd, self._index = cache.head_dim, cache.device.index
         self.nkv, self._scale = cache.c.n_kv_head, 1 / math.sqrt(cache.head_dim)
         self._keep = (pages, row_start, lens, shared_pages)
         self.b = PagedBatchC(n_seq=n, rows=rows, max_pages=pages.shape[1], shared_len=shared_len, pages=pages.data_ptr(), row_start=row_start.data_ptr(),
@@ -84,37 +85,37 @@ class Step:
 
     def _here(self):
         """Makes the cache's device the current one, where another is."""
-        return _HERE if torch.cuda.current_device() == self.device.index else torch.cuda.device(self.device)
+        return _HERE if torch.cuda.current_device() == self._index else torch.cuda.device(self._index)
 
     def _stream(self):
-        return torch.cuda.current_stream(self.device).cuda_stream
+        return torch.cuda.current_stream(self._index).cuda_stream
 
-    def _rows(self, name, t, heads, dtype=None, apart=False):
-        """Checks [rows, heads, head_dim]; returns its address and its strides of rows and (apart: any) heads."""
-        hd = self.cache.head_dim
+    def _rows(self, name, t, heads, dtype, apart=False):
+        """Checks [rows, heads, head_dim] of dtype; returns its address and its strides of rows and (apart: any) heads."""
+        hd = self.hd
         if t.shape != (self.rows, heads, hd) or t.device != self.device:
             raise ValueError("%s: [%d, %d, %d] on the cache's device" % (name, self.rows, heads, hd))
-        if t.dtype not in TYPES or (dtype is not None and t.dtype != dtype):
+        if t.dtype is not dtype or dtype not in TYPES:
             raise ValueError("%s: float32, float16 or bfloat16, the same for all rows of a call" % name)
         row, head, one = t.stride()
         if one != 1:
             raise ValueError("%s: the last dimension contiguous" % name)
-        if heads == 1:
-            head = hd
-        elif head != hd and (not apart or head < hd):
-            raise ValueError("%s: heads %s" % (name, "that overlap" if apart else "side by side"))
-        need = (heads - 1) * head + hd
-        if row < need:
+        if head != hd:
+            if heads == 1:
+                head = hd
+            elif not apart or head < hd:
+                raise ValueError("%s: heads %s" % (name, "that overlap" if apart else "side by side"))
+        if row < (heads - 1) * head + hd:
             if self.rows > 1:
                 raise ValueError("%s: rows that overlap" % name)
-            row = need
+            row = (heads - 1) * head + hd
         return t.data_ptr(), row, head
 
     def append(self, k, v, q=None, q_out=None, rope_dims=0, theta=1e4, q_norm=None, k_norm=None, eps=1e-6):
         """Stores the rows' keys (normed, turned) and values at their positions; returns the rows' queries, normed and turned (None without q).
         k, v [rows, kv heads, head_dim]; q [rows, heads, head_dim] (any stride of heads); q_norm, k_norm float32 [head_dim]."""
-        hd, nkv, dt = self.cache.head_dim, self.nkv, k.dtype
-        kp, ks, _ = self._rows("k", k, nkv)
+        hd, nkv, dt = self.hd, self.nkv, k.dtype
+        kp, ks, _ = self._rows("k", k, nkv, dt)
         vp, vs, _ = self._rows("v", v, nkv, dt)
         qp = qs = qh = op = os = qn = kn = 0
         if q is not None:
@@ -144,8 +145,8 @@ class Step:
     def attend(self, q, out=None, scale=None, gate=None, lse=None):
         """Attention of the rows over their sequences' positions up to their own, shared ones first.  q [rows, heads, head_dim]; gate: the
         same (any stride of heads), out *= sigmoid(gate); lse float32 [rows, heads] receives the logarithm of the softmax's denominator; scale 1 / sqrt(head_dim)."""
-        qp, qs, _ = self._rows("q", q, self.n_head)
         dt = q.dtype
+        qp, qs, _ = self._rows("q", q, self.n_head, dt)
         if out is None:
             out = torch.empty(q.shape, dtype=dt, device=q.device)
         op, os, _ = self._rows("out", out, self.n_head, dt)

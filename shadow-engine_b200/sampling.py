@@ -35,7 +35,7 @@ def sample_rows(logits, uniform, temperature=None, top_k=None, top_p=None, min_p
     ptrs = (at("temperature", temperature, f32), at("top_k", top_k, torch.int32), at("top_p", top_p, f32), at("min_p", min_p, f32), at("uniform", uniform, torch.float64),
             at("out", out, torch.int32), at("prob", prob, f32))
     with _HERE if torch.cuda.current_device() == dev.index else torch.cuda.device(dev):
-        rc = L.sz_sample_rows(TYPES[logits.dtype], logits.data_ptr(), stride, rows, vocab, *ptrs, torch.cuda.current_stream(dev).cuda_stream)
+        rc = L.sz_sample_rows(TYPES[logits.dtype], logits.data_ptr(), stride, rows, vocab, *ptrs, torch.cuda.current_stream(dev.index).cuda_stream)
     if rc:
         szlib.check(rc)
     return out
