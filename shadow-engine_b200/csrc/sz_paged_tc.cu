@@ -178,6 +178,7 @@ sz_pg_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
         it.end = pg_tile_end(d, row_of(bl + 1) - row_of(bl), end_of(bl), it.t, C::TQ);
         return it;
     };
+    const PgItem first = work ? locate(u0) : PgItem();      // (by all warps at once: the roles' own copies of this code would be fetched one beside the other)
     int failed = 0;
     if (warp == TMA_WARP || warp == TMA_WARP + 1) {
         // ---- loads, of keys and of values: units in order.  Pages are looked up a window of units ahead (32 entries of the table, one a lane): one after the
@@ -189,7 +190,7 @@ sz_pg_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
         u8* const to = kind ? vring : ring;
         u32 g = 0;                                         // units so far
         for (u32 u = u0; u < u1 && !failed;) {
-            const PgItem it = locate(u);
+            const PgItem it = u == u0 ? first : locate(u);
             const int T = (int)min((u32)(it.n - it.i), u1 - u);
             const int32_t* table = pt.shared ? d.shared_pages : d.pages + (size_t)it.b * d.max_pages;
             auto window = [&](int w) {
@@ -241,7 +242,7 @@ sz_pg_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
         const u64 qd = pt_desc(sz_smem_addr(sq), 16, 1024), kd = pt_desc(sz_smem_addr(ring), 16, 1024);
         u32 piece = 0, done = 0;                           // pieces; units before this one
         for (u32 u = u0; u < u1 && !failed; piece++) {
-            const PgItem it = locate(u);
+            const PgItem it = u == u0 ? first : locate(u);
             const int T = (int)min((u32)(it.n - it.i), u1 - u);
             for (int q = 0; q < C::NQ && !failed; q++) if (!pt_wait_warp(&S.q_full[q], piece)) failed = 2;
             for (int j = 0; j < T && !failed; j++) {
@@ -276,7 +277,7 @@ sz_pg_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
         const u64 vd = pt_desc(sz_smem_addr(vring), C::BLK, 1024);
         u32 piece = 0, done = 0;
         for (u32 u = u0; u < u1 && !failed; piece++) {
-            const PgItem it = locate(u);
+            const PgItem it = u == u0 ? first : locate(u);
             const int T = (int)min((u32)(it.n - it.i), u1 - u);
             for (int j = 0; j < T && !failed; j++) {
                 const u32 g = done + j;
@@ -311,7 +312,7 @@ sz_pg_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
         const u32 lanes = (u32)((warp & 3) * 32) << 16;
         u32 piece = 0, done = 0;                           // done: units so far
         for (u32 u = u0; u < u1 && !failed; piece++) {
-            const PgItem it = locate(u);
+            const PgItem it = u == u0 ? first : locate(u);
             const int T = (int)min((u32)(it.n - it.i), u1 - u);
             const int r0 = row_of(it.b), m = (pt.shared ? row_of(d.n_seq) : row_of(it.b + 1)) - r0;
             const int v = q * 128 + row, vec = it.t * C::TQ + v, qr = vec / d.G, head = it.h * d.G + vec % d.G;
@@ -323,7 +324,7 @@ sz_pg_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
             {   // the query vector into the K-major order: chunk c of 8 dimensions of row r at chunk c ^ (r & 7) of its 128 bytes
                 const uint4* src = (const uint4*)(io.q + (long long)(r0 + qr) * io.q_stride + (long long)head * HD * 2);
                 u8* dst = sq + q * C::QT + row * 128;
-#pragma unroll 8
+#pragma unroll 16
                 for (int c = 0; c < HD / 8; c++) {
                     const uint4 w = qr < m ? __ldg(src + c) : make_uint4(0, 0, 0, 0);
                     *(uint4*)(dst + c / 8 * C::QBLK + (((c & 7) ^ (row & 7)) << 4)) = w;
@@ -430,7 +431,10 @@ sz_pg_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
             const int b0 = pg_block_of(share, us), b1 = pg_block_of(share, us + it.n - 1);
             const bool alone = b0 == b1, direct = alone && pt.direct, odd = S.odd[piece & 1] == piece + 1;
             const size_t to = alone ? (size_t)(r0 + qr) * (d.nkv * d.G) + head : (size_t)(2 * blockIdx.x + ((int)blockIdx.x == b0 ? 1 : 0)) * C::TQ + v;
-            float* const w = (alone ? pt.row_o : pt.o) + to * HD;
+            float* const w = qr < m ? (alone ? pt.row_o : pt.o) + to * HD : nullptr;
+            // parts go out through the warp's own 4 KB of the queries' first block (whose products are done): a lane's own row, 16 bytes at a time,
+            // would be 32 lines a store, 11,000 cycles for two tiles of 128 columns
+            u8* const turn = sq + q * C::QT + (warp & 3) * 4096;
             u8* const op = io.out + (long long)(r0 + qr) * io.out_stride + (long long)head * HD * 2;
             const u8* const gp = io.gate ? io.gate + (long long)(r0 + qr) * io.gate_stride + (long long)head * io.gate_head_stride : nullptr;
             const bool none = lim <= 0 || l == 0.f;
@@ -440,8 +444,7 @@ sz_pg_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
                 float o[32];
                 pt_ld32(tmem + lanes + 256 + q * HD + k, o);
                 pt_loaded(o);
-                if (qr >= m) continue;
-                if (odd) {                                 // the values that were cleared, where this row sees them
+                if (odd && qr < m) {                                 // the values that were cleared, where this row sees them
                     const int32_t* table = pt.shared ? d.shared_pages : d.pages + (size_t)it.b * d.max_pages;
                     for (int t = max(it.i * C::UT, all & ~(C::UT - 1)); t < min(lim, (it.i + T) * C::UT); t++) {
                         const int page = __ldg(table + (t >> d.ps_log2));
@@ -457,9 +460,19 @@ sz_pg_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
                 }
                 if (!direct) {
 #pragma unroll
-                    for (int e = 0; e < 32; e += 4) *(float4*)(w + k + e) = make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+                    for (int c = 0; c < 8; c++) *(float4*)(turn + lane * 128 + ((c ^ (lane & 7)) << 4)) = make_float4(o[4 * c], o[4 * c + 1], o[4 * c + 2], o[4 * c + 3]);
+                    __syncwarp();
+#pragma unroll
+                    for (int i = 0; i < 8; i++) {
+                        const int r = 4 * i + (lane >> 3), c = lane & 7;
+                        float* const at = (float*)__shfl_sync(0xffffffffu, (unsigned long long)w, r);
+                        const float4 f = *(const float4*)(turn + r * 128 + ((c ^ (r & 7)) << 4));
+                        if (at) *(float4*)(at + k + 4 * c) = f;
+                    }
+                    __syncwarp();
                     continue;
                 }
+                if (qr >= m) continue;
 #pragma unroll
                 for (int e = 0; e < 32; e += 8) {
                     u32 y[4], z[4] = {};
