@@ -17,8 +17,8 @@
 //   last four   keys, and values, by tiled TMA, a box a page (8 .. 64 positions x 64 dimensions, 128-byte swizzle), each through a ring of 64 positions x
 //               128 dimensions; the two issuing warps.
 // Operands: queries and keys K-major, values MN-major (their rows are the positions, which the product sums over), weights from tensor memory.
-// Measured: 2,045 rows of 16 heads of 256 on 2 behind 7,555 positions, bf16: 362 us, 0.79 PFLOP/s (the products alone at the measured rate 175); 64 rows of 32 heads
-// of 128 over 24,576 shared positions 53 us (42).  What bounds it is the chain of a tile - scores, softmax, weights, product -: at head_dim 256 tensor memory
+// Measured: 2,045 rows of 16 heads of 256 on 2 behind 7,555 positions, bf16: 308 us, 0.93 PFLOP/s (the products alone at the measured rate 175); 64 rows of 32 heads
+// of 128 over 24,576 shared positions some 47 us (16 of bytes or products).  What bounds it is the chain of a tile - scores, softmax, weights, product -: at head_dim 256 tensor memory
 // holds one tile's sums and two buffers of its scores, so that the softmax of a unit has the products of its neighbours only to run beside; up to 128
 // the exponentials (16,384 for 128 vectors and 128 positions) take the multiprocessor as long as both products take the tensor core.
 // Rounding: a weight has 8 (bf16) or 11 bits, as the result; its sum is of the unrounded ones.  (Errors of independent weights average out:
@@ -321,13 +321,15 @@ sz_pg_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
             const int room = pg_room(d);
             const int lim = qr >= m ? 0 : pt.shared ? d.shared_len : (int)max(0ll, min(oend - (m - 1 - qr), (long long)room));
             const int all = pt.shared ? d.shared_len : (int)max(0ll, min(oend - (m - 1 - it.t * C::TQ / d.G), (long long)room));
-            {   // the query vector into the K-major order: chunk c of 8 dimensions of row r at chunk c ^ (r & 7) of its 128 bytes
-                const uint4* src = (const uint4*)(io.q + (long long)(r0 + qr) * io.q_stride + (long long)head * HD * 2);
-                u8* dst = sq + q * C::QT + row * 128;
-#pragma unroll 16
-                for (int c = 0; c < HD / 8; c++) {
-                    const uint4 w = qr < m ? __ldg(src + c) : make_uint4(0, 0, 0, 0);
-                    *(uint4*)(dst + c / 8 * C::QBLK + (((c & 7) ^ (row & 7)) << 4)) = w;
+            {   // the warp's query vectors into the K-major order: chunk c of 8 dimensions of row r at chunk c ^ (r & 7) of its 128 bytes; four rows' 128 bytes at a time
+                const u8* const src = qr < m ? io.q + (long long)(r0 + qr) * io.q_stride + (long long)head * HD * 2 : nullptr;
+                u8* const dst = sq + q * C::QT + (warp & 3) * 4096;
+#pragma unroll 4
+                for (int i = 0; i < 8; i++) {
+                    const int r = 4 * i + (lane >> 3), c = lane & 7;
+                    const uint4* const from = (const uint4*)__shfl_sync(0xffffffffu, (unsigned long long)src, r);
+#pragma unroll
+                    for (int k = 0; k < HD / 64; k++) *(uint4*)(dst + k * C::QBLK + r * 128 + ((c ^ (r & 7)) << 4)) = from ? __ldg(from + 8 * k + c) : make_uint4(0, 0, 0, 0);
                 }
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 pt_arrive_warp(&S.q_full[q]);
@@ -433,7 +435,7 @@ sz_pg_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
             const size_t to = alone ? (size_t)(r0 + qr) * (d.nkv * d.G) + head : (size_t)(2 * blockIdx.x + ((int)blockIdx.x == b0 ? 1 : 0)) * C::TQ + v;
             float* const w = qr < m ? (alone ? pt.row_o : pt.o) + to * HD : nullptr;
             // parts go out through the warp's own 4 KB of the queries' first block (whose products are done): a lane's own row, 16 bytes at a time,
-            // would be 32 lines a store, 11,000 cycles for two tiles of 128 columns
+            // would be 32 lines a store, 11,000 cycles for two tiles of 128 columns (the chunk of 2,045 rows 349 -> 314 us)
             u8* const turn = sq + q * C::QT + (warp & 3) * 4096;
             u8* const op = io.out + (long long)(r0 + qr) * io.out_stride + (long long)head * HD * 2;
             const u8* const gp = io.gate ? io.gate + (long long)(r0 + qr) * io.gate_stride + (long long)head * io.gate_head_stride : nullptr;
