@@ -172,7 +172,7 @@ __device__ int pg_plan(const PgBatch& d, int shared, int unit, int tq, u32* tile
 //   quarter of the step that the result itself is rounded to).
 // f16 pieces are kept in range: queries are divided by a power of two near their largest element, weights are 2^15 times themselves (so
 // that small ones do not run into f16's subnormals), and both are taken back in f32.  A packed value's scale goes into the weight (times a
-// power of two that follows the scales, CSC), a packed key's into the 32-dimension partial scores in f32: codes themselves are exact in f16.
+// power of two that follows the scales a row sees, csc), a packed key's into the 32-dimension partial scores in f32: codes themselves are exact in f16.
 // Measured: 64 sequences, 163 rows of 32 heads of 128 on 8, bf16, contexts of 3,000 to 15,000: 398 us (360 are the bytes at the measured copy rate: memory
 // bounds it).  Few rows wait for one thing after the other instead: plan, pages, keys, products, values, products.  Four rows of 16 heads of 256 on 2
 // over 24,576 packed positions 55 us, 101 such rows behind 9,599 shared ones 252: 12 instructions (codes to f16, scales, pieces of weights) for
@@ -356,8 +356,8 @@ sz_pg_attend_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_const
         if (NQT > 1) __syncthreads();
     };
 
-    float o[C::NT][4], p[C::SG][8], m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f, csc = 1.f;
-    bool fresh = true;                                    // the maxima moved since the values' scale was chosen
+    float o[C::NT][4], p[C::SG][8], m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f, csc0 = 1.f, csc1 = 1.f;
+    bool fresh = true;                                    // the maxima moved since the values' scales were chosen
     int lim0 = 0, lim1 = 0;
     float f0 = 0.f, f1 = 0.f;
     int cslot = 0;
@@ -413,7 +413,7 @@ sz_pg_attend_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_const
             f0 = s_fac[qt * 16 + g8]; f1 = s_fac[qt * 16 + g8 + 8];
 #pragma unroll
             for (int b = 0; b < C::NT; b++) { o[b][0] = 0.f; o[b][1] = 0.f; o[b][2] = 0.f; o[b][3] = 0.f; }
-            m0 = m1 = -INFINITY; l0 = l1 = 0.f; csc = 1.f; fresh = true;
+            m0 = m1 = -INFINITY; l0 = l1 = 0.f; csc0 = csc1 = 1.f; fresh = true;
         }
         // ---- the unit's keys: scores, maxima, weights
         arrived(cslot);
@@ -491,6 +491,7 @@ sz_pg_attend_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_const
             }
         }
         bool hidden = false;                              // a position that is there, but not for this lane's rows
+        bool part = false;                                // one that is not there, or not for them
         float x0 = -INFINITY, x1 = -INFINITY;
 #pragma unroll
         for (int g = 0; g < C::SG; g++)
@@ -503,6 +504,7 @@ sz_pg_attend_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_const
                     s[g][n][c] = a ? s[g][n][c] * f0 : -INFINITY;
                     s[g][n][2 + c] = b ? s[g][n][2 + c] * f1 : -INFINITY;
                     hidden |= ok && c0 + pi < it.end && !(a && b);
+                    part |= !(a && b);
                     x0 = fmaxf(x0, s[g][n][c]); x1 = fmaxf(x1, s[g][n][2 + c]);
                 }
 #pragma unroll
@@ -597,33 +599,57 @@ sz_pg_attend_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_const
             }
         } else {
             const u8* vr = ring + (size_t)cslot * C::HALF + (size_t)pw * C::HB;
-            bool odd;                                     // a scale that is infinite or NaN: it must not reach a hidden position's weight of 0
-            {   // the power of two that brings this unit's largest value scale to [2^-1, 1) (weights: 2^15 at most)
-                u32 top = 0;
+            bool odd;                                     // a scale that is infinite or NaN, or not a row's: it must not reach a hidden position's weight of 0
+            {   // the powers of two that bring the largest value scale each of the lane's rows sees to [2^-1, 1) (weights: 2^15 at most).  What a row does
+                // not see - later rows' positions, slots that nothing was written to - has no say: one scale of 65,504 there would leave its weights
+                // f16's subnormals.  Where all rows see all positions, which is the rule, one maximum does for all.
+                u32 t0 = 0, t1 = 0;
+                const bool clear = !__any_sync(0xffffffffu, part);
+                if (clear) {
 #pragma unroll
-                for (int i = 0; i < (16 * C::SG * HD / 64 + 31) / 32; i++) {
-                    const int x = lane + 32 * i, r = x / (HD / 64), w2 = x % (HD / 64);
-                    if (16 * C::SG * HD / 64 % 32 == 0 || r < 16 * C::SG) {
-                        const u32 w = *(const u32*)(vr + (size_t)r * C::HB + HD + 4 * w2);
-                        top = max(top, max(w & 0x7fffu, (w >> 16) & 0x7fffu));
+                    for (int i = 0; i < (16 * C::SG * HD / 64 + 31) / 32; i++) {
+                        const int x = lane + 32 * i, r = x / (HD / 64), w2 = x % (HD / 64);
+                        if (16 * C::SG * HD / 64 % 32 == 0 || r < 16 * C::SG) {
+                            const u32 w = *(const u32*)(vr + (size_t)r * C::HB + HD + 4 * w2);
+                            t0 = max(t0, max(w & 0x7fffu, (w >> 16) & 0x7fffu));
+                        }
                     }
-                }
-                top = __reduce_max_sync(0xffffffffu, top);
-                const int ex = top >> 10 ? (int)(top >> 10) - 14 : -14;             // scale < 2^ex
-                const float want = __uint_as_float((u32)(127 - ex) << 23);
-                if (want < csc || (fresh && want != csc)) {
-                    const float by = want / csc;                                     // (powers of two: exact)
+                    t0 = t1 = __reduce_max_sync(0xffffffffu, t0);
+                } else {
+#pragma unroll 1
+                    for (int r = q4; r < 16 * C::SG; r += 4) {      // the four lanes of a row share its positions
+                        u32 big = 0;
 #pragma unroll
-                    for (int b = 0; b < C::NT; b++) { o[b][0] *= by; o[b][1] *= by; o[b][2] *= by; o[b][3] *= by; }
-                    csc = want;
+                        for (int i = 0; i < HD / 64; i++) {
+                            const u32 w = *(const u32*)(vr + (size_t)r * C::HB + HD + 4 * i);
+                            big = max(big, max(w & 0x7fffu, (w >> 16) & 0x7fffu));
+                        }
+                        const bool ok = (okb >> r) & 1u;
+                        if (ok && c0 + r < lim0) t0 = max(t0, big);
+                        if (ok && c0 + r < lim1) t1 = max(t1, big);
+                    }
+                    __syncwarp();
+#pragma unroll
+                    for (int k = 1; k < 4; k <<= 1) { t0 = max(t0, __shfl_xor_sync(0xffffffffu, t0, k)); t1 = max(t1, __shfl_xor_sync(0xffffffffu, t1, k)); }
+                }
+                auto moved = [&](u32 top, float csc) {    // what the row's sums are multiplied by (powers of two: exact)
+                    const int ex = top >> 10 ? (int)(top >> 10) - 14 : -14;         // scale < 2^ex
+                    const float want = __uint_as_float((u32)(127 - ex) << 23);
+                    return top && (want < csc || (fresh && want != csc)) ? want / csc : 1.f;
+                };
+                const float by0 = moved(t0, csc0), by1 = moved(t1, csc1);
+                if (__any_sync(0xffffffffu, by0 != 1.f || by1 != 1.f)) {
+#pragma unroll
+                    for (int b = 0; b < C::NT; b++) { o[b][0] *= by0; o[b][1] *= by0; o[b][2] *= by1; o[b][3] *= by1; }
+                    csc0 *= by0; csc1 *= by1;
                 }
                 fresh = false;
-                odd = top >= 0x7c00u;
+                odd = !clear || t0 >= 0x7c00u;
             }
 #pragma unroll
             for (int g = 0; g < C::SG; g++)
 #pragma unroll
-                for (int e = 0; e < 8; e++) p[g][e] *= csc;      // (a power of two: exact, but for weights of 2^-100 and less)
+                for (int e = 0; e < 8; e++) p[g][e] *= e & 2 ? csc1 : csc0;      // (a power of two: exact, but for weights of 2^-100 and less)
 #pragma unroll
             for (int g = 0; g < C::SG; g++) {
                 u32 vs[4];
@@ -669,14 +695,14 @@ sz_pg_attend_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_const
         // ---- the block's last unit of the item: its parts go out, every way's by itself - but at the block's end, where the ring lies idle, the ways
         // are added up there first, and one part goes out for all (the others' maxima say that they are empty).  One long conversation is split
         // over all blocks: its parts, 16 KB a warp, took longer to write and to join than to make.
-        const float back = CT == PG_BF16 ? 1.f : 1.f / 32768.f, un = back / csc;
+        const float back = CT == PG_BF16 ? 1.f : 1.f / 32768.f, un0 = back / csc0, un1 = back / csc1;
 #pragma unroll
         for (int k = 1; k < 4; k <<= 1) { l0 += __shfl_xor_sync(0xffffffffu, l0, k); l1 += __shfl_xor_sync(0xffffffffu, l1, k); }
         l0 *= back; l1 *= back;
         if (l0 != l0 && m0 == -INFINITY) m0 = 0.f;        // (scores that are all NaN have no maximum, and are not an empty part)
         if (l1 != l1 && m1 == -INFINITY) m1 = 0.f;
 #pragma unroll
-        for (int b = 0; b < C::NT; b++) { o[b][0] *= un; o[b][1] *= un; o[b][2] *= un; o[b][3] *= un; }
+        for (int b = 0; b < C::NT; b++) { o[b][0] *= un0; o[b][1] *= un0; o[b][2] *= un1; o[b][3] *= un1; }
         if (C::WAYS > 1 && u + 1 == u1) {
             constexpr int ST = HD + 8;                    // floats a row: rows begin at different banks
             static_assert((C::WAYS - 1) * NQT * 16 * ST * 4 <= C::NR * C::HALF && (C::WAYS - 1) * NQT * 16 * 8 <= C::QB, "the parts fit the ring");

@@ -624,3 +624,53 @@ def test_what_the_scratch_held_does_not_matter(n, m, shared, io, cache):
     for byte in (0, 255, 63):
         c.step._mem[at + 256:].fill_(byte)           # (the first 256 bytes hold the status)
         assert torch.equal(c.check(), first)
+
+
+@pytest.mark.parametrize("cache", ["f16", "bf16", "q8"])
+@pytest.mark.parametrize("lens,ms,shared", [([130, 77], [3, 1], 0), ([300, 260, 290], [2, 1, 30], 250)])
+def test_f32_rows_keep_their_accuracy(cache, lens, ms, shared):
+    """Heads of 64, scores of six and less with magnitudes |q_i k_i| scale below 16 in sum.  A score's f32 sums cut 2^-23 of it in each of four steps, a query's pieces
+    leave 2^-23 of every product: 4 6 2^-23 + 16 2^-23 = 2^-17.7 at most, a weight as much, and the quotient of two sums of weights twice
+    that: below 2^-16 of the weighted magnitudes, with weights of 22 bits and more.  (One piece of 11 bits would be four to ten times over it.)"""
+    c = Case(lens, ms, nh=8, nkv=2, hd=64, io="f32", cache=cache, shared=shared, seed=40)
+    out = c.step.attend(c.q)
+    want, mag, _ = c.want()
+    off = (out.double() - want).abs() / (2.0 ** -24 * want.abs() + 2.0 ** -16 * mag)
+    assert float(off.max()) < 1.0, float(off.max())
+
+
+def spoil(pool, hd, page, slots, scale, groups=slice(None)):
+    """Packed heads at `slots` of a page: codes of 127 under scales of `scale`."""
+    at = pool[page, :, slots]
+    at[..., :hd] = 127
+    sc = at[..., hd:hd + hd // 16].contiguous().view(torch.float16)
+    sc[..., groups] = scale
+    at[..., hd:hd + hd // 16] = sc.view(torch.uint8)
+    pool[page, :, slots] = at
+
+
+@pytest.mark.parametrize("bad", [65504.0, math.inf, math.nan])
+@pytest.mark.parametrize("io,hd,m,size", [("f32", 64, 4, 1.0), ("f32", 256, 4, 1e-3), ("bf16", 128, 4, 1e-3), ("f32", 128, 20, 0.01), ("f16", 256, 20, 0.01), ("bf16", 64, 9, 1.0)])
+def test_what_hidden_packed_positions_hold_does_not_matter(io, hd, m, size, bad):
+    """As above for packed heads: a scale that no row may see, or only a later one, chooses nothing for the others - not a bit."""
+    c = Case([70, 33], [m, 2], cache="q8", io=io, nh=8, nkv=2, hd=hd, seed=41, scale_kv=size)
+    before = c.check().clone()
+    last = c.pages[0, (70 - 1) // 16]
+    spoil(c.k, hd, last, slice(70 % 16, None), bad)
+    spoil(c.v, hd, last, slice(70 % 16, None), bad)
+    assert torch.equal(c.step.attend(c.q), before)
+    spoil(c.v, hd, last, slice(69 % 16, 70 % 16), bad, slice(0, 1))                    # the last row's own: its output, and no other row's
+    out = c.step.attend(c.q)
+    assert torch.equal(out[:m - 1], before[:m - 1]) and torch.equal(out[m:], before[m:])
+    if not math.isfinite(bad):
+        assert not bool(torch.isfinite(out[m - 1, :, :32]).any()) and bool(torch.isfinite(out[m - 1, :, 32:]).all())
+
+
+def test_scales_far_apart_on_one_head():
+    """A unit's largest value scale is 2^29 times its smallest: the small ones' positions keep their bits in rows that do not see the large one."""
+    for m in (3, 20):
+        c = Case([64 + m], [m], cache="q8", io="f32", nh=4, nkv=1, hd=64, seed=42, scale_kv=1e-3)
+        c.v[c.pages[0, (64 + m - 1) // 16], :, (64 + m - 1) % 16] = q8_pack(1e6 * c.rnd(1, 64))
+        out = c.step.attend(c.q)
+        want, mag, _ = c.want()
+        assert float(((out.double() - want).abs() / (2.0 ** -16 * mag + 2.0 ** -24 * want.abs()))[:m - 1].max()) < 1.0
