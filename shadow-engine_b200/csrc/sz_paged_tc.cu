@@ -12,8 +12,8 @@
 // unit without waiting for its products.  (One warp for both: 2,860 cycles for two tiles and 64 positions, whose instructions need 1,280.  Units of 128
 // positions with one buffer a tile, where softmax, products and scores take turns: 5,900 for 128.)
 //   warps 0 .. 3 (and 4 .. 7 for the second tile)   a thread has a query vector, lane = row of tensor memory: it reads its 64 scores
-//               (tcgen05.ld), moves its maximum - only when the largest is 2^8 above what it divides by, for then the sums have to be read,
-//               scaled and written back; weights up to 256 cost f32 and the 16-bit types nothing -, writes the weights (tcgen05.st) and keeps their sum.
+//               (tcgen05.ld), moves what it divides by - only when the largest weight would be beyond 2^8 (f16: 2^15), for then the sums have to be
+//               read, scaled and written back -, writes the weights (tcgen05.st) and keeps their sum.
 //   last four   keys, and values, by tiled TMA, a box a page (8 .. 64 positions x 64 dimensions, 128-byte swizzle), each through a ring of 64 positions x
 //               128 dimensions; the two issuing warps.
 // Operands: queries and keys K-major, values MN-major (their rows are the positions, which the product sums over), weights from tensor memory.
@@ -21,8 +21,11 @@
 // of 128 over 24,576 shared positions some 47 us (16 of bytes or products).  What bounds it is the chain of a tile - scores, softmax, weights, product -: at head_dim 256 tensor memory
 // holds one tile's sums and two buffers of its scores, so that the softmax of a unit has the products of its neighbours only to run beside; up to 128
 // the exponentials (16,384 for 128 vectors and 128 positions) take the multiprocessor as long as both products take the tensor core.
-// Rounding: a weight has 8 (bf16) or 11 bits, as the result; its sum is of the unrounded ones.  (Errors of independent weights average out:
-// the result's error stays below 1.3 of its last rounding's.)
+// Rounding: a weight is one number of the rows' type, 8 (bf16) or 11 bits as the result; its sum is of the unrounded ones.  Errors of independent
+// weights average out to those of one rounding: the result is 1.4 times as far off as its last rounding alone (f32 rows 1.66e-3 of the results' norm, bf16
+// weights 2.33e-3).  A second piece, as the few-vector kernel has it, would double the product with the values.  bf16 has f32's range; in f16 the
+// largest weight lies between 2^11 and 2^15, so that those down to 2^-25 of it keep all their bits and those below 2^-36 are lost.  (With the largest
+// at 1 .. 2^8, as for bf16, a weight of e^-13 was 0.2 % off and one of e^-17 44 %: four half steps of the result, and nothing left of it, where the rest has no value.)
 // A page out of range arrives as zeros (its box lies outside the pool's map) and its positions are masked.  Every wait is bounded.
 //
 // What a row does not see must not reach it, whatever it is: scores of such positions are replaced, but a weight of 0 times a value that is infinite
@@ -85,6 +88,9 @@ __device__ __forceinline__ bool pt_wait(u64* bar, u32 phase) { return sz_mbar_wa
 __device__ __forceinline__ bool pt_wait_warp(u64* bar, u32 phase) { return __all_sync(0xffffffffu, pt_wait(bar, phase)); }
 __device__ __forceinline__ void pt_arrive_warp(u64* bar) { __syncwarp(); if ((threadIdx.x & 31) == 0) sz_mbar_arrive(bar); }
 
+// What a row divides by when it moves: the largest score less PT_UP (so the largest weight is 2^PT_UP); it moves where the largest would pass 2^PT_TOP.
+template <bool BF> constexpr float PT_UP = BF ? 0.f : 11.f;
+template <bool BF> constexpr float PT_TOP = BF ? 8.f : 15.f;
 __device__ __forceinline__ float pt_max3(float a, float b, float c) { float r; asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c)); return r; }
 template <int HD>
 struct PtCfg {
@@ -334,7 +340,7 @@ sz_pg_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 pt_arrive_warp(&S.q_full[q]);
             }
-            float mx = -INFINITY, l = 0.f;                 // what the row divides by (in units of log 2), the sum of its weights
+            float mx = -INFINITY, l = 0.f;                 // what the row's weights are divided by (its logarithm, base 2), their sum
             for (int j = 0; j < T; j++) {
                 const int buf = q * 2 + (int)(done & 1);
                 if (!pt_wait_warp(&S.s_full[buf], done >> 1)) { failed = 7; break; }
@@ -361,10 +367,10 @@ sz_pg_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
                 }
                 const float top = pt_max3(pt_max3(big[0], big[1], s[C::UT - 4]), pt_max3(big[2], big[3], s[C::UT - 3]), pt_max3(s[C::UT - 2], s[C::UT - 1], s[C::UT - 1])) * io.scale_log2;
                 if (!(top < INFINITY)) l = NAN;            // (a score that is NaN or infinite: so is the row)
-                const bool up = top > mx + 8.f || (mx == -INFINITY && top > -INFINITY);
+                const bool up = top > mx + PT_TOP<BF> || (mx == -INFINITY && top > -INFINITY);
                 if (__any_sync(0xffffffffu, up)) {
-                    const float by = !up ? 1.f : mx == -INFINITY ? 0.f : pg_ex2(mx - top);
-                    if (up) { mx = top; l *= by; }
+                    const float by = !up ? 1.f : mx == -INFINITY ? 0.f : pg_ex2(mx - (top - PT_UP<BF>));
+                    if (up) { mx = top - PT_UP<BF>; l *= by; }
                     if (j > 0) {                           // the sums so far, once the last product is in them
                         if (!pt_wait_warp(&S.pv_done[q * 2 + ((done - 1) & 1)], (done - 1) >> 1)) { failed = 8; break; }
                         pt_after();

@@ -674,3 +674,28 @@ def test_scales_far_apart_on_one_head():
         out = c.step.attend(c.q)
         want, mag, _ = c.want()
         assert float(((out.double() - want).abs() / (2.0 ** -16 * mag + 2.0 ** -24 * want.abs()))[:m - 1].max()) < 1.0
+
+
+@pytest.mark.parametrize("nats", [10, 13, 17])
+@pytest.mark.parametrize("hd", [64, 128, 256])
+@pytest.mark.parametrize("kind", ["f16", "bf16"])
+def test_a_tail_far_below_the_first_position(kind, hd, nats):
+    """A position of value 0 in front that takes nearly all the weight, and thousands far below it whose values are the answer: a weight e^-17 of the largest
+    keeps its type's bits (f16 11, bf16 8), so that each is off by half a step of its own size, and the sum by no more; the scores are equal, so nothing averages out.
+    f32's part of it: a score of `nats` and less is off by hd / 16 steps of 2^-23 of it, 2^-16 at most."""
+    n, nkv = 1024, 8                                                                 # (tiles and heads enough that a block takes nearly all of an item's positions)
+    c = Case([n + 1] * 640, [1] * 640, nh=64, nkv=nkv, hd=hd, io=kind, cache=kind, shared=n, page=64, seed=43)
+    c.q.zero_()
+    c.q[:, :, 0] = 4.0
+    c.k.zero_()
+    c.k[c.shared_pages[0], :, 0, 0] = 8.0 * nats                                     # its score: 4 * 8 nats / 32; all others': 0
+    c.v.abs_()
+    c.v[c.shared_pages[0], :, 0] = 0
+    out = c.step.attend(c.q, scale=1 / 32)
+    assert c.step.status() == 0
+    w = torch.full((n + 1,), math.exp(-nats), dtype=torch.float64, device="cuda")
+    w[0] = 1
+    for b in (0, 17, 333, 639):
+        want = torch.einsum("t,thd->hd", w, c.positions(c.v, b)).repeat_interleave(64 // nkv, 0) / w.sum()
+        off = (out[b].double() - want).abs() / (2 * HALF_STEP[c.io] * want + 2.0 ** -16 * want + (2.0 ** -25 if kind == "f16" else 0))      # (f16's subnormals: half of 2^-24)
+        assert float(off.max()) < 1.0, float(off.max())
