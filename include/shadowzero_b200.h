@@ -303,8 +303,11 @@ int sz_paged_append(const sz_paged_cache* cache, const sz_paged_batch* batch, co
  * is given; head h reads key head h / (n_head / n_kv_head).  q, out [rows][n_head][head_dim], gate's heads gate_head_stride apart, all of
  * io_type; lse (f32 [rows][n_head], 0: not wanted): the logarithm of the softmax's denominator, for hosts that join it with further keys.  A row
  * without a position of its own (lens[b] - shared_len below the sequence's rows: a padded sequence) gives zeros and -inf.
- * Scores, softmax and sums are f32; f32 queries keep theirs over any cache type, weights are split likewise (f16 and bf16 outputs: to
- * 16 bits and more before the last rounding). */
+ * Scores, softmax and sums are f32; the factors of the two products are 16-bit numbers or sums of two or three.  f32 rows: queries and weights
+ * keep 22 bits (bf16 caches: 24).  f16 rows: weights 22 bits (bf16 caches: 24); bf16 rows: 16 over a bf16 cache, 22 over f16, 11 over a packed one.  Where a call has
+ * many 16-bit rows over a cache of their own type - 96 and more query vectors a key head, of a sequence on average or, over shared
+ * positions, of the batch - weights keep the rows' own 11 (f16) or 8 bits (bf16), and results are 1.4 times as far off as by their last
+ * rounding alone: a row's last bit depends on how many rows the call has.  Weights of less than 2^-36 (f16 caches and rows) of a row's largest are lost. */
 int sz_paged_attend(const sz_paged_cache* cache, const sz_paged_batch* batch, int io_type, int n_head, float scale, uint64_t q, int64_t q_stride, uint64_t gate,
                     int64_t gate_stride, int64_t gate_head_stride, uint64_t out, int64_t out_stride, uint64_t lse, uint64_t scratch, int64_t scratch_bytes,
                     uint64_t stream);
