@@ -331,13 +331,13 @@ sz_pg_attend_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_const
             }
             if (lane == 0) sz_mbar_expect_tx(bar, (u32)(16 * C::HB));
             __syncwarp();
-            if (lane < boxes) {
-                u8* const dst = CT == PG_Q8 ? ring + (size_t)lslot * C::HALF + (size_t)(warp * 16 + piece * rows_box) * C::HB
-                                            : ring + (size_t)lslot * C::HALF + (size_t)(lane % C::BOXES) * PG_T * 128 + (size_t)(warp * 16 + piece * rows_box) * 128;
-                asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(sz_smem_addr(dst)),
-                             "l"(which ? &vmap : &kmap), "r"(lane % C::BOXES * 64), "r"(c & ((1 << d.ps_log2) - 1)), "r"(ld.h), "r"(at_page), "r"(sz_smem_addr(bar))
-                             : "memory");
-            }
+            // (under a predicate, not a branch: what comes next, ldmatrix and mma.sync, is for the whole warp)
+            u8* const dst = CT == PG_Q8 ? ring + (size_t)lslot * C::HALF + (size_t)(warp * 16 + piece * rows_box) * C::HB
+                                        : ring + (size_t)lslot * C::HALF + (size_t)(lane % C::BOXES) * PG_T * 128 + (size_t)(warp * 16 + piece * rows_box) * 128;
+            asm volatile("{ .reg .pred q; setp.ne.b32 q, %7, 0;\n"
+                         "  @q cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6]; }" ::"r"(sz_smem_addr(dst)),
+                         "l"(which ? &vmap : &kmap), "r"(lane % C::BOXES * 64), "r"(c & ((1 << d.ps_log2) - 1)), "r"(ld.h), "r"(at_page), "r"(sz_smem_addr(bar)), "r"((u32)(lane < boxes))
+                         : "memory");
         }
         if (which && ++lu < u1) {                         // on to the next unit
             if (++ld.i == ld.n) ld = locate(lu);

@@ -14,6 +14,7 @@
 //   warps 0 .. 3 (and 4 .. 7 for the second tile)   a thread has a query vector, lane = row of tensor memory: it reads its 64 scores
 //               (tcgen05.ld), moves what it divides by - only when the largest weight would be beyond 2^8 (f16: 2^15), for then the sums have to be
 //               read, scaled and written back -, writes the weights (tcgen05.st) and keeps their sum.
+// (tcgen05.ld, st, their waits and alloc are for whole warps: wherever lanes went different ways before one, __syncwarp brings them together.)
 //   last four   keys, and values, by tiled TMA, a box a page (8 .. 64 positions x 64 dimensions, 128-byte swizzle), each through a ring of 64 positions x
 //               128 dimensions; the two issuing warps.
 // Operands: queries and keys K-major, values MN-major (their rows are the positions, which the product sums over), weights from tensor memory.
@@ -133,6 +134,7 @@ sz_pg_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
         sz_mbar_fence_init();
     }
     if (warp == 0) {
+        __syncwarp();
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(sz_smem_addr(&S.tmem)), "r"(512u) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
@@ -374,6 +376,7 @@ sz_pg_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
                     if (j > 0) {                           // the sums so far, once the last product is in them
                         if (!pt_wait_warp(&S.pv_done[q * 2 + ((done - 1) & 1)], (done - 1) >> 1)) { failed = 8; break; }
                         pt_after();
+                        __syncwarp();
 #pragma unroll 1
                         for (int k = 0; k < HD; k += 32) {
                             float o[32];
@@ -385,6 +388,7 @@ sz_pg_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
                             pt_st16(tmem + lanes + 256 + q * HD + k + 16, (const u32*)o + 16);
                         }
                     }
+                    __syncwarp();
                 }
                 const float sub = mx == -INFINITY ? 0.f : mx;
                 float sum[4] = {0.f, 0.f, 0.f, 0.f};
@@ -425,6 +429,7 @@ sz_pg_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
                     }
                     if (failed) break;
                     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                    __syncwarp();
                 }
                 pt_stored();
                 pt_before();
@@ -450,6 +455,7 @@ sz_pg_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
 #pragma unroll 1
             for (int k = 0; k < HD; k += 32) {
                 float o[32];
+                __syncwarp();                                        // (loads from tensor memory want the whole warp, and not all lanes have a row to write)
                 pt_ld32(tmem + lanes + 256 + q * HD + k, o);
                 pt_loaded(o);
                 if (odd && qr < m) {                                 // the values that were cleared, where this row sees them
@@ -480,20 +486,22 @@ sz_pg_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
                     __syncwarp();
                     continue;
                 }
-                if (qr >= m) continue;
+                if (qr < m) {
 #pragma unroll
-                for (int e = 0; e < 32; e += 8) {
-                    u32 y[4], z[4] = {};
-                    if (gp) { const uint4 g = __ldg((const uint4*)(gp + 2 * (k + e))); z[0] = g.x; z[1] = g.y; z[2] = g.z; z[3] = g.w; }
+                    for (int e = 0; e < 32; e += 8) {
+                        u32 y[4], z[4] = {};
+                        if (gp) { const uint4 g = __ldg((const uint4*)(gp + 2 * (k + e))); z[0] = g.x; z[1] = g.y; z[2] = g.z; z[3] = g.w; }
 #pragma unroll
-                    for (int x = 0; x < 4; x++) {
-                        float a = none ? 0.f : o[e + 2 * x] * inv, b = none ? 0.f : o[e + 2 * x + 1] * inv;
-                        if (gp) { const float2 g = pg_unpack<CT>(z[x]); a *= sz_sigmoid(g.x); b *= sz_sigmoid(g.y); }
-                        y[x] = pg_pack<CT>(a, b);
+                        for (int x = 0; x < 4; x++) {
+                            float a = none ? 0.f : o[e + 2 * x] * inv, b = none ? 0.f : o[e + 2 * x + 1] * inv;
+                            if (gp) { const float2 g = pg_unpack<CT>(z[x]); a *= sz_sigmoid(g.x); b *= sz_sigmoid(g.y); }
+                            y[x] = pg_pack<CT>(a, b);
+                        }
+                        *(uint4*)(op + 2 * (k + e)) = make_uint4(y[0], y[1], y[2], y[3]);
                     }
-                    *(uint4*)(op + 2 * (k + e)) = make_uint4(y[0], y[1], y[2], y[3]);
                 }
             }
+            __syncwarp();
             if (l != l && mx == -INFINITY) mx = 0.f;       // (scores that are all NaN have no maximum, and are not an empty part)
             if (qr < m && !direct) (alone ? pt.row_ml : pt.ml)[to] = make_float2(mx, l);
             if (qr < m && direct && io.lse) io.lse[to] = none ? -INFINITY : (mx + log2f(l)) * 0.6931471805599453f;

@@ -699,3 +699,15 @@ def test_a_tail_far_below_the_first_position(kind, hd, nats):
         want = torch.einsum("t,thd->hd", w, c.positions(c.v, b)).repeat_interleave(64 // nkv, 0) / w.sum()
         off = (out[b].double() - want).abs() / (2 * HALF_STEP[c.io] * want + 2.0 ** -16 * want + (2.0 ** -25 if kind == "f16" else 0))      # (f16's subnormals: half of 2^-24)
         assert float(off.max()) < 1.0, float(off.max())
+
+
+@pytest.mark.parametrize("kind,hd,nh,m", [("bf16", 256, 8, 13), ("f16", 128, 8, 13), ("bf16", 64, 3, 33), ("bf16", 256, 16, 45)])
+def test_a_tile_that_ends_inside_a_warp(kind, hd, nh, m):
+    """Vectors that fill a part of a warp's 32, written straight to the output, gated; and once more with a value that is not finite where only later rows see it."""
+    c = Case([500, 200], [m, m], nh=nh, nkv=1, hd=hd, io=kind, cache=kind, page=16, seed=44, pad=2)
+    gate = c.rnd(c.rows, nh, hd).to(c.io)
+    before = c.check(gate=gate).clone()
+    c.v[c.pages[0, (500 - 2) // 16], :, (500 - 2) % 16, 3] = math.inf                # the last two rows see it
+    out = c.step.attend(c.q, gate=gate)
+    assert torch.equal(out[m:2 * m], before[m:2 * m]) and torch.equal(out[:m - 2], before[:m - 2])
+    assert bool(torch.isinf(out[m - 2:m, :, 3]).all()) and bool(torch.isfinite(out[m - 2:m, :, 4:]).all()) and bool(torch.isfinite(out[m - 2:m, :, :3]).all())
