@@ -92,10 +92,11 @@ __global__ void __launch_bounds__(256, R == 1 ? 0 : 4) sz_pg_append_kernel(const
     if (R == 1 && x < a.heads)                  // its elements are under way while the row is looked up
         pg_load_n<E, IO>((kind1 == 0 ? a.q + (long long)r0 * a.q_stride + h1 * a.q_head_stride : (kind1 == 1 ? a.k + (long long)r0 * a.k_stride : a.v + (long long)r0 * a.v_stride) + h1 * (HD * ESZ)) + d0 * ESZ, one);
     for (int i = threadIdx.x; i < d.n_seq; i += 256) {
-        const int b0 = pg_row(d, i), b1 = pg_row(d, i + 1), len = __ldg(d.lens + i);
+        const int b0 = pg_row(d, i), b1 = pg_row(d, i + 1), end = __ldg(d.row_start + i + 1), len = __ldg(d.lens + i);
         for (int row = max(b0, r0); row < min(b1, r0 + R); row++) {      // (the block's rows of this sequence)
-            const int pos = len - (b1 - row), o = pos - d.shared_len;
-            if (pos < 0) continue;
+            const long long at = (long long)len - ((long long)end - row);
+            if (at < 0) continue;
+            const int pos = (int)at, o = pos - d.shared_len;
             long long off = -1;
             u32 bad = 0;
             if (o < 0) bad = PG_E_SHARED;
@@ -276,7 +277,7 @@ __global__ void __launch_bounds__(256) sz_pg_merge_kernel(const __grid_constant_
     const int b = pg_seq_of<256>(d, r);
     if (b < 0 || h >= nh) return;                                    // (h: W = 8 has one head a block)
     const int r0 = pg_row(d, b), m = pg_row(d, b + 1) - r0;
-    const bool sees = (long long)__ldg(d.lens + b) - d.shared_len - (m - 1 - (r - r0)) > 0;     // a position of its own
+    const bool sees = pg_end(d, b) - (m - 1 - (r - r0)) > 0;     // a position of its own
     PgList l[2] = {};
     if (sees) {
         l[PG_OWN] = pg_list(d, a.p[PG_OWN], r, r0, b, h);

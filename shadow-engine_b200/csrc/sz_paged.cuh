@@ -56,6 +56,11 @@ struct PgPart {
 };
 
 __device__ __forceinline__ int pg_row(const PgBatch& d, int i) { return min(max(__ldg(d.row_start + i), 0), d.rows); }
+// Where the own positions of sequence i's last row that is there end: before lens[i] where row_start goes on behind the rows of the call.
+__device__ __forceinline__ int pg_end(const PgBatch& d, int i) {
+    const long long over = max(__ldg(d.row_start + i + 1), d.rows) - d.rows;
+    return (int)max(0ll, (long long)__ldg(d.lens + i) - d.shared_len - over);
+}
 // Of a sequence with m rows whose own positions end at `end` (exclusive), tile t of tq vectors: where what its last row sees ends ..
 __device__ __forceinline__ int pg_room(const PgBatch& d) { return (int)min((long long)d.max_pages << d.ps_log2, 0x7fffffc0ll); }
 __device__ __forceinline__ int pg_tile_end(const PgBatch& d, int m, long long end, int t, int tq) {
@@ -111,7 +116,7 @@ __device__ u32 pg_scan(u32 v, u32& total, u32* sm) {                // exclusive
 template <int NTH>
 __device__ int pg_plan(const PgBatch& d, int shared, int unit, int tq, u32* tiles, u32* units, u32* sm, int* rows, int* ends) {
     if (rows)
-        for (int b = threadIdx.x; b <= d.n_seq; b += NTH) { rows[b] = pg_row(d, b); ends[b] = b < d.n_seq ? __ldg(d.lens + b) - d.shared_len : 0; }
+        for (int b = threadIdx.x; b <= d.n_seq; b += NTH) { rows[b] = pg_row(d, b); ends[b] = b < d.n_seq ? pg_end(d, b) : 0; }
     if (shared) {
         const int vec = (pg_row(d, d.n_seq) - pg_row(d, 0)) * d.G, E = max(0, (vec + tq - 1) / tq);
         const u32 un = (u32)((d.shared_len + unit - 1) / unit);
@@ -147,7 +152,7 @@ __device__ int pg_plan(const PgBatch& d, int shared, int unit, int tq, u32* tile
             int lo = 0, hi = d.n_seq - 1;                           // the last sequence whose tiles begin at or before e
             while (lo < hi) { const int mid = (lo + hi + 1) >> 1; if (tiles[mid] <= (u32)e) lo = mid; else hi = mid - 1; }
             const int m = pg_row(d, lo + 1) - pg_row(d, lo);
-            n = (u32)((pg_tile_end(d, m, (long long)__ldg(d.lens + lo) - d.shared_len, e - (int)tiles[lo], tq) + unit - 1) / unit);
+            n = (u32)((pg_tile_end(d, m, pg_end(d, lo), e - (int)tiles[lo], tq) + unit - 1) / unit);
         }
         const u32 at = pg_scan<NTH>(n, total, sm);
         if (e < E) units[e] = carry + at;
@@ -280,7 +285,7 @@ sz_pg_attend_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_const
     const u32 u0 = pg_first(share, blockIdx.x), u1 = pg_first(share, blockIdx.x + 1);
     const int room = pg_room(d);
     auto row_of = [&](int b) { return pt.planned ? pg_row(d, b) : s_rows[b]; };
-    auto end_of = [&](int b) { return (long long)(pt.planned ? __ldg(d.lens + b) - d.shared_len : s_ends[b]); };
+    auto end_of = [&](int b) { return (long long)(pt.planned ? pg_end(d, b) : s_ends[b]); };
 
     auto locate = [&](u32 u) {
         PgItem it;

@@ -166,7 +166,7 @@ sz_pg_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
     const PgShare share = work ? pg_share(U, blocks) : PgShare{1u, 0u};
     const u32 u0 = work ? pg_first(share, blockIdx.x) : 0, u1 = work ? pg_first(share, blockIdx.x + 1) : 0;
     auto row_of = [&](int b) { return pt.planned ? pg_row(d, b) : S.rows[b]; };
-    auto end_of = [&](int b) { return (long long)(pt.planned ? __ldg(d.lens + b) - d.shared_len : S.ends[b]); };
+    auto end_of = [&](int b) { return (long long)(pt.planned ? pg_end(d, b) : S.ends[b]); };
     // the next piece of the block's share: an item, units i .. i + T of it
     auto locate = [&](u32 u) {
         PgItem it;

@@ -711,3 +711,31 @@ def test_a_tile_that_ends_inside_a_warp(kind, hd, nh, m):
     out = c.step.attend(c.q, gate=gate)
     assert torch.equal(out[m:2 * m], before[m:2 * m]) and torch.equal(out[:m - 2], before[:m - 2])
     assert bool(torch.isinf(out[m - 2:m, :, 3]).all()) and bool(torch.isfinite(out[m - 2:m, :, 4:]).all()) and bool(torch.isfinite(out[m - 2:m, :, :3]).all())
+
+
+@pytest.mark.parametrize("m,kept,io,cache,shared", [(5, 2, "f32", "f16", 0), (5, 2, "bf16", "q8", 32), (40, 33, "bf16", "bf16", 0), (40, 33, "bf16", "bf16", 64), (1500, 1300, "bf16", "bf16", 0)])
+def test_rows_that_are_not_there_are_left_out(m, kept, io, cache, shared):
+    """row_start goes on behind the rows that the call has: those that it has keep their places and their results, the others' places are left alone."""
+    whole = Case([shared + 60, shared + m + 20], [2, m], nh=8, nkv=2, hd=64, io=io, cache=cache, shared=shared, seed=45)
+    kin, vin = whole.rnd(2 + m, 2, 64).to(whole.io), whole.rnd(2 + m, 2, 64).to(whole.io)
+    k0, v0 = whole.k.clone(), whole.v.clone()
+    qw = whole.step.append(kin, vin, q=whole.q, rope_dims=32)
+    assert whole.step.status() == 0
+    k1, v1 = whole.k.clone(), whole.v.clone()
+    n = 2 + kept
+    part = paged.Step(whole.cache, whole.pages, whole.row_start, whole.len_t, n, 8, shared_pages=whole.shared_pages, shared_len=shared)
+    whole.k.copy_(k0)
+    whole.v.copy_(v0)
+    assert torch.equal(part.append(kin[:n].contiguous(), vin[:n].contiguous(), q=whole.q[:n].contiguous(), rope_dims=32), qw[:n])
+    assert part.status() == 8
+    for have, first, then in ((whole.k, k0, k1), (whole.v, v0, v1)):
+        expect = then.clone()
+        for t in range(shared + 20 + kept, shared + 20 + m):                            # the left out rows' places: as they were
+            page, slot = int(whole.pages[1, (t - shared) // 16]), (t - shared) % 16
+            expect[page, :, slot] = first[page, :, slot]
+        assert torch.equal(have, expect)
+    whole.k.copy_(k1)
+    whole.v.copy_(v1)
+    out = part.attend(whole.q[:n].contiguous())
+    want, mag, _ = whole.want()
+    assert float(((out.double() - want[:n]).abs() / whole.tolerance(want, mag)[:n]).max()) < 1.0
