@@ -203,14 +203,15 @@ sz_pg_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
             const int32_t* table = pt.shared ? d.shared_pages : d.pages + (size_t)it.b * d.max_pages;
             auto window = [&](int w) {
                 const int c = (it.i + w * ahead) * C::UT + lane * rows_box;
-                return c < it.end ? __ldg(table + (c >> d.ps_log2)) : -2;       // (behind the end: not there, and no error)
+                return c < it.end ? __ldg(table + (c >> d.ps_log2)) : -1;
             };
             int now = window(0), next = window(1);
             for (int j = 0; j < T && !failed; j++, g++) {
                 const int k0 = j % ahead * pieces;
                 if (j && k0 == 0) { now = next; next = window(j / ahead + 1); }
                 const u32 there = __ballot_sync(0xffffffffu, (u32)now < (u32)d.n_pages) >> k0;
-                if (kind == 0 && lane >= k0 && lane < k0 + pieces && now != -2 && (u32)now >= (u32)d.n_pages) atomicOr(d.err, PG_E_PAGE);
+                if (kind == 0 && lane >= k0 && lane < k0 + pieces && (u32)now >= (u32)d.n_pages && (it.i + j) * C::UT + (lane - k0) * rows_box < it.end)
+                    atomicOr(d.err, PG_E_PAGE);            // (behind the end: not there, and no error)
 #pragma unroll
                 for (int nb = 0; nb < C::NB; nb++) {
                     const u32 n = g * C::NB + nb;

@@ -739,3 +739,12 @@ def test_rows_that_are_not_there_are_left_out(m, kept, io, cache, shared):
     out = part.attend(whole.q[:n].contiguous())
     want, mag, _ = whole.want()
     assert float(((out.double() - want[:n]).abs() / whole.tolerance(want, mag)[:n]).max()) < 1.0
+
+
+@pytest.mark.parametrize("m,shared", [(2, 0), (130, 0), (130, 1024)])
+@pytest.mark.parametrize("bad", [-2, -1, -2147483648])
+def test_any_page_id_out_of_range_is_reported(m, shared, bad):
+    c = Case([shared + 700], [m], nh=4, nkv=1, hd=128, io="bf16", cache="bf16", page=16, shared=shared, seed=46)
+    (c.shared_pages if shared else c.pages[0])[5] = bad
+    c.step.attend(c.q)
+    assert c.step.status() == 1
