@@ -86,9 +86,9 @@ __device__ __forceinline__ void sa_st32(void* p, int rank, u32 v) { asm volatile
 __device__ __forceinline__ void sa_st64(void* p, int rank, u64 v) { asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(sa_at(p, rank)), "l"(v) : "memory"); }
 __device__ __forceinline__ u32 sa_add32(void* p, int rank, u32 v) { u32 o; asm volatile("atom.shared::cluster.add.u32 %0, [%1], %2;" : "=r"(o) : "r"(sa_at(p, rank)), "r"(v) : "memory"); return o; }
 
-// larger logits first: a key that ascends as the logit descends, the id below it
+// larger logits first: a key that ascends as the logit descends, the id below it (-0 is 0: equal logits go by id)
 __device__ __forceinline__ u64 sa_key(float v, u32 id) {
-    const u32 b = __float_as_uint(v), up = b & 0x80000000u ? ~b : b | 0x80000000u;
+    const u32 x = __float_as_uint(v), b = x == 0x80000000u ? 0u : x, up = b & 0x80000000u ? ~b : b | 0x80000000u;
     return ((u64)(~up) << SA_ID) | id;
 }
 __device__ __forceinline__ float sa_value(u64 key) {

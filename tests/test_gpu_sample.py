@@ -227,3 +227,19 @@ def test_most_equal_logits_in_one_block():
     for r in range(rows):
         goal = float(u[r]) * c[-1]
         assert tok[r] == order[min(int((c <= goal).sum()), vocab - 1)] or np.abs(c - goal).min() < 2.0 ** -30 * c[-1], r
+
+
+def test_zeros_of_both_signs_are_equal():
+    """0 and -0 are one logit: the lower id first, whichever it is; a reading of the bits would put every 0 before every -0."""
+    tok = check(torch.tensor([[-0.0, 0.0]]), np.ones(1), np.ones(1, dtype=np.int64), np.ones(1), np.zeros(1), np.array([0.5]))
+    assert tok[0] == 0
+    for vocab, dtype in ((7, torch.float32), (700, torch.bfloat16), (5000, torch.float16), (40001, torch.float32)):
+        rng = np.random.default_rng(vocab)
+        rows = 12
+        lg = torch.from_numpy(np.where(rng.random((rows, vocab)) < 0.5, np.float32(-0.0), np.float32(0.0))).to(dtype)
+        lg[6:] = torch.where(torch.from_numpy(rng.random((6, vocab)) < 0.3), torch.tensor(-1.0, dtype=dtype), lg[6:])
+        u = rng.random(rows)
+        tok = check(lg, np.ones(rows), np.full(rows, vocab), np.ones(rows), np.zeros(rows), u)
+        assert list(tok[:6]) == [int(u[r] * vocab) for r in range(6)]
+        T, k, p, mp, u = settings(rng, rows, vocab)
+        check(lg, T, k, p, mp, u)
