@@ -748,3 +748,20 @@ def test_any_page_id_out_of_range_is_reported(m, shared, bad):
     (c.shared_pages if shared else c.pages[0])[5] = bad
     c.step.attend(c.q)
     assert c.step.status() == 1
+
+
+@pytest.mark.parametrize("io,cache", [("f32", "f16"), ("f32", "bf16"), ("f32", "q8"), ("bf16", "bf16"), ("f16", "f16"), ("bf16", "q8")])
+def test_a_sequence_alone_and_in_a_batch(io, cache):
+    """What else the batch holds moves the cuts between blocks and, for 16-bit rows over their own type, chooses the kernel: both results lie within the tolerance of
+    the same values, so within twice that of each other (f32: of what test_f32_rows_keep_their_accuracy allows)."""
+    big = Case([333, 1200, 64, 901, 77], [2, 60, 1, 3, 40], nh=16, nkv=2, hd=64, io=io, cache=cache, seed=49)
+    out = big.step.attend(big.q)
+    want, mag, _ = big.want()
+    r = 0
+    for b, m in enumerate(big.ms):
+        alone = paged.Step(big.cache, big.pages[b:b + 1].contiguous(), torch.tensor([0, m], dtype=torch.int32, device="cuda"), big.len_t[b:b + 1].clone(), m, 16)
+        one = alone.attend(big.q[r:r + m].contiguous())
+        w, g = want[r:r + m], mag[r:r + m]
+        tol = 2.0 ** -24 * w.abs() + 2.0 ** -16 * g if io == "f32" else HALF_STEP[big.io] * (w.abs() + g) + 2.0 ** -10 * g
+        assert float(((one.double() - out[r:r + m].double()).abs() / (2 * tol)).max()) < 1.0
+        r += m

@@ -7,6 +7,7 @@ import numpy as np
 import pytest
 import torch
 
+from oracle import binding as ob
 from tests.util import pkg
 
 szlib, sampling = pkg.lib, pkg.sampling
@@ -243,3 +244,24 @@ def test_zeros_of_both_signs_are_equal():
         assert list(tok[:6]) == [int(u[r] * vocab) for r in range(6)]
         T, k, p, mp, u = settings(rng, rows, vocab)
         check(lg, T, k, p, mp, u)
+
+
+@pytest.mark.parametrize("vocab", [3, 1000, 32003, 151936])
+def test_the_oracles_draws(vocab):
+    """The oracle's Sampler::sample over whole rows, from the same seed and position.  Its sums are f64 one after the other: vocab 2^-53 of them, far below the
+    2^-30 from a border that check() allows."""
+    oracle = ob.lib()
+    rng = np.random.default_rng(vocab + 1)
+    rows = 32
+    lg = torch.from_numpy(rng.normal(size=(rows, vocab)).astype(np.float32) * 2.5)
+    lg[5] = torch.round(lg[5])                                     # many equal ones, both zeros among them
+    T, k, p, mp, _ = settings(rng, rows, vocab)
+    k = np.minimum(k, vocab)
+    u = np.array([oracle.szo_uniform(7, r) for r in range(rows)])
+    tok = check(lg, T, k, p, mp, u)
+    host = lg.numpy()
+    for r in range(rows):
+        raw = (np.float32(T[r]).tobytes() + np.int32(k[r]).tobytes() + np.float32(p[r]).tobytes() + np.float32(mp[r]).tobytes() + np.uint64(7).tobytes())
+        row = np.ascontiguousarray(host[r])
+        want = oracle.szo_sample(C.cast(C.create_string_buffer(raw, 24), C.c_void_p), row.ctypes.data_as(C.c_void_p), vocab, r)
+        assert int(tok[r]) == int(want) or plain(host[r], T[r], k[r], p[r], mp[r], u[r])[2] < 2.0 ** -30, r
