@@ -128,13 +128,13 @@ __global__ void __launch_bounds__(256, R == 1 ? 0 : 4) sz_pg_append_kernel(const
     const int j = R == 1 ? 0 : warp;
     const long long r = r0 + j, off = s_off[j];
     if (s_pos[j] < 0) return;
-    // partners of a lane's dimensions: another lane's, where the halves are whole lanes; f' = c f + s partner, nothing turned: 1, 0
-    const bool lower = d0 < half, by_lane = half % E == 0;
+    // partners of a lane's dimensions: another lane's, where the halves are whole lanes; f' = c f + s partner
+    const bool lower = d0 < half, turned = d0 < 2 * half, by_lane = half % E == 0;
     const int partner = half ? (lower ? lane + half / E : lane - half / E) & 31 : lane;
     float c[E], s[E];
 #pragma unroll
     for (int e = 0; e < E; e++) {
-        const float2 t = by_lane && d0 + e < 2 * half ? turn[j][lower ? d0 + e : d0 + e - half] : make_float2(1.f, 0.f);
+        const float2 t = by_lane && turned ? turn[j][lower ? d0 + e : d0 + e - half] : make_float2(1.f, 0.f);
         c[e] = t.x;
         s[e] = lower ? -t.y : t.y;
     }
@@ -172,8 +172,8 @@ __global__ void __launch_bounds__(256, R == 1 ? 0 : 4) sz_pg_append_kernel(const
             if (by_lane) {
 #pragma unroll
                 for (int e = 0; e < E; e++) {
-                    const float p = __shfl_sync(0xffffffffu, f[e], partner);
-                    f[e] = fmaf(f[e], c[e], p * s[e]);
+                    const float p = __shfl_sync(0xffffffffu, f[e], partner), t = fmaf(f[e], c[e], p * s[e]);
+                    f[e] = turned ? t : f[e];              // (not by 1 and 0: 0 times another dimension's infinity)
                 }
             } else {                            // through shared memory
 #pragma unroll

@@ -765,3 +765,24 @@ def test_a_sequence_alone_and_in_a_batch(io, cache):
         tol = 2.0 ** -24 * w.abs() + 2.0 ** -16 * g if io == "f32" else HALF_STEP[big.io] * (w.abs() + g) + 2.0 ** -10 * g
         assert float(((one.double() - out[r:r + m].double()).abs() / (2 * tol)).max()) < 1.0
         r += m
+
+
+@pytest.mark.parametrize("io,cache", [("f32", "f16"), ("bf16", "bf16"), ("f16", "bf16")])
+@pytest.mark.parametrize("hd,dims", [(256, 64), (64, 32), (128, 2), (128, 64), (256, 256)])
+@pytest.mark.parametrize("rows", [3, 1190])
+def test_append_of_heads_that_are_not_finite(io, cache, hd, dims, rows):
+    """An infinity or NaN reaches its own dimension and the one it is turned with; every other dimension of the head is what it would be without."""
+    c = Case([rows + 4], [rows], nh=4, nkv=2, hd=hd, io=io, cache=cache, page=64, seed=47)
+    kin, vin = c.rnd(rows, 2, hd).to(c.io), c.rnd(rows, 2, hd).to(c.io)
+    clean = c.step.append(kin, vin, q=c.q, rope_dims=dims).clone()
+    k0 = c.k.clone()
+    for bad in (math.inf, -math.inf, math.nan):
+        for d in sorted({0, dims // 2 - 1, dims // 2, dims - 1, min(dims, hd - 1), hd - 1}):
+            q, k = c.q.clone(), kin.clone()
+            q[:, :, d] = bad
+            k[:, :, d] = bad
+            got = c.step.append(k, vin, q=q, rope_dims=dims)
+            hit = {d, (d + dims // 2) % dims} if d < dims else {d}
+            keep = [x for x in range(hd) if x not in hit]
+            assert torch.equal(got[:, :, keep], clean[:, :, keep]) and torch.equal(c.k[..., keep], k0[..., keep])
+            assert not bool(torch.isfinite(got[:, :, d]).any())
