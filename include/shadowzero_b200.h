@@ -288,7 +288,7 @@ typedef struct sz_paged_rope {
  * call with another shared_len or fewer rows fits where this one does).  Calls that can overlap on the GPU need one each, captured
  * graphs too.  sz_paged_status(scratch, 1, NULL, stream) once after it is allocated; sz_paged_status(scratch, 0, &code, stream)
  * synchronises and reports (and keeps) what calls have met: bit 0: a page id out of range, bit 1: a position behind the table's end, bit 2: a
- * row of sz_paged_append at a shared position, bit 3: row_start past `rows` (the position, or the row, is then left out) or descending (no row attends to its own positions), bit 4: a bounded wait ran out. */
+ * row of sz_paged_append at a shared position, bit 3: row_start past `rows` (the position, or the row, is then left out) or descending (nothing is appended, and no row attends to its own positions), bit 4: a bounded wait ran out. */
 int sz_paged_scratch_bytes(const sz_paged_cache* cache, const sz_paged_batch* batch, int n_head, int64_t* bytes);
 int sz_paged_status(uint64_t scratch, int init, int* code, uint64_t stream);
 /* Stores row r's key and value heads at its position and, where q is given, writes its query heads, normed and turned, to q_out.

@@ -91,8 +91,10 @@ __global__ void __launch_bounds__(256, R == 1 ? 0 : 4) sz_pg_append_kernel(const
     sz_pdl_trigger();
     if (R == 1 && x < a.heads)                  // its elements are under way while the row is looked up
         pg_load_n<E, IO>((kind1 == 0 ? a.q + (long long)r0 * a.q_stride + h1 * a.q_head_stride : (kind1 == 1 ? a.k + (long long)r0 * a.k_stride : a.v + (long long)r0 * a.v_stride) + h1 * (HD * ESZ)) + d0 * ESZ, one);
+    int falls = 0;                              // a row_start that descends: a row would be two sequences'
     for (int i = threadIdx.x; i < d.n_seq; i += 256) {
         const int b0 = pg_row(d, i), b1 = pg_row(d, i + 1), end = __ldg(d.row_start + i + 1), len = __ldg(d.lens + i);
+        falls |= b1 < b0;
         for (int row = max(b0, r0); row < min(b1, r0 + R); row++) {      // (the block's rows of this sequence)
             const long long at = (long long)len - ((long long)end - row);
             if (at < 0) continue;
@@ -110,8 +112,9 @@ __global__ void __launch_bounds__(256, R == 1 ? 0 : 4) sz_pg_append_kernel(const
             s_pos[row - r0] = pos; s_off[row - r0] = off;
         }
     }
-    if (r0 == 0 && threadIdx.x == 0 && blockIdx.y == 0 && __ldg(d.row_start + d.n_seq) > d.rows) atomicOr(d.err, PG_E_ROWS);
-    __syncthreads();
+    falls = __syncthreads_or(falls);
+    if (r0 == 0 && threadIdx.x == 0 && blockIdx.y == 0 && (falls || __ldg(d.row_start + d.n_seq) > d.rows)) atomicOr(d.err, PG_E_ROWS);
+    if (falls) return;                          // nothing is stored then
     for (int i = threadIdx.x; i < half * R; i += 256) {
         const int j = i / half, k = i - j * half, pos = s_pos[j];
         if (pos < 0) continue;

@@ -786,3 +786,16 @@ def test_append_of_heads_that_are_not_finite(io, cache, hd, dims, rows):
             keep = [x for x in range(hd) if x not in hit]
             assert torch.equal(got[:, :, keep], clean[:, :, keep]) and torch.equal(c.k[..., keep], k0[..., keep])
             assert not bool(torch.isfinite(got[:, :, d]).any())
+
+
+@pytest.mark.parametrize("rows", [6, 1200])
+def test_append_reports_a_descending_row_start(rows):
+    """A row would be two sequences': nothing is stored, nothing given back, the status tells."""
+    c = Case([rows + 9, rows + 70, 40], [rows // 2, rows // 2 - 1, 1], nh=4, nkv=2, hd=64, io="bf16", cache="bf16", page=64, seed=48)
+    kin = c.rnd(rows, 2, 64).bfloat16()
+    k0, v0 = c.k.clone(), c.v.clone()
+    c.row_start.copy_(torch.tensor([0, rows - 1, rows // 2, rows], dtype=torch.int32))
+    q_out = torch.full_like(c.q, 3.0)
+    c.step.append(kin, kin, q=c.q, q_out=q_out, rope_dims=32)
+    assert c.step.status() == 8
+    assert torch.equal(c.k, k0) and torch.equal(c.v, v0) and bool((q_out == 3.0).all())
