@@ -69,6 +69,8 @@ class Step:
             raise ValueError("pages and row_start: one row a sequence, one entry more than sequences")
         if shared_len and shared_pages.shape[0] * cache.c.page_size < shared_len:
             raise ValueError("shared_pages hold %d positions, shared_len is %d" % (shared_pages.shape[0] * cache.c.page_size, shared_len))
+        if cache.device.type != "cuda":
+            raise ValueError("the pools and tables lie on a GPU, not on %s" % cache.device)
         self.cache, self.n_head, self.rows, self.device = cache, n_head, rows, cache.device
         self.hd, self._index = cache.head_dim, cache.device.index
         self.nkv, self._scale = cache.c.n_kv_head, 1 / math.sqrt(cache.head_dim)

@@ -34,6 +34,8 @@ def sample_rows(logits, uniform, temperature=None, top_k=None, top_p=None, min_p
     f32 = torch.float32
     ptrs = (at("temperature", temperature, f32), at("top_k", top_k, torch.int32), at("top_p", top_p, f32), at("min_p", min_p, f32), at("uniform", uniform, torch.float64),
             at("out", out, torch.int32), at("prob", prob, f32))
+    if dev.type != "cuda":
+        raise ValueError("logits, settings and results lie on a GPU, not on %s" % dev)
     with _HERE if torch.cuda.current_device() == dev.index else torch.cuda.device(dev):
         rc = L.sz_sample_rows(TYPES[logits.dtype], logits.data_ptr(), stride, rows, vocab, *ptrs, torch.cuda.current_stream(dev.index).cuda_stream)
     if rc:

@@ -140,3 +140,17 @@ def test_more_work_than_a_call_takes_is_refused():
     c = cache(n_kv_head=8, page_size=1024, n_pages=1 << 20, page_stride=8 * 1024 * 256, head_stride=1024 * 256)
     assert attend(L, c=c, b=batch(n_seq=1, rows=1 << 20, max_pages=4096), nh=128, qs=128 * 128, os_=128 * 128, size=1 << 62) == szlib.E_ARG
     assert b"more work" in L.sz_last_error()
+
+
+def test_the_python_side_refuses_tensors_that_are_not_on_a_gpu():
+    """Everything else about these calls is right: the kernels would read host addresses."""
+    lg, u = torch.zeros(3, 10), torch.zeros(3, dtype=torch.float64)
+    out = torch.full((3,), 7, dtype=torch.int32)
+    for kw in (dict(), dict(out=out), dict(temperature=torch.ones(3), prob=torch.zeros(3))):
+        with pytest.raises(ValueError, match="GPU"):
+            sampling.sample_rows(lg, u, **kw)
+    assert bool((out == 7).all())
+    k = torch.zeros(4, 2, 16, 64, dtype=torch.bfloat16)
+    i = lambda *s: torch.zeros(*s, dtype=torch.int32)  # noqa: E731
+    with pytest.raises(ValueError, match="GPU"):
+        paged.Step(paged.Cache(k, k.clone(), 64), i(2, 3), i(3), i(2), 4, 4)
