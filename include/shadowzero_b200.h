@@ -323,7 +323,7 @@ int sz_paged_attend(const sz_paged_cache* cache, const sz_paged_batch* batch, in
  * counts as -inf; a row without a finite largest logit gives the lowest id of its largest, prob 1.
  * logits: [rows][vocab] of logits_type (SZ_TYPE_F32, F16 or BF16), row stride in elements; vocab 1 .. 262,144.  temperature, top_p, min_p f32 [rows], top_k
  * int32 [rows] - any may be 0: 1, no limit, 1 and 0 -, uniform f64 [rows] in [0, 1), token int32 [rows], prob f32 [rows] (0: not wanted).
- * Needs no scratch; deterministic (sums are integers). */
+ * Needs no scratch; deterministic (sums are integers).  Logits are read several times: rows that somebody writes meanwhile give some token. */
 int sz_sample_rows(int logits_type, uint64_t logits, int64_t logits_stride, int rows, int vocab, uint64_t temperature, uint64_t top_k, uint64_t top_p,
                    uint64_t min_p, uint64_t uniform, uint64_t token, uint64_t prob, uint64_t stream);
 

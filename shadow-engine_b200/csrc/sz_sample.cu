@@ -272,7 +272,7 @@ __global__ void __launch_bounds__(SA_NTH, 2) sz_sample_kernel(const __grid_const
         sa_sync(a.C);
         if (rank == 0 && tid == 0) {
             for (int c = 0; c < a.C; c++) id = min(id, sa_ld32(&S->top_id, c));
-            a.token[row] = (int32_t)id;
+            a.token[row] = (int32_t)min(id, (u32)a.vocab - 1);       // (none: somebody writes meanwhile)
             if (a.prob) a.prob[row] = 1.f;
         }
         sa_sync(a.C);                                                // (the others' shared memory is read until here)
@@ -336,7 +336,7 @@ __global__ void __launch_bounds__(SA_NTH, 2) sz_sample_kernel(const __grid_const
                         for (int k = 0; k < 4; k++) {
                             const float x = sa_x(R, v[h + k]);
                             float d;
-                            const u32 b = lo0 + 4u * (u32)sa_bin(x, d);
+                            const u32 b = lo0 + 4u * min((u32)sa_bin(x, d), (u32)SA_BINS - 1);      // (a logit that grew since its largest was taken has no bin)
                             const bool in = v[h + k] >= R.cut;
                             at[k] = in ? b : none;
                             r[k] = sa_term(d);

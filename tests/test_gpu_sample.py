@@ -265,3 +265,28 @@ def test_the_oracles_draws(vocab):
         row = np.ascontiguousarray(host[r])
         want = oracle.szo_sample(C.cast(C.create_string_buffer(raw, 24), C.c_void_p), row.ctypes.data_as(C.c_void_p), vocab, r)
         assert int(tok[r]) == int(want) or plain(host[r], T[r], k[r], p[r], mp[r], u[r])[2] < 2.0 ** -30, r
+
+
+@pytest.mark.parametrize("rows,vocab,dtype", [(250, 60001, torch.bfloat16), (64, 151936, torch.float32), (3, 40000, torch.float32)])
+def test_logits_that_change_underneath(rows, vocab, dtype):
+    """Another stream writes the rows while they are drawn from, values far above the largest that the call has seen among them: every call ends, with tokens of
+    the vocabulary, and the next one over logits at rest is right."""
+    g = torch.Generator(device="cuda").manual_seed(rows)
+    rest = (2.5 * torch.randn(rows, vocab, device="cuda", generator=g)).to(dtype)
+    other = [(rest.float() * 10 + 100).to(dtype), torch.full_like(rest, math.inf), torch.full_like(rest, math.nan), (rest.float() * 1e30).to(dtype), torch.full_like(rest, -math.inf), rest]
+    u = torch.rand(rows, dtype=torch.float64, device="cuda", generator=g)
+    p = torch.full((rows,), 0.9, device="cuda")
+    want = sampling.sample_rows(rest, u, top_p=p)
+    lg, side, got = rest.clone(), torch.cuda.Stream(), []
+    side.wait_stream(torch.cuda.current_stream())
+    for i in range(40):
+        with torch.cuda.stream(side):
+            for x in other:
+                lg.copy_(x)
+        got.append(sampling.sample_rows(lg, u, top_p=p))
+        got.append(sampling.sample_rows(lg, u))
+    torch.cuda.synchronize()
+    for t in got:
+        assert bool(((t >= 0) & (t < vocab)).all())
+    lg.copy_(rest)
+    assert torch.equal(sampling.sample_rows(lg, u, top_p=p), want)
