@@ -357,7 +357,11 @@ sz_pg_attend_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_const
     bool dead = false;                                    // a wait ran out: no further ones
     u32 cphase = 0;
     auto arrived = [&](int slot) {                        // .. at the consumers, before the half that was used last is filled again
-        if (!dead && !sz_mbar_wait_warp(&s_full[NQT == 1 ? slot * 4 + warp : slot], cphase)) { dead = true; if (lane == 0) atomicOr(d.err, PG_E_WAIT); }
+        if (!dead && !sz_mbar_wait_warp(&s_full[NQT == 1 ? slot * 4 + warp : slot], cphase)) {
+            dead = true;
+            if (lane == 0) atomicOr(d.err, PG_E_WAIT);
+            steps_left = -1 - steps_left;                 // nothing more is asked for
+        }
         if (NQT > 1) __syncthreads();
     };
 
@@ -768,6 +772,10 @@ sz_pg_attend_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_const
                 for (int b = 0; b < C::NT; b++) *(float2*)(w + 8 * b + 2 * q4) = make_float2(o[b][2 * hf], o[b][2 * hf + 1]);
             }
         }
+    }
+    if (dead) {                                           // what is under way is waited for, once more with a limit: the block's memory is another's soon
+        const int n = (int)(2 * (u1 - u0)) + 1 + steps_left;      // halves asked for
+        for (int i = max(0, n - C::NR); i < n; i++) sz_mbar_wait_warp(&s_full[NQT == 1 ? i % C::NR * 4 + warp : i % C::NR], (u32)(i / C::NR) & 1u);
     }
     // (only now: blocks of the merge that wait on a multiprocessor early took places of this kernel's - 64 sequences 414 -> 530 us)
     sz_pdl_trigger();

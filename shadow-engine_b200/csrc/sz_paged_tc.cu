@@ -103,7 +103,7 @@ struct PtCfg {
     static constexpr int SMEM = 1024 + NQ * QT + 2 * SLOTS * SLOT;                                 // (1,024 to align)
 };
 struct PtBars {
-    u64 full[2][4], empty[2][4], s_full[4], p_full[4], pv_done[4], q_full[2], o_free[2];      // (per tile two where units have turns: one at most is ahead of a waiter)
+    u64 full[2][4], empty[2][4], s_full[4], p_full[4], pv_done[4], q_full[2], o_free[2], last[2];      // (per tile two where units have turns: one at most is ahead of a waiter)
     u32 tmem, failed;
     u32 odd[2];                      // of every other piece: its number + 1, once a value that is not finite was cleared
     __align__(16) u32 ok[8][4];                    // which positions of a unit are there, of eight units: the eighth next one's keys are asked for after this one's weights were used
@@ -128,7 +128,7 @@ sz_pg_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
     if (tid == 0) {
         for (int i = 0; i < 8; i++) { sz_mbar_init(&S.full[0][i], 1); sz_mbar_init(&S.empty[0][i], 1); }
         for (int i = 0; i < 4; i++) { sz_mbar_init(&S.s_full[i], 1); sz_mbar_init(&S.p_full[i], 4); sz_mbar_init(&S.pv_done[i], 1); }
-        for (int i = 0; i < 2; i++) { sz_mbar_init(&S.q_full[i], 4); sz_mbar_init(&S.o_free[i], 4); }
+        for (int i = 0; i < 2; i++) { sz_mbar_init(&S.q_full[i], 4); sz_mbar_init(&S.o_free[i], 4); sz_mbar_init(&S.last[i], 1); }
         S.failed = 0;
         S.odd[0] = S.odd[1] = 0;
         sz_mbar_fence_init();
@@ -196,7 +196,7 @@ sz_pg_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
         const u32 one = pt_elect();
         const CUtensorMap* const map = kind ? &vmap : &kmap;
         u8* const to = kind ? vring : ring;
-        u32 g = 0;                                         // units so far
+        u32 g = 0, fills = 0;                              // units so far; slots filled
         for (u32 u = u0; u < u1 && !failed;) {
             const PgItem it = u == u0 ? first : locate(u);
             const int T = (int)min((u32)(it.n - it.i), u1 - u);
@@ -225,6 +225,7 @@ sz_pg_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
                         }
                         __syncwarp();
                     }
+                    fills = n + 1;
                     u64* const bar = &S.full[kind][sl];
                     const u32 dst = sz_smem_addr(to) + (u32)(sl * C::SLOT);
                     asm volatile("{ .reg .pred q; setp.ne.b32 q, %2, 0; @q mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1; }" ::"r"(sz_smem_addr(bar)), "r"((u32)C::SLOT), "r"(one) : "memory");
@@ -243,6 +244,8 @@ sz_pg_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
             }
             u += T;
         }
+        // (a role that gave up a wait leaves copies and products to nobody: each role sees its own to their end, bounded)
+        for (u32 n = fills > C::SLOTS ? fills - C::SLOTS : 0; n < fills; n++) if (!pt_wait_warp(&S.full[kind][n % C::SLOTS], n / C::SLOTS)) failed = 11;
         __syncwarp();
     } else if (warp == S_WARP) {
         // ---- the scores' products: a unit's, once its buffer's last weights have been used
@@ -278,6 +281,8 @@ sz_pg_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
             done += T;
             u += T;
         }
+        pt_commit(&S.last[0], one);
+        if (!pt_wait_warp(&S.last[0], 0)) failed = 12;
         __syncwarp();
     } else if (warp == PV_WARP) {
         // ---- the sums' products: a unit's, once its weights are there
@@ -314,6 +319,8 @@ sz_pg_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
             done += T;
             u += T;
         }
+        pt_commit(&S.last[1], one);
+        if (!pt_wait_warp(&S.last[1], 0)) failed = 12;
         __syncwarp();
     } else {
         // ---- softmax: thread = query vector
@@ -510,6 +517,7 @@ sz_pg_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
             pt_arrive_warp(&S.o_free[q]);
             u += T;
         }
+        pt_stored();
     }
     sz_pdl_trigger();
     if (failed) atomicMax(&S.failed, (u32)failed);
