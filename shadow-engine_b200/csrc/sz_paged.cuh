@@ -644,7 +644,7 @@ sz_pg_attend_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_const
                 auto moved = [&](u32 top, float csc) {    // what the row's sums are multiplied by (powers of two: exact)
                     const int ex = top >> 10 ? (int)(top >> 10) - 14 : -14;         // scale < 2^ex
                     const float want = __uint_as_float((u32)(127 - ex) << 23);
-                    return top && (want < csc || (fresh && want != csc)) ? want / csc : 1.f;
+                    return top && (want < csc || (fresh && want != csc)) ? __uint_as_float(__float_as_uint(want) - __float_as_uint(csc) + 0x3f800000u) : 1.f;      // (their quotient, by the exponents)
                 };
                 const float by0 = moved(t0, csc0), by1 = moved(t1, csc1);
                 if (__any_sync(0xffffffffu, by0 != 1.f || by1 != 1.f)) {
