@@ -49,8 +49,11 @@ class Cache:
         if any(n > 1 and st < k.shape[3] for n, st in zip(k.shape, k.stride()[:3])):
             raise ValueError("pools whose heads overlap")
         e = k.element_size()
+        head = k.shape[3] * e
+        # (of a dimension of one the stride says nothing)
+        page_stride, head_stride = (st * e if n > 1 else head for n, st in zip(k.shape[:2], k.stride()[:2]))
         self.c = PagedCacheC(type=szlib.TYPE_Q8_KV if packed else TYPES[k.dtype], n_kv_head=k.shape[1], head_dim=head_dim, page_size=k.shape[2], n_pages=k.shape[0],
-                             k=k.data_ptr(), v=v.data_ptr(), page_stride=max(k.stride(0) * e, k.shape[3] * e), head_stride=k.stride(1) * e, pos_stride=k.stride(2) * e)
+                             k=k.data_ptr(), v=v.data_ptr(), page_stride=page_stride, head_stride=head_stride, pos_stride=k.stride(2) * e)
 
 
 class Step:
@@ -107,10 +110,10 @@ class Step:
                 head = hd
             elif not apart or head < hd:
                 raise ValueError("%s: heads %s" % (name, "that overlap" if apart else "side by side"))
-        if row < (heads - 1) * head + hd:
-            if self.rows > 1:
-                raise ValueError("%s: rows that overlap" % name)
+        if self.rows == 1:
             row = (heads - 1) * head + hd
+        elif row < (heads - 1) * head + hd:
+            raise ValueError("%s: rows that overlap" % name)
         return t.data_ptr(), row, head
 
     def append(self, k, v, q=None, q_out=None, rope_dims=0, theta=1e4, q_norm=None, k_norm=None, eps=1e-6):

@@ -799,3 +799,14 @@ def test_append_reports_a_descending_row_start(rows):
     c.step.append(kin, kin, q=c.q, q_out=q_out, rope_dims=32)
     assert c.step.status() == 8
     assert torch.equal(c.k, k0) and torch.equal(c.v, v0) and bool((q_out == 3.0).all())
+
+
+def test_one_row_has_any_stride():
+    """Rows 130 elements apart are no multiple of 16 bytes; of a single one only its address counts."""
+    c = Case([33], [1], nh=2, nkv=1, hd=64, io="bf16", cache="bf16", seed=94)
+    want, kv = c.step.attend(c.q, gate=c.q).clone(), c.rnd(1, 1, 64).bfloat16()
+    wide = lambda x: torch.zeros(130, dtype=x.dtype, device="cuda").as_strided(x.shape, (130, 64, 1)).copy_(x)  # noqa: E731
+    assert torch.equal(c.step.attend(wide(c.q), gate=wide(c.q)), want)
+    first = c.step.append(kv, kv, q=c.q, rope_dims=32)
+    k1 = c.k.clone()
+    assert torch.equal(c.step.append(wide(kv), wide(kv), q=wide(c.q), rope_dims=32), first) and torch.equal(c.k, k1)

@@ -154,3 +154,15 @@ def test_the_python_side_refuses_tensors_that_are_not_on_a_gpu():
     i = lambda *s: torch.zeros(*s, dtype=torch.int32)  # noqa: E731
     with pytest.raises(ValueError, match="GPU"):
         paged.Step(paged.Cache(k, k.clone(), 64), i(2, 3), i(3), i(2), 4, 4)
+
+
+def test_a_dimension_of_one_has_any_stride():
+    """One page, or one key head: what a view's stride there is says nothing about the pool."""
+    base = torch.zeros(4096, dtype=torch.bfloat16)
+    one = base.as_strided((1, 1, 16, 64), (3, 5, 64, 1))
+    c = paged.Cache(one, base[2048:].as_strided((1, 1, 16, 64), (3, 5, 64, 1)), 64).c
+    n, L = C.c_int64(), szlib.load()
+    assert L.sz_paged_scratch_bytes(C.byref(c), C.byref(batch()), 4, C.byref(n)) == szlib.OK
+    packed = torch.zeros(4096, dtype=torch.uint8).as_strided((2, 1, 16, 80), (1280, 7, 80, 1))
+    c = paged.Cache(packed, packed, 64).c
+    assert c.page_stride == 1280 and L.sz_paged_scratch_bytes(C.byref(c), C.byref(batch()), 4, C.byref(n)) == szlib.OK
