@@ -573,6 +573,7 @@ extern "C" int sz_paged_attend(const sz_paged_cache* cache, const sz_paged_batch
         PgPart& p = s.a.p[i];
         p.on = i == PG_OWN || batch->shared_len > 0;
         p.shared = i == PG_SHARED;
+        p.ways = 1;                                                        // (the merge counts parts by it, of a launch that is not there too)
         if (!p.on) continue;
         kern[i] = kernels(pg_tiles_of(i == PG_SHARED ? all : per_seq));
         p.unit = tc_of[i] ? pg_tc_unit(hd) : PG_T;
