@@ -810,3 +810,122 @@ def test_one_row_has_any_stride():
     first = c.step.append(kv, kv, q=c.q, rope_dims=32)
     k1 = c.k.clone()
     assert torch.equal(c.step.append(wide(kv), wide(kv), q=wide(c.q), rope_dims=32), first) and torch.equal(c.k, k1)
+
+
+# ---- calls at the ends of what is allowed --------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("io,cache,m", [("f32", "f16", 2), ("f32", "q8", 2), ("bf16", "bf16", 130)])
+def test_pools_of_more_than_four_gigabytes(io, cache, m):
+    """Pages whose bytes lie behind 2^32: the last of a pool of 5 GB, beside its first."""
+    nkv, hd, ps = 2, 256, 16
+    head = paged.head_bytes(hd) if cache == "q8" else hd
+    kind = torch.uint8 if cache == "q8" else IO[cache]
+    size = nkv * ps * head * torch.empty(0, dtype=kind).element_size()
+    n = 5 * 2 ** 30 // size
+    c = Case([200, 77], [m, 1], nh=8, nkv=nkv, hd=hd, io=io, cache=cache, page=ps, seed=50)
+    want = c.check().clone()
+    k, v = torch.empty(n, nkv, ps, head, dtype=kind, device="cuda"), torch.empty(n, nkv, ps, head, dtype=kind, device="cuda")
+    old = c.pages.clamp(min=0).long()
+    new = torch.where(c.pages >= 0, torch.where(c.pages % 2 == 0, n - 1 - c.pages, c.pages), c.pages)
+    k[new.clamp(min=0).long().reshape(-1)] = c.k[old.reshape(-1)]
+    v[new.clamp(min=0).long().reshape(-1)] = c.v[old.reshape(-1)]
+    c.k, c.v, c.pages = k, v, new.to(torch.int32).contiguous()
+    c.make_step()
+    assert torch.equal(c.check(), want)
+    kin = c.rnd(c.rows, nkv, hd).to(c.io)
+    c.step.append(kin, kin)
+    assert c.step.status() == 0
+    for b, (x, mm) in enumerate(zip(c.lens, c.ms)):
+        page = int(c.pages[b, (x - 1) // ps])
+        row = kin[sum(c.ms[:b + 1]) - 1].double()
+        have = values(c.k[page, :, (x - 1) % ps], hd)
+        assert float((have - row).abs().max()) < 2.0 ** -8 * float(row.abs().max())
+
+
+@pytest.mark.parametrize("kind", ["bf16", "f16"])
+@pytest.mark.parametrize("nh", [128, 4096])
+def test_one_row_of_many_heads_on_one(kind, nh):
+    Case([700, 65], [1, 1], nh=nh, nkv=1, hd=64, io=kind, cache=kind, seed=51).check()
+
+
+@pytest.mark.parametrize("io,cache,m", [("f32", "q8", 3), ("bf16", "bf16", 3), ("bf16", "bf16", 60), ("f16", "f16", 60)])
+@pytest.mark.parametrize("scale", [0.0, -0.2, 1.0])
+def test_any_finite_scale(io, cache, m, scale):
+    """0: the mean of the values; below 0: the smallest product weighs most.  (1: scores of 60, whose f32 sums cut 2^-23 of them in each of four steps, and weights
+    2^-15 by that - f32's part stays below a quarter of the tolerance's.)"""
+    Case([300, 90], [m, 2], nh=8, nkv=2, hd=64, io=io, cache=cache, seed=52).check(scale=scale)
+
+
+@pytest.mark.parametrize("hd", [64, 256])
+@pytest.mark.parametrize("page", [8, 1024])
+def test_many_rows_smallest_and_largest_pages(hd, page):
+    Case([1500, 300], [60, 111], nh=8, nkv=2, hd=hd, io="bf16", cache="bf16", page=page, seed=page + hd, shared=0).check()
+    Case([1500 + i for i in range(16)], [2] * 16, nh=16, nkv=2, hd=hd, io="f16", cache="f16", page=page, seed=page + hd, shared=1391).check()
+
+
+@pytest.mark.parametrize("hd", [64, 128, 256])
+def test_many_rows_before_the_first_position(hd):
+    """A padded prompt: more rows than positions, and a sequence of none."""
+    c = Case([60, 300, 0], [130, 100, 40], nh=4, nkv=1, hd=hd, io="bf16", cache="bf16", seed=53, pad=7)
+    out = c.check()
+    assert bool((out[:70] == 0).all()) and bool((out[230:270] == 0).all())
+
+
+@pytest.mark.parametrize("bad", [math.nan, math.inf, 65504.0])
+@pytest.mark.parametrize("io,cache,seqs", [("f32", "f16", 3), ("f32", "q8", 3), ("bf16", "q8", 30), ("bf16", "bf16", 3), ("bf16", "bf16", 30), ("f16", "f16", 30)])
+def test_what_lies_behind_the_shared_positions_does_not_matter(io, cache, seqs, bad):
+    """The shared list's last page goes on behind shared_len, with anything."""
+    c = Case([141 + 3 * i for i in range(seqs)], [1 + i % 2 for i in range(seqs)], nh=8, nkv=2, hd=128, io=io, cache=cache, shared=133, page=32, seed=54)
+    before = c.check().clone()
+    last = c.shared_pages[-1]
+    for pool in (c.k, c.v):
+        if cache == "q8":
+            spoil(pool, 128, last, slice(133 % 32, None), bad)
+        else:
+            pool[last, :, 133 % 32:] = bad
+    assert torch.equal(c.step.attend(c.q), before)
+
+
+def test_as_many_sequences_as_a_call_takes():
+    c = Case([1 + i % 9 for i in range(4096)], [1] * 4096, nh=2, nkv=2, hd=64, page=16, io="bf16", cache="bf16", seed=55, pad=1)
+    out = torch.full_like(c.q, 7.0)
+    c.step.attend(c.q, out=out)
+    assert c.step.status() == 0 and bool((out[4096:] == 7.0).all())
+    k, v = values(c.k[c.pages[:, 0].long()], 64), values(c.v[c.pages[:, 0].long()], 64)          # [sequence, head, position, dimension]
+    s = torch.einsum("bhd,bhtd->bht", c.q[:4096].double(), k) / 8
+    s = s.masked_fill(torch.arange(16, device="cuda") >= c.len_t[:, None, None], -math.inf)
+    w = torch.softmax(s, -1)
+    want, mag = torch.einsum("bht,bhtd->bhd", w, v), torch.einsum("bht,bhtd->bhd", w, v.abs())
+    assert float(((out[:4096].double() - want).abs() / (HALF_STEP[c.io] * want.abs() + 2.0 ** -10 * mag + 1e-30)).max()) < 1.0
+
+
+@pytest.mark.parametrize("io,cache,ms", [("bf16", "bf16", [100, 3]), ("f32", "q8", [2, 3]), ("f16", "f16", [1, 1])])
+def test_two_steps_at_once(io, cache, ms):
+    """Two batches over one cache, a Step and a stream each, and their captured graphs side by side: neither sees the other's scratch."""
+    a = Case([900, 70], ms, nh=8, nkv=2, hd=128, io=io, cache=cache, seed=56)
+    pages, rs, lens = a.pages.flip(0).contiguous(), torch.tensor([0, 2, 3], dtype=torch.int32, device="cuda"), a.len_t.flip(0).contiguous()
+    b = paged.Step(a.cache, pages, rs, lens, 3, 8)
+    qb = a.rnd(3, 8, 128).to(a.io)
+    wa, wb = a.step.attend(a.q).clone(), b.attend(qb).clone()
+    outs, graphs, streams = [torch.empty_like(wa), torch.empty_like(wb)], [], [torch.cuda.Stream(), torch.cuda.Stream()]
+    for step, q, out, st in ((a.step, a.q, outs[0], streams[0]), (b, qb, outs[1], streams[1])):
+        st.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(st):
+            for _ in range(20):
+                step.attend(q, out=out)
+    torch.cuda.synchronize()
+    assert torch.equal(outs[0], wa) and torch.equal(outs[1], wb)
+    for step, q, out in ((a.step, a.q, outs[0]), (b, qb, outs[1])):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            step.attend(q, out=out)
+            step.attend(q, out=out)
+        graphs.append(g)
+    for out in outs:
+        out.zero_()
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for g, st in zip(graphs, streams):
+            with torch.cuda.stream(st):
+                g.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(outs[0], wa) and torch.equal(outs[1], wb)
