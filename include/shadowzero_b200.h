@@ -253,7 +253,7 @@ int sz_mma_cols_status(uint64_t scratch, int init, int* code, uint64_t stream);
  * positions may be one list of pages for ALL sequences of a call (a system prompt): they are read once for the batch, not once a sequence.
  * lens[b] counts all positions of sequence b, the shared ones and the rows of this call included: its rows row_start[b] .. row_start[b + 1)
  * of the inputs and outputs are its LAST positions.  Tables and lengths are device memory, read when the kernels run, so that a captured
- * graph serves a growing batch; rows at and behind row_start[n_seq] (a padded batch) are left as they were.
+ * graph serves a growing batch (they must not change while a call that reads them runs); rows at and behind row_start[n_seq] (a padded batch) are left as they were.
  * The cache's heads: f16 or bf16 values, or the session's packed form (SZ_TYPE_Q8_KV: head_dim int8, then head_dim / 32 f16 scales
  * zero-padded to 16 bytes; kernels/forward.cu:3652-3687).  head_dim 64, 128 or 256; n_head a multiple of n_kv_head. */
 #define SZ_TYPE_Q8_KV 1101

@@ -31,7 +31,7 @@ __device__ int pg_seq_of(const PgBatch& d, int r) {
 // a rotation's partner is hd / 32 dimensions of another lane.  Sums of squares and rotations in f32, one rounding to the stored type.
 // R = 1 row a block, a warp a head, for few rows: latency bounds those - sequence, length, page, head, one after the other -, so the head is read
 // while its row is looked up.  R = PG_APP where that still gives every multiprocessor a block: a warp a row, its heads two at a time (their loads
-// and their norms' shuffles side by side).  16 + 2 + 2 heads of 256, bf16: 1 row 3.4 us, 4,093 rows 22.2 against 51 with R = 1 (83 MB: 12.8 us of
+// and their norms' shuffles side by side).  16 + 2 + 2 heads of 256, bf16: 1 row 3.9 us, 4,093 rows 22.3 against 51 with R = 1 (83 MB: 12.8 us of
 // them; the chains of norm, rotation and store of one wave of warps are the rest); 163 rows of 32 + 8 + 8 heads of 128 5.2.
 // A row's angles are taken once a block, in f64 (a far position's angle has no digits left in f32), reduced to [-pi, pi] there, and the sine and
 // cosine of the reduced angle in f32 with its rounding put back by their derivatives.

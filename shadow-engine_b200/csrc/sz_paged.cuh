@@ -178,10 +178,10 @@ __device__ int pg_plan(const PgBatch& d, int shared, int unit, int tq, u32* tile
 // f16 pieces are kept in range: queries are divided by a power of two near their largest element, weights are 2^15 times themselves (so
 // that small ones do not run into f16's subnormals), and both are taken back in f32.  A packed value's scale goes into the weight (times a
 // power of two that follows the scales a row sees, csc), a packed key's into the 32-dimension partial scores in f32: codes themselves are exact in f16.
-// Measured: 64 sequences, 163 rows of 32 heads of 128 on 8, bf16, contexts of 3,000 to 15,000: 398 us (360 are the bytes at the measured copy rate: memory
+// Measured: 64 sequences, 163 rows of 32 heads of 128 on 8, bf16, contexts of 3,000 to 15,000: 406 us (360 are the bytes at the measured copy rate: memory
 // bounds it).  Few rows wait for one thing after the other instead: plan, pages, keys, products, values, products.  Four rows of 16 heads of 256 on 2
-// over 24,576 packed positions 55 us, 101 such rows behind 9,599 shared ones 252: 12 instructions (codes to f16, scales, pieces of weights) for
-// every matrix instruction, on the 8 warps that 128 registers of sums each leave room for (issue slots 51 %).
+// over 24,576 packed positions 56 us, 101 such rows behind 9,599 shared ones 277: 12 instructions (codes to f16, scales, pieces of weights) for
+// every matrix instruction, on the 8 warps that 128 registers of sums each leave room for (issue slots 41 %).
 template <int CT, bool WIDE, int HD, int NQT>
 struct PgCfg {
     static constexpr int NW = NQT == 1 ? 4 : 8, NTH = 32 * NW, WAYS = NW / NQT, SG = PG_T / 16 / WAYS, TQ = 16 * NQT;

@@ -18,7 +18,7 @@
 //   last four   keys, and values, by tiled TMA, a box a page (8 .. 64 positions x 64 dimensions, 128-byte swizzle), each through a ring of 64 positions x
 //               128 dimensions; the two issuing warps.
 // Operands: queries and keys K-major, values MN-major (their rows are the positions, which the product sums over), weights from tensor memory.
-// Measured: 2,045 rows of 16 heads of 256 on 2 behind 7,555 positions, bf16: 308 us, 0.93 PFLOP/s (the products alone at the measured rate 175); 64 rows of 32 heads
+// Measured: 2,045 rows of 16 heads of 256 on 2 behind 7,555 positions, bf16: 317 us, 0.91 PFLOP/s, 336 and 0.86 in a loop of a second (the products alone at the measured rate 175); 64 rows of 32 heads
 // of 128 over 24,576 shared positions some 47 us (16 of bytes or products).  What bounds it is the chain of a tile - scores, softmax, weights, product -: at head_dim 256 tensor memory
 // holds one tile's sums and two buffers of its scores, so that the softmax of a unit has the products of its neighbours only to run beside; up to 128
 // the exponentials (16,384 for 128 vectors and 128 positions) take the multiprocessor as long as both products take the tensor core.

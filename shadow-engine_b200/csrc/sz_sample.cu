@@ -15,9 +15,9 @@
 // 2^-45 (2^18 candidates stay below 2^63); the listed candidates' weights are f64 exponentials.
 //
 // A row is a cluster of 1 to 8 blocks, each with its part of the row, in shared memory where two blocks fit so.  What bounds it: with few rows
-// the chain of steps (load, maximum, sums, scan, gather, order; a cluster barrier between), with many the sums' instructions - 28 and two
-// atomics in shared memory an element - and the passes of the rows that ask for several elements.  Rows of 151,936, chat settings: 1 row 13.4 us;
-// 64 rows of mixed settings, f32, 51 us (39 MB: 6 us of them); 250 rows of bf16 drawn from whole, 93 us (76 MB: 12 us of them).
+// the chain of steps (load, maximum, sums, scan, gather, order; a cluster barrier between), with many the sums' instructions - 29 and two
+// atomics in shared memory an element - and the passes of the rows that ask for several elements.  Rows of 151,936, chat settings: 1 row 13.9 us;
+// 64 rows of mixed settings, f32, 51 us (39 MB: 6 us of them); 250 rows of bf16 drawn from whole, 98 us (76 MB: 12 us of them).
 #include "sz_common.cuh"
 
 #include <cuda_bf16.h>

@@ -58,7 +58,8 @@ class Cache:
 
 class Step:
     """The tables of a batch over a cache, and the scratch of its calls.  pages int32 [sequences, pages of one], row_start int32 [sequences + 1],
-    lens int32 [sequences] (all positions, the step's rows included) are the caller's tensors: change their values from step to step.
+    lens int32 [sequences] (all positions, the step's rows included) are the caller's tensors: change their values from step to step, behind the
+    calls that read them.
     shared_pages int32: the pages of the first shared_len positions, the same for all sequences.  Calls on one Step follow one another on
     a stream - the one it was made on, or another that waits for that -, and it is kept until they are done; what may overlap needs a Step each."""
 
