@@ -327,6 +327,70 @@ int sz_paged_attend(const sz_paged_cache* cache, const sz_paged_batch* batch, in
 int sz_sample_rows(int logits_type, uint64_t logits, int64_t logits_stride, int rows, int vocab, uint64_t temperature, uint64_t top_k, uint64_t top_p,
                    uint64_t min_p, uint64_t uniform, uint64_t token, uint64_t prob, uint64_t stream);
 
+/* ---- log probabilities of given tokens, with the rows' entropies and best alternatives --------------------------------------------------
+ * What a host answers a request for log probabilities with, and what it scores given text with (the reference has neither: its sampler keeps
+ * weights of the candidates to itself, crates/shadowzero-serve/src/sampler.rs:159-210).  With x = (logit - largest) / temperature, over the whole row and with no candidate dropped:
+ *   logprob[r] = x of tokens[r] minus the logarithm of the sum of e^x;  rank[r] = how many logits are larger than that token's, or equal with a lower id;
+ *   entropy[r] = - sum p log p (natural logarithms);  top_ids, top_logprobs [rows][top]: the row's largest logits (equal ones by id), top 0 .. 64, behind a
+ *   vocabulary of fewer -1 and -inf.
+ * A token outside 0 .. vocab - 1 (a padded row): -inf and rank -1.  A NaN logit counts as -inf.  A temperature of 0 or less, or NaN, or one whose reciprocal is not a
+ * number, and a row without a finite largest logit: the best token has it all (0, the others -inf, entropy 0), as in sz_sample_rows.
+ * logits: [rows][vocab] of logits_type (SZ_TYPE_F32, F16 or BF16), row stride in elements; vocab 1 .. 262,144; tokens, rank int32 [rows], temperature (0: 1), logprob,
+ * entropy f32 [rows]; results that are 0 are not wanted, tokens may be 0 where neither logprob nor rank is.  Sums and exponents are f32; the largest is left out of the sum of the others, so that a
+ * probability next to 1 keeps its distance from it.  Needs no scratch; the same bits for the same row and number of rows. */
+int sz_logprob_rows(int logits_type, uint64_t logits, int64_t logits_stride, int rows, int vocab, uint64_t tokens, uint64_t temperature, int top, uint64_t logprob, uint64_t rank,
+                    uint64_t entropy, uint64_t top_ids, uint64_t top_logprobs, uint64_t stream);
+
+/* ---- the DeltaNet layer of a served step: sequences whose states lie in a pool ------------------------------------------------------------
+ * The recurrent half of a host's own layers, beside the paged attention above: a sequence's state (f32 [v_heads][head_dim][head_dim], key
+ * dimension, then value dimension: SZ_STATE_DELTA_S's layout) and the rows its convolution carries (conv_type [conv_k - 1][channels], the oldest
+ * first: SZ_STATE_DELTA_CONV's; channels = (2 k_heads + v_heads) head_dim: queries, keys, values) lie in a slot of a pool.  Rows, row_start and lens are those of
+ * sz_paged_batch: the same tables serve both.  Sequence b starts from slot from[b] - or, where its rows are its first (lens[b] is not above their number), from
+ * nothing, whatever lies there - and what it leaves goes to slot to[b] (to = 0: the same).  take[b] (take = 0: all) says how many of its rows count:
+ * those behind them are neither read nor written.  So a host that verifies drafts writes to other slots and, once it knows what is kept, runs the kept
+ * rows again from the old ones (sz_delta_rows without q and out is that replay), or keeps the new slot where all were.  A sequence without rows is left alone.
+ * Tables are device memory, read when the kernels run; they must not change meanwhile.  Two sequences may start from one slot (a fork).  One that reads or
+ * writes a slot which an earlier one of the call writes, or writes one that an earlier one reads, is left out and reported. */
+typedef struct sz_delta_pool {
+    int32_t n_slots;
+    int32_t k_heads, v_heads, head_dim;   /* v_heads a multiple of k_heads, up to 1024; head_dim 64 or 128 */
+    int32_t grouped;                      /* value head h reads key head h % k_heads (0: the reference's tiling, forward.rs:862-864) or h / (v_heads / k_heads) (1) */
+    int32_t conv_k;                       /* rows of the convolution, 2 .. 8 */
+    int32_t conv_type, reserved;          /* SZ_TYPE_F32, F16 or BF16 */
+    uint64_t state, conv;                 /* 16-byte aligned; each call needs its own only */
+    int64_t state_stride, conv_stride;    /* bytes between slots, multiples of 16 */
+} sz_delta_pool;
+typedef struct sz_delta_batch {
+    int32_t n_seq;                        /* 1 .. 4096 */
+    int32_t rows;                         /* rows of the inputs and outputs; those at and behind row_start[n_seq] are left as they were */
+    int32_t max_rows;                     /* what the caller knows to be the most rows of one sequence (0: rows).  It chooses kernels: more rows are slower, not wrong */
+    int32_t reserved;
+    uint64_t row_start, lens;             /* int32 [n_seq + 1], not descending, and [n_seq] */
+    uint64_t from, to, take;              /* int32 [n_seq] */
+} sz_delta_batch;
+typedef struct sz_delta_gates {
+    uint64_t a, dt;                       /* f32 [v_heads]: a row's decay is exp(a softplus(alpha + dt)); a is not positive (a decay above 1 counts as 1) */
+    uint64_t norm;                        /* f32 [head_dim]: the output norm's weights; 0: the outputs are neither normed nor gated */
+    float eps, reserved;
+} sz_delta_gates;
+/* The scratch of both calls (256-byte aligned); calls that can overlap on the GPU need one each, captured graphs too.  sz_delta_status(scratch, 1, NULL, stream) once after
+ * it is allocated; sz_delta_status(scratch, 0, &code, stream) synchronises and reports (and keeps) what calls have met: bit 0: a slot out of
+ * range, bit 1: row_start past `rows` or descending, bit 2: a slot that another sequence of the call uses (the sequence is then left out), bit 3: a bounded wait ran out. */
+int sz_delta_scratch_bytes(const sz_delta_pool* pool, const sz_delta_batch* batch, int io_type, int64_t* bytes);
+int sz_delta_status(uint64_t scratch, int init, int* code, uint64_t stream);
+/* y[r][c] = silu(bias[c] + sum over t of w[c][t] x[r - (conv_k - 1) + t][c]) (forward.rs:829-846), rows before the sequence's first from its slot, and the last
+ * conv_k - 1 rows into it.  x, y [rows][channels] of io_type (SZ_TYPE_F32, F16 or BF16), row strides in elements, rows 16-byte aligned, apart from each other; w f32 [channels][conv_k], bias f32
+ * [channels] (0: none).  Sums in f32.  Uses the pool's conv only. */
+int sz_delta_conv(const sz_delta_pool* pool, const sz_delta_batch* batch, int io_type, uint64_t x, int64_t x_stride, uint64_t w, uint64_t bias, uint64_t y, int64_t y_stride,
+                  uint64_t scratch, int64_t scratch_bytes, uint64_t stream);
+/* The gated delta rule (forward.rs:847-894), per row and value head h with its key head's q and k over their lengths (q over sqrt(head_dim), too), beta' = sigmoid(beta):
+ *   S = decay S;  S += k (beta' (v - S^T k))^T;  o = S^T q;  out = o, or o / sqrt(mean(o^2) + eps) * norm * sigmoid(z).
+ * q, k [rows][k_heads][head_dim], v, z, out [rows][v_heads][head_dim], alpha, beta [rows][v_heads], all of io_type, row strides in elements, heads side by side; rows 16-byte aligned (those
+ * of alpha and beta: an element).  q, z and out may be 0 (the states alone: a replay); z and norm come together.  Uses the pool's state only. */
+int sz_delta_rows(const sz_delta_pool* pool, const sz_delta_batch* batch, const sz_delta_gates* gates, int io_type, uint64_t q, int64_t q_stride, uint64_t k, int64_t k_stride,
+                  uint64_t v, int64_t v_stride, uint64_t alpha, int64_t alpha_stride, uint64_t beta, int64_t beta_stride, uint64_t z, int64_t z_stride, uint64_t out,
+                  int64_t out_stride, uint64_t scratch, int64_t scratch_bytes, uint64_t stream);
+
 /* ---- the session: the verify surface ------------------------------------------------------------------------------------
  * Replaces the verify subset of GpuSession (crates/shadowzero-cuda/src/session.rs): step_batch_verify_top (6061-6072), rollback
  * (6217-6276), note_verify, capacity, tokens, and prefill by passes.  One engine thread owns a session (engine.rs:340-420).

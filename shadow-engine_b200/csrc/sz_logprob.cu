@@ -1,0 +1,387 @@
+// What given tokens weigh in whole rows of logits (sz_logprob_rows): their log probabilities and ranks, the rows' entropies and best alternatives.
+//
+// With x_i = (v_i - max) / T and s = the sum of e^x over all but one largest, log p = x - log1p(s) and the entropy is log1p(s) - sum(e^x x) / (1 + s):
+// no difference of like numbers, whatever the distribution.  One pass over the row: a warp keeps the largest so far (the same for its lanes, so that a
+// new one is rare) and both sums beside it.  A thread's elements come in groups of LP_G vectors; what a group's largest is stays in shared memory, and the
+// best `top` are looked for afterwards in the few groups that can hold them: a bound that `top` threads reach, by halving, then what is not below it.
+// A row is a cluster of 1 to 8 blocks, each with its part of it.
+#include "sz_common.cuh"
+
+#include <cuda_bf16.h>
+
+#include <math.h>
+
+namespace {
+
+constexpr int LP_NTH = 512, LP_G = 4, LP_MAX_VOCAB = 1 << 18, LP_ID = 18, LP_TOP = 64, LP_LIST = 2048, LP_PLACES = 3 * 148;
+constexpr int LP_NW = LP_NTH / 32;
+
+struct LpArgs {
+    const u8* logits;
+    long long stride;                // bytes
+    int rows, vocab, per, C, top;    // per: elements of a block's part
+    int groups;                      // of a thread
+    const int32_t* tokens;
+    const float* temperature;
+    float *logprob, *entropy;
+    int32_t *rank, *top_ids;
+    float* top_logprobs;
+};
+
+struct LpSmem {
+    u64 list[LP_LIST];               // keys of the candidates
+    u64 best[8 * LP_TOP];            // block 0: what the blocks found, in order
+    u64 mine[LP_TOP];
+    float wm[LP_NW], ws[LP_NW], wx[LP_NW];
+    u32 wc[LP_NW];
+    float m, s, x, thr;              // of the block's part
+    u32 c, n, found;
+};
+
+template <int TYPE> struct LpVec { static constexpr int ESZ = TYPE == SZ_TYPE_F32 ? 4 : 2, N = 16 / ESZ; };
+template <int TYPE>
+__device__ __forceinline__ float lp_at(const u32* w, int i) {       // element i of vectors side by side
+    if constexpr (TYPE == SZ_TYPE_F32) return __uint_as_float(w[i]);
+    else if constexpr (TYPE == SZ_TYPE_F16) return __half2float(__ushort_as_half((u16)(w[i / 2] >> (16 * (i & 1)))));
+    else return __uint_as_float(i & 1 ? w[i / 2] & 0xffff0000u : w[i / 2] << 16);
+}
+template <int TYPE>
+__device__ __forceinline__ float lp_one(const u8* p) {
+    if constexpr (TYPE == SZ_TYPE_F32) return __ldg((const float*)p);
+    else if constexpr (TYPE == SZ_TYPE_F16) return __half2float(__ushort_as_half(__ldg((const u16*)p)));
+    else return __uint_as_float((u32)__ldg((const u16*)p) << 16);
+}
+// NaN counts as -inf
+__device__ __forceinline__ float lp_clean(float v) { return fmaxf(v, -INFINITY); }
+// larger logits first, equal ones (0 and -0 too) by id
+__device__ __forceinline__ u32 lp_up(float v) { const u32 x = __float_as_uint(v), b = x == 0x80000000u ? 0u : x; return b & 0x80000000u ? ~b : b | 0x80000000u; }
+__device__ __forceinline__ float lp_down(u32 up) { return __uint_as_float(up & 0x80000000u ? up & 0x7fffffffu : ~up); }
+__device__ __forceinline__ u64 lp_key(float v, u32 id) { return ((u64)(~lp_up(v)) << LP_ID) | id; }
+__device__ __forceinline__ u32 lp_remote(const void* p, int rank) {
+    u32 a;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(sz_smem_addr(p)), "r"(rank));
+    return a;
+}
+__device__ __forceinline__ void lp_st64(void* p, int rank, u64 v) { asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(lp_remote(p, rank)), "l"(v) : "memory"); }
+__device__ __forceinline__ u32 lp_ld32(const void* p, int rank) { u32 v; asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(lp_remote(p, rank)) : "memory"); return v; }
+__device__ __forceinline__ float lp_exp2(float x) { float y; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x)); return y; }
+__device__ __forceinline__ void lp_sync(int C) { if (C > 1) sz_cluster_sync(); else __syncthreads(); }
+
+// (largest, sum of the others' weights beside it, sum of weights times exponents) of two parts; exponents to the base 2
+struct LpSum { float m, s, x; };
+__device__ __forceinline__ LpSum lp_join(const LpSum a, const LpSum b, float c) {
+    const LpSum hi = a.m >= b.m ? a : b, lo = a.m >= b.m ? b : a;
+    if (lo.m == -INFINITY) return hi;
+    const float d = fmaxf((lo.m - hi.m) * c, -200.f), w = lp_exp2(d);      // (of equal infinities: whatever, such a row is its first largest alone)
+    return {hi.m, fmaf(w, 1.f + lo.s, hi.s), fmaf(w, fmaf(1.f + lo.s, d, lo.x), hi.x)};
+}
+
+template <int TYPE>
+__global__ void __launch_bounds__(LP_NTH, 2)
+sz_logprob_kernel(const LpArgs a) {
+    using V = LpVec<TYPE>;
+    constexpr int N = V::N, GE = LP_G * N;               // elements of a vector and of a group
+    extern __shared__ __align__(16) u8 lp_smem[];
+    LpSmem* const S = (LpSmem*)lp_smem;
+    float* const gmax = (float*)(lp_smem + sizeof(LpSmem));        // [group][thread]
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, row = blockIdx.x / a.C, rank = blockIdx.x % a.C;
+    if (tid == 0) S->n = S->found = 0;
+    if (a.C > 1) sz_cluster_arrive();                    // (block 0's shared memory is written to once all have begun)
+    sz_pdl_wait();
+    sz_pdl_trigger();
+    const u8* const base = a.logits + (size_t)row * a.stride;
+    const int e0 = min(rank * a.per, a.vocab), e1 = min(e0 + a.per, a.vocab);      // the block's part
+    // in 16-byte vectors of memory: vector 0 holds element e0, `shift` elements in
+    const int shift = (int)(((size_t)base + (size_t)e0 * V::ESZ) & 15) / V::ESZ, nvec = e1 > e0 ? (shift + e1 - e0 + N - 1) / N : 0;
+    const int id0 = e0 - shift;                          // id of vector 0's first element
+    const u8* const vbase = base + (long long)id0 * V::ESZ;
+    int token = a.tokens ? a.tokens[row] : -1;
+    if ((u32)token >= (u32)a.vocab) token = -1;
+    const float tv = token >= 0 ? lp_clean(lp_one<TYPE>(base + (size_t)token * V::ESZ)) : INFINITY;
+    const int before = min(token, e1);                   // (what lies beside the part is -inf here, and nobody's)
+    const float T = a.temperature ? a.temperature[row] : 1.f, inv_t = 1.f / T;
+    const bool alone = !(T > 0.f) || !(inv_t <= 3.4e38f);            // the best token has it all
+    const float c = alone ? 0.f : inv_t * 1.4426950408889634f;
+    auto load = [&](int v, u32* w) {
+        if (v >= nvec) {
+#pragma unroll
+            for (int i = 0; i < 4; i++) w[i] = TYPE == SZ_TYPE_F32 ? 0xff800000u : TYPE == SZ_TYPE_F16 ? 0xfc00fc00u : 0xff80ff80u;
+        } else if ((v == 0 && shift) || (v == nvec - 1 && id0 + nvec * N > e1)) {      // element by element, those of the part
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                if constexpr (TYPE == SZ_TYPE_F32) {
+                    const int id = id0 + v * N + i;
+                    w[i] = id >= e0 && id < e1 ? __ldg((const u32*)(vbase + (size_t)(v * N + i) * 4)) : 0xff800000u;
+                } else {
+                    u32 h[2];
+#pragma unroll
+                    for (int j = 0; j < 2; j++) {
+                        const int id = id0 + v * N + 2 * i + j;
+                        h[j] = id >= e0 && id < e1 ? __ldg((const u16*)(vbase + (size_t)(v * N + 2 * i + j) * 2)) : TYPE == SZ_TYPE_F16 ? 0xfc00u : 0xff80u;
+                    }
+                    w[i] = h[0] | h[1] << 16;
+                }
+            }
+        } else {
+            const uint4 q = __ldg((const uint4*)(vbase + (size_t)v * 16));
+            w[0] = q.x; w[1] = q.y; w[2] = q.z; w[3] = q.w;
+        }
+    };
+    float m = -INFINITY, s = 0.f, x = 0.f, tmax = -INFINITY;         // of the warp (m), of the thread (the others)
+    u32 cnt = 0;
+#pragma unroll 1
+    for (int g = 0; g < a.groups; g++) {
+        u32 w[4 * LP_G];
+        const int v0 = g * LP_G * LP_NTH + tid;
+#pragma unroll
+        for (int j = 0; j < LP_G; j++) load(v0 + j * LP_NTH, w + 4 * j);
+        float gm = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < GE; i++) gm = fmaxf(gm, lp_at<TYPE>(w, i));
+        if (a.top) gmax[g * LP_NTH + tid] = gm;
+        tmax = fmaxf(tmax, gm);
+        // larger than the token's logit, or equal with a lower id
+        if (gm >= tv && token >= 0) {
+#pragma unroll
+            for (int i = 0; i < GE; i++) {
+                const float v = lp_clean(lp_at<TYPE>(w, i));
+                const int id = id0 + (v0 + (i / N) * LP_NTH) * N + i % N;
+                cnt += (v > tv || (v == tv && id < before && id >= e0)) ? 1u : 0u;
+            }
+        }
+        const float wm = lp_down(__reduce_max_sync(0xffffffffu, lp_up(gm)));
+        bool skip = false;
+        if (wm > m) {                                    // (the same for the whole warp)
+            if (m > -INFINITY) {                             // the old largest is one of the others now: lane 0 has it
+                const float d = fmaxf((m - wm) * c, -200.f), f = lp_exp2(d);
+                const float t = s + (lane == 0 ? 1.f : 0.f);
+                x = f * fmaf(t, d, x);
+                s = f * t;
+            }
+            m = wm;
+            skip = lane == __ffs(__ballot_sync(0xffffffffu, gm == wm)) - 1;
+        }
+        if (__any_sync(0xffffffffu, skip)) {             // one of the largest is left out
+#pragma unroll
+            for (int i = 0; i < GE; i++) {
+                const float v = lp_at<TYPE>(w, i);
+                const float e = fmaxf((v - m) * c, -200.f), p = skip && v == m ? 0.f : lp_exp2(e);
+                if (v == m) skip = false;
+                s += p;
+                x = fmaf(p, e, x);
+            }
+        } else {
+            float gs = 0.f, gx = 0.f;
+#pragma unroll
+            for (int i = 0; i < GE; i++) {
+                const float e = fmaxf((lp_at<TYPE>(w, i) - m) * c, -200.f), p = lp_exp2(e);
+                gs += p;
+                gx = fmaf(p, e, gx);
+            }
+            s += gs;
+            x += gx;
+        }
+    }
+    // ---- the block's part, then the row's
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) { s += __shfl_xor_sync(0xffffffffu, s, o); x += __shfl_xor_sync(0xffffffffu, x, o); }
+    cnt = __reduce_add_sync(0xffffffffu, cnt);
+    if (lane == 0) { S->wm[warp] = m; S->ws[warp] = s; S->wx[warp] = x; S->wc[warp] = cnt; }
+    __syncthreads();
+    if (warp == 0) {
+        LpSum t = lane < LP_NW ? LpSum{S->wm[lane], S->ws[lane], S->wx[lane]} : LpSum{-INFINITY, 0.f, 0.f};
+        u32 n = lane < LP_NW ? S->wc[lane] : 0;
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) t = lp_join(t, {__shfl_xor_sync(0xffffffffu, t.m, o), __shfl_xor_sync(0xffffffffu, t.s, o), __shfl_xor_sync(0xffffffffu, t.x, o)}, c);
+        n = __reduce_add_sync(0xffffffffu, n);
+        if (lane == 0) { S->m = t.m; S->s = t.s; S->x = t.x; S->c = n; }
+    }
+    __syncthreads();
+    const int top = a.top, have = e1 - e0, want = min(top, have);
+    if (a.C > 1) sz_cluster_wait();
+    if (want > 0) {
+        // ---- the part's best: a bound that `want` threads' largest reach
+        float thr = S->m;
+        if (want > 1) {
+            u32 hi = lp_up(S->m), lo = lp_up(-INFINITY);
+            // (lo: reached by all that have anything; hi: by one at least)
+            for (int step = 0; step < 32 && hi - lo > 1; step++) {
+                const u32 mid = step == 0 ? lp_up(S->m - 4.f / fmaxf(c, 0.25f)) : lo + (hi - lo) / 2;
+                if (mid <= lo || mid >= hi) continue;
+                const int n = __syncthreads_count(lp_up(tmax) >= mid);
+                if (n >= want) lo = mid; else hi = mid;
+                if (n >= want && n <= want + 16) break;
+            }
+            thr = lp_down(lo);
+        }
+        auto gather = [&](float from, bool equal) {
+            for (int g = 0; g < a.groups; g++) {
+                const float gm = gmax[g * LP_NTH + tid];
+                if (!(equal ? gm >= from : gm > from)) continue;
+                for (int j = 0; j < LP_G; j++) {
+                    const int v = (g * LP_G + j) * LP_NTH + tid;
+                    if (v >= nvec) break;
+                    u32 w[4];
+                    load(v, w);
+#pragma unroll
+                    for (int i = 0; i < N; i++) {
+                        const int id = id0 + v * N + i;
+                        const float f = lp_clean(lp_at<TYPE>(w, i));
+                        if (id < e0 || id >= e1 || !(equal ? f >= from : f > from)) continue;
+                        const u32 at = atomicAdd(&S->n, 1u);
+                        if (at < LP_LIST) S->list[at] = lp_key(f, id);
+                    }
+                }
+            }
+        };
+        gather(thr, true);
+        __syncthreads();
+        u32 n = S->n;
+        if (n > (u32)LP_LIST) {                          // thousands that reach it (equal ones, masked rows): the bound is made exact
+            u32 lo = lp_up(-INFINITY), hi = lp_up(S->m);
+            __syncthreads();
+            if (tid == 0) S->n = 0;
+            while (lo < hi) {                            // the want-th largest of the groups' largest: `lo` is reached by `want` of them at least
+                const u32 mid = lo + (hi - lo + 1) / 2;
+                u32 k = 0;
+                for (int g = 0; g < a.groups; g++) k += lp_up(gmax[g * LP_NTH + tid]) >= mid;
+                k = __reduce_add_sync(0xffffffffu, k);
+                if (lane == 0) S->wc[warp] = k;
+                __syncthreads();
+                u32 sum = 0;
+                for (int i = 0; i < LP_NW; i++) sum += S->wc[i];
+                __syncthreads();
+                if (sum >= (u32)want) lo = mid; else hi = mid - 1;
+            }
+            thr = lp_down(lo);
+            gather(thr, false);                          // (of fewer than `want` groups: they fit)
+            __syncthreads();
+            n = S->n;
+            // .. and equal ones from the lowest id on
+            for (int v0 = 0; n < (u32)want && v0 < nvec; v0 += LP_NTH) {
+                u32 w[4], k = 0, before = 0;
+                load(v0 + tid, w);
+#pragma unroll
+                for (int i = 0; i < N; i++) {
+                    const int id = id0 + (v0 + tid) * N + i;
+                    k += id >= e0 && id < e1 && lp_clean(lp_at<TYPE>(w, i)) == thr;
+                }
+                u32 upto = k;
+#pragma unroll
+                for (int o = 1; o < 32; o *= 2) { const u32 y = __shfl_up_sync(0xffffffffu, upto, o); if (lane >= o) upto += y; }
+                if (lane == 31) S->wc[warp] = upto;
+                __syncthreads();
+                u32 all = 0;
+                for (int i = 0; i < LP_NW; i++) { if (i < warp) before += S->wc[i]; all += S->wc[i]; }
+                u32 at = n + before + upto - k;
+#pragma unroll
+                for (int i = 0; i < N; i++) {
+                    const int id = id0 + (v0 + tid) * N + i;
+                    if (id >= e0 && id < e1 && lp_clean(lp_at<TYPE>(w, i)) == thr) { if (at < (u32)want) S->list[at] = lp_key(thr, id); at++; }
+                }
+                __syncthreads();
+                n = min(n + all, (u32)want);
+            }
+            __syncthreads();
+        }
+        // each one's place among them; the first go to block 0
+        for (u32 i = tid; i < n; i += LP_NTH) {
+            const u64 key = S->list[i];
+            u32 at = 0;
+#pragma unroll 4
+            for (u32 j = 0; j < n; j++) at += S->list[j] < key;
+            if (at < (u32)want) { if (a.C > 1) lp_st64(&S->best[rank * LP_TOP + at], 0, key); else S->best[at] = key; }
+        }
+    }
+    if (top)                                             // (a part with fewer elements than are asked for)
+        for (int i = want + tid; i < top; i += LP_NTH) { if (a.C > 1) lp_st64(&S->best[rank * LP_TOP + i], 0, ~0ull); else S->best[i] = ~0ull; }
+    lp_sync(a.C);
+    if (rank == 0) {
+        LpSum t = {S->m, S->s, S->x};
+        u32 n = S->c;
+        for (int r = 1; r < a.C; r++) {
+            t = lp_join(t, {__uint_as_float(lp_ld32(&S->m, r)), __uint_as_float(lp_ld32(&S->s, r)), __uint_as_float(lp_ld32(&S->x, r))}, c);
+            n += lp_ld32(&S->c, r);
+        }
+        const bool one = alone || !(fabsf(t.m) < INFINITY);
+        const float lz = log1pf(t.s);
+        if (tid == 0) {
+            if (a.logprob) a.logprob[row] = token < 0 ? -INFINITY : one ? (n == 0 ? 0.f : -INFINITY) : (tv - t.m) * inv_t - lz;
+            if (a.rank) a.rank[row] = token < 0 ? -1 : (int32_t)n;
+            if (a.entropy) a.entropy[row] = one ? 0.f : lz - t.x * 0.6931471805599453f / (1.f + t.s);
+        }
+        if (top) {
+            auto give = [&](int at, u64 key) {
+                const float v = lp_down(~(u32)(key >> LP_ID));
+                a.top_ids[(size_t)row * top + at] = key == ~0ull ? -1 : (int32_t)(key & ((1u << LP_ID) - 1));
+                a.top_logprobs[(size_t)row * top + at] = key == ~0ull ? -INFINITY : one ? (at == 0 ? 0.f : -INFINITY) : (v - t.m) * inv_t - lz;
+            };
+            if (a.C == 1) { if (tid < top) give(tid, S->best[tid]); }
+            else
+                for (int i = tid; i < a.C * LP_TOP; i += LP_NTH) {
+                    if (i % LP_TOP >= top) continue;
+                    const u64 key = S->best[i];
+                    int at = 0;
+                    for (int r = 0; r < a.C; r++)
+                        for (int j = 0; j < top; j++) { const u64 o = S->best[r * LP_TOP + j]; at += o < key || (o == key && r * LP_TOP + j < i); }
+                    if (at < top) give(at, key);
+                }
+        }
+    }
+    lp_sync(a.C);                                        // (shared memory is read by block 0 until here)
+}
+
+template <int TYPE>
+int lp_launch(const LpArgs& a, cudaStream_t st) {
+    const size_t smem = sizeof(LpSmem) + (a.top ? (size_t)a.groups * LP_NTH * 4 : 0);
+    const int rc = sz_allow_smem((const void*)sz_logprob_kernel<TYPE>, 112 * 1024);
+    if (rc) return rc;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)a.rows * a.C);
+    cfg.blockDim = dim3(LP_NTH);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = (unsigned)a.C;
+    attr[1].val.clusterDim.y = 1;
+    attr[1].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = a.C > 1 ? 2 : 1;
+    SZ_CUDA(cudaLaunchKernelEx(&cfg, sz_logprob_kernel<TYPE>, a));
+    sz_trace_mark("logprob_rows", st);
+    return SZ_OK;
+}
+
+}  // namespace
+
+extern "C" int sz_logprob_rows(int logits_type, uint64_t logits, int64_t logits_stride, int rows, int vocab, uint64_t tokens, uint64_t temperature, int top, uint64_t logprob, uint64_t rank,
+                               uint64_t entropy, uint64_t top_ids, uint64_t top_logprobs, uint64_t stream) {
+    const char* who = "sz_logprob_rows";
+    if (logits_type != SZ_TYPE_F32 && logits_type != SZ_TYPE_F16 && logits_type != SZ_TYPE_BF16) return sz_fail(SZ_E_TYPE, "%s: logits of type %d", who, logits_type);
+    const int esz = logits_type == SZ_TYPE_F32 ? 4 : 2;
+    if (rows < 1 || rows > (1 << 20) || vocab < 1 || vocab > LP_MAX_VOCAB || (rows > 1 && logits_stride < vocab) || logits_stride > (1ll << 40))
+        return sz_fail(SZ_E_ARG, "%s: %d rows (1 .. 1048576) of %d logits (1 .. %d), %lld apart", who, rows, vocab, LP_MAX_VOCAB, (long long)logits_stride);
+    if (top < 0 || top > LP_TOP || (top && (!top_ids || !top_logprobs))) return sz_fail(SZ_E_ARG, "%s: %d best (0 .. %d), with places for their ids and log probabilities", who, top, LP_TOP);
+    if (!tokens && (logprob || rank)) return sz_fail(SZ_E_ARG, "%s: log probabilities and ranks of no tokens", who);
+    if (!logprob && !rank && !entropy && !top) return sz_fail(SZ_E_ARG, "%s: nothing is asked for", who);
+    if (!logits || (logits & (esz - 1)) || ((tokens | temperature | logprob | rank | entropy | top_ids | top_logprobs) & 3)) return sz_fail(SZ_E_ARG, "%s: null or misaligned argument", who);
+    LpArgs a = {};
+    a.logits = (const u8*)logits; a.stride = logits_stride * esz; a.rows = rows; a.vocab = vocab; a.top = top;
+    a.tokens = (const int32_t*)tokens; a.temperature = (const float*)temperature;
+    a.logprob = (float*)logprob; a.entropy = (float*)entropy; a.rank = (int32_t*)rank; a.top_ids = (int32_t*)top_ids; a.top_logprobs = (float*)top_logprobs;
+    // blocks a row: waves of blocks times what one takes
+    const int most = vocab > 16384 ? 8 : vocab > 4096 ? 4 : vocab > 1024 ? 2 : 1;
+    double least = 0;
+    for (int C = 1; C <= most; C *= 2) {
+        const double cost = (double)(((long long)rows * C + LP_PLACES - 1) / LP_PLACES) * (20000.0 + (double)vocab / C);
+        if (C == 1 || cost < least) { least = cost; a.C = C; }
+    }
+    a.per = ((vocab + a.C - 1) / a.C + 7) & ~7;
+    const int vec = 16 / esz;
+    a.groups = ((a.per + vec - 1) / vec + 1 + LP_G * LP_NTH - 1) / (LP_G * LP_NTH);      // (a part may begin and end inside vectors)
+    cudaStream_t st = (cudaStream_t)stream;
+    return logits_type == SZ_TYPE_F32 ? lp_launch<SZ_TYPE_F32>(a, st) : logits_type == SZ_TYPE_F16 ? lp_launch<SZ_TYPE_F16>(a, st) : lp_launch<SZ_TYPE_BF16>(a, st);
+}

@@ -159,6 +159,11 @@ SYMBOLS = {
     "sz_paged_attend": (C.c_int, [C.c_void_p, C.c_void_p, C.c_int, C.c_int, C.c_float, C.c_uint64, C.c_int64, C.c_uint64, C.c_int64, C.c_int64, C.c_uint64, C.c_int64,
                                   C.c_uint64, C.c_uint64, C.c_int64, C.c_uint64]),
     "sz_sample_rows": (C.c_int, [C.c_int, C.c_uint64, C.c_int64, C.c_int, C.c_int] + [C.c_uint64] * 8),
+    "sz_logprob_rows": (C.c_int, [C.c_int, C.c_uint64, C.c_int64, C.c_int, C.c_int, C.c_uint64, C.c_uint64, C.c_int] + [C.c_uint64] * 6),
+    "sz_delta_scratch_bytes": (C.c_int, [C.c_void_p, C.c_void_p, C.c_int, C.POINTER(C.c_int64)]),
+    "sz_delta_status": (C.c_int, [C.c_uint64, C.c_int, C.POINTER(C.c_int), C.c_uint64]),
+    "sz_delta_conv": (C.c_int, [C.c_void_p, C.c_void_p, C.c_int, C.c_uint64, C.c_int64, C.c_uint64, C.c_uint64, C.c_uint64, C.c_int64, C.c_uint64, C.c_int64, C.c_uint64]),
+    "sz_delta_rows": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_int] + [C.c_uint64, C.c_int64] * 8 + [C.c_uint64]),
     "sz_ep_unique_id": (C.c_int, [C.c_void_p]),
     "sz_ep_init": (C.c_int, [C.c_int, C.c_int, C.c_void_p]),
     "sz_ep_world": (C.c_int, []),
