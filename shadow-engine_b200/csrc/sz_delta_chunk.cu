@@ -71,7 +71,7 @@ __device__ __forceinline__ void dl_split(float a, float b, u32& hi, u32& lo) {
     lo = dl_h2(a - f.x, b - f.y);
 }
 __device__ __forceinline__ void dl_mma(float* c, const u32* a, u32 b0, u32 b1) {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 __device__ __forceinline__ void dl_ldsm(u32* r, u32 addr) {
@@ -79,6 +79,25 @@ __device__ __forceinline__ void dl_ldsm(u32* r, u32 addr) {
 }
 __device__ __forceinline__ void dl_ldsm_t(u32* r, u32 addr) {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void dl_stsm_t(u32 addr, const u32* r) {
+    asm volatile("stmatrix.sync.aligned.m8n8.x4.trans.shared.b16 [%0], {%1,%2,%3,%4};" ::"r"(addr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]) : "memory");
+}
+__device__ __forceinline__ void dl_scale4(float* x, float f) {
+    const u64 f2 = dl_pack2(f, f), a = dl_mul2(dl_pack2(x[0], x[1]), f2), b = dl_mul2(dl_pack2(x[2], x[3]), f2);
+    x[0] = dl_lo(a); x[1] = dl_hi(a); x[2] = dl_lo(b); x[3] = dl_hi(b);
+}
+// sigmoid: where 16 bits are kept of what it is multiplied with, by the fast exponential and quotient (2^-21 relative); for f32 with the rounding of the exponent put
+// back and a Newton step on the fast reciprocal (2^-22), a third of the time of sz_sigmoid
+template <int TYPE> __device__ __forceinline__ float dl_sigmoid(float x) {
+    if (TYPE != SZ_TYPE_F32) return __fdividef(1.f, 1.f + __expf(-x));
+    constexpr float L = 1.4426950408889634f, L_LOW = 1.925963033500e-8f;      // log2(e), and what f32 leaves of it
+    const float y = -x > 85.f ? 85.f : -x, e = y * L, rest = fmaf(y, L_LOW, fmaf(y, L, -e));
+    float w, r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(w) : "f"(e));
+    const float den = 1.f + fmaf(w, rest * 0.6931471805599453f, w);
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(den));
+    return r * fmaf(-den, r, 2.f);
 }
 // byte of the 16-byte piece c of row r of a tile [rows][D] of f16: pieces exchanged so that ldmatrix meets no bank twice
 template <int D> __device__ __forceinline__ u32 dl_at(int r, int c) { return (u32)(r * D * 2 + ((c ^ (r & 7)) << 4)); }
@@ -292,33 +311,49 @@ sz_delta_prep_kernel(const DlBatch d, const DlRule a, int idx0, u8* __restrict__
 }
 
 // ---- the chain over a sequence's chunks --------------------------------------------------------------------------------------------------------
-template <int D, int TYPE, int NG> struct DlMain {
+// A block has three kinds of warps, which meet at mbarriers only: NC of the chain (16 value dimensions and 64 key dimensions each), as many for the outputs, which
+// take S and D as the chain's products had them (f16, from shared memory), and one that copies the chunks' operands into a ring.  The blocks of a head form a
+// cluster: where outputs are normed, a row's sums of squares go to all of them, and a chunk's outputs leave while the next one's are made.
+template <int D, int TYPE, int NG, bool OUT> struct DlMain {
     using C = DlChunk<D, TYPE>;
-    static constexpr int ESZ = DlIo<TYPE>::ESZ, NQ = D / 64, NW = NG * NQ, NTH = 32 * NW, CS = D / 16 / NG;      // warps on one 16 dimensions; warps; blocks of a head
+    static constexpr int ESZ = DlIo<TYPE>::ESZ, NQ = D / 64, NC = NG * NQ, CS = D / 16 / NG;      // warps on one 16 dimensions; of the chain; blocks of a head
+    static constexpr int CONSUMERS = OUT ? 2 * NC : NC, NTH = 32 * (CONSUMERS + 1);
     static constexpr int VS = 16 * NG * ESZ + 16;                                          // bytes between rows of v and z in shared memory
-    static constexpr int STAGE = C::ROWS + C::HEAD + 2 * CK * VS, STAGES = D == 128 && TYPE == SZ_TYPE_F32 ? 1 : 2;
-    static constexpr int XB = NQ == 2 ? 12 * 32 * 16 : 0;                                  // what a warp gives its partner
-    static constexpr int OS = 16 * ESZ + 16, OB = CK / NQ * OS;                            // a warp's outputs on their way
-    static constexpr int SSQ = 2 * CS * NG * CK * 4;
-    static constexpr size_t SMEM = (size_t)STAGES * STAGE + NW * (XB + OB) + SSQ + 64;
+    static constexpr bool STAGED = TYPE != SZ_TYPE_F32;                                    // gates and outputs through shared memory (f32: whole sectors a warp without)
+    static constexpr int STAGE = C::ROWS + C::HEAD + (STAGED ? 2 : 1) * CK * VS, STAGES = D == 128 && TYPE == SZ_TYPE_F32 ? 1 : 2;
+    static constexpr int XB = NQ == 2 ? 2 * 8 * 32 * 16 : 0;                               // what a chain's warp gives its partner (two chunks' turns)
+    static constexpr int FB = OUT ? (C::FULL ? 2 : 1) * 4 * 32 * 16 : 0;                   // a product's factor of 16 x 64 in f16: S of a warp, D of a group; two turns of each
+    static constexpr int OS = 16 * ESZ + 16, OB = OUT && STAGED ? CK / NQ * OS : 0;                  // a warp's outputs on their way
+    static constexpr int SSQ = OUT ? 4 * CS * NG * CK * 4 : 0;                             // [turn of four][block][group][row]
+    static constexpr int BARS = 2 * STAGES + 6 * NG + 4;
+    static constexpr size_t SMEM = (size_t)STAGES * STAGE + NC * (XB + 2 * FB + OB) + NG * 2 * FB + SSQ + BARS * 8 + 2 * (NC + NG) * 4;
 };
 
 template <int D, int TYPE, int NG, bool OUT>
-__global__ void __launch_bounds__(DlMain<D, TYPE, NG>::NTH, 1)
+__global__ void __launch_bounds__(DlMain<D, TYPE, NG, OUT>::NTH, 1)
 sz_delta_chunk_kernel(const DlBatch d, const DlRule a, int idx0, int idx1, const u8* __restrict__ scratch, long long one) {
-    using M = DlMain<D, TYPE, NG>;
+    using M = DlMain<D, TYPE, NG, OUT>;
     using C = DlChunk<D, TYPE>;
-    constexpr int ESZ = M::ESZ, NQ = M::NQ, NK = C::NK, CS = M::CS, ST = M::STAGES, OT = 8 / NQ;      // OT: 8-row tiles whose outputs a warp finishes
+    constexpr int ESZ = M::ESZ, NQ = M::NQ, NK = C::NK, NC = M::NC, CS = M::CS, ST = M::STAGES, OT = 8 / NQ;      // OT: 8-row tiles whose outputs a warp finishes
+    constexpr int FP = C::FULL ? 2 : 1;
     extern __shared__ __align__(16) u8 sm[];
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, p = warp / NQ, q = warp % NQ, g = lane >> 2, t = lane & 3;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
+    const int w = warp < NC ? warp : warp - NC, p = w / NQ, q = w % NQ;
     const int h = blockIdx.x / CS, rank = blockIdx.x % CS, kx = a.grouped ? h / (a.vh / a.kh) : h % a.kh;
     u8* const xb = sm + ST * M::STAGE;
-    u8* const ob = xb + M::NW * M::XB + warp * M::OB;
-    float* const ssq = (float*)(xb + M::NW * (M::XB + M::OB));            // [parity][block][group][row]
-    u64* const bar = (u64*)(ssq + M::SSQ / 4);
+    uint4* const sf = (uint4*)(xb + NC * M::XB);                          // [turn][chain's warp][number][16 key dimensions][lane]
+    uint4* const df = (uint4*)((u8*)sf + NC * 2 * M::FB);                 // [turn][group][number][16 rows][lane]
+    u8* const ob = (u8*)df + NG * 2 * M::FB + (warp - NC) * M::OB;
+    float* const ssq = (float*)((u8*)df + NG * 2 * M::FB + NC * M::OB);
+    u64* const bars = (u64*)((u8*)ssq + M::SSQ);
+    u64 *const full = bars, *const empty = full + ST, *const s_there = empty + ST, *const d_there = s_there + 2 * NG, *const s_free = d_there + 2 * NG, *const sq_there = s_free + 2 * NG;
+    float* const s_unit = (float*)(bars + M::BARS);                       // [turn][chain's warp], then [turn][group]: what a unit of S, of D is
+    float* const d_unit = s_unit + 2 * NC;
     const bool norm = OUT && a.norm != nullptr, joined = norm && CS > 1;
     if (tid == 0) {
-        for (int i = 0; i < ST; i++) sz_mbar_init(&bar[i], 1);
+        for (int i = 0; i < ST; i++) { sz_mbar_init(&full[i], 1 + 32); sz_mbar_init(&empty[i], M::CONSUMERS); }
+        for (int i = 0; i < 2 * NG; i++) { sz_mbar_init(&s_there[i], NQ); sz_mbar_init(&d_there[i], NQ); sz_mbar_init(&s_free[i], NQ); }
+        for (int i = 0; i < 4; i++) sz_mbar_init(&sq_there[i], CS * NC);
         sz_mbar_fence_init();
     }
     sz_pdl_wait();
@@ -327,352 +362,437 @@ sz_delta_chunk_kernel(const DlBatch d, const DlRule a, int idx0, int idx1, const
     if (lg.b < 0) return;                                                 // (the blocks of a head are all of one sequence: they leave together)
     const DlSeq s = dl_seq(d, lg.b, lane, false);
     const int chunks = (s.n + CK - 1) / CK;
-    const int c0 = max(0, idx0 - lg.base), c1 = min(chunks, idx1 - lg.base);
+    const int c0 = max(0, idx0 - lg.base), c1 = min(chunks, idx1 - lg.base), nc = max(0, c1 - c0);
     // (a sequence none of whose rows count still moves its state, in the pass that has its first place)
     const bool only = s.on && chunks == 0 && lg.base >= idx0 && lg.base < idx1;
-    if (!s.on || (c0 >= c1 && !only)) return;
+    if (!s.on || (nc == 0 && !only)) return;
     const int dv = (rank * NG + p) * 16;                                  // the warp's value dimensions
-    __syncthreads();
-    // S^T: dimensions g, g + 8; key dimensions 64 q + 8 m + 2 t, + 1
-    float S[8][4];
-    int es = 0;                                                           // .. in units of 2^es
-    {
-        const int from = c0 > 0 ? s.to : s.from;
-        const float* src = (const float*)(a.state + (size_t)max(from, 0) * a.state_stride) + ((size_t)h * D + 64 * q + 2 * t) * D + dv + g;
-#pragma unroll
-        for (int m = 0; m < 8; m++)
-#pragma unroll
-            for (int e = 0; e < 4; e++) S[m][e] = from >= 0 ? src[(size_t)(8 * m + (e & 1)) * D + 8 * (e >> 1)] : 0.f;
-    }
-    auto issue = [&](int c) {
-        u8* const st = sm + ((c - c0) % ST) * M::STAGE;
-        const int n = min(CK, s.n - c * CK);
-        if (tid == 0) {
-            const u8* src = scratch + (size_t)(lg.base + c - idx0) * one;
-            u64* const full = &bar[(c - c0) % ST];
-            asm volatile("fence.proxy.async;" ::: "memory");
-            sz_mbar_expect_tx(full, (OUT ? C::ROWS : C::ROWS / 2) + C::HEAD);
-            sz_bulk_g2s(st, src + (size_t)kx * C::ROWS, OUT ? C::ROWS : C::ROWS / 2, full);
-            sz_bulk_g2s(st + C::ROWS, src + (size_t)a.kh * C::ROWS + (size_t)h * C::HEAD, C::HEAD, full);
-        }
-        constexpr int PIECES = 16 * NG * ESZ / 16;
-        const size_t row0 = (size_t)s.r0 + (size_t)c * CK;
-        for (int i = tid; i < CK * PIECES; i += M::NTH) {
-            const int r = i / PIECES, x = i % PIECES;
-            const u32 to = sz_smem_addr(st + C::ROWS + C::HEAD + r * M::VS + 16 * x);
-            const int take = r < n ? 16 : 0;                              // (rows behind the last are zeros, and not read)
-            const size_t row = row0 + (r < n ? r : 0), col = (size_t)(h * D + rank * NG * 16) * ESZ + 16 * x;
-            asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(a.v + row * a.v_stride + col), "r"(take) : "memory");
-            if (norm) asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to + CK * M::VS), "l"(a.z + row * a.z_stride + col), "r"(take) : "memory");
-        }
-        sz_cp_async_commit();
-    };
-    // 16 value dimensions of a tile's rows, transposed: dimensions g, g + 8 of rows 8 m + 2 t, + 1
-    auto turned = [&](const u8* tile, int m, float* f) {                  // (two tiles of 8 rows: m, m + 1)
+    if (joined) sz_cluster_sync(); else __syncthreads();                  // (mbarriers are ready, in all blocks of the head)
+    bool dead = false;
+    auto wait = [&](u64* bar, int turn) { if (!dead && !sz_mbar_wait_warp(bar, turn & 1)) { dead = true; if (lane == 0) atomicOr(d.err, DL_E_WAIT); } };
+    auto arrive = [&](u64* bar) { __syncwarp(); if (lane == 0) sz_mbar_arrive(bar); };
+    // 16 value dimensions of two 8-row tiles m, m + 1 of a tile of rows, transposed: dimensions g, g + 8 of rows 8 m + 2 t, + 1
+    auto turned = [&](const u8* tile, int m, float* f) {
         if constexpr (TYPE == SZ_TYPE_F32) {
 #pragma unroll
             for (int i = 0; i < 2; i++)
 #pragma unroll
                 for (int e = 0; e < 4; e++) f[4 * i + e] = *(const float*)(tile + (8 * (m + i) + 2 * t + (e & 1)) * M::VS + (16 * p + g + 8 * (e >> 1)) * 4);
         } else {
-            u32 w[4];
-            dl_ldsm_t(w, sz_smem_addr(tile + (8 * m + ((lane >> 4) << 3) + (lane & 7)) * M::VS + (16 * p + ((lane >> 3) & 1) * 8) * 2));
-            dl_unpack<TYPE, 8>(w, f);
+            u32 r[4];
+            dl_ldsm_t(r, sz_smem_addr(tile + (8 * m + ((lane >> 4) << 3) + (lane & 7)) * M::VS + (16 * p + ((lane >> 3) & 1) * 8) * 2));
+            dl_unpack<TYPE, 8>(r, f);
         }
     };
-    float O[4 * OT];                                                      // outputs of the chunk before, on their way to their norm
-    float nw[2] = {0.f, 0.f};
-    if (norm) { nw[0] = a.norm[dv + g]; nw[1] = a.norm[dv + g + 8]; }
-    // the tiles whose outputs the warp finishes: pairs of like work
-    auto mine = [&](int i) { return NQ == 1 ? i : q == 0 ? (i < 2 ? i : i + 4) : i + 2; };
-    auto finish = [&](int c) {                                            // outputs of chunk c: their norm's factor, into shared memory by rows, out
-        const int n = min(CK, s.n - c * CK);
-#pragma unroll
-        for (int i = 0; i < OT; i++) {
-            float r0 = 1.f, r1 = 1.f;
-            const int row = 8 * mine(i) + 2 * t;
-            if (norm) {
-                float2 sum = make_float2(0.f, 0.f);
-                const float* w = ssq + (size_t)((c - c0) & 1) * CS * NG * CK + row;
-#pragma unroll
-                for (int j = 0; j < CS * NG; j++) { const float2 y = *(const float2*)(w + j * CK); sum.x += y.x; sum.y += y.y; }
-                r0 = rsqrtf(sum.x * (1.f / D) + a.eps); r1 = rsqrtf(sum.y * (1.f / D) + a.eps);
+    if (warp == M::CONSUMERS) {
+        // ---- copies
+        if (lane == 0) asm volatile("fence.proxy.async;" ::: "memory");   // (they read what the kernel before has written)
+        // (a chunk's operands in two pieces; v and z row by row in 16 bytes a lane: a copy of a row at a time by the TMA engine takes 58 cycles, 7,500 a chunk)
+        constexpr int PIECES = NG * ESZ, STEP = 32 / PIECES;              // of 16 bytes, a row's; rows the warp takes at once
+        const u32 col = (u32)(h * D + rank * NG * 16) * ESZ + 16 * (lane % PIECES);
+        for (int i = 0; i < nc; i++) {
+            const int c = c0 + i, slot = i % ST, n = min(CK, s.n - c * CK);
+            u8* const st = sm + slot * M::STAGE;
+            if (i >= ST) wait(&empty[slot], i / ST - 1);
+            if (lane == 0) {
+                const u8* src = scratch + (size_t)(lg.base + c - idx0) * one;
+                sz_mbar_expect_tx(&full[slot], (OUT ? C::ROWS : C::ROWS / 2) + C::HEAD);
+                sz_bulk_g2s(st, src + (size_t)kx * C::ROWS, OUT ? C::ROWS : C::ROWS / 2, &full[slot]);
+                sz_bulk_g2s(st + C::ROWS, src + (size_t)a.kh * C::ROWS + (size_t)h * C::HEAD, C::HEAD, &full[slot]);
             }
-            O[4 * i] *= r0; O[4 * i + 1] *= r1; O[4 * i + 2] *= r0; O[4 * i + 3] *= r1;
-            // row 8 i + 2 t (+ 1) of the warp's, dimension g (+ 8)
-#pragma unroll
-            for (int e = 0; e < 4; e++) {
-                u8* const at = ob + (8 * i + 2 * t + (e & 1)) * M::OS + (g + 8 * (e >> 1)) * ESZ;
-                if constexpr (TYPE == SZ_TYPE_F32) *(float*)at = O[4 * i + e];
-                else if constexpr (TYPE == SZ_TYPE_F16) *(__half*)at = __float2half_rn(O[4 * i + e]);
-                else *(__nv_bfloat16*)at = __float2bfloat16_rn(O[4 * i + e]);
+            __syncwarp();
+            const u32 to = sz_smem_addr(st + C::ROWS + C::HEAD + (lane / PIECES) * M::VS + 16 * (lane % PIECES));
+            const size_t row0 = (size_t)s.r0 + (size_t)c * CK;
+#pragma unroll 4
+            for (int k = 0; k < CK / STEP; k++) {                         // (rows behind the last are zeros, and not read)
+                const int r = k * STEP + lane / PIECES;
+                const size_t row = row0 + (r < n ? r : 0);
+                const u32 there = r < n ? 16 : 0;
+                asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to + k * STEP * M::VS), "l"(a.v + row * a.v_stride + col), "r"(there) : "memory");
+                if (M::STAGED && norm) asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to + (k * STEP + CK) * M::VS), "l"(a.z + row * a.z_stride + col), "r"(there) : "memory");
             }
+            asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(sz_smem_addr(&full[slot])) : "memory");
         }
-        __syncwarp();
-        constexpr int PIECES = ESZ;                                       // of 16 bytes, a row's 16 dimensions
-        for (int i = lane; i < 8 * OT * PIECES; i += 32) {
-            const int r = i / PIECES, x = i % PIECES, row = 8 * mine(r / 8) + r % 8;
-            if (row < n) *(uint4*)(a.out + ((size_t)s.r0 + (size_t)c * CK + row) * a.out_stride + (size_t)(h * D + dv) * ESZ + 16 * x) = *(const uint4*)(ob + r * M::OS + 16 * x);
-        }
-        __syncwarp();
-    };
-    if (joined) sz_cluster_sync();                                        // (all blocks of the head have begun)
-    bool dead = false;
-    if (c0 < c1) issue(c0);
-#pragma unroll 1
-    for (int c = c0; c < c1; c++) {
-        const int slot = (c - c0) % ST;
-        const bool more = c + 1 < c1;
-        if (ST == 2 && more) { issue(c + 1); sz_cp_async_wait<1>(); }
-        else sz_cp_async_wait<0>();
-        if (!dead && !sz_mbar_wait_warp(&bar[slot], ((c - c0) / ST) & 1)) { dead = true; if (lane == 0) atomicOr(d.err, DL_E_WAIT); }
-        __syncthreads();
-        const u8* const st = sm + slot * M::STAGE;
-        const u32 sk = sz_smem_addr(st), sq = sk + NK * C::TILE;
-        const u8* const hp = st + C::ROWS;
-        const DlScalars* const sc = (const DlScalars*)(hp + (C::FULL ? 4 : 3) * DL_FRAG);
-        const u8* const vt = st + C::ROWS + C::HEAD;
-        // ---- the state into f16's range
+        for (int i = max(0, nc - ST); i < nc; i++) wait(&full[i % ST], i / ST);      // (nothing is under way when the block ends, whoever gave up)
+        return;
+    }
+    if (warp < NC) {
+        // ---- the chain.  S^T: dimensions g, g + 8; key dimensions 64 q + 8 m + 2 t, + 1
+        float S[8][4];
+        int es = 0;                                                       // .. in units of 2^es
         {
-            float mx = 0.f;
+            const int from = c0 > 0 ? s.to : s.from;
+            const float* src = (const float*)(a.state + (size_t)max(from, 0) * a.state_stride) + ((size_t)h * D + 64 * q + 2 * t) * D + dv + g;
 #pragma unroll
             for (int m = 0; m < 8; m++)
 #pragma unroll
-                for (int e = 0; e < 4; e++) mx = fmaxf(mx, fabsf(S[m][e]));
-            const u32 top = __reduce_max_sync(0xffffffffu, __float_as_uint(mx)) >> 23;
-            const int ex = (int)top - 127;
-            if (top != 0 && top != 255 && (ex > 13 || ex < 4)) {
-                const int up = max(-120, min(120, 10 - ex));
-                const float f = dl_pow2(up);
-#pragma unroll
-                for (int m = 0; m < 8; m++)
-#pragma unroll
-                    for (int e = 0; e < 4; e++) S[m][e] *= f;
-                es -= up;
-            }
+                for (int e = 0; e < 4; e++) S[m][e] = from >= 0 ? src[(size_t)(8 * m + (e & 1)) * D + 8 * (e >> 1)] : 0.f;
         }
-        // ---- (K S)^T and (Q S)^T: dimensions x rows
-        float X[8][4], Y[8][4];
+        auto exponent = [&](float (*x)[4]) {                              // of the largest of the warp's numbers, and 127
+            float mx[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int m = 0; m < 8; m++)
+            for (int m = 0; m < 8; m++)
 #pragma unroll
-            for (int e = 0; e < 4; e++) X[m][e] = Y[m][e] = 0.f;
+                for (int e = 0; e < 4; e++) mx[e] = fmaxf(mx[e], fabsf(x[m][e]));
+            return (int)(__reduce_max_sync(0xffffffffu, __float_as_uint(fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])))) >> 23);
+        };
+#pragma unroll 1
+        for (int i = 0; i < nc; i++) {
+            const int slot = i % ST, turn = i & 1;
+            const u8* const st = sm + slot * M::STAGE;
+            const u32 sk = sz_smem_addr(st);
+            const u8* const hp = st + C::ROWS;
+            const DlScalars* const sc = (const DlScalars*)(hp + (C::FULL ? 4 : 3) * DL_FRAG);
+            {                                                             // the state into f16's range
+                const int top = exponent(S), ex = top - 127;
+                if (top != 0 && top != 255 && (ex > 13 || ex < 4)) {
+                    const int up = max(-120, min(120, 10 - ex));
 #pragma unroll
-        for (int ks = 0; ks < 4; ks++) {
-            u32 hi[4], lo[4];
+                    for (int m = 0; m < 8; m++) dl_scale4(S[m], dl_pow2(up));
+                    es -= up;
+                }
+            }
+            if (OUT && i >= 2) wait(&s_free[turn * NG + p], i / 2 - 1);   // (the outputs have taken what lies there)
+            wait(&full[slot], i / ST);
+            // ---- (K S)^T: dimensions x rows.  (Terms one after the other over all rows, so that no product waits for the one before it.)
+            float X[8][4];
 #pragma unroll
-            for (int e = 0; e < 4; e++) dl_split(S[2 * ks + (e >> 1)][2 * (e & 1)], S[2 * ks + (e >> 1)][2 * (e & 1) + 1], hi[e], lo[e]);
+            for (int m = 0; m < 8; m++)
+#pragma unroll
+                for (int e = 0; e < 4; e++) X[m][e] = 0.f;
+#pragma unroll
+            for (int ks = 0; ks < 4; ks++) {
+                u32 hi[4], lo[4], b[4][4];
+                auto load = [&](u32 tile) {
+#pragma unroll
+                    for (int m = 0; m < 4; m++) dl_ldsm(b[m], tile + dl_at<D>(16 * m + ((lane >> 4) << 3) + (lane & 7), 8 * q + 2 * ks + ((lane >> 3) & 1)));
+                };
+                auto times = [&](const u32* f) {
+#pragma unroll
+                    for (int m = 0; m < 8; m++) dl_mma(X[m], f, b[m / 2][2 * (m & 1)], b[m / 2][2 * (m & 1) + 1]);
+                };
+                load(sk);
+#pragma unroll
+                for (int e = 0; e < 4; e++) dl_split(S[2 * ks + (e >> 1)][2 * (e & 1)], S[2 * ks + (e >> 1)][2 * (e & 1) + 1], hi[e], lo[e]);
+                if (OUT) {
+                    sf[(((turn * NC + w) * FP) * 4 + ks) * 32 + lane] = *(uint4*)hi;
+                    if (C::FULL) sf[(((turn * NC + w) * FP + 1) * 4 + ks) * 32 + lane] = *(uint4*)lo;
+                }
+                times(hi);
+                times(lo);
+                if (NK == 2) { load(sk + C::TILE); times(hi); }
+            }
+            const float true_s = dl_pow2(es);
+            if (OUT) { if (lane == 0) s_unit[turn * NC + w] = true_s; arrive(&s_there[turn * NG + p]); }
+#pragma unroll
+            for (int m = 0; m < 8; m++) dl_scale4(X[m], true_s);
+            if constexpr (NQ == 2) {                                      // with the other key dimensions'
+                float4* const to = (float4*)(xb + w * M::XB) + turn * 8 * 32 + lane;
+                const float4* const from = (const float4*)(xb + (w ^ 1) * M::XB) + turn * 8 * 32 + lane;
+#pragma unroll
+                for (int m = 0; m < 8; m++) to[m * 32] = make_float4(X[m][0], X[m][1], X[m][2], X[m][3]);
+                asm volatile("bar.sync %0, 64;" ::"r"(1 + p) : "memory");
+#pragma unroll
+                for (int m = 0; m < 8; m++) {
+                    const float4 y = from[m * 32];
+                    X[m][0] += y.x; X[m][1] += y.y; X[m][2] += y.z; X[m][3] += y.w;
+                }
+            }
+            // ---- R = V - e^G K S, in units of 2^ew
 #pragma unroll
             for (int m = 0; m < 8; m += 2) {
-                const u32 at = dl_at<D>(8 * m + ((lane >> 4) << 3) + (lane & 7), 8 * q + 2 * ks + ((lane >> 3) & 1));
-                u32 b[4], b2[4];
-                dl_ldsm(b, sk + at);
-                if (NK == 2) dl_ldsm(b2, sk + C::TILE + at);
-#pragma unroll
-                for (int i = 0; i < 2; i++) {
-                    dl_mma(X[m + i], hi, b[2 * i], b[2 * i + 1]);
-                    dl_mma(X[m + i], lo, b[2 * i], b[2 * i + 1]);
-                    if (NK == 2) dl_mma(X[m + i], hi, b2[2 * i], b2[2 * i + 1]);
-                }
-                if (OUT) {
-                    dl_ldsm(b, sq + at);
-                    if (NK == 2) dl_ldsm(b2, sq + C::TILE + at);
-#pragma unroll
-                    for (int i = 0; i < 2; i++) {
-                        dl_mma(Y[m + i], hi, b[2 * i], b[2 * i + 1]);
-                        if (C::FULL) dl_mma(Y[m + i], lo, b[2 * i], b[2 * i + 1]);
-                        if (NK == 2) dl_mma(Y[m + i], hi, b2[2 * i], b2[2 * i + 1]);
-                    }
-                }
-            }
-        }
-        const float true_s = dl_pow2(es);
-#pragma unroll
-        for (int m = 0; m < 8; m++)
-#pragma unroll
-            for (int e = 0; e < 4; e++) { X[m][e] *= true_s; if (OUT) Y[m][e] *= true_s; }
-        if constexpr (NQ == 2) {                                          // with the other key dimensions'
-            float4* const to = (float4*)(xb + warp * M::XB);
-            const float4* const from = (const float4*)(xb + (warp ^ 1) * M::XB);
-#pragma unroll
-            for (int m = 0; m < 8; m++) to[m * 32 + lane] = make_float4(X[m][0], X[m][1], X[m][2], X[m][3]);
-            if (OUT)
-#pragma unroll
-                for (int i = 0; i < 4; i++) {                             // the tiles that the partner finishes
-                    const int mq0 = i + 2, mq1 = i < 2 ? i : i + 4;       // .. of q = 1, of q = 0
-                    to[(8 + i) * 32 + lane] = q == 0 ? make_float4(Y[mq0][0], Y[mq0][1], Y[mq0][2], Y[mq0][3]) : make_float4(Y[mq1][0], Y[mq1][1], Y[mq1][2], Y[mq1][3]);
-                }
-            asm volatile("bar.sync %0, 64;" ::"r"(1 + p) : "memory");
-#pragma unroll
-            for (int m = 0; m < 8; m++) {
-                const float4 y = from[m * 32 + lane];
-                X[m][0] += y.x; X[m][1] += y.y; X[m][2] += y.z; X[m][3] += y.w;
-            }
-            if (OUT)
-#pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    const float4 y = from[(8 + i) * 32 + lane];
-                    const int m0 = i < 2 ? i : i + 4, m1 = i + 2;
-                    // (own tiles side by side in Y's first four)
-                    const float o0 = q == 0 ? Y[m0][0] : Y[m1][0], o1 = q == 0 ? Y[m0][1] : Y[m1][1], o2 = q == 0 ? Y[m0][2] : Y[m1][2], o3 = q == 0 ? Y[m0][3] : Y[m1][3];
-                    Y[i][0] = o0 + y.x; Y[i][1] = o1 + y.y; Y[i][2] = o2 + y.z; Y[i][3] = o3 + y.w;
-                }
-        }
-        // ---- R = V - e^G K S, in units of 2^ew
-        float mx = 0.f;
-#pragma unroll
-        for (int m = 0; m < 8; m += 2) {
-            float v[8];
-            turned(vt, m, v);
-#pragma unroll
-            for (int i = 0; i < 2; i++) {
-                const float2 gr = *(const float2*)(sc->gr + 8 * (m + i) + 2 * t);
-#pragma unroll
-                for (int e = 0; e < 4; e++) {
-                    X[m + i][e] = fmaf(-(e & 1 ? gr.y : gr.x), X[m + i][e], v[4 * i + e]);
-                    mx = fmaxf(mx, fabsf(X[m + i][e]));
-                }
-            }
-        }
-        int ew = es;
-        {
-            const u32 top = __reduce_max_sync(0xffffffffu, __float_as_uint(mx)) >> 23;
-            if (top != 0 && top != 255) ew = max(max((int)top - 127 - 8, -120), es - 100);      // (changes are at most 64 times the largest of R: below 2^15)
-        }
-        u32 rh[4][4], rl[4][4];
-        {
-            const float f = dl_pow2(-ew);
-#pragma unroll
-            for (int ks = 0; ks < 4; ks++)
-#pragma unroll
-                for (int e = 0; e < 4; e++) dl_split(X[2 * ks + (e >> 1)][2 * (e & 1)] * f, X[2 * ks + (e >> 1)][2 * (e & 1) + 1] * f, rh[ks][e], rl[ks][e]);
-        }
-        // ---- the rows' changes D^T = R^T T^T
-#pragma unroll
-        for (int m = 0; m < 8; m++) {
-#pragma unroll
-            for (int e = 0; e < 4; e++) X[m][e] = 0.f;
-#pragma unroll
-            for (int ks = 0; ks <= m / 2; ks++) {
-                const uint2 th = ((const uint2*)hp)[(dl_tile(m) + ks) * 32 + lane], tl = ((const uint2*)(hp + DL_FRAG))[(dl_tile(m) + ks) * 32 + lane];
-                dl_mma(X[m], rh[ks], th.x, th.y);
-                dl_mma(X[m], rl[ks], th.x, th.y);
-                dl_mma(X[m], rh[ks], tl.x, tl.y);
-            }
-        }
-        // ---- outputs: e^G Q S + P D
-        if (OUT) {
-            if (norm && c > c0) {                                         // the chunk before: its sums are here
-                if (joined) sz_cluster_wait();
-                finish(c - 1);
-            }
-            u32 dh[4][4], dlo[4][4];
-#pragma unroll
-            for (int ks = 0; ks < 4; ks++)
-#pragma unroll
-                for (int e = 0; e < 4; e++) {
-                    if (C::FULL) dl_split(X[2 * ks + (e >> 1)][2 * (e & 1)], X[2 * ks + (e >> 1)][2 * (e & 1) + 1], dh[ks][e], dlo[ks][e]);
-                    else dh[ks][e] = dl_h2(X[2 * ks + (e >> 1)][2 * (e & 1)], X[2 * ks + (e >> 1)][2 * (e & 1) + 1]);
-                }
-            const float tw = dl_pow2(ew) * (1.f / DL_P);
-            const u8* const zt = vt + CK * M::VS;
-#pragma unroll
-            for (int i = 0; i < OT; i += 2) {
-                const int m0 = mine(i);                                   // (tiles m0, m0 + 1: their 16-row columns end with theirs)
-                float acc[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
-#pragma unroll
-                for (int u = 0; u < 2; u++)
-#pragma unroll
-                    for (int ks = 0; ks < 4; ks++)
-                        if (ks <= m0 / 2) {
-                            const int at = (dl_tile(m0 + u) + ks) * 32 + lane;
-                            const uint2 ph = ((const uint2*)(hp + 2 * DL_FRAG))[at];
-                            dl_mma(acc[u], dh[ks], ph.x, ph.y);
-                            if (C::FULL) {
-                                const uint2 pl = ((const uint2*)(hp + 3 * DL_FRAG))[at];
-                                dl_mma(acc[u], dlo[ks], ph.x, ph.y);
-                                dl_mma(acc[u], dh[ks], pl.x, pl.y);
-                            }
-                        }
-                float z[8];
-                if (norm) turned(zt, m0, z);
+                float v[8];
+                turned(st + C::ROWS + C::HEAD, m, v);
 #pragma unroll
                 for (int u = 0; u < 2; u++) {
-                    const float2 gq = *(const float2*)(sc->gq + 8 * (m0 + u) + 2 * t);
+                    const float2 gr = *(const float2*)(sc->gr + 8 * (m + u) + 2 * t);
 #pragma unroll
-                    for (int e = 0; e < 4; e++) O[4 * (i + u) + e] = fmaf(e & 1 ? gq.y : gq.x, Y[i + u][e], acc[u][e] * tw);
-                    if (norm) {
-                        float s0 = fmaf(O[4 * (i + u)], O[4 * (i + u)], O[4 * (i + u) + 2] * O[4 * (i + u) + 2]);
-                        float s1 = fmaf(O[4 * (i + u) + 1], O[4 * (i + u) + 1], O[4 * (i + u) + 3] * O[4 * (i + u) + 3]);
-#pragma unroll
-                        for (int o = 4; o < 32; o *= 2) { s0 += __shfl_xor_sync(0xffffffffu, s0, o); s1 += __shfl_xor_sync(0xffffffffu, s1, o); }
-                        float* const at = ssq + ((size_t)((c - c0) & 1) * CS * NG + rank * NG + p) * CK + 8 * (m0 + u) + 2 * t;
-                        if (CS == 1) { if (g == 0) *(float2*)at = make_float2(s0, s1); }
-                        else if (g < CS) {                                // lanes of g: to block g of the head
-                            u32 there;
-                            asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(there) : "r"(sz_smem_addr(at)), "r"(g));
-                            asm volatile("st.shared::cluster.v2.f32 [%0], {%1, %2};" ::"r"(there), "f"(s0), "f"(s1) : "memory");
-                        }
-#pragma unroll
-                        for (int e = 0; e < 4; e++) O[4 * (i + u) + e] *= nw[e >> 1] * sz_sigmoid(z[4 * u + e]);
-                    }
+                    for (int e = 0; e < 4; e++) X[m + u][e] = fmaf(-(e & 1 ? gr.y : gr.x), X[m + u][e], v[4 * u + e]);
                 }
             }
-            if (joined) sz_cluster_arrive();
-            if (!norm) finish(c);
-        }
-        // ---- the state: e^G_C S + K^T (e^(G_C - G_j) D)
-        {
+            int ew = es;
+            {
+                const int top = exponent(X);
+                if (top != 0 && top != 255) ew = max(max(top - 127 - 8, -120), es - 100);      // (changes are at most 64 times the largest of R: below 2^15)
+            }
+            u32 rh[4][4], rl[4][4];
+            {
+                const float f = dl_pow2(-ew);
+#pragma unroll
+                for (int m = 0; m < 8; m++) dl_scale4(X[m], f);
+#pragma unroll
+                for (int ks = 0; ks < 4; ks++)
+#pragma unroll
+                    for (int e = 0; e < 4; e++) dl_split(X[2 * ks + (e >> 1)][2 * (e & 1)], X[2 * ks + (e >> 1)][2 * (e & 1) + 1], rh[ks][e], rl[ks][e]);
+            }
+            // ---- the rows' changes D^T = R^T T^T
+#pragma unroll
+            for (int m = 0; m < 8; m++)
+#pragma unroll
+                for (int e = 0; e < 4; e++) X[m][e] = 0.f;
+#pragma unroll
+            for (int ks = 0; ks < 4; ks++) {
+                uint2 f[8];
+#pragma unroll
+                for (int m = 2 * ks; m < 8; m++) f[m] = ((const uint2*)hp)[(dl_tile(m) + ks) * 32 + lane];
+#pragma unroll
+                for (int m = 2 * ks; m < 8; m++) dl_mma(X[m], rh[ks], f[m].x, f[m].y);
+#pragma unroll
+                for (int m = 2 * ks; m < 8; m++) dl_mma(X[m], rl[ks], f[m].x, f[m].y);
+#pragma unroll
+                for (int m = 2 * ks; m < 8; m++) f[m] = ((const uint2*)(hp + DL_FRAG))[(dl_tile(m) + ks) * 32 + lane];
+#pragma unroll
+                for (int m = 2 * ks; m < 8; m++) dl_mma(X[m], rh[ks], f[m].x, f[m].y);
+            }
+            if (OUT) {                                                    // for the outputs: half of it a warp
+#pragma unroll
+                for (int k = 0; k < 4 / NQ; k++) {
+                    u32 hi[4], lo[4];
+#pragma unroll
+                    for (int e = 0; e < 4; e++) {
+                        const int m0 = 2 * k + (e >> 1), m1 = (4 / NQ) * 2 % 8 + m0;      // (of q = 0, of q = 1)
+                        const float x0 = NQ == 2 && q ? X[m1][2 * (e & 1)] : X[m0][2 * (e & 1)], x1 = NQ == 2 && q ? X[m1][2 * (e & 1) + 1] : X[m0][2 * (e & 1) + 1];
+                        if (C::FULL) dl_split(x0, x1, hi[e], lo[e]); else hi[e] = dl_h2(x0, x1);
+                    }
+                    df[(((turn * NG + p) * FP) * 4 + q * (4 / NQ) + k) * 32 + lane] = *(uint4*)hi;
+                    if (C::FULL) df[(((turn * NG + p) * FP + 1) * 4 + q * (4 / NQ) + k) * 32 + lane] = *(uint4*)lo;
+                }
+                if (lane == 0 && q == 0) d_unit[turn * NG + p] = dl_pow2(ew) * (1.f / DL_P);
+                arrive(&d_there[turn * NG + p]);
+            }
+            // ---- the state: e^G_C S + K^T (e^(G_C - G_j) D)
 #pragma unroll
             for (int m = 0; m < 8; m++) {
-                const float2 w = *(const float2*)(sc->wj + 8 * m + 2 * t);
-                X[m][0] *= w.x; X[m][1] *= w.y; X[m][2] *= w.x; X[m][3] *= w.y;
+                const float2 wj = *(const float2*)(sc->wj + 8 * m + 2 * t);
+                X[m][0] *= wj.x; X[m][1] *= wj.y; X[m][2] *= wj.x; X[m][3] *= wj.y;
             }
             const float f = sc->gc * dl_pow2(max(es - ew, -126));
 #pragma unroll
-            for (int m = 0; m < 8; m++)
-#pragma unroll
-                for (int e = 0; e < 4; e++) S[m][e] *= f;
+            for (int m = 0; m < 8; m++) dl_scale4(S[m], f);
             es = ew;
 #pragma unroll
             for (int ks = 0; ks < 4; ks++) {
-                u32 hi[4], lo[4];
+                u32 hi[4], lo[4], b[4][4];
+                auto load = [&](u32 tile) {
+#pragma unroll
+                    for (int m = 0; m < 4; m++) dl_ldsm_t(b[m], tile + dl_at<D>(16 * ks + (((lane >> 3) & 1) << 3) + (lane & 7), 8 * q + 2 * m + (lane >> 4)));
+                };
+                auto times = [&](const u32* x) {
+#pragma unroll
+                    for (int m = 0; m < 8; m++) dl_mma(S[m], x, b[m / 2][2 * (m & 1)], b[m / 2][2 * (m & 1) + 1]);
+                };
+                load(sk);
 #pragma unroll
                 for (int e = 0; e < 4; e++) dl_split(X[2 * ks + (e >> 1)][2 * (e & 1)], X[2 * ks + (e >> 1)][2 * (e & 1) + 1], hi[e], lo[e]);
+                times(hi);
+                times(lo);
+                if (NK == 2) { load(sk + C::TILE); times(hi); }
+            }
+            arrive(&empty[slot]);
+        }
+        float* to = (float*)(a.state + (size_t)s.to * a.state_stride) + ((size_t)h * D + 64 * q + 2 * t) * D + dv + g;
+        const float f0 = dl_pow2(es / 2), f1 = dl_pow2(es - es / 2);      // (in two steps: 2^es alone may be out of range)
 #pragma unroll
-                for (int m = 0; m < 8; m += 2) {
-                    const u32 at = dl_at<D>(16 * ks + (((lane >> 3) & 1) << 3) + (lane & 7), 8 * q + m + (lane >> 4));
-                    u32 b[4], b2[4];
-                    dl_ldsm_t(b, sk + at);
-                    if (NK == 2) dl_ldsm_t(b2, sk + C::TILE + at);
+        for (int m = 0; m < 8; m++)
 #pragma unroll
-                    for (int i = 0; i < 2; i++) {
-                        dl_mma(S[m + i], hi, b[2 * i], b[2 * i + 1]);
-                        dl_mma(S[m + i], lo, b[2 * i], b[2 * i + 1]);
-                        if (NK == 2) dl_mma(S[m + i], hi, b2[2 * i], b2[2 * i + 1]);
+            for (int e = 0; e < 4; e++) to[(size_t)(8 * m + (e & 1)) * D + 8 * (e >> 1)] = S[m][e] * f0 * f1;
+        return;
+    }
+    if constexpr (OUT) {
+        // ---- the outputs: e^G Q S + P D, of OT 8-row tiles a warp (of pairs of like work)
+        auto mine = [&](int i) { return NQ == 1 ? i : q == 0 ? (i < 2 ? i : i + 4) : i + 2; };
+        float O[4 * OT];
+        float nw[2] = {0.f, 0.f};
+        if (norm) { nw[0] = a.norm[dv + g]; nw[1] = a.norm[dv + g + 8]; }
+        auto wait_sums = [&](int k) {                                     // (from other blocks' stores: acquired at the cluster's scope)
+            u64* const bar = &sq_there[k & 3];
+            bool there = dead;
+            for (u32 i = 0; !there && i < 20000000u; i++) {
+                u32 ok;
+                asm volatile("{ .reg .pred p; mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2; selp.u32 %0, 1, 0, p; }" : "=r"(ok) : "r"(sz_smem_addr(bar)), "r"((u32)(k / 4) & 1) : "memory");
+                there = ok != 0;
+            }
+            if (!__all_sync(0xffffffffu, there)) { dead = true; if (lane == 0) atomicOr(d.err, DL_E_WAIT); }
+        };
+        auto finish = [&](int k) {                                        // of the k-th chunk: their norm's factor, into shared memory by rows, out
+            const int c = c0 + k, n = min(CK, s.n - c * CK);
+#pragma unroll
+            for (int i = 0; i < OT; i++) {
+                const int row = 8 * mine(i) + 2 * t;
+                if (norm) {
+                    // (a lane of g has the sums of one group of 16 dimensions)
+                    float2 sum = *(const float2*)(ssq + ((size_t)(k & 3) * CS * NG + g % (CS * NG)) * CK + row);
+#pragma unroll
+                    for (int o = 4; o < 4 * CS * NG; o *= 2) { sum.x += __shfl_xor_sync(0xffffffffu, sum.x, o); sum.y += __shfl_xor_sync(0xffffffffu, sum.y, o); }
+                    const float r0 = rsqrtf(sum.x * (1.f / D) + a.eps), r1 = rsqrtf(sum.y * (1.f / D) + a.eps);
+                    O[4 * i] *= r0; O[4 * i + 1] *= r1; O[4 * i + 2] *= r0; O[4 * i + 3] *= r1;
+                }
+                // row 8 i + 2 t (+ 1) of the warp's, dimension g (+ 8)
+                if constexpr (!M::STAGED) {
+                    u8* const at = a.out + ((size_t)s.r0 + (size_t)c * CK + row) * a.out_stride + (size_t)(h * D + dv + g) * 4;
+#pragma unroll
+                    for (int e = 0; e < 4; e++) if (row + (e & 1) < n) *(float*)(at + (e & 1) * a.out_stride + 32 * (e >> 1)) = O[4 * i + e];
+                } else if (i & 1) {
+                    u32 r[4];
+#pragma unroll
+                    for (int e = 0; e < 4; e++) {
+                        const float* o = O + 4 * (i - 1) + 2 * e;
+                        if constexpr (TYPE == SZ_TYPE_F16) r[e] = dl_h2(o[0], o[1]);
+                        else { const __nv_bfloat162 b = __floats2bfloat162_rn(o[0], o[1]); r[e] = *(const u32*)&b; }
                     }
+                    dl_stsm_t(sz_smem_addr(ob + (8 * (i - 1) + ((lane >> 4) << 3) + (lane & 7)) * M::OS + ((lane >> 3) & 1) * 16), r);
                 }
             }
+            if (!M::STAGED) return;
+            __syncwarp();
+            constexpr int PIECES = ESZ;                                   // of 16 bytes, a row's 16 dimensions
+#pragma unroll
+            for (int i = 0; i < OT * PIECES / 4; i++) {
+                const int r = (32 * i + lane) / PIECES, x = (32 * i + lane) % PIECES, row = 8 * mine(r / 8) + r % 8;
+                if (row < n) *(uint4*)(a.out + ((size_t)s.r0 + (size_t)c * CK + row) * a.out_stride + (size_t)(h * D + dv) * ESZ + 16 * x) = *(const uint4*)(ob + r * M::OS + 16 * x);
+            }
+            __syncwarp();
+        };
+#pragma unroll 1
+        for (int k = 0; k < nc; k++) {
+            const int slot = k % ST, turn = k & 1;
+            const u8* const st = sm + slot * M::STAGE;
+            const u32 sq = sz_smem_addr(st) + NK * C::TILE;
+            const u8* const hp = st + C::ROWS;
+            const DlScalars* const sc = (const DlScalars*)(hp + (C::FULL ? 4 : 3) * DL_FRAG);
+            const u8* const zt = st + C::ROWS + C::HEAD + CK * M::VS;
+            float zd[M::STAGED ? 1 : 4 * OT];                             // (f32: the gates, asked for early)
+            if (!M::STAGED && norm) {
+                const int n = min(CK, s.n - (c0 + k) * CK);
+#pragma unroll
+                for (int i = 0; i < OT; i++)
+#pragma unroll
+                    for (int e = 0; e < 4; e++) {
+                        const int row = 8 * mine(i) + 2 * t + (e & 1);
+                        zd[M::STAGED ? 0 : 4 * i + e] = row < n ? *(const float*)(a.z + ((size_t)s.r0 + (size_t)(c0 + k) * CK + row) * a.z_stride + (size_t)(h * D + dv + g + 8 * (e >> 1)) * 4) : 0.f;
+                    }
+            }
+            wait(&full[slot], k / ST);
+            wait(&s_there[turn * NG + p], k / 2);
+            float Y[NQ][OT][4];
+#pragma unroll
+            for (int j = 0; j < NQ; j++)
+#pragma unroll
+                for (int i = 0; i < OT; i++)
+#pragma unroll
+                    for (int e = 0; e < 4; e++) Y[j][i][e] = 0.f;
+#pragma unroll
+            for (int ks = 0; ks < 4; ks++)
+#pragma unroll
+                for (int j = 0; j < NQ; j++) {
+                    u32 hi[4], lo[4];
+                    *(uint4*)hi = sf[(((turn * NC + p * NQ + j) * FP) * 4 + ks) * 32 + lane];
+                    if (C::FULL) *(uint4*)lo = sf[(((turn * NC + p * NQ + j) * FP + 1) * 4 + ks) * 32 + lane];
+#pragma unroll
+                    for (int i = 0; i < OT; i += 2) {
+                        const u32 at = dl_at<D>(8 * mine(i) + ((lane >> 4) << 3) + (lane & 7), 8 * j + 2 * ks + ((lane >> 3) & 1));
+                        u32 b[4];
+                        dl_ldsm(b, sq + at);
+                        dl_mma(Y[j][i], hi, b[0], b[1]);
+                        dl_mma(Y[j][i + 1], hi, b[2], b[3]);
+                        if (C::FULL) { dl_mma(Y[j][i], lo, b[0], b[1]); dl_mma(Y[j][i + 1], lo, b[2], b[3]); }
+                        if (NK == 2) {
+                            dl_ldsm(b, sq + C::TILE + at);
+                            dl_mma(Y[j][i], hi, b[0], b[1]);
+                            dl_mma(Y[j][i + 1], hi, b[2], b[3]);
+                        }
+                    }
+                }
+#pragma unroll
+            for (int j = 0; j < NQ; j++) {
+                const float f = s_unit[turn * NC + p * NQ + j];
+#pragma unroll
+                for (int i = 0; i < OT; i++)
+#pragma unroll
+                    for (int e = 0; e < 4; e++) Y[0][i][e] = j == 0 ? Y[0][i][e] * f : fmaf(Y[j][i][e], f, Y[0][i][e]);
+            }
+            wait(&d_there[turn * NG + p], k / 2);
+            float acc[OT][4];
+#pragma unroll
+            for (int i = 0; i < OT; i++)
+#pragma unroll
+                for (int e = 0; e < 4; e++) acc[i][e] = 0.f;
+#pragma unroll
+            for (int ks = 0; ks < 4; ks++) {
+                u32 hi[4], lo[4];
+                *(uint4*)hi = df[(((turn * NG + p) * FP) * 4 + ks) * 32 + lane];
+                if (C::FULL) *(uint4*)lo = df[(((turn * NG + p) * FP + 1) * 4 + ks) * 32 + lane];
+#pragma unroll
+                for (int part = 0; part < (C::FULL ? 3 : 1); part++)      // high high, low high, high low
+#pragma unroll
+                    for (int i = 0; i < OT; i++)
+                        if (ks <= mine(i) / 2) {
+                            const uint2 f = ((const uint2*)(hp + (part == 2 ? 3 : 2) * DL_FRAG))[(dl_tile(mine(i)) + ks) * 32 + lane];
+                            dl_mma(acc[i], part == 1 ? lo : hi, f.x, f.y);
+                        }
+            }
+            const float tw = d_unit[turn * NG + p];
+            arrive(&s_free[turn * NG + p]);
+            float N[4 * OT];
+#pragma unroll
+            for (int i = 0; i < OT; i++) {
+                const float2 gq = *(const float2*)(sc->gq + 8 * mine(i) + 2 * t);
+#pragma unroll
+                for (int e = 0; e < 4; e++) N[4 * i + e] = fmaf(e & 1 ? gq.y : gq.x, Y[0][i][e], acc[i][e] * tw);
+            }
+            if (norm) {
+#pragma unroll
+                for (int i = 0; i < OT; i++) {
+                    const float* o = N + 4 * i;
+                    float s0 = fmaf(o[0], o[0], o[2] * o[2]), s1 = fmaf(o[1], o[1], o[3] * o[3]);
+#pragma unroll
+                    for (int x = 4; x < 32; x *= 2) { s0 += __shfl_xor_sync(0xffffffffu, s0, x); s1 += __shfl_xor_sync(0xffffffffu, s1, x); }
+                    float* const at = ssq + ((size_t)(k & 3) * CS * NG + rank * NG + p) * CK + 8 * mine(i) + 2 * t;
+                    if constexpr (CS == 1) { if (g == 0) *(float2*)at = make_float2(s0, s1); }
+                    else if (g < CS) {                                    // lanes of g: to block g of the head
+                        u32 there;
+                        asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(there) : "r"(sz_smem_addr(at)), "r"(g));
+                        asm volatile("st.shared::cluster.v2.f32 [%0], {%1, %2};" ::"r"(there), "f"(s0), "f"(s1) : "memory");
+                    }
+                }
+                // they are there.  (Four turns: a warp that sends the k-th chunk's has seen all of the k - 2nd's, whose senders had read the k - 4th's.  Said before the chunk before is stored: a release waits for every store of its thread)
+                if constexpr (CS == 1) arrive(&sq_there[k & 3]);
+                else {
+                    __syncwarp();
+                    if (t == 0 && g < CS) {
+                        u32 bar;
+                        asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(bar) : "r"(sz_smem_addr(&sq_there[k & 3])), "r"(g));
+                        asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+                    }
+                }
+#pragma unroll
+                for (int i = 0; i < OT; i += 2) {
+                    float z[8];
+                    if constexpr (M::STAGED) turned(zt, mine(i), z);
+                    else
+#pragma unroll
+                        for (int e = 0; e < 8; e++) z[e] = zd[4 * i + e];
+#pragma unroll
+                    for (int e = 0; e < 8; e++) N[4 * i + e] *= nw[(e >> 1) & 1] * dl_sigmoid<TYPE>(z[e]);
+                }
+            }
+            arrive(&empty[slot]);
+            if (norm && k > 0) { wait_sums(k - 1); finish(k - 1); }       // the chunk before
+#pragma unroll
+            for (int e = 0; e < 4 * OT; e++) O[e] = N[e];
+            if (!norm) finish(k);
         }
-        __syncthreads();                                                  // (the stage is free, and the sums of squares of this block are there)
-        if (ST == 1 && more) issue(c + 1);
+        if (norm && nc > 0) {
+            wait_sums(nc - 1);
+            finish(nc - 1);
+        }
     }
-    if (norm && c0 < c1) {
-        if (joined) sz_cluster_wait();
-        finish(c1 - 1);
-    }
-    float* to = (float*)(a.state + (size_t)s.to * a.state_stride) + ((size_t)h * D + 64 * q + 2 * t) * D + dv + g;
-    const float f0 = dl_pow2(es / 2), f1 = dl_pow2(es - es / 2);          // (in two steps: 2^es alone may be out of range)
-#pragma unroll
-    for (int m = 0; m < 8; m++)
-#pragma unroll
-        for (int e = 0; e < 4; e++) to[(size_t)(8 * m + (e & 1)) * D + 8 * (e >> 1)] = S[m][e] * f0 * f1;
 }
 
 template <int D, int TYPE, int NG, bool OUT>
 int dl_chunk_go(const DlBatch& b, const DlRule& r, int longest, int64_t total, int64_t per, uint64_t scratch, cudaStream_t st) {
     using P = DlPrep<D, TYPE>;
-    using M = DlMain<D, TYPE, NG>;
+    using M = DlMain<D, TYPE, NG, OUT>;
     static_assert(M::SMEM <= 227 * 1024 && P::SMEM <= 113 * 1024, "");
     const auto prep = sz_delta_prep_kernel<D, TYPE, OUT>;
     const auto chain = sz_delta_chunk_kernel<D, TYPE, NG, OUT>;
