@@ -10,9 +10,14 @@ constexpr int DL_SM = 148;           // multiprocessors (a GPU with another numb
 
 // ---- the causal convolution --------------------------------------------------------------------------------------------------------------
 // y[r][c] = silu(bias[c] + sum_t w[c][t] x[r - (K - 1) + t][c]); rows before a sequence's first are those its slot carries (K - 1, the oldest first).  The taps are
-// added in f32 from the oldest on.  A thread has 16 bytes of neighbouring channels and `tile` rows, one after the other, with the window in registers;
-// the one that has a sequence's first row leaves the new carried rows, which are rows of the call or of the old slot (so nothing is read after
-// somebody else wrote it).  Memory bound: what a tile reads twice are its first K - 1 rows, from L2.
+// added in f32 from the oldest on.  A thread has DL_V neighbouring channels and `tile` rows, one after the other, with the window in registers and the next
+// DL_AHEAD rows asked for; the one that has a sequence's first row leaves the new carried rows, which are rows of the call or of the old slot (so nothing is
+// read after somebody else wrote it).  Memory bound: what a tile reads twice are its first K - 1 rows, from L2.
+constexpr int DL_AHEAD = 4, DL_V = 4;
+template <int ESZ> struct DlRaw { typedef uint2 T; };
+template <> struct DlRaw<4> { typedef uint4 T; };
+__device__ __forceinline__ void dl_none(uint2& x) { x = make_uint2(0, 0); }
+__device__ __forceinline__ void dl_none(uint4& x) { x = make_uint4(0, 0, 0, 0); }
 struct DlConv {
     const u8* x;
     u8* y;
@@ -42,95 +47,154 @@ __device__ __forceinline__ int dl_seq_of(const DlBatch& d, int r, int lane) {
 template <int TYPE, int K>
 __global__ void __launch_bounds__(128)
 sz_delta_conv_kernel(const DlBatch d, const DlConv a) {
-    constexpr int ESZ = DlIo<TYPE>::ESZ, V = 16 / ESZ;
+    constexpr int ESZ = DlIo<TYPE>::ESZ, V = DL_V;
+    using Raw = typename DlRaw<ESZ>::T;
     const int lane = threadIdx.x & 31, c0 = (blockIdx.x * 128 + threadIdx.x) * V;
     const bool mine = c0 < a.ch;                        // (a warp stays together: its lanes look sequences up together)
-    float w[K][V], bias[V];
+    u64 w[K][V / 2], bias[V / 2];
 #pragma unroll
-    for (int i = 0; i < V; i++) bias[i] = 0.f;
+    for (int i = 0; i < V / 2; i++) bias[i] = 0;
     if (mine) {
         float wt[K * V];
         const float4* src = (const float4*)(a.w + (size_t)c0 * K);
 #pragma unroll
         for (int i = 0; i < K * V / 4; i++) *(float4*)(wt + 4 * i) = __ldg(src + i);
 #pragma unroll
-        for (int i = 0; i < V; i++)
+        for (int i = 0; i < V / 2; i++)
 #pragma unroll
-            for (int t = 0; t < K; t++) w[t][i] = wt[i * K + t];
+            for (int t = 0; t < K; t++) w[t][i] = dl_pack2(wt[2 * i * K + t], wt[(2 * i + 1) * K + t]);
         if (a.bias)
 #pragma unroll
-            for (int i = 0; i < V; i += 4) *(float4*)(bias + i) = __ldg((const float4*)(a.bias + c0 + i));
+            for (int i = 0; i < V / 2; i++) { const float2 x = __ldg((const float2*)(a.bias + c0 + 2 * i)); bias[i] = dl_pack2(x.x, x.y); }
     }
     sz_pdl_wait();
     sz_pdl_trigger();
     const int first = blockIdx.y * a.tile, end = min(first + a.tile, d.rows);
-    auto row = [&](int r, float* f) { dl_load<TYPE, V>(a.x + (size_t)r * a.x_stride + (size_t)c0 * ESZ, f); };
-    auto carried = [&](int slot, int i, float* f) {     // row i of a slot
-        const u8* p = a.conv + (size_t)slot * a.conv_stride;
-        if (a.conv_type == SZ_TYPE_F32) dl_load<SZ_TYPE_F32, V>(p + ((size_t)i * a.ch + c0) * 4, f);
-        else if (a.conv_type == SZ_TYPE_F16) dl_load<SZ_TYPE_F16, V>(p + ((size_t)i * a.ch + c0) * 2, f);
-        else dl_load<SZ_TYPE_BF16, V>(p + ((size_t)i * a.ch + c0) * 2, f);
+    const u8* const xc = a.x + (size_t)c0 * ESZ;
+    auto ask = [&](int r) {                             // row r (x is not written meanwhile: y lies elsewhere)
+        Raw q;
+        dl_none(q);
+        if (mine && r < end) q = __ldcg((const Raw*)(xc + (size_t)r * a.x_stride));
+        return q;
     };
-    int b = d.n_seq == 1 ? 0 : dl_seq_of(d, first, lane);
-    if (b < 0) b = 0;
+    auto pairs = [&](const Raw& q, u64* f) {
+        float x[V];
+        dl_unpack<TYPE, V>((const u32*)&q, x);
+#pragma unroll
+        for (int i = 0; i < V / 2; i++) f[i] = dl_pack2(x[2 * i], x[2 * i + 1]);
+    };
+    auto carried = [&](int slot, int i, u64* f) {       // row i of a slot
+        const u8* p = a.conv + (size_t)slot * a.conv_stride;
+        float x[V];
+        if (a.conv_type == SZ_TYPE_F32) dl_load<SZ_TYPE_F32, V>(p + ((size_t)i * a.ch + c0) * 4, x);
+        else if (a.conv_type == SZ_TYPE_F16) dl_load<SZ_TYPE_F16, V>(p + ((size_t)i * a.ch + c0) * 2, x);
+        else dl_load<SZ_TYPE_BF16, V>(p + ((size_t)i * a.ch + c0) * 2, x);
+#pragma unroll
+        for (int e = 0; e < V / 2; e++) f[e] = dl_pack2(x[2 * e], x[2 * e + 1]);
+    };
+    Raw ahead[DL_AHEAD];
+#pragma unroll
+    for (int j = 0; j < DL_AHEAD; j++) ahead[j] = ask(first + j);
+    u64 win[K][V / 2];                                  // the rows before the next one, and it
+    int b = -1, from = first, upto = first;             // the current sequence's rows here: from .. upto
+    int next = first;                                   // where the one behind it begins
+    auto give = [&](int r, const u64 (*x)[V / 2]) {     // row r, of K rows
+        float y[V];
+#pragma unroll
+        for (int i = 0; i < V / 2; i++) {
+            u64 acc = bias[i];
+#pragma unroll
+            for (int t = 0; t < K; t++) dl_fma2(acc, w[t][i], x[t][i]);
+            y[2 * i] = dl_lo(acc) * dl_sigmoid<TYPE>(dl_lo(acc));
+            y[2 * i + 1] = dl_hi(acc) * dl_sigmoid<TYPE>(dl_hi(acc));
+        }
+        dl_store<TYPE, V>(a.y + (size_t)r * a.y_stride + (size_t)c0 * ESZ, y);
+    };
     int r = first;
-    for (; b < d.n_seq && r < end; b++) {
-        const int begin = d.row_start[b];
-        if (begin >= end) break;
-        if (d.row_start[b + 1] <= r && d.row_start[b + 1] >= begin) continue;
-        const DlSeq s = dl_seq(d, b, lane, blockIdx.x == 0);
-        if (!s.on) continue;
-        r = max(r, s.r0);
-        const int upto = min(s.r0 + s.n, end);
-        if (!mine) { r = max(r, upto); continue; }
-        // the rows before r: of the sequence, of its slot, or zeros
-        float win[K][V];
+#pragma unroll 1
+    while (r < end) {
+        if (r >= from && r < next && r + DL_AHEAD <= min(upto, end)) {      // DL_AHEAD rows of the current sequence
+            if (mine) {
+                u64 x[K - 1 + DL_AHEAD][V / 2];
 #pragma unroll
-        for (int t = 0; t < K - 1; t++) {
-            const int p = r - (K - 1) + t - s.r0;       // row p of the sequence
-            if (p >= 0) row(s.r0 + p, win[t]);
-            else if (s.from >= 0) carried(s.from, K - 1 + p, win[t]);
-            else
+                for (int t = 0; t < K - 1; t++)
 #pragma unroll
-                for (int i = 0; i < V; i++) win[t][i] = 0.f;
+                    for (int i = 0; i < V / 2; i++) x[t][i] = win[t][i];
+#pragma unroll
+                for (int j = 0; j < DL_AHEAD; j++) pairs(ahead[j], x[K - 1 + j]);
+#pragma unroll
+                for (int j = 0; j < DL_AHEAD; j++) ahead[j] = ask(r + DL_AHEAD + j);
+#pragma unroll
+                for (int j = 0; j < DL_AHEAD; j++) give(r + j, x + j);
+#pragma unroll
+                for (int t = 0; t < K - 1; t++)
+#pragma unroll
+                    for (int i = 0; i < V / 2; i++) win[t][i] = x[t + DL_AHEAD][i];
+            }
+            r += DL_AHEAD;
+            continue;
         }
-        if (r == s.r0) {                                // what is carried on: rows n - (K - 1) .. n of [the slot's rows; the sequence's]
-            u8* p = a.conv + (size_t)s.to * a.conv_stride;
+        const Raw now = ahead[0];
 #pragma unroll
-            for (int t = 0; t < K - 1; t++) {
-                const int at = s.n - (K - 1) + t;       // (below 0: row n + t of the window)
-                float nw[V];
-                if (at >= 0) row(s.r0 + at, nw);
-                else
+        for (int j = 0; j + 1 < DL_AHEAD; j++) ahead[j] = ahead[j + 1];
+        ahead[DL_AHEAD - 1] = ask(r + DL_AHEAD);
+        if (r >= next) {                            // another sequence
+            b = b < 0 && d.n_seq > 1 ? dl_seq_of(d, r, lane) : max(b, 0);
+            while (b >= 0 && b < d.n_seq && d.row_start[b + 1] <= r && d.row_start[b + 1] >= d.row_start[b]) b++;
+            from = upto = 0;
+            if (b >= d.n_seq) next = end;           // (rows behind the last sequence)
+            else if (b < 0) { b = -1; next = max(r + 1, d.row_start[0]); }
+            else if (d.row_start[b] > r) next = d.row_start[b];      // (rows before the first sequence)
+            else {
+                const int nb = d.row_start[b + 1];
+                next = nb > r ? nb : end;           // (a descending table: reported, and nobody's rows)
+                const DlSeq s = dl_seq(d, b, lane, blockIdx.x == 0);
+                if (s.on) {
+                    from = s.r0;
+                    upto = s.r0 + s.n;
+                    if (mine && (r < upto || r == s.r0)) {
+                        // the rows before r: of the sequence, of its slot, or zeros
 #pragma unroll
-                    for (int i = 0; i < V; i++) {
-                        nw[i] = win[0][i];
+                        for (int t = 0; t < K - 1; t++) {
+                            const int p = r - (K - 1) + t - s.r0;    // row p of the sequence
+                            if (p >= 0) { const Raw q = __ldcg((const Raw*)(xc + (size_t)(s.r0 + p) * a.x_stride)); pairs(q, win[t]); }
+                            else if (s.from >= 0) carried(s.from, K - 1 + p, win[t]);
+                            else
 #pragma unroll
-                        for (int u = 1; u < K - 1; u++) nw[i] = u == s.n + t ? win[u][i] : nw[i];
+                                for (int i = 0; i < V / 2; i++) win[t][i] = 0;
+                        }
+                        if (r == s.r0) {            // what is carried on: rows n - (K - 1) .. n of [the slot's rows; the sequence's]
+                            u8* p = a.conv + (size_t)s.to * a.conv_stride;
+#pragma unroll
+                            for (int t = 0; t < K - 1; t++) {
+                                const int at = s.n - (K - 1) + t;       // (below 0: row n + t of the slot)
+                                u64 nw[V / 2];
+                                if (at >= 0) { const Raw q = __ldcg((const Raw*)(xc + (size_t)(s.r0 + at) * a.x_stride)); pairs(q, nw); }
+                                else if (s.from >= 0) carried(s.from, s.n + t, nw);      // (rows below t alone are overwritten by now)
+                                else
+#pragma unroll
+                                    for (int i = 0; i < V / 2; i++) nw[i] = 0;
+                                float f[V];
+#pragma unroll
+                                for (int i = 0; i < V / 2; i++) { f[2 * i] = dl_lo(nw[i]); f[2 * i + 1] = dl_hi(nw[i]); }
+                                if (a.conv_type == SZ_TYPE_F32) dl_store<SZ_TYPE_F32, V>(p + ((size_t)t * a.ch + c0) * 4, f);
+                                else if (a.conv_type == SZ_TYPE_F16) dl_store<SZ_TYPE_F16, V>(p + ((size_t)t * a.ch + c0) * 2, f);
+                                else dl_store<SZ_TYPE_BF16, V>(p + ((size_t)t * a.ch + c0) * 2, f);
+                            }
+                        }
                     }
-                if (a.conv_type == SZ_TYPE_F32) dl_store<SZ_TYPE_F32, V>(p + ((size_t)t * a.ch + c0) * 4, nw);
-                else if (a.conv_type == SZ_TYPE_F16) dl_store<SZ_TYPE_F16, V>(p + ((size_t)t * a.ch + c0) * 2, nw);
-                else dl_store<SZ_TYPE_BF16, V>(p + ((size_t)t * a.ch + c0) * 2, nw);
+                }
             }
         }
-#pragma unroll 4
-        for (; r < upto; r++) {
-            row(r, win[K - 1]);
-            float y[V];
-#pragma unroll
-            for (int i = 0; i < V; i++) {
-                float acc = bias[i];
-#pragma unroll
-                for (int t = 0; t < K; t++) acc = fmaf(w[t][i], win[t][i], acc);
-                y[i] = sz_silu(acc);
-            }
-            dl_store<TYPE, V>(a.y + (size_t)r * a.y_stride + (size_t)c0 * ESZ, y);
+        if (r >= from && r < upto && mine) {
+            pairs(now, win[K - 1]);
+            give(r, win);
 #pragma unroll
             for (int t = 0; t < K - 1; t++)
 #pragma unroll
-                for (int i = 0; i < V; i++) win[t][i] = win[t + 1][i];
+                for (int i = 0; i < V / 2; i++) win[t][i] = win[t + 1][i];
         }
-        r = max(r, upto);
+        r++;
     }
     if (blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x < 32) {       // (tables that no row leads to)
         bool bad = false;
@@ -148,7 +212,7 @@ sz_delta_conv_kernel(const DlBatch d, const DlConv a) {
 // sequences the states' bytes bound it (64 sequences of 32 heads of 128: 268 MB), with few the chain load - exchange - store.
 constexpr int DL_SET = 8;
 template <int D> struct DlSet {
-    float k[DL_SET][D], q[DL_SET][D], o[DL_SET][D];
+    float k[DL_SET][D], q[DL_SET][D], v[DL_SET][D], o[DL_SET][D];
     float g[DL_SET], beta[DL_SET], kq[DL_SET];
 };
 
@@ -164,12 +228,37 @@ sz_delta_rows_kernel(const DlBatch d, const DlRule a) {
     if (!s.on || (a.least && d.row_start[b + 1] - d.row_start[b] >= a.least)) return;
     const int kx = a.grouped ? h / (a.vh / a.kh) : h % a.kh;
     const int j0 = 16 * warp + 4 * (lane & 3), i0 = M * (lane >> 2);              // the lane's value and key dimensions
+    // a set's rows, R a warp: asked for (the first ones before the state), then normed into shared memory
+    constexpr int R = DL_SET / NW, W = E * ESZ / 4;
+    u32 kw[R][W], qw[R][W], vw[R][W], zw[R][W];
+    float al[R], be[R];
+    const float ah = a.a[h], dth = a.dt[h];
+    auto raw = [&](const u8* p, u32* w) {
+        if constexpr (W == 4) *(uint4*)w = __ldcg((const uint4*)p);
+        else if constexpr (W == 2) *(uint2*)w = __ldcg((const uint2*)p);
+        else w[0] = __ldcg((const u32*)p);
+    };
+    auto ask = [&](int r0) {
+#pragma unroll
+        for (int i = 0; i < R; i++) {
+            const int j = warp + i * NW;
+            if (r0 + j >= s.n) continue;
+            const size_t r = s.r0 + r0 + j;
+            raw(a.k + r * a.k_stride + (size_t)(kx * D + lane * E) * ESZ, kw[i]);
+            if (OUT) raw(a.q + r * a.q_stride + (size_t)(kx * D + lane * E) * ESZ, qw[i]);
+            raw(a.v + r * a.v_stride + (size_t)(h * D + lane * E) * ESZ, vw[i]);
+            if (OUT && a.norm) raw(a.z + r * a.z_stride + (size_t)(h * D + lane * E) * ESZ, zw[i]);
+            al[i] = dl_load1<TYPE>(a.alpha + r * a.alpha_stride + (size_t)h * ESZ);
+            be[i] = dl_load1<TYPE>(a.beta + r * a.beta_stride + (size_t)h * ESZ);
+        }
+    };
+    ask(0);
     u64 S[M / 2][4];
     if (s.from >= 0) {
         const float* p = (const float*)(a.state + (size_t)s.from * a.state_stride) + ((size_t)h * D + i0) * D + j0;
 #pragma unroll
         for (int m = 0; m < M / 2; m++) {
-            const float4 e = *(const float4*)(p + (size_t)(2 * m) * D), o = *(const float4*)(p + (size_t)(2 * m + 1) * D);
+            const float4 e = __ldcg((const float4*)(p + (size_t)(2 * m) * D)), o = __ldcg((const float4*)(p + (size_t)(2 * m + 1) * D));
             S[m][0] = dl_pack2(e.x, o.x); S[m][1] = dl_pack2(e.y, o.y); S[m][2] = dl_pack2(e.z, o.z); S[m][3] = dl_pack2(e.w, o.w);
         }
     } else {
@@ -178,19 +267,21 @@ sz_delta_rows_kernel(const DlBatch d, const DlRule a) {
 #pragma unroll
             for (int c = 0; c < 4; c++) S[m][c] = 0;
     }
-    const float ah = a.a[h], dth = a.dt[h];
     for (int r0 = 0; r0 < s.n; r0 += DL_SET) {
         const int nr = min(DL_SET, s.n - r0);
-        for (int j = warp; j < nr; j += NW) {
-            const size_t r = s.r0 + r0 + j;
-            float kv[E], qv[E], kk = 0.f, qq = 0.f, kq = 0.f;
-            dl_load<TYPE, E>(a.k + r * a.k_stride + (size_t)(kx * D + lane * E) * ESZ, kv);
-            if (OUT) dl_load<TYPE, E>(a.q + r * a.q_stride + (size_t)(kx * D + lane * E) * ESZ, qv);
-            const float al = dl_load1<TYPE>(a.alpha + r * a.alpha_stride + (size_t)h * ESZ), be = dl_load1<TYPE>(a.beta + r * a.beta_stride + (size_t)h * ESZ);
+#pragma unroll
+        for (int i = 0; i < R; i++) {
+            const int j = warp + i * NW;
+            if (j >= nr) continue;
+            float kv[E], qv[E], vv[E], kk = 0.f, qq = 0.f, kq = 0.f;
+            dl_unpack<TYPE, E>(kw[i], kv);
+            if (OUT) dl_unpack<TYPE, E>(qw[i], qv);
+            dl_unpack<TYPE, E>(vw[i], vv);
 #pragma unroll
             for (int e = 0; e < E; e++) {
                 kk = fmaf(kv[e], kv[e], kk);
                 if (OUT) { qq = fmaf(qv[e], qv[e], qq); kq = fmaf(kv[e], qv[e], kq); }
+                sh.v[j][lane * E + e] = vv[e];
             }
             kk = sz_warp_sum(kk);
             const float nk = (float)sz_rsqrt64((double)kk + 1e-6);
@@ -204,13 +295,12 @@ sz_delta_rows_kernel(const DlBatch d, const DlRule a) {
                 for (int e = 0; e < E; e++) sh.q[j][lane * E + e] = qv[e] * nq;
                 if (lane == 0) sh.kq[j] = kq * nk * nq;
             }
-            if (lane == 0) { sh.g[j] = expf(dl_log_decay(al, ah, dth)); sh.beta[j] = sz_sigmoid(be); }
+            if (lane == 0) { sh.g[j] = expf(dl_log_decay(al[i], ah, dth)); sh.beta[j] = sz_sigmoid(be[i]); }
         }
         __syncthreads();
         for (int j = 0; j < nr; j++) {
-            const size_t r = s.r0 + r0 + j;
-            float v[4];
-            dl_load<TYPE, 4>(a.v + r * a.v_stride + (size_t)(h * D + j0) * ESZ, v);
+            const float4 v4 = *(const float4*)(sh.v[j] + j0);
+            const float v[4] = {v4.x, v4.y, v4.z, v4.w};
             const float g = sh.g[j], beta = sh.beta[j];
             const u64 g2 = dl_pack2(g, g);
             u64 x[4] = {0, 0, 0, 0}, y[4] = {0, 0, 0, 0}, kr[M / 2];
@@ -252,8 +342,10 @@ sz_delta_rows_kernel(const DlBatch d, const DlRule a) {
         }
         __syncthreads();
         if (OUT)
-            for (int j = warp; j < nr; j += NW) {
-                const size_t r = s.r0 + r0 + j;
+#pragma unroll
+            for (int i = 0; i < R; i++) {
+                const int j = warp + i * NW;
+                if (j >= nr) continue;
                 float o[E];
 #pragma unroll
                 for (int e = 0; e < E; e++) o[e] = sh.o[j][lane * E + e];
@@ -262,12 +354,13 @@ sz_delta_rows_kernel(const DlBatch d, const DlRule a) {
 #pragma unroll
                     for (int e = 0; e < E; e++) ss = fmaf(o[e], o[e], ss);
                     const float rr = (float)sz_rsqrt64((double)sz_warp_sum(ss) * (1.0 / D) + (double)a.eps);
-                    dl_load<TYPE, E>(a.z + r * a.z_stride + (size_t)(h * D + lane * E) * ESZ, z);
+                    dl_unpack<TYPE, E>(zw[i], z);
 #pragma unroll
-                    for (int e = 0; e < E; e++) o[e] = o[e] * rr * a.norm[lane * E + e] * sz_sigmoid(z[e]);
+                    for (int e = 0; e < E; e++) o[e] = o[e] * rr * a.norm[lane * E + e] * dl_sigmoid<TYPE>(z[e]);
                 }
-                dl_store<TYPE, E>(a.out + r * a.out_stride + (size_t)(h * D + lane * E) * ESZ, o);
+                dl_store<TYPE, E>(a.out + (size_t)(s.r0 + r0 + j) * a.out_stride + (size_t)(h * D + lane * E) * ESZ, o);
             }
+        if (r0 + DL_SET < s.n) ask(r0 + DL_SET);
     }
     float* p = (float*)(a.state + (size_t)s.to * a.state_stride) + ((size_t)h * D + i0) * D + j0;
 #pragma unroll
@@ -377,7 +470,7 @@ extern "C" int sz_delta_conv(const sz_delta_pool* pool, const sz_delta_batch* ba
     a.w = (const float*)w; a.bias = (const float*)bias;
     a.conv = (u8*)pool->conv; a.conv_stride = pool->conv_stride; a.conv_type = pool->conv_type; a.ch = ch;
     // rows a thread has: as many as leave every multiprocessor 16 warps, up to 32 (a tile's first rows are read twice)
-    const int vecs = (ch * esz / 16 + 127) / 128;
+    const int vecs = (ch / DL_V + 127) / 128;
     a.tile = 1;
     while (a.tile < 32 && (int64_t)vecs * ((batch->rows + 2 * a.tile - 1) / (2 * a.tile)) >= 4 * DL_SM) a.tile *= 2;
     const dim3 grid(vecs, (batch->rows + a.tile - 1) / a.tile);

@@ -82,6 +82,18 @@ __device__ __forceinline__ float dl_load1(const u8* p) {
     else return __uint_as_float((u32) * (const u16*)p << 16);
 }
 
+// sigmoid: where 16 bits are kept of what it is multiplied with, by the fast exponential and quotient (2^-21 relative); for f32 with the rounding of the exponent put
+// back and a Newton step on the fast reciprocal (2^-22), a third of the time of sz_sigmoid
+template <int TYPE> __device__ __forceinline__ float dl_sigmoid(float x) {
+    if (TYPE != SZ_TYPE_F32) return __fdividef(1.f, 1.f + __expf(-x));
+    constexpr float L = 1.4426950408889634f, L_LOW = 1.925963033500e-8f;      // log2(e), and what f32 leaves of it
+    const float y = -x > 85.f ? 85.f : -x, e = y * L, rest = fmaf(y, L_LOW, fmaf(y, L, -e));
+    float w, r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(w) : "f"(e));
+    const float den = 1.f + fmaf(w, rest * 0.6931471805599453f, w);
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(den));
+    return r * fmaf(-den, r, 2.f);
+}
 // The logarithm of a row's decay, a softplus(alpha + dt), and its beta.  A decay above 1 (a positive `a`) counts as 1.
 __device__ __forceinline__ float dl_log_decay(float alpha, float a, float dt) {
     const float x = alpha + dt, g = a * (x > 20.f ? x : log1pf(expf(x)));

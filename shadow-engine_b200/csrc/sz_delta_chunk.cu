@@ -87,18 +87,6 @@ __device__ __forceinline__ void dl_scale4(float* x, float f) {
     const u64 f2 = dl_pack2(f, f), a = dl_mul2(dl_pack2(x[0], x[1]), f2), b = dl_mul2(dl_pack2(x[2], x[3]), f2);
     x[0] = dl_lo(a); x[1] = dl_hi(a); x[2] = dl_lo(b); x[3] = dl_hi(b);
 }
-// sigmoid: where 16 bits are kept of what it is multiplied with, by the fast exponential and quotient (2^-21 relative); for f32 with the rounding of the exponent put
-// back and a Newton step on the fast reciprocal (2^-22), a third of the time of sz_sigmoid
-template <int TYPE> __device__ __forceinline__ float dl_sigmoid(float x) {
-    if (TYPE != SZ_TYPE_F32) return __fdividef(1.f, 1.f + __expf(-x));
-    constexpr float L = 1.4426950408889634f, L_LOW = 1.925963033500e-8f;      // log2(e), and what f32 leaves of it
-    const float y = -x > 85.f ? 85.f : -x, e = y * L, rest = fmaf(y, L_LOW, fmaf(y, L, -e));
-    float w, r;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(w) : "f"(e));
-    const float den = 1.f + fmaf(w, rest * 0.6931471805599453f, w);
-    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(den));
-    return r * fmaf(-den, r, 2.f);
-}
 // byte of the 16-byte piece c of row r of a tile [rows][D] of f16: pieces exchanged so that ldmatrix meets no bank twice
 template <int D> __device__ __forceinline__ u32 dl_at(int r, int c) { return (u32)(r * D * 2 + ((c ^ (r & 7)) << 4)); }
 // the first of the tiles of 8 rows n of a lower triangle (its 16-column tiles are side by side)

@@ -13,7 +13,7 @@
 
 namespace {
 
-constexpr int LP_NTH = 512, LP_G = 4, LP_MAX_VOCAB = 1 << 18, LP_ID = 18, LP_TOP = 64, LP_LIST = 2048, LP_PLACES = 3 * 148;
+constexpr int LP_NTH = 512, LP_G = 4, LP_MAX_VOCAB = 1 << 18, LP_ID = 18, LP_TOP = 64, LP_LIST = 2048, LP_PLACES = 2 * 148;
 constexpr int LP_NW = LP_NTH / 32;
 
 struct LpArgs {
@@ -47,9 +47,9 @@ __device__ __forceinline__ float lp_at(const u32* w, int i) {       // element i
 }
 template <int TYPE>
 __device__ __forceinline__ float lp_one(const u8* p) {
-    if constexpr (TYPE == SZ_TYPE_F32) return __ldg((const float*)p);
-    else if constexpr (TYPE == SZ_TYPE_F16) return __half2float(__ushort_as_half(__ldg((const u16*)p)));
-    else return __uint_as_float((u32)__ldg((const u16*)p) << 16);
+    if constexpr (TYPE == SZ_TYPE_F32) return __ldcg((const float*)p);
+    else if constexpr (TYPE == SZ_TYPE_F16) return __half2float(__ushort_as_half(__ldcg((const u16*)p)));
+    else return __uint_as_float((u32)__ldcg((const u16*)p) << 16);
 }
 // NaN counts as -inf
 __device__ __forceinline__ float lp_clean(float v) { return fmaxf(v, -INFINITY); }
@@ -67,6 +67,11 @@ __device__ __forceinline__ u32 lp_ld32(const void* p, int rank) { u32 v; asm vol
 __device__ __forceinline__ float lp_exp2(float x) { float y; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x)); return y; }
 __device__ __forceinline__ void lp_sync(int C) { if (C > 1) sz_cluster_sync(); else __syncthreads(); }
 
+// f32x2 arithmetic
+__device__ __forceinline__ u64 lp_pack(float a, float b) { u64 d; asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "f"(a), "f"(b)); return d; }
+__device__ __forceinline__ u64 lp_add2(u64 a, u64 b) { u64 d; asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b)); return d; }
+__device__ __forceinline__ u64 lp_mul2(u64 a, u64 b) { u64 d; asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b)); return d; }
+__device__ __forceinline__ void lp_fma2(u64& a, u64 f, u64 x) { asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(a) : "l"(f), "l"(x)); }
 // (largest, sum of the others' weights beside it, sum of weights times exponents) of two parts; exponents to the base 2
 struct LpSum { float m, s, x; };
 __device__ __forceinline__ LpSum lp_join(const LpSum a, const LpSum b, float c) {
@@ -91,10 +96,10 @@ sz_logprob_kernel(const LpArgs a) {
     sz_pdl_trigger();
     const u8* const base = a.logits + (size_t)row * a.stride;
     const int e0 = min(rank * a.per, a.vocab), e1 = min(e0 + a.per, a.vocab);      // the block's part
-    // in 16-byte vectors of memory: vector 0 holds element e0, `shift` elements in
-    const int shift = (int)(((size_t)base + (size_t)e0 * V::ESZ) & 15) / V::ESZ, nvec = e1 > e0 ? (shift + e1 - e0 + N - 1) / N : 0;
-    const int id0 = e0 - shift;                          // id of vector 0's first element
-    const u8* const vbase = base + (long long)id0 * V::ESZ;
+    // whole 16-byte vectors of memory from element `id0` on, and up to N - 1 elements before and behind them
+    const int lead = min(e1 - e0, (int)((16 - (((size_t)base + (size_t)e0 * V::ESZ) & 15)) & 15) / V::ESZ);
+    const int id0 = e0 + lead, nvec = (e1 - id0) / N;
+    const u8* const vbase = base + (size_t)id0 * V::ESZ;
     int token = a.tokens ? a.tokens[row] : -1;
     if ((u32)token >= (u32)a.vocab) token = -1;
     const float tv = token >= 0 ? lp_clean(lp_one<TYPE>(base + (size_t)token * V::ESZ)) : INFINITY;
@@ -102,42 +107,43 @@ sz_logprob_kernel(const LpArgs a) {
     const float T = a.temperature ? a.temperature[row] : 1.f, inv_t = 1.f / T;
     const bool alone = !(T > 0.f) || !(inv_t <= 3.4e38f);            // the best token has it all
     const float c = alone ? 0.f : inv_t * 1.4426950408889634f;
+    constexpr u32 NONE = TYPE == SZ_TYPE_F32 ? 0xff800000u : TYPE == SZ_TYPE_F16 ? 0xfc00fc00u : 0xff80ff80u;      // -inf
     auto load = [&](int v, u32* w) {
-        if (v >= nvec) {
+        const uint4 q = __ldcg((const uint4*)(vbase + (size_t)v * 16));
+        w[0] = q.x; w[1] = q.y; w[2] = q.z; w[3] = q.w;
+    };
+    auto edge = [&](int v, u32* w) {                     // vector -1: the elements before the first, nvec: those behind the last
 #pragma unroll
-            for (int i = 0; i < 4; i++) w[i] = TYPE == SZ_TYPE_F32 ? 0xff800000u : TYPE == SZ_TYPE_F16 ? 0xfc00fc00u : 0xff80ff80u;
-        } else if ((v == 0 && shift) || (v == nvec - 1 && id0 + nvec * N > e1)) {      // element by element, those of the part
+        for (int i = 0; i < 4; i++) {
+            constexpr int P = 4 / V::ESZ;                // elements a word
+            w[i] = 0;
 #pragma unroll
-            for (int i = 0; i < 4; i++) {
-                if constexpr (TYPE == SZ_TYPE_F32) {
-                    const int id = id0 + v * N + i;
-                    w[i] = id >= e0 && id < e1 ? __ldg((const u32*)(vbase + (size_t)(v * N + i) * 4)) : 0xff800000u;
-                } else {
-                    u32 h[2];
-#pragma unroll
-                    for (int j = 0; j < 2; j++) {
-                        const int id = id0 + v * N + 2 * i + j;
-                        h[j] = id >= e0 && id < e1 ? __ldg((const u16*)(vbase + (size_t)(v * N + 2 * i + j) * 2)) : TYPE == SZ_TYPE_F16 ? 0xfc00u : 0xff80u;
-                    }
-                    w[i] = h[0] | h[1] << 16;
-                }
+            for (int k = 0; k < P; k++) {
+                const int id = id0 + v * N + i * P + k;
+                u32 e = NONE >> (32 - 8 * V::ESZ);
+                if (id >= e0 && id < e1) { if constexpr (TYPE == SZ_TYPE_F32) e = __ldcg((const u32*)(base + (size_t)id * 4)); else e = __ldcg((const u16*)(base + (size_t)id * 2)); }
+                w[i] |= e << (8 * V::ESZ * k) % 32;
             }
-        } else {
-            const uint4 q = __ldg((const uint4*)(vbase + (size_t)v * 16));
-            w[0] = q.x; w[1] = q.y; w[2] = q.z; w[3] = q.w;
         }
     };
     float m = -INFINITY, s = 0.f, x = 0.f, tmax = -INFINITY;         // of the warp (m), of the thread (the others)
     u32 cnt = 0;
-#pragma unroll 1
-    for (int g = 0; g < a.groups; g++) {
-        u32 w[4 * LP_G];
-        const int v0 = g * LP_G * LP_NTH + tid;
-#pragma unroll
-        for (int j = 0; j < LP_G; j++) load(v0 + j * LP_NTH, w + 4 * j);
+    const int whole = nvec / (LP_G * LP_NTH), last = a.groups - 1;       // (the last group: what lies beside the vectors)
+    // one group: vectors v0, v0 + LP_NTH, .. (elements that are nobody's are -inf)
+    auto take = [&](int g, int v0, const u32* w) {
         float gm = -INFINITY;
+        if constexpr (TYPE == SZ_TYPE_F32) {
 #pragma unroll
-        for (int i = 0; i < GE; i++) gm = fmaxf(gm, lp_at<TYPE>(w, i));
+            for (int i = 0; i < GE; i++) gm = fmaxf(gm, lp_at<TYPE>(w, i));
+        } else {                                         // two at a time
+            u32 p = NONE;
+#pragma unroll
+            for (int i = 0; i < 4 * LP_G; i++) {
+                if constexpr (TYPE == SZ_TYPE_F16) { const __half2 h = __hmax2(*(const __half2*)&p, *(const __half2*)(w + i)); p = *(const u32*)&h; }
+                else { const __nv_bfloat162 h = __hmax2(*(const __nv_bfloat162*)&p, *(const __nv_bfloat162*)(w + i)); p = *(const u32*)&h; }
+            }
+            gm = fmaxf(lp_at<TYPE>(&p, 0), lp_at<TYPE>(&p, 1));
+        }
         if (a.top) gmax[g * LP_NTH + tid] = gm;
         tmax = fmaxf(tmax, gm);
         // larger than the token's logit, or equal with a lower id
@@ -145,8 +151,9 @@ sz_logprob_kernel(const LpArgs a) {
 #pragma unroll
             for (int i = 0; i < GE; i++) {
                 const float v = lp_clean(lp_at<TYPE>(w, i));
-                const int id = id0 + (v0 + (i / N) * LP_NTH) * N + i % N;
-                cnt += (v > tv || (v == tv && id < before && id >= e0)) ? 1u : 0u;
+                const int at = v0 + (i / N) * LP_NTH, id = id0 + at * N + i % N;
+                const bool there = g == last ? tid < 2 && i < N : at < nvec;
+                cnt += (v > tv || (there && v == tv && id < before && id >= e0)) ? 1u : 0u;
             }
         }
         const float wm = lp_down(__reduce_max_sync(0xffffffffu, lp_up(gm)));
@@ -171,16 +178,44 @@ sz_logprob_kernel(const LpArgs a) {
                 x = fmaf(p, e, x);
             }
         } else {
-            float gs = 0.f, gx = 0.f;
+            const u64 m2 = lp_pack(-m, -m), c2 = lp_pack(c, c);
+            u64 gs = 0, gx = 0;
 #pragma unroll
-            for (int i = 0; i < GE; i++) {
-                const float e = fmaxf((lp_at<TYPE>(w, i) - m) * c, -200.f), p = lp_exp2(e);
-                gs += p;
-                gx = fmaf(p, e, gx);
+            for (int i = 0; i < GE; i += 2) {
+                const u64 e2 = lp_mul2(lp_add2(lp_pack(lp_at<TYPE>(w, i), lp_at<TYPE>(w, i + 1)), m2), c2);
+                const float e = fmaxf(__uint_as_float((u32)e2), -200.f), f = fmaxf(__uint_as_float((u32)(e2 >> 32)), -200.f);
+                const u64 p = lp_pack(lp_exp2(e), lp_exp2(f));
+                gs = lp_add2(gs, p);
+                lp_fma2(gx, p, lp_pack(e, f));
             }
-            s += gs;
-            x += gx;
+            s += __uint_as_float((u32)gs) + __uint_as_float((u32)(gs >> 32));
+            x += __uint_as_float((u32)gx) + __uint_as_float((u32)(gx >> 32));
         }
+    };
+#pragma unroll 1
+    for (int g = 0; g < last; g++) {
+        u32 w[4 * LP_G];
+        const int v0 = g * LP_G * LP_NTH + tid;
+        if (g < whole) {
+#pragma unroll
+            for (int j = 0; j < LP_G; j++) load(v0 + j * LP_NTH, w + 4 * j);
+        } else {
+#pragma unroll
+            for (int j = 0; j < LP_G; j++) {
+                w[4 * j] = w[4 * j + 1] = w[4 * j + 2] = w[4 * j + 3] = NONE;
+                if (v0 + j * LP_NTH < nvec) load(v0 + j * LP_NTH, w + 4 * j);
+            }
+        }
+        take(g, v0, w);
+    }
+    if (a.top) gmax[last * LP_NTH + tid] = -INFINITY;
+    if (warp == 0) {                                     // threads 0 and 1: before and behind
+        u32 w[4 * LP_G];
+#pragma unroll
+        for (int i = 0; i < 4 * LP_G; i++) w[i] = NONE;
+        const int v = tid == 0 ? -1 : tid == 1 ? nvec : 0x3fffff;        // (a vector that no element is in)
+        if (tid < 2) edge(v, w);
+        take(last, v, w);
     }
     // ---- the block's part, then the row's
 #pragma unroll
@@ -219,10 +254,10 @@ sz_logprob_kernel(const LpArgs a) {
                 const float gm = gmax[g * LP_NTH + tid];
                 if (!(equal ? gm >= from : gm > from)) continue;
                 for (int j = 0; j < LP_G; j++) {
-                    const int v = (g * LP_G + j) * LP_NTH + tid;
-                    if (v >= nvec) break;
+                    const int v = g == last ? (tid == 0 ? -1 : nvec) : (g * LP_G + j) * LP_NTH + tid;
+                    if (g == last ? j > 0 || tid > 1 : v >= nvec) break;
                     u32 w[4];
-                    load(v, w);
+                    if (g == last) edge(v, w); else load(v, w);
 #pragma unroll
                     for (int i = 0; i < N; i++) {
                         const int id = id0 + v * N + i;
@@ -258,9 +293,11 @@ sz_logprob_kernel(const LpArgs a) {
             __syncthreads();
             n = S->n;
             // .. and equal ones from the lowest id on
-            for (int v0 = 0; n < (u32)want && v0 < nvec; v0 += LP_NTH) {
+            for (int v0 = -1; n < (u32)want && v0 <= nvec; v0 += LP_NTH) {
                 u32 w[4], k = 0, before = 0;
-                load(v0 + tid, w);
+                const int at_v = v0 + tid;
+                w[0] = w[1] = w[2] = w[3] = NONE;
+                if (at_v == -1 || at_v == nvec) edge(at_v, w); else if (at_v < nvec) load(at_v, w);
 #pragma unroll
                 for (int i = 0; i < N; i++) {
                     const int id = id0 + (v0 + tid) * N + i;
@@ -381,7 +418,7 @@ extern "C" int sz_logprob_rows(int logits_type, uint64_t logits, int64_t logits_
     }
     a.per = ((vocab + a.C - 1) / a.C + 7) & ~7;
     const int vec = 16 / esz;
-    a.groups = ((a.per + vec - 1) / vec + 1 + LP_G * LP_NTH - 1) / (LP_G * LP_NTH);      // (a part may begin and end inside vectors)
+    a.groups = (a.per / vec + LP_G * LP_NTH - 1) / (LP_G * LP_NTH) + 1;      // (a part may begin and end inside vectors)
     cudaStream_t st = (cudaStream_t)stream;
     return logits_type == SZ_TYPE_F32 ? lp_launch<SZ_TYPE_F32>(a, st) : logits_type == SZ_TYPE_F16 ? lp_launch<SZ_TYPE_F16>(a, st) : lp_launch<SZ_TYPE_BF16>(a, st);
 }
