@@ -13,8 +13,7 @@
 
 namespace {
 
-constexpr int LP_NTH = 512, LP_G = 4, LP_MAX_VOCAB = 1 << 18, LP_ID = 18, LP_TOP = 64, LP_LIST = 2048, LP_PLACES = 2 * 148;
-constexpr int LP_NW = LP_NTH / 32;
+constexpr int LP_G = 4, LP_MAX_VOCAB = 1 << 18, LP_ID = 18, LP_TOP = 64, LP_LIST = 2048, LP_SM = 148;
 
 struct LpArgs {
     const u8* logits;
@@ -28,14 +27,17 @@ struct LpArgs {
     float* top_logprobs;
 };
 
-struct LpSmem {
+template <int LP_NTH> struct LpSmem {
+    static constexpr int LP_NW = LP_NTH / 32;
     u64 list[LP_LIST];               // keys of the candidates
     u64 best[8 * LP_TOP];            // block 0: what the blocks found, in order
-    u64 mine[LP_TOP];
+    u32 tmax[LP_NTH];
     float wm[LP_NW], ws[LP_NW], wx[LP_NW];
     u32 wc[LP_NW];
-    float m, s, x, thr;              // of the block's part
-    u32 c, n, found;
+    float4 part[8];                  // block 0: the parts' sums, and how many are larger than the token's
+    u32 upto[8 * LP_TOP];            // .. how many of all are before each of theirs
+    float m, thr;                    // of the block's part
+    u32 n;
 };
 
 template <int TYPE> struct LpVec { static constexpr int ESZ = TYPE == SZ_TYPE_F32 ? 4 : 2, N = 16 / ESZ; };
@@ -63,7 +65,9 @@ __device__ __forceinline__ u32 lp_remote(const void* p, int rank) {
     return a;
 }
 __device__ __forceinline__ void lp_st64(void* p, int rank, u64 v) { asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(lp_remote(p, rank)), "l"(v) : "memory"); }
-__device__ __forceinline__ u32 lp_ld32(const void* p, int rank) { u32 v; asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(lp_remote(p, rank)) : "memory"); return v; }
+__device__ __forceinline__ void lp_st128(void* p, int rank, float4 v) {
+    asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(lp_remote(p, rank)), "f"(v.x), "f"(v.y), "f"(v.z), "f"(v.w) : "memory");
+}
 __device__ __forceinline__ float lp_exp2(float x) { float y; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x)); return y; }
 __device__ __forceinline__ void lp_sync(int C) { if (C > 1) sz_cluster_sync(); else __syncthreads(); }
 
@@ -81,16 +85,18 @@ __device__ __forceinline__ LpSum lp_join(const LpSum a, const LpSum b, float c) 
     return {hi.m, fmaf(w, 1.f + lo.s, hi.s), fmaf(w, fmaf(1.f + lo.s, d, lo.x), hi.x)};
 }
 
-template <int TYPE>
-__global__ void __launch_bounds__(LP_NTH, 2)
+template <int TYPE, int LP_NTH>
+__global__ void __launch_bounds__(LP_NTH, 1024 / LP_NTH)
 sz_logprob_kernel(const LpArgs a) {
     using V = LpVec<TYPE>;
+    using Sm = LpSmem<LP_NTH>;
+    constexpr int LP_NW = LP_NTH / 32;
     constexpr int N = V::N, GE = LP_G * N;               // elements of a vector and of a group
     extern __shared__ __align__(16) u8 lp_smem[];
-    LpSmem* const S = (LpSmem*)lp_smem;
-    float* const gmax = (float*)(lp_smem + sizeof(LpSmem));        // [group][thread]
+    Sm* const S = (Sm*)lp_smem;
+    float* const gmax = (float*)(lp_smem + sizeof(Sm));        // [group][thread]
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, row = blockIdx.x / a.C, rank = blockIdx.x % a.C;
-    if (tid == 0) S->n = S->found = 0;
+    if (tid == 0) S->n = 0;
     if (a.C > 1) sz_cluster_arrive();                    // (block 0's shared memory is written to once all have begun)
     sz_pdl_wait();
     sz_pdl_trigger();
@@ -100,18 +106,34 @@ sz_logprob_kernel(const LpArgs a) {
     const int lead = min(e1 - e0, (int)((16 - (((size_t)base + (size_t)e0 * V::ESZ) & 15)) & 15) / V::ESZ);
     const int id0 = e0 + lead, nvec = (e1 - id0) / N;
     const u8* const vbase = base + (size_t)id0 * V::ESZ;
-    int token = a.tokens ? a.tokens[row] : -1;
-    if ((u32)token >= (u32)a.vocab) token = -1;
-    const float tv = token >= 0 ? lp_clean(lp_one<TYPE>(base + (size_t)token * V::ESZ)) : INFINITY;
-    const int before = min(token, e1);                   // (what lies beside the part is -inf here, and nobody's)
-    const float T = a.temperature ? a.temperature[row] : 1.f, inv_t = 1.f / T;
-    const bool alone = !(T > 0.f) || !(inv_t <= 3.4e38f);            // the best token has it all
-    const float c = alone ? 0.f : inv_t * 1.4426950408889634f;
     constexpr u32 NONE = TYPE == SZ_TYPE_F32 ? 0xff800000u : TYPE == SZ_TYPE_F16 ? 0xfc00fc00u : 0xff80ff80u;      // -inf
     auto load = [&](int v, u32* w) {
         const uint4 q = __ldcg((const uint4*)(vbase + (size_t)v * 16));
         w[0] = q.x; w[1] = q.y; w[2] = q.z; w[3] = q.w;
     };
+    const int whole = nvec / (LP_G * LP_NTH), last = a.groups - 1;       // (the last group: what lies beside the vectors)
+    auto ask = [&](int g, u32* w) {                      // the vectors of a group
+        const int v0 = g * LP_G * LP_NTH + tid;
+        if (g < whole) {
+#pragma unroll
+            for (int j = 0; j < LP_G; j++) load(v0 + j * LP_NTH, w + 4 * j);
+        } else {
+#pragma unroll
+            for (int j = 0; j < LP_G; j++) {
+                w[4 * j] = w[4 * j + 1] = w[4 * j + 2] = w[4 * j + 3] = NONE;
+                if (v0 + j * LP_NTH < nvec) load(v0 + j * LP_NTH, w + 4 * j);
+            }
+        }
+    };
+    u32 ahead[4 * LP_G];
+    ask(0, ahead);
+    int token = a.tokens ? a.tokens[row] : -1;
+    if ((u32)token >= (u32)a.vocab) token = -1;
+    const float tv = token >= 0 ? lp_clean(lp_one<TYPE>(base + (size_t)token * V::ESZ)) : INFINITY;
+    const float tv_next = lp_down(lp_up(tv) + 1);        // (of a finite one; of the largest: infinity)
+    const float T = a.temperature ? a.temperature[row] : 1.f, inv_t = 1.f / T;
+    const bool alone = !(T > 0.f) || !(inv_t <= 3.4e38f);            // the best token has it all
+    const float c = alone ? 0.f : inv_t * 1.4426950408889634f;
     auto edge = [&](int v, u32* w) {                     // vector -1: the elements before the first, nvec: those behind the last
 #pragma unroll
         for (int i = 0; i < 4; i++) {
@@ -128,7 +150,6 @@ sz_logprob_kernel(const LpArgs a) {
     };
     float m = -INFINITY, s = 0.f, x = 0.f, tmax = -INFINITY;         // of the warp (m), of the thread (the others)
     u32 cnt = 0;
-    const int whole = nvec / (LP_G * LP_NTH), last = a.groups - 1;       // (the last group: what lies beside the vectors)
     // one group: vectors v0, v0 + LP_NTH, .. (elements that are nobody's are -inf)
     auto take = [&](int g, int v0, const u32* w) {
         float gm = -INFINITY;
@@ -146,19 +167,36 @@ sz_logprob_kernel(const LpArgs a) {
         }
         if (a.top) gmax[g * LP_NTH + tid] = gm;
         tmax = fmaxf(tmax, gm);
-        // larger than the token's logit, or equal with a lower id
+        // larger than the token's logit, or equal with a lower id: not below it before the token, not below the next number behind it
         if (gm >= tv && token >= 0) {
+            if (tv == -INFINITY || g == last) {
+#pragma unroll 1
+                for (int i = 0; i < GE; i++) {
+                    const int at = v0 + (i / N) * LP_NTH, id = id0 + at * N + i % N;
+                    const bool there = g == last ? tid < 2 && i < N : at < nvec;
+                    if (!there || id < e0 || id >= e1) continue;
+                    const float v = lp_clean(lp_one<TYPE>(base + (size_t)id * V::ESZ));
+                    cnt += v > tv || (v == tv && id < token) ? 1u : 0u;
+                }
+            } else {
 #pragma unroll
-            for (int i = 0; i < GE; i++) {
-                const float v = lp_clean(lp_at<TYPE>(w, i));
-                const int at = v0 + (i / N) * LP_NTH, id = id0 + at * N + i % N;
-                const bool there = g == last ? tid < 2 && i < N : at < nvec;
-                cnt += (v > tv || (there && v == tv && id < before && id >= e0)) ? 1u : 0u;
+                for (int j = 0; j < LP_G; j++) {
+                    const int id = id0 + (v0 + j * LP_NTH) * N;
+                    if (id <= token && token < id + N) {             // the token's own vector
+#pragma unroll
+                        for (int i = 0; i < N; i++) { const float v = lp_at<TYPE>(w + 4 * j, i); cnt += v > tv || (v == tv && id + i < token) ? 1u : 0u; }
+                    } else {
+                        const float from = id < token ? tv : tv_next;
+#pragma unroll
+                        for (int i = 0; i < N; i++) cnt += lp_at<TYPE>(w + 4 * j, i) >= from ? 1u : 0u;
+                    }
+                }
             }
         }
         const float wm = lp_down(__reduce_max_sync(0xffffffffu, lp_up(gm)));
+        const bool wm_new = wm > m;
         bool skip = false;
-        if (wm > m) {                                    // (the same for the whole warp)
+        if (wm_new) {                                    // (the same for the whole warp)
             if (m > -INFINITY) {                             // the old largest is one of the others now: lane 0 has it
                 const float d = fmaxf((m - wm) * c, -200.f), f = lp_exp2(d);
                 const float t = s + (lane == 0 ? 1.f : 0.f);
@@ -168,18 +206,22 @@ sz_logprob_kernel(const LpArgs a) {
             m = wm;
             skip = lane == __ffs(__ballot_sync(0xffffffffu, gm == wm)) - 1;
         }
-        if (__any_sync(0xffffffffu, skip)) {             // one of the largest is left out
+        const u64 m2 = lp_pack(-m, -m), c2 = lp_pack(c, c);
+        u64 gs = 0, gx = 0;
+        if (wm_new) {                                    // .. where there is a new largest, it (and what equals it in its lane) weighs nothing here
+            int n = skip ? -1 : 0;                           // .. the others of these are put back: they weigh 1
 #pragma unroll
-            for (int i = 0; i < GE; i++) {
-                const float v = lp_at<TYPE>(w, i);
-                const float e = fmaxf((v - m) * c, -200.f), p = skip && v == m ? 0.f : lp_exp2(e);
-                if (v == m) skip = false;
-                s += p;
-                x = fmaf(p, e, x);
+            for (int i = 0; i < GE; i += 2) {
+                const u64 e2 = lp_mul2(lp_add2(lp_pack(lp_at<TYPE>(w, i), lp_at<TYPE>(w, i + 1)), m2), c2);
+                float e = fmaxf(__uint_as_float((u32)e2), -200.f), f = fmaxf(__uint_as_float((u32)(e2 >> 32)), -200.f);
+                if (skip && lp_at<TYPE>(w, i) == m) { n++; e = -200.f; }
+                if (skip && lp_at<TYPE>(w, i + 1) == m) { n++; f = -200.f; }
+                const u64 p = lp_pack(lp_exp2(e), lp_exp2(f));
+                gs = lp_add2(gs, p);
+                lp_fma2(gx, p, lp_pack(e, f));
             }
+            s += (float)n;
         } else {
-            const u64 m2 = lp_pack(-m, -m), c2 = lp_pack(c, c);
-            u64 gs = 0, gx = 0;
 #pragma unroll
             for (int i = 0; i < GE; i += 2) {
                 const u64 e2 = lp_mul2(lp_add2(lp_pack(lp_at<TYPE>(w, i), lp_at<TYPE>(w, i + 1)), m2), c2);
@@ -188,24 +230,17 @@ sz_logprob_kernel(const LpArgs a) {
                 gs = lp_add2(gs, p);
                 lp_fma2(gx, p, lp_pack(e, f));
             }
-            s += __uint_as_float((u32)gs) + __uint_as_float((u32)(gs >> 32));
-            x += __uint_as_float((u32)gx) + __uint_as_float((u32)(gx >> 32));
         }
+        s += __uint_as_float((u32)gs) + __uint_as_float((u32)(gs >> 32));
+        x += __uint_as_float((u32)gx) + __uint_as_float((u32)(gx >> 32));
     };
 #pragma unroll 1
     for (int g = 0; g < last; g++) {
         u32 w[4 * LP_G];
         const int v0 = g * LP_G * LP_NTH + tid;
-        if (g < whole) {
 #pragma unroll
-            for (int j = 0; j < LP_G; j++) load(v0 + j * LP_NTH, w + 4 * j);
-        } else {
-#pragma unroll
-            for (int j = 0; j < LP_G; j++) {
-                w[4 * j] = w[4 * j + 1] = w[4 * j + 2] = w[4 * j + 3] = NONE;
-                if (v0 + j * LP_NTH < nvec) load(v0 + j * LP_NTH, w + 4 * j);
-            }
-        }
+        for (int i = 0; i < 4 * LP_G; i++) w[i] = ahead[i];
+        ask(g + 1, ahead);
         take(g, v0, w);
     }
     if (a.top) gmax[last * LP_NTH + tid] = -INFINITY;
@@ -223,49 +258,67 @@ sz_logprob_kernel(const LpArgs a) {
     cnt = __reduce_add_sync(0xffffffffu, cnt);
     if (lane == 0) { S->wm[warp] = m; S->ws[warp] = s; S->wx[warp] = x; S->wc[warp] = cnt; }
     __syncthreads();
+    float4 mine = make_float4(0.f, 0.f, 0.f, 0.f);       // (warp 0's)
     if (warp == 0) {
         LpSum t = lane < LP_NW ? LpSum{S->wm[lane], S->ws[lane], S->wx[lane]} : LpSum{-INFINITY, 0.f, 0.f};
         u32 n = lane < LP_NW ? S->wc[lane] : 0;
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) t = lp_join(t, {__shfl_xor_sync(0xffffffffu, t.m, o), __shfl_xor_sync(0xffffffffu, t.s, o), __shfl_xor_sync(0xffffffffu, t.x, o)}, c);
         n = __reduce_add_sync(0xffffffffu, n);
-        if (lane == 0) { S->m = t.m; S->s = t.s; S->x = t.x; S->c = n; }
+        mine = {t.m, t.s, t.x, __uint_as_float(n)};
+        if (lane == 0) S->m = t.m;
     }
     __syncthreads();
     const int top = a.top, have = e1 - e0, want = min(top, have);
     if (a.C > 1) sz_cluster_wait();
+    if (tid == 0) { if (a.C > 1) lp_st128(&S->part[rank], 0, mine); else S->part[0] = mine; }
     if (want > 0) {
         // ---- the part's best: a bound that `want` threads' largest reach
         float thr = S->m;
-        if (want > 1) {
-            u32 hi = lp_up(S->m), lo = lp_up(-INFINITY);
-            // (lo: reached by all that have anything; hi: by one at least)
-            for (int step = 0; step < 32 && hi - lo > 1; step++) {
-                const u32 mid = step == 0 ? lp_up(S->m - 4.f / fmaxf(c, 0.25f)) : lo + (hi - lo) / 2;
-                if (mid <= lo || mid >= hi) continue;
-                const int n = __syncthreads_count(lp_up(tmax) >= mid);
-                if (n >= want) lo = mid; else hi = mid;
-                if (n >= want && n <= want + 16) break;
+        if (want > 1) {                                  // (one warp looks at all threads' largest: no barrier a step)
+            S->tmax[tid] = lp_up(tmax);
+            __syncthreads();
+            if (warp == 0) {
+                u32 k[LP_NW];
+#pragma unroll
+                for (int i = 0; i < LP_NW; i++) k[i] = S->tmax[32 * i + lane];
+                u32 hi = lp_up(thr), lo = lp_up(-INFINITY);
+                // (lo: reached by all that have anything; hi: by one at least)
+                for (int step = 0; step < 32 && hi - lo > 1; step++) {
+                    const u32 mid = step == 0 ? lp_up(thr - 4.f / fmaxf(c, 0.25f)) : lo + (hi - lo) / 2;
+                    if (mid <= lo || mid >= hi) continue;
+                    u32 n = 0;
+#pragma unroll
+                    for (int i = 0; i < LP_NW; i++) n += k[i] >= mid;
+                    n = __reduce_add_sync(0xffffffffu, n);
+                    if (n >= (u32)want) lo = mid; else hi = mid;
+                    if (n >= (u32)want && n <= (u32)want + 16) break;
+                }
+                if (lane == 0) S->thr = lp_down(lo);
             }
-            thr = lp_down(lo);
+            __syncthreads();
+            thr = S->thr;
         }
         auto gather = [&](float from, bool equal) {
             for (int g = 0; g < a.groups; g++) {
                 const float gm = gmax[g * LP_NTH + tid];
                 if (!(equal ? gm >= from : gm > from)) continue;
-                for (int j = 0; j < LP_G; j++) {
-                    const int v = g == last ? (tid == 0 ? -1 : nvec) : (g * LP_G + j) * LP_NTH + tid;
-                    if (g == last ? j > 0 || tid > 1 : v >= nvec) break;
-                    u32 w[4];
-                    if (g == last) edge(v, w); else load(v, w);
+                u32 w[4 * LP_G];
+                int at[LP_G];
 #pragma unroll
-                    for (int i = 0; i < N; i++) {
-                        const int id = id0 + v * N + i;
-                        const float f = lp_clean(lp_at<TYPE>(w, i));
-                        if (id < e0 || id >= e1 || !(equal ? f >= from : f > from)) continue;
-                        const u32 at = atomicAdd(&S->n, 1u);
-                        if (at < LP_LIST) S->list[at] = lp_key(f, id);
-                    }
+                for (int j = 0; j < LP_G; j++) {
+                    at[j] = g == last ? (tid == 0 ? -1 : nvec) : (g * LP_G + j) * LP_NTH + tid;
+                    if (g == last ? j > 0 || tid > 1 : at[j] >= nvec) at[j] = -2;
+                    else if (g == last) edge(at[j], w + 4 * j);
+                    else load(at[j], w + 4 * j);
+                }
+#pragma unroll
+                for (int i = 0; i < GE; i++) {
+                    const int id = id0 + at[i / N] * N + i % N;
+                    const float f = lp_clean(lp_at<TYPE>(w + 4 * (i / N), i % N));
+                    if (at[i / N] == -2 || id < e0 || id >= e1 || !(equal ? f >= from : f > from)) continue;
+                    const u32 place = atomicAdd(&S->n, 1u);
+                    if (place < LP_LIST) S->list[place] = lp_key(f, id);
                 }
             }
         };
@@ -334,11 +387,12 @@ sz_logprob_kernel(const LpArgs a) {
         for (int i = want + tid; i < top; i += LP_NTH) { if (a.C > 1) lp_st64(&S->best[rank * LP_TOP + i], 0, ~0ull); else S->best[i] = ~0ull; }
     lp_sync(a.C);
     if (rank == 0) {
-        LpSum t = {S->m, S->s, S->x};
-        u32 n = S->c;
+        LpSum t = {S->part[0].x, S->part[0].y, S->part[0].z};
+        u32 n = __float_as_uint(S->part[0].w);
         for (int r = 1; r < a.C; r++) {
-            t = lp_join(t, {__uint_as_float(lp_ld32(&S->m, r)), __uint_as_float(lp_ld32(&S->s, r)), __uint_as_float(lp_ld32(&S->x, r))}, c);
-            n += lp_ld32(&S->c, r);
+            const float4 o = S->part[r];
+            t = lp_join(t, {o.x, o.y, o.z}, c);
+            n += __float_as_uint(o.w);
         }
         const bool one = alone || !(fabsf(t.m) < INFINITY);
         const float lz = log1pf(t.s);
@@ -354,24 +408,35 @@ sz_logprob_kernel(const LpArgs a) {
                 a.top_logprobs[(size_t)row * top + at] = key == ~0ull ? -INFINITY : one ? (at == 0 ? 0.f : -INFINITY) : (v - t.m) * inv_t - lz;
             };
             if (a.C == 1) { if (tid < top) give(tid, S->best[tid]); }
-            else
-                for (int i = tid; i < a.C * LP_TOP; i += LP_NTH) {
-                    if (i % LP_TOP >= top) continue;
-                    const u64 key = S->best[i];
-                    int at = 0;
-                    for (int r = 0; r < a.C; r++)
-                        for (int j = 0; j < top; j++) { const u64 o = S->best[r * LP_TOP + j]; at += o < key || (o == key && r * LP_TOP + j < i); }
-                    if (at < top) give(at, key);
+            else {                                       // a key's place: how many are before it in each list (they are in order)
+                for (int i = tid; i < a.C * top; i += LP_NTH) S->upto[i] = 0;
+                __syncthreads();
+                for (int i = tid; i < a.C * top * a.C; i += LP_NTH) {
+                    const int r = i % a.C, k = i / a.C, own = k / top;
+                    const u64 key = S->best[own * LP_TOP + k % top];
+                    int lo = 0, hi = top;                // (equal ones, of parts that have fewer: by part)
+                    if (r == own) lo = hi = k % top;
+                    while (lo < hi) {
+                        const int mid = (lo + hi) / 2;
+                        const u64 o = S->best[r * LP_TOP + mid];
+                        if (o < key || (o == key && r < own)) lo = mid + 1; else hi = mid;
+                    }
+                    if (lo) atomicAdd(&S->upto[k], (u32)lo);
                 }
+                __syncthreads();
+                for (int i = tid; i < a.C * top; i += LP_NTH) if (S->upto[i] < (u32)top) give((int)S->upto[i], S->best[(i / top) * LP_TOP + i % top]);
+            }
         }
     }
     lp_sync(a.C);                                        // (shared memory is read by block 0 until here)
 }
 
-template <int TYPE>
-int lp_launch(const LpArgs& a, cudaStream_t st) {
-    const size_t smem = sizeof(LpSmem) + (a.top ? (size_t)a.groups * LP_NTH * 4 : 0);
-    const int rc = sz_allow_smem((const void*)sz_logprob_kernel<TYPE>, 112 * 1024);
+template <int TYPE, int LP_NTH>
+int lp_launch(LpArgs a, cudaStream_t st) {
+    constexpr int VEC = LpVec<TYPE>::N;
+    a.groups = (a.per / VEC + LP_G * LP_NTH - 1) / (LP_G * LP_NTH) + 1;      // (a part may begin and end inside vectors)
+    const size_t smem = sizeof(LpSmem<LP_NTH>) + (a.top ? (size_t)a.groups * LP_NTH * 4 : 0);
+    const int rc = sz_allow_smem((const void*)sz_logprob_kernel<TYPE, LP_NTH>, 112 * 1024);
     if (rc) return rc;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)a.rows * a.C);
@@ -387,7 +452,7 @@ int lp_launch(const LpArgs& a, cudaStream_t st) {
     attr[1].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = a.C > 1 ? 2 : 1;
-    SZ_CUDA(cudaLaunchKernelEx(&cfg, sz_logprob_kernel<TYPE>, a));
+    SZ_CUDA(cudaLaunchKernelEx(&cfg, sz_logprob_kernel<TYPE, LP_NTH>, a));
     sz_trace_mark("logprob_rows", st);
     return SZ_OK;
 }
@@ -409,16 +474,18 @@ extern "C" int sz_logprob_rows(int logits_type, uint64_t logits, int64_t logits_
     a.logits = (const u8*)logits; a.stride = logits_stride * esz; a.rows = rows; a.vocab = vocab; a.top = top;
     a.tokens = (const int32_t*)tokens; a.temperature = (const float*)temperature;
     a.logprob = (float*)logprob; a.entropy = (float*)entropy; a.rank = (int32_t*)rank; a.top_ids = (int32_t*)top_ids; a.top_logprobs = (float*)top_logprobs;
-    // blocks a row: waves of blocks times what one takes
+    // blocks a row: waves of blocks times what one takes; with few rows (none has to wait) blocks of twice the threads
     const int most = vocab > 16384 ? 8 : vocab > 4096 ? 4 : vocab > 1024 ? 2 : 1;
+    const bool few = (long long)rows * most <= 2 * LP_SM;
+    const int places = few ? 2 * LP_SM : 4 * LP_SM;
     double least = 0;
     for (int C = 1; C <= most; C *= 2) {
-        const double cost = (double)(((long long)rows * C + LP_PLACES - 1) / LP_PLACES) * (20000.0 + (double)vocab / C);
+        const double cost = (double)(((long long)rows * C + places - 1) / places) * (20000.0 + (double)vocab / C);
         if (C == 1 || cost < least) { least = cost; a.C = C; }
     }
     a.per = ((vocab + a.C - 1) / a.C + 7) & ~7;
-    const int vec = 16 / esz;
-    a.groups = (a.per / vec + LP_G * LP_NTH - 1) / (LP_G * LP_NTH) + 1;      // (a part may begin and end inside vectors)
     cudaStream_t st = (cudaStream_t)stream;
-    return logits_type == SZ_TYPE_F32 ? lp_launch<SZ_TYPE_F32>(a, st) : logits_type == SZ_TYPE_F16 ? lp_launch<SZ_TYPE_F16>(a, st) : lp_launch<SZ_TYPE_BF16>(a, st);
+#define SZ_LP(N_) (logits_type == SZ_TYPE_F32 ? lp_launch<SZ_TYPE_F32, N_>(a, st) : logits_type == SZ_TYPE_F16 ? lp_launch<SZ_TYPE_F16, N_>(a, st) : lp_launch<SZ_TYPE_BF16, N_>(a, st))
+    return few ? SZ_LP(512) : SZ_LP(256);
+#undef SZ_LP
 }

@@ -6,6 +6,7 @@ import torch
 
 from . import lib as szlib
 from .paged import _HERE, TYPES
+from .sampling import _raw_stream
 
 
 class DeltaPoolC(C.Structure):
@@ -72,6 +73,9 @@ class Step:
             raise ValueError("the pool and tables lie on a GPU, not on %s" % states.device)
         self.pool, self.rows, self.device, self._index = states, rows, states.device, states.device.index
         self._keep = (row_start, lens, slots, to, take)
+        p = states
+        self._wide, self._narrow, self._heads, self._chan = (rows, p.vh, p.hd), (rows, p.kh, p.hd), (rows, p.vh), (rows, p.channels)
+        self._in = (p.hd, 1)
         ptr = lambda t: 0 if t is None else t.data_ptr()  # noqa: E731
         self.b = DeltaBatchC(n_seq=n, rows=rows, max_rows=max_rows or 0, row_start=ptr(row_start), lens=ptr(lens), from_=ptr(slots), to=ptr(to), take=ptr(take))
         self._c, self._b = C.byref(states.c), C.byref(self.b)
@@ -87,27 +91,26 @@ class Step:
         return _HERE if torch.cuda.current_device() == self._index else torch.cuda.device(self._index)
 
     def _stream(self):
-        return torch.cuda.current_stream(self._index).cuda_stream
+        return _raw_stream(self._index)
 
-    def _rows(self, name, t, shape, dtype):
-        """Checks [rows, *shape] of dtype, what belongs to a row side by side; returns its address and the stride of rows."""
-        if t.shape != (self.rows,) + shape or t.device != self.device:
-            raise ValueError("%s: %s on the pool's device" % (name, [self.rows, *shape]))
+    def _rows(self, name, t, shape, inner, dtype):
+        """Checks [rows, *shape] of dtype, what belongs to a row side by side (strides `inner`); returns its address and the stride of rows."""
+        st = t.stride()
+        if t.dtype is dtype and t.shape == shape and st[1:] == inner and t.get_device() == self._index and st[0] >= shape[1] * inner[0]:
+            return t.data_ptr(), st[0]
+        if t.shape != shape or t.device != self.device:
+            raise ValueError("%s: %s on the pool's device" % (name, list(shape)))
         if t.dtype is not dtype or dtype not in TYPES:
             raise ValueError("%s: float32, float16 or bfloat16, the same for all rows of a call" % name)
-        st, width = t.stride(), 1
-        for i in range(len(shape), 0, -1):
-            if st[i] != width and t.shape[i] > 1:
-                raise ValueError("%s: heads side by side, the last dimension contiguous" % name)
-            width *= t.shape[i]
-        if self.rows == 1:
-            return t.data_ptr(), width
-        if st[0] < width:
+        if any(n > 1 and a != b for n, a, b in zip(shape[1:], st[1:], inner)):
+            raise ValueError("%s: heads side by side, the last dimension contiguous" % name)
+        width = shape[1] * inner[0]
+        if self.rows > 1 and st[0] < width:
             raise ValueError("%s: rows that overlap" % name)
-        return t.data_ptr(), st[0]
+        return t.data_ptr(), st[0] if self.rows > 1 else width
 
     def _f32(self, name, t, *shape):
-        if t.dtype != torch.float32 or t.shape != shape or not t.is_contiguous() or t.device != self.device:
+        if t.dtype is not torch.float32 or t.shape != shape or not t.is_contiguous() or t.get_device() != self._index:
             raise ValueError("%s: contiguous float32 %s on the pool's device" % (name, list(shape)))
         return t.data_ptr()
 
@@ -117,10 +120,10 @@ class Step:
         p = self.pool
         if p.conv is None:
             raise ValueError("the pool has no carried rows")
-        xp, xs = self._rows("x", x, (p.channels,), x.dtype)
+        xp, xs = self._rows("x", x, self._chan, (1,), x.dtype)
         if out is None:
             out = torch.empty((self.rows, p.channels), dtype=x.dtype, device=x.device)
-        op, os = self._rows("out", out, (p.channels,), x.dtype)
+        op, os = self._rows("out", out, self._chan, (1,), x.dtype)
         wp, bp = self._f32("w", w, p.channels, p.conv_k), 0 if bias is None else self._f32("bias", bias, p.channels)
         with self._here():
             rc = self.lib.sz_delta_conv(self._c, self._b, TYPES[x.dtype], xp, xs, wp, bp, op, os, self.scratch, self.scratch_bytes, self._stream())
@@ -135,7 +138,7 @@ class Step:
         p, dtype = self.pool, k.dtype
         if out is None:
             out = torch.empty((self.rows, p.vh, p.hd), dtype=dtype, device=k.device)
-        return self._rule(self._rows("q", q, (p.kh, p.hd), dtype), k, v, alpha, beta, a, dt, z, norm, eps, out)
+        return self._rule(self._rows("q", q, self._narrow, self._in, dtype), k, v, alpha, beta, a, dt, z, norm, eps, out)
 
     def replay(self, k, v, alpha, beta, a, dt):
         """The states alone, without outputs (after a refusal of drafts: `take` says how many rows are kept)."""
@@ -147,10 +150,10 @@ class Step:
             raise ValueError("the pool has no states")
         if (z is None) != (norm is None):
             raise ValueError("z and norm come together")
-        wide = (p.vh, p.hd)
-        args = q + self._rows("k", k, (p.kh, p.hd), dtype) + self._rows("v", v, wide, dtype) + self._rows("alpha", alpha, (p.vh,), dtype) + self._rows("beta", beta, (p.vh,), dtype)
-        args += (0, 0) if z is None else self._rows("z", z, wide, dtype)
-        args += (0, 0) if out is None else self._rows("out", out, wide, dtype)
+        rows, wide, inner = self._rows, self._wide, self._in
+        args = q + rows("k", k, self._narrow, inner, dtype) + rows("v", v, wide, inner, dtype) + rows("alpha", alpha, self._heads, (1,), dtype) + rows("beta", beta, self._heads, (1,), dtype)
+        args += (0, 0) if z is None else rows("z", z, wide, inner, dtype)
+        args += (0, 0) if out is None else rows("out", out, wide, inner, dtype)
         gates = DeltaGatesC(self._f32("a", a, p.vh), self._f32("dt", dt, p.vh), 0 if norm is None else self._f32("norm", norm, p.hd), eps, 0.0)
         io = TYPES[dtype]
         with self._here():

@@ -7,6 +7,12 @@ import torch
 from . import lib as szlib
 from .paged import _HERE, TYPES
 
+try:                                                     # (the stream's handle alone: an object for it takes 3 us)
+    from torch._C import _cuda_getCurrentRawStream as _raw_stream
+except ImportError:
+    def _raw_stream(index):
+        return torch.cuda.current_stream(index).cuda_stream
+
 
 def sample_rows(logits, uniform, temperature=None, top_k=None, top_p=None, min_p=None, out=None, prob=None):
     """logits [rows, vocab] (float32, float16 or bfloat16, vocab <= 262144), uniform float64 [rows] in [0, 1); temperature, top_p, min_p float32
@@ -56,7 +62,7 @@ def logprob_rows(logits, tokens=None, top=0, temperature=None, out=None):
     L = szlib.load()
     if logits.dim() != 2 or logits.dtype not in TYPES or (logits.shape[1] > 1 and logits.stride(1) != 1):
         raise ValueError("logits: [rows, vocab] of float32, float16 or bfloat16, rows contiguous")
-    (rows, vocab), stride, dev = logits.shape, logits.stride(0), logits.device
+    (rows, vocab), stride, dev, index = logits.shape, logits.stride(0), logits.device, logits.get_device()
     if stride < vocab:
         if rows > 1:
             raise ValueError("logits: rows that overlap")
@@ -69,7 +75,7 @@ def logprob_rows(logits, tokens=None, top=0, temperature=None, out=None):
     def at(name, t, dt, *of):
         if t is None:
             return 0
-        if t.dtype != dt or t.shape != of or t.device != dev or not t.is_contiguous():
+        if t.dtype is not dt or t.shape != of or t.get_device() != index or not t.is_contiguous():
             raise ValueError("%s: %s %s on the logits' device" % (name, dt, list(of)))
         return t.data_ptr()
 
@@ -83,7 +89,7 @@ def logprob_rows(logits, tokens=None, top=0, temperature=None, out=None):
     if dev.type != "cuda":
         raise ValueError("logits, tokens and results lie on a GPU, not on %s" % dev)
     with _HERE if torch.cuda.current_device() == dev.index else torch.cuda.device(dev):
-        rc = L.sz_logprob_rows(TYPES[logits.dtype], logits.data_ptr(), stride, rows, vocab, tp, hp, top, *ptrs, torch.cuda.current_stream(dev.index).cuda_stream)
+        rc = L.sz_logprob_rows(TYPES[logits.dtype], logits.data_ptr(), stride, rows, vocab, tp, hp, top, *ptrs, _raw_stream(index))
     if rc:
         szlib.check(rc)
     return out
