@@ -31,13 +31,13 @@ template <int LP_NTH> struct LpSmem {
     static constexpr int LP_NW = LP_NTH / 32;
     u64 list[LP_LIST];               // keys of the candidates
     u64 best[8 * LP_TOP];            // block 0: what the blocks found, in order
+    u32 hit[8 * LP_TOP];             // groups that can hold any of the best
     u32 tmax[LP_NTH];
     float wm[LP_NW], ws[LP_NW], wx[LP_NW];
     u32 wc[LP_NW];
     float4 part[8];                  // block 0: the parts' sums, and how many are larger than the token's
-    u32 upto[8 * LP_TOP];            // .. how many of all are before each of theirs
     float m, thr;                    // of the block's part
-    u32 n;
+    u32 n, hits;
 };
 
 template <int TYPE> struct LpVec { static constexpr int ESZ = TYPE == SZ_TYPE_F32 ? 4 : 2, N = 16 / ESZ; };
@@ -125,8 +125,10 @@ sz_logprob_kernel(const LpArgs a) {
             }
         }
     };
-    u32 ahead[4 * LP_G];
-    ask(0, ahead);
+    // few rows: a group ahead (with many, other blocks' warps are under way meanwhile, and registers are few)
+    constexpr bool AHEAD = LP_NTH == 512;
+    u32 ahead[AHEAD ? 4 * LP_G : 1];
+    if constexpr (AHEAD) ask(0, ahead);
     int token = a.tokens ? a.tokens[row] : -1;
     if ((u32)token >= (u32)a.vocab) token = -1;
     const float tv = token >= 0 ? lp_clean(lp_one<TYPE>(base + (size_t)token * V::ESZ)) : INFINITY;
@@ -238,13 +240,15 @@ sz_logprob_kernel(const LpArgs a) {
     for (int g = 0; g < last; g++) {
         u32 w[4 * LP_G];
         const int v0 = g * LP_G * LP_NTH + tid;
+        if constexpr (AHEAD) {
 #pragma unroll
-        for (int i = 0; i < 4 * LP_G; i++) w[i] = ahead[i];
-        ask(g + 1, ahead);
+            for (int i = 0; i < 4 * LP_G; i++) w[i] = ahead[i];
+            ask(g + 1, ahead);
+        } else ask(g, w);
         take(g, v0, w);
     }
     if (a.top) gmax[last * LP_NTH + tid] = -INFINITY;
-    if (warp == 0) {                                     // threads 0 and 1: before and behind
+    if (warp == 0 && (lead || (e1 - id0) % N)) {         // threads 0 and 1: before and behind
         u32 w[4 * LP_G];
 #pragma unroll
         for (int i = 0; i < 4 * LP_G; i++) w[i] = NONE;
@@ -282,11 +286,13 @@ sz_logprob_kernel(const LpArgs a) {
                 u32 k[LP_NW];
 #pragma unroll
                 for (int i = 0; i < LP_NW; i++) k[i] = S->tmax[32 * i + lane];
-                u32 hi = lp_up(thr), lo = lp_up(-INFINITY);
-                // (lo: reached by all that have anything; hi: by one at least)
+                u32 hi = lp_up(thr), lo = k[0];
+#pragma unroll
+                for (int i = 1; i < LP_NW; i++) lo = min(lo, k[i]);
+                lo = __reduce_min_sync(0xffffffffu, lo);
+                // (lo: reached by all; hi: by one at least)
                 for (int step = 0; step < 32 && hi - lo > 1; step++) {
-                    const u32 mid = step == 0 ? lp_up(thr - 4.f / fmaxf(c, 0.25f)) : lo + (hi - lo) / 2;
-                    if (mid <= lo || mid >= hi) continue;
+                    const u32 mid = lo + (hi - lo) / 2;
                     u32 n = 0;
 #pragma unroll
                     for (int i = 0; i < LP_NW; i++) n += k[i] >= mid;
@@ -299,27 +305,28 @@ sz_logprob_kernel(const LpArgs a) {
             __syncthreads();
             thr = S->thr;
         }
+        // the elements not below a bound (or above it): the groups that hold any are listed, then each element is one thread's
         auto gather = [&](float from, bool equal) {
+            u32* const hits = S->hit;
+            constexpr u32 HITS = 8 * LP_TOP;
+            if (tid == 0) S->hits = 0;
+            __syncthreads();
             for (int g = 0; g < a.groups; g++) {
                 const float gm = gmax[g * LP_NTH + tid];
-                if (!(equal ? gm >= from : gm > from)) continue;
-                u32 w[4 * LP_G];
-                int at[LP_G];
-#pragma unroll
-                for (int j = 0; j < LP_G; j++) {
-                    at[j] = g == last ? (tid == 0 ? -1 : nvec) : (g * LP_G + j) * LP_NTH + tid;
-                    if (g == last ? j > 0 || tid > 1 : at[j] >= nvec) at[j] = -2;
-                    else if (g == last) edge(at[j], w + 4 * j);
-                    else load(at[j], w + 4 * j);
-                }
-#pragma unroll
-                for (int i = 0; i < GE; i++) {
-                    const int id = id0 + at[i / N] * N + i % N;
-                    const float f = lp_clean(lp_at<TYPE>(w + 4 * (i / N), i % N));
-                    if (at[i / N] == -2 || id < e0 || id >= e1 || !(equal ? f >= from : f > from)) continue;
-                    const u32 place = atomicAdd(&S->n, 1u);
-                    if (place < LP_LIST) S->list[place] = lp_key(f, id);
-                }
+                if (equal ? gm >= from : gm > from) { const u32 at = atomicAdd(&S->hits, 1u); if (at < HITS) hits[at] = (u32)(g * LP_NTH + tid); }
+            }
+            __syncthreads();
+            const u32 n = S->hits;
+            if (n > HITS) { if (tid == 0) S->n = LP_LIST + 1; return; }
+            for (u32 i = tid; i < n * GE; i += LP_NTH) {
+                const u32 hit = hits[i / GE], e = i % GE;
+                const int g = hit / LP_NTH, who = hit % LP_NTH, v = g == last ? (who == 0 ? -1 : nvec) : (g * LP_G + (int)(e / N)) * LP_NTH + who;
+                const int id = id0 + v * N + (int)(e % N);
+                if (id < e0 || id >= e1 || (g == last ? e >= N || who > 1 : v >= nvec)) continue;
+                const float f = lp_clean(lp_one<TYPE>(base + (size_t)id * V::ESZ));
+                if (!(equal ? f >= from : f > from)) continue;
+                const u32 place = atomicAdd(&S->n, 1u);
+                if (place < LP_LIST) S->list[place] = lp_key(f, id);
             }
         };
         gather(thr, true);
@@ -408,23 +415,28 @@ sz_logprob_kernel(const LpArgs a) {
                 a.top_logprobs[(size_t)row * top + at] = key == ~0ull ? -INFINITY : one ? (at == 0 ? 0.f : -INFINITY) : (v - t.m) * inv_t - lz;
             };
             if (a.C == 1) { if (tid < top) give(tid, S->best[tid]); }
-            else {                                       // a key's place: how many are before it in each list (they are in order)
-                for (int i = tid; i < a.C * top; i += LP_NTH) S->upto[i] = 0;
+            else {
+                // a list's last key has `top` before it or at its place: what is behind any list's last is not among the best, which leaves about as many as
+                // are asked for; each one's place among them is counted
+                u64 bound = ~0ull;
+                for (int r = 0; r < a.C; r++) bound = min(bound, S->best[r * LP_TOP + top - 1]);
+                if (tid == 0) S->n = 0;
                 __syncthreads();
-                for (int i = tid; i < a.C * top * a.C; i += LP_NTH) {
-                    const int r = i % a.C, k = i / a.C, own = k / top;
-                    const u64 key = S->best[own * LP_TOP + k % top];
-                    int lo = 0, hi = top;                // (equal ones, of parts that have fewer: by part)
-                    if (r == own) lo = hi = k % top;
-                    while (lo < hi) {
-                        const int mid = (lo + hi) / 2;
-                        const u64 o = S->best[r * LP_TOP + mid];
-                        if (o < key || (o == key && r < own)) lo = mid + 1; else hi = mid;
-                    }
-                    if (lo) atomicAdd(&S->upto[k], (u32)lo);
+                for (int i = tid; i < a.C * LP_TOP; i += LP_NTH) {
+                    if (i % LP_TOP >= top) continue;
+                    const u64 key = S->best[i];
+                    if (key <= bound && key != ~0ull) S->list[atomicAdd(&S->n, 1u)] = key;
                 }
                 __syncthreads();
-                for (int i = tid; i < a.C * top; i += LP_NTH) if (S->upto[i] < (u32)top) give((int)S->upto[i], S->best[(i / top) * LP_TOP + i % top]);
+                const u32 k = S->n;
+                for (u32 i = tid; i < k; i += LP_NTH) {
+                    const u64 key = S->list[i];
+                    u32 at = 0;
+#pragma unroll 4
+                    for (u32 j = 0; j < k; j++) at += S->list[j] < key;
+                    if (at < (u32)top) give((int)at, key);
+                }
+                for (u32 i = k + tid; i < (u32)top; i += LP_NTH) give((int)i, ~0ull);      // (a vocabulary of fewer)
             }
         }
     }
