@@ -94,20 +94,27 @@ __host__ __device__ constexpr int dl_tile(int n) { return (n / 2) * (n / 2 + 1) 
 __device__ __forceinline__ float dl_pow2(int e) { return e < -126 ? 0.f : __uint_as_float((u32)(min(e, 127) + 127) << 23); }
 
 // ---- what does not need the state -----------------------------------------------------------------------------------------------------------
-constexpr int DL_AS = 68, DL_TS = 72;                    // strides of a value head's A (by columns) and T (by rows), which share their place
+// The inverse goes by blocks of 16 rows: those on the diagonal in f32, a column a lane, top down; the others column of blocks by column of blocks,
+//   X_ab = - X_aa sum_{b <= c < a} A_ac X_cb,
+// on mma.sync with two f16 numbers a factor, transposed, so that a product's result is the next one's factor.  e^(G_i - G_j) of different blocks is the product of two
+// exponentials that meet at the first row of i's block (both at most 1), of one block an exponential of its own.
+constexpr int DL_OFF = 12, DL_DS = 20;                   // 8 x 16 tiles below the diagonal's blocks; stride of a block on it
 template <int D, int TYPE> struct DlPrep {
-    static constexpr int ROWS = DlChunk<D, TYPE>::ROWS, A = CK * DL_TS * 4;
-    static constexpr size_t SMEM = ROWS + 2 * A;
+    static constexpr int ROWS = DlChunk<D, TYPE>::ROWS;
+    static constexpr int AF = DL_OFF * 32 * 8 * 2, DG = 4 * 16 * DL_DS * 4, HEAD = AF + DG;      // a value head's A (high, low), and its blocks on the diagonal, then their inverses
+    static constexpr size_t SMEM = ROWS > 2 * HEAD ? ROWS : 2 * HEAD;                            // (where the rows were)
 };
+__device__ __forceinline__ u32 dl_turn(u32 a) { u32 d; asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a)); return d; }
 
 template <int D, int TYPE, bool OUT>
-__global__ void __launch_bounds__(128)
+__global__ void __launch_bounds__(128, TYPE == SZ_TYPE_F32 ? 2 : 4)
 sz_delta_prep_kernel(const DlBatch d, const DlRule a, int idx0, u8* __restrict__ scratch, long long one) {
     using C = DlChunk<D, TYPE>;
-    constexpr int ESZ = DlIo<TYPE>::ESZ, NK = C::NK, E = D / 8;
+    using P = DlPrep<D, TYPE>;
+    constexpr int ESZ = DlIo<TYPE>::ESZ, NK = C::NK, E = D / 8, W = E * ESZ / 16;
     extern __shared__ __align__(16) u8 sm[];
     __shared__ double sG[2][CK];
-    __shared__ float sRk[CK], sRq[CK], sBeta[2][CK];
+    __shared__ float sRk[CK], sRq[CK], sBeta[2][CK], sE[2][CK], sB[2][4][CK];      // e^(G_i - G_first of its block); e^(G_first of a block - G_j) rho_k
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, kx = blockIdx.y, g = lane >> 2, t = lane & 3;
     sz_pdl_wait();
     sz_pdl_trigger();
@@ -120,16 +127,52 @@ sz_delta_prep_kernel(const DlBatch d, const DlRule a, int idx0, u8* __restrict__
     const size_t row0 = (size_t)s.r0 + (size_t)c * CK;
     u8* const mine = scratch + (size_t)blockIdx.x * one;
     u8* const rows = mine + (size_t)kx * C::ROWS;
+    const int ratio = a.vh / a.kh;
+    auto head = [&](int i) { return a.grouped ? kx * ratio + i : i * a.kh + kx; };      // the key head's i-th value head
+    // a pair's gates: two rows a lane of warps 0 and 1, and the sums of the decays' logarithms
+    float al[2] = {0.f, 0.f}, be[2] = {0.f, 0.f};
+    auto ask_gates = [&](int v0) {
+        if (warp < 2 && v0 + warp < ratio)
+#pragma unroll
+            for (int i = 0; i < 2; i++)
+                if (2 * lane + i < n) {
+                    const size_t row = row0 + 2 * lane + i;
+                    al[i] = dl_load1<TYPE>(a.alpha + row * a.alpha_stride + (size_t)head(v0 + warp) * ESZ);
+                    be[i] = dl_load1<TYPE>(a.beta + row * a.beta_stride + (size_t)head(v0 + warp) * ESZ);
+                }
+    };
+    auto sum_gates = [&](int v0) {
+        if (warp < 2 && v0 + warp < ratio) {
+            const int h = head(v0 + warp);
+            double G[2];
+#pragma unroll
+            for (int i = 0; i < 2; i++) {
+                const bool in = 2 * lane + i < n;
+                G[i] = in ? (double)dl_log_decay(al[i], a.a[h], a.dt[h]) : 0.0;
+                sBeta[warp][2 * lane + i] = in ? sz_sigmoid(be[i]) : 0.f;
+            }
+            double sum = G[0] + G[1];
+#pragma unroll
+            for (int o = 1; o < 32; o *= 2) { const double y = __shfl_up_sync(0xffffffffu, sum, o); if (lane >= o) sum += y; }
+            sG[warp][2 * lane] = sum - G[1];
+            sG[warp][2 * lane + 1] = sum;
+        }
+    };
+    ask_gates(0);
     // the rows, scaled by powers of two: eight lanes a row
     const int sub = lane & 7;
-#pragma unroll 1
-    for (int i = 0; i < (OUT ? 8 : 4); i++) {
-        const bool isq = i >= 4;
-        const int r = warp * 16 + (i & 3) * 4 + (lane >> 3);
-        float f[E];
+    uint4 raw[ESZ == 2 && OUT ? 8 : 4][W];
+    auto ask = [&](int i, bool isq) {                        // .. of the warp's 16, every fourth
+        const int r = warp * 16 + i * 4 + (lane >> 3);
+        const u8* p = (isq ? a.q + (row0 + r) * a.q_stride : a.k + (row0 + r) * a.k_stride) + (size_t)(kx * D + sub * E) * ESZ;
+        uint4* to = raw[(ESZ == 2 && isq ? 4 : 0) + i];
 #pragma unroll
-        for (int e = 0; e < E; e++) f[e] = 0.f;
-        if (r < n) dl_load<TYPE, E>((isq ? a.q + (row0 + r) * a.q_stride : a.k + (row0 + r) * a.k_stride) + (size_t)(kx * D + sub * E) * ESZ, f);
+        for (int x = 0; x < W; x++) to[x] = r < n ? __ldcg((const uint4*)p + x) : make_uint4(0, 0, 0, 0);
+    };
+    auto keep = [&](int i, bool isq) {
+        const int r = warp * 16 + i * 4 + (lane >> 3);
+        float f[E];
+        dl_unpack<TYPE, E>((const u32*)raw[(ESZ == 2 && isq ? 4 : 0) + i], f);
         float ss = 0.f, mx = 0.f;
 #pragma unroll
         for (int e = 0; e < E; e++) { ss = fmaf(f[e], f[e], ss); mx = fmaxf(mx, fabsf(f[e])); }
@@ -150,6 +193,21 @@ sz_delta_prep_kernel(const DlBatch d, const DlRule a, int idx0, u8* __restrict__
             *(uint4*)(rows + at) = *(uint4*)(hi + 4 * p);
             if (NK == 2) { *(uint4*)(sm + C::TILE + at) = *(uint4*)(lo + 4 * p); *(uint4*)(rows + C::TILE + at) = *(uint4*)(lo + 4 * p); }
         }
+    };
+#pragma unroll
+    for (int i = 0; i < 4; i++) ask(i, false);
+    if (OUT && ESZ == 2)
+#pragma unroll
+        for (int i = 0; i < 4; i++) ask(i, true);
+    sum_gates(0);
+#pragma unroll
+    for (int i = 0; i < 4; i++) keep(i, false);
+    if (OUT) {
+        if (ESZ == 4)
+#pragma unroll
+            for (int i = 0; i < 4; i++) ask(i, true);
+#pragma unroll
+        for (int i = 0; i < 4; i++) keep(i, true);
     }
     __syncthreads();
     // k.k and q.k of the warp's 16 rows with those up to them: row g (+ 8), columns 8 m + 2 t (+ 1)
@@ -186,52 +244,60 @@ sz_delta_prep_kernel(const DlBatch d, const DlRule a, int idx0, u8* __restrict__
                 }
             }
     }
-    const int ratio = a.vh / a.kh;
-    const int half = warp >> 1, part = warp & 1;             // the pair's value head of the warp's inverse, and its 32 columns
+    const int half = warp >> 1, part = warp & 1;             // the pair's value head whose inverse the warp works on, with one more warp
 #pragma unroll 1
     for (int v0 = 0; v0 < ratio; v0 += 2) {
-        auto head = [&](int i) { return a.grouped ? kx * ratio + v0 + i : (v0 + i) * a.kh + kx; };
-        if (part == 0 && v0 + half < ratio) {                // gates of two rows a lane, and the sums of their logarithms
-            const int h = head(half);
-            double G[2];
+        const int heads = min(2, ratio - v0);
+        // the exponentials that rows of different blocks share
+        {
+            const int i = tid >> 6, r = tid & 63;
+            if (i < heads) {
+                sE[i][r] = expf((float)(sG[i][r] - sG[i][r & ~15]));
 #pragma unroll
-            for (int i = 0; i < 2; i++) {
-                const int r = 2 * lane + i;
-                float lgd = 0.f, be = 0.f;
-                if (r < n) {
-                    lgd = dl_log_decay(dl_load1<TYPE>(a.alpha + (row0 + r) * a.alpha_stride + (size_t)h * ESZ), a.a[h], a.dt[h]);
-                    be = sz_sigmoid(dl_load1<TYPE>(a.beta + (row0 + r) * a.beta_stride + (size_t)h * ESZ));
-                }
-                G[i] = (double)lgd;
-                sBeta[half][r] = be;
+                for (int b = 1; b < 4; b++) if (r < 16 * b) sB[i][b][r] = expf((float)(sG[i][16 * b] - sG[i][r])) * sRk[r];
             }
-            double sum = G[0] + G[1];
-#pragma unroll
-            for (int o = 1; o < 32; o *= 2) { const double y = __shfl_up_sync(0xffffffffu, sum, o); if (lane >= o) sum += y; }
-            sG[half][2 * lane] = sum - G[1];
-            sG[half][2 * lane + 1] = sum;
         }
-        __syncthreads();
-        // A by columns into shared memory, P as it is taken
+        if (v0 + 2 < ratio) ask_gates(v0 + 2);
+        __syncthreads();                                     // (and nobody needs the rows in shared memory any more)
+        // A into shared memory - below the diagonal's blocks as the products take it, those by columns -, P as it is taken
 #pragma unroll 1
-        for (int i = 0; i < 2 && v0 + i < ratio; i++) {
-            float* const At = (float*)(sm + C::ROWS) + i * (CK * DL_TS);
-            u8* const hp = mine + (size_t)a.kh * C::ROWS + (size_t)head(i) * C::HEAD;
+        for (int i = 0; i < heads; i++) {
+            u8* const af = sm + i * P::HEAD;
+            float* const dg = (float*)(af + P::AF) + warp * 16 * DL_DS;
+            u8* const hp = mine + (size_t)a.kh * C::ROWS + (size_t)head(v0 + i) * C::HEAD;
+            float ra[2], rp[2];
+#pragma unroll
+            for (int u = 0; u < 2; u++) {
+                const int r = 16 * warp + g + 8 * u;
+                ra[u] = sBeta[i][r] * sRk[r];
+                rp[u] = sRq[r] * DL_P;
+            }
 #pragma unroll
             for (int m = 0; m < 8; m++)
                 if (m <= 2 * warp + 1) {
-                    float p[4];
+                    const bool own = m >= 2 * warp;          // on the diagonal
+                    float x[4], p[4];
 #pragma unroll
                     for (int e = 0; e < 4; e++) {
-                        const int r = 16 * warp + g + 8 * (e >> 1), j = 8 * m + 2 * t + (e & 1);
-                        const float f = j <= r ? expf((float)(sG[i][r] - sG[i][j])) * sRk[j] : 0.f;
-                        if (j < r) At[j * DL_AS + r] = sBeta[i][r] * f * sRk[r] * kk[m][e];
-                        p[e] = j <= r ? f * sRq[r] * qk[m][e] * DL_P : 0.f;
+                        const int u = e >> 1, r = 16 * warp + g + 8 * u, j = 8 * m + 2 * t + (e & 1);
+                        float f;
+                        if (own) f = j <= r ? expf((float)(sG[i][r] - sG[i][j])) * sRk[j] : 0.f;
+                        else f = sE[i][r] * sB[i][warp][j];
+                        x[e] = ra[u] * f * kk[m][e];
+                        p[e] = rp[u] * f * qk[m][e];
+                        if (own && j > r) p[e] = 0.f;        // (whatever the product there is)
+                        if (own) dg[(j & 15) * DL_DS + (r & 15)] = x[e];
                     }
-                    if (OUT) {
 #pragma unroll
-                        for (int u = 0; u < 2; u++) {        // rows 8 (2 warp + u) + g: number m & 1 of the tile m / 2
-                            u32 hi, lo;
+                    for (int u = 0; u < 2; u++) {            // rows 8 (2 warp + u) + g: number m & 1 of the tile m / 2
+                        u32 hi, lo;
+                        if (!own) {
+                            dl_split(x[2 * u], x[2 * u + 1], hi, lo);
+                            u32* const at = (u32*)af + ((warp * (warp - 1) + u * warp + m / 2) * 32 + lane) * 2 + (m & 1);
+                            *at = hi;
+                            *(at + P::AF / 8) = lo;
+                        }
+                        if (OUT) {
                             dl_split(p[2 * u], p[2 * u + 1], hi, lo);
                             u32* const at = (u32*)(hp + 2 * DL_FRAG) + ((dl_tile(2 * warp + u) + m / 2) * 32 + lane) * 2 + (m & 1);
                             *at = hi;
@@ -241,52 +307,105 @@ sz_delta_prep_kernel(const DlBatch d, const DlRule a, int idx0, u8* __restrict__
                 }
         }
         __syncthreads();
-        // column j of (I + A)^-1 a thread: its elements from the top down, each one taken from those below it as soon as it is known
-        const bool live = v0 + half < ratio;
-        float x[CK];
-        float* const At = (float*)(sm + C::ROWS) + half * (CK * DL_TS);
-        const int col = part * 32 + lane;
-        if (live) {
+        // the blocks on the diagonal: column `col` of (I + A)^-1 a lane, its elements from the top down, each one taken from those below it as soon as it is known
+        {
+            const int i = tid >> 6, b = (tid >> 4) & 3, col = tid & 15;
+            float* const dg = (float*)(sm + i * P::HEAD + P::AF) + b * 16 * DL_DS;
+            float x[16];
+            if (i < heads) {
 #pragma unroll
-            for (int i = 0; i < CK; i++) x[i] = i == col ? 1.f : 0.f;
+                for (int r = 0; r < 16; r++) x[r] = r == col ? 1.f : 0.f;
 #pragma unroll
-            for (int m = 0; m < CK - 1; m++)
-                if (m >= 32 || part == 0) {                  // (columns from 32 on are nothing above their own row)
+                for (int m = 0; m < 15; m++)
 #pragma unroll
-                    for (int i4 = (m + 1) & ~3; i4 < CK; i4 += 4) {
-                        const float4 w = *(const float4*)(At + m * DL_AS + i4);
+                    for (int r4 = (m + 1) & ~3; r4 < 16; r4 += 4) {
+                        const float4 w = *(const float4*)(dg + m * DL_DS + r4);
                         const float wa[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
-                        for (int e = 0; e < 4; e++) if (i4 + e > m) x[i4 + e] = fmaf(-wa[e], x[m], x[i4 + e]);
+                        for (int e = 0; e < 4; e++) if (r4 + e > m) x[r4 + e] = fmaf(-wa[e], x[m], x[r4 + e]);
                     }
-                }
-        }
-        __syncthreads();                                     // (T takes A's place)
-        if (live) {
-            const float be = sBeta[half][col];
+            }
+            __syncwarp();                                    // (a block is 16 lanes' of one warp)
+            if (i < heads)
 #pragma unroll
-            for (int i = 0; i < CK; i++) At[i * DL_TS + col] = x[i] * be;
+                for (int r = 0; r < 16; r++) dg[r * DL_DS + col] = x[r];      // by rows now
         }
         __syncthreads();
-        if (live) {
-            const int h = head(half);
-            u8* const hp = mine + (size_t)a.kh * C::ROWS + (size_t)h * C::HEAD;
+        if (half < heads) {
+            const u8* const af = sm + half * P::HEAD;
+            const float* const dg = (const float*)(af + P::AF);
+            u8* const hp = mine + (size_t)a.kh * C::ROWS + (size_t)head(v0 + half) * C::HEAD;
+            uint2* const th = (uint2*)hp;
+            uint2* const tl = (uint2*)(hp + DL_FRAG);
+            // T of the blocks on the diagonal: two blocks a warp
 #pragma unroll
-            for (int m = 0; m < 8; m++)
+            for (int k = 0; k < 4; k++) {
+                const int b = 2 * part + (k >> 1), m = 2 * b + (k & 1);
+                const float* w = dg + b * 16 * DL_DS + (8 * (k & 1) + g) * DL_DS + 2 * t;
+                const float* bt = sBeta[half] + 16 * b + 2 * t;
+                uint2 hi, lo;
+                dl_split(w[0] * bt[0], w[1] * bt[1], hi.x, lo.x);
+                dl_split(w[8] * bt[8], w[9] * bt[9], hi.y, lo.y);
+                th[(dl_tile(m) + b) * 32 + lane] = hi;
+                tl[(dl_tile(m) + b) * 32 + lane] = lo;
+            }
+            // the columns of blocks below them: the first, or the second and third
 #pragma unroll
-                for (int k2 = 0; k2 <= m / 2; k2++)
-                    if (((dl_tile(m) + k2) & 1) == part) {
-                        const float* w = At + (8 * m + g) * DL_TS + 16 * k2 + 2 * t;
-                        const float2 w0 = *(const float2*)w, w1 = *(const float2*)(w + 8);
-                        uint2 hi, lo;
-                        dl_split(w0.x, w0.y, hi.x, lo.x);
-                        dl_split(w1.x, w1.y, hi.y, lo.y);
-                        const int at = (dl_tile(m) + k2) * 32 + lane;
-                        ((uint2*)hp)[at] = hi;
-                        ((uint2*)(hp + DL_FRAG))[at] = lo;
+            for (int b = 0; b < 3; b++)
+                if ((b > 0) == (part == 1)) {
+                    u32 xh[3][4], xl[3][4];                  // X_cb^T, c = b ..
+                    {
+                        const float* w = dg + b * 16 * DL_DS + 2 * t * DL_DS + g;
+#pragma unroll
+                        for (int e = 0; e < 4; e++) {
+                            const float* y = w + (e >> 1) * 8 * DL_DS + (e & 1) * 8;
+                            dl_split(y[0], y[DL_DS], xh[0][e], xl[0][e]);
+                        }
                     }
+                    const float* bt = sBeta[half] + 16 * b + g;
+                    const float be0 = -bt[0], be1 = -bt[8];
+#pragma unroll
+                    for (int ab = b + 1; ab < 4; ab++) {
+                        float y[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}}, z[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+#pragma unroll
+                        for (int cb = b; cb < ab; cb++)
+#pragma unroll
+                            for (int u = 0; u < 2; u++) {
+                                const uint2* at = (const uint2*)af + (ab * (ab - 1) + u * ab + cb) * 32 + lane;
+                                const uint2 wh = at[0], wl = at[P::AF / 16];
+                                dl_mma(y[u], xh[cb - b], wh.x, wh.y);
+                                dl_mma(y[u], xl[cb - b], wh.x, wh.y);
+                                dl_mma(y[u], xh[cb - b], wl.x, wl.y);
+                            }
+                        u32 yh[4], yl[4];
+#pragma unroll
+                        for (int e = 0; e < 4; e++) dl_split(y[e >> 1][2 * (e & 1)], y[e >> 1][2 * (e & 1) + 1], yh[e], yl[e]);
+#pragma unroll
+                        for (int u = 0; u < 2; u++) {
+                            const float* w = dg + ab * 16 * DL_DS + (8 * u + g) * DL_DS + 2 * t;
+                            u32 wh[2], wl[2];
+                            dl_split(w[0], w[1], wh[0], wl[0]);
+                            dl_split(w[8], w[9], wh[1], wl[1]);
+                            dl_mma(z[u], yh, wh[0], wh[1]);
+                            dl_mma(z[u], yl, wh[0], wh[1]);
+                            dl_mma(z[u], yh, wl[0], wl[1]);
+                        }
+                        if (ab < 3)
+#pragma unroll
+                            for (int e = 0; e < 4; e++) dl_split(-z[e >> 1][2 * (e & 1)], -z[e >> 1][2 * (e & 1) + 1], xh[ab - b][e], xl[ab - b][e]);
+#pragma unroll
+                        for (int u = 0; u < 2; u++) {        // rows 8 (2 ab + u) .., columns 16 b ..: turned around, times beta of their column
+                            u32 h0, l0, h1, l1;
+                            dl_split(z[u][0] * be0, z[u][1] * be0, h0, l0);
+                            dl_split(z[u][2] * be1, z[u][3] * be1, h1, l1);
+                            const int at = (dl_tile(2 * ab + u) + b) * 32 + lane;
+                            th[at] = make_uint2(dl_turn(h0), dl_turn(h1));
+                            tl[at] = make_uint2(dl_turn(l0), dl_turn(l1));
+                        }
+                    }
+                }
             DlScalars* const sc = (DlScalars*)(hp + (C::FULL ? 4 : 3) * DL_FRAG);
-            const int r = col;
+            const int r = 32 * part + lane;
             const double G = sG[half][r], GC = sG[half][CK - 1];
             const float eg = expf((float)G);
             sc->gr[r] = eg * sRk[r];
@@ -294,7 +413,11 @@ sz_delta_prep_kernel(const DlBatch d, const DlRule a, int idx0, u8* __restrict__
             sc->wj[r] = expf((float)(GC - G)) * sRk[r];
             if (r == 0) sc->gc = expf((float)GC);
         }
-        __syncthreads();                                     // (the next pair's gates)
+        if (v0 + 2 < ratio) {
+            __syncthreads();                                 // (the next pair's gates take these' place)
+            sum_gates(v0 + 2);
+            __syncthreads();
+        }
     }
 }
 
@@ -781,7 +904,7 @@ template <int D, int TYPE, int NG, bool OUT>
 int dl_chunk_go(const DlBatch& b, const DlRule& r, int longest, int64_t total, int64_t per, uint64_t scratch, cudaStream_t st) {
     using P = DlPrep<D, TYPE>;
     using M = DlMain<D, TYPE, NG, OUT>;
-    static_assert(M::SMEM <= 227 * 1024 && P::SMEM <= 113 * 1024, "");
+    static_assert(M::SMEM <= 227 * 1024 && P::SMEM <= 72 * 1024, "");
     const auto prep = sz_delta_prep_kernel<D, TYPE, OUT>;
     const auto chain = sz_delta_chunk_kernel<D, TYPE, NG, OUT>;
     int rc = sz_allow_smem((const void*)prep, (int)P::SMEM);
