@@ -26,17 +26,18 @@ constexpr int DL_FRAG = DL_TILES * 32 * 8;               // bytes of a triangle 
 constexpr float DL_P = 1024.f;                           // P's elements are at most 1 / sqrt(d): times this they keep their 22 bits
 constexpr int64_t DL_SLAB = 96ll << 20;                  // scratch that a pass over chunks may take (what the first kernel leaves is in L2 for the second)
 
-struct DlScalars { float gr[CK], gq[CK], wj[CK], gc, pad[15]; };      // e^G rho_k, e^G rho_q, e^(G_C - G_j) rho_k; e^G_C
+struct DlScalars { float gr[CK], wj[CK], gc, pad[15]; };              // e^G rho_k, e^(G_C - G_j) rho_k; e^G_C
 
 template <int D, int TYPE> struct DlChunk {
     static constexpr int NK = TYPE == SZ_TYPE_F32 ? 2 : 1;                // f16 numbers of an element of k and q
     static constexpr bool FULL = TYPE != SZ_TYPE_BF16;                    // outputs' products with both numbers of a factor
     static constexpr int TILE = CK * D * 2, ROWS = 2 * NK * TILE;         // a key head's rows: k (high, low), q (high, low)
-    static constexpr int HEAD = (FULL ? 4 : 3) * DL_FRAG + (int)sizeof(DlScalars);      // a value head's T (high, low), P (high, low), scalars
+    // a value head's T (high, low) and scalars, for the chain; P (high, low) and e^G rho_q, for the outputs
+    static constexpr int HA = 2 * DL_FRAG + (int)sizeof(DlScalars), HB = (FULL ? 2 : 1) * DL_FRAG + CK * 4, HEAD = HA + HB;
 };
 int64_t dl_chunk_one(int d, int kh, int vh, int io_type) {
     const int nk = io_type == SZ_TYPE_F32 ? 2 : 1;
-    return (int64_t)kh * 2 * nk * CK * d * 2 + (int64_t)vh * ((io_type == SZ_TYPE_BF16 ? 3 : 4) * DL_FRAG + (int)sizeof(DlScalars));
+    return (int64_t)kh * 2 * nk * CK * d * 2 + (int64_t)vh * ((io_type == SZ_TYPE_BF16 ? 3 : 4) * DL_FRAG + CK * 4 + (int)sizeof(DlScalars));
 }
 
 // The sequences of many rows, in order: the y-th of them (y >= 0), or the one whose chunks have index idx.  Chunk c of a sequence has index
@@ -299,7 +300,7 @@ sz_delta_prep_kernel(const DlBatch d, const DlRule a, int idx0, u8* __restrict__
                         }
                         if (OUT) {
                             dl_split(p[2 * u], p[2 * u + 1], hi, lo);
-                            u32* const at = (u32*)(hp + 2 * DL_FRAG) + ((dl_tile(2 * warp + u) + m / 2) * 32 + lane) * 2 + (m & 1);
+                            u32* const at = (u32*)(hp + C::HA) + ((dl_tile(2 * warp + u) + m / 2) * 32 + lane) * 2 + (m & 1);
                             *at = hi;
                             if (C::FULL) *(at + DL_FRAG / 4) = lo;
                         }
@@ -404,12 +405,12 @@ sz_delta_prep_kernel(const DlBatch d, const DlRule a, int idx0, u8* __restrict__
                         }
                     }
                 }
-            DlScalars* const sc = (DlScalars*)(hp + (C::FULL ? 4 : 3) * DL_FRAG);
+            DlScalars* const sc = (DlScalars*)(hp + 2 * DL_FRAG);
             const int r = 32 * part + lane;
             const double G = sG[half][r], GC = sG[half][CK - 1];
             const float eg = expf((float)G);
             sc->gr[r] = eg * sRk[r];
-            if (OUT) sc->gq[r] = eg * sRq[r];
+            if (OUT) ((float*)(hp + C::HEAD))[r - CK] = eg * sRq[r];
             sc->wj[r] = expf((float)(GC - G)) * sRk[r];
             if (r == 0) sc->gc = expf((float)GC);
         }
@@ -428,16 +429,18 @@ sz_delta_prep_kernel(const DlBatch d, const DlRule a, int idx0, u8* __restrict__
 template <int D, int TYPE, int NG, bool OUT> struct DlMain {
     using C = DlChunk<D, TYPE>;
     static constexpr int ESZ = DlIo<TYPE>::ESZ, NQ = D / 64, NC = NG * NQ, CS = D / 16 / NG;      // warps on one 16 dimensions; of the chain; blocks of a head
-    static constexpr int CONSUMERS = OUT ? 2 * NC : NC, NTH = 32 * (CONSUMERS + 1);
-    static constexpr int VS = 16 * NG * ESZ + 16;                                          // bytes between rows of v and z in shared memory
+    static constexpr int NO = OUT ? 2 : 0, NTH = 32 * (NC + NG * NO + 1);                         // warps on the outputs of 16 dimensions, half of the rows each
     static constexpr bool STAGED = TYPE != SZ_TYPE_F32;                                    // gates and outputs through shared memory (f32: whole sectors a warp without)
-    static constexpr int STAGE = C::ROWS + C::HEAD + (STAGED ? 2 : 1) * CK * VS, STAGES = D == 128 && TYPE == SZ_TYPE_F32 ? 1 : 2;
+    static constexpr int VS = 16 * NG * ESZ + 16;                                          // bytes between rows of v and z in shared memory
+    // a chunk's operands in two rings, of the chain (k, T, scalars, v) and of the outputs (q, P, e^G, z), each as deep as there is room
+    static constexpr int A = C::ROWS / 2 + C::HA + CK * VS, B = OUT ? C::ROWS / 2 + C::HB + (STAGED ? CK * VS : 0) : 0;
+    static constexpr int SA = D == 128 ? (TYPE == SZ_TYPE_BF16 ? 3 : TYPE == SZ_TYPE_F16 ? 2 : 1) : (TYPE == SZ_TYPE_F32 ? 2 : 3), SB = D == 128 && TYPE == SZ_TYPE_F32 ? 1 : 2;
     static constexpr int XB = NQ == 2 ? 2 * 8 * 32 * 16 : 0;                               // what a chain's warp gives its partner (two chunks' turns)
     static constexpr int FB = OUT ? (C::FULL ? 2 : 1) * 4 * 32 * 16 : 0;                   // a product's factor of 16 x 64 in f16: S of a warp, D of a group; two turns of each
-    static constexpr int OS = 16 * ESZ + 16, OB = OUT && STAGED ? CK / NQ * OS : 0;                  // a warp's outputs on their way
+    static constexpr int OS = 16 * ESZ + 16, OB = OUT && STAGED ? CK / 2 * OS : 0;         // a warp's outputs on their way
     static constexpr int SSQ = OUT ? 4 * CS * NG * CK * 4 : 0;                             // [turn of four][block][group][row]
-    static constexpr int BARS = 2 * STAGES + 6 * NG + 4;
-    static constexpr size_t SMEM = (size_t)STAGES * STAGE + NC * (XB + 2 * FB + OB) + NG * 2 * FB + SSQ + BARS * 8 + 2 * (NC + NG) * 4;
+    static constexpr int BARS = 2 * SA + 2 * SB + 6 * NG + 4;
+    static constexpr size_t SMEM = (size_t)SA * A + (size_t)SB * B + NC * (XB + 2 * FB) + NG * (2 * FB + NO * OB) + SSQ + BARS * 8 + 2 * (NC + NG) * 4;
 };
 
 template <int D, int TYPE, int NG, bool OUT>
@@ -445,26 +448,31 @@ __global__ void __launch_bounds__(DlMain<D, TYPE, NG, OUT>::NTH, 1)
 sz_delta_chunk_kernel(const DlBatch d, const DlRule a, int idx0, int idx1, const u8* __restrict__ scratch, long long one) {
     using M = DlMain<D, TYPE, NG, OUT>;
     using C = DlChunk<D, TYPE>;
-    constexpr int ESZ = M::ESZ, NQ = M::NQ, NK = C::NK, NC = M::NC, CS = M::CS, ST = M::STAGES, OT = 8 / NQ;      // OT: 8-row tiles whose outputs a warp finishes
+    constexpr int ESZ = M::ESZ, NQ = M::NQ, NK = C::NK, NC = M::NC, CS = M::CS, SA = M::SA, SB = M::SB, NO = M::NO, OT = 4;      // OT: 8-row tiles whose outputs a warp finishes
     constexpr int FP = C::FULL ? 2 : 1;
     extern __shared__ __align__(16) u8 sm[];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
-    const int w = warp < NC ? warp : warp - NC, p = w / NQ, q = w % NQ;
+    const int w = warp < NC ? warp : warp - NC, p = warp < NC ? w / NQ : w / 2, q = warp < NC ? w % NQ : w % 2;      // (an output's warp: q is its half of the rows)
     const int h = blockIdx.x / CS, rank = blockIdx.x % CS, kx = a.grouped ? h / (a.vh / a.kh) : h % a.kh;
-    u8* const xb = sm + ST * M::STAGE;
+    u8* const rb = sm + SA * M::A;
+    u8* const xb = rb + SB * M::B;
     uint4* const sf = (uint4*)(xb + NC * M::XB);                          // [turn][chain's warp][number][16 key dimensions][lane]
     uint4* const df = (uint4*)((u8*)sf + NC * 2 * M::FB);                 // [turn][group][number][16 rows][lane]
-    u8* const ob = (u8*)df + NG * 2 * M::FB + (warp - NC) * M::OB;
-    float* const ssq = (float*)((u8*)df + NG * 2 * M::FB + NC * M::OB);
+    u8* const ob = (u8*)df + NG * 2 * M::FB + w * M::OB;
+    float* const ssq = (float*)((u8*)df + NG * (2 * M::FB + NO * M::OB));
     u64* const bars = (u64*)((u8*)ssq + M::SSQ);
-    u64 *const full = bars, *const empty = full + ST, *const s_there = empty + ST, *const d_there = s_there + 2 * NG, *const s_free = d_there + 2 * NG, *const sq_there = s_free + 2 * NG;
+    u64 *const fulla = bars, *const emptya = fulla + SA, *const fullb = emptya + SA, *const emptyb = fullb + SB, *const s_there = emptyb + SB, *const d_there = s_there + 2 * NG,
+        *const s_free = d_there + 2 * NG, *const sq_there = s_free + 2 * NG;
     float* const s_unit = (float*)(bars + M::BARS);                       // [turn][chain's warp], then [turn][group]: what a unit of S, of D is
     float* const d_unit = s_unit + 2 * NC;
     const bool norm = OUT && a.norm != nullptr, joined = norm && CS > 1;
     if (tid == 0) {
-        for (int i = 0; i < ST; i++) { sz_mbar_init(&full[i], 1 + 32); sz_mbar_init(&empty[i], M::CONSUMERS); }
-        for (int i = 0; i < 2 * NG; i++) { sz_mbar_init(&s_there[i], NQ); sz_mbar_init(&d_there[i], NQ); sz_mbar_init(&s_free[i], NQ); }
-        for (int i = 0; i < 4; i++) sz_mbar_init(&sq_there[i], CS * NC);
+        for (int i = 0; i < SA; i++) { sz_mbar_init(&fulla[i], 1 + 32); sz_mbar_init(&emptya[i], NC); }
+        if (OUT) {
+            for (int i = 0; i < SB; i++) { sz_mbar_init(&fullb[i], 1 + 32); sz_mbar_init(&emptyb[i], NG * NO); }
+            for (int i = 0; i < 2 * NG; i++) { sz_mbar_init(&s_there[i], NQ); sz_mbar_init(&d_there[i], NQ); sz_mbar_init(&s_free[i], NO); }
+            for (int i = 0; i < 4; i++) sz_mbar_init(&sq_there[i], CS * NG * NO);
+        }
         sz_mbar_fence_init();
     }
     sz_pdl_wait();
@@ -480,7 +488,12 @@ sz_delta_chunk_kernel(const DlBatch d, const DlRule a, int idx0, int idx1, const
     const int dv = (rank * NG + p) * 16;                                  // the warp's value dimensions
     if (joined) sz_cluster_sync(); else __syncthreads();                  // (mbarriers are ready, in all blocks of the head)
     bool dead = false;
-    auto wait = [&](u64* bar, int turn) { if (!dead && !sz_mbar_wait_warp(bar, turn & 1)) { dead = true; if (lane == 0) atomicOr(d.err, DL_E_WAIT); } };
+    auto wait = [&](u64* bar, int turn) {                                 // (a look first: what is there already costs less than the wait that may sleep)
+        u32 ok;
+        asm volatile("{ .reg .pred p; mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2; selp.u32 %0, 1, 0, p; }" : "=r"(ok) : "r"(sz_smem_addr(bar)), "r"((u32)turn & 1) : "memory");
+        if (__all_sync(0xffffffffu, ok)) return;
+        if (!dead && !sz_mbar_wait_warp(bar, turn & 1)) { dead = true; if (lane == 0) atomicOr(d.err, DL_E_WAIT); }
+    };
     auto arrive = [&](u64* bar) { __syncwarp(); if (lane == 0) sz_mbar_arrive(bar); };
     // 16 value dimensions of two 8-row tiles m, m + 1 of a tile of rows, transposed: dimensions g, g + 8 of rows 8 m + 2 t, + 1
     auto turned = [&](const u8* tile, int m, float* f) {
@@ -495,36 +508,58 @@ sz_delta_chunk_kernel(const DlBatch d, const DlRule a, int idx0, int idx1, const
             dl_unpack<TYPE, 8>(r, f);
         }
     };
-    if (warp == M::CONSUMERS) {
+    if (warp == NC + NG * NO) {
         // ---- copies
         if (lane == 0) asm volatile("fence.proxy.async;" ::: "memory");   // (they read what the kernel before has written)
         // (a chunk's operands in two pieces; v and z row by row in 16 bytes a lane: a copy of a row at a time by the TMA engine takes 58 cycles, 7,500 a chunk)
         constexpr int PIECES = NG * ESZ, STEP = 32 / PIECES;              // of 16 bytes, a row's; rows the warp takes at once
         const u32 col = (u32)(h * D + rank * NG * 16) * ESZ + 16 * (lane % PIECES);
-        for (int i = 0; i < nc; i++) {
-            const int c = c0 + i, slot = i % ST, n = min(CK, s.n - c * CK);
-            u8* const st = sm + slot * M::STAGE;
-            if (i >= ST) wait(&empty[slot], i / ST - 1);
-            if (lane == 0) {
-                const u8* src = scratch + (size_t)(lg.base + c - idx0) * one;
-                sz_mbar_expect_tx(&full[slot], (OUT ? C::ROWS : C::ROWS / 2) + C::HEAD);
-                sz_bulk_g2s(st, src + (size_t)kx * C::ROWS, OUT ? C::ROWS : C::ROWS / 2, &full[slot]);
-                sz_bulk_g2s(st + C::ROWS, src + (size_t)a.kh * C::ROWS + (size_t)h * C::HEAD, C::HEAD, &full[slot]);
-            }
-            __syncwarp();
-            const u32 to = sz_smem_addr(st + C::ROWS + C::HEAD + (lane / PIECES) * M::VS + 16 * (lane % PIECES));
+        auto tile = [&](u8* at, const u8* src, long long stride, int c) { // 16 NG dimensions of a chunk's rows (those behind the last are zeros, and not read)
+            const int n = min(CK, s.n - c * CK);
+            const u32 to = sz_smem_addr(at + (lane / PIECES) * M::VS + 16 * (lane % PIECES));
             const size_t row0 = (size_t)s.r0 + (size_t)c * CK;
 #pragma unroll 4
-            for (int k = 0; k < CK / STEP; k++) {                         // (rows behind the last are zeros, and not read)
+            for (int k = 0; k < CK / STEP; k++) {
                 const int r = k * STEP + lane / PIECES;
-                const size_t row = row0 + (r < n ? r : 0);
-                const u32 there = r < n ? 16 : 0;
-                asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to + k * STEP * M::VS), "l"(a.v + row * a.v_stride + col), "r"(there) : "memory");
-                if (M::STAGED && norm) asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to + (k * STEP + CK) * M::VS), "l"(a.z + row * a.z_stride + col), "r"(there) : "memory");
+                asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to + k * STEP * M::VS), "l"(src + (row0 + (r < n ? r : 0)) * stride + col), "r"(r < n ? 16 : 0) : "memory");
             }
-            asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(sz_smem_addr(&full[slot])) : "memory");
+        };
+        auto both = [&](u8* st, const u8* x, int nx, const u8* y, int ny, u64* full) {
+            if (lane == 0) {
+                sz_mbar_expect_tx(full, nx + ny);
+                sz_bulk_g2s(st, x, nx, full);
+                sz_bulk_g2s(st + nx, y, ny, full);
+            }
+            __syncwarp();
+        };
+        auto copy_a = [&](int i) {
+            const int slot = i % SA;
+            u8* const st = sm + slot * M::A;
+            const u8* const src = scratch + (size_t)(lg.base + c0 + i - idx0) * one;
+            if (i >= SA) wait(&emptya[slot], i / SA - 1);
+            both(st, src + (size_t)kx * C::ROWS, C::ROWS / 2, src + (size_t)a.kh * C::ROWS + (size_t)h * C::HEAD, C::HA, &fulla[slot]);
+            tile(st + C::ROWS / 2 + C::HA, a.v, a.v_stride, c0 + i);
+            asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(sz_smem_addr(&fulla[slot])) : "memory");
+        };
+        auto copy_b = [&](int i) {
+            const int slot = i % SB;
+            u8* const st = rb + slot * M::B;
+            const u8* const src = scratch + (size_t)(lg.base + c0 + i - idx0) * one;
+            if (i >= SB) wait(&emptyb[slot], i / SB - 1);
+            both(st, src + (size_t)kx * C::ROWS + C::ROWS / 2, C::ROWS / 2, src + (size_t)a.kh * C::ROWS + (size_t)h * C::HEAD + C::HA, C::HB, &fullb[slot]);
+            if (M::STAGED && norm) tile(st + C::ROWS / 2 + C::HB, a.z, a.z_stride, c0 + i);
+            asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(sz_smem_addr(&fullb[slot])) : "memory");
+        };
+        // (the chain's a chunk ahead where its ring is the deeper one)
+        constexpr int LEAD = SA > SB ? 1 : 0;
+        if (LEAD && nc > 0) copy_a(0);
+        for (int i = 0; i < nc; i++) {
+            if (!LEAD) copy_a(i);
+            if (OUT) copy_b(i);
+            if (LEAD && i + 1 < nc) copy_a(i + 1);
         }
-        for (int i = max(0, nc - ST); i < nc; i++) wait(&full[i % ST], i / ST);      // (nothing is under way when the block ends, whoever gave up)
+        for (int i = max(0, nc - SA); i < nc; i++) wait(&fulla[i % SA], i / SA);     // (nothing is under way when the block ends, whoever gave up)
+        if (OUT) for (int i = max(0, nc - SB); i < nc; i++) wait(&fullb[i % SB], i / SB);
         return;
     }
     if (warp < NC) {
@@ -549,11 +584,11 @@ sz_delta_chunk_kernel(const DlBatch d, const DlRule a, int idx0, int idx1, const
         };
 #pragma unroll 1
         for (int i = 0; i < nc; i++) {
-            const int slot = i % ST, turn = i & 1;
-            const u8* const st = sm + slot * M::STAGE;
+            const int slot = i % SA, turn = i & 1;
+            const u8* const st = sm + slot * M::A;
             const u32 sk = sz_smem_addr(st);
-            const u8* const hp = st + C::ROWS;
-            const DlScalars* const sc = (const DlScalars*)(hp + (C::FULL ? 4 : 3) * DL_FRAG);
+            const u8* const hp = st + C::ROWS / 2;
+            const DlScalars* const sc = (const DlScalars*)(hp + 2 * DL_FRAG);
             {                                                             // the state into f16's range
                 const int top = exponent(S), ex = top - 127;
                 if (top != 0 && top != 255 && (ex > 13 || ex < 4)) {
@@ -564,7 +599,7 @@ sz_delta_chunk_kernel(const DlBatch d, const DlRule a, int idx0, int idx1, const
                 }
             }
             if (OUT && i >= 2) wait(&s_free[turn * NG + p], i / 2 - 1);   // (the outputs have taken what lies there)
-            wait(&full[slot], i / ST);
+            wait(&fulla[slot], i / SA);
             // ---- (K S)^T: dimensions x rows.  (Terms one after the other over all rows, so that no product waits for the one before it.)
             float X[8][4];
 #pragma unroll
@@ -613,7 +648,7 @@ sz_delta_chunk_kernel(const DlBatch d, const DlRule a, int idx0, int idx1, const
 #pragma unroll
             for (int m = 0; m < 8; m += 2) {
                 float v[8];
-                turned(st + C::ROWS + C::HEAD, m, v);
+                turned(hp + C::HA, m, v);
 #pragma unroll
                 for (int u = 0; u < 2; u++) {
                     const float2 gr = *(const float2*)(sc->gr + 8 * (m + u) + 2 * t);
@@ -699,7 +734,7 @@ sz_delta_chunk_kernel(const DlBatch d, const DlRule a, int idx0, int idx1, const
                 times(lo);
                 if (NK == 2) { load(sk + C::TILE); times(hi); }
             }
-            arrive(&empty[slot]);
+            arrive(&emptya[slot]);
         }
         float* to = (float*)(a.state + (size_t)s.to * a.state_stride) + ((size_t)h * D + 64 * q + 2 * t) * D + dv + g;
         const float f0 = dl_pow2(es / 2), f1 = dl_pow2(es - es / 2);      // (in two steps: 2^es alone may be out of range)
@@ -711,7 +746,7 @@ sz_delta_chunk_kernel(const DlBatch d, const DlRule a, int idx0, int idx1, const
     }
     if constexpr (OUT) {
         // ---- the outputs: e^G Q S + P D, of OT 8-row tiles a warp (of pairs of like work)
-        auto mine = [&](int i) { return NQ == 1 ? i : q == 0 ? (i < 2 ? i : i + 4) : i + 2; };
+        auto mine = [&](int i) { return q == 0 ? (i < 2 ? i : i + 4) : i + 2; };
         float O[4 * OT];
         float nw[2] = {0.f, 0.f};
         if (norm) { nw[0] = a.norm[dv + g]; nw[1] = a.norm[dv + g + 8]; }
@@ -766,12 +801,12 @@ sz_delta_chunk_kernel(const DlBatch d, const DlRule a, int idx0, int idx1, const
         };
 #pragma unroll 1
         for (int k = 0; k < nc; k++) {
-            const int slot = k % ST, turn = k & 1;
-            const u8* const st = sm + slot * M::STAGE;
-            const u32 sq = sz_smem_addr(st) + NK * C::TILE;
-            const u8* const hp = st + C::ROWS;
-            const DlScalars* const sc = (const DlScalars*)(hp + (C::FULL ? 4 : 3) * DL_FRAG);
-            const u8* const zt = st + C::ROWS + C::HEAD + CK * M::VS;
+            const int slot = k % SB, turn = k & 1;
+            const u8* const st = rb + slot * M::B;
+            const u32 sq = sz_smem_addr(st);
+            const u8* const hp = st + C::ROWS / 2;
+            const float* const sc = (const float*)(hp + (C::FULL ? 2 : 1) * DL_FRAG);
+            const u8* const zt = hp + C::HB;
             float zd[M::STAGED ? 1 : 4 * OT];                             // (f32: the gates, asked for early)
             if (!M::STAGED && norm) {
                 const int n = min(CK, s.n - (c0 + k) * CK);
@@ -783,7 +818,7 @@ sz_delta_chunk_kernel(const DlBatch d, const DlRule a, int idx0, int idx1, const
                         zd[M::STAGED ? 0 : 4 * i + e] = row < n ? *(const float*)(a.z + ((size_t)s.r0 + (size_t)(c0 + k) * CK + row) * a.z_stride + (size_t)(h * D + dv + g + 8 * (e >> 1)) * 4) : 0.f;
                     }
             }
-            wait(&full[slot], k / ST);
+            wait(&fullb[slot], k / SB);
             wait(&s_there[turn * NG + p], k / 2);
             float Y[NQ][OT][4];
 #pragma unroll
@@ -838,7 +873,7 @@ sz_delta_chunk_kernel(const DlBatch d, const DlRule a, int idx0, int idx1, const
 #pragma unroll
                     for (int i = 0; i < OT; i++)
                         if (ks <= mine(i) / 2) {
-                            const uint2 f = ((const uint2*)(hp + (part == 2 ? 3 : 2) * DL_FRAG))[(dl_tile(mine(i)) + ks) * 32 + lane];
+                            const uint2 f = ((const uint2*)(hp + (part == 2 ? 1 : 0) * DL_FRAG))[(dl_tile(mine(i)) + ks) * 32 + lane];
                             dl_mma(acc[i], part == 1 ? lo : hi, f.x, f.y);
                         }
             }
@@ -847,7 +882,7 @@ sz_delta_chunk_kernel(const DlBatch d, const DlRule a, int idx0, int idx1, const
             float N[4 * OT];
 #pragma unroll
             for (int i = 0; i < OT; i++) {
-                const float2 gq = *(const float2*)(sc->gq + 8 * mine(i) + 2 * t);
+                const float2 gq = *(const float2*)(sc + 8 * mine(i) + 2 * t);
 #pragma unroll
                 for (int e = 0; e < 4; e++) N[4 * i + e] = fmaf(e & 1 ? gq.y : gq.x, Y[0][i][e], acc[i][e] * tw);
             }
@@ -887,7 +922,7 @@ sz_delta_chunk_kernel(const DlBatch d, const DlRule a, int idx0, int idx1, const
                     for (int e = 0; e < 8; e++) N[4 * i + e] *= nw[(e >> 1) & 1] * dl_sigmoid<TYPE>(z[e]);
                 }
             }
-            arrive(&empty[slot]);
+            arrive(&emptyb[slot]);
             if (norm && k > 0) { wait_sums(k - 1); finish(k - 1); }       // the chunk before
 #pragma unroll
             for (int e = 0; e < 4 * OT; e++) O[e] = N[e];
