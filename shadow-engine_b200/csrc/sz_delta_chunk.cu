@@ -423,13 +423,14 @@ sz_delta_prep_kernel(const DlBatch d, const DlRule a, int idx0, u8* __restrict__
 }
 
 // ---- the chain over a sequence's chunks --------------------------------------------------------------------------------------------------------
-// A block has three kinds of warps, which meet at mbarriers only: NC of the chain (16 value dimensions and 64 key dimensions each), as many for the outputs, which
-// take S and D as the chain's products had them (f16, from shared memory), and one that copies the chunks' operands into a ring.  The blocks of a head form a
-// cluster: where outputs are normed, a row's sums of squares go to all of them, and a chunk's outputs leave while the next one's are made.
+// A block has four kinds of warps, which meet at mbarriers only: NC of the chain (16 value dimensions and 64 key dimensions each); two for the outputs of every 16
+// dimensions, which take S and D as the chain's products had them (f16, from shared memory); one that copies the chunks' operands into two rings; and one for the
+// outputs' norms.  The blocks of a head form a cluster: a row's sums of squares go to all of them, and a chunk's outputs leave while the next one's are made.
+// (The releases that this takes wait for every store of their thread, 1,300 cycles a chunk where the outputs' warps made them.)
 template <int D, int TYPE, int NG, bool OUT> struct DlMain {
     using C = DlChunk<D, TYPE>;
     static constexpr int ESZ = DlIo<TYPE>::ESZ, NQ = D / 64, NC = NG * NQ, CS = D / 16 / NG;      // warps on one 16 dimensions; of the chain; blocks of a head
-    static constexpr int NO = OUT ? 2 : 0, NTH = 32 * (NC + NG * NO + 1);                         // warps on the outputs of 16 dimensions, half of the rows each
+    static constexpr int NO = OUT ? 2 : 0, NTH = 32 * (NC + NG * NO + (OUT ? 2 : 1));             // warps on the outputs of 16 dimensions, half of the rows each; of copies, of norms
     static constexpr bool STAGED = TYPE != SZ_TYPE_F32;                                    // gates and outputs through shared memory (f32: whole sectors a warp without)
     static constexpr int VS = 16 * NG * ESZ + 16;                                          // bytes between rows of v and z in shared memory
     // a chunk's operands in two rings, of the chain (k, T, scalars, v) and of the outputs (q, P, e^G, z), each as deep as there is room
@@ -438,8 +439,8 @@ template <int D, int TYPE, int NG, bool OUT> struct DlMain {
     static constexpr int XB = NQ == 2 ? 2 * 8 * 32 * 16 : 0;                               // what a chain's warp gives its partner (two chunks' turns)
     static constexpr int FB = OUT ? (C::FULL ? 2 : 1) * 4 * 32 * 16 : 0;                   // a product's factor of 16 x 64 in f16: S of a warp, D of a group; two turns of each
     static constexpr int OS = 16 * ESZ + 16, OB = OUT && STAGED ? CK / 2 * OS : 0;         // a warp's outputs on their way
-    static constexpr int SSQ = OUT ? 4 * CS * NG * CK * 4 : 0;                             // [turn of four][block][group][row]
-    static constexpr int BARS = 2 * SA + 2 * SB + 6 * NG + 4;
+    static constexpr int SSQ = OUT ? 2 * (NG + CS + 1) * CK * 4 : 0;                       // a row's sums of squares and its norm's factor, two turns: [group], [block], the factor
+    static constexpr int BARS = 2 * SA + 2 * SB + 6 * NG + 6;
     static constexpr size_t SMEM = (size_t)SA * A + (size_t)SB * B + NC * (XB + 2 * FB) + NG * (2 * FB + NO * OB) + SSQ + BARS * 8 + 2 * (NC + NG) * 4;
 };
 
@@ -462,7 +463,8 @@ sz_delta_chunk_kernel(const DlBatch d, const DlRule a, int idx0, int idx1, const
     float* const ssq = (float*)((u8*)df + NG * (2 * M::FB + NO * M::OB));
     u64* const bars = (u64*)((u8*)ssq + M::SSQ);
     u64 *const fulla = bars, *const emptya = fulla + SA, *const fullb = emptya + SA, *const emptyb = fullb + SB, *const s_there = emptyb + SB, *const d_there = s_there + 2 * NG,
-        *const s_free = d_there + 2 * NG, *const sq_there = s_free + 2 * NG;
+        *const s_free = d_there + 2 * NG, *const sums_there = s_free + 2 * NG, *const all_there = sums_there + 2, *const factor_there = all_there + 2;
+    float *const all = ssq + 2 * NG * CK, *const factor = all + 2 * CS * CK;
     float* const s_unit = (float*)(bars + M::BARS);                       // [turn][chain's warp], then [turn][group]: what a unit of S, of D is
     float* const d_unit = s_unit + 2 * NC;
     const bool norm = OUT && a.norm != nullptr, joined = norm && CS > 1;
@@ -471,7 +473,7 @@ sz_delta_chunk_kernel(const DlBatch d, const DlRule a, int idx0, int idx1, const
         if (OUT) {
             for (int i = 0; i < SB; i++) { sz_mbar_init(&fullb[i], 1 + 32); sz_mbar_init(&emptyb[i], NG * NO); }
             for (int i = 0; i < 2 * NG; i++) { sz_mbar_init(&s_there[i], NQ); sz_mbar_init(&d_there[i], NQ); sz_mbar_init(&s_free[i], NO); }
-            for (int i = 0; i < 4; i++) sz_mbar_init(&sq_there[i], CS * NG * NO);
+            for (int i = 0; i < 2; i++) { sz_mbar_init(&sums_there[i], NG * NO); sz_mbar_init(&all_there[i], CS); sz_mbar_init(&factor_there[i], 1); }
         }
         sz_mbar_fence_init();
     }
@@ -560,6 +562,46 @@ sz_delta_chunk_kernel(const DlBatch d, const DlRule a, int idx0, int idx1, const
         }
         for (int i = max(0, nc - SA); i < nc; i++) wait(&fulla[i % SA], i / SA);     // (nothing is under way when the block ends, whoever gave up)
         if (OUT) for (int i = max(0, nc - SB); i < nc; i++) wait(&fullb[i % SB], i / SB);
+        return;
+    }
+    if (OUT && warp == NC + NG * NO + 1) {
+        // ---- the outputs' norms: a row's sums of squares over this block's groups go to all blocks of the head, theirs come here, and what divides the row is
+        // ready for the warps that finish it.  Two turns are enough: a warp sends its k-th sums after it has used the k - 2nd factor, and a block its k-th after it has
+        // all of the k - 1st, whose senders had read the k - 2nd.
+        if (!norm) return;
+        for (int k = 0; k < nc; k++) {
+            const int turn = k & 1;
+            wait(&sums_there[turn], k / 2);
+            float2 sum = make_float2(0.f, 0.f);
+#pragma unroll
+            for (int j = 0; j < NG; j++) { const float2 y = *(const float2*)(ssq + (turn * NG + j) * CK + 2 * lane); sum.x += y.x; sum.y += y.y; }
+            if constexpr (CS > 1) {
+#pragma unroll
+                for (int r = 0; r < CS; r++) {
+                    u32 there;
+                    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(there) : "r"(sz_smem_addr(all + (turn * CS + rank) * CK + 2 * lane)), "r"(r));
+                    asm volatile("st.shared::cluster.v2.f32 [%0], {%1, %2};" ::"r"(there), "f"(sum.x), "f"(sum.y) : "memory");
+                }
+                __syncwarp();
+                if (lane < CS) {
+                    u32 bar;
+                    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(bar) : "r"(sz_smem_addr(&all_there[turn])), "r"(lane));
+                    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+                }
+                bool there = dead;                                        // (from other blocks' stores: acquired at the cluster's scope)
+                for (u32 i = 0; !there && i < 20000000u; i++) {
+                    u32 ok;
+                    asm volatile("{ .reg .pred p; mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2; selp.u32 %0, 1, 0, p; }" : "=r"(ok) : "r"(sz_smem_addr(&all_there[turn])), "r"((u32)(k / 2) & 1) : "memory");
+                    there = ok != 0;
+                }
+                if (!__all_sync(0xffffffffu, there)) { dead = true; if (lane == 0) atomicOr(d.err, DL_E_WAIT); }
+                sum = make_float2(0.f, 0.f);
+#pragma unroll
+                for (int r = 0; r < CS; r++) { const float2 y = *(const float2*)(all + (turn * CS + r) * CK + 2 * lane); sum.x += y.x; sum.y += y.y; }
+            }
+            *(float2*)(factor + turn * CK + 2 * lane) = make_float2(rsqrtf(sum.x * (1.f / D) + a.eps), rsqrtf(sum.y * (1.f / D) + a.eps));
+            arrive(&factor_there[turn]);
+        }
         return;
     }
     if (warp < NC) {
@@ -750,27 +792,14 @@ sz_delta_chunk_kernel(const DlBatch d, const DlRule a, int idx0, int idx1, const
         float O[4 * OT];
         float nw[2] = {0.f, 0.f};
         if (norm) { nw[0] = a.norm[dv + g]; nw[1] = a.norm[dv + g + 8]; }
-        auto wait_sums = [&](int k) {                                     // (from other blocks' stores: acquired at the cluster's scope)
-            u64* const bar = &sq_there[k & 3];
-            bool there = dead;
-            for (u32 i = 0; !there && i < 20000000u; i++) {
-                u32 ok;
-                asm volatile("{ .reg .pred p; mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2; selp.u32 %0, 1, 0, p; }" : "=r"(ok) : "r"(sz_smem_addr(bar)), "r"((u32)(k / 4) & 1) : "memory");
-                there = ok != 0;
-            }
-            if (!__all_sync(0xffffffffu, there)) { dead = true; if (lane == 0) atomicOr(d.err, DL_E_WAIT); }
-        };
         auto finish = [&](int k) {                                        // of the k-th chunk: their norm's factor, into shared memory by rows, out
             const int c = c0 + k, n = min(CK, s.n - c * CK);
 #pragma unroll
             for (int i = 0; i < OT; i++) {
                 const int row = 8 * mine(i) + 2 * t;
                 if (norm) {
-                    // (a lane of g has the sums of one group of 16 dimensions)
-                    float2 sum = *(const float2*)(ssq + ((size_t)(k & 3) * CS * NG + g % (CS * NG)) * CK + row);
-#pragma unroll
-                    for (int o = 4; o < 4 * CS * NG; o *= 2) { sum.x += __shfl_xor_sync(0xffffffffu, sum.x, o); sum.y += __shfl_xor_sync(0xffffffffu, sum.y, o); }
-                    const float r0 = rsqrtf(sum.x * (1.f / D) + a.eps), r1 = rsqrtf(sum.y * (1.f / D) + a.eps);
+                    const float2 f = *(const float2*)(factor + (k & 1) * CK + row);
+                    const float r0 = f.x, r1 = f.y;
                     O[4 * i] *= r0; O[4 * i + 1] *= r1; O[4 * i + 2] *= r0; O[4 * i + 3] *= r1;
                 }
                 // row 8 i + 2 t (+ 1) of the warp's, dimension g (+ 8)
@@ -893,24 +922,9 @@ sz_delta_chunk_kernel(const DlBatch d, const DlRule a, int idx0, int idx1, const
                     float s0 = fmaf(o[0], o[0], o[2] * o[2]), s1 = fmaf(o[1], o[1], o[3] * o[3]);
 #pragma unroll
                     for (int x = 4; x < 32; x *= 2) { s0 += __shfl_xor_sync(0xffffffffu, s0, x); s1 += __shfl_xor_sync(0xffffffffu, s1, x); }
-                    float* const at = ssq + ((size_t)(k & 3) * CS * NG + rank * NG + p) * CK + 8 * mine(i) + 2 * t;
-                    if constexpr (CS == 1) { if (g == 0) *(float2*)at = make_float2(s0, s1); }
-                    else if (g < CS) {                                    // lanes of g: to block g of the head
-                        u32 there;
-                        asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(there) : "r"(sz_smem_addr(at)), "r"(g));
-                        asm volatile("st.shared::cluster.v2.f32 [%0], {%1, %2};" ::"r"(there), "f"(s0), "f"(s1) : "memory");
-                    }
+                    if (g == 0) *(float2*)(ssq + (turn * NG + p) * CK + 8 * mine(i) + 2 * t) = make_float2(s0, s1);
                 }
-                // they are there.  (Four turns: a warp that sends the k-th chunk's has seen all of the k - 2nd's, whose senders had read the k - 4th's.  Said before the chunk before is stored: a release waits for every store of its thread)
-                if constexpr (CS == 1) arrive(&sq_there[k & 3]);
-                else {
-                    __syncwarp();
-                    if (t == 0 && g < CS) {
-                        u32 bar;
-                        asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(bar) : "r"(sz_smem_addr(&sq_there[k & 3])), "r"(g));
-                        asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
-                    }
-                }
+                arrive(&sums_there[turn]);
 #pragma unroll
                 for (int i = 0; i < OT; i += 2) {
                     float z[8];
@@ -923,13 +937,13 @@ sz_delta_chunk_kernel(const DlBatch d, const DlRule a, int idx0, int idx1, const
                 }
             }
             arrive(&emptyb[slot]);
-            if (norm && k > 0) { wait_sums(k - 1); finish(k - 1); }       // the chunk before
+            if (norm && k > 0) { wait(&factor_there[turn ^ 1], (k - 1) / 2); finish(k - 1); }       // the chunk before
 #pragma unroll
             for (int e = 0; e < 4 * OT; e++) O[e] = N[e];
             if (!norm) finish(k);
         }
         if (norm && nc > 0) {
-            wait_sums(nc - 1);
+            wait(&factor_there[(nc - 1) & 1], (nc - 1) / 2);
             finish(nc - 1);
         }
     }
