@@ -379,14 +379,18 @@ typedef struct sz_delta_gates {
 int sz_delta_scratch_bytes(const sz_delta_pool* pool, const sz_delta_batch* batch, int io_type, int64_t* bytes);
 int sz_delta_status(uint64_t scratch, int init, int* code, uint64_t stream);
 /* y[r][c] = silu(bias[c] + sum over t of w[c][t] x[r - (conv_k - 1) + t][c]) (forward.rs:829-846), rows before the sequence's first from its slot, and the last
- * conv_k - 1 rows into it.  x, y [rows][channels] of io_type (SZ_TYPE_F32, F16 or BF16), row strides in elements, rows 16-byte aligned, apart from each other; w f32 [channels][conv_k], bias f32
+ * conv_k - 1 rows into it.  x, y [rows][channels] of io_type (SZ_TYPE_F32, F16 or BF16), row strides in elements, rows 16-byte aligned, y apart from x; w f32 [channels][conv_k], bias f32
  * [channels] (0: none).  Sums in f32.  Uses the pool's conv only. */
 int sz_delta_conv(const sz_delta_pool* pool, const sz_delta_batch* batch, int io_type, uint64_t x, int64_t x_stride, uint64_t w, uint64_t bias, uint64_t y, int64_t y_stride,
                   uint64_t scratch, int64_t scratch_bytes, uint64_t stream);
-/* The gated delta rule (forward.rs:847-894), per row and value head h with its key head's q and k over their lengths (q over sqrt(head_dim), too), beta' = sigmoid(beta):
+/* The gated delta rule (forward.rs:847-894), per row and value head h with its key head's q and k over their lengths (the root of their squares' sum and 1e-6; q over
+ * sqrt(head_dim), too), beta' = sigmoid(beta):
  *   S = decay S;  S += k (beta' (v - S^T k))^T;  o = S^T q;  out = o, or o / sqrt(mean(o^2) + eps) * norm * sigmoid(z).
  * q, k [rows][k_heads][head_dim], v, z, out [rows][v_heads][head_dim], alpha, beta [rows][v_heads], all of io_type, row strides in elements, heads side by side; rows 16-byte aligned (those
- * of alpha and beta: an element).  q, z and out may be 0 (the states alone: a replay); z and norm come together.  Uses the pool's state only. */
+ * of alpha and beta: an element).  q, z and out may be 0 (the states alone: a replay); z and norm come together; out lies apart from the inputs.  Uses the pool's state only.
+ * A sequence of 32 rows and more goes in chunks of 64, where the call is said to have such (max_rows): matrix products whose factors are held in 22 bits (those of the
+ * last products of bf16 outputs in 11), sums in f32 as row by row; a number that is not finite spoils the rest of its sequence then, and the rows of its chunk before it,
+ * too.  Numbers of less than 2^-35 of the largest in 16 value dimensions of a state, or of a chunk's changes, are lost there. */
 int sz_delta_rows(const sz_delta_pool* pool, const sz_delta_batch* batch, const sz_delta_gates* gates, int io_type, uint64_t q, int64_t q_stride, uint64_t k, int64_t k_stride,
                   uint64_t v, int64_t v_stride, uint64_t alpha, int64_t alpha_stride, uint64_t beta, int64_t beta_stride, uint64_t z, int64_t z_stride, uint64_t out,
                   int64_t out_stride, uint64_t scratch, int64_t scratch_bytes, uint64_t stream);

@@ -25,7 +25,7 @@ struct DlConv {
     const float *w, *bias;
     u8* conv;
     long long conv_stride;
-    int conv_type, ch, tile;
+    int conv_type, ch, tile;         // tile 0: a block a sequence
 };
 
 // The sequence of row r: the last that begins at or before it (-1: none), found by a warp in steps of 32 entries.
@@ -69,7 +69,8 @@ sz_delta_conv_kernel(const DlBatch d, const DlConv a) {
     }
     sz_pdl_wait();
     sz_pdl_trigger();
-    const int first = blockIdx.y * a.tile, end = min(first + a.tile, d.rows);
+    const int own = a.tile ? -1 : blockIdx.y;
+    const int first = a.tile ? blockIdx.y * a.tile : max(d.row_start[own], 0), end = min(a.tile ? first + a.tile : d.row_start[own + 1], d.rows);
     const u8* const xc = a.x + (size_t)c0 * ESZ;
     auto ask = [&](int r) {                             // row r (x is not written meanwhile: y lies elsewhere)
         Raw q;
@@ -96,7 +97,7 @@ sz_delta_conv_kernel(const DlBatch d, const DlConv a) {
 #pragma unroll
     for (int j = 0; j < DL_AHEAD; j++) ahead[j] = ask(first + j);
     u64 win[K][V / 2];                                  // the rows before the next one, and it
-    int b = -1, from = first, upto = first;             // the current sequence's rows here: from .. upto
+    int b = own, from = first, upto = first;            // the current sequence's rows here: from .. upto
     int next = first;                                   // where the one behind it begins
     auto give = [&](int r, const u64 (*x)[V / 2]) {     // row r, of K rows
         float y[V];
@@ -394,6 +395,14 @@ int dl_check_rows(uint64_t p, int64_t stride, int64_t n, int rows, int esz, int 
         return sz_fail(SZ_E_ARG, "%s: %s: rows of %lld elements, %lld apart, %d-byte aligned", who, name, (long long)n, (long long)stride, align);
     return SZ_OK;
 }
+// Whether rows of n and m elements, with the same number of rows, lie apart: not in one range, or side by side in rows of one stride
+bool dl_apart(uint64_t p, int64_t ps, int64_t n, uint64_t q, int64_t qs, int64_t m, int rows, int esz) {
+    const uint64_t pe = p + ((uint64_t)(rows - 1) * ps + n) * esz, qe = q + ((uint64_t)(rows - 1) * qs + m) * esz;
+    if (p >= qe || q >= pe) return true;
+    if (ps != qs || rows < 2) return false;
+    const uint64_t row = (uint64_t)ps * esz, at = p > q ? (row - (p - q) % row) % row : (q - p) % row;      // where a row of q begins in one of p's
+    return at >= (uint64_t)n * esz && at + (uint64_t)m * esz <= row;
+}
 DlBatch dl_batch(const sz_delta_pool* p, const sz_delta_batch* b, uint64_t scratch) {
     DlBatch d = {};
     d.n_seq = b->n_seq; d.rows = b->rows; d.n_slots = p->n_slots;
@@ -402,9 +411,17 @@ DlBatch dl_batch(const sz_delta_pool* p, const sz_delta_batch* b, uint64_t scrat
     d.err = (u32*)scratch;
     return d;
 }
-// The most rows that a sequence of the call is said to have, and from how many on they go in chunks.
+// The most rows that a sequence of the call is said to have.
 int dl_most(const sz_delta_batch* b) { return b->max_rows && b->max_rows < b->rows ? b->max_rows : b->rows; }
-constexpr int DL_LEAST = 32;
+// From how many rows on a sequence goes in chunks (0: none of the call does).  Row by row costs by the row, a chunk what it costs, and its blocks are one a multiprocessor: the more
+// of them have to wait for each other, the later they are worth it.  us, row by row / in chunks: 1 sequence of 32 heads of 128 (128 blocks), 32 rows 22.8 / 23.7, 40
+// 27.5 / 23.7; 8 sequences (1,024), 48 rows 55 / 74, 64 72 / 75, 96 105 / 93; 64 (8,192), 64 rows 485 / 614, 96 708 / 770, 128 931 / 844; heads of 64, whatever the
+// number of blocks (4 to 1,024), 40 rows 19 / 20, 20 / 21, 61 / 63, 48 22 / 20, 24 / 21, 72 / 64.
+int dl_least(const sz_delta_pool* p, const sz_delta_batch* b) {
+    const int64_t blocks = (int64_t)p->v_heads * 4 * min(b->n_seq, b->rows / 32 + 1);
+    const int least = p->head_dim == 64 ? 44 : blocks <= DL_SM ? 36 : blocks <= 16 * DL_SM ? 68 : 112;
+    return dl_most(b) >= least ? least : 0;
+}
 
 template <int TYPE>
 using DlConvFn = void (*)(const DlBatch, const DlConv);
@@ -429,7 +446,8 @@ extern "C" int sz_delta_scratch_bytes(const sz_delta_pool* pool, const sz_delta_
     if (rc) return rc;
     if (!dl_io(io_type)) return sz_fail(SZ_E_TYPE, "%s: inputs of type %d", who, io_type);
     if (!bytes) return sz_fail(SZ_E_ARG, "%s: null result", who);
-    *bytes = 256 + (dl_most(batch) >= DL_LEAST ? dl_chunk_bytes(pool->head_dim, pool->k_heads, pool->v_heads, io_type, batch->n_seq, batch->rows, DL_LEAST) : 0);
+    const int least = dl_least(pool, batch);
+    *bytes = 256 + (least ? dl_chunk_bytes(pool->head_dim, pool->k_heads, pool->v_heads, io_type, batch->n_seq, batch->rows, least) : 0);
     return SZ_OK;
 }
 
@@ -461,8 +479,7 @@ extern "C" int sz_delta_conv(const sz_delta_pool* pool, const sz_delta_batch* ba
         return sz_fail(SZ_E_ARG, "%s: carried rows: slots of %lld bytes, %lld apart, 16-byte aligned", who, (long long)slot, (long long)pool->conv_stride);
     if ((rc = dl_check_rows(x, x_stride, ch, batch->rows, esz, 16, "x", who)) || (rc = dl_check_rows(y, y_stride, ch, batch->rows, esz, 16, "y", who))) return rc;
     if (!w || ((w | bias) & 15)) return sz_fail(SZ_E_ARG, "%s: weights and bias 16-byte aligned", who);
-    const uint64_t xe = x + ((uint64_t)(batch->rows - 1) * x_stride + ch) * esz, ye = y + ((uint64_t)(batch->rows - 1) * y_stride + ch) * esz;
-    if (batch->rows > 1 && x < ye && y < xe) return sz_fail(SZ_E_ARG, "%s: y lies over x", who);
+    if (!dl_apart(x, x_stride, ch, y, y_stride, ch, batch->rows, esz)) return sz_fail(SZ_E_ARG, "%s: y lies over x", who);
     if (!scratch || (scratch & 255) || scratch_bytes < 256) return sz_fail(SZ_E_SCRATCH, "%s: the scratch is 256-byte aligned and holds the status word at least", who);
     const DlBatch d = dl_batch(pool, batch, scratch);
     DlConv a = {};
@@ -471,9 +488,12 @@ extern "C" int sz_delta_conv(const sz_delta_pool* pool, const sz_delta_batch* ba
     a.conv = (u8*)pool->conv; a.conv_stride = pool->conv_stride; a.conv_type = pool->conv_type; a.ch = ch;
     // rows a thread has: as many as leave every multiprocessor 16 warps, up to 32 (a tile's first rows are read twice)
     const int vecs = (ch / DL_V + 127) / 128;
+    // a block a sequence where they have a few rows each: one look-up instead of one for every sequence that a tile meets (64 sequences, 163 rows: 10.8 us by tiles, 10.1 so)
+    const bool by_seq = batch->n_seq > 1 && dl_most(batch) <= 8;
     a.tile = 1;
     while (a.tile < 32 && (int64_t)vecs * ((batch->rows + 2 * a.tile - 1) / (2 * a.tile)) >= 4 * DL_SM) a.tile *= 2;
-    const dim3 grid(vecs, (batch->rows + a.tile - 1) / a.tile);
+    if (by_seq) a.tile = 0;
+    const dim3 grid(vecs, by_seq ? batch->n_seq : (batch->rows + a.tile - 1) / a.tile);
     if (grid.y > 65535) return sz_fail(SZ_E_ARG, "%s: %d rows of %d channels are more than a call takes", who, batch->rows, ch);
     const DlConvFn<SZ_TYPE_F32> fn = io_type == SZ_TYPE_F32 ? dl_conv_fn<SZ_TYPE_F32>(pool->conv_k) : io_type == SZ_TYPE_F16 ? dl_conv_fn<SZ_TYPE_F16>(pool->conv_k) : dl_conv_fn<SZ_TYPE_BF16>(pool->conv_k);
     SZ_CUDA(sz_launch("delta_conv", fn, grid, dim3(128), 0, (cudaStream_t)stream, true, d, a));
@@ -501,6 +521,10 @@ extern "C" int sz_delta_rows(const sz_delta_pool* pool, const sz_delta_batch* ba
         (rc = dl_check_rows(alpha, alpha_stride, pool->v_heads, rows, esz, esz, "alpha", who)) || (rc = dl_check_rows(beta, beta_stride, pool->v_heads, rows, esz, esz, "beta", who)) ||
         (z && (rc = dl_check_rows(z, z_stride, vw, rows, esz, 16, "z", who))))
         return rc;
+    if (out && !(dl_apart(out, out_stride, vw, q, q_stride, kw, rows, esz) && dl_apart(out, out_stride, vw, k, k_stride, kw, rows, esz) && dl_apart(out, out_stride, vw, v, v_stride, vw, rows, esz) &&
+                 dl_apart(out, out_stride, vw, alpha, alpha_stride, pool->v_heads, rows, esz) && dl_apart(out, out_stride, vw, beta, beta_stride, pool->v_heads, rows, esz) &&
+                 (!z || dl_apart(out, out_stride, vw, z, z_stride, vw, rows, esz))))
+        return sz_fail(SZ_E_ARG, "%s: out lies over an input", who);
     int64_t need = 0;
     if ((rc = sz_delta_scratch_bytes(pool, batch, io_type, &need))) return rc;
     if (!scratch || (scratch & 255) || scratch_bytes < need) return sz_fail(SZ_E_SCRATCH, "%s: %lld bytes of scratch given, %lld needed, 256-byte aligned", who, (long long)scratch_bytes, (long long)need);
@@ -512,7 +536,7 @@ extern "C" int sz_delta_rows(const sz_delta_pool* pool, const sz_delta_batch* ba
     a.a = (const float*)gates->a; a.dt = (const float*)gates->dt; a.norm = (const float*)gates->norm; a.eps = gates->eps; a.q_scale = 1.f / sqrtf((float)D);
     a.kh = pool->k_heads; a.vh = pool->v_heads; a.grouped = pool->grouped;
     a.state = (u8*)pool->state; a.state_stride = pool->state_stride;
-    a.least = dl_most(batch) >= DL_LEAST ? DL_LEAST : 0;
+    a.least = dl_least(pool, batch);
     cudaStream_t st = (cudaStream_t)stream;
     using Fn = void (*)(const DlBatch, const DlRule);
 #define SZ_DL_T(D_, O) (io_type == SZ_TYPE_F32 ? (Fn)sz_delta_rows_kernel<D_, SZ_TYPE_F32, O> : io_type == SZ_TYPE_F16 ? (Fn)sz_delta_rows_kernel<D_, SZ_TYPE_F16, O> : (Fn)sz_delta_rows_kernel<D_, SZ_TYPE_BF16, O>)

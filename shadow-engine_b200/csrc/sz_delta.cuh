@@ -94,10 +94,11 @@ template <int TYPE> __device__ __forceinline__ float dl_sigmoid(float x) {
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(den));
     return r * fmaf(-den, r, 2.f);
 }
-// The logarithm of a row's decay, a softplus(alpha + dt), and its beta.  A decay above 1 (a positive `a`) counts as 1.
+// The logarithm of a row's decay, a softplus(alpha + dt).  A decay above 1 (a positive `a`) counts as 1; one below e^-1000 is 0 in f32 as it is, and sums of these
+// keep the others' digits (in f64).
 __device__ __forceinline__ float dl_log_decay(float alpha, float a, float dt) {
     const float x = alpha + dt, g = a * (x > 20.f ? x : log1pf(expf(x)));
-    return g > 0.f ? 0.f : g;
+    return g > 0.f ? 0.f : g < -1000.f ? -1000.f : g;
 }
 
 // Sequence b as one warp sees it (all lanes with the same b).  An earlier sequence with rows that writes a slot which b reads or writes, or reads one

@@ -43,7 +43,7 @@ class States:
                 continue
             if shape is None:
                 shape = (t.shape[1] if t.dim() == 3 else 1, ch)
-            if t.shape != (one.shape[0],) + shape or t.device != self.device or not t[0].is_contiguous() or (t.shape[0] > 1 and t.stride(0) < t[0].numel()):
+            if one.shape[0] < 1 or t.shape != (one.shape[0],) + shape or t.device != self.device or not t[0].is_contiguous() or (t.shape[0] > 1 and t.stride(0) < t[0].numel()):
                 raise ValueError("%s: [%d, %s], a slot contiguous" % (name, one.shape[0], ", ".join(map(str, shape))))
             if t.dtype not in TYPES or (name == "state" and t.dtype != torch.float32):
                 raise ValueError("%s: %s" % (name, "float32" if name == "state" else "float32, float16 or bfloat16"))

@@ -31,7 +31,7 @@ def conv(L, p=None, b=None, io=szlib.TYPE_BF16, x=1 << 20, xs=512, w=4096, bias=
     return L.sz_delta_conv(C.byref(p or pool()), C.byref(b or batch()), io, x, xs, w, bias, y, ys, scratch, size, 0)
 
 
-def rule(L, p=None, b=None, g=None, io=szlib.TYPE_BF16, q=4096, qs=128, k=4096, ks=128, v=4096, vs=256, al=4096, als=4, be=4096, bes=4, z=0, zs=0, out=8192, outs=256, scratch=4096, size=1 << 40):
+def rule(L, p=None, b=None, g=None, io=szlib.TYPE_BF16, q=4096, qs=128, k=4096, ks=128, v=4096, vs=256, al=4096, als=4, be=4096, bes=4, z=0, zs=0, out=1 << 20, outs=256, scratch=4096, size=1 << 40):
     return L.sz_delta_rows(C.byref(p or pool()), C.byref(b or batch()), C.byref(g or gates()), io, q, qs, k, ks, v, vs, al, als, be, bes, z, zs, out, outs, scratch, size, 0)
 
 
@@ -86,6 +86,21 @@ def test_rule_refuses():
                 dict(z=4096, zs=256), dict(outs=252)):
         assert rule(L, **bad) == szlib.E_ARG, bad
     assert rule(L, g=gates(norm=4096), z=4096, zs=256, q=0, out=0) == szlib.E_ARG
+
+
+def test_outputs_over_inputs_are_refused():
+    """Other blocks read what one writes; rows side by side in one buffer are apart."""
+    L = szlib.load()
+    for bad in (dict(out=4096), dict(out=4096 + 256 * 2), dict(out=4096 - 2 * 256), dict(v=1 << 20), dict(k=(1 << 20) + 1024), dict(al=(1 << 20) + 8), dict(be=(1 << 20) + 2046)):
+        assert rule(L, **bad) == szlib.E_ARG, bad
+        assert b"over an input" in L.sz_last_error()
+    assert rule(L, g=gates(norm=4096), z=1 << 20, zs=256) == szlib.E_ARG
+    assert conv(L, x=1 << 20, xs=1024, y=(1 << 20) + 512, ys=1024) == szlib.E_ARG and b"over x" in L.sz_last_error()
+    assert conv(L, b=batch(rows=1), x=1 << 20, y=1 << 20) == szlib.E_ARG and b"over x" in L.sz_last_error()
+    # side by side: past this check (and refused for the scratch)
+    assert conv(L, x=1 << 20, xs=1024, y=(1 << 20) + 1024, ys=1024, scratch=0) == szlib.E_SCRATCH
+    assert conv(L, x=(1 << 20) + 1024, xs=1024, y=1 << 20, ys=1024, scratch=0) == szlib.E_SCRATCH
+    assert rule(L, v=(1 << 20) + 512, vs=512, out=1 << 20, outs=512, scratch=0) == szlib.E_SCRATCH
 
 
 def test_status_refuses():

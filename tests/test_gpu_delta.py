@@ -157,9 +157,14 @@ def test_conv_of_one_sequence(rows, io):
         Case([rows], [past], kh=2, vh=2, io=io).check_conv(bias=False)
 
 
-@pytest.mark.parametrize("n", [33, 64, 1100, 4096])
-def test_conv_of_many_sequences(n):
-    Case([(i * 7) % 4 for i in range(n)], [(i % 3) * 5 for i in range(n)], kh=1, vh=1, io="bf16", fork=True).check_conv()
+@pytest.mark.parametrize("n", [2, 33, 64, 1100, 4096])
+@pytest.mark.parametrize("max_rows", [None, 3])
+def test_conv_of_many_sequences(n, max_rows):
+    Case([(i * 7) % 4 for i in range(n)], [(i % 3) * 5 for i in range(n)], kh=1, vh=1, io="bf16", fork=True, max_rows=max_rows, pad=2).check_conv()
+
+
+def test_conv_of_more_rows_than_were_said():
+    Case([0, 100, 1, 40], [3, 0, 4, 9], io="bf16", max_rows=2, pad=3).check_conv()
 
 
 @pytest.mark.parametrize("io, carried", [("bf16", "f32"), ("f32", "f16"), ("f16", "bf16")])
@@ -196,7 +201,7 @@ def test_rule_of_few_rows(d, io, kh, vh, grouped):
 
 @pytest.mark.parametrize("d", [64, 128])
 @pytest.mark.parametrize("io", ["f32", "bf16", "f16"])
-@pytest.mark.parametrize("rows", [15, 16, 17, 63, 64, 65, 127, 128, 129, 200, 449])
+@pytest.mark.parametrize("rows", [15, 16, 17, 35, 36, 43, 44, 63, 64, 65, 127, 128, 129, 200, 449])
 def test_rule_of_one_sequence(d, io, rows):
     for past in (0, 9):
         Case([rows], [past], d=d, io=io, gate=past == 0, seed=rows).check_rule()
@@ -318,13 +323,86 @@ def test_forks_read_one_slot():
     c.check_conv()
 
 
+def test_more_chunks_than_a_pass_takes():
+    """6,300 rows of the benchmark's heads: more than 96 MB of what the chunks leave, so the chain goes on in a second pass; a short sequence in each."""
+    c = Case([6150, 97, 53], [0, 4, 0], kh=16, vh=32, d=128, io="bf16", gate=False, seed=2)
+    need = delta.C.c_int64()
+    szlib.check(c.step.lib.sz_delta_scratch_bytes(c.step._c, c.step._b, szlib.TYPE_BF16, delta.C.byref(need)))
+    assert need.value < 100 << 20
+    c.check_rule()
+
+
+@pytest.mark.parametrize("rows", [3, 70])
+def test_pools_past_four_gigabytes(rows):
+    """Slots 3 GB apart: a slot's place passes 32 bits."""
+    c = Case([rows, rows], [5, 0], d=64, io="bf16", slots=[2, 1], to=[1, 2], n_slots=3)
+    apart = 3 << 30
+    mem = torch.zeros(2 * apart + (1 << 20), dtype=torch.uint8, device="cuda")
+    state = mem.view(torch.float32).as_strided((3, c.vh, c.d, c.d), (apart // 4, c.d * c.d, c.d, 1))
+    ref = Case([rows, rows], [5, 0], d=64, io="bf16", slots=[2, 0], to=[1, 2], n_slots=3)
+    state.copy_(c.state)
+    step = delta.Step(delta.States(c.kh, c.vh, c.d, state=state), c.row_start, c.lens, torch.tensor([2, 0], dtype=torch.int32, device="cuda"), c.rows,
+                      to=torch.tensor([1, 2], dtype=torch.int32, device="cuda"))
+    # (the second is new, and writes where the first reads: left out)
+    out = torch.full((c.rows, c.vh, c.d), 77.0, dtype=c.io, device="cuda")
+    step.rule(c.q, c.k, c.v, c.alpha, c.beta, c.a, c.dt, z=c.z, norm=c.norm, out=out)
+    assert step.status() == 4
+    got = ref.run()
+    assert ref.step.status() == 4
+    assert torch.equal(out[:rows], got[:rows]) and bool((out[rows:] == 77).all()) and torch.equal(state, ref.state)
+    carried = mem.view(torch.bfloat16).as_strided((3, c.conv_k - 1, c.ch), (apart // 2, c.ch, 1))
+    carried.copy_(c.carried)
+    slots = torch.tensor([2, 1], dtype=torch.int32, device="cuda")
+    conv = delta.Step(delta.States(c.kh, c.vh, c.d, conv=carried), c.row_start, c.lens, slots, c.rows)
+    y = conv.conv(c.x, c.w)
+    same = Case([rows, rows], [5, 0], d=64, io="bf16", slots=[2, 1], to=[2, 1], n_slots=3)
+    assert torch.equal(y, same.step.conv(same.x, same.w)) and torch.equal(carried, same.carried) and conv.status() == 0
+
+
+def test_decays_of_nothing():
+    """Rows whose decay is 0, by an infinite or a huge exponent, among others: what was before them is gone, what comes after is as ever."""
+    c = Case([150, 7], [3, 3], d=64, io="f32", gate=False)
+    for r, x in ((4, math.inf), (70, 1e30), (71, math.inf), (100, 3e4), (140, math.inf), (152, math.inf)):
+        c.alpha[r] = x
+    c.a[0] = -1e-3
+    c.check_rule()
+
+
+@pytest.mark.parametrize("rows", [6, 150])
+def test_what_is_not_finite_stays_in_its_sequence_and_head(rows):
+    c, ref = (Case([rows] * 3, [4, 0, 2], kh=2, vh=4, d=64, io="bf16", fork=True) for _ in range(2))
+    want = ref.run()
+    c.v[rows + 2, 1] = math.nan
+    c.v[rows + 3, 1, 5] = math.inf
+    got = c.run()
+    assert c.step.status() == 0
+    bad = torch.zeros_like(got, dtype=torch.bool)
+    bad[rows:2 * rows, 1] = True
+    assert torch.equal(got[~bad], want[~bad]) and bool(got[rows + 2, 1].isnan().any())
+    assert torch.equal(got[rows:rows + 2], want[rows:rows + 2]) or rows > 31
+    for b in (0, 2):
+        assert torch.equal(c.state[c.to[b]], ref.state[ref.to[b]])
+    assert torch.equal(c.state[c.to[1]][[0, 2, 3]], ref.state[ref.to[1]][[0, 2, 3]])
+
+
+def test_a_batch_whose_prompts_are_worth_chunks_later():
+    """Many blocks: sequences of up to 111 rows go row by row, longer ones in chunks."""
+    n = 20
+    Case([1 + (i * 37) % 130 for i in range(n)], [5 * (i % 3) for i in range(n)], kh=16, vh=32, d=128, io="bf16", gate=False).check_rule()
+
+
+def test_more_rows_than_were_said():
+    """max_rows chooses kernels, not results: a sequence of more rows is right, row by row."""
+    Case([100, 1, 40], [0, 4, 9], d=128, io="bf16", max_rows=4).check_rule()
+
+
 # ---- tables that do not fit ---------------------------------------------------------------------------------------------------------------
 @pytest.mark.parametrize("rows", [3, 80])
 @pytest.mark.parametrize("call", ["conv", "rule"])
 def test_tables_that_do_not_fit_are_reported(rows, call):
     """The sequence is left out, the others are not; nothing outside the pool or the rows is touched (the kernels check every entry before they use it)."""
     def go(code, slots=(1, 2, 3), to=None, starts=None, untouched=(), past=(5, 5, 5)):
-        c = Case([rows] * 3, list(past), d=64, io="f32", slots=list(slots), to=None if to is None else list(to), n_slots=6)
+        c = Case([rows] * 3, list(past), d=64, io="f32", slots=list(slots), to=None if to is None else list(to), n_slots=6, max_rows=None if rows > 3 else 3)
         if starts is not None:
             c.row_start.copy_(torch.tensor(starts, dtype=torch.int32))
         state, carried = c.state.clone(), c.carried.clone()
