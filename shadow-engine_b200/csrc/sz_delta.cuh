@@ -105,6 +105,10 @@ __device__ __forceinline__ float dl_log_decay(float alpha, float a, float dt) {
 // that b writes, keeps b out: whatever the order of the blocks, the results are the same.
 __device__ __forceinline__ DlSeq dl_seq(const DlBatch& d, int b, int lane, bool report) {
     DlSeq s;
+    // (a lane's first sequence before b is asked for together with b itself: one wait, not three)
+    int p0 = 0, p1 = 0, pt = 0, pf = 0, pl = 0;
+    auto ask = [&](int i) { p0 = d.row_start[i]; p1 = d.row_start[i + 1]; pt = d.to[i]; pf = d.from[i]; pl = d.lens[i]; };
+    if (lane < b) ask(lane);
     const int r0 = d.row_start[b], r1 = d.row_start[b + 1], len = d.lens[b];
     const int from = d.from[b], to = d.to[b], take = d.take ? d.take[b] : 0x7fffffff;
     u32 bad = 0;
@@ -118,10 +122,9 @@ __device__ __forceinline__ DlSeq dl_seq(const DlBatch& d, int b, int lane, bool 
     if (count > 0 && !bad) {
         bool clash = false;
         for (int i = lane; i < b; i += 32) {
-            const int c = d.row_start[i + 1] - d.row_start[i];
-            if (c <= 0) continue;
-            const int ti = d.to[i], fi = d.lens[i] > c ? d.from[i] : -1;
-            clash |= ti == to || ti == s.from || fi == to;
+            if (i >= 32) ask(i);
+            const int c = p1 - p0, reads = pl > c ? pf : -1;
+            clash |= c > 0 && (pt == to || pt == s.from || reads == to);
         }
         if (__any_sync(0xffffffffu, clash)) bad |= DL_E_CLASH;
     }

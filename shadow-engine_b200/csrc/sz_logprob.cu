@@ -4,7 +4,8 @@
 // no difference of like numbers, whatever the distribution.  One pass over the row: a warp keeps the largest so far (the same for its lanes, so that a
 // new one is rare) and both sums beside it.  A thread's elements come in groups of LP_G vectors; what a group's largest is stays in shared memory, and the
 // best `top` are looked for afterwards in the few groups that can hold them: a bound that `top` threads reach, by halving, then what is not below it.
-// A row is a cluster of 1 to 8 blocks, each with its part of it.
+// A row is a cluster of 1 to 8 blocks, each with its part of it.  Rows of 151,936: one of f32, top 5, 8.1 us (the chain load, bound, gather, order and two barriers of the
+// cluster); 64 of f32, top 20, with temperatures, 19 (39 MB: 5.9); 1,021 of bf16, top 1, 87 (310 MB: 47; the exponentials' pipe alone takes 35, and an element some 8 instructions).
 #include "sz_common.cuh"
 
 #include <cuda_bf16.h>
