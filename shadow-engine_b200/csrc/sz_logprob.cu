@@ -4,8 +4,8 @@
 // no difference of like numbers, whatever the distribution.  One pass over the row: a warp keeps the largest so far (the same for its lanes, so that a
 // new one is rare) and both sums beside it.  A thread's elements come in groups of LP_G vectors; what a group's largest is stays in shared memory, and the
 // best `top` are looked for afterwards in the few groups that can hold them: a bound that `top` threads reach, by halving, then what is not below it.
-// A row is a cluster of 1 to 8 blocks, each with its part of it.  Rows of 151,936: one of f32, top 5, 8.1 us (the chain load, bound, gather, order and two barriers of the
-// cluster); 64 of f32, top 20, with temperatures, 19 (39 MB: 5.9); 1,021 of bf16, top 1, 87 (310 MB: 47; the exponentials' pipe alone takes 35, and an element some 8 instructions).
+// A row is a cluster of 1 to 8 blocks, each with its part of it.  Rows of 151,936: one of f32, top 5, 8.3 us (the chain load, bound, gather, order and two barriers of the
+// cluster); 64 of f32, top 20, 14.3 (39 MB: 5.9); 1,021 of bf16, top 1, 69 where they score their best, 87 with a fifth of them scoring any token (310 MB: 47; the exponentials' pipe alone takes 35, and an element some 8 instructions).
 #include "sz_common.cuh"
 
 #include <cuda_bf16.h>
@@ -487,15 +487,14 @@ extern "C" int sz_logprob_rows(int logits_type, uint64_t logits, int64_t logits_
     a.logits = (const u8*)logits; a.stride = logits_stride * esz; a.rows = rows; a.vocab = vocab; a.top = top;
     a.tokens = (const int32_t*)tokens; a.temperature = (const float*)temperature;
     a.logprob = (float*)logprob; a.entropy = (float*)entropy; a.rank = (int32_t*)rank; a.top_ids = (int32_t*)top_ids; a.top_logprobs = (float*)top_logprobs;
-    // blocks a row: waves of blocks times what one takes; with few rows (none has to wait) blocks of twice the threads
+    // Up to one row a multiprocessor: blocks of 512 threads, as many a row (up to 8) as all have a multiprocessor each; more rows: 256 threads, four blocks a multiprocessor, one
+    // a row.  Device us of rows of 151,936 with 512 threads and 1, 2, 4, 8 blocks a row, with 256 threads and one: 1 row of f32 16.2, 12.4, 9.5, 8.3, 25; 16 rows 17.5, 13.9,
+    // 11.6, 12.6, 26; 37 rows 17.6, 14.1, 14.9, 21.9, 26; 64 rows 17.8, 14.3, 15.3, 26, 26; 128 rows 17.4, 19, 26.5, 44, 27; 250 of bf16 25.3, 34, 50, 91, 24.8; 1,021
+    // 75, 101, 166, 315, 69.
     const int most = vocab > 16384 ? 8 : vocab > 4096 ? 4 : vocab > 1024 ? 2 : 1;
-    const bool few = (long long)rows * most <= 2 * LP_SM;
-    const int places = few ? 2 * LP_SM : 4 * LP_SM;
-    double least = 0;
-    for (int C = 1; C <= most; C *= 2) {
-        const double cost = (double)(((long long)rows * C + places - 1) / places) * (20000.0 + (double)vocab / C);
-        if (C == 1 || cost < least) { least = cost; a.C = C; }
-    }
+    const bool few = rows <= LP_SM;
+    a.C = 1;
+    while (few && 2 * a.C <= most && (long long)rows * 2 * a.C <= LP_SM) a.C *= 2;
     a.per = ((vocab + a.C - 1) / a.C + 7) & ~7;
     cudaStream_t st = (cudaStream_t)stream;
 #define SZ_LP(N_) (logits_type == SZ_TYPE_F32 ? lp_launch<SZ_TYPE_F32, N_>(a, st) : logits_type == SZ_TYPE_F16 ? lp_launch<SZ_TYPE_F16, N_>(a, st) : lp_launch<SZ_TYPE_BF16, N_>(a, st))

@@ -10,7 +10,7 @@ szlib, delta, sampling = pkg.lib, pkg.delta, pkg.sampling
 
 
 def pool(**kw):
-    d = dict(n_slots=4, k_heads=2, v_heads=4, head_dim=64, grouped=0, conv_k=4, conv_type=szlib.TYPE_BF16, state=4096, conv=8192, state_stride=4 * 64 * 64 * 4, conv_stride=3 * 512 * 2)
+    d = dict(n_slots=4, k_heads=2, v_heads=4, head_dim=64, grouped=0, conv_k=3, conv_type=szlib.TYPE_BF16, state=4096, conv=8192, state_stride=4 * 64 * 64 * 4, conv_stride=2 * 512 * 2)
     d.update(kw)
     return delta.DeltaPoolC(**d)
 
@@ -67,7 +67,7 @@ def test_calls_refuse_bad_tables_and_pools(call):
 
 def test_conv_refuses():
     L = szlib.load()
-    for bad in (dict(conv=0), dict(conv=4104), dict(conv_stride=3 * 512 * 2 - 16), dict(conv_stride=3 * 512 * 2 + 8), dict(conv_k=1), dict(conv_k=9)):
+    for bad in (dict(conv=0), dict(conv=4104), dict(conv_stride=2 * 512 * 2 - 16), dict(conv_stride=2 * 512 * 2 + 8), dict(conv_k=1), dict(conv_k=9)):
         assert conv(L, p=pool(**bad)) == szlib.E_ARG, bad
     assert conv(L, p=pool(conv_type=szlib.TYPE_Q8_0)) == szlib.E_TYPE
     for bad in (dict(x=0), dict(y=0), dict(x=(1 << 20) + 8), dict(xs=511), dict(xs=516), dict(ys=500), dict(w=0), dict(w=4100), dict(bias=4104), dict(y=1 << 20), dict(y=(1 << 20) + 512)):
@@ -125,9 +125,9 @@ def ints(*s):
 
 
 def test_the_python_side_checks_shapes():
-    state, carried = torch.zeros(5, 4, 64, 64), torch.zeros(5, 3, 512, dtype=torch.bfloat16)
+    state, carried = torch.zeros(5, 4, 64, 64), torch.zeros(5, 2, 512, dtype=torch.bfloat16)
     p = delta.States(2, 4, 64, state, carried)
-    assert (p.conv_k, p.channels, p.c.state_stride, p.c.conv_stride) == (4, 512, 65536, 3072)
+    assert (p.conv_k, p.channels, p.c.state_stride, p.c.conv_stride) == (3, 512, 65536, 2048)
     apart = delta.States(2, 4, 64, state=torch.zeros(5, 2, 4, 64, 64)[:, 1])
     assert apart.c.state_stride == 131072
     for args, kw in (((2, 4, 64), {}), ((2, 4, 64, state.half()), {}), ((2, 4, 64, state[:, :3]), {}), ((2, 4, 64, state.transpose(2, 3)), {}), ((2, 4, 64, state, carried[:4]), {}),
