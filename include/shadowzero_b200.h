@@ -389,8 +389,8 @@ int sz_delta_conv(const sz_delta_pool* pool, const sz_delta_batch* batch, int io
  * q, k [rows][k_heads][head_dim], v, z, out [rows][v_heads][head_dim], alpha, beta [rows][v_heads], all of io_type, row strides in elements, heads side by side; rows 16-byte aligned (those
  * of alpha and beta: an element).  q, z and out may be 0 (the states alone: a replay); z and norm come together; out lies apart from the inputs.  Uses the pool's state only.
  * A sequence of many rows - from 36 on, or up to 112, by the heads and the number of sequences of the call - goes in chunks of 64, where the call is said to have such
- * (max_rows; a row's last bits depend on which way it goes): matrix products whose factors are held in 22 bits (those of the
- * last products of bf16 outputs in 11), sums in f32 as row by row; a number that is not finite spoils the rest of its sequence then, and the rows of its chunk before it,
+ * (max_rows; a row's last bits depend on which way it goes): matrix products whose factors are held in 22 bits, sums in
+ * f32 as row by row; a number that is not finite spoils the rest of its sequence then, and the rows of its chunk before it,
  * too.  Numbers of less than 2^-35 of the largest in 16 value dimensions of a state, or of a chunk's changes, are lost there. */
 int sz_delta_rows(const sz_delta_pool* pool, const sz_delta_batch* batch, const sz_delta_gates* gates, int io_type, uint64_t q, int64_t q_stride, uint64_t k, int64_t k_stride,
                   uint64_t v, int64_t v_stride, uint64_t alpha, int64_t alpha_stride, uint64_t beta, int64_t beta_stride, uint64_t z, int64_t z_stride, uint64_t out,

@@ -10,15 +10,15 @@
 //  sz_delta_chunk_kernel, a block of warps for 16 NG value dimensions of a sequence's value head: the chain over its chunks, on mma.sync.  Everything is
 //   transposed, so that a warp's 16 value dimensions are a product's rows: S^T (f32) stays in its registers, and what one product gives is in the layout in which
 //   the next one takes it.  At 128 key dimensions two warps have 64 of them each and add up K S and Q S through shared memory.
-// 4,093 rows of 32 heads of 128 on 16, bf16: 48 us and 165 (137 MB: 21 of them); a chunk of the chain is 4,100 - 4,700 cycles, 1,500 of them its warp's products, the rest what lies
-// between one and the next: the largest of the state 150, the partner's part 310, R 290, two numbers of a factor 270 and 220, waits 400.
+// 4,093 rows of 32 heads of 128 on 16, bf16: 48 us and 172 (137 MB: 21 of them).  The chain lies in what is between one product and the next: the largest of the state 150 cycles, the
+// partner's part 310, R 290, two numbers of a factor 270 and 220, waits 400.
 // tcgen05 would have the products' time, but every one of the chain's links would go through tensor memory and back (300 - 400 cycles a wait, three
 // a chunk) and S through a conversion by four warps: no sooner.
 //
 // Numbers.  A row k = rho 2^e (k 2^-e) enters the products as k 2^-e with its largest element in [1, 2): a bf16 or f16 row is exact in f16, an f32 row is two f16
 // numbers (22 bits); the rows' lengths and powers are factors in f32.  S, R = V - e^G K S and D enter as two f16 numbers each, in units of a power of two that
-// the warp takes from the largest there is: 22 bits, and what is less than 2^-35 of that largest is lost.  Sums are f32.  T and the decays' sums: f32 and f64.  The
-// last products of a bf16 output take one f16 number a factor (11 bits, where the output keeps 8).
+// the warp takes from the largest there is: 22 bits, and what is less than 2^-35 of that largest is lost.  Sums are f32.  T and the decays' sums: f32 and f64.
+// (One f16 number a factor in the last products of bf16 outputs, 11 bits where they keep 8: their difference from rounded f32 outputs is 1.1 10^-3 of their size instead of 10^-5, and 4,093 rows take 202 us.)
 #include "sz_delta.cuh"
 
 namespace {
@@ -32,14 +32,13 @@ struct DlScalars { float gr[CK], wj[CK], gc, pad[15]; };              // e^G rho
 
 template <int D, int TYPE> struct DlChunk {
     static constexpr int NK = TYPE == SZ_TYPE_F32 ? 2 : 1;                // f16 numbers of an element of k and q
-    static constexpr bool FULL = TYPE != SZ_TYPE_BF16;                    // outputs' products with both numbers of a factor
     static constexpr int TILE = CK * D * 2, ROWS = 2 * NK * TILE;         // a key head's rows: k (high, low), q (high, low)
     // a value head's T (high, low) and scalars, for the chain; P (high, low) and e^G rho_q, for the outputs
-    static constexpr int HA = 2 * DL_FRAG + (int)sizeof(DlScalars), HB = (FULL ? 2 : 1) * DL_FRAG + CK * 4, HEAD = HA + HB;
+    static constexpr int HA = 2 * DL_FRAG + (int)sizeof(DlScalars), HB = 2 * DL_FRAG + CK * 4, HEAD = HA + HB;
 };
 int64_t dl_chunk_one(int d, int kh, int vh, int io_type) {
     const int nk = io_type == SZ_TYPE_F32 ? 2 : 1;
-    return (int64_t)kh * 2 * nk * CK * d * 2 + (int64_t)vh * ((io_type == SZ_TYPE_BF16 ? 3 : 4) * DL_FRAG + CK * 4 + (int)sizeof(DlScalars));
+    return (int64_t)kh * 2 * nk * CK * d * 2 + (int64_t)vh * (4 * DL_FRAG + CK * 4 + (int)sizeof(DlScalars));
 }
 
 // The sequences of many rows, in order: the y-th of them (y >= 0), or the one whose chunks have index idx.  Chunk c of a sequence has index
@@ -304,7 +303,7 @@ sz_delta_prep_kernel(const DlBatch d, const DlRule a, int idx0, u8* __restrict__
                             dl_split(p[2 * u], p[2 * u + 1], hi, lo);
                             u32* const at = (u32*)(hp + C::HA) + ((dl_tile(2 * warp + u) + m / 2) * 32 + lane) * 2 + (m & 1);
                             *at = hi;
-                            if (C::FULL) *(at + DL_FRAG / 4) = lo;
+                            *(at + DL_FRAG / 4) = lo;
                         }
                     }
                 }
@@ -425,22 +424,24 @@ sz_delta_prep_kernel(const DlBatch d, const DlRule a, int idx0, u8* __restrict__
 }
 
 // ---- the chain over a sequence's chunks --------------------------------------------------------------------------------------------------------
-// A block has four kinds of warps, which meet at mbarriers only: NC of the chain (16 value dimensions and 64 key dimensions each); two for the outputs of every 16
+// A block has four kinds of warps, which meet at mbarriers only: NC of the chain (16 value dimensions and 64 key dimensions each); two or four for the outputs of every 16
 // dimensions, which take S and D as the chain's products had them (f16, from shared memory); one that copies the chunks' operands into two rings; and one for the
 // outputs' norms.  The blocks of a head form a cluster: a row's sums of squares go to all of them, and a chunk's outputs leave while the next one's are made.
 // (The releases that this takes wait for every store of their thread, 1,300 cycles a chunk where the outputs' warps made them.)
 template <int D, int TYPE, int NG, bool OUT> struct DlMain {
     using C = DlChunk<D, TYPE>;
     static constexpr int ESZ = DlIo<TYPE>::ESZ, NQ = D / 64, NC = NG * NQ, CS = D / 16 / NG;      // warps on one 16 dimensions; of the chain; blocks of a head
-    static constexpr int NO = OUT ? 2 : 0, NTH = 32 * (NC + NG * NO + (OUT ? 2 : 1));             // warps on the outputs of 16 dimensions, half of the rows each; of copies, of norms
+    // warps on the outputs of 16 dimensions, which share the rows: with two of them a chunk's outputs take longer than the chain's part at 128 dimensions (4,093 rows of bf16 259 us, with four
+    // 221; of f32, whose rings have room for one chunk only, 387 and 397); and of copies, of norms
+    static constexpr int NO = !OUT ? 0 : D == 128 && TYPE != SZ_TYPE_F32 ? 4 : 2, NS = OUT ? NO : 1, NTH = 32 * (NC + NG * NO + (OUT ? 2 : 1));
     static constexpr bool STAGED = TYPE != SZ_TYPE_F32;                                    // gates and outputs through shared memory (f32: whole sectors a warp without)
     static constexpr int VS = 16 * NG * ESZ + 16;                                          // bytes between rows of v and z in shared memory
     // a chunk's operands in two rings, of the chain (k, T, scalars, v) and of the outputs (q, P, e^G, z), each as deep as there is room
     static constexpr int A = C::ROWS / 2 + C::HA + CK * VS, B = OUT ? C::ROWS / 2 + C::HB + (STAGED ? CK * VS : 0) : 0;
-    static constexpr int SA = D == 128 ? (TYPE == SZ_TYPE_BF16 ? 3 : TYPE == SZ_TYPE_F16 ? 2 : 1) : (TYPE == SZ_TYPE_F32 ? 2 : 3), SB = D == 128 && TYPE == SZ_TYPE_F32 ? 1 : 2;
-    static constexpr int XB = NQ == 2 ? 2 * 8 * 32 * 16 : 0;                               // what a chain's warp gives its partner (two chunks' turns)
-    static constexpr int FB = OUT ? (C::FULL ? 2 : 1) * 4 * 32 * 16 : 0;                   // a product's factor of 16 x 64 in f16: S of a warp, D of a group; two turns of each
-    static constexpr int OS = 16 * ESZ + 16, OB = OUT && STAGED ? CK / 2 * OS : 0;         // a warp's outputs on their way
+    static constexpr int SA = D == 128 ? (TYPE == SZ_TYPE_F32 ? 1 : 2) : (TYPE == SZ_TYPE_F32 ? 2 : 3), SB = D == 128 && TYPE == SZ_TYPE_F32 ? 1 : 2;
+    static constexpr int XB = NQ == 2 ? (8 + 4) * 32 * 16 : 0;                             // what a chain's warp gives its partner: its part of K S, half of D
+    static constexpr int FB = OUT ? 2 * 4 * 32 * 16 : 0;                                   // a product's factor of 16 x 64 in two f16 numbers: S of a warp, D of a group; two turns of each
+    static constexpr int OS = 16 * ESZ + 16, OB = OUT && STAGED ? CK / NS * OS : 0;        // a warp's outputs on their way
     static constexpr int SSQ = OUT ? 2 * (NG + CS + 1) * CK * 4 : 0;                       // a row's sums of squares and its norm's factor, two turns: [group], [block], the factor
     static constexpr int BARS = 2 * SA + 2 * SB + 6 * NG + 6;
     static constexpr size_t SMEM = (size_t)SA * A + (size_t)SB * B + NC * (XB + 2 * FB) + NG * (2 * FB + NO * OB) + SSQ + BARS * 8 + 2 * (NC + NG) * 4;
@@ -451,11 +452,10 @@ __global__ void __launch_bounds__(DlMain<D, TYPE, NG, OUT>::NTH, 1)
 sz_delta_chunk_kernel(const DlBatch d, const DlRule a, int idx0, int idx1, const u8* __restrict__ scratch, long long one) {
     using M = DlMain<D, TYPE, NG, OUT>;
     using C = DlChunk<D, TYPE>;
-    constexpr int ESZ = M::ESZ, NQ = M::NQ, NK = C::NK, NC = M::NC, CS = M::CS, SA = M::SA, SB = M::SB, NO = M::NO, OT = 4;      // OT: 8-row tiles whose outputs a warp finishes
-    constexpr int FP = C::FULL ? 2 : 1;
+    constexpr int ESZ = M::ESZ, NQ = M::NQ, NK = C::NK, NC = M::NC, CS = M::CS, SA = M::SA, SB = M::SB, NO = M::NO, NS = M::NS, OT = 8 / NS;      // OT: 8-row tiles whose outputs a warp finishes
     extern __shared__ __align__(16) u8 sm[];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
-    const int w = warp < NC ? warp : warp - NC, p = warp < NC ? w / NQ : w / 2, q = warp < NC ? w % NQ : w % 2;      // (an output's warp: q is its half of the rows)
+    const int w = warp < NC ? warp : warp - NC, p = warp < NC ? w / NQ : w / NS, q = warp < NC ? w % NQ : w % NS;      // (an output's warp: q is its share of the rows)
     const int h = blockIdx.x / CS, rank = blockIdx.x % CS, kx = a.grouped ? h / (a.vh / a.kh) : h % a.kh;
     u8* const rb = sm + SA * M::A;
     u8* const xb = rb + SB * M::B;
@@ -665,8 +665,8 @@ sz_delta_chunk_kernel(const DlBatch d, const DlRule a, int idx0, int idx1, const
 #pragma unroll
                 for (int e = 0; e < 4; e++) dl_split(S[2 * ks + (e >> 1)][2 * (e & 1)], S[2 * ks + (e >> 1)][2 * (e & 1) + 1], hi[e], lo[e]);
                 if (OUT) {
-                    sf[(((turn * NC + w) * FP) * 4 + ks) * 32 + lane] = *(uint4*)hi;
-                    if (C::FULL) sf[(((turn * NC + w) * FP + 1) * 4 + ks) * 32 + lane] = *(uint4*)lo;
+                    sf[(((turn * NC + w) * 2) * 4 + ks) * 32 + lane] = *(uint4*)hi;
+                    sf[(((turn * NC + w) * 2 + 1) * 4 + ks) * 32 + lane] = *(uint4*)lo;
                 }
                 times(hi);
                 times(lo);
@@ -677,8 +677,8 @@ sz_delta_chunk_kernel(const DlBatch d, const DlRule a, int idx0, int idx1, const
 #pragma unroll
             for (int m = 0; m < 8; m++) dl_scale4(X[m], true_s);
             if constexpr (NQ == 2) {                                      // with the other key dimensions'
-                float4* const to = (float4*)(xb + w * M::XB) + turn * 8 * 32 + lane;
-                const float4* const from = (const float4*)(xb + (w ^ 1) * M::XB) + turn * 8 * 32 + lane;
+                float4* const to = (float4*)(xb + w * M::XB) + lane;
+                const float4* const from = (const float4*)(xb + (w ^ 1) * M::XB) + lane;
 #pragma unroll
                 for (int m = 0; m < 8; m++) to[m * 32] = make_float4(X[m][0], X[m][1], X[m][2], X[m][3]);
                 asm volatile("bar.sync %0, 64;" ::"r"(1 + p) : "memory");
@@ -715,25 +715,42 @@ sz_delta_chunk_kernel(const DlBatch d, const DlRule a, int idx0, int idx1, const
 #pragma unroll
                     for (int e = 0; e < 4; e++) dl_split(X[2 * ks + (e >> 1)][2 * (e & 1)], X[2 * ks + (e >> 1)][2 * (e & 1) + 1], rh[ks][e], rl[ks][e]);
             }
-            // ---- the rows' changes D^T = R^T T^T
+            // ---- the rows' changes D^T = R^T T^T: a pair of warps halves the rows
+            auto change = [&](float (*x)[4], int tiles, auto tile_of) {
 #pragma unroll
-            for (int m = 0; m < 8; m++)
+                for (int j = 0; j < tiles; j++)
 #pragma unroll
-                for (int e = 0; e < 4; e++) X[m][e] = 0.f;
+                    for (int e = 0; e < 4; e++) x[j][e] = 0.f;
 #pragma unroll
-            for (int ks = 0; ks < 4; ks++) {
-                uint2 f[8];
+                for (int ks = 0; ks < 4; ks++) {
+                    uint2 f[8];
 #pragma unroll
-                for (int m = 2 * ks; m < 8; m++) f[m] = ((const uint2*)hp)[(dl_tile(m) + ks) * 32 + lane];
+                    for (int j = 0; j < tiles; j++) if (ks <= tile_of(j) / 2) f[j] = ((const uint2*)hp)[(dl_tile(tile_of(j)) + ks) * 32 + lane];
 #pragma unroll
-                for (int m = 2 * ks; m < 8; m++) dl_mma(X[m], rh[ks], f[m].x, f[m].y);
+                    for (int j = 0; j < tiles; j++) if (ks <= tile_of(j) / 2) dl_mma(x[j], rh[ks], f[j].x, f[j].y);
 #pragma unroll
-                for (int m = 2 * ks; m < 8; m++) dl_mma(X[m], rl[ks], f[m].x, f[m].y);
+                    for (int j = 0; j < tiles; j++) if (ks <= tile_of(j) / 2) dl_mma(x[j], rl[ks], f[j].x, f[j].y);
 #pragma unroll
-                for (int m = 2 * ks; m < 8; m++) f[m] = ((const uint2*)(hp + DL_FRAG))[(dl_tile(m) + ks) * 32 + lane];
+                    for (int j = 0; j < tiles; j++) if (ks <= tile_of(j) / 2) f[j] = ((const uint2*)(hp + DL_FRAG))[(dl_tile(tile_of(j)) + ks) * 32 + lane];
 #pragma unroll
-                for (int m = 2 * ks; m < 8; m++) dl_mma(X[m], rh[ks], f[m].x, f[m].y);
-            }
+                    for (int j = 0; j < tiles; j++) if (ks <= tile_of(j) / 2) dl_mma(x[j], rh[ks], f[j].x, f[j].y);
+                }
+            };
+            if constexpr (NQ == 2) {
+                float Z[4][4];
+                if (q == 0) change(Z, 4, [](int j) { return j < 2 ? j : j + 4; });
+                else change(Z, 4, [](int j) { return j + 2; });
+                float4* const to = (float4*)(xb + w * M::XB) + 8 * 32 + lane;
+                const float4* const from = (const float4*)(xb + (w & ~1) * M::XB) + 8 * 32 + lane;
+#pragma unroll
+                for (int j = 0; j < 4; j++) to[j * 32] = make_float4(Z[j][0], Z[j][1], Z[j][2], Z[j][3]);
+                asm volatile("bar.sync %0, 64;" ::"r"(1 + p) : "memory");
+#pragma unroll
+                for (int m = 0; m < 8; m++) {
+                    const float4 y = from[(m >= 2 && m < 6 ? M::XB / 16 : 0) + (m < 2 ? m : m < 6 ? m - 2 : m - 4) * 32];
+                    X[m][0] = y.x; X[m][1] = y.y; X[m][2] = y.z; X[m][3] = y.w;
+                }
+            } else change(X, 8, [](int j) { return j; });
             if (OUT) {                                                    // for the outputs: half of it a warp
 #pragma unroll
                 for (int k = 0; k < 4 / NQ; k++) {
@@ -742,10 +759,10 @@ sz_delta_chunk_kernel(const DlBatch d, const DlRule a, int idx0, int idx1, const
                     for (int e = 0; e < 4; e++) {
                         const int m0 = 2 * k + (e >> 1), m1 = (4 / NQ) * 2 % 8 + m0;      // (of q = 0, of q = 1)
                         const float x0 = NQ == 2 && q ? X[m1][2 * (e & 1)] : X[m0][2 * (e & 1)], x1 = NQ == 2 && q ? X[m1][2 * (e & 1) + 1] : X[m0][2 * (e & 1) + 1];
-                        if (C::FULL) dl_split(x0, x1, hi[e], lo[e]); else hi[e] = dl_h2(x0, x1);
+                        dl_split(x0, x1, hi[e], lo[e]);
                     }
-                    df[(((turn * NG + p) * FP) * 4 + q * (4 / NQ) + k) * 32 + lane] = *(uint4*)hi;
-                    if (C::FULL) df[(((turn * NG + p) * FP + 1) * 4 + q * (4 / NQ) + k) * 32 + lane] = *(uint4*)lo;
+                    df[(((turn * NG + p) * 2) * 4 + q * (4 / NQ) + k) * 32 + lane] = *(uint4*)hi;
+                    df[(((turn * NG + p) * 2 + 1) * 4 + q * (4 / NQ) + k) * 32 + lane] = *(uint4*)lo;
                 }
                 if (lane == 0 && q == 0) d_unit[turn * NG + p] = dl_pow2(ew) * (1.f / DL_P);
                 arrive(&d_there[turn * NG + p]);
@@ -790,7 +807,7 @@ sz_delta_chunk_kernel(const DlBatch d, const DlRule a, int idx0, int idx1, const
     }
     if constexpr (OUT) {
         // ---- the outputs: e^G Q S + P D, of OT 8-row tiles a warp (of pairs of like work)
-        auto mine = [&](int i) { return q == 0 ? (i < 2 ? i : i + 4) : i + 2; };
+        auto mine = [&](int i) { return OT == 2 ? 2 * q + i : q == 0 ? (i < 2 ? i : i + 4) : i + 2; };
         float O[4 * OT];
         float nw[2] = {0.f, 0.f};
         if (norm) { nw[0] = a.norm[dv + g]; nw[1] = a.norm[dv + g + 8]; }
@@ -836,7 +853,7 @@ sz_delta_chunk_kernel(const DlBatch d, const DlRule a, int idx0, int idx1, const
             const u8* const st = rb + slot * M::B;
             const u32 sq = sz_smem_addr(st);
             const u8* const hp = st + C::ROWS / 2;
-            const float* const sc = (const float*)(hp + (C::FULL ? 2 : 1) * DL_FRAG);
+            const float* const sc = (const float*)(hp + 2 * DL_FRAG);
             const u8* const zt = hp + C::HB;
             float zd[M::STAGED ? 1 : 4 * OT];                             // (f32: the gates, asked for early)
             if (!M::STAGED && norm) {
@@ -863,8 +880,8 @@ sz_delta_chunk_kernel(const DlBatch d, const DlRule a, int idx0, int idx1, const
 #pragma unroll
                 for (int j = 0; j < NQ; j++) {
                     u32 hi[4], lo[4];
-                    *(uint4*)hi = sf[(((turn * NC + p * NQ + j) * FP) * 4 + ks) * 32 + lane];
-                    if (C::FULL) *(uint4*)lo = sf[(((turn * NC + p * NQ + j) * FP + 1) * 4 + ks) * 32 + lane];
+                    *(uint4*)hi = sf[(((turn * NC + p * NQ + j) * 2) * 4 + ks) * 32 + lane];
+                    *(uint4*)lo = sf[(((turn * NC + p * NQ + j) * 2 + 1) * 4 + ks) * 32 + lane];
 #pragma unroll
                     for (int i = 0; i < OT; i += 2) {
                         const u32 at = dl_at<D>(8 * mine(i) + ((lane >> 4) << 3) + (lane & 7), 8 * j + 2 * ks + ((lane >> 3) & 1));
@@ -872,7 +889,8 @@ sz_delta_chunk_kernel(const DlBatch d, const DlRule a, int idx0, int idx1, const
                         dl_ldsm(b, sq + at);
                         dl_mma(Y[j][i], hi, b[0], b[1]);
                         dl_mma(Y[j][i + 1], hi, b[2], b[3]);
-                        if (C::FULL) { dl_mma(Y[j][i], lo, b[0], b[1]); dl_mma(Y[j][i + 1], lo, b[2], b[3]); }
+                        dl_mma(Y[j][i], lo, b[0], b[1]);
+                        dl_mma(Y[j][i + 1], lo, b[2], b[3]);
                         if (NK == 2) {
                             dl_ldsm(b, sq + C::TILE + at);
                             dl_mma(Y[j][i], hi, b[0], b[1]);
@@ -897,10 +915,10 @@ sz_delta_chunk_kernel(const DlBatch d, const DlRule a, int idx0, int idx1, const
 #pragma unroll
             for (int ks = 0; ks < 4; ks++) {
                 u32 hi[4], lo[4];
-                *(uint4*)hi = df[(((turn * NG + p) * FP) * 4 + ks) * 32 + lane];
-                if (C::FULL) *(uint4*)lo = df[(((turn * NG + p) * FP + 1) * 4 + ks) * 32 + lane];
+                *(uint4*)hi = df[(((turn * NG + p) * 2) * 4 + ks) * 32 + lane];
+                *(uint4*)lo = df[(((turn * NG + p) * 2 + 1) * 4 + ks) * 32 + lane];
 #pragma unroll
-                for (int part = 0; part < (C::FULL ? 3 : 1); part++)      // high high, low high, high low
+                for (int part = 0; part < 3; part++)                      // high high, low high, high low
 #pragma unroll
                     for (int i = 0; i < OT; i++)
                         if (ks <= mine(i) / 2) {
