@@ -11,8 +11,8 @@ constexpr int DL_SM = 148;           // multiprocessors (a GPU with another numb
 // ---- the causal convolution --------------------------------------------------------------------------------------------------------------
 // y[r][c] = silu(bias[c] + sum_t w[c][t] x[r - (K - 1) + t][c]); rows before a sequence's first are those its slot carries (K - 1, the oldest first).  The taps are
 // added in f32 from the oldest on.  A thread has DL_V neighbouring channels and `tile` rows, one after the other, with the window in registers and the next
-// DL_AHEAD rows asked for; the one that has a sequence's first row leaves the new carried rows, which are rows of the call or of the old slot (so nothing is
-// read after somebody else wrote it).  8,192 channels over 4 rows, bf16: 4,093 rows 38.5 us (134 MB, 20.5 us of them; a row of 4 channels is some 45 instructions, two
+// DL_AHEAD rows asked for.  The block that has a sequence's first row is the only one that looks at its slot: it does the rows up to the K - 1st, those of the next tile
+// among them, and then leaves the new carried rows, which are rows of the call or of the old slot (the place is the same where a sequence goes on in place).  8,192 channels over 4 rows, bf16: 4,093 rows 38.5 us (134 MB, 20.5 us of them; a row of 4 channels is some 45 instructions, two
 // exponentials' pipe a channel among them; with 8 rows ahead 42, in tiles of 16 rows 41), 163 rows of 64 sequences 9.3, one row 3.4 (a launch and the chain table,
 // slot, carried rows, store).  What a tile reads twice are its first K - 1 rows, from L2.
 constexpr int DL_AHEAD = 4, DL_V = 4;
@@ -72,7 +72,8 @@ sz_delta_conv_kernel(const DlBatch d, const DlConv a) {
     sz_pdl_wait();
     sz_pdl_trigger();
     const int own = a.tile ? -1 : blockIdx.y;
-    const int first = a.tile ? blockIdx.y * a.tile : max(d.row_start[own], 0), end = min(a.tile ? first + a.tile : d.row_start[own + 1], d.rows);
+    const int first = a.tile ? blockIdx.y * a.tile : max(d.row_start[own], 0);
+    int end = min(a.tile ? first + a.tile : d.row_start[own + 1], d.rows);
     const u8* const xc = a.x + (size_t)c0 * ESZ;
     auto ask = [&](int r) {                             // row r (x is not written meanwhile: y lies elsewhere)
         Raw q;
@@ -153,15 +154,22 @@ sz_delta_conv_kernel(const DlBatch d, const DlConv a) {
                 next = nb > r ? nb : end;           // (a descending table: reported, and nobody's rows)
                 const DlSeq s = dl_seq(d, b, lane, blockIdx.x == 0);
                 if (s.on) {
-                    from = s.r0;
+                    // (a tile that begins inside a sequence: from its K - 1st row on, the others are the block's that has its first)
+                    from = r == s.r0 ? r : max(r, s.r0 + K - 1);
                     upto = s.r0 + s.n;
-                    if (mine && (r < upto || r == s.r0)) {
-                        // the rows before r: of the sequence, of its slot, or zeros
+                    if (r == s.r0 && min(upto, r + K - 1) > end) {
+                        const int was = end;
+                        end = min(upto, r + K - 1);
+#pragma unroll
+                        for (int j = 0; j < DL_AHEAD; j++) if (r + 1 + j >= was) ahead[j] = ask(r + 1 + j);
+                    }
+                    if (mine && (from < upto || r == s.r0)) {
+                        // the rows before `from`: of the sequence, of its slot, or zeros
 #pragma unroll
                         for (int t = 0; t < K - 1; t++) {
-                            const int p = r - (K - 1) + t - s.r0;    // row p of the sequence
+                            const int p = from - (K - 1) + t - s.r0; // row p of the sequence
                             if (p >= 0) { const Raw q = __ldcg((const Raw*)(xc + (size_t)(s.r0 + p) * a.x_stride)); pairs(q, win[t]); }
-                            else if (s.from >= 0) carried(s.from, K - 1 + p, win[t]);
+                            else if (s.from >= 0) carried(s.from, K - 1 + p, win[t]);      // (r is the first row)
                             else
 #pragma unroll
                                 for (int i = 0; i < V / 2; i++) win[t][i] = 0;
