@@ -1008,7 +1008,8 @@ int64_t dl_total(int n_seq, int rows, int least) { return rows / CK + (n_seq < r
 
 int64_t dl_chunk_bytes(int d, int kh, int vh, int io_type, int n_seq, int rows, int least) {
     const int64_t one = dl_chunk_one(d, kh, vh, io_type), total = dl_total(n_seq, rows, least), per = DL_SLAB / one < 8 ? 8 : DL_SLAB / one;
-    return one * (total < per ? total : per);
+    // (where not all chunks fit: the whole slab, whatever a chunk takes, so that no type of rows needs more than f32, whose chunks are the largest)
+    return total <= per ? one * total : one * per > DL_SLAB ? one * per : DL_SLAB;
 }
 
 int dl_chunk_launch(int d, int io_type, const DlBatch& b, const DlRule& r, uint64_t scratch, cudaStream_t st) {

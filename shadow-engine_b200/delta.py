@@ -80,7 +80,7 @@ class Step:
         self.b = DeltaBatchC(n_seq=n, rows=rows, max_rows=max_rows or 0, row_start=ptr(row_start), lens=ptr(lens), from_=ptr(slots), to=ptr(to), take=ptr(take))
         self._c, self._b = C.byref(states.c), C.byref(self.b)
         need = C.c_int64()
-        szlib.check(self.lib.sz_delta_scratch_bytes(self._c, self._b, szlib.TYPE_F32, C.byref(need)))      # (no type needs more)
+        szlib.check(self.lib.sz_delta_scratch_bytes(self._c, self._b, szlib.TYPE_F32, C.byref(need)))      # (no type of rows needs more)
         with self._here():
             self._mem = torch.empty(need.value + 256, dtype=torch.uint8, device=self.device)
             self.scratch, self.scratch_bytes = self._mem.data_ptr() + (-self._mem.data_ptr()) % 256, need.value

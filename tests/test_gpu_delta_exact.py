@@ -22,3 +22,9 @@ def test_outputs_of_16_bits_are_those_of_32_rounded(io, d, rows):
     near = want.to(c.io).double()
     off = float((got.double() - near).square().sum().sqrt() / want.square().sum().sqrt())
     assert off <= (2.0 ** -12 if io == "bf16" else 2.0 ** -13.5), off
+
+
+@pytest.mark.parametrize("io", ["bf16", "f16"])
+def test_a_prompt_past_the_slab_of_heads_whose_f32_chunks_fill_it_worse(io):
+    """A whole number of f32 chunks may take less of the scratch's slab than one of 16-bit chunks: the step's scratch holds either."""
+    Case([16400], [3], kh=8, vh=16, d=64, io=io, grouped=True, gate=False, v_scale=0.5).check_rule()
