@@ -350,7 +350,8 @@ int sz_logprob_rows(int logits_type, uint64_t logits, int64_t logits_stride, int
  * those behind them are neither read nor written.  So a host that verifies drafts writes to other slots and, once it knows what is kept, runs the kept
  * rows again from the old ones (sz_delta_rows without q and out is that replay), or keeps the new slot where all were.  A sequence without rows is left alone.
  * Tables are device memory, read when the kernels run; they must not change meanwhile.  Two sequences may start from one slot (a fork).  One that reads or
- * writes a slot which an earlier one of the call writes, or writes one that an earlier one reads, is left out and reported. */
+ * writes a slot which an earlier one of the call writes, or writes one that an earlier one reads, is left out and reported (earlier ones whose slots or rows are out of
+ * range touch none and do not count). */
 typedef struct sz_delta_pool {
     int32_t n_slots;
     int32_t k_heads, v_heads, head_dim;   /* v_heads a multiple of k_heads, up to 1024; head_dim 64 or 128 */

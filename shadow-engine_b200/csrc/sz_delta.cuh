@@ -102,7 +102,7 @@ __device__ __forceinline__ float dl_log_decay(float alpha, float a, float dt) {
 }
 
 // Sequence b as one warp sees it (all lanes with the same b).  An earlier sequence with rows that writes a slot which b reads or writes, or reads one
-// that b writes, keeps b out: whatever the order of the blocks, the results are the same.
+// that b writes, keeps b out: whatever the order of the blocks, the results are the same.  One whose own entries do not fit touches no slot and keeps nobody out.
 __device__ __forceinline__ DlSeq dl_seq(const DlBatch& d, int b, int lane, bool report) {
     DlSeq s;
     // (a lane's first sequence before b is asked for together with b itself: one wait, not three)
@@ -123,8 +123,9 @@ __device__ __forceinline__ DlSeq dl_seq(const DlBatch& d, int b, int lane, bool 
         bool clash = false;
         for (int i = lane; i < b; i += 32) {
             if (i >= 32) ask(i);
-            const int c = p1 - p0, reads = pl > c ? pf : -1;
-            clash |= c > 0 && (pt == to || pt == s.from || reads == to);
+            const bool reads = pl > p1 - p0;
+            if (p0 < 0 || p1 <= p0 || p1 > d.rows || (u32)pt >= (u32)d.n_slots || (reads && (u32)pf >= (u32)d.n_slots)) continue;      // (without rows, or left out itself)
+            clash |= pt == to || pt == s.from || (reads && pf == to);
         }
         if (__any_sync(0xffffffffu, clash)) bad |= DL_E_CLASH;
     }

@@ -53,3 +53,36 @@ def test_drafts_of_a_batch(io, max_rows):
 
 def test_prompts_that_go_on():
     in_place([1, 30, 1, 700, 2, 63, 64, 3, 400], [7] * 9, kh=16, vh=32, d=128, io="bf16")
+
+
+@pytest.mark.parametrize("rows", [3, 80])
+@pytest.mark.parametrize("slots, to, past, starts, out", [
+    ((1, 2, 3), (-1, 2, 3), (5, 0, 5), None, (0,)),                  # goes nowhere; the next one is new and comes from nowhere
+    ((-1, 2, 3), (-1, 2, 3), (5, 0, 0), None, (0,)),
+    ((1, 2, 1), (2, 99, 1), (0, 5, 5), None, (1,)),                  # reads what the first writes, besides
+    ((99, 4, 2), (4, 4, 2), (5, 5, 5), None, (0,)),                  # would write where the next one goes on
+    ((1, 2, 1), (1, 2, 1), (5, 5, 5), -4, (0,)),                     # rows out of range, in the slot of another
+])
+def test_a_sequence_that_does_not_fit_takes_no_other_with_it(rows, slots, to, past, starts, out):
+    """The others' results are those beside a sequence that fits."""
+    for call in ("conv", "rule"):
+        c = Case([rows] * 3, list(past), d=64, io="f32", slots=list(slots), to=list(to), n_slots=6, seed=4)
+        ref = Case([rows] * 3, list(past), d=64, io="f32",
+                   slots=[5 if b in out else x for b, x in enumerate(slots)], to=[5 if b in out else x for b, x in enumerate(to)], n_slots=6, seed=4)
+        if starts is not None:
+            c.row_start[0] = starts
+        wrong = 1 if starts is None else 2
+        got, want = (torch.full((s.rows, s.ch) if call == "conv" else (s.rows, s.vh, s.d), 77.0, device="cuda") for s in (c, ref))
+        for s, y in ((c, got), (ref, want)):
+            if call == "conv":
+                s.step.conv(s.x, s.w, out=y)
+            else:
+                s.run(y)
+        assert c.step.status() == wrong and ref.step.status() == 0
+        for b in range(3):
+            cut = slice(rows * b, rows * b + rows)
+            if b in out:
+                assert bool((got[cut] == 77).all())
+            else:
+                assert torch.equal(got[cut], want[cut]) and bool((got[cut] != 77).any())
+                assert torch.equal(c.state[c.to[b]], ref.state[ref.to[b]]) and torch.equal(c.carried[c.to[b]], ref.carried[ref.to[b]])
