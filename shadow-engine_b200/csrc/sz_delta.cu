@@ -53,23 +53,7 @@ sz_delta_conv_kernel(const DlBatch d, const DlConv a) {
     using Raw = typename DlRaw<ESZ>::T;
     const int lane = threadIdx.x & 31, c0 = (blockIdx.x * 128 + threadIdx.x) * V;
     const bool mine = c0 < a.ch;                        // (a warp stays together: its lanes look sequences up together)
-    u64 w[K][V / 2], bias[V / 2];
-#pragma unroll
-    for (int i = 0; i < V / 2; i++) bias[i] = 0;
-    if (mine) {
-        float wt[K * V];
-        const float4* src = (const float4*)(a.w + (size_t)c0 * K);
-#pragma unroll
-        for (int i = 0; i < K * V / 4; i++) *(float4*)(wt + 4 * i) = __ldg(src + i);
-#pragma unroll
-        for (int i = 0; i < V / 2; i++)
-#pragma unroll
-            for (int t = 0; t < K; t++) w[t][i] = dl_pack2(wt[2 * i * K + t], wt[(2 * i + 1) * K + t]);
-        if (a.bias)
-#pragma unroll
-            for (int i = 0; i < V / 2; i++) { const float2 x = __ldg((const float2*)(a.bias + c0 + 2 * i)); bias[i] = dl_pack2(x.x, x.y); }
-    }
-    sz_pdl_wait();
+    sz_pdl_wait();                                      // (weights and bias, too, may come from the kernel before)
     sz_pdl_trigger();
     const int own = a.tile ? -1 : blockIdx.y;
     const int first = a.tile ? blockIdx.y * a.tile : max(d.row_start[own], 0);
@@ -99,6 +83,22 @@ sz_delta_conv_kernel(const DlBatch d, const DlConv a) {
     Raw ahead[DL_AHEAD];
 #pragma unroll
     for (int j = 0; j < DL_AHEAD; j++) ahead[j] = ask(first + j);
+    u64 w[K][V / 2], bias[V / 2];
+#pragma unroll
+    for (int i = 0; i < V / 2; i++) bias[i] = 0;
+    if (mine) {
+        float wt[K * V];
+        const float4* src = (const float4*)(a.w + (size_t)c0 * K);
+#pragma unroll
+        for (int i = 0; i < K * V / 4; i++) *(float4*)(wt + 4 * i) = src[i];
+#pragma unroll
+        for (int i = 0; i < V / 2; i++)
+#pragma unroll
+            for (int t = 0; t < K; t++) w[t][i] = dl_pack2(wt[2 * i * K + t], wt[(2 * i + 1) * K + t]);
+        if (a.bias)
+#pragma unroll
+            for (int i = 0; i < V / 2; i++) { const float2 x = *(const float2*)(a.bias + c0 + 2 * i); bias[i] = dl_pack2(x.x, x.y); }
+    }
     u64 win[K][V / 2];                                  // the rows before the next one, and it
     int b = own, from = first, upto = first;            // the current sequence's rows here: from .. upto
     int next = first;                                   // where the one behind it begins

@@ -86,3 +86,20 @@ def test_a_sequence_that_does_not_fit_takes_no_other_with_it(rows, slots, to, pa
             else:
                 assert torch.equal(got[cut], want[cut]) and bool((got[cut] != 77).any())
                 assert torch.equal(c.state[c.to[b]], ref.state[ref.to[b]]) and torch.equal(c.carried[c.to[b]], ref.carried[ref.to[b]])
+
+
+def test_weights_that_the_kernel_before_writes():
+    """`conv(x, weight.float(), ..)`, again and again: weights, bias and rows are those that are there when the call's turn comes."""
+    c = Case([3, 1], [9, 4], kh=16, vh=32, d=128, io="bf16", fork=True)
+    half, bias = c.w.bfloat16(), c.bias.bfloat16()
+    w, b = torch.zeros_like(c.w), torch.zeros_like(c.bias)
+    got = []
+    for i in range(40):
+        w.copy_(half * (i + 1))
+        b.copy_(bias * (i - 7))
+        got.append(c.step.conv(c.x, w, bias=b))
+    for i, y in enumerate(got):
+        w, b = (half * (i + 1)).float(), (bias * (i - 7)).float()
+        torch.cuda.synchronize()
+        assert torch.equal(y, c.step.conv(c.x, w, bias=b)), i
+    assert c.step.status() == 0
