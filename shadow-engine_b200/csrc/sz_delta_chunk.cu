@@ -1,11 +1,11 @@
 // The gated delta rule over many rows of a sequence, in chunks of CK = 64 (sz_delta.cuh has the row-by-row form's neighbours).
 //
 // With S the state before a chunk, G_i the sum of the decays' logarithms up to its row i, and k, q the normed rows, the rows' changes d_i solve a triangular system:
-//   (I + A) D = diag(beta) (V - diag(e^G) K S),   A_ij = beta_i e^(G_i - G_j) k_i.k_j for j < i
+//   (I + A) D = R = diag(beta) (V - diag(e^G) K S),   A_ij = beta_i e^(G_i - G_j) k_i.k_j for j < i
 //   O = diag(e^G) Q S + P D,   P_ij = e^(G_i - G_j) q_i.k_j for j <= i
 //   S' = e^G_C S + sum_j e^(G_C - G_j) k_j d_j^T
 // so that a chunk is a few matrix products instead of 64 steps.  Two kernels:
-//  sz_delta_prep_kernel, a block a chunk and key head: what does not need S - the products of its rows, T = (I + A)^-1 diag(beta) and P of every value head of the
+//  sz_delta_prep_kernel, a block a chunk and key head: what does not need S - the products of its rows, T = (I + A)^-1 and P of every value head of the
 //   key head - side by side, over all chunks at once;
 //  sz_delta_chunk_kernel, a block of warps for 16 NG value dimensions of a sequence's value head: the chain over its chunks, on mma.sync.  Everything is
 //   transposed, so that a warp's 16 value dimensions are a product's rows: S^T (f32) stays in its registers, and what one product gives is in the layout in which
@@ -16,7 +16,8 @@
 // a chunk) and S through a conversion by four warps: no sooner.
 //
 // Numbers.  A row k = rho 2^e (k 2^-e) enters the products as k 2^-e with its largest element in [1, 2): a bf16 or f16 row is exact in f16, an f32 row is two f16
-// numbers (22 bits); the rows' lengths and powers are factors in f32.  S, R = V - e^G K S and D enter as two f16 numbers each, in units of a power of two that
+// numbers (22 bits); the rows' lengths and powers are factors in f32, and so is beta: a chunk whose gates are all but closed keeps the digits of its small changes, where T diag(beta) in f16
+// has none below 2^-25.  (T's elements are at most 1, its diagonal is 1.)  S, R and D enter as two f16 numbers each, in units of a power of two that
 // the warp takes from the largest there is: 22 bits, and what is less than 2^-35 of that largest is lost.  Sums are f32.  T and the decays' sums: f32 and f64.
 // (One f16 number a factor in the last products of bf16 outputs, 11 bits where they keep 8: their difference from rounded f32 outputs is 1.1 10^-3 of their size instead of 10^-5, and 4,093 rows take 202 us.)
 #include "sz_delta.cuh"
@@ -28,7 +29,7 @@ constexpr int DL_FRAG = DL_TILES * 32 * 8;               // bytes of a triangle 
 constexpr float DL_P = 1024.f;                           // P's elements are at most 1 / sqrt(d): times this they keep their 22 bits
 constexpr int64_t DL_SLAB = 96ll << 20;                  // scratch that a pass over chunks may take (what the first kernel leaves is in L2 for the second)
 
-struct DlScalars { float gr[CK], wj[CK], gc, pad[15]; };              // e^G rho_k, e^(G_C - G_j) rho_k; e^G_C
+struct DlScalars { float gr[CK], beta[CK], wj[CK], gc, pad[15]; };    // beta e^G rho_k, beta, e^(G_C - G_j) rho_k; e^G_C
 
 template <int D, int TYPE> struct DlChunk {
     static constexpr int NK = TYPE == SZ_TYPE_F32 ? 2 : 1;                // f16 numbers of an element of k and q
@@ -344,10 +345,9 @@ sz_delta_prep_kernel(const DlBatch d, const DlRule a, int idx0, u8* __restrict__
             for (int k = 0; k < 4; k++) {
                 const int b = 2 * part + (k >> 1), m = 2 * b + (k & 1);
                 const float* w = dg + b * 16 * DL_DS + (8 * (k & 1) + g) * DL_DS + 2 * t;
-                const float* bt = sBeta[half] + 16 * b + 2 * t;
                 uint2 hi, lo;
-                dl_split(w[0] * bt[0], w[1] * bt[1], hi.x, lo.x);
-                dl_split(w[8] * bt[8], w[9] * bt[9], hi.y, lo.y);
+                dl_split(w[0], w[1], hi.x, lo.x);
+                dl_split(w[8], w[9], hi.y, lo.y);
                 th[(dl_tile(m) + b) * 32 + lane] = hi;
                 tl[(dl_tile(m) + b) * 32 + lane] = lo;
             }
@@ -364,8 +364,6 @@ sz_delta_prep_kernel(const DlBatch d, const DlRule a, int idx0, u8* __restrict__
                             dl_split(y[0], y[DL_DS], xh[0][e], xl[0][e]);
                         }
                     }
-                    const float* bt = sBeta[half] + 16 * b + g;
-                    const float be0 = -bt[0], be1 = -bt[8];
 #pragma unroll
                     for (int ab = b + 1; ab < 4; ab++) {
                         float y[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}}, z[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
@@ -396,10 +394,10 @@ sz_delta_prep_kernel(const DlBatch d, const DlRule a, int idx0, u8* __restrict__
 #pragma unroll
                             for (int e = 0; e < 4; e++) dl_split(-z[e >> 1][2 * (e & 1)], -z[e >> 1][2 * (e & 1) + 1], xh[ab - b][e], xl[ab - b][e]);
 #pragma unroll
-                        for (int u = 0; u < 2; u++) {        // rows 8 (2 ab + u) .., columns 16 b ..: turned around, times beta of their column
+                        for (int u = 0; u < 2; u++) {        // rows 8 (2 ab + u) .., columns 16 b ..: turned around
                             u32 h0, l0, h1, l1;
-                            dl_split(z[u][0] * be0, z[u][1] * be0, h0, l0);
-                            dl_split(z[u][2] * be1, z[u][3] * be1, h1, l1);
+                            dl_split(-z[u][0], -z[u][1], h0, l0);
+                            dl_split(-z[u][2], -z[u][3], h1, l1);
                             const int at = (dl_tile(2 * ab + u) + b) * 32 + lane;
                             th[at] = make_uint2(dl_turn(h0), dl_turn(h1));
                             tl[at] = make_uint2(dl_turn(l0), dl_turn(l1));
@@ -410,7 +408,8 @@ sz_delta_prep_kernel(const DlBatch d, const DlRule a, int idx0, u8* __restrict__
             const int r = 32 * part + lane;
             const double G = sG[half][r], GC = sG[half][CK - 1];
             const float eg = expf((float)G);
-            sc->gr[r] = eg * sRk[r];
+            sc->gr[r] = sBeta[half][r] * (eg * sRk[r]);
+            sc->beta[r] = sBeta[half][r];
             if (OUT) ((float*)(hp + C::HEAD))[r - CK] = eg * sRq[r];
             sc->wj[r] = expf((float)(GC - G)) * sRk[r];
             if (r == 0) sc->gc = expf((float)GC);
@@ -688,16 +687,16 @@ sz_delta_chunk_kernel(const DlBatch d, const DlRule a, int idx0, int idx1, const
                     X[m][0] += y.x; X[m][1] += y.y; X[m][2] += y.z; X[m][3] += y.w;
                 }
             }
-            // ---- R = V - e^G K S, in units of 2^ew
+            // ---- R = beta (V - e^G K S), in units of 2^ew
 #pragma unroll
             for (int m = 0; m < 8; m += 2) {
                 float v[8];
                 turned(hp + C::HA, m, v);
 #pragma unroll
                 for (int u = 0; u < 2; u++) {
-                    const float2 gr = *(const float2*)(sc->gr + 8 * (m + u) + 2 * t);
+                    const float2 gr = *(const float2*)(sc->gr + 8 * (m + u) + 2 * t), be = *(const float2*)(sc->beta + 8 * (m + u) + 2 * t);
 #pragma unroll
-                    for (int e = 0; e < 4; e++) X[m + u][e] = fmaf(-(e & 1 ? gr.y : gr.x), X[m + u][e], v[4 * u + e]);
+                    for (int e = 0; e < 4; e++) X[m + u][e] = fmaf(-(e & 1 ? gr.y : gr.x), X[m + u][e], (e & 1 ? be.y : be.x) * v[4 * u + e]);
                 }
             }
             int ew = es;

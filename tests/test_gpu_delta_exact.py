@@ -28,3 +28,21 @@ def test_outputs_of_16_bits_are_those_of_32_rounded(io, d, rows):
 def test_a_prompt_past_the_slab_of_heads_whose_f32_chunks_fill_it_worse(io):
     """A whole number of f32 chunks may take less of the scratch's slab than one of 16-bit chunks: the step's scratch holds either."""
     Case([16400], [3], kh=8, vh=16, d=64, io=io, grouped=True, gate=False, v_scale=0.5).check_rule()
+
+
+@pytest.mark.parametrize("io", ["f32", "bf16"])
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("rows", [20, 300])
+@pytest.mark.parametrize("gate", [-8.0, -12.0, -16.0, -40.0])
+def test_changes_behind_gates_that_are_all_but_closed(io, d, rows, gate):
+    """A new sequence's state is its small changes alone.  An element is a sum over rows of k (2^-23 off by its length), a change (R and T as two f16 numbers, 2^-21 in all; beta's
+    exponential and quotient 2^-22; sums of 64 products 2^-22) and a decay, the exponential of a sum of up to 16 that matters (16 half steps, 2^-20): below 2^-18.5 of the column's length, sums over rows
+    and chunks of errors of either sign not above that of one times 2^0.5."""
+    c = Case([rows], [0], d=d, io=io, gate=False, seed=rows + d)
+    c.beta.fill_(gate)
+    _, _, pool, _ = c.want_rule()
+    want = pool[c.to[0]]
+    c.run()
+    assert c.step.status() == 0
+    off = (c.state[c.to[0]].double() - want).square().sum(1).sqrt() / want.square().sum(1).sqrt()
+    assert float(off.max()) <= 2.0 ** -18, float(off.max())
