@@ -29,7 +29,7 @@ constexpr int DL_FRAG = DL_TILES * 32 * 8;               // bytes of a triangle 
 constexpr float DL_P = 1024.f;                           // P's elements are at most 1 / sqrt(d): times this they keep their 22 bits
 constexpr int64_t DL_SLAB = 96ll << 20;                  // scratch that a pass over chunks may take (what the first kernel leaves is in L2 for the second)
 
-struct DlScalars { float gr[CK], beta[CK], wj[CK], gc, pad[15]; };    // beta e^G rho_k, beta, e^(G_C - G_j) rho_k; e^G_C
+struct DlScalars { float gr[CK], beta[CK], wj[CK], gc; int ex; float pad[14]; };      // - beta e^G rho_k, beta, 2^-ex e^(G_C - G_j) rho_k; e^G_C, and what makes the largest wj 1 to 2
 
 template <int D, int TYPE> struct DlChunk {
     static constexpr int NK = TYPE == SZ_TYPE_F32 ? 2 : 1;                // f16 numbers of an element of k and q
@@ -408,10 +408,14 @@ sz_delta_prep_kernel(const DlBatch d, const DlRule a, int idx0, u8* __restrict__
             const int r = 32 * part + lane;
             const double G = sG[half][r], GC = sG[half][CK - 1];
             const float eg = expf((float)G);
-            sc->gr[r] = sBeta[half][r] * (eg * sRk[r]);
+            sc->gr[r] = -sBeta[half][r] * (eg * sRk[r]);
             sc->beta[r] = sBeta[half][r];
             if (OUT) ((float*)(hp + C::HEAD))[r - CK] = eg * sRq[r];
-            sc->wj[r] = expf((float)(GC - G)) * sRk[r];
+            const float wj = expf((float)(GC - G)) * sRk[r], wo = expf((float)(GC - sG[half][r ^ 32])) * sRk[r ^ 32];
+            const int top = (int)(__reduce_max_sync(0xffffffffu, __float_as_uint(fmaxf(wj, wo))) >> 23);
+            const int ex = top == 0 || top == 255 ? 0 : max(-100, min(0, top - 127));
+            sc->wj[r] = wj * dl_pow2(-ex);
+            if (r == 0) sc->ex = ex;
             if (r == 0) sc->gc = expf((float)GC);
         }
         if (v0 + 2 < ratio) {
@@ -694,15 +698,22 @@ sz_delta_chunk_kernel(const DlBatch d, const DlRule a, int idx0, int idx1, const
                 turned(hp + C::HA, m, v);
 #pragma unroll
                 for (int u = 0; u < 2; u++) {
-                    const float2 gr = *(const float2*)(sc->gr + 8 * (m + u) + 2 * t), be = *(const float2*)(sc->beta + 8 * (m + u) + 2 * t);
+                    const u64 gr = *(const u64*)(sc->gr + 8 * (m + u) + 2 * t), be = *(const u64*)(sc->beta + 8 * (m + u) + 2 * t);
 #pragma unroll
-                    for (int e = 0; e < 4; e++) X[m + u][e] = fmaf(-(e & 1 ? gr.y : gr.x), X[m + u][e], (e & 1 ? be.y : be.x) * v[4 * u + e]);
+                    for (int e = 0; e < 4; e += 2) {
+                        u64 y = dl_mul2(dl_pack2(v[4 * u + e], v[4 * u + e + 1]), be);
+                        dl_fma2(y, gr, dl_pack2(X[m + u][e], X[m + u][e + 1]));
+                        X[m + u][e] = dl_lo(y); X[m + u][e + 1] = dl_hi(y);
+                    }
                 }
             }
-            int ew = es;
+            int ew = 0, next_es = es;
             {
                 const int top = exponent(X);
-                if (top != 0 && top != 255) ew = max(max(top - 127 - 8, -120), es - 100);      // (changes are at most 64 times the largest of R: below 2^15)
+                if (top != 0 && top != 255) {
+                    ew = max(top - 127 - 8, -120);                        // (changes are at most 64 times the largest of R: below 2^15)
+                    next_es = max(ew + sc->ex, es - 100);                 // .. and the state's next ones (short keys: the changes times their factors keep their digits)
+                }
             }
             u32 rh[4][4], rl[4][4];
             {
@@ -766,16 +777,17 @@ sz_delta_chunk_kernel(const DlBatch d, const DlRule a, int idx0, int idx1, const
                 if (lane == 0 && q == 0) d_unit[turn * NG + p] = dl_pow2(ew) * (1.f / DL_P);
                 arrive(&d_there[turn * NG + p]);
             }
-            // ---- the state: e^G_C S + K^T (e^(G_C - G_j) D)
+            // ---- the state: e^G_C S + K^T (e^(G_C - G_j) D), in units of 2^next_es
+            const float unit = dl_pow2(ew + sc->ex - next_es);            // (1 but for a state that is 2^92 times the changes)
 #pragma unroll
             for (int m = 0; m < 8; m++) {
-                const float2 wj = *(const float2*)(sc->wj + 8 * m + 2 * t);
-                X[m][0] *= wj.x; X[m][1] *= wj.y; X[m][2] *= wj.x; X[m][3] *= wj.y;
+                const u64 wj = dl_mul2(*(const u64*)(sc->wj + 8 * m + 2 * t), dl_pack2(unit, unit)), lo = dl_mul2(dl_pack2(X[m][0], X[m][1]), wj), hi = dl_mul2(dl_pack2(X[m][2], X[m][3]), wj);
+                X[m][0] = dl_lo(lo); X[m][1] = dl_hi(lo); X[m][2] = dl_lo(hi); X[m][3] = dl_hi(hi);
             }
-            const float f = sc->gc * dl_pow2(max(es - ew, -126));
+            const float f = sc->gc * dl_pow2(max(es - next_es, -126));
 #pragma unroll
             for (int m = 0; m < 8; m++) dl_scale4(S[m], f);
-            es = ew;
+            es = next_es;
 #pragma unroll
             for (int ks = 0; ks < 4; ks++) {
                 u32 hi[4], lo[4], b[4][4];

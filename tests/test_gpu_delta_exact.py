@@ -46,3 +46,18 @@ def test_changes_behind_gates_that_are_all_but_closed(io, d, rows, gate):
     assert c.step.status() == 0
     off = (c.state[c.to[0]].double() - want).square().sum(1).sqrt() / want.square().sum(1).sqrt()
     assert float(off.max()) <= 2.0 ** -18, float(off.max())
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("rows", [20, 300])
+@pytest.mark.parametrize("size", [1e-3, 1e-6, 1e-9, 1e-12])
+def test_short_keys(d, rows, size):
+    """Keys far below the 1e-3 that the norm adds in: states of a new sequence are as small, and as exact.  (The bound of above, and one bit for the sums of several chunks.)"""
+    c = Case([rows], [0], d=d, io="f32", gate=False, seed=rows + d)
+    c.k.mul_(size)
+    _, _, pool, _ = c.want_rule()
+    want = pool[c.to[0]]
+    c.run()
+    assert c.step.status() == 0
+    off = (c.state[c.to[0]].double() - want).square().sum(1).sqrt() / want.square().sum(1).sqrt()
+    assert float(off.max()) <= 2.0 ** -17, float(off.max())
