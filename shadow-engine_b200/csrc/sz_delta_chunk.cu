@@ -2,7 +2,7 @@
 //
 // With S the state before a chunk, G_i the sum of the decays' logarithms up to its row i, and k, q the normed rows, the rows' changes d_i solve a triangular system:
 //   (I + A) D = R = diag(beta) (V - diag(e^G) K S),   A_ij = beta_i e^(G_i - G_j) k_i.k_j for j < i
-//   O = diag(e^G) Q S + P D,   P_ij = e^(G_i - G_j) q_i.k_j for j <= i
+//   O = diag(e^G) Q S + P D,   P_ij = e^(G_i - G_j) q_i.k_j for j <= i (held without q_i's length)
 //   S' = e^G_C S + sum_j e^(G_C - G_j) k_j d_j^T
 // so that a chunk is a few matrix products instead of 64 steps.  Two kernels:
 //  sz_delta_prep_kernel, a block a chunk and key head: what does not need S - the products of its rows, T = (I + A)^-1 and P of every value head of the
@@ -26,7 +26,6 @@ namespace {
 
 constexpr int CK = 64, DL_TILES = 20;                    // rows of a chunk; 8 x 16 tiles of a lower triangle
 constexpr int DL_FRAG = DL_TILES * 32 * 8;               // bytes of a triangle in f16, in the order in which the matrix instruction takes it
-constexpr float DL_P = 1024.f;                           // P's elements are at most 1 / sqrt(d): times this they keep their 22 bits
 constexpr int64_t DL_SLAB = 96ll << 20;                  // scratch that a pass over chunks may take (what the first kernel leaves is in L2 for the second)
 
 struct DlScalars { float gr[CK], beta[CK], wj[CK], gc; int ex; float pad[14]; };      // - beta e^G rho_k, beta, 2^-ex e^(G_C - G_j) rho_k; e^G_C, and what makes the largest wj 1 to 2
@@ -34,12 +33,12 @@ struct DlScalars { float gr[CK], beta[CK], wj[CK], gc; int ex; float pad[14]; };
 template <int D, int TYPE> struct DlChunk {
     static constexpr int NK = TYPE == SZ_TYPE_F32 ? 2 : 1;                // f16 numbers of an element of k and q
     static constexpr int TILE = CK * D * 2, ROWS = 2 * NK * TILE;         // a key head's rows: k (high, low), q (high, low)
-    // a value head's T (high, low) and scalars, for the chain; P (high, low) and e^G rho_q, for the outputs
-    static constexpr int HA = 2 * DL_FRAG + (int)sizeof(DlScalars), HB = 2 * DL_FRAG + CK * 4, HEAD = HA + HB;
+    // a value head's T (high, low) and scalars, for the chain; P (high, low), e^G rho_q and rho_q, for the outputs
+    static constexpr int HA = 2 * DL_FRAG + (int)sizeof(DlScalars), HB = 2 * DL_FRAG + 2 * CK * 4, HEAD = HA + HB;
 };
 int64_t dl_chunk_one(int d, int kh, int vh, int io_type) {
     const int nk = io_type == SZ_TYPE_F32 ? 2 : 1;
-    return (int64_t)kh * 2 * nk * CK * d * 2 + (int64_t)vh * (4 * DL_FRAG + CK * 4 + (int)sizeof(DlScalars));
+    return (int64_t)kh * 2 * nk * CK * d * 2 + (int64_t)vh * (4 * DL_FRAG + 2 * CK * 4 + (int)sizeof(DlScalars));
 }
 
 // The sequences of many rows, in order: the y-th of them (y >= 0), or the one whose chunks have index idx.  Chunk c of a sequence has index
@@ -268,12 +267,11 @@ sz_delta_prep_kernel(const DlBatch d, const DlRule a, int idx0, u8* __restrict__
             u8* const af = sm + i * P::HEAD;
             float* const dg = (float*)(af + P::AF) + warp * 16 * DL_DS;
             u8* const hp = mine + (size_t)a.kh * C::ROWS + (size_t)head(v0 + i) * C::HEAD;
-            float ra[2], rp[2];
+            float ra[2];
 #pragma unroll
             for (int u = 0; u < 2; u++) {
                 const int r = 16 * warp + g + 8 * u;
                 ra[u] = sBeta[i][r] * sRk[r];
-                rp[u] = sRq[r] * DL_P;
             }
 #pragma unroll
             for (int m = 0; m < 8; m++)
@@ -287,7 +285,7 @@ sz_delta_prep_kernel(const DlBatch d, const DlRule a, int idx0, u8* __restrict__
                         if (own) f = j <= r ? expf((float)(sG[i][r] - sG[i][j])) * sRk[j] : 0.f;
                         else f = sE[i][r] * sB[i][warp][j];
                         x[e] = ra[u] * f * kk[m][e];
-                        p[e] = rp[u] * f * qk[m][e];
+                        p[e] = f * qk[m][e];
                         if (own && j > r) p[e] = 0.f;        // (whatever the product there is)
                         if (own) dg[(j & 15) * DL_DS + (r & 15)] = x[e];
                     }
@@ -410,7 +408,7 @@ sz_delta_prep_kernel(const DlBatch d, const DlRule a, int idx0, u8* __restrict__
             const float eg = expf((float)G);
             sc->gr[r] = -sBeta[half][r] * (eg * sRk[r]);
             sc->beta[r] = sBeta[half][r];
-            if (OUT) ((float*)(hp + C::HEAD))[r - CK] = eg * sRq[r];
+            if (OUT) { ((float*)(hp + C::HEAD))[r - 2 * CK] = eg * sRq[r]; ((float*)(hp + C::HEAD))[r - CK] = sRq[r]; }
             const float wj = expf((float)(GC - G)) * sRk[r], wo = expf((float)(GC - sG[half][r ^ 32])) * sRk[r ^ 32];
             const int top = (int)(__reduce_max_sync(0xffffffffu, __float_as_uint(fmaxf(wj, wo))) >> 23);
             const int ex = top == 0 || top == 255 ? 0 : max(-100, min(0, top - 127));
@@ -774,7 +772,7 @@ sz_delta_chunk_kernel(const DlBatch d, const DlRule a, int idx0, int idx1, const
                     df[(((turn * NG + p) * 2) * 4 + q * (4 / NQ) + k) * 32 + lane] = *(uint4*)hi;
                     df[(((turn * NG + p) * 2 + 1) * 4 + q * (4 / NQ) + k) * 32 + lane] = *(uint4*)lo;
                 }
-                if (lane == 0 && q == 0) d_unit[turn * NG + p] = dl_pow2(ew) * (1.f / DL_P);
+                if (lane == 0 && q == 0) d_unit[turn * NG + p] = dl_pow2(ew);
                 arrive(&d_there[turn * NG + p]);
             }
             // ---- the state: e^G_C S + K^T (e^(G_C - G_j) D), in units of 2^next_es
@@ -942,9 +940,9 @@ sz_delta_chunk_kernel(const DlBatch d, const DlRule a, int idx0, int idx1, const
             float N[4 * OT];
 #pragma unroll
             for (int i = 0; i < OT; i++) {
-                const float2 gq = *(const float2*)(sc + 8 * mine(i) + 2 * t);
+                const float2 gq = *(const float2*)(sc + 8 * mine(i) + 2 * t), rq = *(const float2*)(sc + CK + 8 * mine(i) + 2 * t);
 #pragma unroll
-                for (int e = 0; e < 4; e++) N[4 * i + e] = fmaf(e & 1 ? gq.y : gq.x, Y[0][i][e], acc[i][e] * tw);
+                for (int e = 0; e < 4; e++) N[4 * i + e] = fmaf(e & 1 ? gq.y : gq.x, Y[0][i][e], acc[i][e] * ((e & 1 ? rq.y : rq.x) * tw));
             }
             if (norm) {
 #pragma unroll
@@ -984,7 +982,7 @@ template <int D, int TYPE, int NG, bool OUT>
 int dl_chunk_go(const DlBatch& b, const DlRule& r, int longest, int64_t total, int64_t per, uint64_t scratch, cudaStream_t st) {
     using P = DlPrep<D, TYPE>;
     using M = DlMain<D, TYPE, NG, OUT>;
-    static_assert(M::SMEM <= 227 * 1024 && P::SMEM <= 72 * 1024, "");
+    static_assert(M::SMEM <= 227 * 1024 && P::SMEM <= 72 * 1024 && sizeof(DlScalars) % 16 == 0, "");
     const auto prep = sz_delta_prep_kernel<D, TYPE, OUT>;
     const auto chain = sz_delta_chunk_kernel<D, TYPE, NG, OUT>;
     int rc = sz_allow_smem((const void*)prep, (int)P::SMEM);

@@ -61,3 +61,18 @@ def test_short_keys(d, rows, size):
     assert c.step.status() == 0
     off = (c.state[c.to[0]].double() - want).square().sum(1).sqrt() / want.square().sum(1).sqrt()
     assert float(off.max()) <= 2.0 ** -17, float(off.max())
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("rows", [20, 300])
+@pytest.mark.parametrize("size", [1.0, 1e-3, 1e-6, 1e-9, 1e-12])
+def test_short_queries(d, rows, size):
+    """Queries as short: a row of outputs is a product of them with the state, whose columns it may turn away from.  (Errors of the above against outputs of 2^-1.5 and more of what their rows could
+    be at most: 2^-15.5.)"""
+    c = Case([rows], [0], d=d, io="f32", gate=False, seed=rows + d)
+    c.q.mul_(size)
+    want, _, _, _ = c.want_rule()
+    got = c.run()
+    assert c.step.status() == 0
+    off = (got.double() - want).square().sum(2).sqrt() / want.square().sum(2).sqrt()
+    assert float(off.max()) <= 2.0 ** -15.5, float(off.max())
