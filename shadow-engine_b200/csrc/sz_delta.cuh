@@ -82,17 +82,19 @@ __device__ __forceinline__ float dl_load1(const u8* p) {
     else return __uint_as_float((u32) * (const u16*)p << 16);
 }
 
-// sigmoid: where 16 bits are kept of what it is multiplied with, by the fast exponential and quotient (2^-21 relative); for f32 with the rounding of the exponent put
-// back and a Newton step on the fast reciprocal (2^-22), a third of the time of sz_sigmoid
+// sigmoid: where 16 bits are kept of what it is multiplied with, by the fast exponential and quotient (2^-21 relative); for f32 e^y = 2^e (1 + rest log 2) with y log2(e) as a sum of two
+// f32 numbers, e and the rest that rounding it leaves (log2(e) itself in two numbers, products by fused multiply-adds), and the fast reciprocal with a step of Newton's method, r (2 - den r): 2^-22, a third
+// of the time of sz_sigmoid.  Beyond 87 it is 1, or 0 (2^-125 and less); of NaN it is NaN.
 template <int TYPE> __device__ __forceinline__ float dl_sigmoid(float x) {
     if (TYPE != SZ_TYPE_F32) return __fdividef(1.f, 1.f + __expf(-x));
     constexpr float L = 1.4426950408889634f, L_LOW = 1.925963033500e-8f;      // log2(e), and what f32 leaves of it
-    const float y = -x > 85.f ? 85.f : -x, e = y * L, rest = fmaf(y, L_LOW, fmaf(y, L, -e));
+    const float y = x < -87.f ? 87.f : x > 87.f ? -87.f : -x, e = y * L, rest = fmaf(y, L_LOW, fmaf(y, L, -e));
     float w, r;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(w) : "f"(e));
     const float den = 1.f + fmaf(w, rest * 0.6931471805599453f, w);
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(den));
-    return r * fmaf(-den, r, 2.f);
+    r *= fmaf(-den, r, 2.f);
+    return x < -87.f ? 0.f : r;
 }
 // The logarithm of a row's decay, a softplus(alpha + dt).  A decay above 1 (a positive `a`) counts as 1; one below e^-1000 is 0 in f32 as it is, and sums of these
 // keep the others' digits (in f64).

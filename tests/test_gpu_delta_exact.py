@@ -76,3 +76,44 @@ def test_short_queries(d, rows, size):
     assert c.step.status() == 0
     off = (got.double() - want).square().sum(2).sqrt() / want.square().sum(2).sqrt()
     assert float(off.max()) <= 2.0 ** -15.5, float(off.max())
+
+
+ENDS = [math.inf, 3e38, 1e30, 200.0, 88.0, 87.0, 86.0, 0.0, -86.0, -87.0, -88.0, -200.0, -1e30, -3e38]
+
+
+@pytest.mark.parametrize("io", ["f32", "bf16", "f16"])
+def test_gates_at_the_ends_of_the_exponential(io):
+    """A gate of +inf is open, of -inf shut; a NaN is one.  (Below -87 a sigmoid is less than 2^-125: 0.)"""
+    for rows in (20, 200):
+        c, ref = (Case([rows], [3], d=64, io=io, seed=1) for _ in range(2))
+        gates = torch.tensor(ENDS + [-math.inf], dtype=torch.float64, device="cuda")
+        for s in (c, ref):
+            s.z[:len(gates)] = gates.to(s.io)[:, None, None]
+        ref.z[:len(gates)] = 0
+        half, out = ref.run().double(), c.run()
+        want = half[:len(gates)] * 2 * torch.sigmoid(c.z[:len(gates), :1, :1].double())
+        step = {"f32": 2.0 ** -20, "bf16": 2.0 ** -7, "f16": 2.0 ** -10}[io]           # (half a step of each of the two, and of the gates)
+        assert bool(((out[:len(gates)].double() - want).abs() <= step * want.abs() + 2.0 ** -24).all())
+        c.z[5] = math.nan
+        out = c.run()
+        assert bool(out[5].isnan().all()) and not bool(out[:5].isnan().any())
+
+
+@pytest.mark.parametrize("io", ["f32", "bf16"])
+@pytest.mark.parametrize("ends", [ENDS, ENDS[1:]])
+def test_convolution_sums_at_the_ends_of_the_exponential(io, ends):
+    """x sigmoid(x) of x: x itself, or nothing.  (An infinite row times a weight of 0 is a NaN, in the sums of the rows behind it, too.)"""
+    n = len(ends)
+    c = Case([n, 1], [0, 0], kh=1, vh=1, d=64, io=io)
+    x = torch.tensor(ends, dtype=torch.float64, device="cuda").to(c.io)
+    c.x[:n] = x[:, None]
+    c.x[n] = math.nan
+    c.w.fill_(0)
+    c.w[:, -1] = 1
+    y = c.step.conv(c.x, c.w).double()
+    s = (torch.cat([torch.zeros(3, dtype=torch.float64, device="cuda"), x.double()]).unfold(0, 4, 1) * c.w[0].double()).sum(1)
+    want = (s * torch.sigmoid(s))[:, None].expand(n, c.ch)
+    assert bool(y[n].isnan().all()) and torch.equal(y[:n].isnan(), want.isnan()) and torch.equal(y[:n].isinf(), want.isinf())
+    fine = want.isfinite()
+    off = (y[:n] - want).abs()
+    assert bool((off <= (2.0 ** -20 if io == "f32" else 2.0 ** -8) * want.abs() + 2.0 ** -118)[fine].all()), off.max(1)
