@@ -96,7 +96,7 @@ class Step:
     def _rows(self, name, t, shape, inner, dtype):
         """Checks [rows, *shape] of dtype, what belongs to a row side by side (strides `inner`); returns its address and the stride of rows."""
         st = t.stride()
-        if t.dtype is dtype and t.shape == shape and st[1:] == inner and t.get_device() == self._index and st[0] >= shape[1] * inner[0]:
+        if t.dtype is dtype and dtype in TYPES and t.shape == shape and st[1:] == inner and t.get_device() == self._index and st[0] >= shape[1] * inner[0]:
             return t.data_ptr(), st[0]
         if t.shape != shape or t.device != self.device:
             raise ValueError("%s: %s on the pool's device" % (name, list(shape)))

@@ -103,3 +103,20 @@ def test_weights_that_the_kernel_before_writes():
         torch.cuda.synchronize()
         assert torch.equal(y, c.step.conv(c.x, w, bias=b)), i
     assert c.step.status() == 0
+
+
+@pytest.mark.parametrize("dtype", [torch.float64, torch.int32])
+def test_rows_of_other_types_are_refused(dtype):
+    """By a ValueError, as everything that does not fit, and before anything runs."""
+    c = Case([3], [0], d=64, io="f32")
+    state, carried = c.state.clone(), c.carried.clone()
+    to = lambda *ts: [t.to(dtype) for t in ts]  # noqa: E731
+    with pytest.raises(ValueError, match="float32, float16 or bfloat16"):
+        c.step.conv(c.x.to(dtype), c.w)
+    with pytest.raises(ValueError, match="float32, float16 or bfloat16"):
+        c.step.rule(*to(c.q, c.k, c.v, c.alpha, c.beta), c.a, c.dt)
+    with pytest.raises(ValueError, match="float32, float16 or bfloat16"):
+        c.step.replay(*to(c.k, c.v, c.alpha, c.beta), c.a, c.dt)
+    with pytest.raises(ValueError, match="float32, float16 or bfloat16"):
+        c.step.rule(c.q, c.k, c.v.to(dtype), c.alpha, c.beta, c.a, c.dt)
+    assert torch.equal(c.state, state) and torch.equal(c.carried, carried) and c.step.status() == 0
