@@ -404,8 +404,9 @@ sz_logprob_kernel(const LpArgs a) {
         }
         const bool one = alone || !(fabsf(t.m) < INFINITY);
         const float lz = log1pf(t.s);
+        auto score = [&](float v) { return v == -INFINITY ? v : (v - t.m) * inv_t - lz; };      // (what is masked stays so at an infinite temperature)
         if (tid == 0) {
-            if (a.logprob) a.logprob[row] = token < 0 ? -INFINITY : one ? (n == 0 ? 0.f : -INFINITY) : (tv - t.m) * inv_t - lz;
+            if (a.logprob) a.logprob[row] = token < 0 ? -INFINITY : one ? (n == 0 ? 0.f : -INFINITY) : score(tv);
             if (a.rank) a.rank[row] = token < 0 ? -1 : (int32_t)n;
             if (a.entropy) a.entropy[row] = one ? 0.f : lz - t.x * 0.6931471805599453f / (1.f + t.s);
         }
@@ -413,7 +414,7 @@ sz_logprob_kernel(const LpArgs a) {
             auto give = [&](int at, u64 key) {
                 const float v = lp_down(~(u32)(key >> LP_ID));
                 a.top_ids[(size_t)row * top + at] = key == ~0ull ? -1 : (int32_t)(key & ((1u << LP_ID) - 1));
-                a.top_logprobs[(size_t)row * top + at] = key == ~0ull ? -INFINITY : one ? (at == 0 ? 0.f : -INFINITY) : (v - t.m) * inv_t - lz;
+                a.top_logprobs[(size_t)row * top + at] = key == ~0ull ? -INFINITY : one ? (at == 0 ? 0.f : -INFINITY) : score(v);
             };
             if (a.C == 1) { if (tid < top) give(tid, S->best[tid]); }
             else {

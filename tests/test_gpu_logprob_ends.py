@@ -1,0 +1,25 @@
+"""Log probabilities at the ends of what a temperature may be."""
+import math
+
+import pytest
+import torch
+
+from tests.util import pkg
+
+sampling = pkg.sampling
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("rows", [2, 300])
+def test_an_infinite_temperature_leaves_masked_tokens_out(rows):
+    """All that is not masked weighs the same."""
+    lg = torch.full((rows, 3001), -math.inf, device="cuda")
+    ids = [7, 100, 1500, 2999, 3000]
+    lg[:, ids] = torch.tensor([1.0, -5.0, 300.0, 0.0, 2.0], device="cuda")
+    tok = torch.tensor([100, 8] * (rows // 2), dtype=torch.int32, device="cuda")
+    res = sampling.logprob_rows(lg, tok, top=8, temperature=torch.full((rows,), math.inf, device="cuda"))
+    want = -math.log(5)
+    assert bool(((res.logprob[::2] - want).abs() < 2.0 ** -20).all()) and bool((res.logprob[1::2] == -math.inf).all())
+    assert bool(((res.entropy + want).abs() < 2.0 ** -20).all())
+    assert res.top_ids[0].tolist()[:5] == [1500, 3000, 7, 2999, 100]
+    assert bool(((res.top_logprobs[:, :5] - want).abs() < 2.0 ** -20).all()) and bool((res.top_logprobs[:, 5:] == -math.inf).all())
