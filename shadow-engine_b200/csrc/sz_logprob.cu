@@ -136,7 +136,7 @@ sz_logprob_kernel(const LpArgs a) {
     const float tv_next = lp_down(lp_up(tv) + 1);        // (of a finite one; of the largest: infinity)
     const float T = a.temperature ? a.temperature[row] : 1.f, inv_t = 1.f / T;
     const bool alone = !(T > 0.f) || !(inv_t <= 3.4e38f);            // the best token has it all
-    const float c = alone ? 0.f : inv_t * 1.4426950408889634f;
+    const float c = alone ? 0.f : fminf(inv_t * 1.4426950408889634f, 3.4e38f);      // (finite, so that equal largest ones, 0 times it, weigh 1)
     auto edge = [&](int v, u32* w) {                     // vector -1: the elements before the first, nvec: those behind the last
 #pragma unroll
         for (int i = 0; i < 4; i++) {

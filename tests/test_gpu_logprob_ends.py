@@ -23,3 +23,18 @@ def test_an_infinite_temperature_leaves_masked_tokens_out(rows):
     assert bool(((res.entropy + want).abs() < 2.0 ** -20).all())
     assert res.top_ids[0].tolist()[:5] == [1500, 3000, 7, 2999, 100]
     assert bool(((res.top_logprobs[:, :5] - want).abs() < 2.0 ** -20).all()) and bool((res.top_logprobs[:, 5:] == -math.inf).all())
+
+
+@pytest.mark.parametrize("rows", [2, 300])
+@pytest.mark.parametrize("temperature", [2e-38, 5e-39, 3e-39])
+def test_equal_ones_share_at_the_smallest_temperatures(rows, temperature):
+    """The reciprocal is a number still, its product with log2(e) may not be one."""
+    lg = torch.randn(rows, 20011, device="cuda", generator=torch.Generator(device="cuda").manual_seed(1)).clamp_max(3.0)
+    ids = [3, 4, 5000, 12345, 20010]
+    lg[:, ids] = 6.5
+    tok = torch.tensor([12345, 6] * (rows // 2), dtype=torch.int32, device="cuda")
+    res = sampling.logprob_rows(lg, tok, top=5, temperature=torch.full((rows,), temperature, device="cuda"))
+    want = -math.log(5)
+    assert bool(((res.logprob[::2] - want).abs() < 2.0 ** -20).all()) and bool((res.logprob[1::2] < -1e37).all())
+    assert bool(((res.entropy + want).abs() < 2.0 ** -20).all())
+    assert res.top_ids[0].tolist() == ids and bool(((res.top_logprobs - want).abs() < 2.0 ** -20).all())
