@@ -537,11 +537,14 @@ sz_delta_chunk_kernel(const DlBatch d, const DlRule a, int idx0, int idx1, const
             }
             __syncwarp();
         };
+        int na = 0, nb = 0;                                               // chunks asked for (none any more after a wait that ran out)
         auto copy_a = [&](int i) {
             const int slot = i % SA;
             u8* const st = sm + slot * M::A;
             const u8* const src = scratch + (size_t)(lg.base + c0 + i - idx0) * one;
             if (i >= SA) wait(&emptya[slot], i / SA - 1);
+            if (dead) return;
+            na = i + 1;
             both(st, src + (size_t)kx * C::ROWS, C::ROWS / 2, src + (size_t)a.kh * C::ROWS + (size_t)h * C::HEAD, C::HA, &fulla[slot]);
             tile(st + C::ROWS / 2 + C::HA, a.v, a.v_stride, c0 + i);
             asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(sz_smem_addr(&fulla[slot])) : "memory");
@@ -551,6 +554,8 @@ sz_delta_chunk_kernel(const DlBatch d, const DlRule a, int idx0, int idx1, const
             u8* const st = rb + slot * M::B;
             const u8* const src = scratch + (size_t)(lg.base + c0 + i - idx0) * one;
             if (i >= SB) wait(&emptyb[slot], i / SB - 1);
+            if (dead) return;
+            nb = i + 1;
             both(st, src + (size_t)kx * C::ROWS + C::ROWS / 2, C::ROWS / 2, src + (size_t)a.kh * C::ROWS + (size_t)h * C::HEAD + C::HA, C::HB, &fullb[slot]);
             if (M::STAGED && norm) tile(st + C::ROWS / 2 + C::HB, a.z, a.z_stride, c0 + i);
             asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(sz_smem_addr(&fullb[slot])) : "memory");
@@ -563,8 +568,11 @@ sz_delta_chunk_kernel(const DlBatch d, const DlRule a, int idx0, int idx1, const
             if (OUT) copy_b(i);
             if (LEAD && i + 1 < nc) copy_a(i + 1);
         }
-        for (int i = max(0, nc - SA); i < nc; i++) wait(&fulla[i % SA], i / SA);     // (nothing is under way when the block ends, whoever gave up)
-        if (OUT) for (int i = max(0, nc - SB); i < nc; i++) wait(&fullb[i % SB], i / SB);
+        // (nothing is under way when the block ends, whoever gave up)
+        bool all = true;
+        for (int i = max(0, na - SA); i < na; i++) all &= sz_mbar_wait_warp(&fulla[i % SA], (i / SA) & 1);
+        for (int i = max(0, nb - SB); i < nb; i++) all &= sz_mbar_wait_warp(&fullb[i % SB], (i / SB) & 1);
+        if (!all && lane == 0) atomicOr(d.err, DL_E_WAIT);
         return;
     }
     if (OUT && warp == NC + NG * NO + 1) {
@@ -605,6 +613,7 @@ sz_delta_chunk_kernel(const DlBatch d, const DlRule a, int idx0, int idx1, const
             *(float2*)(factor + turn * CK + 2 * lane) = make_float2(rsqrtf(sum.x * (1.f / D) + a.eps), rsqrtf(sum.y * (1.f / D) + a.eps));
             arrive(&factor_there[turn]);
         }
+        if (CS > 1) sz_cluster_sync();                                    // (.. with the other blocks' warps of this task: none leaves while another may still write to it, had a wait run out)
         return;
     }
     if (warp < NC) {
