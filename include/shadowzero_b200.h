@@ -389,7 +389,7 @@ int sz_delta_conv(const sz_delta_pool* pool, const sz_delta_batch* batch, int io
  *   S = decay S;  S += k (beta' (v - S^T k))^T;  o = S^T q;  out = o, or o / sqrt(mean(o^2) + eps) * norm * sigmoid(z).
  * q, k [rows][k_heads][head_dim], v, z, out [rows][v_heads][head_dim], alpha, beta [rows][v_heads], all of io_type, row strides in elements, heads side by side; rows 16-byte aligned (those
  * of alpha and beta: an element).  q, z and out may be 0 (the states alone: a replay); z and norm come together; out lies apart from the inputs.  Uses the pool's state only.
- * A sequence of many rows - from 36 on, or up to 112, by the heads and the number of sequences of the call - goes in chunks of 64, where the call is said to have such
+ * A sequence of many rows - from 40 on, or up to 128, by the heads and the number of sequences of the call - goes in chunks of 64, where the call is said to have such
  * (max_rows; a row's last bits depend on which way it goes): matrix products whose factors are held in 22 bits, sums in
  * f32 as row by row; a number that is not finite spoils the rest of its sequence then, and the rows of its chunk before it,
  * too.  Numbers of less than 2^-35 of the largest in 16 value dimensions of a state, or of a chunk's changes, are lost there. */

@@ -425,12 +425,13 @@ DlBatch dl_batch(const sz_delta_pool* p, const sz_delta_batch* b, uint64_t scrat
 // The most rows that a sequence of the call is said to have.
 int dl_most(const sz_delta_batch* b) { return b->max_rows && b->max_rows < b->rows ? b->max_rows : b->rows; }
 // From how many rows on a sequence goes in chunks (0: none of the call does).  Row by row costs by the row, a chunk what it costs, and its blocks are one a multiprocessor: the more
-// of them have to wait for each other, the later they are worth it.  us, row by row / in chunks: 1 sequence of 32 heads of 128 (128 blocks), 32 rows 22.8 / 23.7, 40
-// 27.5 / 23.7; 8 sequences (1,024), 48 rows 55 / 74, 64 72 / 75, 96 105 / 93; 64 (8,192), 64 rows 485 / 614, 96 708 / 770, 128 931 / 844; heads of 64, whatever the
-// number of blocks (4 to 1,024), 40 rows 19 / 20, 20 / 21, 61 / 63, 48 22 / 20, 24 / 21, 72 / 64.
+// of them have to wait for each other, the later they are worth it.  us, row by row / in chunks, bf16: sequences of 32 heads of 128 (128 blocks each), one of 36 rows 26.1 / 27.7, of 40
+// 28.2 / 27.6; two of 44 rows 31.1 / 32.7, of 48 33.2 / 32.7; three of 56 rows 38.1 / 39.8, of 64 43.0 / 40.4; four of 64 rows 43.1 / 48.4, of 80 52.7 / 59.4, of 96 62.5 / 60.1; eight of 72 rows 81 / 105, of 96
+// 106 / 107, of 112 123 / 108; 16 of 72 rows 160 / 198, of 96 209 / 198; 32 of 112 rows 423 / 435, of 128 481 / 440; 64 of 112 rows 828 / 948, of 128 941 / 962, of 160 1,166 / 1,153.  Heads of 64, of 4 and of 16
+// heads, one of 40 rows 20.2 / 21.7, 20.3 / 24.6, of 48 23.6 / 21.9, 23.9 / 24.6; 64 of 4 heads, 48 rows 28.7 / 30.4, 52 31.1 / 30.0.
 int dl_least(const sz_delta_pool* p, const sz_delta_batch* b) {
     const int64_t blocks = (int64_t)p->v_heads * 4 * min(b->n_seq, b->rows / 32 + 1);
-    const int least = p->head_dim == 64 ? 44 : blocks <= DL_SM ? 36 : blocks <= 16 * DL_SM ? 68 : 112;
+    const int least = p->head_dim == 64 ? 48 : blocks <= DL_SM ? 40 : blocks <= 2 * DL_SM ? 48 : blocks <= 3 * DL_SM ? 60 : blocks <= 16 * DL_SM ? 96 : 128;
     return dl_most(b) >= least ? least : 0;
 }
 

@@ -7,7 +7,7 @@ from tests.test_delta_host import batch, pool, rule
 from tests.util import pkg
 
 szlib = pkg.lib
-ROWS = [1, 35, 36, 64, 112, 700, 2048, 4093, 4096, 6500, 8192, 12300, 16384, 16400, 40000, 1 << 17, 1 << 20]
+ROWS = [1, 39, 40, 64, 128, 700, 2048, 4093, 4096, 6500, 8192, 12300, 16384, 16400, 40000, 1 << 17, 1 << 20]
 
 
 def need(io, kh, vh, d, n_seq, rows, max_rows):
@@ -26,7 +26,7 @@ def test_no_type_of_rows_needs_more_than_f32(kh, vh, d):
             for max_rows in (0, 4, 300):
                 f32, f16, bf16 = (need(t, kh, vh, d, n_seq, rows, max_rows) for t in (szlib.TYPE_F32, szlib.TYPE_F16, szlib.TYPE_BF16))
                 assert f32 >= f16 and f32 >= bf16, (n_seq, rows, max_rows, f32, f16, bf16)
-                assert f32 <= 256 + max(96 << 20, 8 * (256 + need(szlib.TYPE_F32, kh, vh, d, 1, 112, 0)))
+                assert f32 <= 256 + max(96 << 20, 8 * (256 + need(szlib.TYPE_F32, kh, vh, d, 1, 128, 0)))
 
 
 @pytest.mark.parametrize("io", [szlib.TYPE_F16, szlib.TYPE_BF16])

@@ -117,3 +117,10 @@ def test_convolution_sums_at_the_ends_of_the_exponential(io, ends):
     fine = want.isfinite()
     off = (y[:n] - want).abs()
     assert bool((off <= (2.0 ** -20 if io == "f32" else 2.0 ** -8) * want.abs() + 2.0 ** -118)[fine].all()), off.max(1)
+
+
+@pytest.mark.parametrize("n, rows", [(1, 39), (1, 40), (2, 47), (2, 48), (3, 59), (3, 60), (4, 95), (4, 96), (19, 127), (19, 128)])
+def test_both_sides_of_the_borders_between_rows_and_chunks(n, rows):
+    Case([rows] * n, [4 * (i % 2) for i in range(n)], kh=16, vh=32, d=128, io="bf16", seed=n).check_rule()
+    if n == 2:
+        Case([rows] * n, [4 * (i % 2) for i in range(n)], kh=8, vh=16, d=64, io="f16", grouped=True, seed=n).check_rule()
