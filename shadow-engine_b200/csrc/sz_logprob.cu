@@ -488,17 +488,20 @@ extern "C" int sz_logprob_rows(int logits_type, uint64_t logits, int64_t logits_
     a.logits = (const u8*)logits; a.stride = logits_stride * esz; a.rows = rows; a.vocab = vocab; a.top = top;
     a.tokens = (const int32_t*)tokens; a.temperature = (const float*)temperature;
     a.logprob = (float*)logprob; a.entropy = (float*)entropy; a.rank = (int32_t*)rank; a.top_ids = (int32_t*)top_ids; a.top_logprobs = (float*)top_logprobs;
-    // Up to one row a multiprocessor: blocks of 512 threads, as many a row (up to 8) as all have a multiprocessor each; more rows: 256 threads, four blocks a multiprocessor, one
-    // a row.  Device us of rows of 151,936 with 512 threads and 1, 2, 4, 8 blocks a row, with 256 threads and one: 1 row of f32 16.2, 12.4, 9.5, 8.3, 25; 16 rows 17.5, 13.9,
+    // Up to one row a multiprocessor: blocks of 512 threads, as many a row (up to 8) as all have a multiprocessor each; more rows: a block a row, of 256 threads, four blocks a
+    // multiprocessor, where a row is up to 352 KB, else of 512 (longer rows leave too few threads with loads under way, and the groups' largest of four such blocks have no place).
+    // Device us of rows of 151,936 with 512 threads and 1, 2, 4, 8 blocks a row, with 256 threads and one: 1 row of f32 16.2, 12.4, 9.5, 8.3, 25; 16 rows 17.5, 13.9,
     // 11.6, 12.6, 26; 37 rows 17.6, 14.1, 14.9, 21.9, 26; 64 rows 17.8, 14.3, 15.3, 26, 26; 128 rows 17.4, 19, 26.5, 44, 27; 250 of bf16 25.3, 34, 50, 91, 24.8; 1,021
-    // 75, 101, 166, 315, 69.
+    // 75, 101, 166, 315, 69.  One block a row, 512 / 256 threads, called one by one, top 20: 250 rows of f32, 32,000 14.2 / 13.3, 64,000 20.9 / 20.7, 96,000 28.6 / 36.2, 151,936
+    // 40.5 / 58.6; 1,021 rows 44.0 / 38.6, 65.3 / 64.9, 87.1 / 92.2, 131 / 170; 250 of bf16, 128,000 29.0 / 28.8, 180,000 36.9 / 37.9, 220,000 45.4 / 51.4, 262,144 50.2 / 71.9; 1,021
+    // 91 / 85, 116 / 110, 141 / 131, 158 / 177.
     const int most = vocab > 16384 ? 8 : vocab > 4096 ? 4 : vocab > 1024 ? 2 : 1;
-    const bool few = rows <= LP_SM;
+    const bool few = rows <= LP_SM, wide = few || (long long)vocab * esz > (352 << 10);
     a.C = 1;
     while (few && 2 * a.C <= most && (long long)rows * 2 * a.C <= LP_SM) a.C *= 2;
     a.per = ((vocab + a.C - 1) / a.C + 7) & ~7;
     cudaStream_t st = (cudaStream_t)stream;
 #define SZ_LP(N_) (logits_type == SZ_TYPE_F32 ? lp_launch<SZ_TYPE_F32, N_>(a, st) : logits_type == SZ_TYPE_F16 ? lp_launch<SZ_TYPE_F16, N_>(a, st) : lp_launch<SZ_TYPE_BF16, N_>(a, st))
-    return few ? SZ_LP(512) : SZ_LP(256);
+    return wide ? SZ_LP(512) : SZ_LP(256);
 #undef SZ_LP
 }
