@@ -28,7 +28,7 @@ constexpr int CK = 64, DL_TILES = 20;                    // rows of a chunk; 8 x
 constexpr int DL_FRAG = DL_TILES * 32 * 8;               // bytes of a triangle in f16, in the order in which the matrix instruction takes it
 constexpr int64_t DL_SLAB = 96ll << 20;                  // scratch that a pass over chunks may take (what the first kernel leaves is in L2 for the second)
 
-struct DlScalars { float gr[CK], beta[CK], wj[CK], gc; int ex; float pad[14]; };      // - beta e^G rho_k, beta, 2^-ex e^(G_C - G_j) rho_k; e^G_C, and what makes the largest wj 1 to 2
+struct DlScalars { float gr[CK], beta[CK], wj[CK], gc; int ex; float pad[14]; };      // - beta e^G rho_k, beta, 2^-ex e^(G_C - G_j) rho_k; e^G_C, and what makes the largest wj 0.5 to 1
 
 template <int D, int TYPE> struct DlChunk {
     static constexpr int NK = TYPE == SZ_TYPE_F32 ? 2 : 1;                // f16 numbers of an element of k and q
@@ -411,7 +411,7 @@ sz_delta_prep_kernel(const DlBatch d, const DlRule a, int idx0, u8* __restrict__
             if (OUT) { ((float*)(hp + C::HEAD))[r - 2 * CK] = eg * sRq[r]; ((float*)(hp + C::HEAD))[r - CK] = sRq[r]; }
             const float wj = expf((float)(GC - G)) * sRk[r], wo = expf((float)(GC - sG[half][r ^ 32])) * sRk[r ^ 32];
             const int top = (int)(__reduce_max_sync(0xffffffffu, __float_as_uint(fmaxf(wj, wo))) >> 23);
-            const int ex = top == 0 || top == 255 ? 0 : max(-100, min(0, top - 127));
+            const int ex = top == 0 || top == 255 ? 0 : max(-100, min(0, top - 126));      // (below 1: a change times it is below 2^15)
             sc->wj[r] = wj * dl_pow2(-ex);
             if (r == 0) sc->ex = ex;
             if (r == 0) sc->gc = expf((float)GC);

@@ -124,3 +124,21 @@ def test_both_sides_of_the_borders_between_rows_and_chunks(n, rows):
     Case([rows] * n, [4 * (i % 2) for i in range(n)], kh=16, vh=32, d=128, io="bf16", seed=n).check_rule()
     if n == 2:
         Case([rows] * n, [4 * (i % 2) for i in range(n)], kh=8, vh=16, d=64, io="f16", grouped=True, seed=n).check_rule()
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("size", [1.0, 3e-3, 1e-4])
+def test_the_largest_changes_there_can_be(d, size):
+    """Every gate open, no decay, keys that are all alike, or one direction and its opposite in turn, values that alternate: changes are sums of values of one sign, as large as they become."""
+    for flip in (False, True):
+        c = Case([320], [0], d=d, kh=1, vh=2, io="f32", gate=False, seed=d)
+        c.a.zero_()
+        c.beta.fill_(60.0)
+        key = torch.zeros(d, device="cuda")
+        key[3] = size
+        c.k.copy_(key.expand_as(c.k))
+        if flip:
+            c.k[1::2].mul_(-1)
+        c.v.fill_(1.999)
+        c.v[1::2].mul_(-1)
+        c.check_rule()
