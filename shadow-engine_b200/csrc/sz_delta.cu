@@ -12,8 +12,8 @@ constexpr int DL_SM = 148;           // multiprocessors (a GPU with another numb
 // y[r][c] = silu(bias[c] + sum_t w[c][t] x[r - (K - 1) + t][c]); rows before a sequence's first are those its slot carries (K - 1, the oldest first).  The taps are
 // added in f32 from the oldest on.  A thread has DL_V neighbouring channels and `tile` rows, one after the other, with the window in registers and the next
 // DL_AHEAD rows asked for.  The block that has a sequence's first row is the only one that looks at its slot: it does the rows up to the K - 1st, those of the next tile
-// among them, and then leaves the new carried rows, which are rows of the call or of the old slot (the place is the same where a sequence goes on in place).  8,192 channels over 4 rows, bf16: 4,093 rows 38.5 us (134 MB, 20.5 us of them; a row of 4 channels is some 45 instructions, two
-// exponentials' pipe a channel among them; with 8 rows ahead 42, in tiles of 16 rows 41), 163 rows of 64 sequences 9.3, one row 3.4 (a launch and the chain table,
+// among them, and then leaves the new carried rows, which are rows of the call or of the old slot (the place is the same where a sequence goes on in place).  8,192 channels over 4 rows, bf16: 4,093 rows 38 us (134 MB, 20.5 us of them; a row of 4 channels is some 45 instructions, two
+// exponentials' pipe a channel among them; with 8 rows ahead 42, in tiles of 16 rows 41), 163 rows of 64 sequences 9.2, one row 3.7, four of one sequence 4.6 (a launch and the chain table,
 // slot, carried rows, store).  What a tile reads twice are its first K - 1 rows, from L2.
 constexpr int DL_AHEAD = 4, DL_V = 4;
 template <int ESZ> struct DlRaw { typedef uint2 T; };
@@ -221,7 +221,7 @@ sz_delta_conv_kernel(const DlBatch d, const DlConv a) {
 // so that both sums over the key dimensions (x and S^T q) go through the lanes' exchange together.  Products are packed pairs of neighbouring key dimensions.
 // Rows come in sets of DL_SET: a warp norms one of them for the block (shared memory), and norms and gates its outputs.  With many
 // sequences the states' bytes bound it (64 sequences of 32 heads of 128, 163 rows of bf16: 274 MB, 41.9 us of 59; 32 of f32 without outputs 20.9 of 31.7), with few the
-// chain load - exchange - store (one row 4.7 us).  The operands are asked for before the state (after it: 74 us).
+// chain load - exchange - store (one row 4.8 us).  The operands are asked for before the state (after it: 74 us).
 constexpr int DL_SET = 8;
 template <int D> struct DlSet {
     float k[DL_SET][D], q[DL_SET][D], v[DL_SET][D], o[DL_SET][D];
@@ -500,7 +500,7 @@ extern "C" int sz_delta_conv(const sz_delta_pool* pool, const sz_delta_batch* ba
     a.conv = (u8*)pool->conv; a.conv_stride = pool->conv_stride; a.conv_type = pool->conv_type; a.ch = ch;
     // rows a thread has: as many as leave every multiprocessor 16 warps, up to 32 (a tile's first rows are read twice)
     const int vecs = (ch / DL_V + 127) / 128;
-    // a block a sequence where they have a few rows each: one look-up instead of one for every sequence that a tile meets (64 sequences, 163 rows: 10.8 us by tiles, 10.1 so; 9.3 since a sequence is looked up with one wait)
+    // a block a sequence where they have a few rows each: one look-up instead of one for every sequence that a tile meets (64 sequences, 163 rows: 10.8 us by tiles, 10.1 so; 9.2 since a sequence is looked up with one wait)
     const bool by_seq = batch->n_seq > 1 && dl_most(batch) <= 8;
     a.tile = 1;
     while (a.tile < 32 && (int64_t)vecs * ((batch->rows + 2 * a.tile - 1) / (2 * a.tile)) >= 4 * DL_SM) a.tile *= 2;

@@ -10,8 +10,8 @@
 //  sz_delta_chunk_kernel, a block of warps for 16 NG value dimensions of a sequence's value head: the chain over its chunks, on mma.sync.  Everything is
 //   transposed, so that a warp's 16 value dimensions are a product's rows: S^T (f32) stays in its registers, and what one product gives is in the layout in which
 //   the next one takes it.  At 128 key dimensions two warps have 64 of them each and add up K S and Q S through shared memory.
-// 4,093 rows of 32 heads of 128 on 16, bf16: 48 us and 172 (137 MB: 21 of them).  The chain lies in what is between one product and the next: the largest of the state 150 cycles, the
-// partner's part 310, R 290, two numbers of a factor 270 and 220, waits 400.
+// 4,093 rows of 32 heads of 128 on 16, bf16: 48 us and 185 (137 MB: 21 of them); a chunk of the chain is some 5,400 cycles, 42 % of them with the matrix pipe at work, the rest what lies between one
+// product and the next: the largest of the state, the partner's part, R, two numbers of a factor, waits.
 // tcgen05 would have the products' time, but every one of the chain's links would go through tensor memory and back (300 - 400 cycles a wait, three
 // a chunk) and S through a conversion by four warps: no sooner.
 //
@@ -19,7 +19,7 @@
 // numbers (22 bits); the rows' lengths and powers are factors in f32, and so is beta: a chunk whose gates are all but closed keeps the digits of its small changes, where T diag(beta) in f16
 // has none below 2^-25.  (T's elements are at most 1, its diagonal is 1.)  S, R and D enter as two f16 numbers each, in units of a power of two that
 // the warp takes from the largest there is: 22 bits, and what is less than 2^-35 of that largest is lost.  Sums are f32.  T and the decays' sums: f32 and f64.
-// (One f16 number a factor in the last products of bf16 outputs, 11 bits where they keep 8: their difference from rounded f32 outputs is 1.1 10^-3 of their size instead of 10^-5, and 4,093 rows take 202 us.)
+// (One f16 number a factor in the last products of bf16 outputs, 11 bits where they keep 8: their difference from rounded f32 outputs is 1.1 10^-3 of their size instead of 3 10^-5; 4,093 rows took 202 us so, and 221 with two.)
 #include "sz_delta.cuh"
 
 namespace {

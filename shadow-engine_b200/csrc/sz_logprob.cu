@@ -5,7 +5,8 @@
 // new one is rare) and both sums beside it.  A thread's elements come in groups of LP_G vectors; what a group's largest is stays in shared memory, and the
 // best `top` are looked for afterwards in the few groups that can hold them: a bound that `top` threads reach, by halving, then what is not below it.
 // A row is a cluster of 1 to 8 blocks, each with its part of it.  Rows of 151,936: one of f32, top 5, 8.3 us (the chain load, bound, gather, order and two barriers of the
-// cluster); 64 of f32, top 20, 14.3 (39 MB: 5.9); 1,021 of bf16, top 1, 69 where they score their best, 87 with a fifth of them scoring any token (310 MB: 47; the exponentials' pipe alone takes 35, and an element some 8 instructions).
+// cluster); 64 of f32, top 20, 17.4 (39 MB: 5.9); 1,021 of bf16, top 1, 69 where they score their best, 87 with a fifth of them scoring any token (310 MB: 47; the exponentials' pipe alone takes 35, and an element some 8 instructions).
+// A token that is masked itself has all that is not before it, and its row's elements are looked at one by one again: 64 such rows of f32 take 76 us instead of 21, 250 of bf16 150 instead of 23.
 #include "sz_common.cuh"
 
 #include <cuda_bf16.h>

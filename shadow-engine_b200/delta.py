@@ -59,7 +59,7 @@ class Step:
     a paged step's tables), slots int32 [sequences]: where a sequence's state is; to: where it goes (None: the same); take: how many of its rows count (None: all).  They
     are the caller's tensors: change their values from step to step, behind the calls that read them.  max_rows: the most rows that a sequence has (it chooses
     kernels).  Calls on one Step follow one another on a stream - the one it was made on, or another that waits for that -, and it is kept until they are done; what
-    may overlap needs a Step each."""
+    may overlap needs a Step each.  Each has a scratch of its own: up to 96 MB where a sequence may have many rows, else 256 bytes."""
 
     def __init__(self, states, row_start, lens, slots, rows, to=None, take=None, max_rows=None):
         self.lib = szlib.load()
